@@ -1,5 +1,5 @@
-"""ctypes binding of ``libdwa_b200.so`` (the C ABI declared in include/dwa_retrieval.h and
-include/dwa_lm.h).
+"""ctypes binding of ``libdwa_b200.so`` (the C ABI declared in include/dwa_retrieval.h,
+include/dwa_lm.h and include/dwa_decode.h).
 
 The library is the only implementation of the retrieval path: there is no
 CPU or PyTorch fallback.  If the shared library is missing, importing this
@@ -23,7 +23,7 @@ DWA_ERR_DEVICE_CHECK = 5
 DWA_ERR_WORKSPACE = 6
 DWA_MAX_K = 128
 
-# Every symbol include/dwa_retrieval.h and include/dwa_lm.h declare, with its ctypes signature.
+# Every symbol the headers in include/ declare, with its ctypes signature.
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -108,6 +108,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dwa_lm_aspect_queries": (_i32, [_c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p,
                                      _f32, _f32, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
                                      _c_void_p]),
+    # include/dwa_decode.h: the paged cache, attention over it, drafted tokens
+    "dwa_kv_write": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64,
+                            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64,
+                            _i64, _c_void_p, _c_void_p]),
+    "dwa_kv_read": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32,
+                           _i64, _i32, _i64, _i64, _c_void_p, _c_void_p, _i32, _c_void_p,
+                           _c_void_p]),
+    "dwa_paged_attention": (_i32, [_c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p,
+                                   _c_void_p, _c_void_p, _i32, _i64, _i32, _i64, _i64, _c_void_p,
+                                   _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _f32, _c_void_p,
+                                   _i64, _c_void_p, _c_void_p]),
+    "dwa_verify_drafts": (_i32, [_c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p,
+                                 _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

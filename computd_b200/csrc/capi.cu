@@ -15,7 +15,9 @@
 
 #include "dwa_retrieval.h"
 #include "dwa_lm.h"
+#include "dwa_decode.h"
 #include "dwa_internal.h"
+#include "paged_attention.cuh"
 
 namespace {
 
@@ -879,6 +881,170 @@ dwa_status dwa_lm_aspect_queries(const void* q, int64_t M, int32_t S, int32_t d_
                                              lambda_sharp, T, use_sigmoid ? 1 : 0, out, ldo, w_out,
                                              params_out, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dwa_lm_aspect_queries launch");
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
+// The paged cache's part of the checks of dwa_kv_write, dwa_kv_read and dwa_paged_attention.
+dwa_status kv_cache_view(const char* fn, const void* k_cache, const void* v_cache,
+                         const float* k_scale, const float* v_scale, int32_t H, int32_t d,
+                         int64_t n_pages, int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                         dwa::KvCacheView* out) {
+  if (H < 1 || n_pages < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad cache sizes (H=%d, n_pages=%lld)", fn, H,
+                (long long)n_pages);
+  if (d < 16 || d > 128 || d % 16 != 0)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: d=%d must be a multiple of 16 in [16, 128]", fn, d);
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: page_size=%d must be 16, 32, 64 or 128", fn,
+                page_size);
+  if (n_pages > INT32_MAX || H > 65535)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many pages or heads", fn);
+  if (!k_cache || !v_cache) return fail(DWA_ERR_INVALID_ARG, "%s: null cache pointer", fn);
+  if (!k_scale != !v_scale)
+    return fail(DWA_ERR_INVALID_ARG, "%s: k_scale and v_scale go together", fn);
+  const int64_t page = static_cast<int64_t>(H) * page_size;
+  if (ld_page < page * d || (k_scale && ld_scale_page < page))
+    return fail(DWA_ERR_INVALID_ARG, "%s: a page stride is below the page's size", fn);
+  if (ld_page % d != 0)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: ld_page=%lld must be a multiple of d=%d", fn,
+                (long long)ld_page, d);
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || (k_scale && (!aligned(k_scale, 4) || !aligned(v_scale, 4))))
+    return fail(DWA_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned (scales 4-byte)", fn);
+  *out = dwa::KvCacheView{k_cache, v_cache, k_scale, v_scale, H, d, n_pages, page_size, ld_page,
+                          k_scale ? ld_scale_page : 0};
+  return DWA_OK;
+}
+}  // namespace
+
+extern "C" {
+
+dwa_status dwa_kv_write(const void* k, const void* v, int32_t src_bf16, int64_t T, int32_t H,
+                        int32_t d, int64_t k_ld_tok, int64_t k_ld_head, int64_t v_ld_tok,
+                        int64_t v_ld_head, const int64_t* slots, void* k_cache, void* v_cache,
+                        float* k_scale, float* v_scale, int64_t n_pages, int32_t page_size,
+                        int64_t ld_page, int64_t ld_scale_page, int32_t* status,
+                        dwa_stream_t stream) {
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view("dwa_kv_write", k_cache, v_cache, k_scale, v_scale, H, d,
+                                    n_pages, page_size, ld_page, ld_scale_page, &c))
+    return st;
+  if (T < 0 || T > INT32_MAX) return fail(DWA_ERR_INVALID_ARG, "dwa_kv_write: bad T=%lld", (long long)T);
+  if (T == 0) return ok();
+  if (!k || !v || !slots) return fail(DWA_ERR_INVALID_ARG, "dwa_kv_write: null pointer");
+  const int per16 = src_bf16 ? 8 : 4;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8) || k_ld_tok % per16 ||
+      k_ld_head % per16 || v_ld_tok % per16 || v_ld_head % per16)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE,
+                "dwa_kv_write: k and v rows must be 16-byte aligned (slots 8-byte)");
+  if (k_ld_tok < 0 || k_ld_head < 0 || v_ld_tok < 0 || v_ld_head < 0)
+    return fail(DWA_ERR_INVALID_ARG, "dwa_kv_write: negative stride");
+  cudaError_t e = dwa::launch_kv_write(c, k, v, src_bf16 ? 1 : 0, T, k_ld_tok, k_ld_head, v_ld_tok,
+                                       v_ld_head, slots, status, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_kv_write launch");
+  return ok();
+}
+
+dwa_status dwa_kv_read(const void* k_cache, const void* v_cache, const float* k_scale,
+                       const float* v_scale, const int64_t* slots, int64_t T, int32_t H, int32_t d,
+                       int64_t n_pages, int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                       void* k_out, void* v_out, int32_t clear_skipped, int32_t* status,
+                       dwa_stream_t stream) {
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view("dwa_kv_read", k_cache, v_cache, k_scale, v_scale, H, d,
+                                    n_pages, page_size, ld_page, ld_scale_page, &c))
+    return st;
+  if (T < 0) return fail(DWA_ERR_INVALID_ARG, "dwa_kv_read: bad T=%lld", (long long)T);
+  if (T == 0) return ok();
+  if (!slots || !k_out || !v_out) return fail(DWA_ERR_INVALID_ARG, "dwa_kv_read: null pointer");
+  if (!aligned(slots, 8) || !aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(DWA_ERR_INVALID_ARG, "dwa_kv_read: outputs must be 16-byte aligned (slots 8-byte)");
+  if (T > INT32_MAX || T * H > INT32_MAX * 32ll)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "dwa_kv_read: too many vectors");
+  cudaError_t e = dwa::launch_kv_read(c, slots, T, k_out, v_out, clear_skipped ? 1 : 0, status,
+                                      static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_kv_read launch");
+  return ok();
+}
+
+dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
+                               const void* k_cache, const void* v_cache, const float* k_scale,
+                               const float* v_scale, int32_t H_kv, int64_t n_pages,
+                               int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                               const int32_t* block_table, int64_t ld_table, int32_t max_pages,
+                               const int32_t* lengths, const int32_t* q_start, int32_t B,
+                               int32_t max_q, float scale, void* out, int64_t out_ld,
+                               int32_t* status, dwa_stream_t stream) {
+  const char* fn = "dwa_paged_attention";
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H_kv, d, n_pages,
+                                    page_size, ld_page, ld_scale_page, &c))
+    return st;
+  if (T < 0 || B < 0 || max_q < 0 || max_pages < 0 || H < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, B=%d, max_q=%d, max_pages=%d, H=%d)", fn,
+                (long long)T, B, max_q, max_pages, H);
+  if (H % H_kv != 0)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: H=%d must be a multiple of H_kv=%d", fn, H, H_kv);
+  if (T > INT32_MAX || static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX ||
+      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows or tokens", fn);
+  if (!(scale >= 0.f) || std::isinf(scale))
+    return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite and not negative", fn);
+  if (T == 0 || B == 0) return ok();
+  if (!q || !out || !lengths || (max_pages > 0 && !block_table))
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!q_start && (T % B != 0 || T / B > max_q))
+    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal chunks of at most "
+                "max_q=%d", fn, (long long)T, B, max_q);
+  if (max_q == 0) return fail(DWA_ERR_INVALID_ARG, "%s: max_q = 0 with rows to compute", fn);
+  const int64_t width = static_cast<int64_t>(H) * d;
+  if (q_ld < width || out_ld < width || (max_pages > 0 && ld_table < max_pages))
+    return fail(DWA_ERR_INVALID_ARG, "%s: a row stride is below its row length", fn);
+  if (q_ld % 8 != 0 || out_ld % 8 != 0 || !aligned(q, 16) || !aligned(out, 16))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: q and out rows must be 16-byte aligned", fn);
+  if (!aligned(block_table, 4) || !aligned(lengths, 4) || !aligned(q_start, 4) || !aligned(status, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: int32 arrays must be 4-byte aligned", fn);
+  dwa::PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.q_ld = q_ld; a.out_ld = out_ld;
+  a.k = k_cache; a.v = v_cache; a.k_scale = k_scale; a.v_scale = v_scale;
+  a.ld_page = ld_page; a.ld_scale_page = c.ld_scale_page; a.n_pages = n_pages;
+  a.table = block_table; a.ld_table = ld_table; a.max_pages = max_pages;
+  a.page_log2 = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  a.lengths = lengths; a.q_start = q_start; a.T = T;
+  a.even = q_start ? 0 : static_cast<int>(T / B);
+  a.max_q = max_q; a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = status;
+  cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_paged_attention launch");
+  return ok();
+}
+
+dwa_status dwa_verify_drafts(const void* target, const void* draft, int32_t probs_bf16,
+                             const int32_t* tokens, const float* accept_u, const float* sample_u,
+                             const int32_t* draft_lengths, int64_t B, int32_t K, int32_t V,
+                             int32_t* n_accepted, int32_t* out_tokens, dwa_stream_t stream) {
+  const char* fn = "dwa_verify_drafts";
+  if (B < 0 || K < 0 || V < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (B=%lld, K=%d, V=%d)", fn, (long long)B, K, V);
+  if (B > INT32_MAX / 8 || V > (1 << 30) || K > (1 << 20))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many sequences, drafts or tokens", fn);
+  if (B == 0) return ok();
+  if (!target || !sample_u || !n_accepted || !out_tokens || (K > 0 && (!tokens || !accept_u)))
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  const uintptr_t es = probs_bf16 ? 2 : 4;
+  if (!aligned(target, es) || !aligned(draft, es) || !aligned(tokens, 4) || !aligned(accept_u, 4) ||
+      !aligned(sample_u, 4) || !aligned(draft_lengths, 4) || !aligned(n_accepted, 4) ||
+      !aligned(out_tokens, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: misaligned array", fn);
+  cudaError_t e = dwa::launch_verify_drafts(target, draft, probs_bf16 ? 1 : 0, tokens, accept_u,
+                                            sample_u, draft_lengths, B, K, V, n_accepted, out_tokens,
+                                            static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_verify_drafts launch");
   return ok();
 }
 

@@ -199,4 +199,27 @@ cudaError_t launch_pool_init_normal(void* out, int64_t rows, int64_t cols, int64
                                     int64_t row_offset, uint64_t seed, float stddev,
                                     cudaStream_t stream);
 
+// ---------------------------------------------------------------- serving (dwa_decode.h)
+// The paged cache as the C ABI describes it.
+struct KvCacheView {
+  const void *k, *v;
+  const float *k_scale, *v_scale;  // null: bf16 cache
+  int H, d;
+  int64_t n_pages;
+  int page_size;
+  int64_t ld_page, ld_scale_page;
+};
+
+cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, int src_bf16,
+                            int64_t T, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
+                            const int64_t* slots, int32_t* status, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvCacheView& c, const int64_t* slots, int64_t T, void* k_out,
+                           void* v_out, int clear_skipped, int32_t* status, cudaStream_t stream);
+struct PagedArgs;
+cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream);
+cudaError_t launch_verify_drafts(const void* target, const void* draft, int probs_bf16,
+                                 const int32_t* tokens, const float* accept_u, const float* sample_u,
+                                 const int32_t* draft_lengths, int64_t B, int K, int V,
+                                 int32_t* n_accepted, int32_t* out_tokens, cudaStream_t stream);
+
 }  // namespace dwa

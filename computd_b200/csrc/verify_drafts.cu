@@ -1,0 +1,260 @@
+// verify_drafts.cu — verification of drafted tokens against the target's
+// probabilities, and the draw that follows them.
+//
+// With p the target's and q the drafter's distribution, keeping draft x with
+// probability min(1, p(x) / q(x)) and otherwise drawing from max(p - q, 0)
+// (normalised) gives tokens distributed as p.  All tests are made in 64 bits:
+// u q and p are compared exactly (24-bit factors), and the running sums are
+// good to 1e-16 of their total, so the outcome does not hang on the order of
+// the sums.
+//
+// Per sequence this reads the few tested probabilities and one row of V (p,
+// and q where a draft fell), 8 V bytes at most: latency for one sequence, HBM
+// for many.  A cluster of blocks shares the row, each warp a contiguous piece;
+// the piece sums go through distributed shared memory, every block finds the
+// piece that holds the draw, and only its warp goes over its piece again.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "dwa_internal.h"
+#include "sm100_ptx.cuh"
+
+namespace dwa {
+
+namespace {
+
+constexpr int kVerifyThreads = 256;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyMaxCluster = 8;
+
+struct VerifyArgs {
+  const void *target, *draft;
+  const int32_t* tokens;
+  const float *accept_u, *sample_u;
+  const int32_t* draft_lengths;
+  int64_t B;
+  int K, V;
+  int piece;  // entries per warp, a multiple of 4
+  int wide;   // rows may be read four entries at a time
+  int32_t *n_accepted, *out_tokens;
+};
+
+template <typename T>
+__device__ __forceinline__ float prob(const T* p) {
+  if constexpr (sizeof(T) == 2)
+    return __uint_as_float(static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p))) << 16);
+  else
+    return __ldg(p);
+}
+
+// Not a positive finite number: nothing.
+__device__ __forceinline__ float mass(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+
+template <typename T>
+__device__ __forceinline__ void probs4(const T* row, int i, int V, int wide, float (&x)[4]) {
+  if (wide) {
+    if constexpr (sizeof(T) == 2) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + i));
+      x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xFFFF0000u);
+      x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xFFFF0000u);
+    } else {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(row + i));
+      x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = i + j < V ? prob(row + i + j) : 0.f;
+  }
+}
+
+// The weights of entries i .. i + 3 (i + 3 < V when wide).  `one` is the index
+// at which a certain drafter's q is 1 (-1: q is the row, or nothing).
+template <typename T>
+__device__ __forceinline__ void weights4(const T* p, const T* q, int one, int i, int V, int wide,
+                                         double (&w)[4]) {
+  float a[4], b[4] = {};
+  probs4(p, i, V, wide, a);
+  if (q != nullptr) probs4(q, i, V, wide, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const double x = static_cast<double>(mass(a[j])) - static_cast<double>(mass(b[j]));
+    w[j] = x > 0.0 && i + j != one ? x : 0.0;
+  }
+}
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  return x;
+}
+
+__device__ __forceinline__ double ld_cluster_f64(const double* local, int rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];"
+               : "=d"(v)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kVerifyThreads)
+    verify_drafts_kernel(const VerifyArgs a, const int cluster) {
+  __shared__ double sums[2][kVerifyWarps];
+  __shared__ double all[kVerifyMaxCluster * kVerifyWarps];
+  const int rank = static_cast<int>(blockIdx.x % cluster);
+  const int64_t b = blockIdx.x / cluster;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int K = a.K, V = a.V;
+  const T* target = static_cast<const T*>(a.target) + b * (K + 1) * V;
+  const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * K * V : nullptr;
+
+  // How many drafts stand: every warp for itself.
+  int n = a.draft_lengths ? a.draft_lengths[b] : K;
+  n = min(max(n, 0), K);
+  int kept = n;
+  for (int i0 = 0; i0 < n && kept == n; i0 += 32) {
+    const int i = i0 + lane;
+    bool stands = true;
+    if (i < n) {
+      const int x = a.tokens[b * K + i];
+      stands = false;
+      if (x >= 0 && x < V) {
+        const double p = mass(prob(target + static_cast<int64_t>(i) * V + x));
+        const double q = draft ? mass(prob(draft + static_cast<int64_t>(i) * V + x)) : 1.0;
+        stands = static_cast<double>(a.accept_u[b * K + i]) * q < p;
+      }
+    }
+    const uint32_t fallen = __ballot_sync(0xFFFFFFFFu, !stands);
+    if (fallen) kept = i0 + __ffs(fallen) - 1;
+  }
+
+  const T* p = target + static_cast<int64_t>(kept) * V;
+  const T* q = kept < n && draft ? draft + static_cast<int64_t>(kept) * V : nullptr;
+  int one = kept < n && !draft ? a.tokens[b * K + kept] : -1;
+  const double u = a.sample_u[b];
+  const int pieces = cluster * kVerifyWarps;
+  const int lo = min((rank * kVerifyWarps + warp) * a.piece, V);
+  const int hi = min(lo + a.piece, V);
+  int token = -1;
+  bool mine = false;  // this warp holds the draw
+  for (int pass = 0; pass < 2; ++pass) {
+    double s = 0.0;
+    for (int i = lo + 4 * lane; i < hi; i += 128) {
+      double w[4];
+      weights4(p, q, one, i, V, a.wide, w);
+      s += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    s = warp_sum(s);
+    if (lane == 0) sums[pass][warp] = s;
+    cluster_sync();
+    if (threadIdx.x < pieces)
+      all[threadIdx.x] =
+          ld_cluster_f64(&sums[pass][threadIdx.x % kVerifyWarps], threadIdx.x / kVerifyWarps);
+    __syncthreads();
+    double total = 0.0;
+    for (int i = 0; i < pieces; ++i) total += all[i];
+    if (total > 0.0) {
+      const double goal = u * total;
+      double before = 0.0;
+      int at = -1, last = 0;
+      double base = 0.0, last_base = 0.0;
+      for (int i = 0; i < pieces; ++i) {  // the first piece whose running sum passes the goal
+        if (all[i] > 0.0) { last = i; last_base = before; }
+        if (at < 0 && before + all[i] > goal) { at = i; base = before; }
+        before += all[i];
+      }
+      if (at < 0) { at = last; base = last_base; }
+      if (at == rank * kVerifyWarps + warp) {
+        mine = true;
+        double run = base;
+        for (int i0 = lo; i0 < hi; i0 += 128) {
+          double w[4] = {};
+          const int i = i0 + 4 * lane;
+          if (i < hi) weights4(p, q, one, i, V, a.wide, w);
+          const double four = (w[0] + w[1]) + (w[2] + w[3]);
+          double incl = four;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= o) incl += y;
+          }
+          // the last entry with weight so far: the answer where rounding keeps
+          // the piece's own running sum at the goal
+          const uint32_t some = __ballot_sync(0xFFFFFFFFu, four > 0.0);
+          if (some) {
+            const int src = 31 - __clz(some);
+            const int j = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;
+            token = __shfl_sync(0xFFFFFFFFu, i + j, src);
+          }
+          const uint32_t past = __ballot_sync(0xFFFFFFFFu, four > 0.0 && run + incl > goal);
+          if (past) {
+            const int src = __ffs(past) - 1;
+            double c = run + (incl - four);
+            int j = 0;
+            for (; j < 3; ++j) {
+              c += w[j];
+              if (w[j] > 0.0 && c > goal) break;
+            }
+            while (j > 0 && !(w[j] > 0.0)) --j;
+            token = __shfl_sync(0xFFFFFFFFu, i + j, src);
+            break;
+          }
+          run += __shfl_sync(0xFFFFFFFFu, incl, 31);
+        }
+      }
+      break;
+    }
+    // nothing left of p - q: draw from p
+    q = nullptr;
+    one = -1;
+    __syncthreads();
+  }
+  // no mass anywhere: the first warp writes token -1
+  bool any = false;
+  for (int i = 0; i < pieces; ++i) any = any || all[i] > 0.0;
+  if (!any && rank == 0 && warp == 0) mine = true;
+  if (mine) {
+    if (lane == 0) a.n_accepted[b] = kept;
+    for (int i = lane; i <= K; i += 32)
+      a.out_tokens[b * (K + 1) + i] = i < kept ? a.tokens[b * K + i] : i == kept ? token : -1;
+  }
+  cluster_sync();  // no block leaves while another reads its sums
+}
+
+}  // namespace
+
+cudaError_t launch_verify_drafts(const void* target, const void* draft, int probs_bf16,
+                                 const int32_t* tokens, const float* accept_u, const float* sample_u,
+                                 const int32_t* draft_lengths, int64_t B, int K, int V,
+                                 int32_t* n_accepted, int32_t* out_tokens, cudaStream_t stream) {
+  VerifyArgs a{};
+  a.target = target; a.draft = draft; a.tokens = tokens;
+  a.accept_u = accept_u; a.sample_u = sample_u; a.draft_lengths = draft_lengths;
+  a.B = B; a.K = K; a.V = V;
+  a.n_accepted = n_accepted; a.out_tokens = out_tokens;
+  // one block per 2048 entries, up to the portable cluster size
+  int cluster = 1;
+  while (cluster < kVerifyMaxCluster && cluster * 2048 < V) cluster *= 2;
+  const int pieces = cluster * kVerifyWarps;
+  a.piece = (((V + pieces - 1) / pieces) + 3) & ~3;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft);
+  a.wide = V % 4 == 0 && at % (probs_bf16 ? 8 : 16) == 0;
+
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(B * cluster));
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return probs_bf16 ? cudaLaunchKernelEx(&cfg, verify_drafts_kernel<uint16_t>, a, cluster)
+                    : cudaLaunchKernelEx(&cfg, verify_drafts_kernel<float>, a, cluster);
+}
+
+}  // namespace dwa
