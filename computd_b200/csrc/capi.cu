@@ -1017,7 +1017,8 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
   a.lengths = lengths; a.q_start = q_start; a.T = T;
   a.even = q_start ? 0 : static_cast<int>(T / B);
   a.max_q = max_q; a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  // not 0: minus infinity times it marks what a row may not see
+  a.scale_log2 = std::max(scale * 1.4426950408889634f, 1.1754944e-38f);
   a.status = status;
   cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dwa_paged_attention launch");

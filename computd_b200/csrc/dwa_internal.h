@@ -217,6 +217,7 @@ cudaError_t launch_kv_read(const KvCacheView& c, const int64_t* slots, int64_t T
                            void* v_out, int clear_skipped, int32_t* status, cudaStream_t stream);
 struct PagedArgs;
 cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream);
+cudaError_t launch_paged_attention_mma(const PagedArgs& a, cudaStream_t stream);
 cudaError_t launch_verify_drafts(const void* target, const void* draft, int probs_bf16,
                                  const int32_t* tokens, const float* accept_u, const float* sample_u,
                                  const int32_t* draft_lengths, int64_t B, int K, int V,

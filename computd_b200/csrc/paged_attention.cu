@@ -40,6 +40,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
+constexpr int kFewRows = 32;  // per key/value head; more go to the tcgen05 kernel
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -580,6 +581,7 @@ cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream) {
+  if (static_cast<int64_t>(a.max_q) * a.group > kFewRows) return launch_paged_attention_mma(a, stream);
   const bool e4m3 = a.k_scale != nullptr;
   if (a.d <= 64) return e4m3 ? launch_rows_nt<true, 64>(a, stream) : launch_rows_nt<false, 64>(a, stream);
   return e4m3 ? launch_rows_nt<true, 128>(a, stream) : launch_rows_nt<false, 128>(a, stream);
