@@ -30,67 +30,94 @@ _BF16, _E4M3, _F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32
 _I32, _I64 = torch.int32, torch.int64
 
 
-def _call(fn: str, device: torch.device, *args) -> None:
-    """One C call on `device`'s current stream, with that device current."""
-    lib = _lib.load()
-    index = device.index
-    if index == torch.cuda.current_device():
-        st = getattr(lib, fn)(*args, torch.cuda.current_stream(device).cuda_stream)
+# The stream and device numbers without the objects that torch.cuda.current_stream makes: a third
+# of a short call's time on the host.
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _call(fn: str, dev: int, *args) -> None:
+    """One C call on device `dev`'s current stream, with that device current."""
+    if dev == _current_device():
+        st = getattr(_lib.load(), fn)(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            st = getattr(lib, fn)(*args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(dev):
+            st = getattr(_lib.load(), fn)(*args, _raw_stream(dev))
     if st:
         _lib.check(st, fn)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 def _cache_args(k_cache, v_cache, k_scale, v_scale):
-    """(device, pointers and sizes of a cache as the C ABI takes them)."""
-    _need(k_cache.is_cuda, "k_cache must live on a CUDA device")
-    dtype, shape = k_cache.dtype, k_cache.shape
-    _need(dtype in (_BF16, _E4M3), "k_cache must be bfloat16 or float8_e4m3fn")
-    _need(len(shape) == 4, "k_cache must be [n_pages, H_kv, page_size, d]")
-    dev, stride = k_cache.device, k_cache.stride()
-    _need(v_cache.dtype == dtype and v_cache.shape == shape and v_cache.stride() == stride
-          and v_cache.device == dev, "v_cache must be like k_cache (type, shape, strides, device)")
+    """(device number, H_kv, d, pointers, sizes) of a cache as the C ABI takes them.
+
+    The checks here and below compare whole shapes and strides and format a message only
+    when they fail: a decoding step's calls are short."""
+    dev, dtype, shape, stride = k_cache.get_device(), k_cache.dtype, k_cache.shape, k_cache.stride()
+    if dev < 0:
+        raise ValueError("k_cache must live on a CUDA device")
+    if len(shape) != 4:
+        raise ValueError("k_cache must be [n_pages, H_kv, page_size, d]")
+    if (v_cache.dtype is not dtype or v_cache.shape != shape or v_cache.stride() != stride
+            or v_cache.get_device() != dev):
+        raise ValueError("v_cache must be like k_cache (type, shape, strides, device)")
     n_pages, heads, page, d = shape
-    _need((d == 1 or stride[3] == 1) and (page == 1 or stride[2] == d)
-          and (heads == 1 or stride[1] == page * d), "a cache's pages must be contiguous inside")
-    ld_page = stride[0] if n_pages > 1 else heads * page * d
-    if dtype is _BF16:
-        _need(k_scale is None and v_scale is None, "a bfloat16 cache has no scales")
-        return dev, (k_cache.data_ptr(), v_cache.data_ptr(), None, None), \
-            (n_pages, page, ld_page, 0), heads, d
-    _need(k_scale is not None and v_scale is not None, "a float8_e4m3fn cache needs k_scale and v_scale")
-    sstride = k_scale.stride()
-    for s in (k_scale, v_scale):
-        _need(s.dtype == _F32 and s.shape == shape[:3] and s.device == dev and s.stride() == sstride,
-              "k_scale and v_scale must be f32 [n_pages, H_kv, page_size] with the same strides on "
-              "the cache's device")
-    _need((page == 1 or sstride[2] == 1) and (heads == 1 or sstride[1] == page),
-          "the scales of a page must be contiguous")
-    return dev, (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()), \
-        (n_pages, page, ld_page, sstride[0] if n_pages > 1 else heads * page), heads, d
+    ld_page = stride[0]
+    if stride[1:] != (page * d, d, 1) or n_pages == 1:
+        ld_page = _strided_page(stride, shape, "a cache's pages must be contiguous inside")
+    if dtype is _E4M3:
+        if k_scale is None or v_scale is None:
+            raise ValueError("a float8_e4m3fn cache needs k_scale and v_scale")
+        sshape, sstride = shape[:3], k_scale.stride()
+        if (k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != sshape
+                or v_scale.shape != sshape or v_scale.stride() != sstride
+                or k_scale.get_device() != dev or v_scale.get_device() != dev):
+            raise ValueError("k_scale and v_scale must be f32 [n_pages, H_kv, page_size] with the same "
+                             "strides on the cache's device")
+        ld_scale = sstride[0]
+        if sstride[1:] != (page, 1) or n_pages == 1:
+            ld_scale = _strided_page(sstride, sshape, "the scales of a page must be contiguous")
+        return dev, heads, d, (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                               v_scale.data_ptr()), (n_pages, page, ld_page, ld_scale)
+    if dtype is not _BF16:
+        raise ValueError("k_cache must be bfloat16 or float8_e4m3fn")
+    if k_scale is not None or v_scale is not None:
+        raise ValueError("a bfloat16 cache has no scales")
+    return dev, heads, d, (k_cache.data_ptr(), v_cache.data_ptr(), None, None), \
+        (n_pages, page, ld_page, 0)
 
 
-def _int_arg(x, dtype, dim, dev, name):
-    _need(x.dtype == dtype and x.dim() == dim and x.device == dev
-          and (dim == 0 or x.shape[-1] <= 1 or x.stride(-1) == 1),
-          f"{name} must be a {dim}-D {dtype} tensor on the cache's device, contiguous along its last "
-          "dimension")
+def _strided_page(stride, shape, what):
+    """The distance between pages where a dimension of size 1 may have any stride."""
+    dense = 1
+    for size, step in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if size > 1 and step != dense:
+            raise ValueError(what)
+        dense *= size
+    return stride[0] if shape[0] > 1 else dense
+
+
+def _array(x, dtype, shape, dev, name):
+    """A contiguous tensor's pointer."""
+    if (x.dtype is not dtype or x.shape != shape or x.get_device() != dev or not x.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on the same device as the "
+                         f"others (got {x.dtype} {list(x.shape)} on {x.device})")
     return x.data_ptr()
 
 
-def _status_arg(status, dev):
-    if status is None:
-        return None
-    _need(status.dtype == _I32 and status.numel() == 1 and status.device == dev,
-          "status must be one int32 on the cache's device")
-    return status.data_ptr()
+def _status(x, dev):
+    if x.dtype is not _I32 or x.numel() != 1 or x.get_device() != dev:
+        raise ValueError("status must be one int32 on the cache's device")
+    return x.data_ptr()
+
+
+def _rows(x, dtypes, heads, d, dev, name):
+    """(T, strides of a token and a head) of [T, heads, d] rows."""
+    shape, stride = x.shape, x.stride()
+    if (x.dtype not in dtypes or len(shape) != 3 or shape[2] != d or x.get_device() != dev
+            or (heads is not None and shape[1] != heads) or stride[2] != 1):
+        raise ValueError(f"{name} must be [T, {heads or 'H'}, {d}] of {dtypes}, contiguous along d, on the "
+                         f"cache's device (got {x.dtype} {list(shape)}, strides {list(stride)}, on {x.device})")
+    # a dimension of size 1 may have any stride
+    return shape[0], stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else d
 
 
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -103,20 +130,14 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     scale = max(amax / 448, 2^-126) and codes e4m3(x / scale).  A vector with a NaN or
     an infinity reads back as NaN.  Slot -1 skips its token; where a slot is named
     twice the later token stays."""
-    dev, ptrs, sizes, heads, d = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    shape = k.shape
-    _need(k.dtype in (_BF16, _F32) and v.dtype == k.dtype, "k and v must both be bfloat16 or float32")
-    _need(len(shape) == 3 and shape[1] == heads and shape[2] == d and v.shape == shape,
-          f"k and v must be [T, {heads}, {d}]")
-    _need(k.device == dev and v.device == dev, "k and v must live on the cache's device")
-    ks, vs = k.stride(), v.stride()
-    _need(ks[2] == 1 and vs[2] == 1, "k and v must be contiguous along d")
-    T = shape[0]
-    slots_ptr = _int_arg(slots, _I64, 1, dev, "slots")
-    _need(slots.shape[0] == T, f"slots must have {T} entries")
+    dev, heads, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
+    T, k_tok, k_head = _rows(k, (_BF16, _F32), heads, d, dev, "k")
+    T_v, v_tok, v_head = _rows(v, (k.dtype,), heads, d, dev, "v")
+    if T_v != T:
+        raise ValueError("k and v must have the same number of tokens")
     _call("dwa_kv_write", dev, k.data_ptr(), v.data_ptr(), 1 if k.dtype is _BF16 else 0, T, heads, d,
-          ks[0] if T > 1 else 0, ks[1] if heads > 1 else 0, vs[0] if T > 1 else 0,
-          vs[1] if heads > 1 else 0, slots_ptr, *ptrs, *sizes, _status_arg(status, dev))
+          k_tok, k_head, v_tok, v_head, _array(slots, _I64, (T,), dev, "slots"), *ptrs, *sizes,
+          None if status is None else _status(status, dev))
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *,
@@ -127,20 +148,17 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
 
     With ``out`` (two contiguous tensors) the rows of slot -1 stay as they were; without
     it they are zeros."""
-    dev, ptrs, sizes, heads, d = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    slots_ptr = _int_arg(slots, _I64, 1, dev, "slots")
-    shape = (slots.shape[0], heads, d)
+    dev, heads, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
+    T = slots.shape[0] if slots.dim() == 1 else 0
+    slots_ptr = _array(slots, _I64, (T,), dev, "slots")
     if out is None:
-        k, v = (torch.empty(shape, dtype=_BF16, device=dev) for _ in range(2))
-        clear = 1
+        k, v = k_cache.new_empty((2, T, heads, d), dtype=_BF16).unbind(0)
+        k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
     else:
         k, v = out
-        clear = 0
-        for x in (k, v):
-            _need(x.dtype == _BF16 and x.shape == shape and x.is_contiguous() and x.device == dev,
-                  f"out must be two contiguous bfloat16 {list(shape)} on the cache's device")
-    _call("dwa_kv_read", dev, *ptrs, slots_ptr, shape[0], heads, d, *sizes, k.data_ptr(),
-          v.data_ptr(), clear, _status_arg(status, dev))
+        k_ptr, v_ptr = (_array(x, _BF16, (T, heads, d), dev, "out") for x in (k, v))
+    _call("dwa_kv_read", dev, *ptrs, slots_ptr, T, heads, d, *sizes, k_ptr, v_ptr,
+          1 if out is None else 0, None if status is None else _status(status, dev))
     return k, v
 
 
@@ -166,39 +184,37 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     What a row may not see does not reach it, NaN and infinities included.  (A new
     token's value that is not finite makes the rows that do see it not finite in its
     channel; an infinity may become NaN there.)"""
-    dev, ptrs, sizes, h_kv, d = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    shape = q.shape
-    _need(q.dtype == _BF16 and len(shape) == 3 and shape[2] == d and q.device == dev,
-          f"q must be a bfloat16 [T, H, {d}] on the cache's device")
-    T, heads, _ = shape
-    qs = q.stride()
-    _need(qs[2] == 1 and (heads <= 1 or qs[1] == d), "q must be contiguous over heads and d")
-    q_ld = qs[0] if T > 1 else heads * d
-    table_ptr = _int_arg(block_table, _I32, 2, dev, "block_table")
-    lengths_ptr = _int_arg(lengths, _I32, 1, dev, "lengths")
-    B, max_pages = block_table.shape
-    _need(lengths.shape[0] == B, f"lengths must have {B} entries")
-    start_ptr = None
-    if q_start is not None:
-        start_ptr = _int_arg(q_start, _I32, 1, dev, "q_start")
-        _need(q_start.shape[0] == B + 1, f"q_start must have {B + 1} entries")
+    dev, h_kv, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
+    T, q_ld, q_head = _rows(q, (_BF16,), None, d, dev, "q")
+    heads = q.shape[1]
+    table_shape = block_table.shape
+    if (block_table.dtype is not _I32 or len(table_shape) != 2 or block_table.get_device() != dev
+            or (table_shape[1] > 1 and block_table.stride(1) != 1)):
+        raise ValueError("block_table must be int32 [B, max_pages], contiguous along its rows, on the "
+                         "cache's device")
+    B, max_pages = table_shape
+    if q_start is None:
+        start_ptr = None
+        if max_q is None:
+            max_q = T // B if B else 0
+    else:
+        start_ptr = _array(q_start, _I32, (B + 1,), dev, "q_start")
         if max_q is None:
             max_q = T
-    elif max_q is None:
-        max_q = T // B if B else 0
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=dev)
+        out = q.new_empty((T, heads, d))
         out_ld = heads * d
     else:
-        _need(out.dtype == _BF16 and out.shape == shape and out.device == dev,
-              f"out must be a bfloat16 {list(shape)} on the cache's device")
-        os = out.stride()
-        _need(os[2] == 1 and (heads <= 1 or os[1] == d), "out must be contiguous over heads and d")
-        out_ld = os[0] if T > 1 else heads * d
-    _call("dwa_paged_attention", dev, q.data_ptr(), T, heads, d, q_ld, *ptrs, h_kv, *sizes, table_ptr,
-          block_table.stride(0) if B > 1 else max_pages, max_pages, lengths_ptr, start_ptr, B,
-          int(max_q), d ** -0.5 if scale is None else float(scale), out.data_ptr(), out_ld,
-          _status_arg(status, dev))
+        T_out, out_ld, out_head = _rows(out, (_BF16,), heads, d, dev, "out")
+        if T_out != T or out_head != d:
+            raise ValueError("out must be like q, contiguous over heads and d")
+    if q_head != d:
+        raise ValueError("q must be contiguous over heads and d")
+    _call("dwa_paged_attention", dev, q.data_ptr(), T, heads, d, q_ld or heads * d, *ptrs, h_kv, *sizes,
+          block_table.data_ptr(), block_table.stride(0) if B > 1 else max_pages, max_pages,
+          _array(lengths, _I32, (B,), dev, "lengths"), start_ptr, B, max_q,
+          d ** -0.5 if scale is None else scale, out.data_ptr(), out_ld or heads * d,
+          None if status is None else _status(status, dev))
     return out
 
 
@@ -217,33 +233,20 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor,
 
     Returns (n_accepted int32 [B], tokens int32 [B, K + 1]: the standing drafts, the drawn
     token, then -1)."""
-    _need(target_probs.is_cuda, "target_probs must live on a CUDA device")
-    dev, dtype = target_probs.device, target_probs.dtype
-    _need(dtype in (_F32, _BF16) and target_probs.dim() == 3 and target_probs.is_contiguous(),
-          "target_probs must be a contiguous float32 or bfloat16 [B, K + 1, V]")
-    B, K1, V = target_probs.shape
+    dev, dtype, shape = target_probs.get_device(), target_probs.dtype, target_probs.shape
+    if dev < 0:
+        raise ValueError("target_probs must live on a CUDA device")
+    if dtype not in (_F32, _BF16) or len(shape) != 3 or shape[1] < 1 or not target_probs.is_contiguous():
+        raise ValueError("target_probs must be a contiguous float32 or bfloat16 [B, K + 1, V]")
+    B, K1, V = shape
     K = K1 - 1
-    _need(K >= 0, "target_probs must have at least one position")
-    draft_ptr = None
-    if draft_probs is not None:
-        _need(draft_probs.dtype == dtype and draft_probs.shape == (B, K, V)
-              and draft_probs.is_contiguous() and draft_probs.device == dev,
-              f"draft_probs must be a contiguous {dtype} [{B}, {K}, {V}] on target_probs' device")
-        draft_ptr = draft_probs.data_ptr()
-    for x, want, shape, name in ((draft_tokens, _I32, (B, K), "draft_tokens"),
-                                 (accept_u, _F32, (B, K), "accept_u"),
-                                 (sample_u, _F32, (B,), "sample_u")):
-        _need(x.dtype == want and x.shape == shape and x.is_contiguous() and x.device == dev,
-              f"{name} must be a contiguous {want} {list(shape)} on target_probs' device")
-    lengths_ptr = None
-    if draft_lengths is not None:
-        _need(draft_lengths.dtype == _I32 and draft_lengths.shape == (B,)
-              and draft_lengths.is_contiguous() and draft_lengths.device == dev,
-              f"draft_lengths must be a contiguous int32 [{B}] on target_probs' device")
-        lengths_ptr = draft_lengths.data_ptr()
-    accepted = torch.empty((B,), dtype=_I32, device=dev)
-    tokens = torch.empty((B, K1), dtype=_I32, device=dev)
-    _call("dwa_verify_drafts", dev, target_probs.data_ptr(), draft_ptr, 1 if dtype is _BF16 else 0,
-          draft_tokens.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), lengths_ptr, B, K, V,
-          accepted.data_ptr(), tokens.data_ptr())
+    accepted = draft_tokens.new_empty((B,), dtype=_I32)
+    tokens = draft_tokens.new_empty((B, K1), dtype=_I32)
+    _call("dwa_verify_drafts", dev, target_probs.data_ptr(),
+          None if draft_probs is None else _array(draft_probs, dtype, (B, K, V), dev, "draft_probs"),
+          1 if dtype is _BF16 else 0, _array(draft_tokens, _I32, (B, K), dev, "draft_tokens"),
+          _array(accept_u, _F32, (B, K), dev, "accept_u"),
+          _array(sample_u, _F32, (B,), dev, "sample_u"),
+          None if draft_lengths is None else _array(draft_lengths, _I32, (B,), dev, "draft_lengths"),
+          B, K, V, accepted.data_ptr(), tokens.data_ptr())
     return accepted, tokens
