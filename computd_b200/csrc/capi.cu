@@ -911,8 +911,9 @@ dwa_status kv_cache_view(const char* fn, const void* k_cache, const void* v_cach
   if (ld_page % d != 0)
     return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: ld_page=%lld must be a multiple of d=%d", fn,
                 (long long)ld_page, d);
-  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || (k_scale && (!aligned(k_scale, 4) || !aligned(v_scale, 4))))
-    return fail(DWA_ERR_INVALID_ARG, "%s: caches must be 16-byte aligned (scales 4-byte)", fn);
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k_scale, 16) || !aligned(v_scale, 16) ||
+      (k_scale && ld_scale_page % 4 != 0))
+    return fail(DWA_ERR_INVALID_ARG, "%s: pages and their scales must be 16-byte aligned", fn);
   *out = dwa::KvCacheView{k_cache, v_cache, k_scale, v_scale, H, d, n_pages, page_size, ld_page,
                           k_scale ? ld_scale_page : 0};
   return DWA_OK;

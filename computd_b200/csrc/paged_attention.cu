@@ -1,29 +1,30 @@
 // paged_attention.cu — attention of a few new rows per key/value head over the
-// paged cache: decoding steps and drafted tokens (and any other chunk, slowly).
+// paged cache: decoding steps and drafted tokens.
 //
 // A row is one (new token, query head); the rows of a key/value head are
 // token-major, its `group` query heads side by side.  Bound by HBM: each
-// cached key and value is read once for up to 8 NT rows.
+// cached key and value is read once for up to 32 rows.
 //
 // The products are transposed so that the few rows lie along the 8 columns of
 // mma.m16n8k16: S^T = K Q^T takes 16 keys by 8 rows, O^T += V^T P^T takes 16
-// channels by 8 rows.  Both big operands go from global memory straight into
-// the fragments, without shared memory or a barrier: the order of the
-// summation index and of the output channels is free, so every lane loads 16
-// neighbouring bytes and whatever channels those are take the places the
-// fragment gives them (Q is loaded in the same order; the output channel of
-// each accumulator is known).  P^T is turned between the products by movmatrix.
-// Each warp keeps the next block's keys in flight while it works on this
-// block's values and the other way round.
+// channels by 8 rows.  The order of the summation index, of the keys in a tile and
+// of the output channels is free, so every lane takes its part of the big operands
+// as 16 neighbouring bytes and whatever channels those are get the places the
+// fragment has for them (Q is loaded in the same order; the channel of each
+// accumulator is known).  P^T is turned between the products by movmatrix.
 //
+// Each warp works alone on blocks of 16 (bf16) or 32 (e4m3) keys, which its own
+// ring of TMA copies brings, 8 KB at a time and three in flight (registers could
+// hold one: 137 us instead of 8x us for 64 ragged sequences of 16 x 128, bf16).
 // The context of one (sequence, head) is split over the warps of a cluster of
-// blocks, 16 or 32 keys at a time in turn, and joined through shared and
-// distributed shared memory in one launch, in a fixed order.
+// blocks, block by block in turn, and joined through shared and distributed shared
+// memory in one launch, in a fixed order.
 //
-// e4m3 codes become bf16 exactly: moving the 7 magnitude bits down by four
-// gives a bf16 of 2^-120 times the value (subnormals too), one product with
-// 2^120 puts it right.  The keys' scales multiply the scores, the values'
-// scales the probabilities.
+// bf16 caches: P is used as the sum of two bf16 parts, so that only the result's
+// rounding is left.  e4m3 caches: codes become fp16 exactly, Q is scaled per row by
+// a power of two into fp16 (nothing is lost), the keys' scales multiply the scores,
+// and P times the values' scales, relative to a running power of two, is rounded to
+// fp16 (2^-11).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -42,19 +43,21 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxCluster = 8;
 constexpr int kFewRows = 32;  // per key/value head; more go to the tcgen05 kernel
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+template <bool kF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+  if constexpr (kF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -63,34 +66,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+// Two e4m3 codes (the low or high half of w) as a pair of fp16, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int high) {
   uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  if (high)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(r) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+        : "=r"(r) : "r"(w));
   return r;
-}
-
-// Bytes 1 and 3 of w, e4m3, as a pair of bf16.
-__device__ __forceinline__ uint32_t e4m3_bytes13(uint32_t w) {
-  const uint32_t small = ((w >> 4) & 0x07F007F0u) | (w & 0x80008000u);
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(small), "r"(0x7B807B80u));  // 2^120
-  return r;
-}
-
-// 16 bytes that are read once.
-__device__ __forceinline__ uint4 ld16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
-               : "=r"(v.x), "=r"(v.y)
-               : "l"(p));
-  return v;
 }
 
 // The halves of w (the values of one key at two channels) that are not finite
@@ -134,27 +119,71 @@ __device__ __forceinline__ int ld_cluster_s32(const int* local, int rank) {
 
 // kE4m3: 8-bit cache.  DP: d rounded up to 64 or 128.  NT: column tiles of 8 rows.
 template <bool kE4m3, int DP, int NT>
-struct Cfg {
-  static constexpr int kSub = kE4m3 ? 2 : 1;     // 16-key tiles per block, so that a block is 4 KB
+struct RowsCfg {
+  static constexpr int kSub = kE4m3 ? 2 : 1;      // 16-key tiles per block
   static constexpr int kKeys = 16 * kSub;
-  static constexpr int kSteps = DP / 16;         // k-steps of S, channel tiles of O
+  static constexpr int kSteps = DP / 16;          // k-steps of S, channel tiles of O
   static constexpr int kRows = 8 * NT;
-  // 16-byte chunks of a key row held by one lane (of the 4 that share it)
-  static constexpr int kChunksK = kE4m3 ? DP / 64 : DP / 32;
-  static constexpr int kWordsK = 4 * kChunksK;   // per key
-  // words of a value row held by one lane (of the 8 that share it)
-  static constexpr int kWordsV = kE4m3 ? DP / 32 : DP / 16;
+  static constexpr int kRowBytes = kE4m3 ? DP : 128;              // of a TMA box
+  static constexpr int kHalves = kE4m3 ? 1 : DP / 64;             // boxes side by side
+  static constexpr int kBoxBytes = 16 * kRowBytes;
+  static constexpr int kBoxes = kSub * kHalves;                   // of K; as many of V
+  static constexpr int kStageBytes = 2 * kBoxes * kBoxBytes;
+  static constexpr int kScaleBytes = kE4m3 ? 2 * kSub * 64 : 0;
+  static constexpr int kStages = DP == 128 ? 3 : 4;
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kPartBytes = kWarps * kRows * DP * 4;      // takes the ring's place
+  static constexpr int kSmem = 1024 + (kRingBytes > kPartBytes ? kRingBytes : kPartBytes) +
+                               kWarps * kStages * kScaleBytes;
 };
 
+// Keys of the rows of a 16-key tile: row r of the fragment is key row_key(r & 7) + (r & 8).
+// With 128-byte rows swizzled by TMA this order keeps the 16-byte reads of both
+// operands free of bank conflicts: neighbouring rows differ in bit 2 (K), every second
+// row's keys differ above bit 0 (V).
+__device__ __forceinline__ int row_key(int r) { return (0x37156240 >> (4 * r)) & 7; }
+
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float lds4f(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                              int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
 template <bool kE4m3, int DP, int NT>
-__global__ void __launch_bounds__(kThreads)
-    paged_rows_kernel(const PagedArgs a, const int row_groups, const int cluster) {
-  using C = Cfg<kE4m3, DP, NT>;
-  // one partial per warp, then (in warp 0's place) one per block
-  __shared__ __align__(16) float part_o[kWarps][C::kRows][DP];
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
+                      const int row_groups, const int cluster) {
+  using C = RowsCfg<kE4m3, DP, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[kWarps][C::kStages];
   __shared__ float part_m[kWarps][C::kRows], part_l[kWarps][C::kRows];
   __shared__ float block_m[C::kRows], block_l[C::kRows];
   __shared__ int first_bad[DP];  // least key with a value that is not finite, by channel
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  // one partial per warp, then (in warp 0's place) one per block
+  float* const part_o = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)));
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -174,9 +203,9 @@ __global__ void __launch_bounds__(kThreads)
     // every group its own rows, and those row_groups groups further on: a
     // sequence with more rows than max_q has more than there are groups
     const int64_t stride = static_cast<int64_t>(row_groups) * C::kRows;
-    for (int64_t base = r0; base < all_rows; base += stride)
+    for (int64_t at = r0; at < all_rows; at += stride)
       for (int i = split * kThreads + threadIdx.x; i < C::kRows * a.d; i += cluster * kThreads) {
-        const int64_t row = base + i / a.d;
+        const int64_t row = at + i / a.d;
         if (row < all_rows)
           a.out[(seq.row0 + row / a.group) * a.out_ld +
                 (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
@@ -187,167 +216,203 @@ __global__ void __launch_bounds__(kThreads)
   const int vis_min = paged_visible(seq, static_cast<int>(r0 / a.group));
   const int vis_max = paged_visible(seq, static_cast<int>((r0 + rows - 1) / a.group));
 
+  // ------------------------------------------------ this warp's ring
+  const uint32_t ring = base + warp * C::kStages * C::kStageBytes;
+  const uint32_t scale_ring =
+      base + C::kSmem - 1024 - (kWarps - warp) * C::kStages * C::kScaleBytes;
+  const uint32_t bar0 = smem_u32(&full_bar[warp][0]);
+  if (lane == 0) {
+    for (int i = 0; i < C::kStages; ++i) mbar_init(bar0 + 8 * i, 1);
+    fence_mbar_init();
+  }
   for (int i = threadIdx.x; i < DP; i += kThreads) first_bad[i] = 0x7FFFFFFF;
   __syncthreads();
 
-  // Q^T fragments: lane (g, t) holds row 8 nt + g at the channels its key chunks have
+  const int n_blocks = (vis_max + C::kKeys - 1) / C::kKeys;
+  const int step = cluster * kWarps;
+  const int page_mask = (1 << a.page_log2) - 1;
+  const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
+  bool bad_page = false;
+  // Lane i < 2 kBoxes brings one box of K or V; for e4m3 lanes 4 to 7 the tiles' scales.
+  const int what = kE4m3 ? (lane >> 1) & 1 : lane / C::kHalves;  // 0: K, 1: V
+  const int sub = kE4m3 ? lane & 1 : 0, half = kE4m3 ? 0 : lane % C::kHalves;
+  const bool brings = kE4m3 ? lane < 8 : lane < 2 * C::kHalves;
+  // the page of this lane's tile of a block, looked up one block ahead of its use
+  auto look_up = [&](int block) -> int {
+    const int key = block * C::kKeys + 16 * sub;
+    return brings && key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
+  };
+  auto bring = [&](int block, int stage, int page) {
+    const int key = block * C::kKeys + 16 * sub;
+    const uint32_t bar = bar0 + 8 * stage;
+    if (lane == 0) {
+      const int tiles = min(C::kSub, (vis_max - block * C::kKeys + 15) >> 4);
+      mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles) *
+                                     (2 * C::kHalves * C::kBoxBytes + (kE4m3 ? 128 : 0)));
+    }
+    __syncwarp();
+    if (brings && key < vis_max) {
+      if (page < 0 || page >= a.n_pages) {  // page 0 in its place; the rows become NaN
+        bad_page = true;
+        page = 0;
+      }
+      if (!kE4m3 || lane < 4) {
+        tma_load_rows(ring + stage * C::kStageBytes +
+                          (what * C::kBoxes + (kE4m3 ? sub : half)) * C::kBoxBytes,
+                      what ? &map_v : &map_k, bar, 64 * half, key & page_mask, hk, page);
+      } else {
+        bulk_load(scale_ring + stage * C::kScaleBytes + (what * C::kSub + sub) * 64,
+                  (what ? a.v_scale : a.k_scale) + page * a.ld_scale_page +
+                      (static_cast<int64_t>(hk) << a.page_log2) + (key & page_mask),
+                  64, bar);
+      }
+    }
+  };
+  int block = split * kWarps + warp;
+  {
+    int at = block;
+    for (int i = 0; i < C::kStages && at < n_blocks; ++i, at += step) bring(at, i, look_up(at));
+  }
+  int next_page = look_up(min(block + C::kStages * step, n_blocks));
+
+  // ------------------------------------------------ Q^T fragments, visible counts
+  // lane (g, t) holds row 8 nt + g at the channels its key chunks have
+  constexpr int kChunk = kE4m3 ? 16 : 8;            // channels per 16 bytes
+  constexpr int kChunksK = DP / (4 * kChunk);       // of a key row, per lane
   uint32_t qf[NT][C::kSteps][2];
+  float factor[NT][2];                              // of the columns' scores, to log2 units
+  int vis[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = 8 * nt + g;
     const int64_t row = r0 + r;
     const uint16_t* src = a.q + (seq.row0 + row / a.group) * a.q_ld +
                           (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d;
+    uint32_t top = 0;
 #pragma unroll
-    for (int c = 0; c < C::kChunksK; ++c) {
-      const int at = (4 * c + t) * (kE4m3 ? 16 : 8);
-      uint32_t w[kE4m3 ? 8 : 4];
+    for (int c = 0; c < kChunksK; ++c)
 #pragma unroll
-      for (int i = 0; i < (kE4m3 ? 2 : 1); ++i) {
+      for (int i = 0; i < kChunk / 8; ++i) {
+        const int at = (4 * c + t) * kChunk + 8 * i;
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && at < a.d) x = __ldg(reinterpret_cast<const uint4*>(src + at) + i);
-        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
-      }
-      if constexpr (kE4m3) {
-        // a word of four codes gives its bytes 0 and 2, then 1 and 3
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[nt][4 * c + i][0] = __byte_perm(w[2 * i], w[2 * i + 1], 0x5410);
-          qf[nt][4 * c + i][1] = __byte_perm(w[2 * i], w[2 * i + 1], 0x7632);
+        if (r < rows && at < a.d) x = __ldg(reinterpret_cast<const uint4*>(src + at));
+        const int k = (c * kChunk + 8 * i) / 4;
+        qf[nt][k][0] = x.x; qf[nt][k][1] = x.y;
+        qf[nt][k + 1][0] = x.z; qf[nt][k + 1][1] = x.w;
+        if (kE4m3) {
+          top = max(top, max((x.x << 16) & 0x7FFF0000u, x.x & 0x7FFF0000u));
+          top = max(top, max((x.y << 16) & 0x7FFF0000u, x.y & 0x7FFF0000u));
+          top = max(top, max((x.z << 16) & 0x7FFF0000u, x.z & 0x7FFF0000u));
+          top = max(top, max((x.w << 16) & 0x7FFF0000u, x.w & 0x7FFF0000u));
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[nt][2 * c + (i >> 1)][i & 1] = w[i];
       }
-    }
-  }
-  // tokens each of this lane's columns (rows 8 nt + 2 t and + 1) may see
-  int vis[NT][2];
+    float f = a.scale_log2;
+    if constexpr (kE4m3) {
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      float f0, f1;
+      f = f16_row_scale(top, a.scale_log2, &f0, &f1);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+      for (int k = 0; k < C::kSteps; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          qf[nt][k][i] = pack_f16(__uint_as_float(qf[nt][k][i] << 16) * f0 * f1,
+                                  __uint_as_float(qf[nt][k][i] & 0xFFFF0000u) * f0 * f1);
+    }
+    // columns of this lane: rows 8 nt + 2 t and + 1
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int r = 8 * nt + 2 * t + j;
-      vis[nt][j] = r < rows ? paged_visible(seq, static_cast<int>((r0 + r) / a.group)) : 0;
+      factor[nt][j] = kE4m3 ? __shfl_sync(0xFFFFFFFFu, f, 4 * (2 * t + j)) : f;
+      const int rc = 8 * nt + 2 * t + j;
+      vis[nt][j] = rc < rows ? paged_visible(seq, static_cast<int>((r0 + rc) / a.group)) : 0;
     }
+  }
 
   float o[NT][C::kSteps][4] = {};
   float m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) { m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f; }
+  float v_ref = 0.f, v_mul = 0.f;  // a power of two above the values' scales; kPScale over it
 
-  const int n_blocks = (vis_max + C::kKeys - 1) / C::kKeys;
-  const int step = cluster * kWarps;
-  const int page_mask = (1 << a.page_log2) - 1;
-  const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
-  const int esize = kE4m3 ? 1 : 2;
-  bool bad_page = false;
-
-  uint32_t kw[C::kSub][2][C::kWordsK], vw[C::kSub][4][C::kWordsV];
-  float ks[C::kSub][2], vs[C::kSub][2];
-
-  // first vector (row of d) of a 16-key tile, -1 where the tile has no page
-  auto tile_vector = [&](int key, int64_t* scale_at) -> int64_t {
-    if (key >= vis_max) return -1;
-    const int page = __ldg(table + (key >> a.page_log2));
-    if (page < 0 || page >= a.n_pages) {
-      bad_page = true;
-      return -1;
-    }
-    const int64_t in_page = (static_cast<int64_t>(hk) << a.page_log2) + (key & page_mask);
-    *scale_at = page * a.ld_scale_page + in_page;
-    return page * a.ld_page + in_page * a.d;
+  // this lane's keys of a tile: rows g (and g + 8) of K, rows 2 t, 2 t + 1 (and + 8) of V
+  constexpr bool kSwizzled = C::kRowBytes == 128;
+  const int key_g = kSwizzled ? row_key(g) : g;
+  const int key_t[2] = {kSwizzled ? row_key(2 * t) : 2 * t, kSwizzled ? row_key(2 * t + 1) : 2 * t + 1};
+  auto chunk_at = [&](int key, int chunk) -> uint32_t {  // of a box
+    return key * C::kRowBytes + ((kSwizzled ? chunk ^ (key & 7) : chunk) << 4);
   };
-  auto load_k = [&](int block) {
+
+  int stage = 0, parity = 0;
+  for (; block < n_blocks; block += step) {
+    const int key0 = block * C::kKeys;
+    if (!mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr)) { bad_page = true; break; }
+    const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kBoxes * C::kBoxBytes;
+    const uint32_t sb = scale_ring + stage * C::kScaleBytes;
+    // two sums per score: half the chain of dependent products
+    float s[C::kSub][NT][4] = {}, s2[C::kSub][NT][4] = {};
 #pragma unroll
-    for (int s = 0; s < C::kSub; ++s) {
-      int64_t scale_at = 0;
-      const int64_t at = tile_vector(block * C::kKeys + 16 * s, &scale_at);
+    for (int u = 0; u < C::kSub; ++u) {
+      if constexpr (kE4m3) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const char* row = static_cast<const char*>(a.k) + (at + static_cast<int64_t>(g + 8 * i) * a.d) * esize;
+        for (int c = 0; c < kChunksK; ++c) {
+          const uint4 lo = lds16(kb + u * C::kBoxBytes + chunk_at(key_g, 4 * c + t));
+          const uint4 hi = lds16(kb + u * C::kBoxBytes + chunk_at(key_g + 8, 4 * c + t));
+          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-        for (int c = 0; c < C::kChunksK; ++c) {
-          const int chunk = 4 * c + t;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (at >= 0 && chunk * 16 < a.d * esize) x = ld16(row + 16 * chunk);
-          kw[s][i][4 * c] = x.x; kw[s][i][4 * c + 1] = x.y;
-          kw[s][i][4 * c + 2] = x.z; kw[s][i][4 * c + 3] = x.w;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t f[4] = {e4m3x2_f16x2(wl[i], 0), e4m3x2_f16x2(wh[i], 0),
+                                   e4m3x2_f16x2(wl[i], 1), e4m3x2_f16x2(wh[i], 1)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<true>(i & 1 ? s2[u][nt] : s[u][nt], f, qf[nt][4 * c + i][0],
+                             qf[nt][4 * c + i][1]);
+          }
         }
-        if constexpr (kE4m3) {
-          ks[s][i] = at >= 0 ? __ldg(a.k_scale + scale_at + g + 8 * i) : 0.f;
-          vs[s][i] = at >= 0 ? __ldg(a.v_scale + scale_at + g + 8 * i) : 0.f;
-        }
-      }
-    }
-  };
-  auto load_v = [&](int block) {
+      } else {
 #pragma unroll
-    for (int s = 0; s < C::kSub; ++s) {
-      int64_t scale_at = 0;
-      const int64_t at = tile_vector(block * C::kKeys + 16 * s, &scale_at);
+        for (int c = 0; c < kChunksK; ++c) {
+          const uint32_t box = kb + (c >> 1) * C::kBoxBytes;
+          const uint4 lo = lds16(box + chunk_at(key_g, 4 * (c & 1) + t));
+          const uint4 hi = lds16(box + chunk_at(key_g + 8, 4 * (c & 1) + t));
+          const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-        const char* row = static_cast<const char*>(a.v) + (at + static_cast<int64_t>(key) * a.d) * esize;
-        if constexpr (C::kWordsV == 2) {  // 8 codes
-          uint2 x = make_uint2(0, 0);
-          if (at >= 0 && 8 * g < a.d) x = ld8(row + 8 * g);
-          vw[s][i][0] = x.x; vw[s][i][1] = x.y;
-        } else {
-#pragma unroll
-          for (int c = 0; c < C::kWordsV / 4; ++c) {
-            const int chunk = 8 * c + g;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (at >= 0 && chunk * 16 < a.d * esize) x = ld16(row + 16 * chunk);
-            vw[s][i][4 * c] = x.x; vw[s][i][4 * c + 1] = x.y;
-            vw[s][i][4 * c + 2] = x.z; vw[s][i][4 * c + 3] = x.w;
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<false>(s[u][nt], f0, qf[nt][2 * c][0], qf[nt][2 * c][1]);
+            mma16816<false>(s2[u][nt], f1, qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
           }
         }
       }
     }
-  };
-
-  int block = split * kWarps + warp;
-  if (block < n_blocks) {
-    load_k(block);
-    load_v(block);
-  }
-  for (; block < n_blocks; block += step) {
-    const int key0 = block * C::kKeys;
-    const int next = block + step;
-    float s[C::kSub][NT][4] = {};
-#pragma unroll
-    for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-      for (int k = 0; k < C::kSteps; ++k) {
-        uint32_t f[4];
-        if constexpr (kE4m3) {
-          f[0] = e4m3_bytes13(kw[u][0][k] << 8);
-          f[1] = e4m3_bytes13(kw[u][1][k] << 8);
-          f[2] = e4m3_bytes13(kw[u][0][k]);
-          f[3] = e4m3_bytes13(kw[u][1][k]);
-        } else {
-          f[0] = kw[u][0][2 * k]; f[1] = kw[u][1][2 * k];
-          f[2] = kw[u][0][2 * k + 1]; f[3] = kw[u][1][2 * k + 1];
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16(s[u][nt], f, qf[nt][k][0], qf[nt][k][1]);
-      }
+    const bool edge = key0 + C::kKeys > vis_min;
     float sk[C::kSub][2], sv[C::kSub][2];
+    bool v_up = false;
+    if constexpr (kE4m3) {
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u)
+      for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sk[u][i] = kE4m3 ? ks[u][i] * a.scale_log2 : a.scale_log2;
-        sv[u][i] = kE4m3 ? vs[u][i] : 1.f;
-      }
-    if (next < n_blocks) load_k(next);
+        for (int i = 0; i < 2; ++i) {
+          sk[u][i] = lds4f(sb + u * 64 + 4 * (key_g + 8 * i));
+          sv[u][i] = lds4f(sb + (C::kSub + u) * 64 + 4 * (key_g + 8 * i));
+          if (edge && key0 + 16 * u + 8 * i + key_g >= vis_max) sv[u][i] = 0.f;
+          v_up = v_up || sv[u][i] > v_ref;
+        }
+    }
+    float v_shrink = 1.f;
+    if (kE4m3 && __any_sync(0xFFFFFFFFu, v_up)) {
+      float top = 0.f;  // of the numbers among the scales
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u) top = fmaxf(top, fmaxf(sv[u][0], sv[u][1]));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+      const float up = power_above(top);
+      v_shrink = v_ref == 0.f ? 0.f : v_ref / up;
+      v_ref = up;
+      v_mul = kPScale / up;
+    }
 
     // scores in units of log2, masked; the columns' maxima over the block
-    const bool edge = key0 + C::kKeys > vis_min;
-    uint32_t pb[C::kSub][NT][2];
-    bool moved = false;
+    bool moved = kE4m3 && v_shrink != 1.f;
     float shrink[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -358,8 +423,9 @@ __global__ void __launch_bounds__(kThreads)
         for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float x = s[u][nt][2 * i + j] * sk[u][i];
-            if (edge && key0 + 16 * u + 8 * i + g >= vis[nt][j]) x = -INFINITY;
+            float x = (s[u][nt][2 * i + j] + s2[u][nt][2 * i + j]) *
+                      (kE4m3 ? sk[u][i] * factor[nt][j] : factor[nt][j]);
+            if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) x = -INFINITY;
             s[u][nt][2 * i + j] = x;
             top = fmaxf(top, x);
           }
@@ -373,86 +439,126 @@ __global__ void __launch_bounds__(kThreads)
           m[nt][j] = top;
           moved = true;
         }
-        const float base = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+        const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
         float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p = fast_exp2(s[u][nt][2 * i + j] - base);
+            float p = fast_exp2(s[u][nt][2 * i + j] - ref);
             sum += p;
-            // a masked key's scale may be anything: its weight is 0, not 0 times that
-            s[u][nt][2 * i + j] =
-                edge && key0 + 16 * u + 8 * i + g >= vis[nt][j] ? 0.f : p * sv[u][i];
+            if constexpr (kE4m3) {
+              p *= sv[u][i] * v_mul;
+              // a masked key's scale may be anything: its weight is 0, not 0 times that
+              if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) p = 0.f;
+            }
+            s[u][nt][2 * i + j] = p;
           }
         l[nt][j] = l[nt][j] * shrink[nt][j] + sum;
       }
-    // probabilities are rounded to bf16 for the tensor cores (2^-9 each, averaged
-    // over the keys); their sum l is kept in f32 from the unrounded ones
+    uint32_t pb[C::kSub][NT][2], pl[C::kSub][NT][2];
 #pragma unroll
     for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          pb[u][nt][i] = transpose8x8(pack_bf16(s[u][nt][2 * i], s[u][nt][2 * i + 1]));
+        for (int i = 0; i < 2; ++i) {
+          const float p0 = s[u][nt][2 * i], p1 = s[u][nt][2 * i + 1];
+          if constexpr (kE4m3) {
+            pb[u][nt][i] = transpose8x8(pack_f16(p0, p1));
+          } else {
+            const uint32_t big = pack_bf16(p0, p1);
+            pb[u][nt][i] = transpose8x8(big);
+            pl[u][nt][i] = transpose8x8(pack_bf16(p0 - __uint_as_float(big << 16),
+                                                  p1 - __uint_as_float(big & 0xFFFF0000u)));
+          }
+        }
     if (__any_sync(0xFFFFFFFFu, moved)) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = shrink[nt][0] * v_shrink, f1 = shrink[nt][1] * v_shrink;
 #pragma unroll
-        for (int k = 0; k < C::kSteps; ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[nt][k][j] *= shrink[nt][j & 1];
-    }
-    if constexpr (!kE4m3) {
-      if (edge) {  // keys that some row may not see: their values must not reach it as 0 * NaN
-#pragma unroll
-        for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 16 * u + 2 * t + (i & 1) + 8 * (i >> 1);
-#pragma unroll
-            for (int w = 0; w < C::kWordsV; ++w) {
-              const int ch = 8 * (8 * (w >> 2) + g) + 2 * (w & 3);
-              if (key >= vis_max) vw[u][i][w] = 0;
-              else if (key >= vis_min)
-                vw[u][i][w] = only_finite(vw[u][i][w], key, &first_bad[ch], &first_bad[ch + 1]);
-            }
-          }
+        for (int k = 0; k < C::kSteps; ++k) {
+          o[nt][k][0] *= f0; o[nt][k][1] *= f1;
+          o[nt][k][2] *= f0; o[nt][k][3] *= f1;
+        }
       }
     }
+    // 16 bytes (8 for e4m3 at 64 channels) of four keys' values at a time
+    constexpr int kPieces = kE4m3 ? 1 : DP / 64;
+    constexpr int kWords = kE4m3 && DP == 64 ? 2 : 4;
 #pragma unroll
     for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
-      for (int k = 0; k < C::kSteps; ++k) {
-        uint32_t f[4];
-        if constexpr (kE4m3) {
-          // tile k: channel 2 k of the chunk in rows 0..7, 2 k + 1 in rows 8..15
-          const int w = k >> 1;
-          const uint32_t lo = (k & 1) ? 0x6020u : 0x4000u;  // byte 2 (k & 1) of both keys
-          const uint32_t hi = (k & 1) ? 0x7030u : 0x5010u;
-          f[0] = e4m3_bytes13(__byte_perm(vw[u][0][w], vw[u][1][w], lo));
-          f[1] = e4m3_bytes13(__byte_perm(vw[u][0][w], vw[u][1][w], hi));
-          f[2] = e4m3_bytes13(__byte_perm(vw[u][2][w], vw[u][3][w], lo));
-          f[3] = e4m3_bytes13(__byte_perm(vw[u][2][w], vw[u][3][w], hi));
-        } else {
-          f[0] = __byte_perm(vw[u][0][k], vw[u][1][k], 0x5410);
-          f[1] = __byte_perm(vw[u][0][k], vw[u][1][k], 0x7632);
-          f[2] = __byte_perm(vw[u][2][k], vw[u][3][k], 0x5410);
-          f[3] = __byte_perm(vw[u][2][k], vw[u][3][k], 0x7632);
+      for (int c = 0; c < kPieces; ++c) {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key_t[i & 1] + 8 * (i >> 1);
+          if constexpr (kWords == 2) {
+            const uint2 x = lds8(vb + u * C::kBoxBytes + key * C::kRowBytes + 8 * g);
+            w[i][0] = x.x; w[i][1] = x.y;
+          } else {
+            const uint4 x = lds16(vb + (kE4m3 ? u : c) * C::kBoxBytes + chunk_at(key, g));
+            w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+          }
+          if (edge) {  // keys that some row may not see: their values must not reach it as 0 * NaN
+            const int at = key0 + 16 * u + key;
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) {
+              const int ch = 8 * (8 * c + g) + 2 * k;
+              if (at >= vis_max) w[i][k] = 0;
+              else if (!kE4m3 && at >= vis_min)
+                w[i][k] = only_finite(w[i][k], at, &first_bad[ch], &first_bad[ch + 1]);
+            }
+          }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[nt][k], f, pb[u][nt][0], pb[u][nt][1]);
+        for (int k = 0; k < kWords; ++k) {
+          if constexpr (kE4m3) {
+            // both keys' codes of a channel side by side, then four codes to fp16
+            const uint32_t a01 = __byte_perm(w[0][k], w[1][k], 0x5140);
+            const uint32_t b01 = __byte_perm(w[2][k], w[3][k], 0x5140);
+            const uint32_t a23 = __byte_perm(w[0][k], w[1][k], 0x7362);
+            const uint32_t b23 = __byte_perm(w[2][k], w[3][k], 0x7362);
+            const uint32_t f0[4] = {e4m3x2_f16x2(a01, 0), e4m3x2_f16x2(a01, 1),
+                                    e4m3x2_f16x2(b01, 0), e4m3x2_f16x2(b01, 1)};
+            const uint32_t f1[4] = {e4m3x2_f16x2(a23, 0), e4m3x2_f16x2(a23, 1),
+                                    e4m3x2_f16x2(b23, 0), e4m3x2_f16x2(b23, 1)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<true>(o[nt][2 * k], f0, pb[u][nt][0], pb[u][nt][1]);
+              mma16816<true>(o[nt][2 * k + 1], f1, pb[u][nt][0], pb[u][nt][1]);
+            }
+          } else {
+            const uint32_t f[4] = {
+                __byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<false>(o[nt][4 * c + k], f, pb[u][nt][0], pb[u][nt][1]);
+              mma16816<false>(o[nt][4 * c + k], f, pl[u][nt][0], pl[u][nt][1]);
+            }
+          }
+        }
       }
-    if (next < n_blocks) load_v(next);
+    __syncwarp();  // every lane has read the stage
+    const int ahead = block + C::kStages * step;
+    if (ahead < n_blocks) {
+      bring(ahead, stage, next_page);
+      next_page = look_up(min(ahead + step, n_blocks));
+    }
+    if (++stage == C::kStages) { stage = 0; parity ^= 1; }
   }
   if (__any_sync(0xFFFFFFFFu, bad_page)) {
     if (lane == 0) paged_report(a.status);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __uint_as_float(0x7FC00000u);
   }
+  __syncthreads();  // the rings' place is the partials' now
 
   // this warp's partial
+  const float v_back = kE4m3 ? v_ref / kPScale : 1.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -471,8 +577,8 @@ __global__ void __launch_bounds__(kThreads)
         for (int k = 0; k < C::kSteps; ++k) {
           // channels 2 k' and 2 k' + 1 of this lane's chunk
           const int ch = kE4m3 ? (DP / 8) * g + 2 * k : 8 * (8 * (k >> 2) + g) + 2 * (k & 3);
-          *reinterpret_cast<float2*>(&part_o[warp][r][ch]) =
-              make_float2(o[nt][k][j], o[nt][k][2 + j]);
+          *reinterpret_cast<float2*>(&part_o[(warp * C::kRows + r) * DP + ch]) =
+              make_float2(o[nt][k][j] * v_back, o[nt][k][2 + j] * v_back);
         }
       }
     }
@@ -489,7 +595,7 @@ __global__ void __launch_bounds__(kThreads)
       const float f = part_m[w][r] == -INFINITY ? 0.f : fast_exp2(part_m[w][r] - top);
       // a warp without keys has l = 0 (or NaN, after a bad page, which has to stay)
       sum += part_m[w][r] == -INFINITY ? part_l[w][r] : f * part_l[w][r];
-      const float2 p = *reinterpret_cast<const float2*>(&part_o[w][r][ch]);
+      const float2 p = *reinterpret_cast<const float2*>(&part_o[(w * C::kRows + r) * DP + ch]);
       x += f * p.x;
       y += f * p.y;
     }
@@ -498,9 +604,10 @@ __global__ void __launch_bounds__(kThreads)
       block_l[r] = sum;
     }
     // only this thread reads or writes these entries
-    *reinterpret_cast<float2*>(&part_o[0][r][ch]) = make_float2(x, y);
+    *reinterpret_cast<float2*>(&part_o[r * DP + ch]) = make_float2(x, y);
   }
-  cluster_sync();
+  if (cluster > 1) cluster_sync();
+  else __syncthreads();
   for (int i = split * kThreads + threadIdx.x; i < rows * (DP / 2); i += cluster * kThreads) {
     const int r = i / (DP / 2), ch = 2 * (i % (DP / 2));
     if (ch >= a.d) continue;
@@ -514,7 +621,7 @@ __global__ void __launch_bounds__(kThreads)
       if (c < cluster) {
         ms[c] = ld_cluster_f32(&block_m[r], c);
         ls[c] = ld_cluster_f32(&block_l[r], c);
-        os[c] = ld_cluster_f32x2(&part_o[0][r][ch], c);
+        os[c] = ld_cluster_f32x2(&part_o[r * DP + ch], c);
         if (!kE4m3) {
           bad0 = min(bad0, ld_cluster_s32(&first_bad[ch], c));
           bad1 = min(bad1, ld_cluster_s32(&first_bad[ch + 1], c));
@@ -540,42 +647,50 @@ __global__ void __launch_bounds__(kThreads)
                                  (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + ch) =
         pack_bf16(x, y);
   }
-  cluster_sync();  // no block leaves while another reads its partial
+  if (cluster > 1) cluster_sync();  // no block leaves while another reads its partial
 }
 
 template <bool kE4m3, int DP, int NT>
 cudaError_t launch_rows(const PagedArgs& a, int cluster, cudaStream_t stream) {
+  using C = RowsCfg<kE4m3, DP, NT>;
+  CUtensorMap mk, mv;
+  if (!make_page_map(&mk, a.k, a, C::kRowBytes, 16) || !make_page_map(&mv, a.v, a, C::kRowBytes, 16))
+    return cudaErrorInvalidValue;
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_groups = static_cast<int>((most_rows + 8 * NT - 1) / (8 * NT));
   const int64_t blocks = static_cast<int64_t>(a.B) * a.H_kv * row_groups * cluster;
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
+  if (cudaError_t e = allow_smem_once<paged_rows_kernel<kE4m3, DP, NT>>(C::kSmem); e != cudaSuccess)
+    return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(cluster);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_rows_kernel<kE4m3, DP, NT>, a, row_groups, cluster);
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, paged_rows_kernel<kE4m3, DP, NT>, mk, mv, a, row_groups, cluster);
 }
 
 template <bool kE4m3, int DP>
 cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
-  const int nt = most_rows <= 8 ? 1 : 2;
+  const int nt = most_rows <= 8 ? 1 : most_rows <= 16 ? 2 : 4;
   const int64_t units = static_cast<int64_t>(a.B) * a.H_kv * ((most_rows + 8 * nt - 1) / (8 * nt));
   // split a context until there are some blocks for every SM, while each warp
   // keeps two blocks of keys
   const int64_t keys = static_cast<int64_t>(a.max_pages) << a.page_log2;
   int cluster = 1;
   while (cluster < kMaxCluster && units * cluster < 4ll * device_sm_count() &&
-         keys > 2ll * cluster * kWarps * Cfg<kE4m3, DP, 1>::kKeys)
+         keys > 2ll * cluster * kWarps * RowsCfg<kE4m3, DP, 1>::kKeys)
     cluster *= 2;
-  return nt == 1 ? launch_rows<kE4m3, DP, 1>(a, cluster, stream)
-                 : launch_rows<kE4m3, DP, 2>(a, cluster, stream);
+  return nt == 1   ? launch_rows<kE4m3, DP, 1>(a, cluster, stream)
+         : nt == 2 ? launch_rows<kE4m3, DP, 2>(a, cluster, stream)
+                   : launch_rows<kE4m3, DP, 4>(a, cluster, stream);
 }
 
 }  // namespace

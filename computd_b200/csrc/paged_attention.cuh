@@ -3,7 +3,9 @@
 // paged_attention_mma.cu: many).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace dwa {
@@ -66,6 +68,64 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
 // Tokens that new token i may see.
 __device__ __forceinline__ int paged_visible(const PagedSeq& s, int i) {
   return max(s.length - s.n + i + 1, 0);
+}
+
+// ---------------------------------------------------------------- arithmetic
+// ex2.approx: 2 ulp of f32, far below the probabilities' own rounding.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// e4m3 caches: P times a value's scale over a running power of two, times this,
+// stays below 65504 with P up to 2^4, and keeps fp16's 11 bits down to 2^-25.
+constexpr float kPScale = 2048.f;
+
+// A row of Q goes into fp16 times the power of two that puts its largest
+// magnitude `top` (f32 bits) in [2^13, 2^14): what falls below fp16's range then is
+// 2^-37 of it.  The power comes as a product of two, either of which f32 holds.
+// Returns the factor of the row's scores (never 0: minus infinity times it has to
+// stay that).
+__device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, float* f0, float* f1) {
+  const int e = top == 0 || top >= 0x7F800000u ? 13 : static_cast<int>(top >> 23) - 127;
+  const int half = (13 - e) / 2, rest = 13 - e - half;
+  *f0 = __uint_as_float(static_cast<uint32_t>(127 + half) << 23);
+  *f1 = __uint_as_float(static_cast<uint32_t>(127 + rest) << 23);
+  return fmaxf(__uint_as_float(static_cast<uint32_t>(127 - half) << 23) *
+                   (scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - rest) << 23)),
+               0x1p-126f);
+}
+
+// The power of two above x (x >= 0), at least 2^-100.
+__device__ __forceinline__ float power_above(float x) {
+  return fmaxf(__uint_as_float(__float_as_uint(x) & 0x7F800000u) * 2.f, 0x1p-100f);
+}
+
+// Tensor map of one of the caches: boxes of `row_bytes` by `box_rows` tokens of one page's
+// head, 128-byte rows swizzled.  Channels beyond d arrive as zeros.
+bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows);
+
+// Lets a kernel have its dynamic shared memory, once per device.
+template <auto kKernel>
+cudaError_t allow_smem_once(int bytes) {
+  static std::atomic<bool> done[64] = {};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
 }
 
 }  // namespace dwa

@@ -43,13 +43,30 @@ namespace dwa {
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
+bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows) {
+  auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const bool e4m3 = a.k_scale != nullptr;
+  const uint64_t es = e4m3 ? 1 : 2;
+  const uint64_t page = 1ull << a.page_log2;
+  // a page's heads, then the pages; a single page may have any stride
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.d), page, static_cast<cuuint64_t>(a.H_kv),
+                        static_cast<cuuint64_t>(a.n_pages)};
+  cuuint64_t strides[3] = {a.d * es, page * a.d * es, a.ld_page * es};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes / es), static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 constexpr int kTile = 128;     // rows per tile, keys per step
 constexpr int kMaxChannels = 128;
 constexpr float kSlack = 4.f;  // log2 of how far P may grow before m follows
-// fp16 probabilities: times 2^11, with kSlack still below 65504
-constexpr float kPScale = 2048.f;
 
 template <bool kE4m3, int DP>
 struct MmaCfg {
@@ -153,21 +170,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack2_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 template <int kRegs>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -281,29 +283,21 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
             a.q + (u.seq.row0 + row / a.group) * a.q_ld +
             (static_cast<int64_t>(u.hk) * a.group + row % a.group) * a.d + 8 * c));
       if constexpr (kE4m3) {
-        // the row's largest magnitude goes to [2^13, 2^14): what falls below fp16's
-        // range then is 2^-37 of it
         uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7FFF0000u, w[k] & 0x7FFF0000u));
 #pragma unroll
         for (int o = kChunks / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        // factors in two steps: either may lie outside f32's range alone
-        const int e = top == 0 || top >= 0x7F800000u ? 13 : static_cast<int>(top >> 23) - 127;
-        const int half = (13 - e) / 2, rest = 13 - e - half;
-        const float f0 = __uint_as_float(static_cast<uint32_t>(127 + half) << 23);
-        const float f1 = __uint_as_float(static_cast<uint32_t>(127 + rest) << 23);
+        float f0, f1;
+        const float factor = f16_row_scale(top, a.scale_log2, &f0, &f1);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          w[k] = pack2_f16(__uint_as_float(w[k] << 16) * f0 * f1,
+          w[k] = pack_f16(__uint_as_float(w[k] << 16) * f0 * f1,
                            __uint_as_float(w[k] & 0xFFFF0000u) * f0 * f1);
         x = make_uint4(w[0], w[1], w[2], w[3]);
         if (c == 0)
-          sh.q_factor[r] = fmaxf(  // not 0: -infinity times it has to stay that
-              __uint_as_float(static_cast<uint32_t>(127 - half) << 23) *
-                  (a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - rest) << 23)),
-              0x1p-126f);
+          sh.q_factor[r] = factor;
       }
       const int tile = r / kTile, tr = r % kTile;
       *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (c >> 3) * C::kBlockBytes + tr * 128 +
@@ -494,12 +488,13 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         break;
       sh.scales[j & 3][it & 1][t] = scale;
       const uint8_t* src = smem + 2 * C::kTileBytes + C::kStages * C::kTileBytes + rs * C::kRawBytes;
+      constexpr int kSwizzle = DP == 128 ? 7 : 0;  // of the code tile's 128-byte rows
       uint8_t* dst = smem + 2 * C::kTileBytes + st * C::kTileBytes;
       constexpr int kChunks = DP / 16;  // 16 codes each
 #pragma unroll 4
       for (int i = t; i < kTile * kChunks; i += 128) {
         const int r = i / kChunks, c = i % kChunks;
-        uint4 x = *reinterpret_cast<const uint4*>(src + i * 16);
+        uint4 x = *reinterpret_cast<const uint4*>(src + r * DP + ((c ^ (r & kSwizzle)) << 4));
         if (j * kTile + r >= u.vis_max) x = make_uint4(0, 0, 0, 0);  // not this sequence's
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t o[8];
@@ -585,12 +580,11 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const bool move = top > m + kSlack || (m == -INFINITY && top > m) || (kE4m3 && v_top > v_ref);
       if (__any_sync(0xFFFFFFFFu, move)) {
         const float m_new = fmaxf(m, top);
-        const float shrink = m == -INFINITY ? 0.f : ex2(m - m_new);
+        const float shrink = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
         float shrink_o = shrink;
         if constexpr (kE4m3) {
           if (v_top > v_ref) {  // the next power of two (v_ref is warp-uniform)
-            const float up =
-                fmaxf(__uint_as_float(__float_as_uint(v_top) & 0x7F800000u) * 2.f, 0x1p-100f);
+            const float up = power_above(v_top);
             shrink_o = v_ref == 0.f ? 0.f : shrink * (v_ref / up);
             v_ref = up;
             v_mul = kPScale / up;
@@ -613,8 +607,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const int c = 2 * hf + c2;
-            float p0 = ex2(fmaf(s[c][k], factor, -base_m));
-            float p1 = ex2(fmaf(s[c][k + 1], factor, -base_m));
+            float p0 = fast_exp2(fmaf(s[c][k], factor, -base_m));
+            float p1 = fast_exp2(fmaf(s[c][k + 1], factor, -base_m));
             l0 += p0;
             l1 += p1;
             if constexpr (kE4m3) {
@@ -625,9 +619,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
                 if (key0 + 32 * c + k >= vis) p0 = 0.f;
                 if (key0 + 32 * c + k + 1 >= vis) p1 = 0.f;
               }
-              p[16 * c2 + (k >> 1)] = pack2_f16(p0, p1);
+              p[16 * c2 + (k >> 1)] = pack_f16(p0, p1);
             } else {
-              p[16 * c2 + (k >> 1)] = pack2_bf16(p0, p1);
+              p[16 * c2 + (k >> 1)] = pack_bf16(p0, p1);
             }
           }
         tmem_st_x32(ts + 32 * hf, p);
@@ -670,8 +664,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
               if (bad) x[q] = __uint_as_float(0x7FC00000u);
             }
             *reinterpret_cast<uint4*>(dst + 32 * c + k) =
-                make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]),
-                           pack2_bf16(x[6], x[7]));
+                make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
+                           pack_bf16(x[6], x[7]));
           }
         }
       }
@@ -685,23 +679,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, bool e4m3, int dp) {
-  auto encode = tensor_map_encoder();
-  if (!encode) return false;
-  const uint64_t es = e4m3 ? 1 : 2;
-  const uint64_t page = 1ull << a.page_log2;
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.d), page, static_cast<cuuint64_t>(a.H_kv),
-                        static_cast<cuuint64_t>(a.n_pages)};
-  cuuint64_t strides[3] = {a.d * es, page * a.d * es, a.ld_page * es};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(e4m3 ? dp : 64), static_cast<cuuint32_t>(page), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  return encode(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                e4m3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Once per device: the shared memory limit, and that the launch brings the
@@ -731,7 +708,8 @@ template <bool kE4m3, int DP>
 cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   using C = MmaCfg<kE4m3, DP>;
   CUtensorMap mk, mv;
-  if (!make_page_map(&mk, a.k, a, kE4m3, DP) || !make_page_map(&mv, a.v, a, kE4m3, DP))
+  const int row_bytes = kE4m3 ? DP : 128, page = 1 << a.page_log2;
+  if (!make_page_map(&mk, a.k, a, row_bytes, page) || !make_page_map(&mv, a.v, a, row_bytes, page))
     return cudaErrorInvalidValue;
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_units = static_cast<int>((most_rows + 2 * kTile - 1) / (2 * kTile));
