@@ -15,7 +15,7 @@
 //
 // Each warp works alone on blocks of 16 (bf16) or 32 (e4m3) keys, which its own
 // ring of TMA copies brings, 8 KB at a time and three in flight (registers could
-// hold one: 137 us instead of 8x us for 64 ragged sequences of 16 x 128, bf16).
+// hold one: 137 us instead of XX us for 64 ragged sequences of 16 x 128, bf16).
 // The context of one (sequence, head) is split over the warps of a cluster of
 // blocks, block by block in turn, and joined through shared and distributed shared
 // memory in one launch, in a fixed order.
@@ -38,10 +38,10 @@ namespace dwa {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxCluster = 8;
-constexpr int kFewRows = 32;  // per key/value head; more go to the tcgen05 kernel
+constexpr int kMaxCluster = 16;
+// Rows per key/value head that this kernel takes; more go to the tcgen05 kernel.  At 20
+// rows (16 sequences of 4096, 8 heads of 128, bf16) that one takes 81 us, this one 165.
+constexpr int kFewRows = 16;
 
 template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -118,8 +118,10 @@ __device__ __forceinline__ int ld_cluster_s32(const int* local, int rank) {
 }
 
 // kE4m3: 8-bit cache.  DP: d rounded up to 64 or 128.  NT: column tiles of 8 rows.
-template <bool kE4m3, int DP, int NT>
+// W: warps per block.
+template <bool kE4m3, int DP, int NT, int W>
 struct RowsCfg {
+  static constexpr int kWarps = W, kThreads = 32 * W;
   static constexpr int kSub = kE4m3 ? 2 : 1;      // 16-key tiles per block
   static constexpr int kKeys = 16 * kSub;
   static constexpr int kSteps = DP / 16;          // k-steps of S, channel tiles of O
@@ -130,7 +132,7 @@ struct RowsCfg {
   static constexpr int kBoxes = kSub * kHalves;                   // of K; as many of V
   static constexpr int kStageBytes = 2 * kBoxes * kBoxBytes;
   static constexpr int kScaleBytes = kE4m3 ? 2 * kSub * 64 : 0;
-  static constexpr int kStages = DP == 128 ? 3 : 4;
+  static constexpr int kStages = DP == 128 ? 2 : 3;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kPartBytes = kWarps * kRows * DP * 4;      // takes the ring's place
   static constexpr int kSmem = 1024 + (kRingBytes > kPartBytes ? kRingBytes : kPartBytes) +
@@ -170,12 +172,13 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
       : "memory");
 }
 
-template <bool kE4m3, int DP, int NT>
-__global__ void __launch_bounds__(kThreads, 2)
+template <bool kE4m3, int DP, int NT, int W>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
                       const int row_groups, const int cluster) {
-  using C = RowsCfg<kE4m3, DP, NT>;
+  using C = RowsCfg<kE4m3, DP, NT, W>;
+  constexpr int kWarps = W, kThreads = 32 * W;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[kWarps][C::kStages];
   __shared__ float part_m[kWarps][C::kRows], part_l[kWarps][C::kRows];
@@ -650,21 +653,18 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (cluster > 1) cluster_sync();  // no block leaves while another reads its partial
 }
 
-template <bool kE4m3, int DP, int NT>
-cudaError_t launch_rows(const PagedArgs& a, int cluster, cudaStream_t stream) {
-  using C = RowsCfg<kE4m3, DP, NT>;
+template <bool kE4m3, int DP, int NT, int W>
+cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStream_t stream) {
+  using C = RowsCfg<kE4m3, DP, NT, W>;
   CUtensorMap mk, mv;
   if (!make_page_map(&mk, a.k, a, C::kRowBytes, 16) || !make_page_map(&mv, a.v, a, C::kRowBytes, 16))
     return cudaErrorInvalidValue;
-  const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
-  const int row_groups = static_cast<int>((most_rows + 8 * NT - 1) / (8 * NT));
-  const int64_t blocks = static_cast<int64_t>(a.B) * a.H_kv * row_groups * cluster;
-  if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
-  if (cudaError_t e = allow_smem_once<paged_rows_kernel<kE4m3, DP, NT>>(C::kSmem); e != cudaSuccess)
-    return e;
+  if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
+  constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W>;
+  if (cudaError_t e = allow_smem_once<kKernel>(C::kSmem, true); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -673,24 +673,36 @@ cudaError_t launch_rows(const PagedArgs& a, int cluster, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, paged_rows_kernel<kE4m3, DP, NT>, mk, mv, a, row_groups, cluster);
+  const int row_groups = static_cast<int>(units / (static_cast<int64_t>(a.B) * a.H_kv));
+  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, row_groups, cluster);
+}
+
+// How a call is cut up: the longest context is split over 2^n blocks of 4 warps
+// until there are 6 blocks for every SM (3 reside) or a warp is left with fewer
+// than 8 steps, whose pipeline then hardly fills; below 2 blocks per SM it is split
+// down to 2 steps all the same.  What still leaves SMs without a block gets 8 warps
+// per block.  (Step: 32 keys of an e4m3 cache, 16 of a bf16 one.)
+template <bool kE4m3, int DP, int NT>
+cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stream) {
+  const int64_t sms = device_sm_count();
+  const int64_t steps = (static_cast<int64_t>(a.max_pages) << a.page_log2) / (kE4m3 ? 32 : 16);
+  int cluster = 1;
+  while (cluster < kMaxCluster) {
+    const int64_t blocks = units * cluster, per_warp = steps / (4 * 2 * cluster);
+    if (!(blocks < 2 * sms ? per_warp >= 2 : blocks < 6 * sms && per_warp >= 8)) break;
+    cluster *= 2;
+  }
+  return units * cluster <= sms && steps >= 16 * cluster
+             ? launch_rows<kE4m3, DP, NT, 8>(a, units, cluster, stream)
+             : launch_rows<kE4m3, DP, NT, 4>(a, units, cluster, stream);
 }
 
 template <bool kE4m3, int DP>
 cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
-  const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
-  const int nt = most_rows <= 8 ? 1 : most_rows <= 16 ? 2 : 4;
-  const int64_t units = static_cast<int64_t>(a.B) * a.H_kv * ((most_rows + 8 * nt - 1) / (8 * nt));
-  // split a context until there are some blocks for every SM, while each warp
-  // keeps two blocks of keys
-  const int64_t keys = static_cast<int64_t>(a.max_pages) << a.page_log2;
-  int cluster = 1;
-  while (cluster < kMaxCluster && units * cluster < 4ll * device_sm_count() &&
-         keys > 2ll * cluster * kWarps * RowsCfg<kE4m3, DP, 1>::kKeys)
-    cluster *= 2;
-  return nt == 1   ? launch_rows<kE4m3, DP, 1>(a, cluster, stream)
-         : nt == 2 ? launch_rows<kE4m3, DP, 2>(a, cluster, stream)
-                   : launch_rows<kE4m3, DP, 4>(a, cluster, stream);
+  const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
+  const int64_t heads = static_cast<int64_t>(a.B) * a.H_kv;
+  if (rows <= 8) return launch_rows_cut<kE4m3, DP, 1>(a, heads, stream);
+  return launch_rows_cut<kE4m3, DP, 2>(a, heads * ((rows + 15) / 16), stream);
 }
 
 }  // namespace

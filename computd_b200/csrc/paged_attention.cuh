@@ -116,14 +116,16 @@ __device__ __forceinline__ float power_above(float x) {
 // head, 128-byte rows swizzled.  Channels beyond d arrive as zeros.
 bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows);
 
-// Lets a kernel have its dynamic shared memory, once per device.
+// Lets a kernel have its dynamic shared memory (and clusters of 16), once per device.
 template <auto kKernel>
-cudaError_t allow_smem_once(int bytes) {
+cudaError_t allow_smem_once(int bytes, bool wide_clusters = false) {
   static std::atomic<bool> done[64] = {};
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
   if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
   cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && wide_clusters)
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
   return e;
 }
