@@ -66,18 +66,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// Two e4m3 codes (the low or high half of w) as a pair of fp16, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int high) {
-  uint32_t r;
-  if (high)
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
-        : "=r"(r) : "r"(w));
-  else
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
-        : "=r"(r) : "r"(w));
-  return r;
-}
-
 // The halves of w (the values of one key at two channels) that are not finite
 // become 0 and note the key.
 __device__ __forceinline__ uint32_t only_finite(uint32_t w, int key, int* first_lo, int* first_hi) {
@@ -90,31 +78,6 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w, int key, int* first_
     w &= 0x0000FFFFu;
   }
   return w;
-}
-
-__device__ __forceinline__ float ld_cluster_f32(const float* local, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];"
-               : "=f"(v)
-               : "r"(map_to_cta(smem_u32(local), rank))
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_f32x2(const float* local, int rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(map_to_cta(smem_u32(local), rank))
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ int ld_cluster_s32(const int* local, int rank) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];"
-               : "=r"(v)
-               : "r"(map_to_cta(smem_u32(local), rank))
-               : "memory");
-  return v;
 }
 
 // kE4m3: 8-bit cache.  DP: d rounded up to 64 or 128.  NT: column tiles of 8 rows.

@@ -8,6 +8,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "sm100_ptx.cuh"
+
 namespace dwa {
 
 struct PagedArgs {
@@ -88,6 +90,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
+// Two e4m3 codes (the low or high half of w) as a pair of fp16, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int high) {
+  uint32_t r;
+  if (high)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(r) : "r"(w));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+        : "=r"(r) : "r"(w));
+  return r;
+}
+
 // e4m3 caches: P times a value's scale over a running power of two, times this,
 // stays below 65504 with P up to 2^4, and keeps fp16's 11 bits down to 2^-25.
 constexpr float kPScale = 2048.f;
@@ -110,6 +124,41 @@ __device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, f
 // The power of two above x (x >= 0), at least 2^-100.
 __device__ __forceinline__ float power_above(float x) {
   return fmaxf(__uint_as_float(__float_as_uint(x) & 0x7F800000u) * 2.f, 0x1p-100f);
+}
+
+// ---------------------------------------------------------------- clusters
+// The same variable in block `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster_f32(const float* local, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];"
+               : "=f"(v)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f32x2(const float* local, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_cluster_s32(const int* local, int rank) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];"
+               : "=r"(v)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(const float* local, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return v;
 }
 
 // Tensor map of one of the caches: boxes of `row_bytes` by `box_rows` tokens of one page's

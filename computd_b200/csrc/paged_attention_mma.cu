@@ -4,27 +4,37 @@
 //
 // A block takes 256 rows of one key/value head (a row is one (new token, query
 // head), token-major) as two tiles of 128, and goes once over the keys they may
-// see, 128 at a time:
+// see (or its share of them), 128 at a time:
 //
-//   S_i = Q_i K^T        tcgen05, Q and K in shared memory, S_i in TMEM
-//   P_i = exp2(S_i - m)  one thread per row: running maximum, sum, P_i back to TMEM
-//   O_i += P_i V         tcgen05, P_i from TMEM, V in shared memory, O_i in TMEM
+//   S   = Q_i K^T          tcgen05, Q and K in shared memory, S in TMEM
+//   P_i = exp2(S - m)      one thread per row: running maximum, sum, P_i to TMEM
+//   O_i += P_i V           tcgen05, P_i from TMEM, V in shared memory, O_i in TMEM
 //
-// TMEM is full: two S of 128 columns (P_i takes the first half of S_i's), two O
-// of 128.  The tiles run in turn, so that one's products overlap the other's
-// exponentials: per 128 keys the two products take 2 x 1024 cycles of the tensor
-// pipe and the exponentials 32768 / 16 = 2048 cycles of the special-function
-// units.  m only moves when a row's maximum grew by more than 2^kSlack (the
-// result does not depend on m; P stays below 2^kSlack), so O is hardly ever
-// rescaled, and then by the row's own thread.
+// TMEM is full: one S of 128 columns that the tiles use in turn, two P of 64, two O
+// of 128.  A row's thread takes its 128 scores into registers at once, so that S is
+// free for the other tile's product while it works, and the next S is there when it
+// is done: the threads never wait for a product, only the tensor pipe for P.  (With
+// an S per tile that P overwrote, each step was a chain of product, exponentials,
+// product: 2.9 us per 2 x 128 rows x 128 keys of 128 channels instead of XXX.)
+// P is handed over in halves of 64 keys.
+//
+// Per step the products take 2048 cycles of the tensor pipe (8192 FLOP a cycle), the
+// exponentials 32768 / 16 = 2048 of the special-function units.  A quarter of them
+// is therefore computed as a polynomial, and everything else in pairs (f32x2).  m
+// only moves when a row's maximum grew by more than 2^kSlack (the result does not
+// depend on m; P stays below 2^kSlack), so O is hardly ever rescaled, and then by
+// the row's own thread.
 //
 // Warps 0-3 and 4-7: the rows of tile 0 and 1.  Warp 8: issues every tcgen05.mma.
-// Warp 9: TMA, one box of 64 channels per page, straight from the pages into the
-// swizzled operand tiles.  bf16 caches: warps 10-11 look over the values of tiles
-// that end behind what every row sees, since 0 * NaN would reach rows that must
-// not see it.  e4m3 caches: warps 12-15 turn codes into fp16 (exact) operand
-// tiles, Q is scaled per row by a power of two into fp16, and P carries the
-// values' scales relative to a running power of two.
+// Warp 9: TMA, straight from the pages into the swizzled operand tiles.  bf16
+// caches: warps 10-11 look over the values of tiles that end behind what every row
+// sees, since 0 * NaN would reach rows that must not see it.  e4m3 caches: warps
+// 12-15 turn codes into fp16 operand tiles (exact for keys, whose scales multiply the
+// scores; values times their scale relative to a running power of two, rounded to
+// 2^-11), and Q is scaled per row by a power of two into fp16.
+//
+// Where there are few units of 256 rows, a cluster of blocks shares the keys of one
+// and joins its parts through distributed shared memory, in a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -34,6 +44,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "dwa_internal.h"
 #include "paged_attention.cuh"
@@ -49,7 +60,6 @@ bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int ro
   const bool e4m3 = a.k_scale != nullptr;
   const uint64_t es = e4m3 ? 1 : 2;
   const uint64_t page = 1ull << a.page_log2;
-  // a page's heads, then the pages; a single page may have any stride
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.d), page, static_cast<cuuint64_t>(a.H_kv),
                         static_cast<cuuint64_t>(a.n_pages)};
   cuuint64_t strides[3] = {a.d * es, page * a.d * es, a.ld_page * es};
@@ -66,7 +76,11 @@ namespace {
 
 constexpr int kTile = 128;     // rows per tile, keys per step
 constexpr int kMaxChannels = 128;
+constexpr int kMaxSplit = 8;
 constexpr float kSlack = 4.f;  // log2 of how far P may grow before m follows
+// e4m3 caches: P in fp16 times 2^11 (with kSlack still below 65504), values times 64
+// over the power of two above their scales (448 * 64 is below it too).
+constexpr float kPBits = 11.f, kVScale = 64.f;
 
 template <bool kE4m3, int DP>
 struct MmaCfg {
@@ -76,40 +90,67 @@ struct MmaCfg {
   static constexpr int kHalves = DP / 64;               // 128-byte wide column blocks
   static constexpr int kBlockBytes = kTile * 128;       // one of them: 16 KB
   static constexpr int kTileBytes = kHalves * kBlockBytes;
-  static constexpr int kStages = kE4m3 ? 3 : 5;         // operand tiles (K and V in turn)
-  static constexpr int kRaw = kE4m3 ? 3 : 0;            // code tiles
-  static constexpr int kRawBytes = kTile * DP;
-  static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kTileBytes + kRaw * kRawBytes;
+  static constexpr int kStages = kE4m3 ? 4 : 5;         // operand tiles (K and V in turn)
+  // Codes arrive in the stage that their fp16 values will take: at 128 channels in the
+  // second column block, where row r's codes lie in row r's place; at 64 behind it.
+  static constexpr int kRawAt = DP == 128 ? kBlockBytes : kTileBytes;
+  static constexpr int kStageBytes = kTileBytes + (kE4m3 && DP == 64 ? kTile * DP : 0);
+  static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kStageBytes;
+  // at the end a split block's parts take Q's and the operands' place
+  static constexpr int kPartLd = DP + 4;                // floats per row of O
+  static constexpr int kPartBytes = 2 * kTile * (kPartLd + 2) * 4;
+  static_assert(kPartBytes <= 2 * kTileBytes + kStages * kStageBytes, "parts fit");
 };
 
 template <bool kE4m3>
 struct MmaShared {
-  uint64_t full[5], ready[5], empty[5], raw_full[3], raw_empty[3];
-  uint64_t s_ready[2], p_ready[2], done[2];
+  uint64_t full[5], ready[5], empty[5];
+  uint64_t s_ready[2], s_free, p_ready[2][2], p_free[2];
   uint32_t tmem;
   int abort;
   int bad_page;
   int any_bad;
-  int first_bad[kMaxChannels];  // least key with a value that is not finite
-  // e4m3 only: what a row of Q was divided by, with the scale; the keys' and
-  // values' scales of four steps
+  int first_bad[kMaxChannels];  // least key with a value that is not finite (e4m3: [0], whole vectors)
+  // e4m3 only: a row's factor of the scores; the keys' scales and v_ref of four steps
   float q_factor[kE4m3 ? 2 * kTile : 1];
-  __align__(16) float scales[kE4m3 ? 4 : 1][2][kE4m3 ? kTile : 4];
+  __align__(16) float k_scale[kE4m3 ? 4 : 1][kE4m3 ? kTile : 4];
+  float v_ref[4];
 };
 
 // ---------------------------------------------------------------- tcgen05 pieces
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// The issuing warp stays converged, so that addresses and descriptors live in uniform
+// registers; `one` is its elected lane.
+// D[tmem] (+)= A[smem] B[smem]^T
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t add) {
-  umma_bf16_ss(d, a, b, idesc, add);
+                                       uint32_t add, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+      : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t add) {
+                                       uint32_t add, uint32_t one) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add)
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(one)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -161,6 +202,26 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr, uint32_t block_byt
   return desc;
 }
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The start-address field; in a cluster an address has the block's rank above it.
+__device__ __forceinline__ uint32_t desc_addr(uint32_t addr) { return (addr >> 4) & 0x3FFFu; }
+__device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
                                             int y, int z, int w) {
   asm volatile(
@@ -168,6 +229,64 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
+}
+
+
+// ---------------------------------------------------------------- pairs of f32
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x for a pair without the special-function unit: x = n + f, |f| <= 1/2, by
+// adding 1.5 2^23 (+ 127, so that the sum's low bits shifted up are 2^n); 2^f by the
+// cubic with the least relative error on that interval (7.5e-5, found by iteratively
+// reweighted least squares; bf16 probabilities are rounded to 2^-9).  x is held at
+// -126, where P is nothing; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(max_nan(a, -126.f), max_nan(b, -126.f));
+  const uint64_t magic = pair(12582912.f + 127.f, 12582912.f + 127.f);
+  const uint64_t back = pair(-12582912.f - 127.f, -12582912.f - 127.f);
+  const uint64_t t = add2(x, magic);
+  const uint64_t f = fma2(add2(t, back), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(f, pair(0.05517166852951050f, 0.05517166852951050f),
+                    pair(0.2426111251115799f, 0.2426111251115799f));
+  y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
+  y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
+  unpair(t, a, b);
+  return mul2(y, pair(__uint_as_float(__float_as_uint(a) << 23),
+                      __uint_as_float(__float_as_uint(b) << 23)));
 }
 
 template <int kRegs>
@@ -179,87 +298,73 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// What a block works on.
-struct Unit {
-  PagedSeq seq;
-  int hk;
-  int64_t r0;        // its first row of the sequence's rows
-  int rows[2];       // rows of each tile
-  int steps[2];      // key tiles of each tile
-  int n_steps;       // of the block
-  int vis_min, vis_max;
-};
 
 template <bool kE4m3, int DP>
 __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const PagedArgs a, const int row_units) {
+                     const PagedArgs a, const int row_units, const int cluster) {
   using C = MmaCfg<kE4m3, DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ MmaShared<kE4m3> sh;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
-  // [Q tile 0][Q tile 1][operand stages][code stages]
-  const uint32_t s_stage = base + 2 * C::kTileBytes;
-  const uint32_t s_raw = s_stage + C::kStages * C::kTileBytes;
+  const uint32_t s_stage = base + 2 * C::kTileBytes;  // [Q tile 0][Q tile 1][stages]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ------------------------------------------------ the block's work
-  Unit u;
-  int64_t unit = blockIdx.x;
+  const int split = static_cast<int>(blockIdx.x % cluster);
+  int64_t unit = blockIdx.x / cluster;
   // late rows (more keys) first
   const int ru = row_units - 1 - static_cast<int>(unit / (static_cast<int64_t>(a.B) * a.H_kv));
   unit %= static_cast<int64_t>(a.B) * a.H_kv;
-  u.hk = static_cast<int>(unit % a.H_kv);
+  const int hk = static_cast<int>(unit % a.H_kv);
   const int b = static_cast<int>(unit / a.H_kv);
-  u.seq = paged_seq(a, b);
-  if (u.seq.bad && u.hk == 0 && ru == 0 && threadIdx.x == 0) paged_report(a.status);
-  const int64_t all_rows = static_cast<int64_t>(u.seq.n) * a.group;
-  u.r0 = static_cast<int64_t>(ru) * 2 * kTile;
-  if (u.r0 >= all_rows) return;
-  if (u.seq.bad) {
+  const PagedSeq seq = paged_seq(a, b);
+  if (seq.bad && hk == 0 && ru == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
+  const int64_t all_rows = static_cast<int64_t>(seq.n) * a.group;
+  const int64_t r0 = static_cast<int64_t>(ru) * 2 * kTile;
+  if (r0 >= all_rows) return;  // the whole cluster
+  if (seq.bad) {
     const int64_t stride = static_cast<int64_t>(row_units) * 2 * kTile;
-    for (int64_t r = u.r0; r < all_rows; r += stride)
-      for (int i = threadIdx.x; i < 2 * kTile * a.d; i += C::kThreads) {
+    for (int64_t r = r0; r < all_rows; r += stride)
+      for (int i = split * C::kThreads + threadIdx.x; i < 2 * kTile * a.d; i += cluster * C::kThreads) {
         const int64_t row = r + i / a.d;
         if (row < all_rows)
-          a.out[(u.seq.row0 + row / a.group) * a.out_ld +
-                (static_cast<int64_t>(u.hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
+          a.out[(seq.row0 + row / a.group) * a.out_ld +
+                (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
       }
     return;
   }
-  u.vis_min = paged_visible(u.seq, static_cast<int>(u.r0 / a.group));
-  u.vis_max = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t left = all_rows - u.r0 - i * kTile;
-    u.rows[i] = static_cast<int>(left < 0 ? 0 : left < kTile ? left : kTile);
-    u.steps[i] = 0;
-    if (u.rows[i] > 0) {
-      const int vis = paged_visible(
-          u.seq, static_cast<int>((u.r0 + i * kTile + u.rows[i] - 1) / a.group));
-      u.steps[i] = (vis + kTile - 1) / kTile;
-      u.vis_max = max(u.vis_max, vis);
-    }
-  }
-  u.n_steps = max(u.steps[0], u.steps[1]);
+  const int64_t left = all_rows - r0;
+  const int rows0 = static_cast<int>(min(left, static_cast<int64_t>(kTile)));
+  const int rows1 = static_cast<int>(max(min(left - kTile, static_cast<int64_t>(kTile)), int64_t{0}));
+  const int vis_min = paged_visible(seq, static_cast<int>(r0 / a.group));
+  const int vis0 = paged_visible(seq, static_cast<int>((r0 + rows0 - 1) / a.group));
+  const int vis1 =
+      rows1 > 0 ? paged_visible(seq, static_cast<int>((r0 + kTile + rows1 - 1) / a.group)) : 0;
+  const int vis_max = max(vis0, vis1);
+  // this block's share of the key tiles, and how far each row tile goes into it
+  const int tiles_all = (vis_max + kTile - 1) / kTile;
+  const int share = (tiles_all + cluster - 1) / cluster;
+  const int first_tile = min(split * share, tiles_all);
+  const int n_steps = min(share, tiles_all - first_tile);
+  const int steps0 = min(max((vis0 + kTile - 1) / kTile - first_tile, 0), n_steps);
+  const int steps1 = min(max((vis1 + kTile - 1) / kTile - first_tile, 0), n_steps);
 
   // ------------------------------------------------ set-up
   auto bar = [&](const uint64_t& x) { return smem_u32(&x); };
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(bar(sh.full[i]), 1);
-      mbar_init(bar(sh.ready[i]), kE4m3 ? 128 : 64);
+      mbar_init(bar(sh.ready[i]), kE4m3 ? 4 : 2);
       mbar_init(bar(sh.empty[i]), 1);
     }
-    for (int i = 0; i < C::kRaw; ++i) {
-      mbar_init(bar(sh.raw_full[i]), 1);
-      mbar_init(bar(sh.raw_empty[i]), 128);
-    }
+    mbar_init(bar(sh.s_free), 4);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(sh.s_ready[i]), 1);
-      mbar_init(bar(sh.p_ready[i]), 128);
-      mbar_init(bar(sh.done[i]), 1);
+      mbar_init(bar(sh.p_ready[i][0]), 4);
+      mbar_init(bar(sh.p_ready[i][1]), 4);
+      mbar_init(bar(sh.p_free[i]), 1);
     }
     sh.abort = 0;
     sh.bad_page = 0;
@@ -276,12 +381,12 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     constexpr int kChunks = DP / 8;  // per row; a row's threads are neighbours in a warp
     for (int i = threadIdx.x; i < 2 * kTile * kChunks; i += C::kThreads) {
       const int r = i / kChunks, c = i % kChunks;
-      const int64_t row = u.r0 + r;
+      const int64_t row = r0 + r;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (row < all_rows && 8 * c < a.d)
         x = __ldg(reinterpret_cast<const uint4*>(
-            a.q + (u.seq.row0 + row / a.group) * a.q_ld +
-            (static_cast<int64_t>(u.hk) * a.group + row % a.group) * a.d + 8 * c));
+            a.q + (seq.row0 + row / a.group) * a.q_ld +
+            (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + 8 * c));
       if constexpr (kE4m3) {
         uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t top = 0;
@@ -294,10 +399,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           w[k] = pack_f16(__uint_as_float(w[k] << 16) * f0 * f1,
-                           __uint_as_float(w[k] & 0xFFFF0000u) * f0 * f1);
+                          __uint_as_float(w[k] & 0xFFFF0000u) * f0 * f1);
         x = make_uint4(w[0], w[1], w[2], w[3]);
-        if (c == 0)
-          sh.q_factor[r] = factor;
+        if (c == 0) sh.q_factor[r] = factor;
       }
       const int tile = r / kTile, tr = r % kTile;
       *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (c >> 3) * C::kBlockBytes + tr * 128 +
@@ -308,252 +412,345 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-  const uint32_t tm_s[2] = {tmem, tmem + 128}, tm_o[2] = {tmem + 256, tmem + 384};
+  const uint32_t tm_s = sh.tmem, tm_p = sh.tmem + 128, tm_o = sh.tmem + 256;  // + 64 i, + 128 i
   int* const status = a.status;
   volatile int* const abort_flag = &sh.abort;
-  const int n_items = 2 * u.n_steps;
+  const int n_items = 2 * n_steps;
+  // a bounded wait of the whole warp, which goes on or gives up together
+  auto warp_wait = [&](const uint64_t& x, int phase) -> bool {
+    const uint32_t at = bar(x), parity = phase & 1;
+    // mostly it is over already: a test costs less than a wait with a time limit
+    if (__all_sync(0xFFFFFFFFu, mbar_test(at, parity))) return true;
+    return static_cast<bool>(__all_sync(0xFFFFFFFFu, mbar_wait(at, parity, status, abort_flag)));
+  };
+  // one arrival per warp, after every lane's accesses
+  auto warp_arrive = [&](const uint64_t& x) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(x));
+  };
 
   if (warp >= 8) {
-   regs_dec<C::kOtherRegs>();
-   if (warp == 9) {
-    // ------------------------------------------------ TMA: K_0 V_0 K_1 V_1 ...
-    const int per_tile = kTile >> a.page_log2;  // pages
-    const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
-    const int page_size = 1 << a.page_log2;
-    int issued = 0;
-    for (int it = 0; it < n_items; ++it) {
-      const int key0 = (it >> 1) * kTile;
-      constexpr int kRing = kE4m3 ? C::kRaw : C::kStages;
-      const int st = it % kRing;
-      const uint32_t full = kE4m3 ? bar(sh.raw_full[st]) : bar(sh.full[st]);
-      const uint32_t empty = kE4m3 ? bar(sh.raw_empty[st]) : bar(sh.empty[st]);
-      const int pages = min(per_tile, (u.vis_max - key0 + page_size - 1) >> a.page_log2);
-      int page = 0;
-      if (lane < pages) {
-        page = __ldg(table + (key0 >> a.page_log2) + lane);
-        if (page < 0 || page >= a.n_pages) {
-          sh.bad_page = 1;  // read page 0 in its place; the rows become NaN
-          page = 0;
+    regs_dec<C::kOtherRegs>();
+    if (warp == 9) {
+      // ---------------------------------------------- TMA: K V K V ...
+      const int page_size = 1 << a.page_log2;
+      const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
+      int issued = 0;
+      for (int it = 0; it < n_items; ++it) {
+        const int key0 = (first_tile + (it >> 1)) * kTile, st = it % C::kStages;
+        const int pages = min(kTile >> a.page_log2, (vis_max - key0 + page_size - 1) >> a.page_log2);
+        int page = 0;
+        if (lane < pages) {
+          page = __ldg(table + (key0 >> a.page_log2) + lane);
+          if (page < 0 || page >= a.n_pages) {
+            sh.bad_page = 1;  // read page 0 in its place; the rows become NaN
+            page = 0;
+          }
         }
-      }
-      if (it >= kRing && !mbar_wait(empty, ((it / kRing) - 1) & 1, status, abort_flag)) break;
-      __syncwarp();
-      const uint32_t box = static_cast<uint32_t>(page_size) * 128;
-      if (lane == 0)
-        mbar_arrive_expect_tx(full, static_cast<uint32_t>(pages) *
-                                        (kE4m3 ? static_cast<uint32_t>(page_size) * DP
-                                               : box * C::kHalves));
-      __syncwarp();
-      if (lane < pages) {
-        const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
-        if constexpr (kE4m3) {
-          tma_load_4d(s_raw + st * C::kRawBytes + lane * page_size * DP, map, full, 0, 0, u.hk, page);
-        } else {
+        if (it >= C::kStages && !warp_wait(sh.empty[st], it / C::kStages - 1)) break;
+        const uint32_t full = bar(sh.full[st]);
+        if (lane == 0)
+          mbar_arrive_expect_tx(full, static_cast<uint32_t>(pages * page_size) *
+                                          (kE4m3 ? DP : 128 * C::kHalves));
+        __syncwarp();
+        if (lane < pages) {
+          const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
+          const uint32_t dst = s_stage + st * C::kStageBytes;
+          if constexpr (kE4m3) {
+            tma_load_4d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, hk, page);
+          } else {
 #pragma unroll
-          for (int h = 0; h < C::kHalves; ++h)
-            tma_load_4d(s_stage + st * C::kTileBytes + h * C::kBlockBytes + lane * box, map, full,
-                        64 * h, 0, u.hk, page);
+            for (int h = 0; h < C::kHalves; ++h)
+              tma_load_4d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, hk,
+                          page);
+          }
         }
+        issued = it + 1;
       }
-      issued = it + 1;
-    }
-    // after an abort nobody else waits for the copies in flight
-    if (*abort_flag) {
-      constexpr int kRing = kE4m3 ? C::kRaw : C::kStages;
-      for (int it = max(0, issued - kRing); it < issued; ++it)
-        mbar_wait(kE4m3 ? bar(sh.raw_full[it % kRing]) : bar(sh.full[it % kRing]),
-                  (it / kRing) & 1, status, nullptr);
-    }
-  } else if (warp == 8) {
-    // ------------------------------------------------ tcgen05.mma
-    if (lane == 0) {
+      // after an abort nobody else waits for the copies in flight
+      if (*abort_flag) {
+        for (int it = max(0, issued - C::kStages); it < issued; ++it)
+          mbar_wait(bar(sh.full[it % C::kStages]), (it / C::kStages) & 1, status, nullptr);
+      }
+    } else if (warp == 8) {
+      // ---------------------------------------------- tcgen05.mma
       constexpr uint32_t kFormat = kE4m3 ? 0u : (1u << 7) | (1u << 10);  // fp16 or bf16 operands
       const uint32_t idesc_s = (1u << 4) | kFormat | (kTile / 8 << 17) | (kTile / 16 << 24);
       const uint32_t idesc_o = (1u << 4) | kFormat | (1u << 16) |
                                (static_cast<uint32_t>(a.d / 8) << 17) | (kTile / 16 << 24);
       const int k_steps = a.d / 16;
-      bool alive = true;
+      const uint32_t one = elect_one();
+      int used = 0;  // products that went through S
+      auto wait = [&](const uint64_t& x, uint32_t parity) {
+        const bool ok = warp_wait(x, parity);
+        tc_fence_after();
+        return ok;
+      };
       auto item_ready = [&](int it) {  // an operand tile is in shared memory
         const int st = it % C::kStages;
-        const uint32_t parity = (it / C::kStages) & 1;
         // bf16 keys come straight from the TMA, everything else through other warps
-        const uint32_t x = !kE4m3 && !(it & 1) ? bar(sh.full[st]) : bar(sh.ready[st]);
-        alive = alive && mbar_wait(x, parity, status, abort_flag);
-        return alive;
+        return wait(!kE4m3 && !(it & 1) ? sh.full[st] : sh.ready[st], (it / C::kStages) & 1);
       };
+      // Only a descriptor's start address changes: its low word by constants, so that the
+      // one issuing thread spends a few instructions per product (a loop that built
+      // descriptors took 150 cycles for each product of 64).
+      const uint32_t k_hi = static_cast<uint32_t>(sw128_kmajor_desc(0) >> 32);
+      const uint32_t k_lo = static_cast<uint32_t>(sw128_kmajor_desc(0));
+      const uint32_t v_hi = static_cast<uint32_t>(value_desc(0, C::kBlockBytes) >> 32);
+      const uint32_t v_lo = static_cast<uint32_t>(value_desc(0, C::kBlockBytes));
       auto scores = [&](int i, int j) {
-        const uint32_t q = base + i * C::kTileBytes;
-        const uint32_t k = s_stage + ((2 * j) % C::kStages) * C::kTileBytes;
-        for (int s = 0; s < k_steps; ++s) {
-          const uint32_t off = (s >> 2) * C::kBlockBytes + (s & 3) * 32;
-          mma_ss(tm_s[i], sw128_kmajor_desc(q + off), sw128_kmajor_desc(k + off), idesc_s, s > 0);
+        if (used > 0 && !wait(sh.s_free, (used - 1) & 1)) return false;
+        ++used;
+        const uint32_t q = k_lo + desc_addr(base + i * C::kTileBytes);
+        const uint32_t k = k_lo + desc_addr(s_stage + ((2 * j) % C::kStages) * C::kStageBytes);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          const uint32_t off = ((s >> 2) * C::kBlockBytes + (s & 3) * 32) >> 4;
+          if (s < k_steps)
+            mma_ss(tm_s, desc64(q + off, k_hi), desc64(k + off, k_hi), idesc_s, s > 0, one);
         }
-        umma_commit(bar(sh.s_ready[i]));
+        commit(bar(sh.s_ready[i]), one);
+        return true;
       };
       auto values = [&](int i, int j) {
-        const uint32_t v = s_stage + ((2 * j + 1) % C::kStages) * C::kTileBytes;
+        const uint32_t v = v_lo + desc_addr(s_stage + ((2 * j + 1) % C::kStages) * C::kStageBytes);
 #pragma unroll
-        for (int s = 0; s < kTile / 16; ++s)
-          mma_ts(tm_o[i], tm_s[i] + 8 * s, value_desc(v + s * 2048, C::kBlockBytes), idesc_o,
-                 j > 0 || s > 0);
-      };
-      if (u.n_steps > 0 && item_ready(0)) {
-        tc_fence_after();
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(sh.p_ready[i][h], j & 1)) return false;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (u.steps[i] > 0) scores(i, 0);
-        umma_commit(bar(sh.empty[0]));
-        for (int j = 0; j < u.n_steps && alive; ++j) {
-          if (!item_ready(2 * j + 1)) break;
-          if (j + 1 < u.n_steps && !item_ready(2 * j + 2)) break;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (j < u.steps[i]) {
-              if (!mbar_wait(bar(sh.p_ready[i]), j & 1, status, abort_flag)) { alive = false; break; }
-              tc_fence_after();
-              values(i, j);
-              if (j + 1 == u.steps[i]) umma_commit(bar(sh.done[i]));
-            }
-            if (i == 1) umma_commit(bar(sh.empty[(2 * j + 1) % C::kStages]));
-            if (j + 1 < u.steps[i]) scores(i, j + 1);
-          }
-          if (alive && j + 1 < u.n_steps) umma_commit(bar(sh.empty[(2 * j + 2) % C::kStages]));
+          for (int s = 4 * h; s < 4 * h + 4; ++s)
+            mma_ts(tm_o + 128 * i, tm_p + 64 * i + 8 * s, desc64(v + s * 128, v_hi), idesc_o,
+                   j > 0 || s > 0, one);
         }
+        commit(bar(sh.p_free[i]), one);
+        return true;
+      };
+      bool ok = n_steps > 0 && item_ready(0);
+      if (ok && steps0 > 0) ok = scores(0, 0);
+      if (ok && steps1 > 0) ok = scores(1, 0);
+      if (ok) commit(bar(sh.empty[0]), one);
+      for (int j = 0; j < n_steps && ok; ++j) {
+        if (j + 1 < n_steps) ok = item_ready(2 * j + 2);
+        if (ok && j + 1 < steps0) ok = scores(0, j + 1);
+        if (ok) ok = item_ready(2 * j + 1);
+        if (ok && j < steps0) ok = values(0, j);
+        if (ok && j + 1 < steps1) ok = scores(1, j + 1);
+        if (ok && j + 1 < n_steps) commit(bar(sh.empty[(2 * j + 2) % C::kStages]), one);
+        if (ok && j < steps1) ok = values(1, j);
+        if (ok) commit(bar(sh.empty[(2 * j + 1) % C::kStages]), one);
       }
-    }
-  } else if (!kE4m3 && warp >= 10) {
-    // ------------------------------------------------ values that not every row sees
-    const int t = threadIdx.x - 320;
-    for (int it = 0; it < n_items; ++it) {  // keys too: a stage holds either in turn
-      const int st = it % C::kStages, key0 = (it >> 1) * kTile;
-      if (!mbar_wait(bar(sh.full[st]), (it / C::kStages) & 1, status, abort_flag)) break;
-      if ((it & 1) && key0 + kTile > u.vis_min) {
-        uint8_t* v = smem + 2 * C::kTileBytes + st * C::kTileBytes;
-        const int first = max(u.vis_min - key0, 0);
-        for (int i = t; i < (kTile - first) * C::kHalves * 8; i += 64) {
-          const int pc = i & 7, r = first + (i >> 3) / C::kHalves, h = (i >> 3) % C::kHalves;
-          uint4* p = reinterpret_cast<uint4*>(v + h * C::kBlockBytes + r * 128 + pc * 16);
-          if (key0 + r >= u.vis_max) {
-            *p = make_uint4(0, 0, 0, 0);
-            continue;
+    } else if (!kE4m3 && warp >= 10) {
+      // ---------------------------------------------- values that not every row sees
+      const int t = threadIdx.x - 320;
+      for (int it = 0; it < n_items; ++it) {  // keys too: a stage holds either in turn
+        const int st = it % C::kStages, key0 = (first_tile + (it >> 1)) * kTile;
+        if (!warp_wait(sh.full[st], it / C::kStages)) break;
+        if ((it & 1) && key0 + kTile > vis_min) {
+          uint8_t* v = smem + 2 * C::kTileBytes + st * C::kStageBytes;
+          const int first = max(vis_min - key0, 0);
+          for (int i = t; i < (kTile - first) * C::kHalves * 8; i += 64) {
+            const int pc = i & 7, r = first + (i >> 3) / C::kHalves, h = (i >> 3) % C::kHalves;
+            uint4* p = reinterpret_cast<uint4*>(v + h * C::kBlockBytes + r * 128 + pc * 16);
+            if (key0 + r >= vis_max) {
+              *p = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            const uint4 x = *p;
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool found = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              found = found || (w[k] & 0x7F80u) == 0x7F80u || (w[k] & 0x7F800000u) == 0x7F800000u;
+            if (found) {
+              const int ch = h * 64 + ((pc ^ (r & 7)) << 3);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((w[k] & 0x7F80u) == 0x7F80u) {
+                  atomicMin(&sh.first_bad[ch + 2 * k], key0 + r);
+                  w[k] &= 0xFFFF0000u;
+                }
+                if ((w[k] & 0x7F800000u) == 0x7F800000u) {
+                  atomicMin(&sh.first_bad[ch + 2 * k + 1], key0 + r);
+                  w[k] &= 0x0000FFFFu;
+                }
+              }
+              sh.any_bad = 1;
+              *p = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
-          const uint4 x = *p;
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          bool found = false;
+          fence_proxy_async_smem();
+        }
+        warp_arrive(sh.ready[st]);
+      }
+    } else if (kE4m3 && warp >= 12) {
+      // ---------------------------------------------- codes to fp16 operand tiles, scales
+      // Warp w has rows 32 w .. 32 w + 31 of a tile, four lanes a row: codes 16 c .. and
+      // 64 + 16 c .. of it (c = lane & 3).  Neighbouring groups of four take rows r and
+      // r ^ 5, so that neither the reads nor the writes meet in a bank.
+      const int w = warp - 12, t = threadIdx.x - 384;
+      const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
+      const int c = lane & 3, pair_row = (lane >> 3) & 3;
+      const int row8 = (lane & 4) ? pair_row ^ 5 : pair_row;  // of eight
+      const int row0 = 32 * w + row8;
+      constexpr int kPer = DP / 64;                 // 16-byte pieces of codes per row and lane
+      constexpr int kSwizzle = DP == 128 ? 7 : 0;   // of the codes' 128-byte rows
+      float v_ref = 0.f;
+      // the scales of keys lane + 32 k of a tile, looked up one item ahead, their pages
+      // two: every warp needs their maximum
+      float scale[4];
+      int page[4];
+      auto pages_of = [&](int it) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int key = (first_tile + (it >> 1)) * kTile + lane + 32 * k;
+          page[k] = it < n_items && key < vis_max ? __ldg(table + (key >> a.page_log2)) : -1;
+        }
+      };
+      auto scales_of = [&](int it) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int key = (first_tile + (it >> 1)) * kTile + lane + 32 * k;
+          scale[k] = 0.f;
+          if (page[k] >= 0 && page[k] < a.n_pages)
+            scale[k] = __ldg(((it & 1) ? a.v_scale : a.k_scale) + page[k] * a.ld_scale_page +
+                             (static_cast<int64_t>(hk) << a.page_log2) +
+                             (key & ((1 << a.page_log2) - 1)));
+        }
+      };
+      pages_of(0);
+      scales_of(0);
+      pages_of(1);
+      for (int it = 0; it < n_items; ++it) {
+        const int st = it % C::kStages, j = it >> 1, key0 = (first_tile + j) * kTile;
+        float own = 0.f, top = 0.f;  // this warp's; the largest number among all
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k == w) own = scale[k];
+          top = fmaxf(top, scale[k]);
+        }
+        scales_of(it + 1);
+        pages_of(it + 2);
+        if (!warp_wait(sh.full[st], it / C::kStages)) break;
+        // What this step's slots held was last read in step j - 4, which is over
+        // since this stage, then step j - 2's, was free for the copy.
+        uint32_t mul = 0;  // of this lane's rows' values: fp16 pair per row, by shuffle
+        if (it & 1) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+          if (v_ref == 0.f || top > v_ref) v_ref = power_above(top);
+          if (t == 0) sh.v_ref[j & 3] = v_ref;
+          // a vector that is NaN and that some row must not see becomes zeros, and is noted
+          if (!(own < INFINITY) && key0 + t >= vis_min) {
+            if (key0 + t < vis_max) {
+              atomicMin(&sh.first_bad[0], key0 + t);
+              sh.any_bad = 1;
+            }
+            own = 0.f;
+          }
+          const float f = own * (kVScale / v_ref);
+          mul = pack_f16(f, f);
+        } else {
+          sh.k_scale[j & 3][t] = own;
+        }
+        uint8_t* stage = smem + 2 * C::kTileBytes + st * C::kStageBytes;
+        uint4 x[4][kPer];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int p = 0; p < kPer; ++p)
+            x[k][p] = *reinterpret_cast<const uint4*>(stage + C::kRawAt + (row0 + 8 * k) * DP +
+                                                      (((c + 4 * p) ^ (row8 & kSwizzle)) << 4));
+        if (key0 + kTile > vis_max) {  // rows from vis_max on are not this sequence's
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            found = found || (w[k] & 0x7F80u) == 0x7F80u || (w[k] & 0x7F800000u) == 0x7F800000u;
-          if (found) {
-            const int ch = h * 64 + ((pc ^ (r & 7)) << 3);
+            if (key0 + row0 + 8 * k >= vis_max)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if ((w[k] & 0x7F80u) == 0x7F80u) {
-                atomicMin(&sh.first_bad[ch + 2 * k], key0 + r);
-                w[k] &= 0xFFFF0000u;
-              }
-              if ((w[k] & 0x7F800000u) == 0x7F800000u) {
-                atomicMin(&sh.first_bad[ch + 2 * k + 1], key0 + r);
-                w[k] &= 0x0000FFFFu;
-              }
+              for (int p = 0; p < kPer; ++p) x[k][p] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();  // the rows' codes are read: their place may be written
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t f = __shfl_sync(0xFFFFFFFFu, mul, row8 + 8 * k);
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) {
+            const uint32_t u[4] = {x[k][p].x, x[k][p].y, x[k][p].z, x[k][p].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              o[e] = e4m3x2_f16x2(u[e >> 1], e & 1);
+              if (it & 1) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(o[e]), "r"(f));
             }
-            sh.any_bad = 1;
-            *p = make_uint4(w[0], w[1], w[2], w[3]);
+            uint8_t* row = stage + p * C::kBlockBytes + (row0 + 8 * k) * 128;
+            *reinterpret_cast<uint4*>(row + (((2 * c) ^ row8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row + (((2 * c + 1) ^ row8) << 4)) =
+                make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         fence_proxy_async_smem();
+        warp_arrive(sh.ready[st]);
       }
-      mbar_arrive(bar(sh.ready[st]));
     }
-  } else if (kE4m3 && warp >= 12) {
-    // ------------------------------------------------ codes to fp16 operand tiles, scales
-    const int t = threadIdx.x - 384;
-    const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
-    constexpr int kRaw = C::kRaw > 0 ? C::kRaw : 1;
-    for (int it = 0; it < n_items; ++it) {
-      const int st = it % C::kStages, rs = it % kRaw, j = it >> 1;
-      const int key = j * kTile + t;
-      // this thread's key's scale; the slot was last read in step j - 4, which is over
-      // before the operand stage that this tile goes to is free
-      float scale = 0.f;
-      if (key < u.vis_max) {
-        const int page = __ldg(table + (key >> a.page_log2));
-        if (page >= 0 && page < a.n_pages)
-          scale = __ldg(((it & 1) ? a.v_scale : a.k_scale) + page * a.ld_scale_page +
-                        (static_cast<int64_t>(u.hk) << a.page_log2) + (key & ((1 << a.page_log2) - 1)));
-      }
-      if (!mbar_wait(bar(sh.raw_full[rs]), (it / kRaw) & 1, status, abort_flag)) break;
-      if (it >= C::kStages &&
-          !mbar_wait(bar(sh.empty[st]), ((it / C::kStages) - 1) & 1, status, abort_flag))
-        break;
-      sh.scales[j & 3][it & 1][t] = scale;
-      const uint8_t* src = smem + 2 * C::kTileBytes + C::kStages * C::kTileBytes + rs * C::kRawBytes;
-      constexpr int kSwizzle = DP == 128 ? 7 : 0;  // of the code tile's 128-byte rows
-      uint8_t* dst = smem + 2 * C::kTileBytes + st * C::kTileBytes;
-      constexpr int kChunks = DP / 16;  // 16 codes each
-#pragma unroll 4
-      for (int i = t; i < kTile * kChunks; i += 128) {
-        const int r = i / kChunks, c = i % kChunks;
-        uint4 x = *reinterpret_cast<const uint4*>(src + r * DP + ((c ^ (r & kSwizzle)) << 4));
-        if (j * kTile + r >= u.vis_max) x = make_uint4(0, 0, 0, 0);  // not this sequence's
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t o[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-              static_cast<__nv_fp8x2_storage_t>(w[k >> 1] >> (16 * (k & 1))), __NV_E4M3);
-          o[k] = static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
-        }
-        uint8_t* row = dst + (c >> 2) * C::kBlockBytes + r * 128;
-        const int c0 = 2 * (c & 3);
-        *reinterpret_cast<uint4*>(row + ((c0 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(row + (((c0 + 1) ^ (r & 7)) << 4)) =
-            make_uint4(o[4], o[5], o[6], o[7]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(bar(sh.raw_empty[rs]));
-      mbar_arrive(bar(sh.ready[st]));
+    __syncwarp();
+    if (cluster > 1) {  // the parts are there; they have been read
+      cluster_sync();
+      cluster_sync();
     }
-   }
   } else {
     regs_inc<C::kSoftmaxRegs>();
     // ------------------------------------------------ softmax: one row per thread
     const int i = warp >> 2;
     const int r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t ts = tm_s[i] + lanes, to = tm_o[i] + lanes;
-    const int64_t row = u.r0 + i * kTile + r;
-    const bool live = r < u.rows[i];
-    const int vis = live ? paged_visible(u.seq, static_cast<int>(row / a.group)) : 0;
-    // least visible count in the tile: steps below it need no mask
-    const int vis_min = u.rows[i] == kTile
-        ? paged_visible(u.seq, static_cast<int>((u.r0 + i * kTile) / a.group)) : 0;
+    const uint32_t ts = tm_s + lanes, tp = tm_p + 64 * i + lanes, to = tm_o + 128 * i + lanes;
+    const int rows = i ? rows1 : rows0, steps = i ? steps1 : steps0;
+    const int64_t row = r0 + i * kTile + r;
+    const bool live = r < rows;
+    const bool warp_live = 32 * (warp & 3) < rows;
+    const int vis = live ? paged_visible(seq, static_cast<int>(row / a.group)) : 0;
+    // least visible count in the warp: steps below it need no mask
+    const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
     const float factor = kE4m3 ? sh.q_factor[i * kTile + r] : a.scale_log2;
-    float m = -INFINITY, l = 0.f;
-    float v_ref = 0.f, v_mul = 0.f;  // power of two at or above the values' scales; kPScale over it
+    float m = -INFINITY, l = 0.f, v_ref = 0.f;
     bool alive = true;
-    for (int j = 0; j < u.steps[i]; ++j) {
-      if (!mbar_wait(bar(sh.s_ready[i]), j & 1, status, abort_flag)) { alive = false; break; }
+    for (int j = 0; j < steps; ++j) {
+      if (!warp_wait(sh.s_ready[i], j)) { alive = false; break; }
       tc_fence_after();
-      const int key0 = j * kTile;
-      const bool edge = key0 + kTile > vis_min;
+      if (!warp_live) {  // no rows of its own: P's lanes hold what they hold, nobody reads O's
+        tc_fence_before();
+        warp_arrive(sh.s_free);
+        if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
+        warp_arrive(sh.p_ready[i][0]);
+        warp_arrive(sh.p_ready[i][1]);
+        continue;
+      }
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_async(ts + 32 * c, s[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld_pin(s[c]);
+      tc_fence_before();
+      warp_arrive(sh.s_free);
+      const int key0 = (first_tile + j) * kTile;
+      const bool edge = key0 + kTile > vis_low;
+      const float* ks = sh.k_scale[kE4m3 ? j & 3 : 0];
       if constexpr (kE4m3) {
         // the step's scales: the values' tile is converted right after the keys'
-        if (!mbar_wait(bar(sh.ready[(2 * j + 1) % C::kStages]), ((2 * j + 1) / C::kStages) & 1, status,
-                       abort_flag)) { alive = false; break; }
-      }
-      const float* ks = sh.scales[kE4m3 ? j & 3 : 0][0];
-      const float* vs = sh.scales[kE4m3 ? j & 3 : 0][1];
-      float s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_sync(ts + 32 * c, s[c]);
-      if constexpr (kE4m3) {
+        if (!warp_wait(sh.ready[(2 * j + 1) % C::kStages], (2 * j + 1) / C::kStages)) {
+          alive = false;
+          break;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
             const float4 x = *reinterpret_cast<const float4*>(ks + 32 * c + k);
-            s[c][k] *= x.x; s[c][k + 1] *= x.y; s[c][k + 2] *= x.z; s[c][k + 3] *= x.w;
+            float y[4];
+            unpair(mul2(pair(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), pair(x.x, x.y)),
+                   y[0], y[1]);
+            unpair(mul2(pair(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])),
+                        pair(x.z, x.w)), y[2], y[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[c][k + e] = __float_as_uint(y[e]);
           }
       }
       if (edge) {
@@ -561,34 +758,28 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if (key0 + 32 * c + k >= vis) s[c][k] = -INFINITY;
+            if (key0 + 32 * c + k >= vis) s[c][k] = 0xFF800000u;
       }
-      float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+      float top[4];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        t0 = fmaxf(t0, s[0][k]); t1 = fmaxf(t1, s[1][k]);
-        t2 = fmaxf(t2, s[2][k]); t3 = fmaxf(t3, s[3][k]);
+      for (int c = 0; c < 4; ++c) {
+        top[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+#pragma unroll
+        for (int k = 2; k < 32; k += 2)
+          top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       }
-      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * factor;
-      float v_top = 0.f;
-      if constexpr (kE4m3) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v_top = fmaxf(v_top, vs[lane + 32 * k]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xFFFFFFFFu, v_top, o));
-      }
-      const bool move = top > m + kSlack || (m == -INFINITY && top > m) || (kE4m3 && v_top > v_ref);
+      const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
+      const float v_now = kE4m3 ? sh.v_ref[j & 3] : 0.f;
+      if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
+      tc_fence_after();
+      const bool move = most > m + kSlack || (m == -INFINITY && most > m) || v_now != v_ref;
       if (__any_sync(0xFFFFFFFFu, move)) {
-        const float m_new = fmaxf(m, top);
+        const float m_new = fmaxf(m, most);
         const float shrink = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
         float shrink_o = shrink;
         if constexpr (kE4m3) {
-          if (v_top > v_ref) {  // the next power of two (v_ref is warp-uniform)
-            const float up = power_above(v_top);
-            shrink_o = v_ref == 0.f ? 0.f : shrink * (v_ref / up);
-            v_ref = up;
-            v_mul = kPScale / up;
-          }
+          shrink_o = v_ref == 0.f ? 0.f : shrink * (v_ref / v_now);
+          v_ref = v_now;
         }
         m = m_new;
         l *= shrink;
@@ -597,87 +788,160 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, shrink_o);
         }
       }
-      const float base_m = m == -INFINITY ? 0.f : m;
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
+      // fp16: P times kPScale, and l with it
+      const float ref = (m == -INFINITY ? 0.f : -m) + (kE4m3 ? kPBits : 0.f);
+      const uint64_t factor2 = pair(factor, factor), ref2 = pair(ref, ref);
+      uint64_t l2[2] = {0, 0};
+      auto half = [&](int h, auto masked) {
         uint32_t p[32];
 #pragma unroll
-        for (int c2 = 0; c2 < 2; ++c2)
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const int c = 2 * hf + c2;
-            float p0 = fast_exp2(fmaf(s[c][k], factor, -base_m));
-            float p1 = fast_exp2(fmaf(s[c][k + 1], factor, -base_m));
-            l0 += p0;
-            l1 += p1;
-            if constexpr (kE4m3) {
-              const float2 x = *reinterpret_cast<const float2*>(vs + 32 * c + k);
-              p0 *= x.x * v_mul;
-              p1 *= x.y * v_mul;
-              if (edge) {  // a masked key's scale may be anything
-                if (key0 + 32 * c + k >= vis) p0 = 0.f;
-                if (key0 + 32 * c + k + 1 >= vis) p1 = 0.f;
-              }
-              p[16 * c2 + (k >> 1)] = pack_f16(p0, p1);
-            } else {
-              p[16 * c2 + (k >> 1)] = pack_bf16(p0, p1);
-            }
+        for (int k = 0; k < 64; k += 2) {
+          const int c = 2 * h + (k >> 5);
+          const uint64_t x = fma2(pair(__uint_as_float(s[c][k & 31]), __uint_as_float(s[c][(k & 31) + 1])),
+                                  factor2, ref2);
+          float p0, p1;
+          uint64_t y;
+          if (!masked && (k >> 1) % 4 == 3) {
+            y = exp2_poly2(x);
+          } else {
+            unpair(x, p0, p1);
+            y = pair(fast_exp2(p0), fast_exp2(p1));
           }
-        tmem_st_x32(ts + 32 * hf, p);
+          l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], y);
+          unpair(y, p0, p1);
+          p[k >> 1] = kE4m3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+        }
+        tmem_st_x32(tp + 32 * h, p);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(sh.p_ready[i][h]);
+      };
+      if (edge) {
+        half(0, std::true_type{});
+        half(1, std::true_type{});
+      } else {
+        half(0, std::false_type{});
+        half(1, std::false_type{});
       }
+      float l0, l1;
+      unpair(add2(l2[0], l2[1]), l0, l1);
       l += l0 + l1;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(bar(sh.p_ready[i]));
     }
-    if (u.steps[i] > 0 && alive) alive = mbar_wait(bar(sh.done[i]), 0, status, abort_flag);
+    if (steps > 0 && alive) alive = warp_wait(sh.p_free[i], steps - 1);
     tc_fence_after();
     // ---------------------------------------------- out
-    const bool nothing = u.steps[i] == 0;
-    float inv = l == 0.f ? 0.f : 1.f / l;
-    if constexpr (kE4m3) inv *= v_ref / kPScale;
-    const bool bad = !alive || sh.bad_page;
-    const bool some_bad = !kE4m3 && sh.any_bad;
-    uint16_t* dst = a.out + (u.seq.row0 + row / a.group) * a.out_ld +
-                    (static_cast<int64_t>(u.hk) * a.group + row % a.group) * a.d;
+    const bool have = steps > 0 && alive;
+    if (!alive || sh.bad_page) l = __uint_as_float(0x7FC00000u);
+    if (sh.bad_page && threadIdx.x == 0) paged_report(a.status);
+    // O is in units of P's power of two, which l has too, and of the values'
+    const float v_back = kE4m3 ? v_ref / kVScale : 1.f;
+    if (cluster == 1) {
+      const float inv = (l == 0.f ? 0.f : 1.f / l) * v_back;
+      const bool some_bad = sh.any_bad;
+      uint16_t* dst = a.out + (seq.row0 + row / a.group) * a.out_ld +
+                      (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d;
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c) {
-      float o[32];
-      if (nothing || !alive) {
+      for (int c = 0; c < DP / 32; ++c) {
+        float o[32];
+        if (have && warp_live) {
+          tmem_ld_32x32b_x32_sync(to + 32 * c, o);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = 0.f;
-      } else {
-        tmem_ld_32x32b_x32_sync(to + 32 * c, o);
-      }
-      if (live) {
+          for (int k = 0; k < 32; ++k) o[k] = 0.f;
+        }
+        if (live) {
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          if (32 * c + k < a.d) {
-            float x[8];
+          for (int k = 0; k < 32; k += 8) {
+            if (32 * c + k < a.d) {
+              float x[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              x[q] = o[k + q] * inv;
-              // a row without keys has nothing in O
-              if (l == 0.f) x[q] = 0.f;
-              if (some_bad && sh.first_bad[32 * c + k + q] < vis) x[q] = __uint_as_float(0x7FC00000u);
-              if (bad) x[q] = __uint_as_float(0x7FC00000u);
+              for (int q = 0; q < 8; ++q) {
+                x[q] = l == 0.f ? 0.f : o[k + q] * inv;
+                if (some_bad && sh.first_bad[kE4m3 ? 0 : 32 * c + k + q] < vis) x[q] = __uint_as_float(0x7FC00000u);
+              }
+              *reinterpret_cast<uint4*>(dst + 32 * c + k) =
+                  make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
+                             pack_bf16(x[6], x[7]));
             }
-            *reinterpret_cast<uint4*>(dst + 32 * c + k) =
-                make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
-                           pack_bf16(x[6], x[7]));
           }
         }
       }
+    } else {
+      // this block's part: rows of O, then their m and l
+      float* part = reinterpret_cast<float*>(smem);
+      float* part_ml = part + 2 * kTile * C::kPartLd;
+      const int mine = i * kTile + r;
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // both tiles' products have read their operands
+      if (warp_live) {
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+          float o[32];
+          if (have) {
+            tmem_ld_32x32b_x32_sync(to + 32 * c, o);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4*>(part + mine * C::kPartLd + 32 * c + k) =
+                make_float4(o[k] * v_back, o[k + 1] * v_back, o[k + 2] * v_back, o[k + 3] * v_back);
+        }
+      }
+      part_ml[2 * mine] = m;
+      part_ml[2 * mine + 1] = l;
+      cluster_sync();
+      // the rows of a unit, dealt to the cluster's warps; a lane has four channels
+      constexpr int kWarps = 8;  // the others gave their registers away
+      for (int rr = split * kWarps + warp; rr < min(left, static_cast<int64_t>(2 * kTile));
+           rr += cluster * kWarps) {
+        float top = -INFINITY, f[kMaxSplit], ls[kMaxSplit];
+        int bad = 0;
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c)
+          if (c < cluster) {
+            f[c] = ld_cluster_f32(part_ml + 2 * rr, c);
+            ls[c] = ld_cluster_f32(part_ml + 2 * rr + 1, c);
+            bad |= ld_cluster_s32(&sh.any_bad, c);
+            top = fmaxf(top, f[c]);
+          }
+        float sum = 0.f, x[4] = {};
+        const int ch = 4 * lane;
+        if (ch < a.d) {
+#pragma unroll
+          for (int c = 0; c < kMaxSplit; ++c)
+            if (c < cluster) {
+              // a part without keys has l = 0 (or NaN, which has to stay)
+              const float w = f[c] == -INFINITY ? 0.f : fast_exp2(f[c] - top);
+              sum += f[c] == -INFINITY ? ls[c] : w * ls[c];
+              const float4 y = ld_cluster_f32x4(part + rr * C::kPartLd + ch, c);
+              x[0] += w * y.x; x[1] += w * y.y; x[2] += w * y.z; x[3] += w * y.w;
+            }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const int64_t row = r0 + rr;
+          const int vis = paged_visible(seq, static_cast<int>(row / a.group));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] *= inv;
+            if (bad) {
+              for (int c = 0; c < cluster; ++c)
+                if (ld_cluster_s32(&sh.first_bad[kE4m3 ? 0 : ch + e], c) < vis) x[e] = __uint_as_float(0x7FC00000u);
+            }
+          }
+          *reinterpret_cast<uint2*>(a.out + (seq.row0 + row / a.group) * a.out_ld +
+                                    (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + ch) =
+              make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        }
+        __syncwarp();
+      }
+      cluster_sync();  // no block leaves while another reads its part
     }
-    if (sh.bad_page && threadIdx.x == 0) paged_report(a.status);
     tc_fence_before();
   }
-  __syncwarp();
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(sh.tmem, 512);
   }
 }
 
@@ -708,17 +972,40 @@ template <bool kE4m3, int DP>
 cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   using C = MmaCfg<kE4m3, DP>;
   CUtensorMap mk, mv;
-  const int row_bytes = kE4m3 ? DP : 128, page = 1 << a.page_log2;
-  if (!make_page_map(&mk, a.k, a, row_bytes, page) || !make_page_map(&mv, a.v, a, row_bytes, page))
+  const int row_bytes = kE4m3 ? DP : 128, box_rows = 1 << a.page_log2;
+  if (!make_page_map(&mk, a.k, a, row_bytes, box_rows) ||
+      !make_page_map(&mv, a.v, a, row_bytes, box_rows))
     return cudaErrorInvalidValue;
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_units = static_cast<int>((most_rows + 2 * kTile - 1) / (2 * kTile));
-  const int64_t blocks = static_cast<int64_t>(a.B) * a.H_kv * row_units;
-  if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
+  const int64_t units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
+  // How many blocks share a unit's keys: what takes the fewest rounds of steps, a
+  // block costing about four steps more than its keys, ten where its part is joined.
+  const int64_t sms = device_sm_count();
+  const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
+  int cluster = 1;
+  int64_t best = 0;
+  for (int c = 1; c <= kMaxSplit; c *= 2) {
+    const int64_t cost = ((units * c + sms - 1) / sms) * ((steps + c - 1) / c + (c > 1 ? 10 : 4));
+    if (c == 1 || cost < best) {
+      best = cost;
+      cluster = c;
+    }
+  }
+  if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
   if (cudaError_t e = configure_mma<kE4m3, DP>(); e != cudaSuccess) return e;
-  paged_mma_kernel<kE4m3, DP>
-      <<<static_cast<unsigned>(blocks), C::kThreads, C::kSmem, stream>>>(mk, mv, a, row_units);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, paged_mma_kernel<kE4m3, DP>, mk, mv, a, row_units, cluster);
 }
 
 }  // namespace
