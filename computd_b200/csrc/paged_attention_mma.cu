@@ -44,7 +44,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
-#include <type_traits>
 
 #include "dwa_internal.h"
 #include "paged_attention.cuh"
@@ -85,8 +84,8 @@ constexpr float kPBits = 11.f, kVScale = 64.f;
 template <bool kE4m3, int DP>
 struct MmaCfg {
   static constexpr int kThreads = kE4m3 ? 512 : 384;
-  static constexpr int kSoftmaxRegs = kE4m3 ? 176 : 208;
-  static constexpr int kOtherRegs = kE4m3 ? 80 : 88;
+  static constexpr int kSoftmaxRegs = kE4m3 ? 184 : 208;
+  static constexpr int kOtherRegs = kE4m3 ? 72 : 88;
   static constexpr int kHalves = DP / 64;               // 128-byte wide column blocks
   static constexpr int kBlockBytes = kTile * 128;       // one of them: 16 KB
   static constexpr int kTileBytes = kHalves * kBlockBytes;
@@ -105,7 +104,7 @@ struct MmaCfg {
 template <bool kE4m3>
 struct MmaShared {
   uint64_t full[5], ready[5], empty[5];
-  uint64_t s_ready[2], s_free, p_ready[2][2], p_free[2];
+  uint64_t s_ready[2], s_free, p_ready[2], p_free[2];
   uint32_t tmem;
   int abort;
   int bad_page;
@@ -214,6 +213,45 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Bounded waits of a whole converged warp, for one barrier or two.  All lanes ask the
+// same and go by votes, so that they cannot part: the warp that issues the products
+// keeps their descriptors in registers that all its lanes share.  Mostly the phase is
+// over already, and a test is cheaper than a wait with a time limit.
+__device__ __forceinline__ bool warp_wait2(uint32_t x, uint32_t parity_x, uint32_t y,
+                                           uint32_t parity_y, int* status, volatile int* abort_flag) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  if (__all_sync(kAll, mbar_test(x, parity_x) & mbar_test(y, parity_y))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    const bool x_done = __all_sync(kAll, mbar_try_wait(x, parity_x));
+    const bool y_done = __all_sync(kAll, mbar_try_wait(y, parity_y));
+    if (x_done && y_done) return true;
+    if (__any_sync(kAll, *abort_flag != 0)) return false;
+    if (__any_sync(kAll, globaltimer_ns() - t0 > kWaitLimitNs)) {
+      if (status) atomicCAS(status, 0, kStatusTimeout);
+      *abort_flag = 1;
+      __syncwarp();
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool warp_wait1(uint32_t x, uint32_t parity, int* status,
+                                           volatile int* abort_flag) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  if (__all_sync(kAll, mbar_test(x, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (__all_sync(kAll, mbar_try_wait(x, parity))) return true;
+    if (__any_sync(kAll, *abort_flag != 0)) return false;
+    if (__any_sync(kAll, globaltimer_ns() - t0 > kWaitLimitNs)) {
+      if (status) atomicCAS(status, 0, kStatusTimeout);
+      *abort_flag = 1;
+      __syncwarp();
+      return false;
+    }
+  }
+}
+
 // The start-address field; in a cluster an address has the block's rank above it.
 __device__ __forceinline__ uint32_t desc_addr(uint32_t addr) { return (addr >> 4) & 0x3FFFu; }
 __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
@@ -261,34 +299,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// 2^x for a pair without the special-function unit: x = n + f, |f| <= 1/2, by
-// adding 1.5 2^23 (+ 127, so that the sum's low bits shifted up are 2^n); 2^f by the
-// cubic with the least relative error on that interval (7.5e-5, found by iteratively
-// reweighted least squares; bf16 probabilities are rounded to 2^-9).  x is held at
-// -126, where P is nothing; NaN stays NaN.
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
-  float a, b;
-  unpair(x, a, b);
-  x = pair(max_nan(a, -126.f), max_nan(b, -126.f));
-  const uint64_t magic = pair(12582912.f + 127.f, 12582912.f + 127.f);
-  const uint64_t back = pair(-12582912.f - 127.f, -12582912.f - 127.f);
-  const uint64_t t = add2(x, magic);
-  const uint64_t f = fma2(add2(t, back), pair(-1.f, -1.f), x);
-  uint64_t y = fma2(f, pair(0.05517166852951050f, 0.05517166852951050f),
-                    pair(0.2426111251115799f, 0.2426111251115799f));
-  y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
-  y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
-  unpair(t, a, b);
-  return mul2(y, pair(__uint_as_float(__float_as_uint(a) << 23),
-                      __uint_as_float(__float_as_uint(b) << 23)));
-}
-
 template <int kRegs>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -362,8 +372,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     mbar_init(bar(sh.s_free), 4);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(sh.s_ready[i]), 1);
-      mbar_init(bar(sh.p_ready[i][0]), 4);
-      mbar_init(bar(sh.p_ready[i][1]), 4);
+      mbar_init(bar(sh.p_ready[i]), 4);
       mbar_init(bar(sh.p_free[i]), 1);
     }
     sh.abort = 0;
@@ -418,10 +427,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int n_items = 2 * n_steps;
   // a bounded wait of the whole warp, which goes on or gives up together
   auto warp_wait = [&](const uint64_t& x, int phase) -> bool {
-    const uint32_t at = bar(x), parity = phase & 1;
-    // mostly it is over already: a test costs less than a wait with a time limit
-    if (__all_sync(0xFFFFFFFFu, mbar_test(at, parity))) return true;
-    return static_cast<bool>(__all_sync(0xFFFFFFFFu, mbar_wait(at, parity, status, abort_flag)));
+    return warp_wait1(bar(x), phase & 1, status, abort_flag);
   };
   // one arrival per warp, after every lane's accesses
   auto warp_arrive = [&](const uint64_t& x) {
@@ -481,28 +487,33 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const int k_steps = a.d / 16;
       const uint32_t one = elect_one();
       int used = 0;  // products that went through S
-      auto wait = [&](const uint64_t& x, uint32_t parity) {
-        const bool ok = warp_wait(x, parity);
+      auto wait2 = [&](uint32_t x, int phase_x, uint32_t y, int phase_y) -> bool {
+        const bool ok = warp_wait2(x, phase_x & 1, y, phase_y & 1, status, abort_flag);
         tc_fence_after();
         return ok;
       };
-      auto item_ready = [&](int it) {  // an operand tile is in shared memory
-        const int st = it % C::kStages;
-        // bf16 keys come straight from the TMA, everything else through other warps
-        return wait(!kE4m3 && !(it & 1) ? sh.full[st] : sh.ready[st], (it / C::kStages) & 1);
+      // an operand tile is in shared memory: bf16 keys come straight from the TMA,
+      // everything else through other warps
+      const uint32_t full0 = bar(sh.full[0]), ready0 = bar(sh.ready[0]);
+      auto item = [&](int it) -> uint32_t {
+        return (!kE4m3 && !(it & 1) ? full0 : ready0) + 8 * (it % C::kStages);
       };
       // Only a descriptor's start address changes: its low word by constants, so that the
-      // one issuing thread spends a few instructions per product (a loop that built
+      // one issuing lane spends a few instructions per product (a loop that built
       // descriptors took 150 cycles for each product of 64).
       const uint32_t k_hi = static_cast<uint32_t>(sw128_kmajor_desc(0) >> 32);
       const uint32_t k_lo = static_cast<uint32_t>(sw128_kmajor_desc(0));
       const uint32_t v_hi = static_cast<uint32_t>(value_desc(0, C::kBlockBytes) >> 32);
       const uint32_t v_lo = static_cast<uint32_t>(value_desc(0, C::kBlockBytes));
-      auto scores = [&](int i, int j) {
-        if (used > 0 && !wait(sh.s_free, (used - 1) & 1)) return false;
+      auto scores = [&](int i, int j) {  // S = Q_i K_j^T, when the last S is read and K_j there
+        const int it = 2 * j, st = it % C::kStages;
+        // before the first there is no S to wait for
+        if (!wait2(item(it), it / C::kStages, used > 0 ? bar(sh.s_free) : item(it),
+                   used > 0 ? used - 1 : it / C::kStages))
+          return false;
         ++used;
         const uint32_t q = k_lo + desc_addr(base + i * C::kTileBytes);
-        const uint32_t k = k_lo + desc_addr(s_stage + ((2 * j) % C::kStages) * C::kStageBytes);
+        const uint32_t k = k_lo + desc_addr(s_stage + st * C::kStageBytes);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
           const uint32_t off = ((s >> 2) * C::kBlockBytes + (s & 3) * 32) >> 4;
@@ -512,27 +523,25 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         commit(bar(sh.s_ready[i]), one);
         return true;
       };
-      auto values = [&](int i, int j) {
-        const uint32_t v = v_lo + desc_addr(s_stage + ((2 * j + 1) % C::kStages) * C::kStageBytes);
+      auto values = [&](int i, int j) {  // O_i += P_i V_j
+        const int it = 2 * j + 1, st = it % C::kStages;
+        if (!wait2(item(it), it / C::kStages, bar(sh.p_ready[i]), j)) return false;
+        const uint32_t v = v_lo + desc_addr(s_stage + st * C::kStageBytes);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!wait(sh.p_ready[i][h], j & 1)) return false;
-#pragma unroll
-          for (int s = 4 * h; s < 4 * h + 4; ++s)
-            mma_ts(tm_o + 128 * i, tm_p + 64 * i + 8 * s, desc64(v + s * 128, v_hi), idesc_o,
-                   j > 0 || s > 0, one);
-        }
+        for (int s = 0; s < kTile / 16; ++s)
+          mma_ts(tm_o + 128 * i, tm_p + 64 * i + 8 * s, desc64(v + s * 128, v_hi), idesc_o,
+                 j > 0 || s > 0, one);
         commit(bar(sh.p_free[i]), one);
         return true;
       };
-      bool ok = n_steps > 0 && item_ready(0);
-      if (ok && steps0 > 0) ok = scores(0, 0);
-      if (ok && steps1 > 0) ok = scores(1, 0);
-      if (ok) commit(bar(sh.empty[0]), one);
+      bool ok = true;
+      if (n_steps > 0) {
+        if (steps0 > 0) ok = scores(0, 0);
+        if (ok && steps1 > 0) ok = scores(1, 0);
+        if (ok) commit(bar(sh.empty[0]), one);
+      }
       for (int j = 0; j < n_steps && ok; ++j) {
-        if (j + 1 < n_steps) ok = item_ready(2 * j + 2);
-        if (ok && j + 1 < steps0) ok = scores(0, j + 1);
-        if (ok) ok = item_ready(2 * j + 1);
+        if (j + 1 < steps0) ok = scores(0, j + 1);
         if (ok && j < steps0) ok = values(0, j);
         if (ok && j + 1 < steps1) ok = scores(1, j + 1);
         if (ok && j + 1 < n_steps) commit(bar(sh.empty[(2 * j + 2) % C::kStages]), one);
@@ -719,8 +728,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         tc_fence_before();
         warp_arrive(sh.s_free);
         if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
-        warp_arrive(sh.p_ready[i][0]);
-        warp_arrive(sh.p_ready[i][1]);
+        warp_arrive(sh.p_ready[i]);
         continue;
       }
       uint32_t s[4][32];
@@ -770,8 +778,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       }
       const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
       const float v_now = kE4m3 ? sh.v_ref[j & 3] : 0.f;
-      if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
-      tc_fence_after();
       const bool move = most > m + kSlack || (m == -INFINITY && most > m) || v_now != v_ref;
       if (__any_sync(0xFFFFFFFFu, move)) {
         const float m_new = fmaxf(m, most);
@@ -784,6 +790,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         m = m_new;
         l *= shrink;
         if (j > 0) {
+          if (!warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, shrink_o);
         }
@@ -792,7 +800,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const float ref = (m == -INFINITY ? 0.f : -m) + (kE4m3 ? kPBits : 0.f);
       const uint64_t factor2 = pair(factor, factor), ref2 = pair(ref, ref);
       uint64_t l2[2] = {0, 0};
-      auto half = [&](int h, auto masked) {
+      auto half = [&](int h) {
         uint32_t p[32];
 #pragma unroll
         for (int k = 0; k < 64; k += 2) {
@@ -800,29 +808,24 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           const uint64_t x = fma2(pair(__uint_as_float(s[c][k & 31]), __uint_as_float(s[c][(k & 31) + 1])),
                                   factor2, ref2);
           float p0, p1;
-          uint64_t y;
-          if (!masked && (k >> 1) % 4 == 3) {
-            y = exp2_poly2(x);
-          } else {
-            unpair(x, p0, p1);
-            y = pair(fast_exp2(p0), fast_exp2(p1));
-          }
+          unpair(x, p0, p1);
+          const uint64_t y = pair(fast_exp2(p0), fast_exp2(p1));
           l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], y);
           unpair(y, p0, p1);
           p[k >> 1] = kE4m3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
         }
+        if (h == 0 && j > 0) {  // the product that read the last P
+          alive = warp_wait(sh.p_free[i], j - 1);
+          tc_fence_after();
+        }
         tmem_st_x32(tp + 32 * h, p);
-        tmem_wait_st();
-        tc_fence_before();
-        warp_arrive(sh.p_ready[i][h]);
       };
-      if (edge) {
-        half(0, std::true_type{});
-        half(1, std::true_type{});
-      } else {
-        half(0, std::false_type{});
-        half(1, std::false_type{});
-      }
+      half(0);
+      half(1);
+      if (!alive) break;
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(sh.p_ready[i]);
       float l0, l1;
       unpair(add2(l2[0], l2[1]), l0, l1);
       l += l0 + l1;
