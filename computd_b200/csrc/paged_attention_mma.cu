@@ -29,9 +29,11 @@
 // Warp 9: TMA, straight from the pages into the swizzled operand tiles.  bf16
 // caches: warps 10-11 look over the values of tiles that end behind what every row
 // sees, since 0 * NaN would reach rows that must not see it.  e4m3 caches: warps
-// 12-15 turn codes into fp16 operand tiles (exact for keys, whose scales multiply the
-// scores; values times their scale relative to a running power of two, rounded to
-// 2^-11), and Q is scaled per row by a power of two into fp16.
+// 12-15 turn codes into fp16 operand tiles (code times scale, over a power of two above
+// the tile's scales, rounded to 2^-11), and Q is scaled per row by a power of two into
+// fp16, exactly.  (With the keys' scales multiplied into the scores instead, every
+// row's thread read 128 of them per step: 1499 us instead of XXX for 4736 rows over
+// 16384 keys, 32 heads.)
 //
 // Where there are few units of 256 rows, a cluster of blocks shares the keys of one
 // and joins its parts through distributed shared memory, in a fixed order.
@@ -77,9 +79,9 @@ constexpr int kTile = 128;     // rows per tile, keys per step
 constexpr int kMaxChannels = 128;
 constexpr int kMaxSplit = 8;
 constexpr float kSlack = 4.f;  // log2 of how far P may grow before m follows
-// e4m3 caches: P in fp16 times 2^11 (with kSlack still below 65504), values times 64
-// over the power of two above their scales (448 * 64 is below it too).
-constexpr float kPBits = 11.f, kVScale = 64.f;
+// e4m3 caches: P in fp16 times 2^11 (with kSlack still below 65504), keys and values
+// times 64 over a power of two above their scales (448 * 64 is below it too).
+constexpr float kPBits = 11.f, kCodeScale = 64.f;
 
 template <bool kE4m3, int DP>
 struct MmaCfg {
@@ -89,7 +91,7 @@ struct MmaCfg {
   static constexpr int kHalves = DP / 64;               // 128-byte wide column blocks
   static constexpr int kBlockBytes = kTile * 128;       // one of them: 16 KB
   static constexpr int kTileBytes = kHalves * kBlockBytes;
-  static constexpr int kStages = kE4m3 ? 4 : 5;         // operand tiles (K and V in turn)
+  static constexpr int kStages = 5;                     // operand tiles (K and V in turn)
   // Codes arrive in the stage that their fp16 values will take: at 128 channels in the
   // second column block, where row r's codes lie in row r's place; at 64 behind it.
   static constexpr int kRawAt = DP == 128 ? kBlockBytes : kTileBytes;
@@ -110,10 +112,12 @@ struct MmaShared {
   int bad_page;
   int any_bad;
   int first_bad[kMaxChannels];  // least key with a value that is not finite (e4m3: [0], whole vectors)
-  // e4m3 only: a row's factor of the scores; the keys' scales and v_ref of four steps
+  // e4m3 only: a row's factor of the scores; the converting warps' largest scales of
+  // four tiles; the powers of two that keys and values of four steps are divided by
   float q_factor[kE4m3 ? 2 * kTile : 1];
-  __align__(16) float k_scale[kE4m3 ? 4 : 1][kE4m3 ? kTile : 4];
-  float v_ref[4];
+  uint64_t tops_ready;
+  uint32_t tops[4][4];
+  float k_ref[4], v_ref[4];
 };
 
 // ---------------------------------------------------------------- tcgen05 pieces
@@ -284,11 +288,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -370,6 +369,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       mbar_init(bar(sh.empty[i]), 1);
     }
     mbar_init(bar(sh.s_free), 4);
+    mbar_init(bar(sh.tops_ready), 4);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(sh.s_ready[i]), 1);
       mbar_init(bar(sh.p_ready[i]), 4);
@@ -603,64 +603,62 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const int row0 = 32 * w + row8;
       constexpr int kPer = DP / 64;                 // 16-byte pieces of codes per row and lane
       constexpr int kSwizzle = DP == 128 ? 7 : 0;   // of the codes' 128-byte rows
-      float v_ref = 0.f;
-      // the scales of keys lane + 32 k of a tile, looked up one item ahead, their pages
-      // two: every warp needs their maximum
-      float scale[4];
-      int page[4];
-      auto pages_of = [&](int it) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = (first_tile + (it >> 1)) * kTile + lane + 32 * k;
-          page[k] = it < n_items && key < vis_max ? __ldg(table + (key >> a.page_log2)) : -1;
-        }
+      // Thread t has key t of a tile: its scale is looked up two items ahead, its page
+      // three, and the warp's largest scale is published one ahead.
+      const int64_t head = static_cast<int64_t>(hk) << a.page_log2;
+      const int page_mask = (1 << a.page_log2) - 1;
+      auto page_of = [&](int it) -> int {
+        const int key = (first_tile + (it >> 1)) * kTile + t;
+        return it < n_items && key < vis_max ? __ldg(table + (key >> a.page_log2)) : -1;
       };
-      auto scales_of = [&](int it) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = (first_tile + (it >> 1)) * kTile + lane + 32 * k;
-          scale[k] = 0.f;
-          if (page[k] >= 0 && page[k] < a.n_pages)
-            scale[k] = __ldg(((it & 1) ? a.v_scale : a.k_scale) + page[k] * a.ld_scale_page +
-                             (static_cast<int64_t>(hk) << a.page_log2) +
-                             (key & ((1 << a.page_log2) - 1)));
-        }
+      auto scale_of = [&](int it, int page) -> float {
+        if (page < 0 || page >= a.n_pages) return 0.f;
+        return __ldg(((it & 1) ? a.v_scale : a.k_scale) + page * a.ld_scale_page + head +
+                     (t & page_mask));
       };
-      pages_of(0);
-      scales_of(0);
-      pages_of(1);
+      auto publish = [&](int it, float x) {  // numbers order like their bits; others count as 0
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, fabsf(x) < INFINITY ? __float_as_uint(fabsf(x)) : 0u);
+        if (lane == 0) sh.tops[it & 3][w] = top;
+        warp_arrive(sh.tops_ready);
+      };
+      float now = scale_of(0, page_of(0)), next = scale_of(1, page_of(1)), v_ref = 0.f;
+      int page = page_of(2);
+      publish(0, now);
       for (int it = 0; it < n_items; ++it) {
         const int st = it % C::kStages, j = it >> 1, key0 = (first_tile + j) * kTile;
-        float own = 0.f, top = 0.f;  // this warp's; the largest number among all
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k == w) own = scale[k];
-          top = fmaxf(top, scale[k]);
-        }
-        scales_of(it + 1);
-        pages_of(it + 2);
+        const float after = scale_of(it + 2, page);
+        page = page_of(it + 3);
+        if (!warp_wait(sh.tops_ready, it)) break;
+        publish(it + 1, next);  // after the wait: no warp can be two phases ahead of another
+        const uint32_t* tops = sh.tops[it & 3];
+        float ref = power_above(__uint_as_float(max(max(tops[0], tops[1]), max(tops[2], tops[3]))));
         if (!warp_wait(sh.full[st], it / C::kStages)) break;
-        // What this step's slots held was last read in step j - 4, which is over
-        // since this stage, then step j - 2's, was free for the copy.
-        uint32_t mul = 0;  // of this lane's rows' values: fp16 pair per row, by shuffle
+        // What this step's slots held was last read in step j - 4, which is over since
+        // this stage, whose tile was of step j - 2 or j - 3, was free for the copy.
         if (it & 1) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-          if (v_ref == 0.f || top > v_ref) v_ref = power_above(top);
-          if (t == 0) sh.v_ref[j & 3] = v_ref;
+          // values of all steps add up in O: their power of two only grows
+          v_ref = ref = fmaxf(ref, v_ref);
+          if (t == 0) sh.v_ref[j & 3] = ref;
           // a vector that is NaN and that some row must not see becomes zeros, and is noted
-          if (!(own < INFINITY) && key0 + t >= vis_min) {
+          if (!(fabsf(now) < INFINITY) && key0 + t >= vis_min) {
             if (key0 + t < vis_max) {
               atomicMin(&sh.first_bad[0], key0 + t);
               sh.any_bad = 1;
             }
-            own = 0.f;
+            now = 0.f;
           }
-          const float f = own * (kVScale / v_ref);
-          mul = pack_f16(f, f);
-        } else {
-          sh.k_scale[j & 3][t] = own;
+        } else if (t == 0) {
+          sh.k_ref[j & 3] = ref;
         }
+        // this key's factor as the sum of two fp16: keys use both, so that a product has
+        // its own rounding only (a score is 128 of them), values the first
+        const float f = now * (kCodeScale / ref);
+        const __half f_hi = __float2half_rn(f);
+        const __half f_lo = __float2half_rn(f - __half2float(f_hi));
+        const uint32_t mul = static_cast<uint32_t>(__half_as_ushort(f_hi)) |
+                             (static_cast<uint32_t>(__half_as_ushort(f_lo)) << 16);
+        now = next;
+        next = after;
         uint8_t* stage = smem + 2 * C::kTileBytes + st * C::kStageBytes;
         uint4 x[4][kPer];
 #pragma unroll
@@ -679,15 +677,21 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         __syncwarp();  // the rows' codes are read: their place may be written
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t f = __shfl_sync(0xFFFFFFFFu, mul, row8 + 8 * k);
+          const uint32_t both = __shfl_sync(0xFFFFFFFFu, mul, row8 + 8 * k);
+          const uint32_t hi = __byte_perm(both, 0, 0x1010), lo = __byte_perm(both, 0, 0x3232);
 #pragma unroll
           for (int p = 0; p < kPer; ++p) {
             const uint32_t u[4] = {x[k][p].x, x[k][p].y, x[k][p].z, x[k][p].w};
             uint32_t o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              o[e] = e4m3x2_f16x2(u[e >> 1], e & 1);
-              if (it & 1) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(o[e]), "r"(f));
+              const uint32_t code = e4m3x2_f16x2(u[e >> 1], e & 1);
+              if (it & 1) {
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(code), "r"(hi));
+              } else {
+                asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[e]) : "r"(code), "r"(lo));
+                asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(o[e]) : "r"(code), "r"(hi));
+              }
             }
             uint8_t* row = stage + p * C::kBlockBytes + (row0 + 8 * k) * 128;
             *reinterpret_cast<uint4*>(row + (((2 * c) ^ row8) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -718,7 +722,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     const int vis = live ? paged_visible(seq, static_cast<int>(row / a.group)) : 0;
     // least visible count in the warp: steps below it need no mask
     const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
-    const float factor = kE4m3 ? sh.q_factor[i * kTile + r] : a.scale_log2;
+    // the scores' factor, to log2 units
+    const float row_factor = kE4m3 ? sh.q_factor[i * kTile + r] / kCodeScale : a.scale_log2;
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
     bool alive = true;
     for (int j = 0; j < steps; ++j) {
@@ -740,26 +745,15 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       warp_arrive(sh.s_free);
       const int key0 = (first_tile + j) * kTile;
       const bool edge = key0 + kTile > vis_low;
-      const float* ks = sh.k_scale[kE4m3 ? j & 3 : 0];
+      float v_now = 0.f, factor = row_factor;
       if constexpr (kE4m3) {
-        // the step's scales: the values' tile is converted right after the keys'
+        // the step's powers of two: the values' tile is converted right after the keys'
         if (!warp_wait(sh.ready[(2 * j + 1) % C::kStages], (2 * j + 1) / C::kStages)) {
           alive = false;
           break;
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(ks + 32 * c + k);
-            float y[4];
-            unpair(mul2(pair(__uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1])), pair(x.x, x.y)),
-                   y[0], y[1]);
-            unpair(mul2(pair(__uint_as_float(s[c][k + 2]), __uint_as_float(s[c][k + 3])),
-                        pair(x.z, x.w)), y[2], y[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[c][k + e] = __float_as_uint(y[e]);
-          }
+        v_now = sh.v_ref[j & 3];
+        factor = fmaxf(row_factor * sh.k_ref[j & 3], 0x1p-126f);
       }
       if (edge) {
 #pragma unroll
@@ -777,7 +771,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
       }
       const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
-      const float v_now = kE4m3 ? sh.v_ref[j & 3] : 0.f;
       const bool move = most > m + kSlack || (m == -INFINITY && most > m) || v_now != v_ref;
       if (__any_sync(0xFFFFFFFFu, move)) {
         const float m_new = fmaxf(m, most);
@@ -837,7 +830,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     if (!alive || sh.bad_page) l = __uint_as_float(0x7FC00000u);
     if (sh.bad_page && threadIdx.x == 0) paged_report(a.status);
     // O is in units of P's power of two, which l has too, and of the values'
-    const float v_back = kE4m3 ? v_ref / kVScale : 1.f;
+    const float v_back = kE4m3 ? v_ref / kCodeScale : 1.f;
     if (cluster == 1) {
       const float inv = (l == 0.f ? 0.f : 1.f / l) * v_back;
       const bool some_bad = sh.any_bad;
