@@ -19,6 +19,7 @@ namespace dwa {
 namespace {
 
 constexpr int kWriteThreads = 256;
+constexpr int kWriteBlocks = 4;    // per SM
 constexpr int kGroupTokens = 64;   // tokens of a block checked for repeated slots at a time
 constexpr int kFilterBits = 1024;  // their slots' low bits
 
@@ -26,22 +27,38 @@ __device__ __forceinline__ void report(int32_t* status) {
   if (status != nullptr) atomicCAS(status, 0, DWA_ERR_DEVICE_CHECK);
 }
 
-// Eight consecutive values of a source row as f32.
+// Eight consecutive values of a source row: 16 bytes of bf16, or 32 of f32.
 template <bool kBf16>
-__device__ __forceinline__ void load8(const void* row, int64_t at, float (&x)[8]) {
-  if (kBf16) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + at));
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Raw8 {
+  uint4 w[kBf16 ? 1 : 2];
+};
+template <bool kBf16>
+__device__ __forceinline__ Raw8<kBf16> load8(const void* row, int64_t at) {
+  Raw8<kBf16> r;
+  if constexpr (kBf16) {
+    r.w[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + at));
+  } else {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(row) + at);
+    r.w[0] = __ldg(p);
+    r.w[1] = __ldg(p + 1);
+  }
+  return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ void as_f32(const Raw8<kBf16>& r, float (&x)[8]) {
+  if constexpr (kBf16) {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       x[2 * i] = __uint_as_float(u[i] << 16);
       x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
     }
   } else {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[4 * i] = __uint_as_float(r.w[i].x); x[4 * i + 1] = __uint_as_float(r.w[i].y);
+      x[4 * i + 2] = __uint_as_float(r.w[i].z); x[4 * i + 3] = __uint_as_float(r.w[i].w);
+    }
   }
 }
 
@@ -50,8 +67,8 @@ __device__ __forceinline__ void load8(const void* row, int64_t at, float (&x)[8]
 // holds values, `keep` whether they are stored.
 template <bool kE4m3>
 __device__ __forceinline__ void store8(const float (&x)[8], bool on, bool keep, int lanes, int lane,
-                                       void* cache, float* scales, int64_t row, int d) {
-  if (!kE4m3) {
+                                       void* cache, float* scales, int64_t row, int64_t srow, int d) {
+  if constexpr (!kE4m3) {
     if (on && keep) {
       uint32_t u[4];
 #pragma unroll
@@ -76,25 +93,35 @@ __device__ __forceinline__ void store8(const float (&x)[8], bool on, bool keep, 
                              : __uint_as_float(0x7FC00000u);
   if (!keep) return;
   if (on) {
+    // x / scale, |x / scale| <= 448 (1 + 2^-23), which rounds to 448 at most.  One
+    // reciprocal for all: with y = 1 / scale rounded, q = x y, the remainder
+    // x - q scale is exact in an fma and q + remainder y is the rounded quotient
+    // (Markstein, 1990), as long as nothing underflows: scale above 2^-80 and
+    // quotients above 2^-11 leave the remainder above 2^-138 (smaller quotients
+    // give the code 0 either way).
+    float q[8];
+    if (scale > 0x1p-80f) {
+      const float y = __frcp_rn(scale);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q0 = x[i] * y;
+        q[i] = fmaf(fmaf(-q0, scale, x[i]), y, q0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = finite ? __fdiv_rn(x[i], scale) : 0.f;
+    }
     uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t lo = 0, hi = 0;
-      if (finite) {
-        // |x / scale| <= 448 (1 + 2^-23), which rounds to 448 at most
-        lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i], scale),
-                                                  __fdiv_rn(x[4 * i + 1], scale)),
-                                      __NV_SATFINITE, __NV_E4M3);
-        hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[4 * i + 2], scale),
-                                                  __fdiv_rn(x[4 * i + 3], scale)),
-                                      __NV_SATFINITE, __NV_E4M3);
-      }
-      w[i] = lo | (hi << 16);
-    }
+    for (int i = 0; i < 2; ++i)
+      w[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]),
+                                                            __NV_SATFINITE, __NV_E4M3)) |
+             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(
+                 make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3)) << 16;
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row * d + 8 * lane) =
         make_uint2(w[0], w[1]);
   }
-  if (lane == 0) scales[row] = scale;
+  if (lane == 0) scales[srow] = scale;
 }
 
 struct WriteArgs {
@@ -121,7 +148,7 @@ struct WriteArgs {
 // list is read once per block (from L2: 19 MB in all for 8192 tokens, against
 // the 200 MB of keys and values at 32 heads of 128).
 template <bool kE4m3, bool kSrcBf16>
-__global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(const WriteArgs a) {
   __shared__ int64_t own[kGroupTokens];
   __shared__ int dropped[kGroupTokens];
   __shared__ uint32_t filter[kFilterBits / 32];
@@ -134,6 +161,18 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WriteArgs
   const int64_t t_end = min((blockIdx.x + 1) * a.tokens_per_block, a.T);
   for (int64_t t0 = blockIdx.x * a.tokens_per_block; t0 < t_end; t0 += kGroupTokens) {
     const int n = static_cast<int>(min(t_end - t0, static_cast<int64_t>(kGroupTokens)));
+    const int vectors = n * a.H;
+    // a round's values are under way while the round before is stored, the first ones
+    // while the slots are checked
+    auto load = [&](int vec, Raw8<kSrcBf16>* k, Raw8<kSrcBf16>* v) {
+      if (vec < vectors && on) {
+        const int i = vec / a.H, h = vec - i * a.H;
+        *k = load8<kSrcBf16>(a.k, (t0 + i) * a.k_tok + h * a.k_head + 8 * lane);
+        *v = load8<kSrcBf16>(a.v, (t0 + i) * a.v_tok + h * a.v_head + 8 * lane);
+      }
+    };
+    Raw8<kSrcBf16> k_now{}, v_now{};
+    load(group, &k_now, &v_now);
     __syncthreads();
     for (int i = threadIdx.x; i < kFilterBits / 32; i += kWriteThreads) filter[i] = 0;
     __syncthreads();
@@ -146,37 +185,41 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(const WriteArgs
       if (fine) atomicOr(&filter[(s & (kFilterBits - 1)) >> 5], 1u << (s & 31));
     }
     __syncthreads();
-    for (int64_t t = t0 + 1 + threadIdx.x; t < a.T; t += kWriteThreads) {
-      const int64_t s = a.slots[t];
-      if ((filter[(s & (kFilterBits - 1)) >> 5] >> (s & 31)) & 1u) {
-        const int before = static_cast<int>(min(t - t0, static_cast<int64_t>(n)));
-        for (int i = 0; i < before; ++i)
-          if (own[i] == s) dropped[i] = 1;
+    constexpr int kBatch = 8;  // slots that a thread looks at together
+    for (int64_t t = t0 + 1 + threadIdx.x; t < a.T; t += kBatch * kWriteThreads) {
+      int64_t s[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        s[j] = t + j * kWriteThreads < a.T ? __ldg(a.slots + t + j * kWriteThreads) : -1;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (s[j] >= 0 && ((filter[(s[j] & (kFilterBits - 1)) >> 5] >> (s[j] & 31)) & 1u)) {
+          const int before = static_cast<int>(min(t + j * kWriteThreads - t0, static_cast<int64_t>(n)));
+          for (int i = 0; i < before; ++i)
+            if (own[i] == s[j]) dropped[i] = 1;
+        }
       }
     }
     __syncthreads();
-    const int vectors = n * a.H;
     for (int base = 0; base < vectors; base += groups) {
       const int vec = base + group;
+      Raw8<kSrcBf16> k_next{}, v_next{};
+      load(vec + groups, &k_next, &v_next);
       const bool here = vec < vectors;
-      const int i = here ? vec / a.H : 0, h = here ? vec % a.H : 0;
-      const int64_t t = t0 + i;
-      float xk[8] = {}, xv[8] = {};
-      if (here && on) {
-        load8<kSrcBf16>(a.k, t * a.k_tok + h * a.k_head + 8 * lane, xk);
-        load8<kSrcBf16>(a.v, t * a.v_tok + h * a.v_head + 8 * lane, xv);
-      }
+      const int i = here ? vec / a.H : 0, h = here ? vec - i * a.H : 0;
       const bool keep = here && !dropped[i];
       const int64_t s = keep ? own[i] : 0;
       const int64_t page = s >> a.page_log2, off = s & ((1 << a.page_log2) - 1);
       const int64_t in_page = (static_cast<int64_t>(h) << a.page_log2) + off;
       const int64_t row = page * a.ld_page + in_page;
       const int64_t srow = page * a.ld_scale_page + in_page;
-      // scales are addressed by their own stride: shift the base so that `row` serves both
-      store8<kE4m3>(xk, on, keep, lanes, lane, a.k_cache,
-                    kE4m3 ? a.k_scale + (srow - row) : nullptr, row, a.d);
-      store8<kE4m3>(xv, on, keep, lanes, lane, a.v_cache,
-                    kE4m3 ? a.v_scale + (srow - row) : nullptr, row, a.d);
+      float x[8];
+      as_f32(k_now, x);
+      store8<kE4m3>(x, here && on, keep, lanes, lane, a.k_cache, a.k_scale, row, srow, a.d);
+      as_f32(v_now, x);
+      store8<kE4m3>(x, here && on, keep, lanes, lane, a.v_cache, a.v_scale, row, srow, a.d);
+      k_now = k_next;
+      v_now = v_next;
     }
   }
 }
@@ -276,7 +319,7 @@ cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, 
   a.ld_page = c.ld_page / c.d; a.ld_scale_page = c.ld_scale_page;
   a.lanes_log2 = log2_at_least(c.d / 8);
   a.status = status;
-  const int64_t most = 8ll * device_sm_count();  // one wave of resident blocks
+  const int64_t most = static_cast<int64_t>(kWriteBlocks) * device_sm_count();
   a.tokens_per_block = (T + most - 1) / most;
   const unsigned grid = static_cast<unsigned>((T + a.tokens_per_block - 1) / a.tokens_per_block);
   if (c.k_scale != nullptr) {

@@ -72,6 +72,11 @@ __device__ __forceinline__ int paged_visible(const PagedSeq& s, int i) {
   return max(s.length - s.n + i + 1, 0);
 }
 
+// The new token of a row (rows are token-major, `group` query heads to a token).
+__device__ __forceinline__ uint32_t row_token(uint32_t row, int group) {
+  return group == 1 ? row : row / static_cast<uint32_t>(group);
+}
+
 // ---------------------------------------------------------------- arithmetic
 // ex2.approx: 2 ulp of f32, far below the probabilities' own rounding.
 __device__ __forceinline__ float fast_exp2(float x) {

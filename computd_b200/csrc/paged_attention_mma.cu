@@ -106,7 +106,7 @@ struct MmaCfg {
 template <bool kE4m3>
 struct MmaShared {
   uint64_t full[5], ready[5], empty[5];
-  uint64_t s_ready[2], s_free, p_ready[2], p_free[2];
+  uint64_t q_ready, s_ready[2], s_free, p_ready[2], p_free[2];
   uint32_t tmem;
   int abort;
   int bad_page;
@@ -321,13 +321,12 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ------------------------------------------------ the block's work
+  const uint32_t heads = static_cast<uint32_t>(a.B) * a.H_kv;  // the grid has 32 bits
   const int split = static_cast<int>(blockIdx.x % cluster);
-  int64_t unit = blockIdx.x / cluster;
+  const uint32_t unit = blockIdx.x / cluster;
   // late rows (more keys) first
-  const int ru = row_units - 1 - static_cast<int>(unit / (static_cast<int64_t>(a.B) * a.H_kv));
-  unit %= static_cast<int64_t>(a.B) * a.H_kv;
-  const int hk = static_cast<int>(unit % a.H_kv);
-  const int b = static_cast<int>(unit / a.H_kv);
+  const int ru = row_units - 1 - static_cast<int>(unit / heads);
+  const int b = static_cast<int>(unit % heads / a.H_kv), hk = static_cast<int>(unit % heads % a.H_kv);
   const PagedSeq seq = paged_seq(a, b);
   if (seq.bad && hk == 0 && ru == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
   const int64_t all_rows = static_cast<int64_t>(seq.n) * a.group;
@@ -370,6 +369,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     }
     mbar_init(bar(sh.s_free), 4);
     mbar_init(bar(sh.tops_ready), 4);
+    mbar_init(bar(sh.q_ready), 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(sh.s_ready[i]), 1);
       mbar_init(bar(sh.p_ready[i]), 4);
@@ -385,39 +385,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
   }
-  // Q into the swizzled operand tiles: 16 bytes (8 channels) per thread
-  {
-    constexpr int kChunks = DP / 8;  // per row; a row's threads are neighbours in a warp
-    for (int i = threadIdx.x; i < 2 * kTile * kChunks; i += C::kThreads) {
-      const int r = i / kChunks, c = i % kChunks;
-      const int64_t row = r0 + r;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row < all_rows && 8 * c < a.d)
-        x = __ldg(reinterpret_cast<const uint4*>(
-            a.q + (seq.row0 + row / a.group) * a.q_ld +
-            (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + 8 * c));
-      if constexpr (kE4m3) {
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7FFF0000u, w[k] & 0x7FFF0000u));
-#pragma unroll
-        for (int o = kChunks / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float f0, f1;
-        const float factor = f16_row_scale(top, a.scale_log2, &f0, &f1);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = pack_f16(__uint_as_float(w[k] << 16) * f0 * f1,
-                          __uint_as_float(w[k] & 0xFFFF0000u) * f0 * f1);
-        x = make_uint4(w[0], w[1], w[2], w[3]);
-        if (c == 0) sh.q_factor[r] = factor;
-      }
-      const int tile = r / kTile, tr = r % kTile;
-      *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (c >> 3) * C::kBlockBytes + tr * 128 +
-                                (((c & 7) ^ (tr & 7)) << 4)) = x;
-    }
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -534,8 +501,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         commit(bar(sh.p_free[i]), one);
         return true;
       };
-      bool ok = true;
-      if (n_steps > 0) {
+      bool ok = warp_wait(sh.q_ready, 0);
+      if (ok && n_steps > 0) {
         if (steps0 > 0) ok = scores(0, 0);
         if (ok && steps1 > 0) ok = scores(1, 0);
         if (ok) commit(bar(sh.empty[0]), one);
@@ -710,16 +677,66 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     }
   } else {
     regs_inc<C::kSoftmaxRegs>();
+    // ------------------------------------------------ Q into the swizzled operand tiles
+    {
+      constexpr int kChunks = DP / 8;  // of 16 bytes per row; a row's lanes are neighbours
+      constexpr int kRowsAtOnce = 256 / kChunks, kRounds = 2 * kTile / kRowsAtOnce;
+      const int c = threadIdx.x % kChunks, first = threadIdx.x / kChunks;
+      const uint16_t* src = a.q + static_cast<int64_t>(hk) * a.group * a.d + 8 * c;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint4 x[kRounds / 2];
+#pragma unroll
+        for (int k = 0; k < kRounds / 2; ++k) {
+          const int r = first + (half * (kRounds / 2) + k) * kRowsAtOnce;
+          const uint32_t row = static_cast<uint32_t>(r0) + r;  // below 2^31: max_q bounds it
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (r < left && 8 * c < a.d) {
+            const uint32_t token = row_token(row, a.group);
+            x[k] = __ldg(reinterpret_cast<const uint4*>(
+                src + (seq.row0 + token) * a.q_ld + (row - token * a.group) * a.d));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kRounds / 2; ++k) {
+          const int r = first + (half * (kRounds / 2) + k) * kRowsAtOnce;
+          if constexpr (kE4m3) {
+            uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              top = max(top, max((w[e] << 16) & 0x7FFF0000u, w[e] & 0x7FFF0000u));
+#pragma unroll
+            for (int o = kChunks / 2; o > 0; o >>= 1)
+              top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            float f0, f1;
+            const float factor = f16_row_scale(top, a.scale_log2, &f0, &f1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_f16(__uint_as_float(w[e] << 16) * f0 * f1,
+                              __uint_as_float(w[e] & 0xFFFF0000u) * f0 * f1);
+            x[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (c == 0) sh.q_factor[r] = factor;
+          }
+          const int tile = r / kTile, tr = r % kTile;
+          *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (c >> 3) * C::kBlockBytes + tr * 128 +
+                                    (((c & 7) ^ (tr & 7)) << 4)) = x[k];
+        }
+      }
+      fence_proxy_async_smem();
+      warp_arrive(sh.q_ready);
+      if constexpr (kE4m3) asm volatile("bar.sync 2, 256;" ::: "memory");  // the rows' factors
+    }
     // ------------------------------------------------ softmax: one row per thread
     const int i = warp >> 2;
     const int r = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tm_s + lanes, tp = tm_p + 64 * i + lanes, to = tm_o + 128 * i + lanes;
     const int rows = i ? rows1 : rows0, steps = i ? steps1 : steps0;
-    const int64_t row = r0 + i * kTile + r;
     const bool live = r < rows;
     const bool warp_live = 32 * (warp & 3) < rows;
-    const int vis = live ? paged_visible(seq, static_cast<int>(row / a.group)) : 0;
+    const uint32_t row0 = static_cast<uint32_t>(r0) + i * kTile;
+    const int vis = live ? paged_visible(seq, row_token(row0 + r, a.group)) : 0;
     // least visible count in the warp: steps below it need no mask
     const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
     // the scores' factor, to log2 units
@@ -832,34 +849,46 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     // O is in units of P's power of two, which l has too, and of the values'
     const float v_back = kE4m3 ? v_ref / kCodeScale : 1.f;
     if (cluster == 1) {
+      // through this warp's rows of Q's tile, which no product needs any more, so that
+      // rows leave whole (a row per thread at 16 bytes a store took 7 us per block)
       const float inv = (l == 0.f ? 0.f : 1.f / l) * v_back;
       const bool some_bad = sh.any_bad;
-      uint16_t* dst = a.out + (seq.row0 + row / a.group) * a.out_ld +
-                      (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d;
+      uint8_t* stage = smem + i * C::kTileBytes + 32 * (warp & 3) * (2 * DP);
+      if (warp_live) {
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        float o[32];
-        if (have && warp_live) {
-          tmem_ld_32x32b_x32_sync(to + 32 * c, o);
-        } else {
+        for (int c = 0; c < DP / 32; ++c) {
+          float o[32];
+          if (have) {
+            tmem_ld_32x32b_x32_sync(to + 32 * c, o);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0.f;
-        }
-        if (live) {
+            for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          }
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
-            if (32 * c + k < a.d) {
-              float x[8];
+            float x[8];
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                x[q] = l == 0.f ? 0.f : o[k + q] * inv;
-                if (some_bad && sh.first_bad[kE4m3 ? 0 : 32 * c + k + q] < vis) x[q] = __uint_as_float(0x7FC00000u);
-              }
-              *reinterpret_cast<uint4*>(dst + 32 * c + k) =
-                  make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
-                             pack_bf16(x[6], x[7]));
+            for (int q = 0; q < 8; ++q) {
+              x[q] = l == 0.f ? 0.f : o[k + q] * inv;
+              if (some_bad && sh.first_bad[kE4m3 ? 0 : 32 * c + k + q] < vis)
+                x[q] = __uint_as_float(0x7FC00000u);
             }
+            *reinterpret_cast<uint4*>(stage + lane * (2 * DP) +
+                                      (((4 * c + k / 8) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
+                           pack_bf16(x[6], x[7]));
           }
+        }
+        __syncwarp();
+        constexpr int kChunks = DP / 8;
+        const int chunk = lane % kChunks;
+        for (int q = lane / kChunks; q < min(rows - 32 * (warp & 3), 32); q += 32 / kChunks) {
+          const uint32_t row = row0 + 32 * (warp & 3) + q, token = row_token(row, a.group);
+          if (8 * chunk < a.d)
+            *reinterpret_cast<uint4*>(a.out + (seq.row0 + token) * a.out_ld +
+                                      (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d +
+                                      8 * chunk) =
+                *reinterpret_cast<const uint4*>(stage + q * (2 * DP) + ((chunk ^ (q & 7)) << 4));
         }
       }
     } else {
@@ -887,48 +916,70 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       part_ml[2 * mine] = m;
       part_ml[2 * mine + 1] = l;
       cluster_sync();
-      // the rows of a unit, dealt to the cluster's warps; a lane has four channels
-      constexpr int kWarps = 8;  // the others gave their registers away
-      for (int rr = split * kWarps + warp; rr < min(left, static_cast<int64_t>(2 * kTile));
-           rr += cluster * kWarps) {
-        float top = -INFINITY, f[kMaxSplit], ls[kMaxSplit];
-        int bad = 0;
-#pragma unroll
-        for (int c = 0; c < kMaxSplit; ++c)
-          if (c < cluster) {
-            f[c] = ld_cluster_f32(part_ml + 2 * rr, c);
-            ls[c] = ld_cluster_f32(part_ml + 2 * rr + 1, c);
-            bad |= ld_cluster_s32(&sh.any_bad, c);
-            top = fmaxf(top, f[c]);
-          }
-        float sum = 0.f, x[4] = {};
-        const int ch = 4 * lane;
-        if (ch < a.d) {
-#pragma unroll
-          for (int c = 0; c < kMaxSplit; ++c)
-            if (c < cluster) {
-              // a part without keys has l = 0 (or NaN, which has to stay)
-              const float w = f[c] == -INFINITY ? 0.f : fast_exp2(f[c] - top);
-              sum += f[c] == -INFINITY ? ls[c] : w * ls[c];
-              const float4 y = ld_cluster_f32x4(part + rr * C::kPartLd + ch, c);
-              x[0] += w * y.x; x[1] += w * y.y; x[2] += w * y.z; x[3] += w * y.w;
-            }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const int64_t row = r0 + rr;
-          const int vis = paged_visible(seq, static_cast<int>(row / a.group));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] *= inv;
-            if (bad) {
-              for (int c = 0; c < cluster; ++c)
-                if (ld_cluster_s32(&sh.first_bad[kE4m3 ? 0 : ch + e], c) < vis) x[e] = __uint_as_float(0x7FC00000u);
-            }
-          }
-          *reinterpret_cast<uint2*>(a.out + (seq.row0 + row / a.group) * a.out_ld +
-                                    (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + ch) =
-              make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+      // The unit's rows, four at a time, dealt to the cluster's warps.  Lane (q, c) gets row
+      // q's m and l in part c and its weight; then a lane has four channels of each row.
+      // All loads of a step are under way together: each takes a microsecond.
+      const int all = static_cast<int>(min(left, static_cast<int64_t>(2 * kTile)));
+      const int q_of = lane >> 3, c_of = lane & 7;
+      const bool bad = __any_sync(0xFFFFFFFFu, c_of < cluster && ld_cluster_s32(&sh.any_bad, min(c_of, cluster - 1)) != 0);
+      for (int first = 4 * (split * 8 + warp); first < all; first += 4 * 8 * cluster) {
+        float pm = -INFINITY, pl = 0.f;
+        if (c_of < cluster) {
+          pm = ld_cluster_f32(part_ml + 2 * (first + q_of), c_of);
+          pl = ld_cluster_f32(part_ml + 2 * (first + q_of) + 1, c_of);
         }
-        __syncwarp();
+        float top = pm;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        // a part without keys has l = 0 (or NaN, which has to stay)
+        float weight = pm == -INFINITY ? 0.f : fast_exp2(pm - top);
+        float sum = pm == -INFINITY ? pl : weight * pl;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        const float inv_row = sum == 0.f ? 0.f : 1.f / sum;
+        const int ch = 4 * lane;
+        float x[4][4] = {};
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c) {
+          if (c < cluster) {
+            float4 y[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              y[q] = ch < DP ? ld_cluster_f32x4(part + (first + q) * C::kPartLd + ch, c)
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float w = __shfl_sync(0xFFFFFFFFu, weight, 8 * q + c);
+              // weight 0: what is there may be anything (rows without a thread's part)
+              x[q][0] += w == 0.f ? 0.f : w * y[q].x;
+              x[q][1] += w == 0.f ? 0.f : w * y[q].y;
+              x[q][2] += w == 0.f ? 0.f : w * y[q].z;
+              x[q][3] += w == 0.f ? 0.f : w * y[q].w;
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float inv = __shfl_sync(0xFFFFFFFFu, inv_row, 8 * q);
+          if (first + q < all && ch < a.d) {
+            const uint32_t row = static_cast<uint32_t>(r0) + first + q;
+            const uint32_t token = row_token(row, a.group);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[q][e] *= inv;
+              if (bad) {
+                const int vis_q = paged_visible(seq, token);
+                for (int c = 0; c < cluster; ++c)
+                  if (ld_cluster_s32(&sh.first_bad[kE4m3 ? 0 : ch + e], c) < vis_q)
+                    x[q][e] = __uint_as_float(0x7FC00000u);
+              }
+            }
+            *reinterpret_cast<uint2*>(a.out + (seq.row0 + token) * a.out_ld +
+                                      (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d +
+                                      ch) =
+                make_uint2(pack_bf16(x[q][0], x[q][1]), pack_bf16(x[q][2], x[q][3]));
+          }
+        }
       }
       cluster_sync();  // no block leaves while another reads its part
     }
@@ -975,15 +1026,17 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_units = static_cast<int>((most_rows + 2 * kTile - 1) / (2 * kTile));
   const int64_t units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
-  // How many blocks share a unit's keys: what takes the fewest rounds of steps, a
-  // block costing about four steps more than its keys, ten where its part is joined.
+  // How many blocks share a unit's keys: what takes clearly the fewest rounds of steps
+  // (a step is about 3000 cycles), if every sequence were as long as the table allows.  A
+  // block costs about three steps more than its keys, a split one eight and more: its
+  // part goes through distributed shared memory.
   const int64_t sms = device_sm_count();
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
   int cluster = 1;
-  int64_t best = 0;
-  for (int c = 1; c <= kMaxSplit; c *= 2) {
-    const int64_t cost = ((units * c + sms - 1) / sms) * ((steps + c - 1) / c + (c > 1 ? 10 : 4));
-    if (c == 1 || cost < best) {
+  int64_t best = ((units + sms - 1) / sms) * (steps + 3);
+  for (int c = 2; c <= kMaxSplit; c *= 2) {
+    const int64_t cost = ((units * c + sms - 1) / sms) * ((steps + c - 1) / c + 6 + c / 2);
+    if (10 * cost < 9 * best) {
       best = cost;
       cluster = c;
     }

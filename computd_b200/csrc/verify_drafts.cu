@@ -16,6 +16,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cstdint>
 
 #include "dwa_internal.h"
@@ -28,6 +29,7 @@ namespace {
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyMaxCluster = 8;
+constexpr int kBatch = 4;
 
 struct VerifyArgs {
   const void *target, *draft;
@@ -52,9 +54,10 @@ __device__ __forceinline__ float prob(const T* p) {
 // Not a positive finite number: nothing.
 __device__ __forceinline__ float mass(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
 
+// Entries i .. i + 3 of a row, zeros from V on.
 template <typename T>
 __device__ __forceinline__ void probs4(const T* row, int i, int V, int wide, float (&x)[4]) {
-  if (wide) {
+  if (wide && i < V) {
     if constexpr (sizeof(T) == 2) {
       const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + i));
       x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xFFFF0000u);
@@ -69,18 +72,14 @@ __device__ __forceinline__ void probs4(const T* row, int i, int V, int wide, flo
   }
 }
 
-// The weights of entries i .. i + 3 (i + 3 < V when wide).  `one` is the index
-// at which a certain drafter's q is 1 (-1: q is the row, or nothing).
-template <typename T>
-__device__ __forceinline__ void weights4(const T* p, const T* q, int one, int i, int V, int wide,
+// The weights of four entries from p's and q's values there (q's zeros where there is
+// none).  `one` is the place, of 0 to 3, at which a certain drafter's q is 1.
+__device__ __forceinline__ void weights4(const float (&p)[4], const float (&q)[4], int one,
                                          double (&w)[4]) {
-  float a[4], b[4] = {};
-  probs4(p, i, V, wide, a);
-  if (q != nullptr) probs4(q, i, V, wide, b);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double x = static_cast<double>(mass(a[j])) - static_cast<double>(mass(b[j]));
-    w[j] = x > 0.0 && i + j != one ? x : 0.0;
+    const double x = static_cast<double>(mass(p[j])) - static_cast<double>(mass(q[j]));
+    w[j] = x > 0.0 && j != one ? x : 0.0;
   }
 }
 
@@ -103,7 +102,6 @@ template <typename T>
 __global__ void __launch_bounds__(kVerifyThreads)
     verify_drafts_kernel(const VerifyArgs a, const int cluster) {
   __shared__ double sums[2][kVerifyWarps];
-  __shared__ double all[kVerifyMaxCluster * kVerifyWarps];
   const int rank = static_cast<int>(blockIdx.x % cluster);
   const int64_t b = blockIdx.x / cluster;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -133,89 +131,121 @@ __global__ void __launch_bounds__(kVerifyThreads)
 
   const T* p = target + static_cast<int64_t>(kept) * V;
   const T* q = kept < n && draft ? draft + static_cast<int64_t>(kept) * V : nullptr;
-  int one = kept < n && !draft ? a.tokens[b * K + kept] : -1;
+  // far below every entry where no drafter was certain
+  int one = kept < n && !draft ? a.tokens[b * K + kept] : INT_MIN / 2;
   const double u = a.sample_u[b];
   const int pieces = cluster * kVerifyWarps;
   const int lo = min((rank * kVerifyWarps + warp) * a.piece, V);
   const int hi = min(lo + a.piece, V);
   int token = -1;
-  bool mine = false;  // this warp holds the draw
+  bool mine = false;  // this warp writes the outcome
   for (int pass = 0; pass < 2; ++pass) {
+    // Rows of 128 entries, kBatch of them under way together.
     double s = 0.0;
-    for (int i = lo + 4 * lane; i < hi; i += 128) {
-      double w[4];
-      weights4(p, q, one, i, V, a.wide, w);
-      s += (w[0] + w[1]) + (w[2] + w[3]);
+    for (int i0 = lo; i0 < hi; i0 += 128 * kBatch) {
+      float x[kBatch][4], y[kBatch][4] = {};
+#pragma unroll
+      for (int r = 0; r < kBatch; ++r) {
+        const int i = i0 + 128 * r + 4 * lane;
+        probs4(p, i, hi, a.wide, x[r]);
+        if (q != nullptr) probs4(q, i, hi, a.wide, y[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < kBatch; ++r) {
+        double w[4];
+        weights4(x[r], y[r], one - (i0 + 128 * r + 4 * lane), w);
+        s += (w[0] + w[1]) + (w[2] + w[3]);
+      }
     }
     s = warp_sum(s);
     if (lane == 0) sums[pass][warp] = s;
     cluster_sync();
-    if (threadIdx.x < pieces)
-      all[threadIdx.x] =
-          ld_cluster_f64(&sums[pass][threadIdx.x % kVerifyWarps], threadIdx.x / kVerifyWarps);
-    __syncthreads();
-    double total = 0.0;
-    for (int i = 0; i < pieces; ++i) total += all[i];
+    // Lane l has the sums of pieces 2 l and 2 l + 1, and by a scan what lies before them;
+    // every block computes the same.
+    double mine0 = 0.0, mine1 = 0.0;
+    if (2 * lane < pieces) {
+      const int c = 2 * lane / kVerifyWarps, k = 2 * lane % kVerifyWarps;
+      mine0 = ld_cluster_f64(&sums[pass][k], c);
+      mine1 = ld_cluster_f64(&sums[pass][k + 1], c);
+    }
+    double before = mine0 + mine1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xFFFFFFFFu, before, o);
+      if (lane >= o) before += y;
+    }
+    const double total = __shfl_sync(0xFFFFFFFFu, before, 31);
     if (total > 0.0) {
       const double goal = u * total;
-      double before = 0.0;
-      int at = -1, last = 0;
-      double base = 0.0, last_base = 0.0;
-      for (int i = 0; i < pieces; ++i) {  // the first piece whose running sum passes the goal
-        if (all[i] > 0.0) { last = i; last_base = before; }
-        if (at < 0 && before + all[i] > goal) { at = i; base = before; }
-        before += all[i];
-      }
-      if (at < 0) { at = last; base = last_base; }
+      before -= mine0 + mine1;  // within rounding: what this decides is decided once, below
+      const double mid = before + mine0;
+      // the first piece whose running sum passes the goal, or the last with any weight
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, (mine0 > 0.0 && mid > goal) ||
+                                                           (mine1 > 0.0 && mid + mine1 > goal));
+      const uint32_t some = __ballot_sync(0xFFFFFFFFu, mine0 > 0.0 || mine1 > 0.0);
+      const int src = past ? __ffs(past) - 1 : 31 - __clz(some);
+      const bool first = past ? mine0 > 0.0 && mid > goal : !(mine1 > 0.0);
+      const int at = __shfl_sync(0xFFFFFFFFu, 2 * lane + (first ? 0 : 1), src);
+      double run = __shfl_sync(0xFFFFFFFFu, first ? before : mid, src);
       if (at == rank * kVerifyWarps + warp) {
         mine = true;
-        double run = base;
-        for (int i0 = lo; i0 < hi; i0 += 128) {
-          double w[4] = {};
-          const int i = i0 + 4 * lane;
-          if (i < hi) weights4(p, q, one, i, V, a.wide, w);
-          const double four = (w[0] + w[1]) + (w[2] + w[3]);
-          double incl = four;
+        bool found = false;
+        for (int i0 = lo; i0 < hi && !found; i0 += 128 * kBatch) {
+          float x[kBatch][4], y[kBatch][4] = {};
+          double row[kBatch];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-            if (lane >= o) incl += y;
+          for (int r = 0; r < kBatch; ++r) {
+            const int i = i0 + 128 * r + 4 * lane;
+            probs4(p, i, hi, a.wide, x[r]);
+            if (q != nullptr) probs4(q, i, hi, a.wide, y[r]);
           }
-          // the last entry with weight so far: the answer where rounding keeps
-          // the piece's own running sum at the goal
-          const uint32_t some = __ballot_sync(0xFFFFFFFFu, four > 0.0);
-          if (some) {
-            const int src = 31 - __clz(some);
-            const int j = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;
-            token = __shfl_sync(0xFFFFFFFFu, i + j, src);
+#pragma unroll
+          for (int r = 0; r < kBatch; ++r) {
+            double w[4];
+            weights4(x[r], y[r], one - (i0 + 128 * r + 4 * lane), w);
+            row[r] = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
           }
-          const uint32_t past = __ballot_sync(0xFFFFFFFFu, four > 0.0 && run + incl > goal);
-          if (past) {
-            const int src = __ffs(past) - 1;
-            double c = run + (incl - four);
-            int j = 0;
-            for (; j < 3; ++j) {
-              c += w[j];
-              if (w[j] > 0.0 && c > goal) break;
+#pragma unroll
+          for (int r = 0; r < kBatch; ++r) {
+            // a row is looked into where the draw is in it, and where it may be the last
+            // with weight: the answer then, where rounding keeps the running sum at the goal
+            if (found || !(row[r] > 0.0)) continue;
+            const int i = i0 + 128 * r + 4 * lane;
+            double w[4];
+            weights4(x[r], y[r], one - i, w);
+            const double four = (w[0] + w[1]) + (w[2] + w[3]);
+            double incl = four;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double z = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+              if (lane >= o) incl += z;
             }
-            while (j > 0 && !(w[j] > 0.0)) --j;
-            token = __shfl_sync(0xFFFFFFFFu, i + j, src);
-            break;
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, four > 0.0 && run + incl > goal);
+            const uint32_t any = __ballot_sync(0xFFFFFFFFu, four > 0.0);
+            int j = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;  // the last with weight
+            if (hit) {
+              double c = run + (incl - four);
+#pragma unroll
+              for (int k = 2; k >= 0; --k) {
+                double head = c + w[0];
+                if (k > 0) head += w[1];
+                if (k > 1) head += w[2];
+                if (w[k] > 0.0 && head > goal) j = k;
+              }
+            }
+            token = __shfl_sync(0xFFFFFFFFu, i + j, hit ? __ffs(hit) - 1 : 31 - __clz(any));
+            found = hit != 0;
+            run += row[r];
           }
-          run += __shfl_sync(0xFFFFFFFFu, incl, 31);
         }
       }
       break;
     }
+    if (pass == 1 && rank == 0 && warp == 0) mine = true;  // no mass anywhere: token -1
     // nothing left of p - q: draw from p
     q = nullptr;
-    one = -1;
-    __syncthreads();
+    one = INT_MIN / 2;
   }
-  // no mass anywhere: the first warp writes token -1
-  bool any = false;
-  for (int i = 0; i < pieces; ++i) any = any || all[i] > 0.0;
-  if (!any && rank == 0 && warp == 0) mine = true;
   if (mine) {
     if (lane == 0) a.n_accepted[b] = kept;
     for (int i = lane; i <= K; i += 32)
