@@ -19,7 +19,8 @@ namespace dwa {
 namespace {
 
 constexpr int kWriteThreads = 256;
-constexpr int kWriteBlocks = 4;    // per SM
+constexpr int kWriteBlocks = 4;    // per SM, from bf16 and from f32
+constexpr int kWriteBlocksF32 = 2;
 constexpr int kGroupTokens = 64;   // tokens of a block checked for repeated slots at a time
 constexpr int kFilterBits = 1024;  // their slots' low bits
 
@@ -27,100 +28,116 @@ __device__ __forceinline__ void report(int32_t* status) {
   if (status != nullptr) atomicCAS(status, 0, DWA_ERR_DEVICE_CHECK);
 }
 
-// Eight consecutive values of a source row: 16 bytes of bf16, or 32 of f32.
+// Sixteen consecutive values of a source row: 32 bytes of bf16, or 64 of f32.
 template <bool kBf16>
-struct Raw8 {
-  uint4 w[kBf16 ? 1 : 2];
+struct Raw16 {
+  uint4 w[kBf16 ? 2 : 4];
 };
 template <bool kBf16>
-__device__ __forceinline__ Raw8<kBf16> load8(const void* row, int64_t at) {
-  Raw8<kBf16> r;
-  if constexpr (kBf16) {
-    r.w[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + at));
-  } else {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(row) + at);
-    r.w[0] = __ldg(p);
-    r.w[1] = __ldg(p + 1);
-  }
+__device__ __forceinline__ Raw16<kBf16> load16(const void* row, int64_t at) {
+  Raw16<kBf16> r;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + at * (kBf16 ? 2 : 4));
+#pragma unroll
+  for (int i = 0; i < (kBf16 ? 2 : 4); ++i) r.w[i] = __ldg(p + i);
   return r;
 }
 template <bool kBf16>
-__device__ __forceinline__ void as_f32(const Raw8<kBf16>& r, float (&x)[8]) {
-  if constexpr (kBf16) {
-    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+__device__ __forceinline__ void as_f32(const Raw16<kBf16>& r, float (&x)[16]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    }
-  } else {
+  for (int i = 0; i < (kBf16 ? 2 : 4); ++i) {
+    const uint32_t u[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      x[4 * i] = __uint_as_float(r.w[i].x); x[4 * i + 1] = __uint_as_float(r.w[i].y);
-      x[4 * i + 2] = __uint_as_float(r.w[i].z); x[4 * i + 3] = __uint_as_float(r.w[i].w);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kBf16) {
+        x[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+        x[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+      } else {
+        x[4 * i + j] = __uint_as_float(u[j]);
+      }
     }
   }
 }
 
-// Stores the eight values of this lane (of `lanes` lanes that hold one vector).
+// x / b correctly rounded, given y = 1 / b correctly rounded: with q = x y the remainder
+// x - q b is exact in an fma, and q + remainder y is the rounded quotient (Markstein,
+// 1990), as long as nothing underflows on the way.
+__device__ __forceinline__ float quotient(float x, float b, float y) {
+  const float q = x * y;
+  return fmaf(fmaf(-q, b, x), y, q);
+}
+
+__device__ __forceinline__ uint4 codes16(const float (&x)[16]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    u[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]),
+                                                          __NV_SATFINITE, __NV_E4M3)) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]),
+                                                          __NV_SATFINITE, __NV_E4M3)) << 16;
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+// Stores the sixteen values of this lane (of `lanes` lanes that hold one vector).
 // Every lane of the warp takes part in the shuffles; `on` says whether it
 // holds values, `keep` whether they are stored.
-template <bool kE4m3>
-__device__ __forceinline__ void store8(const float (&x)[8], bool on, bool keep, int lanes, int lane,
-                                       void* cache, float* scales, int64_t row, int64_t srow, int d) {
+template <bool kE4m3, bool kBf16>
+__device__ __forceinline__ void store16(const Raw16<kBf16>& raw, bool on, bool keep, int lanes, int lane,
+                                        void* cache, float* scales, int64_t row, int64_t srow, int d) {
   if constexpr (!kE4m3) {
     if (on && keep) {
-      uint32_t u[4];
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + row * d + 16 * lane);
+      if constexpr (kBf16) {
+        dst[0] = raw.w[0];
+        dst[1] = raw.w[1];
+      } else {
+        float x[16];
+        as_f32(raw, x);
+        uint32_t u[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          u[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
+        dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
       }
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + row * d + 8 * lane) =
-          make_uint4(u[0], u[1], u[2], u[3]);
     }
     return;
   }
+  float x[16];
+  as_f32(raw, x);
   // The largest magnitude as bits: NaN orders above infinity above every finite number.
   uint32_t top = 0;
   if (on) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
   }
   for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  const bool finite = top < 0x7F800000u;
-  const float scale = finite ? fmaxf(__fdiv_rn(__uint_as_float(top), 448.f), 0x1p-126f)
-                             : __uint_as_float(0x7FC00000u);
   if (!keep) return;
-  if (on) {
-    // x / scale, |x / scale| <= 448 (1 + 2^-23), which rounds to 448 at most.  One
-    // reciprocal for all: with y = 1 / scale rounded, q = x y, the remainder
-    // x - q scale is exact in an fma and q + remainder y is the rounded quotient
-    // (Markstein, 1990), as long as nothing underflows: scale above 2^-80 and
-    // quotients above 2^-11 leave the remainder above 2^-138 (smaller quotients
-    // give the code 0 either way).
-    float q[8];
-    if (scale > 0x1p-80f) {
-      const float y = __frcp_rn(scale);
+  const float amax = __uint_as_float(top);
+  const bool finite = top < 0x7F800000u;
+  uint4 w = make_uint4(0, 0, 0, 0);
+  float scale = __uint_as_float(0x7FC00000u);
+  if (finite) {
+    // Tiny vectors are scaled up by 2^100, exactly, so that no remainder underflows: amax is
+    // above 2^-70 or the scale above 2^-26 then.  (Remainders of quotients above 2^-11 are
+    // above 2^-137; smaller quotients give the code 0 either way.)
+    float up = 1.f, down = 1.f, least = 0x1p-126f, most = amax;
+    if (!(amax > 0x1p-70f)) {
+      up = 0x1p100f;
+      down = 0x1p-100f;
+      least = 0x1p-26f;
+      most *= up;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float q0 = x[i] * y;
-        q[i] = fmaf(fmaf(-q0, scale, x[i]), y, q0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = finite ? __fdiv_rn(x[i], scale) : 0.f;
+      for (int i = 0; i < 16; ++i) x[i] *= up;
     }
-    uint32_t w[2];
+    const float s = fmaxf(quotient(most, 448.f, 1.f / 448.f), least);
+    const float y = __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]),
-                                                            __NV_SATFINITE, __NV_E4M3)) |
-             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(
-                 make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3)) << 16;
-    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(cache) + row * d + 8 * lane) =
-        make_uint2(w[0], w[1]);
+    for (int i = 0; i < 16; ++i) x[i] = quotient(x[i], s, y);
+    w = codes16(x);  // |x / s| <= 448 (1 + 2^-23), which rounds to 448 at most
+    scale = s * down;
   }
+  if (on) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(cache) + row * d + 16 * lane) = w;
   if (lane == 0) scales[srow] = scale;
 }
 
@@ -136,19 +153,19 @@ struct WriteArgs {
   int page_log2;
   int64_t ld_page, ld_scale_page;  // in vectors (rows of d) and in scales
   int64_t tokens_per_block;
-  int lanes_log2;  // lanes per vector: the power of two >= d / 8
+  int lanes_log2;  // lanes per vector: the power of two >= d / 16
   int32_t* status;
 };
 
 // A block owns a run of tokens.  `lanes` neighbouring lanes hold one (token,
-// head) vector of K and of V, 8 values each; the amax is a shuffle over them.
+// head) vector of K and of V, 16 values each; the amax is a shuffle over them.
 // Where slots repeat the last token must stay, whichever block writes first:
 // each block drops its tokens whose slot a later token names.  It looks the
 // slots after its own up in a filter of its own slots' low bits, so the whole
 // list is read once per block (from L2: 19 MB in all for 8192 tokens, against
 // the 200 MB of keys and values at 32 heads of 128).
 template <bool kE4m3, bool kSrcBf16>
-__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, kSrcBf16 ? kWriteBlocks : kWriteBlocksF32) kv_write_kernel(const WriteArgs a) {
   __shared__ int64_t own[kGroupTokens];
   __shared__ int dropped[kGroupTokens];
   __shared__ uint32_t filter[kFilterBits / 32];
@@ -157,22 +174,29 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(c
   const int lane = threadIdx.x & (lanes - 1);
   const int group = threadIdx.x >> a.lanes_log2;
   const int groups = kWriteThreads >> a.lanes_log2;
-  const bool on = 8 * lane < a.d;
+  const bool on = 16 * lane < a.d;
   const int64_t t_end = min((blockIdx.x + 1) * a.tokens_per_block, a.T);
   for (int64_t t0 = blockIdx.x * a.tokens_per_block; t0 < t_end; t0 += kGroupTokens) {
     const int n = static_cast<int>(min(t_end - t0, static_cast<int64_t>(kGroupTokens)));
     const int vectors = n * a.H;
     // a round's values are under way while the round before is stored, the first ones
     // while the slots are checked
-    auto load = [&](int vec, Raw8<kSrcBf16>* k, Raw8<kSrcBf16>* v) {
-      if (vec < vectors && on) {
-        const int i = vec / a.H, h = vec - i * a.H;
-        *k = load8<kSrcBf16>(a.k, (t0 + i) * a.k_tok + h * a.k_head + 8 * lane);
-        *v = load8<kSrcBf16>(a.v, (t0 + i) * a.v_tok + h * a.v_head + 8 * lane);
+    auto load = [&](int i, int h, Raw16<kSrcBf16>* k, Raw16<kSrcBf16>* v) {
+      if (i < n && on) {
+        *k = load16<kSrcBf16>(a.k, (t0 + i) * a.k_tok + h * a.k_head + 16 * lane);
+        *v = load16<kSrcBf16>(a.v, (t0 + i) * a.v_tok + h * a.v_head + 16 * lane);
       }
     };
-    Raw8<kSrcBf16> k_now{}, v_now{};
-    load(group, &k_now, &v_now);
+    auto forward = [&](int* i, int* h) {  // to this group's next vector
+      *h += groups;
+      while (*h >= a.H) {
+        *h -= a.H;
+        ++*i;
+      }
+    };
+    Raw16<kSrcBf16> k_now{}, v_now{};
+    int i_now = group / a.H, h_now = group % a.H;
+    load(i_now, h_now, &k_now, &v_now);
     __syncthreads();
     for (int i = threadIdx.x; i < kFilterBits / 32; i += kWriteThreads) filter[i] = 0;
     __syncthreads();
@@ -202,24 +226,23 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(c
     }
     __syncthreads();
     for (int base = 0; base < vectors; base += groups) {
-      const int vec = base + group;
-      Raw8<kSrcBf16> k_next{}, v_next{};
-      load(vec + groups, &k_next, &v_next);
-      const bool here = vec < vectors;
-      const int i = here ? vec / a.H : 0, h = here ? vec - i * a.H : 0;
-      const bool keep = here && !dropped[i];
-      const int64_t s = keep ? own[i] : 0;
+      int i_next = i_now, h_next = h_now;
+      forward(&i_next, &h_next);
+      Raw16<kSrcBf16> k_next{}, v_next{};
+      load(i_next, h_next, &k_next, &v_next);
+      const bool here = i_now < n;
+      const bool keep = here && !dropped[here ? i_now : 0];
+      const int64_t s = keep ? own[i_now] : 0;
       const int64_t page = s >> a.page_log2, off = s & ((1 << a.page_log2) - 1);
-      const int64_t in_page = (static_cast<int64_t>(h) << a.page_log2) + off;
+      const int64_t in_page = (static_cast<int64_t>(h_now) << a.page_log2) + off;
       const int64_t row = page * a.ld_page + in_page;
       const int64_t srow = page * a.ld_scale_page + in_page;
-      float x[8];
-      as_f32(k_now, x);
-      store8<kE4m3>(x, here && on, keep, lanes, lane, a.k_cache, a.k_scale, row, srow, a.d);
-      as_f32(v_now, x);
-      store8<kE4m3>(x, here && on, keep, lanes, lane, a.v_cache, a.v_scale, row, srow, a.d);
+      store16<kE4m3>(k_now, here && on, keep, lanes, lane, a.k_cache, a.k_scale, row, srow, a.d);
+      store16<kE4m3>(v_now, here && on, keep, lanes, lane, a.v_cache, a.v_scale, row, srow, a.d);
       k_now = k_next;
       v_now = v_next;
+      i_now = i_next;
+      h_now = h_next;
     }
   }
 }
@@ -240,61 +263,99 @@ struct ReadArgs {
 };
 
 constexpr int kReadThreads = 256;
+constexpr int kReadVectors = 2;
 
-// Sixteen values of this lane as bf16: one 16-byte load of codes (or two of
-// bf16), two 16-byte stores.
+// Sixteen values of a lane on their way: 16 bytes of codes and their scale, or 32 bytes of bf16.
 template <bool kE4m3>
-__device__ __forceinline__ void read16(const void* cache, const float* scales, int64_t row,
-                                       int64_t srow, int d, int lane, bool fine, uint32_t fill,
-                                       uint16_t* out) {
-  uint32_t o[8];
-  if (!fine) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fill;
-  } else if (kE4m3) {
-    const uint4 w = __ldg(
-        reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + row * d + 16 * lane));
-    const float scale = __ldg(scales + srow);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+struct Held16 {
+  uint4 w[kE4m3 ? 1 : 2];
+  float scale;
+};
+template <bool kE4m3>
+__device__ __forceinline__ Held16<kE4m3> fetch16(const void* cache, const float* scales, int64_t row,
+                                                 int64_t srow, int d, int lane) {
+  Held16<kE4m3> x;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(cache) +
+                                                  (row * d + 16 * lane) * (kE4m3 ? 1 : 2));
+  x.w[0] = __ldg(p);
+  if constexpr (kE4m3) x.scale = __ldg(scales + srow);
+  else x.w[1] = __ldg(p + 1);
+  return x;
+}
+// Two 16-byte stores of bf16; streaming, since nobody reads the cache's copy again soon.
+template <bool kE4m3>
+__device__ __forceinline__ void put16(const Held16<kE4m3>& x, uint16_t* out) {
+  uint4 o[2];
+  if constexpr (kE4m3) {
+    const uint32_t u[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
+    uint32_t r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
           static_cast<__nv_fp8x2_storage_t>(u[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
       const float2 f = __half22float2(__half2(h));
-      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
-      o[i] = *reinterpret_cast<const uint32_t*>(&b);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * x.scale, f.y * x.scale);
+      r[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
+    o[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    o[1] = make_uint4(r[4], r[5], r[6], r[7]);
   } else {
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(cache) + row * d +
-                                                    16 * lane);
-    const uint4 w = __ldg(p), x = __ldg(p + 1);
-    o[0] = w.x; o[1] = w.y; o[2] = w.z; o[3] = w.w;
-    o[4] = x.x; o[5] = x.y; o[6] = x.z; o[7] = x.w;
+    o[0] = x.w[0];
+    o[1] = x.w[1];
   }
-  uint4* dst = reinterpret_cast<uint4*>(out + 16 * lane);
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  __stcs(reinterpret_cast<uint4*>(out), o[0]);
+  __stcs(reinterpret_cast<uint4*>(out) + 1, o[1]);
 }
 
+// A group of lanes brings kReadVectors (token, head) vectors of K and of V, a block's
+// groups neighbouring ones at a time; all its loads are under way before the first store.
 template <bool kE4m3>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a) {
   const int lane = threadIdx.x & ((1 << a.lanes_log2) - 1);
-  const int64_t vec =
-      (static_cast<int64_t>(blockIdx.x) * kReadThreads + threadIdx.x) >> a.lanes_log2;
-  if (vec >= a.T * a.H || 16 * lane >= a.d) return;
-  const int64_t t = vec / a.H;
-  const int h = static_cast<int>(vec - t * a.H);
-  const int64_t s = __ldg(a.slots + t);
-  const bool skipped = s == -1;
-  if (skipped && !a.clear_skipped) return;
-  const bool fine = s >= 0 && s < a.n_slots;
-  if (!fine && !skipped) report(a.status);
-  const uint32_t fill = skipped ? 0u : 0x7FC07FC0u;  // zeros, or NaN for a slot outside the cache
-  const int64_t page = s >> a.page_log2, off = s & ((1 << a.page_log2) - 1);
-  const int64_t in_page = (static_cast<int64_t>(h) << a.page_log2) + off;
-  const int64_t row = page * a.ld_page + in_page, srow = page * a.ld_scale_page + in_page;
-  read16<kE4m3>(a.k_cache, a.k_scale, row, srow, a.d, lane, fine, fill, a.k_out + vec * a.d);
-  read16<kE4m3>(a.v_cache, a.v_scale, row, srow, a.d, lane, fine, fill, a.v_out + vec * a.d);
+  const int groups = kReadThreads >> a.lanes_log2;
+  if (16 * lane >= a.d) return;
+  const int64_t vectors = a.T * a.H;
+  const int64_t vec0 = static_cast<int64_t>(blockIdx.x) * groups * kReadVectors + (threadIdx.x >> a.lanes_log2);
+  int64_t s[kReadVectors];
+  int h[kReadVectors];
+#pragma unroll
+  for (int i = 0; i < kReadVectors; ++i) {
+    const int64_t vec = vec0 + static_cast<int64_t>(i) * groups;
+    const int64_t t = vec / a.H;
+    h[i] = static_cast<int>(vec - t * a.H);
+    s[i] = vec < vectors ? __ldg(a.slots + t) : -1;
+  }
+  Held16<kE4m3> k[kReadVectors], v[kReadVectors];
+#pragma unroll
+  for (int i = 0; i < kReadVectors; ++i) {
+    if (s[i] >= 0 && s[i] < a.n_slots) {
+      const int64_t page = s[i] >> a.page_log2, off = s[i] & ((1 << a.page_log2) - 1);
+      const int64_t in_page = (static_cast<int64_t>(h[i]) << a.page_log2) + off;
+      const int64_t row = page * a.ld_page + in_page, srow = page * a.ld_scale_page + in_page;
+      k[i] = fetch16<kE4m3>(a.k_cache, a.k_scale, row, srow, a.d, lane);
+      v[i] = fetch16<kE4m3>(a.v_cache, a.v_scale, row, srow, a.d, lane);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kReadVectors; ++i) {
+    const int64_t vec = vec0 + static_cast<int64_t>(i) * groups;
+    const bool skipped = s[i] == -1;
+    if (vec >= vectors || (skipped && !a.clear_skipped)) continue;
+    uint16_t* k_out = a.k_out + vec * a.d + 16 * lane;
+    uint16_t* v_out = a.v_out + vec * a.d + 16 * lane;
+    if (s[i] >= 0 && s[i] < a.n_slots) {
+      put16<kE4m3>(k[i], k_out);
+      put16<kE4m3>(v[i], v_out);
+    } else {
+      if (!skipped) report(a.status);
+      const uint32_t fill = skipped ? 0u : 0x7FC07FC0u;  // zeros, or NaN for a slot outside the cache
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        reinterpret_cast<uint4*>(k_out)[j] = make_uint4(fill, fill, fill, fill);
+        reinterpret_cast<uint4*>(v_out)[j] = make_uint4(fill, fill, fill, fill);
+      }
+    }
+  }
 }
 
 int log2_at_least(int n) {
@@ -317,9 +378,9 @@ cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, 
   a.page_log2 = log2_at_least(c.page_size);
   a.n_slots = c.n_pages << a.page_log2;
   a.ld_page = c.ld_page / c.d; a.ld_scale_page = c.ld_scale_page;
-  a.lanes_log2 = log2_at_least(c.d / 8);
+  a.lanes_log2 = log2_at_least(c.d / 16);
   a.status = status;
-  const int64_t most = static_cast<int64_t>(kWriteBlocks) * device_sm_count();
+  const int64_t most = static_cast<int64_t>(src_bf16 ? kWriteBlocks : kWriteBlocksF32) * device_sm_count();
   a.tokens_per_block = (T + most - 1) / most;
   const unsigned grid = static_cast<unsigned>((T + a.tokens_per_block - 1) / a.tokens_per_block);
   if (c.k_scale != nullptr) {
@@ -344,7 +405,7 @@ cudaError_t launch_kv_read(const KvCacheView& c, const int64_t* slots, int64_t T
   a.lanes_log2 = log2_at_least(c.d / 16);
   a.clear_skipped = clear_skipped;
   a.status = status;
-  const int64_t per_block = kReadThreads >> a.lanes_log2;
+  const int64_t per_block = (kReadThreads >> a.lanes_log2) * kReadVectors;
   const unsigned grid = static_cast<unsigned>((T * c.H + per_block - 1) / per_block);
   if (c.k_scale != nullptr) kv_read_kernel<true><<<grid, kReadThreads, 0, stream>>>(a);
   else kv_read_kernel<false><<<grid, kReadThreads, 0, stream>>>(a);

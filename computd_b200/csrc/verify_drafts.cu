@@ -99,7 +99,7 @@ __device__ __forceinline__ double ld_cluster_f64(const double* local, int rank) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads)
+__global__ void __launch_bounds__(kVerifyThreads, 4)
     verify_drafts_kernel(const VerifyArgs a, const int cluster) {
   __shared__ double sums[2][kVerifyWarps];
   const int rank = static_cast<int>(blockIdx.x % cluster);
@@ -109,14 +109,15 @@ __global__ void __launch_bounds__(kVerifyThreads)
   const T* target = static_cast<const T*>(a.target) + b * (K + 1) * V;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * K * V : nullptr;
 
-  // How many drafts stand: every warp for itself.
+  // How many drafts stand: every warp for itself.  The tests' values are fetched
+  // without waiting for the number of drafts.
   int n = a.draft_lengths ? a.draft_lengths[b] : K;
-  n = min(max(n, 0), K);
-  int kept = n;
-  for (int i0 = 0; i0 < n && kept == n; i0 += 32) {
+  const double u = a.sample_u[b];
+  int kept = K;
+  for (int i0 = 0; i0 < K && kept == K; i0 += 32) {
     const int i = i0 + lane;
     bool stands = true;
-    if (i < n) {
+    if (i < K) {
       const int x = a.tokens[b * K + i];
       stands = false;
       if (x >= 0 && x < V) {
@@ -128,12 +129,13 @@ __global__ void __launch_bounds__(kVerifyThreads)
     const uint32_t fallen = __ballot_sync(0xFFFFFFFFu, !stands);
     if (fallen) kept = i0 + __ffs(fallen) - 1;
   }
+  n = min(max(n, 0), K);
+  kept = min(kept, n);
 
   const T* p = target + static_cast<int64_t>(kept) * V;
   const T* q = kept < n && draft ? draft + static_cast<int64_t>(kept) * V : nullptr;
   // far below every entry where no drafter was certain
   int one = kept < n && !draft ? a.tokens[b * K + kept] : INT_MIN / 2;
-  const double u = a.sample_u[b];
   const int pieces = cluster * kVerifyWarps;
   const int lo = min((rank * kVerifyWarps + warp) * a.piece, V);
   const int hi = min(lo + a.piece, V);

@@ -35,15 +35,21 @@ _I32, _I64 = torch.int32, torch.int64
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _call(fn: str, dev: int, *args) -> None:
+_entries: dict[str, object] = {}  # C entry points by name, once looked up
+
+
+def _call(name: str, dev: int, *args) -> None:
     """One C call on device `dev`'s current stream, with that device current."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
     if dev == _current_device():
-        st = getattr(_lib.load(), fn)(*args, _raw_stream(dev))
+        st = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            st = getattr(_lib.load(), fn)(*args, _raw_stream(dev))
+            st = fn(*args, _raw_stream(dev))
     if st:
-        _lib.check(st, fn)
+        _lib.check(st, name)
 
 
 def _cache_args(k_cache, v_cache, k_scale, v_scale):
