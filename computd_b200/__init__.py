@@ -10,7 +10,8 @@ provides device memory, streams and torch.distributed plumbing only.
 from ._lib import DWA_MAX_K, DWAArgumentError, DWAError, load as load_library
 from .assembler import WeightAssembler, assemble_finish, lowrank_delta, usage_ema_update
 from .assembly import normalise_alpha, weighted_gather_into, weighted_value_sum
-from .kv_cache import kv_cache_read, kv_cache_write, paged_attention, verify_drafts
+from .kv_cache import (PagedKVCache, kv_cache_read, kv_cache_write, paged_attention,
+                       verify_drafts)
 from .pool import ShardSpec, init_normal, new_normal
 from .retrieval import (HostPipeline, HybridParts, MultiAspectRetrieval, PeerExchange, Retriever,
                         chip_topk, exchange_candidates, project_keys, project_keys_packed,
@@ -22,7 +23,7 @@ __all__ = [
     "DWA_MAX_K", "DWAArgumentError", "DWAError", "load_library",
     "WeightAssembler", "assemble_finish", "lowrank_delta", "usage_ema_update",
     "normalise_alpha", "weighted_gather_into", "weighted_value_sum", "MultiAspectRetrieval",
-    "kv_cache_read", "kv_cache_write", "paged_attention", "verify_drafts",
+    "PagedKVCache", "kv_cache_read", "kv_cache_write", "paged_attention", "verify_drafts",
     "ShardSpec", "init_normal", "new_normal",
     "HostPipeline", "HybridParts", "PeerExchange", "Retriever", "chip_topk", "project_keys",
     "project_keys_packed", "exchange_candidates", "reduce_partials",

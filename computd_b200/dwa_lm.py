@@ -40,6 +40,13 @@ over a process group (one cross-shard merge per block, owner-computes value
 sums).  Dense layers (attention, projections, PartA/PartB) are plain
 torch/cuBLAS; retrieval, key projection, assembly delta and its LayerNorm
 finish run in libdwa_b200.so.
+
+``DWALM.extend`` is the same model over a paged key/value cache, for generation
+(the reference runs whole windows for every token, src/training/trainer.py:258-338):
+it takes the newest tokens of any number of sequences (prompts in pieces, single
+tokens, drafted ones), writes their keys and values and attends to the pages with
+``kv_cache``'s kernels.  ``DWALM.verify`` scores drafted tokens that way and
+decides with ``verify_drafts`` which of them stand.
 """
 from __future__ import annotations
 
@@ -51,6 +58,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .assembler import WeightAssembler
+from .kv_cache import PagedKVCache, verify_drafts
 from .lm_ops import aspect_queries, rope_qk
 from .retrieval import MultiAspectRetrieval, Retriever, project_keys_packed
 
@@ -112,6 +120,25 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return torch.cat([x1 * cos - x2 * sin, x1 * sin + x2 * cos], dim=-1)
 
 
+@dataclass(frozen=True)
+class ChunkStep:
+    """What the blocks of one ``DWALM.extend`` share: the rows' rotations and cache slots, and
+    the sequences they belong to."""
+
+    cache: PagedKVCache
+    cos: torch.Tensor          # bf16 [T, dh / 2] by row
+    sin: torch.Tensor
+    slots: torch.Tensor        # int64 [T]
+    block_table: torch.Tensor
+    lengths: torch.Tensor
+    q_start: torch.Tensor
+    max_q: int
+
+
+def _rope_theta(dh: int, device) -> torch.Tensor:
+    return 1.0 / (10000.0 ** (torch.arange(0, dh, 2, device=device) / dh))
+
+
 class CausalSelfAttention(nn.Module):
     """parts.py:30-83: LayerNorm -> QKV -> RoPE -> causal softmax attention -> proj, residual."""
 
@@ -122,8 +149,8 @@ class CausalSelfAttention(nn.Module):
         self.norm = nn.LayerNorm(d, device=device, dtype=dtype)
         self.qkv = nn.Linear(d, 3 * d, bias=False, device=device, dtype=dtype)
         self.proj = nn.Linear(d, d, bias=False, device=device, dtype=dtype)
-        theta = 1.0 / (10000.0 ** (torch.arange(0, self.dh, 2, device=device) / self.dh))
-        f = torch.outer(torch.arange(seq_len, device=device, dtype=torch.float32), theta)
+        f = torch.outer(torch.arange(seq_len, device=device, dtype=torch.float32),
+                        _rope_theta(self.dh, device))
         self.register_buffer("cos", f.cos().to(dtype), persistent=False)
         self.register_buffer("sin", f.sin().to(dtype), persistent=False)
 
@@ -135,6 +162,19 @@ class CausalSelfAttention(nn.Module):
         v = qkv[..., 2 * C:].view(B, S, self.h, self.dh).transpose(1, 2)
         o = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         return x + self.proj(o.transpose(1, 2).reshape(B, S, C))
+
+    def extend(self, x: torch.Tensor, step: ChunkStep, layer: int) -> torch.Tensor:
+        """The same for the newest tokens of the sequences in ``step`` (x [1, T, C], packed):
+        their keys and values go into the cache, their queries attend to it."""
+        _, T, C = x.shape
+        qkv = self.qkv(self.norm(x))
+        q, k = rope_qk(qkv, step.cos, step.sin, self.h, self.dh)
+        q, k = (t.transpose(1, 2)[0] for t in (q, k))  # the kernel's token-major buffers
+        v = qkv[0, :, 2 * C:].view(T, self.h, self.dh)
+        step.cache.write(layer, k, v, step.slots)
+        o = step.cache.attend(layer, q, step.block_table, step.lengths, q_start=step.q_start,
+                              max_q=step.max_q)
+        return x + self.proj(o.view(1, T, C))
 
 
 class DWABlock(nn.Module):
@@ -174,9 +214,17 @@ class DWABlock(nn.Module):
 
     def forward(self, h: torch.Tensor, retriever: Retriever,
                 vectors: torch.Tensor | None = None) -> torch.Tensor:
+        return self._assemble(self.attn(h), retriever, vectors)
+
+    def extend(self, h: torch.Tensor, retriever: Retriever, vectors: torch.Tensor | None,
+               step: ChunkStep, layer: int) -> torch.Tensor:
+        """``forward`` over the cache: h [1, T, C], the rows of ``step``."""
+        return self._assemble(self.attn.extend(h, step, layer), retriever, vectors)
+
+    def _assemble(self, h: torch.Tensor, retriever: Retriever,
+                  vectors: torch.Tensor | None) -> torch.Tensor:
         B, S_len, C = h.shape
         cfg = self.cfg
-        h = self.attn(h)
         z = self.query_proj(h)
         q, w = self.queries(z)  # also the retrieval's {lambda, w . tau, T} in self._params
         if cfg.r > 0:
@@ -232,9 +280,11 @@ class DWALM(nn.Module):
             self.vectors = None
             values = pool_values
         # one retrieval plan shared by all blocks (same pool, same token count)
-        self.retriever = Retriever(pool_keys, values, cfg.tokens, cfg.top_k,
-                                   lambda_sharp=cfg.lambda_sharp, T=cfg.T,
-                                   use_sigmoid=cfg.use_sigmoid, group=group)
+        self._plan = lambda tokens: Retriever(pool_keys, values, tokens, cfg.top_k,
+                                              lambda_sharp=cfg.lambda_sharp, T=cfg.T,
+                                              use_sigmoid=cfg.use_sigmoid, group=group)
+        self.retriever = self._plan(cfg.tokens)
+        self._chunk_retrievers = {cfg.tokens: self.retriever}
 
     @torch.no_grad()
     def forward(self, token_ids: torch.Tensor) -> torch.Tensor:
@@ -242,6 +292,74 @@ class DWALM(nn.Module):
         for blk in self.blocks:
             h = blk(h, self.retriever, self.vectors)
         return self.fc2(F.gelu(self.fc1(self.head_norm(h))))
+
+    def new_cache(self, n_pages: int, page_size: int = 64,
+                  dtype: torch.dtype = torch.bfloat16) -> PagedKVCache:
+        """An empty cache for this model (bfloat16, or float8_e4m3fn at half the size)."""
+        cfg = self.cfg
+        return PagedKVCache(cfg.n_layers, n_pages, page_size, cfg.n_heads, cfg.d_model // cfg.n_heads,
+                            dtype=dtype, device=self.embed.weight.device)
+
+    @torch.no_grad()
+    def extend(self, token_ids: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor,
+               lengths: torch.Tensor, q_start: torch.Tensor | None = None,
+               max_q: int | None = None) -> torch.Tensor:
+        """Logits [T, vocab] of the newest tokens of B sequences, whose earlier tokens are cached.
+
+        ``token_ids`` [T] packs the new tokens: rows q_start[b] to q_start[b + 1] - 1 (int32
+        [B + 1]) of sequence b, or T / B rows each without ``q_start``.  ``lengths`` int32 [B]
+        counts each sequence's tokens, the new ones with them, and ``block_table`` int32
+        [B, max_pages] holds its pages.  ``max_q`` bounds the new tokens of any sequence.
+        Rows behind the last sequence (a padded batch) come out as whatever they are.
+
+        The retrieval is planned once per row count T (a captured graph needs a call with its
+        T before), so a server pads T to a few counts; on a row-sharded pool every rank calls
+        with the same tokens."""
+        T = token_ids.shape[0]
+        if token_ids.dim() != 1:
+            raise ValueError("token_ids must be [T]")
+        B = lengths.shape[0]
+        if q_start is None:
+            if B == 0 or T % B:
+                raise ValueError(f"without q_start {T} rows must be equal chunks of {B} sequences")
+            q_start = torch.arange(0, T + 1, T // B, dtype=torch.int32, device=token_ids.device) \
+                if T else torch.zeros(B + 1, dtype=torch.int32, device=token_ids.device)
+            max_q = T // B
+        if T == 0:
+            return torch.empty((0, self.cfg.vocab), dtype=self.fc2.weight.dtype, device=token_ids.device)
+        retriever = self._chunk_retrievers.get(T)
+        if retriever is None:
+            retriever = self._chunk_retrievers[T] = self._plan(T)
+        slots, positions = cache.slots(block_table, lengths, q_start, T)
+        dh = self.cfg.d_model // self.cfg.n_heads
+        f = torch.outer(positions.float(), _rope_theta(dh, positions.device))
+        dtype = self.embed.weight.dtype
+        step = ChunkStep(cache, f.cos().to(dtype), f.sin().to(dtype), slots, block_table, lengths,
+                         q_start, T if max_q is None else max_q)
+        h = self.embed_norm(self.embed_proj(self.embed(token_ids[None])))
+        for i, blk in enumerate(self.blocks):
+            h = blk.extend(h, retriever, self.vectors, step, i)
+        return self.fc2(F.gelu(self.fc1(self.head_norm(h))))[0]
+
+    @torch.no_grad()
+    def verify(self, last_tokens: torch.Tensor, draft_tokens: torch.Tensor,
+               draft_probs: torch.Tensor | None, accept_u: torch.Tensor, sample_u: torch.Tensor,
+               cache: PagedKVCache, block_table: torch.Tensor, lengths: torch.Tensor, *,
+               temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One speculative step: score K drafted tokens of every sequence at once and keep what
+        ``verify_drafts`` lets stand.
+
+        ``last_tokens`` int [B] (each sequence's newest token, not yet cached) and ``draft_tokens``
+        int32 [B, K] are appended to the ``lengths`` (int32 [B]) cached tokens; the pages in
+        ``block_table`` must have room for K + 1 more.  Returns (n_accepted int32 [B], tokens
+        int32 [B, K + 1] as ``verify_drafts``, new lengths int32 [B]: the cached tokens that
+        stay, the last of ``tokens`` being the next step's ``last_tokens``)."""
+        B, K = draft_tokens.shape
+        chunk = torch.cat([last_tokens.view(B, 1).to(draft_tokens.dtype), draft_tokens], 1)
+        logits = self.extend(chunk.reshape(-1).long(), cache, block_table, lengths + (K + 1))
+        probs = torch.softmax(logits.float().view(B, K + 1, -1) / temperature, -1)
+        accepted, tokens = verify_drafts(probs, draft_tokens, draft_probs, accept_u, sample_u)
+        return accepted, tokens, lengths + 1 + accepted
 
 
 class GraphedForward:

@@ -224,6 +224,84 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return out
 
 
+class PagedKVCache:
+    """The keys and values of a model's layers on one set of pages.
+
+    ``n_pages`` pages of ``page_size`` (16, 32, 64 or 128) tokens in each of
+    ``n_layers`` layers, ``n_kv_heads`` heads of ``head_dim`` (a multiple of 16 up to
+    128), bfloat16 or float8_e4m3fn.  A page number means the same tokens in every
+    layer, so one block table serves them all; which pages belong to which sequence is
+    the caller's.  The methods are this module's calls on one layer."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, *,
+                 dtype: torch.dtype = _BF16, device=None):
+        if dtype not in (_BF16, _E4M3):
+            raise ValueError("dtype must be bfloat16 or float8_e4m3fn")
+        if page_size not in (16, 32, 64, 128):
+            raise ValueError("page_size must be 16, 32, 64 or 128")
+        if head_dim % 16 or not 16 <= head_dim <= 128:
+            raise ValueError("head_dim must be a multiple of 16 up to 128")
+        if min(n_layers, n_pages, n_kv_heads) < 1:
+            raise ValueError("n_layers, n_pages and n_kv_heads must be positive")
+        self.n_layers, self.n_pages, self.page_size = int(n_layers), int(n_pages), int(page_size)
+        shape = (self.n_layers, self.n_pages, int(n_kv_heads), self.page_size, int(head_dim))
+        self.k, self.v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self.k_scale = self.v_scale = None
+        if dtype is _E4M3:
+            self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=_F32, device=device)
+                                          for _ in range(2))
+        # DWA_ERR_DEVICE_CHECK once a call met a bad slot, page, length or row range
+        self.status = torch.zeros((), dtype=_I32, device=device)
+
+    def _layer(self, layer: int):
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of {self.n_layers}")
+        if self.k_scale is None:
+            return self.k[layer], self.v[layer], {"status": self.status}
+        return self.k[layer], self.v[layer], {"k_scale": self.k_scale[layer],
+                                              "v_scale": self.v_scale[layer], "status": self.status}
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """``kv_cache_write`` into one layer."""
+        k_cache, v_cache, more = self._layer(layer)
+        kv_cache_write(k, v, k_cache, v_cache, slots, **more)
+
+    def read(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """``kv_cache_read`` from one layer."""
+        k_cache, v_cache, more = self._layer(layer)
+        return kv_cache_read(k_cache, v_cache, slots, **more)
+
+    def attend(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+               **kw) -> torch.Tensor:
+        """``paged_attention`` over one layer."""
+        k_cache, v_cache, more = self._layer(layer)
+        return paged_attention(q, k_cache, v_cache, block_table, lengths, **more, **kw)
+
+    def slots(self, block_table: torch.Tensor, lengths: torch.Tensor, q_start: torch.Tensor,
+              n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(slots int64, positions int64) of the newest tokens of every sequence, row by row of
+        a packed chunk of ``n_tokens`` rows: row q_start[b] + i is token lengths[b] - n + i of
+        sequence b.  Rows behind q_start[-1], and new tokens that ``lengths`` leaves no
+        place for, get slot -1."""
+        row = torch.arange(n_tokens, device=q_start.device)
+        start, length, table = q_start.long(), lengths.long(), block_table.long()
+        seq = (torch.searchsorted(start, row, right=True) - 1).clamp(0, length.shape[0] - 1)
+        position = length[seq] - start[seq + 1] + row
+        fine = (row < start[-1]) & (position >= 0) & (position < table.shape[1] * self.page_size)
+        at = torch.where(fine, position, 0)
+        page = table[seq, at // self.page_size]
+        return torch.where(fine, page * self.page_size + at % self.page_size, -1), at
+
+    def check(self) -> None:
+        """Raise ``DWAError`` if a call so far met a bad slot, page, length or row range (waits
+        for the device)."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            raise _lib.DWAError(code, "PagedKVCache", "a slot, page number, length or row range was "
+                                "outside the cache or the call")
+
+
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor,
                   draft_probs: torch.Tensor | None, accept_u: torch.Tensor, sample_u: torch.Tensor, *,
                   draft_lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
