@@ -5,7 +5,9 @@ Usage: ``python -m computd_b200.build [--force] [--verbose]``.
 Each ``csrc/*.cu`` is compiled with nvcc for ``sm_100a`` only (tcgen05/TMA
 need the architecture-specific target) into ``computd_b200/_build/`` and
 linked with a static CUDA runtime, so the library does not depend on the
-runtime version torch ships.  Objects are rebuilt when a source or header is
+runtime version torch ships.  ``csrc/host/serving.cpp``, the Python side of the
+serving calls, becomes the extension module ``computd_b200/_serving.so`` (host
+compiler, torch's headers).  Objects are rebuilt when a source or header is
 newer than them.
 """
 from __future__ import annotations
@@ -23,6 +25,8 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libdwa_b200.so"
+HOST_SOURCE = CSRC / "host" / "serving.cpp"
+HOST_PATH = PKG_DIR / "_serving.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -75,8 +79,38 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool, extra: list[str]) -
         raise RuntimeError(f"nvcc failed on {src.name}")
 
 
+def _build_host(verbose: bool) -> None:
+    """The extension module of the serving calls, against the installed torch and Python."""
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda_inc = Path(nvcc_path()).resolve().parent.parent / "include"
+    cxx = shutil.which("c++") or shutil.which("g++")
+    if not cxx:
+        raise RuntimeError("a C++ compiler is required to build computd_b200/_serving.so")
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    lib = torch_dir / "lib"
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE_DIR}",
+           *(f"-isystem{p}" for p in (torch_dir / "include",
+                                      torch_dir / "include/torch/csrc/api/include", cuda_inc,
+                                      sysconfig.get_paths()["include"])),
+           str(HOST_SOURCE), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on {HOST_SOURCE.name}")
+    os.replace(tmp, HOST_PATH)
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compile and link the library; returns its path."""
+    """Compile and link the library and the serving extension; returns the library's path."""
     nvcc = nvcc_path()
     extra = list(extra_flags or [])
     BUILD_DIR.mkdir(exist_ok=True)
@@ -88,9 +122,12 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         objs.append(obj)
         if force or _stale(obj, [src, *headers, Path(__file__)]):
             jobs.append((src, obj))
-    if jobs:
-        with cf.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
+    host = force or _stale(HOST_PATH, [HOST_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__)])
+    if jobs or host:
+        with cf.ThreadPoolExecutor(max_workers=min(len(jobs) + 1, os.cpu_count() or 4)) as ex:
             futs = [ex.submit(_compile, nvcc, s, o, verbose, extra) for s, o in jobs]
+            if host:
+                futs.append(ex.submit(_build_host, verbose))
             for f in futs:
                 f.result()
     if force or jobs or _stale(LIB_PATH, objs):

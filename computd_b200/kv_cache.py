@@ -16,114 +16,42 @@ float8_e4m3fn with f32 scales [n_pages, H_kv, page_size]); pages may be strided,
 what is inside a page is contiguous.  Slot s is token s % page_size of page
 s // page_size.  Every call is asynchronous on the current stream, allocates
 nothing but its outputs, never waits for the device and can be captured in a
-CUDA graph.  Values that only the device sees (slots, page numbers, lengths) are
+CUDA graph; none has gradients.  Values that only the device sees (slots, page numbers, lengths) are
 checked there: a bad one leads to no access but to NaN rows (or a skipped write),
 and to ``DWA_ERR_DEVICE_CHECK`` in ``status``, an int32 device word, when given.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
 
-_BF16, _E4M3, _F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32
-_I32, _I64 = torch.int32, torch.int64
+_BF16, _E4M3, _F32, _I32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
 
 
-# The stream and device numbers without the objects that torch.cuda.current_stream makes: a third
-# of a short call's time on the host.
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_host_module = None
 
 
-_entries: dict[str, object] = {}  # C entry points by name, once looked up
-
-
-def _call(name: str, dev: int, *args) -> None:
-    """One C call on device `dev`'s current stream, with that device current."""
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(_lib.load(), name)
-    if dev == _current_device():
-        st = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, _raw_stream(dev))
-    if st:
-        _lib.check(st, name)
-
-
-def _cache_args(k_cache, v_cache, k_scale, v_scale):
-    """(device number, H_kv, d, pointers, sizes) of a cache as the C ABI takes them.
-
-    The checks here and below compare whole shapes and strides and format a message only
-    when they fail: a decoding step's calls are short."""
-    dev, dtype, shape, stride = k_cache.get_device(), k_cache.dtype, k_cache.shape, k_cache.stride()
-    if dev < 0:
-        raise ValueError("k_cache must live on a CUDA device")
-    if len(shape) != 4:
-        raise ValueError("k_cache must be [n_pages, H_kv, page_size, d]")
-    if (v_cache.dtype is not dtype or v_cache.shape != shape or v_cache.stride() != stride
-            or v_cache.get_device() != dev):
-        raise ValueError("v_cache must be like k_cache (type, shape, strides, device)")
-    n_pages, heads, page, d = shape
-    ld_page = stride[0]
-    if stride[1:] != (page * d, d, 1) or n_pages == 1:
-        ld_page = _strided_page(stride, shape, "a cache's pages must be contiguous inside")
-    if dtype is _E4M3:
-        if k_scale is None or v_scale is None:
-            raise ValueError("a float8_e4m3fn cache needs k_scale and v_scale")
-        sshape, sstride = shape[:3], k_scale.stride()
-        if (k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != sshape
-                or v_scale.shape != sshape or v_scale.stride() != sstride
-                or k_scale.get_device() != dev or v_scale.get_device() != dev):
-            raise ValueError("k_scale and v_scale must be f32 [n_pages, H_kv, page_size] with the same "
-                             "strides on the cache's device")
-        ld_scale = sstride[0]
-        if sstride[1:] != (page, 1) or n_pages == 1:
-            ld_scale = _strided_page(sstride, sshape, "the scales of a page must be contiguous")
-        return dev, heads, d, (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                               v_scale.data_ptr()), (n_pages, page, ld_page, ld_scale)
-    if dtype is not _BF16:
-        raise ValueError("k_cache must be bfloat16 or float8_e4m3fn")
-    if k_scale is not None or v_scale is not None:
-        raise ValueError("a bfloat16 cache has no scales")
-    return dev, heads, d, (k_cache.data_ptr(), v_cache.data_ptr(), None, None), \
-        (n_pages, page, ld_page, 0)
-
-
-def _strided_page(stride, shape, what):
-    """The distance between pages where a dimension of size 1 may have any stride."""
-    dense = 1
-    for size, step in zip(reversed(shape[1:]), reversed(stride[1:])):
-        if size > 1 and step != dense:
-            raise ValueError(what)
-        dense *= size
-    return stride[0] if shape[0] > 1 else dense
-
-
-def _array(x, dtype, shape, dev, name):
-    """A contiguous tensor's pointer."""
-    if (x.dtype is not dtype or x.shape != shape or x.get_device() != dev or not x.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on the same device as the "
-                         f"others (got {x.dtype} {list(x.shape)} on {x.device})")
-    return x.data_ptr()
-
-
-def _status(x, dev):
-    if x.dtype is not _I32 or x.numel() != 1 or x.get_device() != dev:
-        raise ValueError("status must be one int32 on the cache's device")
-    return x.data_ptr()
-
-
-def _rows(x, dtypes, heads, d, dev, name):
-    """(T, strides of a token and a head) of [T, heads, d] rows."""
-    shape, stride = x.shape, x.stride()
-    if (x.dtype not in dtypes or len(shape) != 3 or shape[2] != d or x.get_device() != dev
-            or (heads is not None and shape[1] != heads) or stride[2] != 1):
-        raise ValueError(f"{name} must be [T, {heads or 'H'}, {d}] of {dtypes}, contiguous along d, on the "
-                         f"cache's device (got {x.dtype} {list(shape)}, strides {list(stride)}, on {x.device})")
-    # a dimension of size 1 may have any stride
-    return shape[0], stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else d
+def _host():
+    """The extension module with the checks and the C calls (csrc/host/serving.cpp), bound to the
+    loaded library: checked in Python, a decoding step's calls take the host two to three
+    times as long as the device."""
+    global _host_module
+    if _host_module is None:
+        lib = _lib.load()
+        try:
+            from . import _serving as host
+        except ImportError as e:
+            raise ImportError("computd_b200/_serving.so is missing or does not fit this torch; build it "
+                              "with `python -m computd_b200.build`. There is no fallback implementation."
+                              ) from e
+        host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                    for name in ("dwa_kv_write", "dwa_kv_read", "dwa_paged_attention",
+                                 "dwa_verify_drafts")), _lib.check)
+        _host_module = host
+    return _host_module
 
 
 def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -136,14 +64,7 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     scale = max(amax / 448, 2^-126) and codes e4m3(x / scale).  A vector with a NaN or
     an infinity reads back as NaN.  Slot -1 skips its token; where a slot is named
     twice the later token stays."""
-    dev, heads, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    T, k_tok, k_head = _rows(k, (_BF16, _F32), heads, d, dev, "k")
-    T_v, v_tok, v_head = _rows(v, (k.dtype,), heads, d, dev, "v")
-    if T_v != T:
-        raise ValueError("k and v must have the same number of tokens")
-    _call("dwa_kv_write", dev, k.data_ptr(), v.data_ptr(), 1 if k.dtype is _BF16 else 0, T, heads, d,
-          k_tok, k_head, v_tok, v_head, _array(slots, _I64, (T,), dev, "slots"), *ptrs, *sizes,
-          None if status is None else _status(status, dev))
+    (_host_module or _host()).kv_write(k, v, k_cache, v_cache, slots, k_scale, v_scale, status)
 
 
 def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *,
@@ -154,18 +75,7 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
 
     With ``out`` (two contiguous tensors) the rows of slot -1 stay as they were; without
     it they are zeros."""
-    dev, heads, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    T = slots.shape[0] if slots.dim() == 1 else 0
-    slots_ptr = _array(slots, _I64, (T,), dev, "slots")
-    if out is None:
-        k, v = k_cache.new_empty((2, T, heads, d), dtype=_BF16).unbind(0)
-        k_ptr, v_ptr = k.data_ptr(), v.data_ptr()
-    else:
-        k, v = out
-        k_ptr, v_ptr = (_array(x, _BF16, (T, heads, d), dev, "out") for x in (k, v))
-    _call("dwa_kv_read", dev, *ptrs, slots_ptr, T, heads, d, *sizes, k_ptr, v_ptr,
-          1 if out is None else 0, None if status is None else _status(status, dev))
-    return k, v
+    return (_host_module or _host()).kv_read(k_cache, v_cache, slots, k_scale, v_scale, out, status)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -190,38 +100,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     What a row may not see does not reach it, NaN and infinities included.  (A new
     token's value that is not finite makes the rows that do see it not finite in its
     channel; an infinity may become NaN there.)"""
-    dev, h_kv, d, ptrs, sizes = _cache_args(k_cache, v_cache, k_scale, v_scale)
-    T, q_ld, q_head = _rows(q, (_BF16,), None, d, dev, "q")
-    heads = q.shape[1]
-    table_shape = block_table.shape
-    if (block_table.dtype is not _I32 or len(table_shape) != 2 or block_table.get_device() != dev
-            or (table_shape[1] > 1 and block_table.stride(1) != 1)):
-        raise ValueError("block_table must be int32 [B, max_pages], contiguous along its rows, on the "
-                         "cache's device")
-    B, max_pages = table_shape
-    if q_start is None:
-        start_ptr = None
-        if max_q is None:
-            max_q = T // B if B else 0
-    else:
-        start_ptr = _array(q_start, _I32, (B + 1,), dev, "q_start")
-        if max_q is None:
-            max_q = T
-    if out is None:
-        out = q.new_empty((T, heads, d))
-        out_ld = heads * d
-    else:
-        T_out, out_ld, out_head = _rows(out, (_BF16,), heads, d, dev, "out")
-        if T_out != T or out_head != d:
-            raise ValueError("out must be like q, contiguous over heads and d")
-    if q_head != d:
-        raise ValueError("q must be contiguous over heads and d")
-    _call("dwa_paged_attention", dev, q.data_ptr(), T, heads, d, q_ld or heads * d, *ptrs, h_kv, *sizes,
-          block_table.data_ptr(), block_table.stride(0) if B > 1 else max_pages, max_pages,
-          _array(lengths, _I32, (B,), dev, "lengths"), start_ptr, B, max_q,
-          d ** -0.5 if scale is None else scale, out.data_ptr(), out_ld or heads * d,
-          None if status is None else _status(status, dev))
-    return out
+    return (_host_module or _host()).attend(q, k_cache, v_cache, block_table, lengths, q_start, max_q,
+                                            k_scale, v_scale, scale, out, status)
 
 
 class PagedKVCache:
@@ -317,20 +197,5 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor,
 
     Returns (n_accepted int32 [B], tokens int32 [B, K + 1]: the standing drafts, the drawn
     token, then -1)."""
-    dev, dtype, shape = target_probs.get_device(), target_probs.dtype, target_probs.shape
-    if dev < 0:
-        raise ValueError("target_probs must live on a CUDA device")
-    if dtype not in (_F32, _BF16) or len(shape) != 3 or shape[1] < 1 or not target_probs.is_contiguous():
-        raise ValueError("target_probs must be a contiguous float32 or bfloat16 [B, K + 1, V]")
-    B, K1, V = shape
-    K = K1 - 1
-    accepted = draft_tokens.new_empty((B,), dtype=_I32)
-    tokens = draft_tokens.new_empty((B, K1), dtype=_I32)
-    _call("dwa_verify_drafts", dev, target_probs.data_ptr(),
-          None if draft_probs is None else _array(draft_probs, dtype, (B, K, V), dev, "draft_probs"),
-          1 if dtype is _BF16 else 0, _array(draft_tokens, _I32, (B, K), dev, "draft_tokens"),
-          _array(accept_u, _F32, (B, K), dev, "accept_u"),
-          _array(sample_u, _F32, (B,), dev, "sample_u"),
-          None if draft_lengths is None else _array(draft_lengths, _I32, (B,), dev, "draft_lengths"),
-          B, K, V, accepted.data_ptr(), tokens.data_ptr())
-    return accepted, tokens
+    return (_host_module or _host()).verify(target_probs, draft_tokens, draft_probs, accept_u, sample_u,
+                                            draft_lengths)
