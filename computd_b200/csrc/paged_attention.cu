@@ -94,12 +94,10 @@ struct RowsCfg {
   static constexpr int kBoxBytes = 16 * kRowBytes;
   static constexpr int kBoxes = kSub * kHalves;                   // of K; as many of V
   static constexpr int kStageBytes = 2 * kBoxes * kBoxBytes;
-  static constexpr int kScaleBytes = kE4m3 ? 2 * kSub * 64 : 0;
-  static constexpr int kStages = DP == 128 ? 2 : 3;
+  static constexpr int kStages = kE4m3 || DP == 128 ? 2 : 3;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kPartBytes = kWarps * kRows * DP * 4;      // takes the ring's place
-  static constexpr int kSmem = 1024 + (kRingBytes > kPartBytes ? kRingBytes : kPartBytes) +
-                               kWarps * kStages * kScaleBytes;
+  static constexpr int kSmem = 1024 + (kRingBytes > kPartBytes ? kRingBytes : kPartBytes);
 };
 
 // Keys of the rows of a 16-key tile: row r of the fragment is key row_key(r & 7) + (r & 8).
@@ -120,18 +118,13 @@ __device__ __forceinline__ uint2 lds8(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ float lds4f(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
-
-__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                              int x, int y, int z, int w) {
+// (channel, token of the page, half of the channels, head, page)
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                              int y, int half, int head, int page) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(half), "r"(head), "r"(page)
       : "memory");
 }
 
@@ -139,7 +132,7 @@ template <bool kE4m3, int DP, int NT, int W>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
-                      const int row_groups, const int cluster) {
+                      const int row_groups, const int cluster, const int wide) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
   constexpr int kWarps = W, kThreads = 32 * W;
   extern __shared__ uint8_t smem_raw[];
@@ -153,12 +146,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  int64_t unit = blockIdx.x / cluster;
+  uint32_t unit = blockIdx.x / cluster;  // the grid has 32 bits
   const int split = static_cast<int>(blockIdx.x % cluster);
   const int rg = static_cast<int>(unit % row_groups);
   unit /= row_groups;
   const int hk = static_cast<int>(unit % a.H_kv);
-  const int b = static_cast<int>(unit / a.H_kv);
+  // the longest sequences first
+  __shared__ int costs[kMostRanked], found;
+  int b = static_cast<int>(unit / a.H_kv);
+  if (a.B > 1 && a.B <= kMostRanked)
+    b = ranked(a.B, b, costs, &found, [&](int i) { return __ldg(a.lengths + i); });
 
   PagedSeq seq = paged_seq(a, b);
   if (seq.bad && hk == 0 && rg == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
@@ -179,13 +176,36 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     return;
   }
   const int rows = static_cast<int>(min(all_rows - r0, static_cast<int64_t>(C::kRows)));
-  const int vis_min = paged_visible(seq, static_cast<int>(r0 / a.group));
-  const int vis_max = paged_visible(seq, static_cast<int>((r0 + rows - 1) / a.group));
+  const uint32_t row0 = static_cast<uint32_t>(r0);  // below 2^31: max_q bounds it
+  const int vis_min = paged_visible(seq, row_token(row0, a.group));
+  const int vis_max = paged_visible(seq, row_token(row0 + rows - 1, a.group));
+
+  // ------------------------------------------------ Q^T fragments, on their way
+  // lane (g, t) holds row 8 nt + g at the channels its key chunks have
+  constexpr int kChunk = kE4m3 ? 16 : 8;            // channels per 16 bytes
+  constexpr int kChunksK = DP / (4 * kChunk);       // of a key row, per lane
+  uint32_t qf[NT][C::kSteps][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = 8 * nt + g;
+    const uint32_t row = row0 + r, token = row_token(row, a.group);
+    const uint16_t* src = a.q + (seq.row0 + token) * a.q_ld +
+                          (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d;
+#pragma unroll
+    for (int c = 0; c < kChunksK; ++c)
+#pragma unroll
+      for (int i = 0; i < kChunk / 8; ++i) {
+        const int at = (4 * c + t) * kChunk + 8 * i;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && at < a.d) x = __ldg(reinterpret_cast<const uint4*>(src + at));
+        const int k = (c * kChunk + 8 * i) / 4;
+        qf[nt][k][0] = x.x; qf[nt][k][1] = x.y;
+        qf[nt][k + 1][0] = x.z; qf[nt][k + 1][1] = x.w;
+      }
+  }
 
   // ------------------------------------------------ this warp's ring
   const uint32_t ring = base + warp * C::kStages * C::kStageBytes;
-  const uint32_t scale_ring =
-      base + C::kSmem - 1024 - (kWarps - warp) * C::kStages * C::kScaleBytes;
   const uint32_t bar0 = smem_u32(&full_bar[warp][0]);
   if (lane == 0) {
     for (int i = 0; i < C::kStages; ++i) mbar_init(bar0 + 8 * i, 1);
@@ -199,81 +219,87 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   const int page_mask = (1 << a.page_log2) - 1;
   const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
   bool bad_page = false;
-  // Lane i < 2 kBoxes brings one box of K or V; for e4m3 lanes 4 to 7 the tiles' scales.
-  const int what = kE4m3 ? (lane >> 1) & 1 : lane / C::kHalves;  // 0: K, 1: V
-  const int sub = kE4m3 ? lane & 1 : 0, half = kE4m3 ? 0 : lane % C::kHalves;
-  const bool brings = kE4m3 ? lane < 8 : lane < 2 * C::kHalves;
-  // the page of this lane's tile of a block, looked up one block ahead of its use
-  auto look_up = [&](int block) -> int {
+  // The first lane brings a block: a box of 16 keys by 128 bytes for each half of the
+  // channels (or 32 keys, or both halves, as the map has them), K then V.  What a copy costs
+  // is its issue, so they are few and their operands the same in all lanes.  The pages are
+  // looked up a block ahead; an e4m3 block's lane holds one key's scales.
+  auto look_up = [&](int block, int sub) -> int {
     const int key = block * C::kKeys + 16 * sub;
-    return brings && key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
+    return key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
   };
-  auto bring = [&](int block, int stage, int page) {
-    const int key = block * C::kKeys + 16 * sub;
-    const uint32_t bar = bar0 + 8 * stage;
+  auto checked = [&](int page) -> int {  // page 0 in a bad one's place; the rows become NaN
+    if (page >= 0 && page < a.n_pages) return page;
+    bad_page = true;
+    return 0;
+  };
+  auto bring = [&](int block, int stage, int page0, int page1, float* ks, float* vs) {
+    const int key = block * C::kKeys;
+    const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * C::kStageBytes;
+    const bool two = C::kSub == 2 && key + 16 < vis_max;  // the block's second tile exists
+    page0 = checked(page0);
+    if (two) page1 = checked(page1);
     if (lane == 0) {
-      const int tiles = min(C::kSub, (vis_max - block * C::kKeys + 15) >> 4);
-      mbar_arrive_expect_tx(bar, static_cast<uint32_t>(tiles) *
-                                     (2 * C::kHalves * C::kBoxBytes + (kE4m3 ? 128 : 0)));
-    }
-    __syncwarp();
-    if (brings && key < vis_max) {
-      if (page < 0 || page >= a.n_pages) {  // page 0 in its place; the rows become NaN
-        bad_page = true;
-        page = 0;
-      }
-      if (!kE4m3 || lane < 4) {
-        tma_load_rows(ring + stage * C::kStageBytes +
-                          (what * C::kBoxes + (kE4m3 ? sub : half)) * C::kBoxBytes,
-                      what ? &map_v : &map_k, bar, 64 * half, key & page_mask, hk, page);
+      mbar_arrive_expect_tx(bar, (C::kSub == 2 && (two || wide) ? 2u : 1u) * 2 * C::kHalves * C::kBoxBytes);
+      const int y = key & page_mask;
+      if (C::kSub == 2) {
+        tma_load_rows(dst, &map_k, bar, 0, y, 0, hk, page0);
+        tma_load_rows(dst + 2 * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
+        if (two && !wide) {
+          const int y1 = (key + 16) & page_mask;
+          tma_load_rows(dst + C::kBoxBytes, &map_k, bar, 0, y1, 0, hk, page1);
+          tma_load_rows(dst + 3 * C::kBoxBytes, &map_v, bar, 0, y1, 0, hk, page1);
+        }
       } else {
-        bulk_load(scale_ring + stage * C::kScaleBytes + (what * C::kSub + sub) * 64,
-                  (what ? a.v_scale : a.k_scale) + page * a.ld_scale_page +
-                      (static_cast<int64_t>(hk) << a.page_log2) + (key & page_mask),
-                  64, bar);
+        tma_load_rows(dst, &map_k, bar, 0, y, 0, hk, page0);
+        tma_load_rows(dst + C::kHalves * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
+        if (C::kHalves == 2 && !wide) {
+          tma_load_rows(dst + C::kBoxBytes, &map_k, bar, 64, y, 0, hk, page0);
+          tma_load_rows(dst + 3 * C::kBoxBytes, &map_v, bar, 64, y, 0, hk, page0);
+        }
+      }
+    }
+    if constexpr (kE4m3) {
+      *ks = *vs = 0.f;
+      if (key + lane < vis_max) {
+        const int64_t at = (lane < 16 ? page0 : page1) * a.ld_scale_page +
+                           (static_cast<int64_t>(hk) << a.page_log2) + ((key + lane) & page_mask);
+        *ks = __ldg(a.k_scale + at);
+        *vs = __ldg(a.v_scale + at);
       }
     }
   };
   int block = split * kWarps + warp;
+  float ks_ahead[2] = {}, vs_ahead[2] = {};  // e4m3: of the blocks in flight, by stage
+  int next0, next1;
   {
-    int at = block;
-    for (int i = 0; i < C::kStages && at < n_blocks; ++i, at += step) bring(at, i, look_up(at));
+    int pages[C::kStages + 1][2];
+#pragma unroll
+    for (int i = 0; i <= C::kStages; ++i) {
+      pages[i][0] = look_up(min(block + i * step, n_blocks), 0);
+      pages[i][1] = C::kSub == 2 ? look_up(min(block + i * step, n_blocks), 1) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i)
+      if (block + i * step < n_blocks)
+        bring(block + i * step, i, pages[i][0], pages[i][1], &ks_ahead[i & 1], &vs_ahead[i & 1]);
+    next0 = pages[C::kStages][0];
+    next1 = pages[C::kStages][1];
   }
-  int next_page = look_up(min(block + C::kStages * step, n_blocks));
 
-  // ------------------------------------------------ Q^T fragments, visible counts
-  // lane (g, t) holds row 8 nt + g at the channels its key chunks have
-  constexpr int kChunk = kE4m3 ? 16 : 8;            // channels per 16 bytes
-  constexpr int kChunksK = DP / (4 * kChunk);       // of a key row, per lane
-  uint32_t qf[NT][C::kSteps][2];
-  float factor[NT][2];                              // of the columns' scores, to log2 units
+  // ------------------------------------------------ Q's scale, visible counts
+  // columns of this lane: rows 8 nt + 2 t and + 1
+  float factor[NT][2];  // of the columns' scores, to log2 units
   int vis[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = 8 * nt + g;
-    const int64_t row = r0 + r;
-    const uint16_t* src = a.q + (seq.row0 + row / a.group) * a.q_ld +
-                          (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d;
-    uint32_t top = 0;
-#pragma unroll
-    for (int c = 0; c < kChunksK; ++c)
-#pragma unroll
-      for (int i = 0; i < kChunk / 8; ++i) {
-        const int at = (4 * c + t) * kChunk + 8 * i;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && at < a.d) x = __ldg(reinterpret_cast<const uint4*>(src + at));
-        const int k = (c * kChunk + 8 * i) / 4;
-        qf[nt][k][0] = x.x; qf[nt][k][1] = x.y;
-        qf[nt][k + 1][0] = x.z; qf[nt][k + 1][1] = x.w;
-        if (kE4m3) {
-          top = max(top, max((x.x << 16) & 0x7FFF0000u, x.x & 0x7FFF0000u));
-          top = max(top, max((x.y << 16) & 0x7FFF0000u, x.y & 0x7FFF0000u));
-          top = max(top, max((x.z << 16) & 0x7FFF0000u, x.z & 0x7FFF0000u));
-          top = max(top, max((x.w << 16) & 0x7FFF0000u, x.w & 0x7FFF0000u));
-        }
-      }
     float f = a.scale_log2;
     if constexpr (kE4m3) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < C::kSteps; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          top = max(top, max((qf[nt][k][i] << 16) & 0x7FFF0000u, qf[nt][k][i] & 0x7FFF0000u));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       float f0, f1;
@@ -285,12 +311,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
           qf[nt][k][i] = pack_f16(__uint_as_float(qf[nt][k][i] << 16) * f0 * f1,
                                   __uint_as_float(qf[nt][k][i] & 0xFFFF0000u) * f0 * f1);
     }
-    // columns of this lane: rows 8 nt + 2 t and + 1
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       factor[nt][j] = kE4m3 ? __shfl_sync(0xFFFFFFFFu, f, 4 * (2 * t + j)) : f;
       const int rc = 8 * nt + 2 * t + j;
-      vis[nt][j] = rc < rows ? paged_visible(seq, static_cast<int>((r0 + rc) / a.group)) : 0;
+      vis[nt][j] = rc < rows ? paged_visible(seq, row_token(row0 + rc, a.group)) : 0;
     }
   }
 
@@ -313,7 +338,6 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     const int key0 = block * C::kKeys;
     if (!mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr)) { bad_page = true; break; }
     const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kBoxes * C::kBoxBytes;
-    const uint32_t sb = scale_ring + stage * C::kScaleBytes;
     // two sums per score: half the chain of dependent products
     float s[C::kSub][NT][4] = {}, s2[C::kSub][NT][4] = {};
 #pragma unroll
@@ -350,6 +374,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       }
     }
     const bool edge = key0 + C::kKeys > vis_min;
+    const float ks_now = stage ? ks_ahead[1] : ks_ahead[0], vs_now = stage ? vs_ahead[1] : vs_ahead[0];
     float sk[C::kSub][2], sv[C::kSub][2];
     bool v_up = false;
     if constexpr (kE4m3) {
@@ -357,9 +382,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          sk[u][i] = lds4f(sb + u * 64 + 4 * (key_g + 8 * i));
-          sv[u][i] = lds4f(sb + (C::kSub + u) * 64 + 4 * (key_g + 8 * i));
-          if (edge && key0 + 16 * u + 8 * i + key_g >= vis_max) sv[u][i] = 0.f;
+          sk[u][i] = __shfl_sync(0xFFFFFFFFu, ks_now, 16 * u + 8 * i + key_g);
+          sv[u][i] = __shfl_sync(0xFFFFFFFFu, vs_now, 16 * u + 8 * i + key_g);
           v_up = v_up || sv[u][i] > v_ref;
         }
     }
@@ -511,8 +535,14 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     __syncwarp();  // every lane has read the stage
     const int ahead = block + C::kStages * step;
     if (ahead < n_blocks) {
-      bring(ahead, stage, next_page);
-      next_page = look_up(min(ahead + step, n_blocks));
+      float ks = 0.f, vs = 0.f;
+      bring(ahead, stage, next0, next1, &ks, &vs);
+      if constexpr (kE4m3) {
+        if (stage) { ks_ahead[1] = ks; vs_ahead[1] = vs; }
+        else { ks_ahead[0] = ks; vs_ahead[0] = vs; }
+      }
+      next0 = look_up(min(ahead + step, n_blocks), 0);
+      if (C::kSub == 2) next1 = look_up(min(ahead + step, n_blocks), 1);
     }
     if (++stage == C::kStages) { stage = 0; parity ^= 1; }
   }
@@ -605,12 +635,12 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
         y += f * os[c].y;
       }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t row = r0 + r;
-    const int seen = paged_visible(seq, static_cast<int>(row / a.group));
+    const uint32_t row = row0 + r, token = row_token(row, a.group);
+    const int seen = paged_visible(seq, token);
     x = bad0 < seen ? __uint_as_float(0x7FC00000u) : x * inv;
     y = bad1 < seen ? __uint_as_float(0x7FC00000u) : y * inv;
-    *reinterpret_cast<uint32_t*>(a.out + (seq.row0 + row / a.group) * a.out_ld +
-                                 (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + ch) =
+    *reinterpret_cast<uint32_t*>(a.out + (seq.row0 + token) * a.out_ld +
+                                 (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d + ch) =
         pack_bf16(x, y);
   }
   if (cluster > 1) cluster_sync();  // no block leaves while another reads its partial
@@ -620,7 +650,11 @@ template <bool kE4m3, int DP, int NT, int W>
 cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStream_t stream) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
   CUtensorMap mk, mv;
-  if (!make_page_map(&mk, a.k, a, C::kRowBytes, 16) || !make_page_map(&mv, a.v, a, C::kRowBytes, 16))
+  // one box where a page holds a whole e4m3 block, or both halves of full bf16 rows
+  const bool wide = kE4m3 ? a.page_log2 >= 5 : a.d == 128;
+  const int box_rows = kE4m3 && wide ? 32 : 16, box_halves = !kE4m3 && wide ? 2 : 1;
+  if (!make_page_map(&mk, a.k, a, C::kRowBytes, box_rows, box_halves) ||
+      !make_page_map(&mv, a.v, a, C::kRowBytes, box_rows, box_halves))
     return cudaErrorInvalidValue;
   if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
   constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W>;
@@ -637,7 +671,7 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
   const int row_groups = static_cast<int>(units / (static_cast<int64_t>(a.B) * a.H_kv));
-  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, row_groups, cluster);
+  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, row_groups, cluster, wide ? 1 : 0);
 }
 
 // How a call is cut up: the longest context is split over 2^n blocks of 4 warps

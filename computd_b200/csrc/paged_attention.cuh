@@ -67,6 +67,24 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
   return s;
 }
 
+// Blocks start in the order of their number, so the ones with the most keys should
+// have the lowest: the index i < n whose cost(i) has this rank among all (equal costs by
+// index).  Every block finds its own; `costs` and `found` are shared memory.
+constexpr int kMostRanked = 128;  // more units than this even out by themselves
+template <typename F>
+__device__ __forceinline__ int ranked(int n, int rank, int* costs, int* found, F&& cost) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) costs[i] = cost(i);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int own = costs[i];
+    int before = 0;
+    for (int j = 0; j < n; ++j) before += costs[j] > own || (costs[j] == own && j < i);
+    if (before == rank) *found = i;
+  }
+  __syncthreads();
+  return *found;
+}
+
 // Tokens that new token i may see.
 __device__ __forceinline__ int paged_visible(const PagedSeq& s, int i) {
   return max(s.length - s.n + i + 1, 0);
@@ -166,9 +184,11 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(const float* local, int rank)
   return v;
 }
 
-// Tensor map of one of the caches: boxes of `row_bytes` by `box_rows` tokens of one page's
-// head, 128-byte rows swizzled.  Channels beyond d arrive as zeros.
-bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows);
+// Tensor map of one of the caches, (channel, token of the page, half of the channels, head,
+// page): boxes of `row_bytes` by `box_rows` tokens of one page's head, 128-byte rows
+// swizzled.  Channels beyond d arrive as zeros; two halves (64 bf16 each) only for d = 128.
+bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows,
+                   int box_halves);
 
 // Lets a kernel have its dynamic shared memory (and clusters of 16), once per device.
 template <auto kKernel>

@@ -55,18 +55,21 @@ namespace dwa {
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
-bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows) {
+bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows,
+                   int box_halves) {
   auto encode = tensor_map_encoder();
   if (!encode) return false;
   const bool e4m3 = a.k_scale != nullptr;
   const uint64_t es = e4m3 ? 1 : 2;
   const uint64_t page = 1ull << a.page_log2;
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.d), page, static_cast<cuuint64_t>(a.H_kv),
-                        static_cast<cuuint64_t>(a.n_pages)};
-  cuuint64_t strides[3] = {a.d * es, page * a.d * es, a.ld_page * es};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(row_bytes / es), static_cast<cuuint32_t>(box_rows), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  return encode(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  const cuuint64_t halves = static_cast<cuuint64_t>(box_halves);
+  cuuint64_t dims[5] = {static_cast<cuuint64_t>(a.d) / halves, page, halves,
+                        static_cast<cuuint64_t>(a.H_kv), static_cast<cuuint64_t>(a.n_pages)};
+  cuuint64_t strides[4] = {a.d * es, a.d * es / halves, page * a.d * es, a.ld_page * es};
+  cuuint32_t box[5] = {static_cast<cuuint32_t>(row_bytes / es), static_cast<cuuint32_t>(box_rows),
+                       static_cast<cuuint32_t>(box_halves), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return encode(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                 const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -264,12 +267,13 @@ __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                            int y, int z, int w) {
+// (channel, token of the page, half of the channels, head, page)
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                            int y, int half, int head, int page) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(half), "r"(head), "r"(page)
       : "memory");
 }
 
@@ -321,12 +325,21 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ------------------------------------------------ the block's work
-  const uint32_t heads = static_cast<uint32_t>(a.B) * a.H_kv;  // the grid has 32 bits
   const int split = static_cast<int>(blockIdx.x % cluster);
-  const uint32_t unit = blockIdx.x / cluster;
-  // late rows (more keys) first
-  const int ru = row_units - 1 - static_cast<int>(unit / heads);
-  const int b = static_cast<int>(unit % heads / a.H_kv), hk = static_cast<int>(unit % heads % a.H_kv);
+  const uint32_t unit = blockIdx.x / cluster;  // the grid has 32 bits
+  // the units with the most keys first; where they are too many to rank, late rows first
+  int* const costs = reinterpret_cast<int*>(smem);  // operands come later
+  const int hk = static_cast<int>(unit % a.H_kv);
+  int pair_of = static_cast<int>(unit / a.H_kv);  // (row unit, sequence)
+  const int pairs = a.B * row_units;
+  if (pairs > 1 && pairs <= kMostRanked)
+    pair_of = ranked(pairs, pair_of, costs, costs + kMostRanked, [&](int i) {
+      const PagedSeq s = paged_seq(a, i % a.B);
+      const int64_t first = static_cast<int64_t>(row_units - 1 - i / a.B) * 2 * kTile;
+      const int64_t end = min(first + 2 * kTile, static_cast<int64_t>(s.n) * a.group);
+      return first < end ? paged_visible(s, static_cast<int>((end - 1) / a.group)) : -1;
+    });
+  const int ru = row_units - 1 - pair_of / a.B, b = pair_of % a.B;
   const PagedSeq seq = paged_seq(a, b);
   if (seq.bad && hk == 0 && ru == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
   const int64_t all_rows = static_cast<int64_t>(seq.n) * a.group;
@@ -430,11 +443,11 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
           const uint32_t dst = s_stage + st * C::kStageBytes;
           if constexpr (kE4m3) {
-            tma_load_4d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, hk, page);
+            tma_load_5d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, 0, hk, page);
           } else {
 #pragma unroll
             for (int h = 0; h < C::kHalves; ++h)
-              tma_load_4d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, hk,
+              tma_load_5d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, 0, hk,
                           page);
           }
         }
@@ -1020,8 +1033,8 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   using C = MmaCfg<kE4m3, DP>;
   CUtensorMap mk, mv;
   const int row_bytes = kE4m3 ? DP : 128, box_rows = 1 << a.page_log2;
-  if (!make_page_map(&mk, a.k, a, row_bytes, box_rows) ||
-      !make_page_map(&mv, a.v, a, row_bytes, box_rows))
+  if (!make_page_map(&mk, a.k, a, row_bytes, box_rows, 1) ||
+      !make_page_map(&mv, a.v, a, row_bytes, box_rows, 1))
     return cudaErrorInvalidValue;
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_units = static_cast<int>((most_rows + 2 * kTile - 1) / (2 * kTile));
