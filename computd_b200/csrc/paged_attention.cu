@@ -14,8 +14,9 @@
 // accumulator is known).  P^T is turned between the products by movmatrix.
 //
 // Each warp works alone on blocks of 16 (bf16) or 32 (e4m3) keys, which its own
-// ring of TMA copies brings, 8 KB at a time and three in flight (registers could
-// hold one: 137 us instead of XX us for 64 ragged sequences of 16 x 128, bf16).
+// ring of TMA copies brings, 8 KB at a time and two in flight, three blocks of four warps
+// to an SM.  (Loaded into registers, one block ahead: 137 us instead of 83 for 64 ragged
+// sequences of 16 heads of 128, bf16, 0.52 GB: 6.2 TB/s.)
 // The context of one (sequence, head) is split over the warps of a cluster of
 // blocks, block by block in turn, and joined through shared and distributed shared
 // memory in one launch, in a fixed order.
@@ -38,7 +39,7 @@ namespace dwa {
 
 namespace {
 
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 8;
 // Rows per key/value head that this kernel takes; more go to the tcgen05 kernel.  At 20
 // rows (16 sequences of 4096, 8 heads of 128, bf16) that one takes 81 us, this one 165.
 constexpr int kFewRows = 16;
@@ -658,7 +659,7 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
     return cudaErrorInvalidValue;
   if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
   constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W>;
-  if (cudaError_t e = allow_smem_once<kKernel>(C::kSmem, true); e != cudaSuccess) return e;
+  if (cudaError_t e = allow_smem_once<kKernel>(C::kSmem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
   cfg.blockDim = dim3(C::kThreads);
@@ -675,10 +676,14 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
 }
 
 // How a call is cut up: the longest context is split over 2^n blocks of 4 warps
-// until there are 6 blocks for every SM (3 reside) or a warp is left with fewer
+// until there are 3 blocks for every SM (as many reside) or a warp is left with fewer
 // than 8 steps, whose pipeline then hardly fills; below 2 blocks per SM it is split
-// down to 2 steps all the same.  What still leaves SMs without a block gets 8 warps
-// per block.  (Step: 32 keys of an e4m3 cache, 16 of a bf16 one.)
+// down to 2 steps all the same.  (32 sequences up to 16384 tokens, 8 heads, e4m3: one
+// block each 212 us, 2 126, 4 132, 8 156; 64 up to 2048, 16 heads, bf16: 83, 97, 128.)
+// What still leaves half the SMs without a block gets 8 warps per block (one sequence of
+// 30000, 8 heads, 8 blocks each: 78 us with 4 warps, 46 with 8), not more: a block of 8
+// fills an SM, and clusters of them do not fit side by side.  (Step: 32 keys of an e4m3
+// cache, 16 of a bf16 one.)
 template <bool kE4m3, int DP, int NT>
 cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stream) {
   const int64_t sms = device_sm_count();
@@ -686,10 +691,10 @@ cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stre
   int cluster = 1;
   while (cluster < kMaxCluster) {
     const int64_t blocks = units * cluster, per_warp = steps / (4 * 2 * cluster);
-    if (!(blocks < 2 * sms ? per_warp >= 2 : blocks < 6 * sms && per_warp >= 8)) break;
+    if (!(blocks < 2 * sms ? per_warp >= 2 : blocks < 3 * sms && per_warp >= 8)) break;
     cluster *= 2;
   }
-  return units * cluster <= sms && steps >= 16 * cluster
+  return units * cluster <= sms / 2 && steps >= 8 * cluster
              ? launch_rows<kE4m3, DP, NT, 8>(a, units, cluster, stream)
              : launch_rows<kE4m3, DP, NT, 4>(a, units, cluster, stream);
 }

@@ -190,16 +190,14 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(const float* local, int rank)
 bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows,
                    int box_halves);
 
-// Lets a kernel have its dynamic shared memory (and clusters of 16), once per device.
+// Lets a kernel have its dynamic shared memory, once per device.
 template <auto kKernel>
-cudaError_t allow_smem_once(int bytes, bool wide_clusters = false) {
+cudaError_t allow_smem_once(int bytes) {
   static std::atomic<bool> done[64] = {};
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
   if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
   cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && wide_clusters)
-    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
   return e;
 }
