@@ -99,6 +99,7 @@ struct RowsCfg {
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kPartBytes = kWarps * kRows * DP * 4;      // takes the ring's place
   static constexpr int kSmem = 1024 + (kRingBytes > kPartBytes ? kRingBytes : kPartBytes);
+  static constexpr int kScales = kE4m3 ? 32 : 1;  // keys with a scale per block
 };
 
 // Keys of the rows of a 16-key tile: row r of the fragment is key row_key(r & 7) + (r & 8).
@@ -119,6 +120,14 @@ __device__ __forceinline__ uint2 lds8(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// This thread's arrival on `bar`, once its cp.async copies so far have landed.
+__device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // (channel, token of the page, half of the channels, head, page)
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
                                               int y, int half, int head, int page) {
@@ -138,6 +147,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   constexpr int kWarps = W, kThreads = 32 * W;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[kWarps][C::kStages];
+  __shared__ float scales[kWarps][C::kStages][2][C::kScales];  // keys', values'
   __shared__ float part_m[kWarps][C::kRows], part_l[kWarps][C::kRows];
   __shared__ float block_m[C::kRows], block_l[C::kRows];
   __shared__ int first_bad[DP];  // least key with a value that is not finite, by channel
@@ -209,7 +219,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   const uint32_t ring = base + warp * C::kStages * C::kStageBytes;
   const uint32_t bar0 = smem_u32(&full_bar[warp][0]);
   if (lane == 0) {
-    for (int i = 0; i < C::kStages; ++i) mbar_init(bar0 + 8 * i, 1);
+    for (int i = 0; i < C::kStages; ++i) mbar_init(bar0 + 8 * i, kE4m3 ? 33 : 1);  // with every lane's scales
     fence_mbar_init();
   }
   for (int i = threadIdx.x; i < DP; i += kThreads) first_bad[i] = 0x7FFFFFFF;
@@ -223,7 +233,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   // The first lane brings a block: a box of 16 keys by 128 bytes for each half of the
   // channels (or 32 keys, or both halves, as the map has them), K then V.  What a copy costs
   // is its issue, so they are few and their operands the same in all lanes.  The pages are
-  // looked up a block ahead; an e4m3 block's lane holds one key's scales.
+  // looked up a block ahead.  An e4m3 block's lane brings one key's scales by cp.async:
+  // loads into registers were waited for at the end of the step.
   auto look_up = [&](int block, int sub) -> int {
     const int key = block * C::kKeys + 16 * sub;
     return key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
@@ -233,7 +244,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     bad_page = true;
     return 0;
   };
-  auto bring = [&](int block, int stage, int page0, int page1, float* ks, float* vs) {
+  auto bring = [&](int block, int stage, int page0, int page1) {
     const int key = block * C::kKeys;
     const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * C::kStageBytes;
     const bool two = C::kSub == 2 && key + 16 < vis_max;  // the block's second tile exists
@@ -260,17 +271,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       }
     }
     if constexpr (kE4m3) {
-      *ks = *vs = 0.f;
       if (key + lane < vis_max) {
         const int64_t at = (lane < 16 ? page0 : page1) * a.ld_scale_page +
                            (static_cast<int64_t>(hk) << a.page_log2) + ((key + lane) & page_mask);
-        *ks = __ldg(a.k_scale + at);
-        *vs = __ldg(a.v_scale + at);
+        copy_async4(smem_u32(&scales[warp][stage][0][lane]), a.k_scale + at);
+        copy_async4(smem_u32(&scales[warp][stage][1][lane]), a.v_scale + at);
       }
+      arrive_when_copied(bar);
     }
   };
   int block = split * kWarps + warp;
-  float ks_ahead[2] = {}, vs_ahead[2] = {};  // e4m3: of the blocks in flight, by stage
   int next0, next1;
   {
     int pages[C::kStages + 1][2];
@@ -282,7 +292,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
 #pragma unroll
     for (int i = 0; i < C::kStages; ++i)
       if (block + i * step < n_blocks)
-        bring(block + i * step, i, pages[i][0], pages[i][1], &ks_ahead[i & 1], &vs_ahead[i & 1]);
+        bring(block + i * step, i, pages[i][0], pages[i][1]);
     next0 = pages[C::kStages][0];
     next1 = pages[C::kStages][1];
   }
@@ -375,7 +385,6 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       }
     }
     const bool edge = key0 + C::kKeys > vis_min;
-    const float ks_now = stage ? ks_ahead[1] : ks_ahead[0], vs_now = stage ? vs_ahead[1] : vs_ahead[0];
     float sk[C::kSub][2], sv[C::kSub][2];
     bool v_up = false;
     if constexpr (kE4m3) {
@@ -383,8 +392,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       for (int u = 0; u < C::kSub; ++u)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          sk[u][i] = __shfl_sync(0xFFFFFFFFu, ks_now, 16 * u + 8 * i + key_g);
-          sv[u][i] = __shfl_sync(0xFFFFFFFFu, vs_now, 16 * u + 8 * i + key_g);
+          sk[u][i] = scales[warp][stage][0][16 * u + 8 * i + key_g];
+          sv[u][i] = scales[warp][stage][1][16 * u + 8 * i + key_g];
+          if (edge && key0 + 16 * u + 8 * i + key_g >= vis_max) sv[u][i] = 0.f;
           v_up = v_up || sv[u][i] > v_ref;
         }
     }
@@ -536,12 +546,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     __syncwarp();  // every lane has read the stage
     const int ahead = block + C::kStages * step;
     if (ahead < n_blocks) {
-      float ks = 0.f, vs = 0.f;
-      bring(ahead, stage, next0, next1, &ks, &vs);
-      if constexpr (kE4m3) {
-        if (stage) { ks_ahead[1] = ks; vs_ahead[1] = vs; }
-        else { ks_ahead[0] = ks; vs_ahead[0] = vs; }
-      }
+      bring(ahead, stage, next0, next1);
       next0 = look_up(min(ahead + step, n_blocks), 0);
       if (C::kSub == 2) next1 = look_up(min(ahead + step, n_blocks), 1);
     }
