@@ -232,19 +232,24 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   bool bad_page = false;
   // The first lane brings a block: a box of 16 keys by 128 bytes for each half of the
   // channels (or 32 keys, or both halves, as the map has them), K then V.  What a copy costs
-  // is its issue, so they are few and their operands the same in all lanes.  The pages are
-  // looked up a block ahead.  An e4m3 block's lane brings one key's scales by cp.async:
+  // is its issue, so they are few and their operands the same in all lanes.  An e4m3 block's lane brings one key's scales by cp.async:
   // loads into registers were waited for at the end of the step.
-  auto look_up = [&](int block, int sub) -> int {
-    const int key = block * C::kKeys + 16 * sub;
-    return key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
+  int held0 = 0, held1 = 0, brought = 0;
+  auto hold = [&](int block) {  // the pages of this warp's next 32 blocks, a block to a lane
+    const int64_t key = (block + static_cast<int64_t>(lane) * step) * C::kKeys;
+    held0 = key < vis_max ? __ldg(table + (key >> a.page_log2)) : 0;
+    held1 = C::kSub == 2 && key + 16 < vis_max ? __ldg(table + ((key + 16) >> a.page_log2)) : 0;
   };
   auto checked = [&](int page) -> int {  // page 0 in a bad one's place; the rows become NaN
     if (page >= 0 && page < a.n_pages) return page;
     bad_page = true;
     return 0;
   };
-  auto bring = [&](int block, int stage, int page0, int page1) {
+  auto bring = [&](int block, int stage) {
+    if (brought % 32 == 0) hold(block);
+    int page0 = __shfl_sync(0xFFFFFFFFu, held0, brought % 32);
+    int page1 = C::kSub == 2 ? __shfl_sync(0xFFFFFFFFu, held1, brought % 32) : 0;
+    ++brought;
     const int key = block * C::kKeys;
     const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * C::kStageBytes;
     const bool two = C::kSub == 2 && key + 16 < vis_max;  // the block's second tile exists
@@ -281,21 +286,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     }
   };
   int block = split * kWarps + warp;
-  int next0, next1;
-  {
-    int pages[C::kStages + 1][2];
 #pragma unroll
-    for (int i = 0; i <= C::kStages; ++i) {
-      pages[i][0] = look_up(min(block + i * step, n_blocks), 0);
-      pages[i][1] = C::kSub == 2 ? look_up(min(block + i * step, n_blocks), 1) : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < C::kStages; ++i)
-      if (block + i * step < n_blocks)
-        bring(block + i * step, i, pages[i][0], pages[i][1]);
-    next0 = pages[C::kStages][0];
-    next1 = pages[C::kStages][1];
-  }
+  for (int i = 0; i < C::kStages; ++i)
+    if (block + i * step < n_blocks) bring(block + i * step, i);
 
   // ------------------------------------------------ Q's scale, visible counts
   // columns of this lane: rows 8 nt + 2 t and + 1
@@ -545,11 +538,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       }
     __syncwarp();  // every lane has read the stage
     const int ahead = block + C::kStages * step;
-    if (ahead < n_blocks) {
-      bring(ahead, stage, next0, next1);
-      next0 = look_up(min(ahead + step, n_blocks), 0);
-      if (C::kSub == 2) next1 = look_up(min(ahead + step, n_blocks), 1);
-    }
+    if (ahead < n_blocks) bring(ahead, stage);
     if (++stage == C::kStages) { stage = 0; parity ^= 1; }
   }
   if (__any_sync(0xFFFFFFFFu, bad_page)) {
