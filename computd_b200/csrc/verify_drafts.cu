@@ -52,7 +52,10 @@ __device__ __forceinline__ float prob(const T* p) {
 }
 
 // Not a positive finite number: nothing.
-__device__ __forceinline__ float mass(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+__device__ __forceinline__ float mass(float x) {
+  x = fmaxf(x, 0.f);  // NaN too
+  return x < INFINITY ? x : 0.f;
+}
 
 // Entries i .. i + 3 of a row, zeros from V on.
 template <typename T>
@@ -78,8 +81,9 @@ __device__ __forceinline__ void weights4(const float (&p)[4], const float (&q)[4
                                          double (&w)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double x = static_cast<double>(mass(p[j])) - static_cast<double>(mass(q[j]));
-    w[j] = x > 0.0 && j != one ? x : 0.0;
+    const float x = mass(p[j]), y = mass(q[j]);  // compared in f32: the 64-bit units are few
+    const double d = static_cast<double>(x) - static_cast<double>(y);
+    w[j] = x > y && j != one ? d : 0.0;
   }
 }
 
