@@ -989,8 +989,8 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
   if (H % H_kv != 0)
     return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: H=%d must be a multiple of H_kv=%d", fn, H, H_kv);
   if (T > INT32_MAX || static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX ||
-      static_cast<int64_t>(max_pages) * page_size > INT32_MAX)
-    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows or tokens", fn);
+      static_cast<int64_t>(max_pages) * page_size > (1 << 30))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, or over 2^30 tokens per sequence", fn);
   if (!(scale >= 0.f) || std::isinf(scale))
     return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite and not negative", fn);
   if (T == 0 || B == 0) return ok();

@@ -21,8 +21,8 @@ namespace {
 constexpr int kWriteThreads = 256;
 constexpr int kWriteBlocks = 4;    // per SM, from bf16 and from f32
 constexpr int kWriteBlocksF32 = 2;
-constexpr int kGroupTokens = 64;   // tokens of a block checked for repeated slots at a time
-constexpr int kFilterBits = 1024;  // their slots' low bits
+constexpr int kGroupTokens = 256;  // tokens of a block checked for repeated slots at a time
+constexpr int kFilterBits = 8192;  // their slots' low bits
 
 __device__ __forceinline__ void report(int32_t* status) {
   if (status != nullptr) atomicCAS(status, 0, DWA_ERR_DEVICE_CHECK);

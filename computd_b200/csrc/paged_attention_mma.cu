@@ -15,15 +15,17 @@
 // free for the other tile's product while it works, and the next S is there when it
 // is done: the threads never wait for a product, only the tensor pipe for P.  (With
 // an S per tile that P overwrote, each step was a chain of product, exponentials,
-// product: 2.9 us per 2 x 128 rows x 128 keys of 128 channels instead of XXX.)
-// P is handed over in halves of 64 keys.
+// product: 2.9 us per 2 x 128 rows x 128 keys of 128 channels instead of 2.2.)
 //
 // Per step the products take 2048 cycles of the tensor pipe (8192 FLOP a cycle), the
-// exponentials 32768 / 16 = 2048 of the special-function units.  A quarter of them
-// is therefore computed as a polynomial, and everything else in pairs (f32x2).  m
-// only moves when a row's maximum grew by more than 2^kSlack (the result does not
-// depend on m; P stays below 2^kSlack), so O is hardly ever rescaled, and then by
-// the row's own thread.
+// exponentials 32768 / 16 = 2048 of the special-function units, and everything else
+// about as much of the other units' time, which is what bounds it: measured 2900 cycles
+// a step, 1.05 to 1.09 PFLOP/s (4736 rows over 16384 keys, 32 heads of 128, bf16: 996 us;
+// e4m3 1171 us, the conversion sharing the issue slots).  A polynomial for a part of the
+// exponentials made it slower (1065 us with a quarter, 1031 with none then).  What can be
+// is done in pairs (f32x2) and triples (max).  m only moves when a row's maximum grew by
+// more than 2^kSlack (the result does not depend on m; P stays below 2^kSlack), so O is
+// hardly ever rescaled, and then by the row's own thread.
 //
 // Warps 0-3 and 4-7: the rows of tile 0 and 1.  Warp 8: issues every tcgen05.mma.
 // Warp 9: TMA, straight from the pages into the swizzled operand tiles.  bf16
@@ -32,7 +34,7 @@
 // 12-15 turn codes into fp16 operand tiles (code times scale, over a power of two above
 // the tile's scales, rounded to 2^-11), and Q is scaled per row by a power of two into
 // fp16, exactly.  (With the keys' scales multiplied into the scores instead, every
-// row's thread read 128 of them per step: 1499 us instead of XXX for 4736 rows over
+// row's thread read 128 of them per step: 1499 us instead of 1333 for 4736 rows over
 // 16384 keys, 32 heads.)
 //
 // Where there are few units of 256 rows, a cluster of blocks shares the keys of one

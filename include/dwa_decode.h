@@ -12,7 +12,9 @@
  * Pages may lie ld_page elements (scales: ld_scale_page) apart; everything
  * inside a page is contiguous.  Slot s is token s % page_size of page
  * s / page_size.  page_size is 16, 32, 64 or 128; d is a multiple of 16 in
- * [16, 128].  NULL scales mean a bf16 cache.
+ * [16, 128].  NULL scales mean a bf16 cache.  Pages and their scales are 16-byte
+ * aligned (ld_page a multiple of d, ld_scale_page of 4).  Codes are numbers
+ * (dwa_kv_write makes no NaN code: what it cannot store has a NaN scale).
  *
  * What only the device can see is checked there: a bad slot, page number,
  * length or row range never leads to an access; it writes DWA_ERR_DEVICE_CHECK
@@ -68,9 +70,10 @@ DWA_API dwa_status dwa_kv_read(const void* k_cache, const void* v_cache, const f
  * with the key and value head h / (H / H_kv); no key, or no score above -inf,
  * gives zeros.  q, out bf16 [T][H][d] with row strides q_ld / out_ld (elements;
  * heads contiguous).  Rows from q_start[B] on are left as they were.  max_q
- * bounds every sequence's new tokens.  Keys that a row may not see do not
- * reach it, whatever their bits.  A new token's value that is not finite makes
- * the rows that do see it not finite in its channel (an infinity may become NaN).
+ * bounds every sequence's new tokens; a sequence may have 2^30 tokens.  Keys that
+ * a row may not see do not reach it, whatever their bits.  A new token's value that
+ * is not finite makes the rows that do see it not finite in its channel (an infinity
+ * may become NaN).
  */
 DWA_API dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
                                        const void* k_cache, const void* v_cache,

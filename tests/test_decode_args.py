@@ -25,6 +25,44 @@ def test_python_calls_refuse_host_tensors():
                       torch.zeros(1, 1, 8), torch.zeros(1, 1), torch.zeros(1))
 
 
+def test_python_calls_refuse_other_objects_and_gradients():
+    c = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        kv_cache_read([1], c, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="grad"):
+        kv_cache_read(c.clone().requires_grad_(), c, torch.zeros(3, dtype=torch.int64))
+
+
+def test_paged_kv_cache_refuses_bad_sizes():
+    from computd_b200 import PagedKVCache
+
+    good = dict(n_layers=1, n_pages=4, page_size=16, n_kv_heads=2, head_dim=64)
+    cache = PagedKVCache(**good, dtype=torch.float8_e4m3fn)
+    assert cache.k.shape == (1, 4, 2, 16, 64) and cache.k_scale.shape == (1, 4, 2, 16)
+    for kw in (dict(page_size=24), dict(head_dim=72), dict(head_dim=256), dict(n_pages=0),
+               dict(dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            PagedKVCache(**{**good, **kw})
+    with pytest.raises(ValueError):
+        cache.read(1, torch.zeros(1, dtype=torch.int64))
+
+
+def test_slots_of_packed_chunks():
+    from computd_b200 import PagedKVCache
+
+    cache = PagedKVCache(1, 9, 16, 1, 16)
+    table = torch.tensor([[3, 5], [8, 0], [1, 2]], dtype=torch.int32)
+    lengths = torch.tensor([18, 3, 40], dtype=torch.int32)  # the last does not fit its pages
+    start = torch.tensor([0, 3, 3, 8], dtype=torch.int32)
+    slots, positions = cache.slots(table, lengths, start, 10)
+    assert positions[:3].tolist() == [15, 16, 17]
+    assert slots.tolist() == [3 * 16 + 15, 5 * 16, 5 * 16 + 1] + [-1] * 5 + [-1, -1]
+    # more new tokens than the length has: the first have no place
+    slots, _ = cache.slots(table, torch.tensor([2, 0, 0], dtype=torch.int32),
+                           torch.tensor([0, 4, 4, 4], dtype=torch.int32), 4)
+    assert slots.tolist() == [-1, -1, 48, 49]
+
+
 def cache(**kw):
     a = dict(k_cache=FAKE, v_cache=FAKE, k_scale=None, v_scale=None, H=2, d=64, n_pages=4,
              page_size=16, ld_page=2 * 16 * 64, ld_scale=32)

@@ -7,6 +7,9 @@ once (half a step, 2^-8 each) and so is the result (2^-8), the scores are f32
 sums of d products (|ds| <= (d + 2) 2^-24 scale sum |q||k|, below 1e-4 for the
 inputs here, in the numerator and in the sum: 2^-11 covers both), so
     |out - exact| <= (2^-8 + 2^-11) sum p |v| / sum p + 2^-8 |exact|.
+(e4m3 caches: probabilities are rounded to 2^-12 and values to 2^-11 at most; keys rounded
+to 2^-12 move a score by at most 2^-12 scale sum |q||k|, below 2^-9 here, in the numerator
+and in the sum: together below 2^-8 + 2^-11 too.)
 """
 import math
 
@@ -234,6 +237,109 @@ def test_unseen_values_do_not_leak(n, d):
         keep[n - 1, 2:] = False
         assert not bool(torch.isfinite(got[~keep]).any())
         check(torch.where(keep, got, 0).to(BF16), torch.where(keep, want, 0), mag)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 9, 140])
+def test_sizes_far_apart(kind, n):
+    """Values from 2^-24 to 2^24 and keys from 2^-16 to 1 from one token to the next, rows of q
+    from 2^-100 to 2^20: 16-bit operands hold them relative to powers of two."""
+    dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(n)
+    cache = Cache(kind, [700, n + 3], 2, 128, 32, seed=21, poison=False)
+    pages = cache.k.shape[0]
+    kf = torch.exp2(torch.randint(-16, 1, (pages, 1, 32, 1), device=dev, generator=g).float())
+    vf = torch.exp2(torch.randint(-24, 25, (pages, 1, 32, 1), device=dev, generator=g).float())
+    if kind == "bf16":
+        cache.k, cache.v = (cache.k.float() * kf).to(BF16), (cache.v.float() * vf).to(BF16)
+    else:
+        cache.k_scale, cache.v_scale = cache.k_scale * kf[..., 0], cache.v_scale * vf[..., 0]
+    q = torch.randn((2 * n, 4, 128), device=dev, generator=g)
+    q = (q * torch.exp2(torch.randint(-100, 1, (2 * n, 1, 1), device=dev, generator=g).float())).to(BF16)
+    want, mag = attention_64(q, cache, [0, n, 2 * n])
+    check(attend(cache, q, [n, n]), want, mag)
+    # scores of 2^20 and more: one key takes all; ties of the products' roundings apart,
+    # the outputs are that key's values
+    big = (q.float().sign() * 2.0 ** 20).to(BF16)
+    got = attend(cache, big, [n, n])
+    assert bool(torch.isfinite(got).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 70])
+def test_scale_zero_and_scores_of_minus_infinity(kind, n):
+    dev = _dev()
+    cache = Cache(kind, [n + 50, n], 2, 64, 16, seed=2)
+    q = torch.randn((2 * n, 4, 64), device=dev).to(BF16)
+    want, mag = attention_64(q, cache, [0, n, 2 * n], scale=0.0)
+    check(attend(cache, q, [n, n], scale=0.0), want, mag)
+    if kind == "bf16":  # every score is minus infinity: nothing is seen
+        q, ids = torch.ones_like(q), cache.table[0, :cache.table.shape[1]].long()
+        cache.k[ids] = -math.inf
+        got = attend(cache, q, [n, n])
+        assert bool((got[:n] == 0).all()) and bool(torch.isfinite(got[n:]).all())
+
+
+def test_refused_arguments():
+    """Wrong types, shapes, strides and devices raise before anything is launched."""
+    import computd_b200 as cb
+
+    dev = _dev()
+    cache = Cache("e4m3", [40, 20], 2, 64, 16, seed=2)
+    q = torch.zeros((2, 4, 64), device=dev, dtype=BF16)
+    sc = cache.scales()
+    good = dict(q=q, k_cache=cache.k, v_cache=cache.v, block_table=cache.table, lengths=cache.len)
+
+    def attend_with(**kw):
+        a = {**good, **sc, **kw}
+        return cb.paged_attention(a.pop("q"), a.pop("k_cache"), a.pop("v_cache"), a.pop("block_table"),
+                                  a.pop("lengths"), **a)
+
+    attend_with()
+    bad = [dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q[0]), dict(q=q.transpose(0, 1)),
+           dict(q=torch.zeros((3, 4, 64), device=dev, dtype=BF16)),  # not equal chunks
+           dict(q=torch.zeros((2, 3, 64), device=dev, dtype=BF16)),  # 3 heads over 2
+           dict(q=q.cpu()), dict(k_cache=cache.k.float()), dict(k_cache=cache.k[0]),
+           dict(k_cache=cache.k.transpose(1, 2), v_cache=cache.v.transpose(1, 2)),
+           dict(v_cache=cache.v[:1]), dict(k_scale=None), dict(v_scale=cache.v_scale.double()),
+           dict(k_scale=cache.k_scale[:1]), dict(block_table=cache.table.long()),
+           dict(block_table=cache.table[0]), dict(block_table=cache.table.cpu()),
+           dict(lengths=cache.len.long()), dict(lengths=cache.len[:1]),
+           dict(q_start=torch.zeros(2, dtype=torch.int32, device=dev)),
+           dict(max_q=0), dict(scale=-1.0), dict(scale=math.nan), dict(out=q.float()),
+           dict(out=torch.zeros((2, 4, 128), device=dev, dtype=BF16)[:, :, ::2]),
+           dict(status=torch.zeros(2, dtype=torch.int32, device=dev)),
+           dict(q=q.clone().requires_grad_())]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            attend_with(**kw)
+    with pytest.raises(TypeError):
+        attend_with(q=[1])
+    k = torch.zeros((5, 2, 64), device=dev, dtype=BF16)
+    slots = torch.arange(5, device=dev)
+    for a in [(k.half(), k.half()), (k, k.float()), (k[:, :1], k[:, :1]), (k, k[:4]),
+              (k[:, :, ::2], k[:, :, ::2]), (k.cpu(), k.cpu())]:
+        with pytest.raises(ValueError):
+            cb.kv_cache_write(*a, cache.k, cache.v, slots, **sc)
+    for s in (slots.int(), slots[:4], slots[None], torch.arange(10, device=dev)[::2]):
+        with pytest.raises(ValueError):
+            cb.kv_cache_write(k, k, cache.k, cache.v, s, **sc)
+    with pytest.raises(ValueError):  # rows that do not start on 16 bytes
+        wide = torch.zeros((5, 2, 65), device=dev, dtype=BF16)
+        cb.kv_cache_write(wide[:, :, 1:], wide[:, :, 1:], cache.k, cache.v, slots, **sc)
+    with pytest.raises(ValueError):
+        cb.kv_cache_read(cache.k, cache.v, slots, out=(k.float(), k), **sc)
+    odd = torch.zeros((4, 2, 16, 24), device=dev, dtype=BF16)
+    with pytest.raises(cb.DWAArgumentError):
+        cb.kv_cache_read(odd, odd, slots)
+    p = torch.zeros((2, 3, 9), device=dev)
+    x, u, r = torch.zeros((2, 2), dtype=torch.int32, device=dev), p[:, :2, 0].contiguous(), p[:, 0, 0].contiguous()
+    cb.verify_drafts(p, x, p[:, :2].contiguous(), u, r)
+    for a in [(p.half(), x, None, u, r), (p, x.long(), None, u, r), (p, x, p[:, :2], u, r),
+              (p, x, p[:, :2].bfloat16(), u, r), (p, x, None, u[:1], r), (p, x, None, u, u),
+              (p.cpu(), x, None, u, r), (p[:, :, ::2], x, None, u, r)]:
+        with pytest.raises(ValueError):
+            cb.verify_drafts(*a)
 
 
 @pytest.mark.parametrize("n", [1, 6, 150])

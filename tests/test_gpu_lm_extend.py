@@ -152,6 +152,22 @@ def test_uneven_chunks_and_padding(dtype):
     cache.check()
 
 
+def test_one_token_of_one_sequence():
+    cfg, model = _model()
+    cache = model.new_cache(4, page_size=16)
+    table = _i32([[2, 0, 1]])
+    rec = Recorder(model)
+    for n in range(1, 20):
+        out = model.extend(_tokens(cfg)[0, n - 1:n], cache, table, _i32([n]))
+        assert out.shape == (1, cfg.vocab)
+        rec.check(cache, table, [n], [1])
+    rec.close()
+    assert model.extend(_tokens(cfg)[0, :0], cache, table, _i32([5]), _i32([0, 0])).shape == (0, cfg.vocab)
+    with pytest.raises(ValueError):
+        model.extend(_tokens(cfg)[0, :3], cache, _table(cfg, model.new_cache(24, page_size=16)), _i32([3, 1]))
+    cache.check()
+
+
 def test_extend_in_a_graph():
     cfg, model = _model(layers=3)
     tokens = _tokens(cfg, 7)
