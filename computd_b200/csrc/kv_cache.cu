@@ -28,23 +28,27 @@ __device__ __forceinline__ void report(int32_t* status) {
   if (status != nullptr) atomicCAS(status, 0, DWA_ERR_DEVICE_CHECK);
 }
 
-// Sixteen consecutive values of a source row: 32 bytes of bf16, or 64 of f32.
-template <bool kBf16>
-struct Raw16 {
-  uint4 w[kBf16 ? 2 : 4];
+// Values of a lane: sixteen make 16 bytes of codes, eight 16 bytes of bf16.
+template <bool kE4m3>
+constexpr int kLaneValues = kE4m3 ? 16 : 8;
+
+// kN consecutive values of a source row.
+template <bool kBf16, int kN>
+struct Raw {
+  uint4 w[kN / (kBf16 ? 8 : 4)];
 };
-template <bool kBf16>
-__device__ __forceinline__ Raw16<kBf16> load16(const void* row, int64_t at) {
-  Raw16<kBf16> r;
+template <bool kBf16, int kN>
+__device__ __forceinline__ Raw<kBf16, kN> load_raw(const void* row, int64_t at) {
+  Raw<kBf16, kN> r;
   const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + at * (kBf16 ? 2 : 4));
 #pragma unroll
-  for (int i = 0; i < (kBf16 ? 2 : 4); ++i) r.w[i] = __ldg(p + i);
+  for (int i = 0; i < kN / (kBf16 ? 8 : 4); ++i) r.w[i] = __ldg(p + i);
   return r;
 }
-template <bool kBf16>
-__device__ __forceinline__ void as_f32(const Raw16<kBf16>& r, float (&x)[16]) {
+template <bool kBf16, int kN>
+__device__ __forceinline__ void as_f32(const Raw<kBf16, kN>& r, float (&x)[kN]) {
 #pragma unroll
-  for (int i = 0; i < (kBf16 ? 2 : 4); ++i) {
+  for (int i = 0; i < kN / (kBf16 ? 8 : 4); ++i) {
     const uint32_t u[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -76,33 +80,29 @@ __device__ __forceinline__ uint4 codes16(const float (&x)[16]) {
                                                           __NV_SATFINITE, __NV_E4M3)) << 16;
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// Stores the sixteen values of this lane (of `lanes` lanes that hold one vector).
+// Stores the eight values of this lane, rounded to bf16.
+template <bool kBf16>
+__device__ __forceinline__ void store_bf16(const Raw<kBf16, 8>& raw, uint16_t* dst) {
+  if constexpr (kBf16) {
+    *reinterpret_cast<uint4*>(dst) = raw.w[0];
+  } else {
+    float x[8];
+    as_f32(raw, x);
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+// Stores the sixteen values of this lane (of `lanes` lanes that hold one vector) as codes.
 // Every lane of the warp takes part in the shuffles; `on` says whether it
 // holds values, `keep` whether they are stored.
-template <bool kE4m3, bool kBf16>
-__device__ __forceinline__ void store16(const Raw16<kBf16>& raw, bool on, bool keep, int lanes, int lane,
-                                        void* cache, float* scales, int64_t row, int64_t srow, int d) {
-  if constexpr (!kE4m3) {
-    if (on && keep) {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(cache) + row * d + 16 * lane);
-      if constexpr (kBf16) {
-        dst[0] = raw.w[0];
-        dst[1] = raw.w[1];
-      } else {
-        float x[16];
-        as_f32(raw, x);
-        uint32_t u[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-          u[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
-        dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
-      }
-    }
-    return;
-  }
+template <bool kBf16>
+__device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, bool keep, int lanes, int lane,
+                                           uint8_t* cache, float* scales, int64_t row, int64_t srow, int d) {
   float x[16];
   as_f32(raw, x);
   // The largest magnitude as bits: NaN orders above infinity above every finite number.
@@ -137,7 +137,7 @@ __device__ __forceinline__ void store16(const Raw16<kBf16>& raw, bool on, bool k
     w = codes16(x);  // |x / s| <= 448 (1 + 2^-23), which rounds to 448 at most
     scale = s * down;
   }
-  if (on) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(cache) + row * d + 16 * lane) = w;
+  if (on) *reinterpret_cast<uint4*>(cache + row * d + 16 * lane) = w;
   if (lane == 0) scales[srow] = scale;
 }
 
@@ -153,12 +153,12 @@ struct WriteArgs {
   int page_log2;
   int64_t ld_page, ld_scale_page;  // in vectors (rows of d) and in scales
   int64_t tokens_per_block;
-  int lanes_log2;  // lanes per vector: the power of two >= d / 16
+  int lanes_log2;  // lanes per vector: the power of two >= d / (values of a lane)
   int32_t* status;
 };
 
 // A block owns a run of tokens.  `lanes` neighbouring lanes hold one (token,
-// head) vector of K and of V, 16 values each; the amax is a shuffle over them.
+// head) vector of K and of V; the amax is a shuffle over them.
 // Where slots repeat the last token must stay, whichever block writes first:
 // each block drops its tokens whose slot a later token names.  It looks the
 // slots after its own up in a filter of its own slots' low bits, so the whole
@@ -174,17 +174,19 @@ __global__ void __launch_bounds__(kWriteThreads, kSrcBf16 ? kWriteBlocks : kWrit
   const int lane = threadIdx.x & (lanes - 1);
   const int group = threadIdx.x >> a.lanes_log2;
   const int groups = kWriteThreads >> a.lanes_log2;
-  const bool on = 16 * lane < a.d;
+  constexpr int kN = kLaneValues<kE4m3>;
+  using Values = Raw<kSrcBf16, kN>;
+  const bool on = kN * lane < a.d;
   const int64_t t_end = min((blockIdx.x + 1) * a.tokens_per_block, a.T);
   for (int64_t t0 = blockIdx.x * a.tokens_per_block; t0 < t_end; t0 += kGroupTokens) {
     const int n = static_cast<int>(min(t_end - t0, static_cast<int64_t>(kGroupTokens)));
     const int vectors = n * a.H;
     // a round's values are under way while the round before is stored, the first ones
     // while the slots are checked
-    auto load = [&](int i, int h, Raw16<kSrcBf16>* k, Raw16<kSrcBf16>* v) {
+    auto load = [&](int i, int h, Values* k, Values* v) {
       if (i < n && on) {
-        *k = load16<kSrcBf16>(a.k, (t0 + i) * a.k_tok + h * a.k_head + 16 * lane);
-        *v = load16<kSrcBf16>(a.v, (t0 + i) * a.v_tok + h * a.v_head + 16 * lane);
+        *k = load_raw<kSrcBf16, kN>(a.k, (t0 + i) * a.k_tok + h * a.k_head + kN * lane);
+        *v = load_raw<kSrcBf16, kN>(a.v, (t0 + i) * a.v_tok + h * a.v_head + kN * lane);
       }
     };
     auto forward = [&](int* i, int* h) {  // to this group's next vector
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kWriteThreads, kSrcBf16 ? kWriteBlocks : kWrit
         ++*i;
       }
     };
-    Raw16<kSrcBf16> k_now{}, v_now{};
+    Values k_now{}, v_now{};
     int i_now = group / a.H, h_now = group % a.H;
     load(i_now, h_now, &k_now, &v_now);
     __syncthreads();
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(kWriteThreads, kSrcBf16 ? kWriteBlocks : kWrit
     for (int base = 0; base < vectors; base += groups) {
       int i_next = i_now, h_next = h_now;
       forward(&i_next, &h_next);
-      Raw16<kSrcBf16> k_next{}, v_next{};
+      Values k_next{}, v_next{};
       load(i_next, h_next, &k_next, &v_next);
       const bool here = i_now < n;
       const bool keep = here && !dropped[here ? i_now : 0];
@@ -237,8 +239,13 @@ __global__ void __launch_bounds__(kWriteThreads, kSrcBf16 ? kWriteBlocks : kWrit
       const int64_t in_page = (static_cast<int64_t>(h_now) << a.page_log2) + off;
       const int64_t row = page * a.ld_page + in_page;
       const int64_t srow = page * a.ld_scale_page + in_page;
-      store16<kE4m3>(k_now, here && on, keep, lanes, lane, a.k_cache, a.k_scale, row, srow, a.d);
-      store16<kE4m3>(v_now, here && on, keep, lanes, lane, a.v_cache, a.v_scale, row, srow, a.d);
+      if constexpr (kE4m3) {
+        store_e4m3(k_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.k_cache), a.k_scale, row, srow, a.d);
+        store_e4m3(v_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.v_cache), a.v_scale, row, srow, a.d);
+      } else if (on && keep) {
+        store_bf16(k_now, static_cast<uint16_t*>(a.k_cache) + row * a.d + kN * lane);
+        store_bf16(v_now, static_cast<uint16_t*>(a.v_cache) + row * a.d + kN * lane);
+      }
       k_now = k_next;
       v_now = v_next;
       i_now = i_next;
@@ -375,7 +382,7 @@ cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, 
   a.page_log2 = log2_at_least(c.page_size);
   a.n_slots = c.n_pages << a.page_log2;
   a.ld_page = c.ld_page / c.d; a.ld_scale_page = c.ld_scale_page;
-  a.lanes_log2 = log2_at_least(c.d / 16);
+  a.lanes_log2 = log2_at_least(c.d / (c.k_scale != nullptr ? kLaneValues<true> : kLaneValues<false>));
   a.status = status;
   const int64_t most = static_cast<int64_t>(src_bf16 ? kWriteBlocks : kWriteBlocksF32) * device_sm_count();
   a.tokens_per_block = (T + most - 1) / most;
