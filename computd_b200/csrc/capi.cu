@@ -991,14 +991,15 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
   if (T > INT32_MAX || static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX ||
       static_cast<int64_t>(max_pages) * page_size > (1 << 30))
     return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, or over 2^30 tokens per sequence", fn);
-  if (!(scale >= 0.f) || std::isinf(scale))
-    return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite and not negative", fn);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale >= 0.f) || std::isinf(scale_log2))
+    return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite (log2(e) times it too) and not negative", fn);
+  if (T > 0 && !q_start && (B == 0 || T % B != 0 || T / B > max_q))
+    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal chunks of at most "
+                "max_q=%d", fn, (long long)T, B, max_q);
   if (T == 0 || B == 0) return ok();
   if (!q || !out || !lengths || (max_pages > 0 && !block_table))
     return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
-  if (!q_start && (T % B != 0 || T / B > max_q))
-    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal chunks of at most "
-                "max_q=%d", fn, (long long)T, B, max_q);
   if (max_q == 0) return fail(DWA_ERR_INVALID_ARG, "%s: max_q = 0 with rows to compute", fn);
   const int64_t width = static_cast<int64_t>(H) * d;
   if (q_ld < width || out_ld < width || (max_pages > 0 && ld_table < max_pages))
@@ -1019,7 +1020,7 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
   a.even = q_start ? 0 : static_cast<int>(T / B);
   a.max_q = max_q; a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d;
   // not 0: minus infinity times it marks what a row may not see
-  a.scale_log2 = std::max(scale * 1.4426950408889634f, 1.1754944e-38f);
+  a.scale_log2 = std::max(scale_log2, 1.1754944e-38f);
   a.status = status;
   cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dwa_paged_attention launch");

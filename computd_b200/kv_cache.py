@@ -92,7 +92,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with them; ``block_table`` int32 [B, max_pages] holds their pages in order.  New
     token i of n attends to the first length - n + i + 1 tokens, query head h to
     key/value head h // (H / H_kv); ``scale`` defaults to d ** -0.5.  A row that sees
-    nothing is zeros; rows from q_start[B] on are left as they were (in ``out``).
+    nothing is zeros; rows from q_start[B] on are left as they were in ``out``, and without
+    it hold anything.
 
     ``max_q`` bounds the new tokens of any one sequence (default: T); the host picks
     the kernel by it, so a close bound is faster.  A sequence with more gets NaN.

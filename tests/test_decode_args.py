@@ -165,6 +165,8 @@ def test_bad_reads(kw, status):
     (dict(max_q=2 ** 31 - 1), _lib.DWA_ERR_UNSUPPORTED_SHAPE),  # times two query heads
     (dict(q_start=None, T=9), _lib.DWA_ERR_INVALID_ARG),       # not B equal chunks
     (dict(q_start=None, max_q=3), _lib.DWA_ERR_INVALID_ARG),
+    (dict(q_start=None, B=0), _lib.DWA_ERR_INVALID_ARG),       # rows of no sequence
+    (dict(scale=3e38), _lib.DWA_ERR_INVALID_ARG),              # log2(e) times it is infinite
     (dict(scale=float("nan")), _lib.DWA_ERR_INVALID_ARG),
     (dict(scale=float("inf")), _lib.DWA_ERR_INVALID_ARG),
     (dict(scale=-1.0), _lib.DWA_ERR_INVALID_ARG),
