@@ -133,6 +133,7 @@ class ChunkStep:
     lengths: torch.Tensor
     q_start: torch.Tensor
     max_q: int
+    padded: bool               # rows may follow the last sequence's
 
 
 def _rope_theta(dh: int, device) -> torch.Tensor:
@@ -172,8 +173,10 @@ class CausalSelfAttention(nn.Module):
         q, k = (t.transpose(1, 2)[0] for t in (q, k))  # the kernel's token-major buffers
         v = qkv[0, :, 2 * C:].view(T, self.h, self.dh)
         step.cache.write(layer, k, v, step.slots)
+        # the attention leaves a padded batch's last rows as they are
+        out = torch.zeros((T, self.h, self.dh), dtype=q.dtype, device=q.device) if step.padded else None
         o = step.cache.attend(layer, q, step.block_table, step.lengths, q_start=step.q_start,
-                              max_q=step.max_q)
+                              max_q=step.max_q, out=out)
         return x + self.proj(o.view(1, T, C))
 
 
@@ -310,15 +313,18 @@ class DWALM(nn.Module):
         [B + 1]) of sequence b, or T / B rows each without ``q_start``.  ``lengths`` int32 [B]
         counts each sequence's tokens, the new ones with them, and ``block_table`` int32
         [B, max_pages] holds its pages.  ``max_q`` bounds the new tokens of any sequence.
-        Rows behind the last sequence (a padded batch) come out as whatever they are.
+        Rows behind the last sequence (a padded batch; their tokens are in the vocabulary too)
+        attend to nothing.
 
         The retrieval is planned once per row count T (a captured graph needs a call with its
-        T before), so a server pads T to a few counts; on a row-sharded pool every rank calls
-        with the same tokens."""
+        T before), so a server pads T to a few counts; calls with the same T share the plan's
+        workspace and belong on one stream.  On a row-sharded pool every rank calls with the
+        same tokens."""
         T = token_ids.shape[0]
         if token_ids.dim() != 1:
             raise ValueError("token_ids must be [T]")
         B = lengths.shape[0]
+        padded = q_start is not None
         if q_start is None:
             if B == 0 or T % B:
                 raise ValueError(f"without q_start {T} rows must be equal chunks of {B} sequences")
@@ -335,7 +341,7 @@ class DWALM(nn.Module):
         f = torch.outer(positions.float(), _rope_theta(dh, positions.device))
         dtype = self.embed.weight.dtype
         step = ChunkStep(cache, f.cos().to(dtype), f.sin().to(dtype), slots, block_table, lengths,
-                         q_start, T if max_q is None else max_q)
+                         q_start, T if max_q is None else max_q, padded)
         h = self.embed_norm(self.embed_proj(self.embed(token_ids[None])))
         for i, blk in enumerate(self.blocks):
             h = blk.extend(h, retriever, self.vectors, step, i)
@@ -345,20 +351,24 @@ class DWALM(nn.Module):
     def verify(self, last_tokens: torch.Tensor, draft_tokens: torch.Tensor,
                draft_probs: torch.Tensor | None, accept_u: torch.Tensor, sample_u: torch.Tensor,
                cache: PagedKVCache, block_table: torch.Tensor, lengths: torch.Tensor, *,
-               temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+               temperature: float = 1.0,
+               draft_lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """One speculative step: score K drafted tokens of every sequence at once and keep what
         ``verify_drafts`` lets stand.
 
         ``last_tokens`` int [B] (each sequence's newest token, not yet cached) and ``draft_tokens``
         int32 [B, K] are appended to the ``lengths`` (int32 [B]) cached tokens; the pages in
-        ``block_table`` must have room for K + 1 more.  Returns (n_accepted int32 [B], tokens
-        int32 [B, K + 1] as ``verify_drafts``, new lengths int32 [B]: the cached tokens that
-        stay, the last of ``tokens`` being the next step's ``last_tokens``)."""
+        ``block_table`` must have room for K + 1 more.  Sequence b has ``draft_lengths[b]``
+        drafts (int32 [B], default K each); what follows them may be any number.  Returns (n_accepted int32 [B],
+        tokens int32 [B, K + 1] as ``verify_drafts``, new lengths int32 [B]: the cached tokens
+        that stay).  tokens[b, n_accepted[b]] is the next step's ``last_tokens[b]``."""
         B, K = draft_tokens.shape
         chunk = torch.cat([last_tokens.view(B, 1).to(draft_tokens.dtype), draft_tokens], 1)
+        chunk = chunk.clamp(0, self.cfg.vocab - 1)  # a draft outside falls below
         logits = self.extend(chunk.reshape(-1).long(), cache, block_table, lengths + (K + 1))
         probs = torch.softmax(logits.float().view(B, K + 1, -1) / temperature, -1)
-        accepted, tokens = verify_drafts(probs, draft_tokens, draft_probs, accept_u, sample_u)
+        accepted, tokens = verify_drafts(probs, draft_tokens, draft_probs, accept_u, sample_u,
+                                         draft_lengths=draft_lengths)
         return accepted, tokens, lengths + 1 + accepted
 
 

@@ -234,6 +234,52 @@ def test_verify_decides_on_the_models_probabilities(dtype, certain):
     cache.check()
 
 
+@pytest.mark.parametrize("certain", [False, True])
+def test_drafts_outside_the_vocabulary_fall(certain):
+    """What follows a sequence's drafts, and drafts outside the vocabulary, reach no table; the
+    outcome is the 64-bit rule's on the model's probabilities."""
+    from test_gpu_decode import verify_64
+
+    cfg, model = _model(seed=4)
+    cache = model.new_cache(24, page_size=16)
+    table = _table(cfg, cache)
+    tokens = _tokens(cfg, 2)
+    model.extend(tokens[:, :9].reshape(-1), cache, table, _i32([9] * 3))
+    drafts = _i32([[5, 7, -1], [-1, -1, -1], [3, cfg.vocab, 2]])
+    u, r = torch.zeros((3, 3), device="cuda"), torch.full((3,), 0.5, device="cuda")
+    q = None if certain else torch.full((3, 3, cfg.vocab), 1 / 64, device="cuda")
+    last = tokens[:, 9]
+    chunk = torch.cat([last.view(3, 1), drafts.clamp(0, cfg.vocab - 1).long()], 1).reshape(-1)
+    logits = model.extend(chunk, cache, table, _i32([13] * 3))
+    probs = torch.softmax(logits.float().view(3, 4, -1), -1)
+    accepted, out, new = model.verify(last, drafts, q, u, r, cache, table, _i32([9] * 3),
+                                      draft_lengths=_i32([2, 0, 3]))
+    kept, want = verify_64(probs.cpu(), None if certain else q.cpu(), drafts.cpu(), u.cpu(), r.cpu(), [2, 0, 3])
+    assert kept == [2, 0, 1]
+    assert accepted.tolist() == kept and out.tolist() == want and new.tolist() == [12, 10, 11]
+
+
+@pytest.mark.parametrize("max_q", [2, 40])
+def test_padding_rows_attend_to_nothing(max_q):
+    """Whatever the allocator hands out: the rows behind the last sequence are finite."""
+    cfg, model = _model()
+    cache = model.new_cache(24, page_size=16)
+    table = _table(cfg, cache)
+    tokens = _tokens(cfg)[:, :2].reshape(-1)
+    pad = torch.zeros(34, dtype=torch.long, device="cuda")
+    start = _i32([0, 2, 4, 6])
+    rec = Recorder(model)
+    for _ in range(3):
+        junk = [torch.full((40, cfg.d_model), float("nan"), dtype=torch.bfloat16, device="cuda")
+                for _ in range(20)]
+        del junk
+        out = model.extend(torch.cat([tokens, pad]), cache, table, _i32([2] * 3), start, max_q)
+        assert bool(torch.isfinite(out).all())
+        for layer in range(cfg.n_layers):
+            assert not bool(rec.o[layer].view(40, -1)[6:].any())
+    rec.close()
+
+
 def test_bad_pages_are_reported():
     import computd_b200 as cb
 
