@@ -306,14 +306,14 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
           top = max(top, max((qf[nt][k][i] << 16) & 0x7FFF0000u, qf[nt][k][i] & 0x7FFF0000u));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      float f0, f1;
-      f = f16_row_scale(top, a.scale_log2, &f0, &f1);
+      float up;
+      f = f16_row_scale(top, a.scale_log2, &up);
 #pragma unroll
       for (int k = 0; k < C::kSteps; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          qf[nt][k][i] = pack_f16(__uint_as_float(qf[nt][k][i] << 16) * f0 * f1,
-                                  __uint_as_float(qf[nt][k][i] & 0xFFFF0000u) * f0 * f1);
+          qf[nt][k][i] = pack_f16(__uint_as_float(qf[nt][k][i] << 16) * up,
+                                  __uint_as_float(qf[nt][k][i] & 0xFFFF0000u) * up);
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {

@@ -129,19 +129,16 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int high) {
 // stays below 65504 with P up to 2^4, and keeps fp16's 11 bits down to 2^-25.
 constexpr float kPScale = 2048.f;
 
-// A row of Q goes into fp16 times the power of two that puts its largest
+// A row of Q goes into fp16 times the power of two *up that puts its largest
 // magnitude `top` (f32 bits) in [2^13, 2^14): what falls below fp16's range then is
-// 2^-37 of it.  The power comes as a product of two, either of which f32 holds.
-// Returns the factor of the row's scores (never 0: minus infinity times it has to
-// stay that).
-__device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, float* f0, float* f1) {
+// 2^-37 of it.  (2^126 is the largest: rows below 2^-113 come to 2^0 or less, and what is
+// lost of them is 2^-24 of 2^-126.)  Returns the factor of the row's scores (never 0:
+// minus infinity times it has to stay that).
+__device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, float* up) {
   const int e = top == 0 || top >= 0x7F800000u ? 13 : static_cast<int>(top >> 23) - 127;
-  const int half = (13 - e) / 2, rest = 13 - e - half;
-  *f0 = __uint_as_float(static_cast<uint32_t>(127 + half) << 23);
-  *f1 = __uint_as_float(static_cast<uint32_t>(127 + rest) << 23);
-  return fmaxf(__uint_as_float(static_cast<uint32_t>(127 - half) << 23) *
-                   (scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - rest) << 23)),
-               0x1p-126f);
+  const int n = min(13 - e, 126);
+  *up = __uint_as_float(static_cast<uint32_t>(127 + n) << 23);
+  return fmaxf(scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - n) << 23), 0x1p-126f);
 }
 
 // The power of two above x (x >= 0), at least 2^-100.
@@ -175,13 +172,19 @@ __device__ __forceinline__ int ld_cluster_s32(const int* local, int rank) {
                : "memory");
   return v;
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(const float* local, int rank) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(map_to_cta(smem_u32(local), rank))
+// Stores into another block's shared memory, at an address of map_to_cta.
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float x, float y, float z, float w) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w)
                : "memory");
-  return v;
+}
+__device__ __forceinline__ void st_cluster_f32x2(uint32_t addr, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void st_cluster_s32(uint32_t addr, int x) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+}
+__device__ __forceinline__ void min_cluster_s32(uint32_t addr, int x) {
+  asm volatile("red.relaxed.cluster.shared::cluster.min.s32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
 }
 
 // Tensor map of one of the caches, (channel, token of the page, half of the channels, head,

@@ -103,8 +103,8 @@ struct MmaCfg {
   static constexpr int kStageBytes = kTileBytes + (kE4m3 && DP == 64 ? kTile * DP : 0);
   static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kStageBytes;
   // at the end a split block's parts take Q's and the operands' place
-  static constexpr int kPartLd = DP + 4;                // floats per row of O
-  static constexpr int kPartBytes = 2 * kTile * (kPartLd + 2) * 4;
+  static constexpr int kPartMl = 2 * kTile * DP * 4;    // behind O
+  static constexpr int kPartBytes = kPartMl + 2 * kTile * 8;
   static_assert(kPartBytes <= 2 * kTileBytes + kStages * kStageBytes, "parts fit");
 };
 
@@ -117,9 +117,8 @@ struct MmaShared {
   int bad_page;
   int any_bad;
   int first_bad[kMaxChannels];  // least key with a value that is not finite (e4m3: [0], whole vectors)
-  // e4m3 only: a row's factor of the scores; the converting warps' largest scales of
-  // four tiles; the powers of two that keys and values of four steps are divided by
-  float q_factor[kE4m3 ? 2 * kTile : 1];
+  // e4m3 only: the converting warps' largest scales of four tiles; the powers of two
+  // that keys and values of four steps are divided by
   uint64_t tops_ready;
   uint32_t tops[4][4];
   float k_ref[4], v_ref[4];
@@ -280,6 +279,23 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
 }
 
 
+// Rows at equal distances as (new token, query head of the group), divided once.
+struct RowWalk {
+  uint32_t token, head;
+  const uint32_t group, tokens, heads;  // of a step
+  __device__ __forceinline__ RowWalk(uint32_t row, int group_, uint32_t by)
+      : token(row_token(row, group_)), head(row - token * group_), group(group_),
+        tokens(row_token(by, group_)), heads(by - tokens * group_) {}
+  __device__ __forceinline__ void next() {
+    token += tokens;
+    head += heads;
+    if (head >= group) {
+      head -= group;
+      ++token;
+    }
+  }
+};
+
 // ---------------------------------------------------------------- pairs of f32
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;
@@ -339,7 +355,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const PagedSeq s = paged_seq(a, i % a.B);
       const int64_t first = static_cast<int64_t>(row_units - 1 - i / a.B) * 2 * kTile;
       const int64_t end = min(first + 2 * kTile, static_cast<int64_t>(s.n) * a.group);
-      return first < end ? paged_visible(s, static_cast<int>((end - 1) / a.group)) : -1;
+      return first < end ? paged_visible(s, row_token(static_cast<uint32_t>(end - 1), a.group)) : -1;
     });
   const int ru = row_units - 1 - pair_of / a.B, b = pair_of % a.B;
   const PagedSeq seq = paged_seq(a, b);
@@ -361,10 +377,10 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int64_t left = all_rows - r0;
   const int rows0 = static_cast<int>(min(left, static_cast<int64_t>(kTile)));
   const int rows1 = static_cast<int>(max(min(left - kTile, static_cast<int64_t>(kTile)), int64_t{0}));
-  const int vis_min = paged_visible(seq, static_cast<int>(r0 / a.group));
-  const int vis0 = paged_visible(seq, static_cast<int>((r0 + rows0 - 1) / a.group));
-  const int vis1 =
-      rows1 > 0 ? paged_visible(seq, static_cast<int>((r0 + kTile + rows1 - 1) / a.group)) : 0;
+  const uint32_t row_0 = static_cast<uint32_t>(r0);  // below 2^31: max_q bounds it
+  const int vis_min = paged_visible(seq, row_token(row_0, a.group));
+  const int vis0 = paged_visible(seq, row_token(row_0 + rows0 - 1, a.group));
+  const int vis1 = rows1 > 0 ? paged_visible(seq, row_token(row_0 + kTile + rows1 - 1, a.group)) : 0;
   const int vis_max = max(vis0, vis1);
   // this block's share of the key tiles, and how far each row tile goes into it
   const int tiles_all = (vis_max + kTile - 1) / kTile;
@@ -373,6 +389,22 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int n_steps = min(share, tiles_all - first_tile);
   const int steps0 = min(max((vis0 + kTile - 1) / kTile - first_tile, 0), n_steps);
   const int steps1 = min(max((vis1 + kTile - 1) / kTile - first_tile, 0), n_steps);
+
+  // ------------------------------------------------ Q's rows, on their way
+  constexpr int kQChunks = DP / 8;  // of 16 bytes per row; a row's lanes are neighbours
+  constexpr int kQRowsAtOnce = 256 / kQChunks, kQRounds = 2 * kTile / kQRowsAtOnce;
+  const int q_chunk = threadIdx.x % kQChunks, q_first = threadIdx.x / kQChunks;
+  uint4 q_held[kQRounds];
+  if (warp < 8) {
+    const uint16_t* src = a.q + static_cast<int64_t>(hk) * a.group * a.d + 8 * q_chunk;
+    RowWalk at(row_0 + q_first, a.group, kQRowsAtOnce);
+#pragma unroll
+    for (int k = 0; k < kQRounds; ++k, at.next()) {
+      q_held[k] = make_uint4(0, 0, 0, 0);
+      if (q_first + k * kQRowsAtOnce < rows0 + rows1 && 8 * q_chunk < a.d)
+        q_held[k] = __ldg(reinterpret_cast<const uint4*>(src + (seq.row0 + at.token) * a.q_ld + at.head * a.d));
+    }
+  }
 
   // ------------------------------------------------ set-up
   auto bar = [&](const uint64_t& x) { return smem_u32(&x); };
@@ -467,6 +499,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const uint32_t idesc_o = (1u << 4) | kFormat | (1u << 16) |
                                (static_cast<uint32_t>(a.d / 8) << 17) | (kTile / 16 << 24);
       const int k_steps = a.d / 16;
+      const bool full_d = a.d == DP;
       const uint32_t one = elect_one();
       int used = 0;  // products that went through S
       auto wait2 = [&](uint32_t x, int phase_x, uint32_t y, int phase_y) -> bool {
@@ -496,11 +529,16 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         ++used;
         const uint32_t q = k_lo + desc_addr(base + i * C::kTileBytes);
         const uint32_t k = k_lo + desc_addr(s_stage + st * C::kStageBytes);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+        auto step = [&](int s) {
           const uint32_t off = ((s >> 2) * C::kBlockBytes + (s & 3) * 32) >> 4;
-          if (s < k_steps)
-            mma_ss(tm_s, desc64(q + off, k_hi), desc64(k + off, k_hi), idesc_s, s > 0, one);
+          mma_ss(tm_s, desc64(q + off, k_hi), desc64(k + off, k_hi), idesc_s, s > 0, one);
+        };
+        if (full_d) {
+#pragma unroll
+          for (int s = 0; s < DP / 16; ++s) step(s);
+        } else {
+#pragma unroll 1
+          for (int s = 0; s < k_steps; ++s) step(s);
         }
         commit(bar(sh.s_ready[i]), one);
         return true;
@@ -532,41 +570,53 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       }
     } else if (!kE4m3 && warp >= 10) {
       // ---------------------------------------------- values that not every row sees
-      const int t = threadIdx.x - 320;
       for (int it = 0; it < n_items; ++it) {  // keys too: a stage holds either in turn
         const int st = it % C::kStages, key0 = (first_tile + (it >> 1)) * kTile;
         if (!warp_wait(sh.full[st], it / C::kStages)) break;
         if ((it & 1) && key0 + kTile > vis_min) {
-          uint8_t* v = smem + 2 * C::kTileBytes + st * C::kStageBytes;
-          const int first = max(vis_min - key0, 0);
-          for (int i = t; i < (kTile - first) * C::kHalves * 8; i += 64) {
-            const int pc = i & 7, r = first + (i >> 3) / C::kHalves, h = (i >> 3) % C::kHalves;
-            uint4* p = reinterpret_cast<uint4*>(v + h * C::kBlockBytes + r * 128 + pc * 16);
-            if (key0 + r >= vis_max) {
-              *p = make_uint4(0, 0, 0, 0);
-              continue;
-            }
-            const uint4 x = *p;
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            bool found = false;
+          // 64 rows by 128 bytes at a time, a lane's eight loads under way together
+          const int pc = lane & 7, r_of = 32 * (warp - 10) + (lane >> 3);
+#pragma unroll 1
+          for (int h = 0; h < C::kHalves; ++h) {
+            uint8_t* v = smem + 2 * C::kTileBytes + st * C::kStageBytes + h * C::kBlockBytes + pc * 16;
+#pragma unroll 1
+            for (int first = max(vis_min - key0, 0); first < kTile; first += 64) {
+              uint32_t found = 0;  // bit k: this lane's piece of row first + 4 k + r_of
+              uint4 x[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              found = found || (w[k] & 0x7F80u) == 0x7F80u || (w[k] & 0x7F800000u) == 0x7F800000u;
-            if (found) {
-              const int ch = h * 64 + ((pc ^ (r & 7)) << 3);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((w[k] & 0x7F80u) == 0x7F80u) {
-                  atomicMin(&sh.first_bad[ch + 2 * k], key0 + r);
-                  w[k] &= 0xFFFF0000u;
-                }
-                if ((w[k] & 0x7F800000u) == 0x7F800000u) {
-                  atomicMin(&sh.first_bad[ch + 2 * k + 1], key0 + r);
-                  w[k] &= 0x0000FFFFu;
-                }
+              for (int k = 0; k < 8; ++k) {
+                const int r = first + 4 * k + r_of;
+                x[k] = r < kTile ? *reinterpret_cast<const uint4*>(v + r * 128) : make_uint4(0, 0, 0, 0);
               }
-              sh.any_bad = 1;
-              *p = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const int r = first + 4 * k + r_of;
+                // an exponent of ones carries into the sign's place
+                const uint32_t carry = ((x[k].x & 0x7F807F80u) + 0x00800080u) | ((x[k].y & 0x7F807F80u) + 0x00800080u) |
+                                       ((x[k].z & 0x7F807F80u) + 0x00800080u) | ((x[k].w & 0x7F807F80u) + 0x00800080u);
+                if (r < kTile && key0 + r >= vis_max)
+                  *reinterpret_cast<uint4*>(v + r * 128) = make_uint4(0, 0, 0, 0);
+                else if (carry & 0x80008000u)
+                  found |= 1u << k;
+              }
+              for (; found; found &= found - 1) {
+                const int r = first + 4 * (__ffs(found) - 1) + r_of, ch = h * 64 + ((pc ^ (r & 7)) << 3);
+                uint32_t* w = reinterpret_cast<uint32_t*>(v + r * 128);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  uint32_t both = w[k];
+                  if ((both & 0x7F80u) == 0x7F80u) {
+                    atomicMin(&sh.first_bad[ch + 2 * k], key0 + r);
+                    both &= 0xFFFF0000u;
+                  }
+                  if ((both & 0x7F800000u) == 0x7F800000u) {
+                    atomicMin(&sh.first_bad[ch + 2 * k + 1], key0 + r);
+                    both &= 0x0000FFFFu;
+                  }
+                  w[k] = both;
+                }
+                sh.any_bad = 1;
+              }
             }
           }
           fence_proxy_async_smem();
@@ -692,59 +742,46 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     }
   } else {
     regs_inc<C::kSoftmaxRegs>();
-    // ------------------------------------------------ Q into the swizzled operand tiles
-    {
-      constexpr int kChunks = DP / 8;  // of 16 bytes per row; a row's lanes are neighbours
-      constexpr int kRowsAtOnce = 256 / kChunks, kRounds = 2 * kTile / kRowsAtOnce;
-      const int c = threadIdx.x % kChunks, first = threadIdx.x / kChunks;
-      const uint16_t* src = a.q + static_cast<int64_t>(hk) * a.group * a.d + 8 * c;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint4 x[kRounds / 2];
-#pragma unroll
-        for (int k = 0; k < kRounds / 2; ++k) {
-          const int r = first + (half * (kRounds / 2) + k) * kRowsAtOnce;
-          const uint32_t row = static_cast<uint32_t>(r0) + r;  // below 2^31: max_q bounds it
-          x[k] = make_uint4(0, 0, 0, 0);
-          if (r < left && 8 * c < a.d) {
-            const uint32_t token = row_token(row, a.group);
-            x[k] = __ldg(reinterpret_cast<const uint4*>(
-                src + (seq.row0 + token) * a.q_ld + (row - token * a.group) * a.d));
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kRounds / 2; ++k) {
-          const int r = first + (half * (kRounds / 2) + k) * kRowsAtOnce;
-          if constexpr (kE4m3) {
-            uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              top = max(top, max((w[e] << 16) & 0x7FFF0000u, w[e] & 0x7FFF0000u));
-#pragma unroll
-            for (int o = kChunks / 2; o > 0; o >>= 1)
-              top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-            float f0, f1;
-            const float factor = f16_row_scale(top, a.scale_log2, &f0, &f1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_f16(__uint_as_float(w[e] << 16) * f0 * f1,
-                              __uint_as_float(w[e] & 0xFFFF0000u) * f0 * f1);
-            x[k] = make_uint4(w[0], w[1], w[2], w[3]);
-            if (c == 0) sh.q_factor[r] = factor;
-          }
-          const int tile = r / kTile, tr = r % kTile;
-          *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (c >> 3) * C::kBlockBytes + tr * 128 +
-                                    (((c & 7) ^ (tr & 7)) << 4)) = x[k];
-        }
-      }
-      fence_proxy_async_smem();
-      warp_arrive(sh.q_ready);
-      if constexpr (kE4m3) asm volatile("bar.sync 2, 256;" ::: "memory");  // the rows' factors
-    }
-    // ------------------------------------------------ softmax: one row per thread
-    const int i = warp >> 2;
+    const int i = warp >> 2;      // this thread's tile and its row there
     const int r = threadIdx.x & 127;
+    float row_factor = a.scale_log2;  // of the scores, to log2 units
+    // ------------------------------------------------ Q into the swizzled operand tiles
+#pragma unroll
+    for (int k = 0; k < kQRounds; ++k) {
+      const int at = q_first + k * kQRowsAtOnce, tile = at / kTile, tr = at % kTile;
+      *reinterpret_cast<uint4*>(smem + tile * C::kTileBytes + (q_chunk >> 3) * C::kBlockBytes + tr * 128 +
+                                (((q_chunk & 7) ^ (tr & 7)) << 4)) = q_held[k];
+    }
+    if constexpr (kE4m3) {
+      // to fp16: a thread its row, in short loops, since code that runs once per block
+      // costs its fetch
+      asm volatile("bar.sync 2, 256;" ::: "memory");
+      uint8_t* row = smem + i * C::kTileBytes + r * 128;
+      auto piece = [&](int c) {
+        return reinterpret_cast<uint4*>(row + (c >> 3) * C::kBlockBytes + (((c & 7) ^ (r & 7)) << 4));
+      };
+      uint32_t tops = 0;  // of the low and the high halves
+#pragma unroll 4
+      for (int c = 0; c < kQChunks; ++c) {
+        const uint4 x = *piece(c);
+        tops = __vmaxu2(__vmaxu2(tops, __vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu)),
+                        __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+      }
+      float up;
+      row_factor = f16_row_scale(max(tops << 16, tops & 0xFFFF0000u), a.scale_log2, &up) / kCodeScale;
+#pragma unroll 4
+      for (int c = 0; c < kQChunks; ++c) {
+        const uint4 x = *piece(c);
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack_f16(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xFFFF0000u) * up);
+        *piece(c) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    fence_proxy_async_smem();
+    warp_arrive(sh.q_ready);
+    // ------------------------------------------------ softmax: one row per thread
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tm_s + lanes, tp = tm_p + 64 * i + lanes, to = tm_o + 128 * i + lanes;
     const int rows = i ? rows1 : rows0, steps = i ? steps1 : steps0;
@@ -754,8 +791,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     const int vis = live ? paged_visible(seq, row_token(row0 + r, a.group)) : 0;
     // least visible count in the warp: steps below it need no mask
     const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
-    // the scores' factor, to log2 units
-    const float row_factor = kE4m3 ? sh.q_factor[i * kTile + r] / kCodeScale : a.scale_log2;
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
     bool alive = true;
     for (int j = 0; j < steps; ++j) {
@@ -870,7 +905,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const bool some_bad = sh.any_bad;
       uint8_t* stage = smem + i * C::kTileBytes + 32 * (warp & 3) * (2 * DP);
       if (warp_live) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
           if (have) {
@@ -880,40 +915,43 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
             for (int k = 0; k < 32; ++k) o[k] = 0.f;
           }
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float x[8];
+          for (int k = 0; k < 32; ++k) o[k] = l == 0.f ? 0.f : o[k] * inv;
+          if (some_bad) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              x[q] = l == 0.f ? 0.f : o[k + q] * inv;
-              if (some_bad && sh.first_bad[kE4m3 ? 0 : 32 * c + k + q] < vis)
-                x[q] = __uint_as_float(0x7FC00000u);
-            }
-            *reinterpret_cast<uint4*>(stage + lane * (2 * DP) +
-                                      (((4 * c + k / 8) ^ (lane & 7)) << 4)) =
-                make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]),
-                           pack_bf16(x[6], x[7]));
+            for (int k = 0; k < 32; ++k)
+              if (sh.first_bad[kE4m3 ? 0 : 32 * c + k] < vis) o[k] = __uint_as_float(0x7FC00000u);
           }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            *reinterpret_cast<uint4*>(stage + lane * (2 * DP) + (((4 * c + k / 8) ^ (lane & 7)) << 4)) =
+                make_uint4(pack_bf16(o[k], o[k + 1]), pack_bf16(o[k + 2], o[k + 3]),
+                           pack_bf16(o[k + 4], o[k + 5]), pack_bf16(o[k + 6], o[k + 7]));
         }
         __syncwarp();
         constexpr int kChunks = DP / 8;
         const int chunk = lane % kChunks;
-        for (int q = lane / kChunks; q < min(rows - 32 * (warp & 3), 32); q += 32 / kChunks) {
-          const uint32_t row = row0 + 32 * (warp & 3) + q, token = row_token(row, a.group);
-          if (8 * chunk < a.d)
-            *reinterpret_cast<uint4*>(a.out + (seq.row0 + token) * a.out_ld +
-                                      (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d +
-                                      8 * chunk) =
+        RowWalk at(row0 + 32 * (warp & 3) + lane / kChunks, a.group, 32 / kChunks);
+        uint16_t* const out = a.out + static_cast<int64_t>(hk) * a.group * a.d + 8 * chunk;
+#pragma unroll 4
+        for (int k = 0; k < kChunks; ++k, at.next()) {
+          const int q = lane / kChunks + k * (32 / kChunks);
+          if (q < rows - 32 * (warp & 3) && 8 * chunk < a.d)
+            *reinterpret_cast<uint4*>(out + (seq.row0 + at.token) * a.out_ld + at.head * a.d) =
                 *reinterpret_cast<const uint4*>(stage + q * (2 * DP) + ((chunk ^ (q & 7)) << 4));
         }
       }
     } else {
-      // this block's part: rows of O, then their m and l
-      float* part = reinterpret_cast<float*>(smem);
-      float* part_ml = part + 2 * kTile * C::kPartLd;
+      // The cluster's blocks share out the unit's rows, and each sends every other its part
+      // of that one's rows: O [32 rows][channel / 4][row] by fours, so that a warp's stores
+      // are contiguous, and m and l.  Stores into another block's shared memory are not
+      // waited for; loads from it, which take a microsecond each, made the join 11 us.
+      const int log2_rows = 8 - (31 - __clz(cluster)), rows_of = 1 << log2_rows;
       const int mine = i * kTile + r;
-      asm volatile("bar.sync 2, 256;" ::: "memory");  // both tiles' products have read their operands
+      const int slot = (split << log2_rows) + (mine & (rows_of - 1));
+      cluster_sync();  // every block's products have read their operands
+      const uint32_t there = map_to_cta(base, mine >> log2_rows);
       if (warp_live) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           float o[32];
           if (have) {
@@ -922,81 +960,72 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 32; ++k) o[k] = 0.f;
           }
+          const uint32_t dst = there + (((slot >> 5) * (DP / 4) + 8 * c) * 32 + (slot & 31)) * 16;
 #pragma unroll
           for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<float4*>(part + mine * C::kPartLd + 32 * c + k) =
-                make_float4(o[k] * v_back, o[k + 1] * v_back, o[k + 2] * v_back, o[k + 3] * v_back);
+            st_cluster_f32x4(dst + 128 * k, o[k] * v_back, o[k + 1] * v_back, o[k + 2] * v_back,
+                             o[k + 3] * v_back);
         }
       }
-      part_ml[2 * mine] = m;
-      part_ml[2 * mine + 1] = l;
+      st_cluster_f32x2(there + C::kPartMl + 8 * slot, m, l);
+      if (sh.any_bad) {
+        for (int at = threadIdx.x; at < cluster * kMaxChannels; at += 256)
+          min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kMaxChannels]), at / kMaxChannels),
+                          sh.first_bad[at % kMaxChannels]);
+        if (threadIdx.x < cluster) st_cluster_s32(map_to_cta(smem_u32(&sh.any_bad), threadIdx.x), 1);
+      }
       cluster_sync();
-      // The unit's rows, four at a time, dealt to the cluster's warps.  Lane (q, c) gets row
-      // q's m and l in part c and its weight; then a lane has four channels of each row.
-      // All loads of a step are under way together: each takes a microsecond.
-      const int all = static_cast<int>(min(left, static_cast<int64_t>(2 * kTile)));
-      const int q_of = lane >> 3, c_of = lane & 7;
-      const bool bad = __any_sync(0xFFFFFFFFu, c_of < cluster && ld_cluster_s32(&sh.any_bad, min(c_of, cluster - 1)) != 0);
-      for (int first = 4 * (split * 8 + warp); first < all; first += 4 * 8 * cluster) {
-        float pm = -INFINITY, pl = 0.f;
-        if (c_of < cluster) {
-          pm = ld_cluster_f32(part_ml + 2 * (first + q_of), c_of);
-          pl = ld_cluster_f32(part_ml + 2 * (first + q_of) + 1, c_of);
-        }
-        float top = pm;
+      // A warp joins eight rows at a time, lane (x, q) channels 4 x + 16 t of row q: all of
+      // a part's loads are under way together, and free of bank conflicts.
+      const bool some_bad = sh.any_bad;
+      const int row_end = rows0 + rows1 - (split << log2_rows);  // of this block's rows
+      const int q = lane & 7, x = lane >> 3;
+      for (int first = 8 * warp; first < min(rows_of, row_end); first += 64) {
+        const int row = first + q;
+        float top = -INFINITY, sum = 0.f;
+        for (int c = 0; c < cluster; ++c)
+          top = fmaxf(top, *reinterpret_cast<const float*>(smem + C::kPartMl + 8 * ((c << log2_rows) + row)));
+        float y[DP / 16][4] = {};
+#pragma unroll 1
+        for (int c = 0; c < cluster; ++c) {
+          const int at = (c << log2_rows) + row;
+          const float2 ml = *reinterpret_cast<const float2*>(smem + C::kPartMl + 8 * at);
+          float4 o[DP / 16];
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        // a part without keys has l = 0 (or NaN, which has to stay)
-        float weight = pm == -INFINITY ? 0.f : fast_exp2(pm - top);
-        float sum = pm == -INFINITY ? pl : weight * pl;
+          for (int t = 0; t < DP / 16; ++t)
+            o[t] = *reinterpret_cast<const float4*>(smem + (((at >> 5) * (DP / 4) + 4 * t + x) * 32 + (at & 31)) * 16);
+          // a part without keys has l = 0 (or NaN, which has to stay)
+          const float weight = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+          sum += ml.x == -INFINITY ? ml.y : weight * ml.y;
+          if (weight != 0.f) {  // else what is there may be anything
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        const float inv_row = sum == 0.f ? 0.f : 1.f / sum;
-        const int ch = 4 * lane;
-        float x[4][4] = {};
-#pragma unroll
-        for (int c = 0; c < kMaxSplit; ++c) {
-          if (c < cluster) {
-            float4 y[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              y[q] = ch < DP ? ld_cluster_f32x4(part + (first + q) * C::kPartLd + ch, c)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float w = __shfl_sync(0xFFFFFFFFu, weight, 8 * q + c);
-              // weight 0: what is there may be anything (rows without a thread's part)
-              x[q][0] += w == 0.f ? 0.f : w * y[q].x;
-              x[q][1] += w == 0.f ? 0.f : w * y[q].y;
-              x[q][2] += w == 0.f ? 0.f : w * y[q].z;
-              x[q][3] += w == 0.f ? 0.f : w * y[q].w;
+            for (int t = 0; t < DP / 16; ++t) {
+              y[t][0] += weight * o[t].x;
+              y[t][1] += weight * o[t].y;
+              y[t][2] += weight * o[t].z;
+              y[t][3] += weight * o[t].w;
             }
           }
         }
+        if (row >= row_end) continue;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const uint32_t of_unit = row_0 + (split << log2_rows) + row, token = row_token(of_unit, a.group);
+        uint16_t* const out = a.out + (seq.row0 + token) * a.out_ld +
+                              (static_cast<int64_t>(hk) * a.group + of_unit - token * a.group) * a.d + 4 * x;
+        if (some_bad) {
+          const int vis_q = paged_visible(seq, token);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float inv = __shfl_sync(0xFFFFFFFFu, inv_row, 8 * q);
-          if (first + q < all && ch < a.d) {
-            const uint32_t row = static_cast<uint32_t>(r0) + first + q;
-            const uint32_t token = row_token(row, a.group);
+          for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[q][e] *= inv;
-              if (bad) {
-                const int vis_q = paged_visible(seq, token);
-                for (int c = 0; c < cluster; ++c)
-                  if (ld_cluster_s32(&sh.first_bad[kE4m3 ? 0 : ch + e], c) < vis_q)
-                    x[q][e] = __uint_as_float(0x7FC00000u);
-              }
-            }
-            *reinterpret_cast<uint2*>(a.out + (seq.row0 + token) * a.out_ld +
-                                      (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d +
-                                      ch) =
-                make_uint2(pack_bf16(x[q][0], x[q][1]), pack_bf16(x[q][2], x[q][3]));
-          }
+            for (int e = 0; e < 4; ++e)
+              if (sh.first_bad[kE4m3 ? 0 : 16 * t + 4 * x + e] < vis_q) y[t][e] = __uint_as_float(0x7FC00000u);
         }
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t)
+          if (16 * t < a.d)  // d is a multiple of 16
+            *reinterpret_cast<uint2*>(out + 16 * t) =
+                make_uint2(pack_bf16(y[t][0] * inv, y[t][1] * inv), pack_bf16(y[t][2] * inv, y[t][3] * inv));
       }
-      cluster_sync();  // no block leaves while another reads its part
     }
     tc_fence_before();
   }
