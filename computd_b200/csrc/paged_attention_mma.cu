@@ -48,6 +48,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 
 #include "dwa_internal.h"
 #include "paged_attention.cuh"
@@ -408,26 +409,62 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
 
   // ------------------------------------------------ set-up
   auto bar = [&](const uint64_t& x) { return smem_u32(&x); };
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(bar(sh.full[i]), 1);
-      mbar_init(bar(sh.ready[i]), kE4m3 ? 4 : 2);
-      mbar_init(bar(sh.empty[i]), 1);
+  const int n_items = 2 * n_steps;  // operand tiles: K V K V ...
+  const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
+  // TMA, straight from the pages: a page to a lane
+  auto bring = [&](int it) {
+    const int page_size = 1 << a.page_log2;
+    const int key0 = (first_tile + (it >> 1)) * kTile, st = it % C::kStages;
+    const int pages = min(kTile >> a.page_log2, (vis_max - key0 + page_size - 1) >> a.page_log2);
+    int page = 0;
+    if (lane < pages) {
+      page = __ldg(table + (key0 >> a.page_log2) + lane);
+      if (page < 0 || page >= a.n_pages) {
+        sh.bad_page = 1;  // read page 0 in its place; the rows become NaN
+        page = 0;
+      }
     }
-    mbar_init(bar(sh.s_free), 4);
-    mbar_init(bar(sh.tops_ready), 4);
-    mbar_init(bar(sh.q_ready), 8);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(sh.s_ready[i]), 1);
-      mbar_init(bar(sh.p_ready[i]), 4);
-      mbar_init(bar(sh.p_free[i]), 1);
+    const uint32_t full = bar(sh.full[st]);
+    if (lane == 0)
+      mbar_arrive_expect_tx(full, static_cast<uint32_t>(pages * page_size) * (kE4m3 ? DP : 128 * C::kHalves));
+    __syncwarp();
+    if (lane < pages) {
+      const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
+      const uint32_t dst = s_stage + st * C::kStageBytes;
+      if constexpr (kE4m3) {
+        tma_load_5d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, 0, hk, page);
+      } else {
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_5d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, 0, hk, page);
+      }
     }
-    sh.abort = 0;
-    sh.bad_page = 0;
-    sh.any_bad = 0;
-    fence_mbar_init();
+  };
+  if (warp == 9) {
+    if (lane == 0) {
+      for (int i = 0; i < C::kStages; ++i) {
+        mbar_init(bar(sh.full[i]), 1);
+        mbar_init(bar(sh.ready[i]), kE4m3 ? 4 : 2);
+        mbar_init(bar(sh.empty[i]), 1);
+      }
+      mbar_init(bar(sh.s_free), 4);
+      mbar_init(bar(sh.tops_ready), 4);
+      mbar_init(bar(sh.q_ready), 8);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(bar(sh.s_ready[i]), 1);
+        mbar_init(bar(sh.p_ready[i]), 4);
+        mbar_init(bar(sh.p_free[i]), 1);
+      }
+      sh.abort = 0;
+      sh.bad_page = 0;
+      sh.any_bad = 0;
+      fence_mbar_init();
+    }
+    __syncwarp();
+    for (int it = 0; it < min(C::kStages, n_items); ++it) bring(it);  // no one to wait for
   }
-  if (threadIdx.x < kMaxChannels) sh.first_bad[threadIdx.x] = 0x7FFFFFFF;
+  if (warp == 10)
+    for (int i = lane; i < kMaxChannels; i += 32) sh.first_bad[i] = 0x7FFFFFFF;
   if (warp == 8) {
     tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
@@ -438,7 +475,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const uint32_t tm_s = sh.tmem, tm_p = sh.tmem + 128, tm_o = sh.tmem + 256;  // + 64 i, + 128 i
   int* const status = a.status;
   volatile int* const abort_flag = &sh.abort;
-  const int n_items = 2 * n_steps;
   // a bounded wait of the whole warp, which goes on or gives up together
   auto warp_wait = [&](const uint64_t& x, int phase) -> bool {
     return warp_wait1(bar(x), phase & 1, status, abort_flag);
@@ -452,39 +488,11 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   if (warp >= 8) {
     regs_dec<C::kOtherRegs>();
     if (warp == 9) {
-      // ---------------------------------------------- TMA: K V K V ...
-      const int page_size = 1 << a.page_log2;
-      const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
-      int issued = 0;
-      for (int it = 0; it < n_items; ++it) {
-        const int key0 = (first_tile + (it >> 1)) * kTile, st = it % C::kStages;
-        const int pages = min(kTile >> a.page_log2, (vis_max - key0 + page_size - 1) >> a.page_log2);
-        int page = 0;
-        if (lane < pages) {
-          page = __ldg(table + (key0 >> a.page_log2) + lane);
-          if (page < 0 || page >= a.n_pages) {
-            sh.bad_page = 1;  // read page 0 in its place; the rows become NaN
-            page = 0;
-          }
-        }
-        if (it >= C::kStages && !warp_wait(sh.empty[st], it / C::kStages - 1)) break;
-        const uint32_t full = bar(sh.full[st]);
-        if (lane == 0)
-          mbar_arrive_expect_tx(full, static_cast<uint32_t>(pages * page_size) *
-                                          (kE4m3 ? DP : 128 * C::kHalves));
-        __syncwarp();
-        if (lane < pages) {
-          const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
-          const uint32_t dst = s_stage + st * C::kStageBytes;
-          if constexpr (kE4m3) {
-            tma_load_5d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, 0, hk, page);
-          } else {
-#pragma unroll
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_5d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, 0, hk,
-                          page);
-          }
-        }
+      // ---------------------------------------------- TMA
+      int issued = min(C::kStages, n_items);
+      for (int it = issued; it < n_items; ++it) {
+        if (!warp_wait(sh.empty[it % C::kStages], it / C::kStages - 1)) break;
+        bring(it);
         issued = it + 1;
       }
       // after an abort nobody else waits for the copies in flight
@@ -629,7 +637,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       // 64 + 16 c .. of it (c = lane & 3).  Neighbouring groups of four take rows r and
       // r ^ 5, so that neither the reads nor the writes meet in a bank.
       const int w = warp - 12, t = threadIdx.x - 384;
-      const int32_t* table = a.table + static_cast<int64_t>(b) * a.ld_table;
       const int c = lane & 3, pair_row = (lane >> 3) & 3;
       const int row8 = (lane & 4) ? pair_row ^ 5 : pair_row;  // of eight
       const int row0 = 32 * w + row8;
@@ -1036,15 +1043,23 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   }
 }
 
-// Once per device: the shared memory limit, and that the launch brings the
-// registers that the warps share out among themselves.
+// What a device has, asked for once: how many clusters of 1, 2, 4 and 8 blocks run at a time
+// (a block fills an SM, and a cluster has to find its SMs in one part of the chip: 15 of 8
+// blocks on 148 SMs).  Also lets the kernel have its shared memory, and checks that the
+// launch brings the registers that the warps share out among themselves.
 template <bool kE4m3, int DP>
-cudaError_t configure_mma() {
+cudaError_t configure_mma(cudaLaunchConfig_t cfg, const int** clusters) {
   using C = MmaCfg<kE4m3, DP>;
   static std::atomic<bool> done[64] = {};
+  static int fit[64][4];
+  static std::mutex once;
   int dev = 0;
   if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
-  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  *clusters = fit[dev];
+  if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  const std::lock_guard<std::mutex> lock(once);
+  if (done[dev].load(std::memory_order_relaxed)) return cudaSuccess;  // meanwhile
   cudaFuncAttributes attr;
   if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_mma_kernel<kE4m3, DP>); e != cudaSuccess)
     return e;
@@ -1055,7 +1070,21 @@ cudaError_t configure_mma() {
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       e != cudaSuccess)
     return e;
-  if (dev < 64) done[dev].store(true, std::memory_order_release);
+  int found[4] = {device_sm_count()};
+  for (int i = 1; i < 4; ++i) {
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = 1u << i;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1u << i);
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&found[i], paged_mma_kernel<kE4m3, DP>, &cfg);
+        e != cudaSuccess)
+      return e;
+  }
+  for (int i = 0; i < 4; ++i) fit[dev][i] = found[i];
+  done[dev].store(true, std::memory_order_release);
   return cudaSuccess;
 }
 
@@ -1070,28 +1099,30 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
   const int row_units = static_cast<int>((most_rows + 2 * kTile - 1) / (2 * kTile));
   const int64_t units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  const int* at_a_time;
+  if (cudaError_t e = configure_mma<kE4m3, DP>(cfg, &at_a_time); e != cudaSuccess) return e;
   // How many blocks share a unit's keys: what takes clearly the fewest rounds of steps
-  // (a step is about 3000 cycles), if every sequence were as long as the table allows.  A
-  // block costs about three steps more than its keys, a split one eight and more: its
+  // (a step is 3000 to 3900 cycles), if every sequence were as long as the table allows.  A
+  // block costs about three steps more than its keys, a split one six and more: its
   // part goes through distributed shared memory.
-  const int64_t sms = device_sm_count();
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
   int cluster = 1;
-  int64_t best = ((units + sms - 1) / sms) * (steps + 3);
-  for (int c = 2; c <= kMaxSplit; c *= 2) {
-    const int64_t cost = ((units * c + sms - 1) / sms) * ((steps + c - 1) / c + 6 + c / 2);
+  int64_t best = ((units + at_a_time[0] - 1) / at_a_time[0]) * (steps + 3);
+  for (int i = 1; 1 << i <= kMaxSplit; ++i) {
+    const int c = 1 << i;
+    if (at_a_time[i] < 1) break;
+    const int64_t cost = ((units + at_a_time[i] - 1) / at_a_time[i]) * ((steps + c - 1) / c + 6 + c / 4);
     if (10 * cost < 9 * best) {
       best = cost;
       cluster = c;
     }
   }
   if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
-  if (cudaError_t e = configure_mma<kE4m3, DP>(); e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
-  cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = static_cast<unsigned>(cluster);
