@@ -3,7 +3,7 @@
 //
 // A row is one (new token, query head); the rows of a key/value head are
 // token-major, its `group` query heads side by side.  Bound by HBM: each
-// cached key and value is read once for up to 32 rows.
+// cached key and value is read once for up to 16 rows.
 //
 // The products are transposed so that the few rows lie along the 8 columns of
 // mma.m16n8k16: S^T = K Q^T takes 16 keys by 8 rows, O^T += V^T P^T takes 16
@@ -23,7 +23,7 @@
 //
 // bf16 caches: P is used as the sum of two bf16 parts, so that only the result's
 // rounding is left.  e4m3 caches: codes become fp16 exactly, Q is scaled per row by
-// a power of two into fp16 (nothing is lost), the keys' scales multiply the scores,
+// a power of two into fp16 (a part below 2^-37 of its largest is lost), the keys' scales multiply the scores,
 // and P times the values' scales, relative to a running power of two, is rounded to
 // fp16 (2^-11).
 #include <cuda_bf16.h>
@@ -41,7 +41,7 @@ namespace {
 
 constexpr int kMaxCluster = 8;
 // Rows per key/value head that this kernel takes; more go to the tcgen05 kernel.  At 20
-// rows (16 sequences of 4096, 8 heads of 128, bf16) that one takes 81 us, this one 165.
+// rows (16 sequences of 4096, 8 heads of 128, bf16) that one takes 58 us, this one (in two passes) 165.
 constexpr int kFewRows = 16;
 
 template <bool kF16>
@@ -89,7 +89,7 @@ struct RowsCfg {
   static constexpr int kSub = kE4m3 ? 2 : 1;      // 16-key tiles per block
   static constexpr int kKeys = 16 * kSub;
   static constexpr int kSteps = DP / 16;          // k-steps of S, channel tiles of O
-  static constexpr int kRows = 8 * NT;
+  static constexpr int kRows = 8 * NT;            // kFewRows at most
   static constexpr int kRowBytes = kE4m3 ? DP : 128;              // of a TMA box
   static constexpr int kHalves = kE4m3 ? 1 : DP / 64;             // boxes side by side
   static constexpr int kBoxBytes = 16 * kRowBytes;
@@ -142,7 +142,7 @@ template <bool kE4m3, int DP, int NT, int W>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
-                      const int row_groups, const int cluster, const int wide) {
+                      const int cluster, const int wide) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
   constexpr int kWarps = W, kThreads = 32 * W;
   extern __shared__ uint8_t smem_raw[];
@@ -157,10 +157,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  uint32_t unit = blockIdx.x / cluster;  // the grid has 32 bits
+  const uint32_t unit = blockIdx.x / cluster;  // the grid has 32 bits
   const int split = static_cast<int>(blockIdx.x % cluster);
-  const int rg = static_cast<int>(unit % row_groups);
-  unit /= row_groups;
   const int hk = static_cast<int>(unit % a.H_kv);
   // the longest sequences first
   __shared__ int costs[kMostRanked], found;
@@ -169,27 +167,20 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     b = ranked(a.B, b, costs, &found, [&](int i) { return __ldg(a.lengths + i); });
 
   PagedSeq seq = paged_seq(a, b);
-  if (seq.bad && hk == 0 && rg == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
+  if (seq.bad && hk == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
   const int64_t all_rows = static_cast<int64_t>(seq.n) * a.group;
-  const int64_t r0 = static_cast<int64_t>(rg) * C::kRows;
-  if (r0 >= all_rows) return;  // the whole cluster
-  if (seq.bad) {
-    // every group its own rows, and those row_groups groups further on: a
-    // sequence with more rows than max_q has more than there are groups
-    const int64_t stride = static_cast<int64_t>(row_groups) * C::kRows;
-    for (int64_t at = r0; at < all_rows; at += stride)
-      for (int i = split * kThreads + threadIdx.x; i < C::kRows * a.d; i += cluster * kThreads) {
-        const int64_t row = at + i / a.d;
-        if (row < all_rows)
-          a.out[(seq.row0 + row / a.group) * a.out_ld +
-                (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
-      }
+  if (all_rows == 0) return;  // the whole cluster
+  if (seq.bad) {  // it may have more rows than max_q
+    for (int64_t i = split * kThreads + threadIdx.x; i < all_rows * a.d; i += cluster * kThreads) {
+      const int64_t row = i / a.d;
+      a.out[(seq.row0 + row / a.group) * a.out_ld +
+            (static_cast<int64_t>(hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
+    }
     return;
   }
-  const int rows = static_cast<int>(min(all_rows - r0, static_cast<int64_t>(C::kRows)));
-  const uint32_t row0 = static_cast<uint32_t>(r0);  // below 2^31: max_q bounds it
-  const int vis_min = paged_visible(seq, row_token(row0, a.group));
-  const int vis_max = paged_visible(seq, row_token(row0 + rows - 1, a.group));
+  const int rows = static_cast<int>(all_rows);  // max_q bounds them to kRows
+  const int vis_min = paged_visible(seq, 0);
+  const int vis_max = paged_visible(seq, seq.n - 1);
 
   // ------------------------------------------------ Q^T fragments, on their way
   // lane (g, t) holds row 8 nt + g at the channels its key chunks have
@@ -199,7 +190,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = 8 * nt + g;
-    const uint32_t row = row0 + r, token = row_token(row, a.group);
+    const uint32_t row = r, token = row_token(row, a.group);
     const uint16_t* src = a.q + (seq.row0 + token) * a.q_ld +
                           (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d;
 #pragma unroll
@@ -319,7 +310,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     for (int j = 0; j < 2; ++j) {
       factor[nt][j] = kE4m3 ? __shfl_sync(0xFFFFFFFFu, f, 4 * (2 * t + j)) : f;
       const int rc = 8 * nt + 2 * t + j;
-      vis[nt][j] = rc < rows ? paged_visible(seq, row_token(row0 + rc, a.group)) : 0;
+      vis[nt][j] = rc < rows ? paged_visible(seq, row_token(rc, a.group)) : 0;
     }
   }
 
@@ -630,7 +621,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
         y += f * os[c].y;
       }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const uint32_t row = row0 + r, token = row_token(row, a.group);
+    const uint32_t row = r, token = row_token(row, a.group);
     const int seen = paged_visible(seq, token);
     x = bad0 < seen ? __uint_as_float(0x7FC00000u) : x * inv;
     y = bad1 < seen ? __uint_as_float(0x7FC00000u) : y * inv;
@@ -665,8 +656,7 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  const int row_groups = static_cast<int>(units / (static_cast<int64_t>(a.B) * a.H_kv));
-  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, row_groups, cluster, wide ? 1 : 0);
+  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, cluster, wide ? 1 : 0);
 }
 
 // How a call is cut up: the longest context is split over 2^n blocks of 4 warps
@@ -698,7 +688,7 @@ cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
   const int64_t heads = static_cast<int64_t>(a.B) * a.H_kv;
   if (rows <= 8) return launch_rows_cut<kE4m3, DP, 1>(a, heads, stream);
-  return launch_rows_cut<kE4m3, DP, 2>(a, heads * ((rows + 15) / 16), stream);
+  return launch_rows_cut<kE4m3, DP, 2>(a, heads, stream);
 }
 
 }  // namespace

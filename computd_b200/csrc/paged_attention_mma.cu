@@ -17,15 +17,21 @@
 // an S per tile that P overwrote, each step was a chain of product, exponentials,
 // product: 2.9 us per 2 x 128 rows x 128 keys of 128 channels instead of 2.2.)
 //
-// Per step the products take 2048 cycles of the tensor pipe (8192 FLOP a cycle), the
-// exponentials 32768 / 16 = 2048 of the special-function units, and everything else
-// about as much of the other units' time, which is what bounds it: measured 2900 cycles
-// a step, 1.05 to 1.09 PFLOP/s (4736 rows over 16384 keys, 32 heads of 128, bf16: 996 us;
-// e4m3 1171 us, the conversion sharing the issue slots).  A polynomial for a part of the
-// exponentials made it slower (1065 us with a quarter, 1031 with none then).  What can be
-// is done in pairs (f32x2) and triples (max).  m only moves when a row's maximum grew by
-// more than 2^kSlack (the result does not depend on m; P stays below 2^kSlack), so O is
-// hardly ever rescaled, and then by the row's own thread.
+// Per step the products take 2048 cycles of the tensor pipe (8192 FLOP a cycle) and the
+// exponentials 32768 / 16 = 2048 of the special-function units.  What bounds it is each
+// row's own chain: S out of TMEM 200 cycles, the maximum 450, 128 exponentials with their
+// sums and packing 1600 (1024 at the units' rate; a warp alone with these registers takes
+// 1400), P into TMEM and the next S 300 to 500.  Measured 3000 cycles a step, e4m3 3900,
+// where the conversion shares the issue slots: 4736 rows over 16384 keys, 32 heads of 128,
+// 1.0 to 1.12 ms (bf16, 0.97 to 1.08 PFLOP/s, the power limit's clock deciding) and 1.17 to
+// 1.3 ms.  Not faster: a polynomial for a quarter of the exponentials (1065 us, 1031 without
+// then), S before the other tile's product (3300 cycles), a warp each for S and O, eight
+// converting warps.  What can be is done in pairs (f32x2) and triples (max).  m only moves
+// when a row's maximum grew by more than 2^kSlack (the result does not depend on m; P
+// stays below 2^kSlack), so O is hardly ever rescaled, and then by the row's own thread.
+//
+// A block costs 9 to 11 thousand cycles before its first scores (launch, the sequence's numbers,
+// Q's 64 KB from all SMs at once) and 4 after its last, a split one 8 to 12.
 //
 // Warps 0-3 and 4-7: the rows of tile 0 and 1.  Warp 8: issues every tcgen05.mma.
 // Warp 9: TMA, straight from the pages into the swizzled operand tiles.  bf16
@@ -951,7 +957,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       // The cluster's blocks share out the unit's rows, and each sends every other its part
       // of that one's rows: O [32 rows][channel / 4][row] by fours, so that a warp's stores
       // are contiguous, and m and l.  Stores into another block's shared memory are not
-      // waited for; loads from it, which take a microsecond each, made the join 11 us.
+      // waited for; loads from it, which take a microsecond each, made the join 11 us; it takes 5.
       const int log2_rows = 8 - (31 - __clz(cluster)), rows_of = 1 << log2_rows;
       const int mine = i * kTile + r;
       const int slot = (split << log2_rows) + (mine & (rows_of - 1));
