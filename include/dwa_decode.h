@@ -64,7 +64,7 @@ DWA_API dwa_status dwa_kv_read(const void* k_cache, const void* v_cache, const f
  * lengths[b] cached tokens (the new ones written already) on the pages
  * block_table[b ld_table + i] (int32, i < ceil(length / page_size)), and its
  * new tokens are rows q_start[b] .. q_start[b + 1] - 1 of q (q_start NULL: T / B
- * rows each).  For new token i of n and query head h,
+ * rows each, which B has to divide).  For new token i of n and query head h,
  *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max),
  *   j < length - n + i + 1,
  * with the key and value head h / (H / H_kv); no key, or no score above -inf,
