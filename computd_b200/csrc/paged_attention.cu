@@ -14,7 +14,7 @@
 // accumulator is known).  P^T is turned between the products by movmatrix.
 //
 // Each warp works alone on blocks of 16 (bf16) or 32 (e4m3) keys, which its own
-// ring of TMA copies brings, 8 KB at a time and two in flight, three blocks of four warps
+// ring of TMA copies brings, up to 8 KB at a time and two in flight, three blocks of four warps
 // to an SM.  (Loaded into registers, one block ahead: 137 us instead of 83 for 64 ragged
 // sequences of 16 heads of 128, bf16, 0.52 GB: 6.2 TB/s.)
 // The context of one (sequence, head) is split over the warps of a cluster of
@@ -108,6 +108,11 @@ struct RowsCfg {
 // row's keys differ above bit 0 (V).
 __device__ __forceinline__ int row_key(int r) { return (0x37156240 >> (4 * r)) & 7; }
 
+// The same for bf16 rows that lie one behind the other, an odd number of 32 bytes each:
+// neighbouring rows' keys differ by 2 and every second row's are all different, modulo 4.
+// (Rows of codes, an odd number of 16 bytes, do in their own order.)
+__device__ __forceinline__ int linear_key(int r) { return r & 1 ? ((r >> 1) + 2) % 4 + 4 : r >> 1; }
+
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -138,7 +143,8 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
       : "memory");
 }
 
-template <bool kE4m3, int DP, int NT, int W>
+// kLinear: the rows of a block lie one behind the other, as in the page.
+template <bool kE4m3, int DP, int NT, int W, bool kLinear>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
@@ -236,6 +242,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     bad_page = true;
     return 0;
   };
+  const int pitch = kLinear ? a.d * (kE4m3 ? 1 : 2) : C::kRowBytes;  // of keys in a tile
   auto bring = [&](int block, int stage) {
     if (brought % 32 == 0) hold(block);
     int page0 = __shfl_sync(0xFFFFFFFFu, held0, brought % 32);
@@ -247,9 +254,23 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     page0 = checked(page0);
     if (two) page1 = checked(page1);
     if (lane == 0) {
-      mbar_arrive_expect_tx(bar, (C::kSub == 2 && (two || wide) ? 2u : 1u) * 2 * C::kHalves * C::kBoxBytes);
+      mbar_arrive_expect_tx(bar, (C::kSub == 2 && (two || wide) ? 2u : 1u) * 2 *
+                                     (kLinear ? 16 * pitch : C::kHalves * C::kBoxBytes));
       const int y = key & page_mask;
-      if (C::kSub == 2) {
+      if constexpr (kLinear) {
+        const uint32_t tile = 16 * pitch, bytes = C::kSub == 2 && wide ? 2 * tile : tile;
+        auto rows_of = [&](const void* cache, int page, int at) {
+          return static_cast<const uint8_t*>(cache) +
+                 (page * a.ld_page + ((static_cast<int64_t>(hk) << a.page_log2) + at) * a.d) * (kE4m3 ? 1 : 2);
+        };
+        bulk_load(dst, rows_of(a.k, page0, y), bytes, bar);
+        bulk_load(dst + C::kBoxes * C::kBoxBytes, rows_of(a.v, page0, y), bytes, bar);
+        if (two && !wide) {
+          const int y1 = (key + 16) & page_mask;
+          bulk_load(dst + tile, rows_of(a.k, page1, y1), tile, bar);
+          bulk_load(dst + C::kBoxes * C::kBoxBytes + tile, rows_of(a.v, page1, y1), tile, bar);
+        }
+      } else if (C::kSub == 2) {
         tma_load_rows(dst, &map_k, bar, 0, y, 0, hk, page0);
         tma_load_rows(dst + 2 * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
         if (two && !wide) {
@@ -321,11 +342,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   float v_ref = 0.f, v_mul = 0.f;  // a power of two above the values' scales; kPScale over it
 
   // this lane's keys of a tile: rows g (and g + 8) of K, rows 2 t, 2 t + 1 (and + 8) of V
-  constexpr bool kSwizzled = C::kRowBytes == 128;
-  const int key_g = kSwizzled ? row_key(g) : g;
-  const int key_t[2] = {kSwizzled ? row_key(2 * t) : 2 * t, kSwizzled ? row_key(2 * t + 1) : 2 * t + 1};
+  constexpr bool kSwizzled = C::kRowBytes == 128 && !kLinear;
+  auto key_of = [](int r) { return kSwizzled ? row_key(r) : kLinear && !kE4m3 ? linear_key(r) : r; };
+  const int key_g = key_of(g);
+  const int key_t[2] = {key_of(2 * t), key_of(2 * t + 1)};
+  const int tile_bytes = 16 * pitch;
   auto chunk_at = [&](int key, int chunk) -> uint32_t {  // of a box
-    return key * C::kRowBytes + ((kSwizzled ? chunk ^ (key & 7) : chunk) << 4);
+    return key * pitch + ((kSwizzled ? chunk ^ (key & 7) : chunk) << 4);
   };
 
   int stage = 0, parity = 0;
@@ -340,8 +363,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       if constexpr (kE4m3) {
 #pragma unroll
         for (int c = 0; c < kChunksK; ++c) {
-          const uint4 lo = lds16(kb + u * C::kBoxBytes + chunk_at(key_g, 4 * c + t));
-          const uint4 hi = lds16(kb + u * C::kBoxBytes + chunk_at(key_g + 8, 4 * c + t));
+          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+          if (!kLinear || 16 * (4 * c + t) < a.d) {  // behind a linear row comes the next
+            lo = lds16(kb + u * tile_bytes + chunk_at(key_g, 4 * c + t));
+            hi = lds16(kb + u * tile_bytes + chunk_at(key_g + 8, 4 * c + t));
+          }
           const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -356,9 +382,13 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       } else {
 #pragma unroll
         for (int c = 0; c < kChunksK; ++c) {
-          const uint32_t box = kb + (c >> 1) * C::kBoxBytes;
-          const uint4 lo = lds16(box + chunk_at(key_g, 4 * (c & 1) + t));
-          const uint4 hi = lds16(box + chunk_at(key_g + 8, 4 * (c & 1) + t));
+          const uint32_t box = kLinear ? kb : kb + (c >> 1) * C::kBoxBytes;
+          const int chunk = kLinear ? 4 * c + t : 4 * (c & 1) + t;
+          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+          if (!kLinear || 8 * chunk < a.d) {
+            lo = lds16(box + chunk_at(key_g, chunk));
+            hi = lds16(box + chunk_at(key_g + 8, chunk));
+          }
           const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -481,10 +511,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
         for (int i = 0; i < 4; ++i) {
           const int key = key_t[i & 1] + 8 * (i >> 1);
           if constexpr (kWords == 2) {
-            const uint2 x = lds8(vb + u * C::kBoxBytes + key * C::kRowBytes + 8 * g);
+            const uint2 x = lds8(vb + u * tile_bytes + key * pitch + 8 * g);
             w[i][0] = x.x; w[i][1] = x.y;
           } else {
-            const uint4 x = lds16(vb + (kE4m3 ? u : c) * C::kBoxBytes + chunk_at(key, g));
+            const uint4 x = lds16(vb + (kE4m3 ? u * tile_bytes : kLinear ? c * 128 : c * C::kBoxBytes) +
+                                  chunk_at(key, g));
             w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
           }
           if (edge) {  // keys that some row may not see: their values must not reach it as 0 * NaN
@@ -632,18 +663,18 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   if (cluster > 1) cluster_sync();  // no block leaves while another reads its partial
 }
 
-template <bool kE4m3, int DP, int NT, int W>
+template <bool kE4m3, int DP, int NT, int W, bool kLinear>
 cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStream_t stream) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
-  CUtensorMap mk, mv;
+  CUtensorMap mk{}, mv{};
   // one box where a page holds a whole e4m3 block, or both halves of full bf16 rows
   const bool wide = kE4m3 ? a.page_log2 >= 5 : a.d == 128;
   const int box_rows = kE4m3 && wide ? 32 : 16, box_halves = !kE4m3 && wide ? 2 : 1;
-  if (!make_page_map(&mk, a.k, a, C::kRowBytes, box_rows, box_halves) ||
-      !make_page_map(&mv, a.v, a, C::kRowBytes, box_rows, box_halves))
+  if (!kLinear && (!make_page_map(&mk, a.k, a, C::kRowBytes, box_rows, box_halves) ||
+                   !make_page_map(&mv, a.v, a, C::kRowBytes, box_rows, box_halves)))
     return cudaErrorInvalidValue;
   if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
-  constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W>;
+  constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W, kLinear>;
   if (cudaError_t e = allow_smem_once<kKernel>(C::kSmem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
@@ -668,7 +699,13 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
 // 30000, 8 heads, 8 blocks each: 78 us with 4 warps, 46 with 8), not more: a block of 8
 // fills an SM, and clusters of them do not fit side by side.  (Step: 32 keys of an e4m3
 // cache, 16 of a bf16 one.)
-template <bool kE4m3, int DP, int NT>
+//
+// Where d is an odd number of 16 channels (16, 48, 80, 112) rows can be read out of
+// shared memory without a swizzle as well as with it, so a block of them comes as it lies
+// in the page, in one bulk copy; a tiled copy goes row by row, two requests to a row that
+// crosses 128 bytes (64 sequences up to 2048, 16 heads of 80: e4m3 60 us, 46 so; bf16 63.7
+// and 62.2.  24 up to 1024 with drafts, e4m3: 18.7 and 15.8).
+template <bool kE4m3, int DP, int NT, bool kLinear>
 cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stream) {
   const int64_t sms = device_sm_count();
   const int64_t steps = (static_cast<int64_t>(a.max_pages) << a.page_log2) / (kE4m3 ? 32 : 16);
@@ -679,16 +716,19 @@ cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stre
     cluster *= 2;
   }
   return units * cluster <= sms / 2 && steps >= 8 * cluster
-             ? launch_rows<kE4m3, DP, NT, 8>(a, units, cluster, stream)
-             : launch_rows<kE4m3, DP, NT, 4>(a, units, cluster, stream);
+             ? launch_rows<kE4m3, DP, NT, 8, kLinear>(a, units, cluster, stream)
+             : launch_rows<kE4m3, DP, NT, 4, kLinear>(a, units, cluster, stream);
 }
 
 template <bool kE4m3, int DP>
 cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
   const int64_t heads = static_cast<int64_t>(a.B) * a.H_kv;
-  if (rows <= 8) return launch_rows_cut<kE4m3, DP, 1>(a, heads, stream);
-  return launch_rows_cut<kE4m3, DP, 2>(a, heads, stream);
+  if (a.d % 32 != 0)
+    return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, true>(a, heads, stream)
+                     : launch_rows_cut<kE4m3, DP, 2, true>(a, heads, stream);
+  return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, false>(a, heads, stream)
+                   : launch_rows_cut<kE4m3, DP, 2, false>(a, heads, stream);
 }
 
 }  // namespace
