@@ -131,9 +131,9 @@ constexpr float kPScale = 2048.f;
 
 // A row of Q goes into fp16 times the power of two *up that puts its largest
 // magnitude `top` (f32 bits) in [2^13, 2^14): what falls below fp16's range then is
-// 2^-37 of it.  (2^126 is the largest: rows below 2^-113 come to 2^0 or less, and what is
-// lost of them is 2^-24 of 2^-126.)  Returns the factor of the row's scores (never 0:
-// minus infinity times it has to stay that).
+// 2^-37 of it.  (2^126 is the largest power; smaller rows come out exact with it, bf16
+// being multiples of 2^-133.)  Returns the factor of the row's scores (never 0: minus
+// infinity times it has to stay that).
 __device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, float* up) {
   const int e = top == 0 || top >= 0x7F800000u ? 13 : static_cast<int>(top >> 23) - 127;
   const int n = min(13 - e, 126);

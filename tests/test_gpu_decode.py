@@ -240,6 +240,61 @@ def test_unseen_values_do_not_leak(n, d):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n,heads,d", [(4, 2, 128), (4, 2, 80), (7, 2, 48), (300, 1, 128), (300, 1, 64)])
+def test_unseen_values_of_split_contexts(kind, n, heads, d):
+    """The same where several blocks share the context: a value that is not finite in the middle of
+    the new tokens."""
+    dev = _dev()
+    length = 7000
+    cache = Cache(kind, [length], heads, d, 32, seed=d + n)
+    g = torch.Generator(device=dev).manual_seed(n)
+    q = torch.randn((n, 2 * heads, d), device=dev, generator=g).to(BF16)
+    want, mag = attention_64(q, cache, [0, n])
+    keep = torch.ones(n, 2 * heads, d, dtype=torch.bool, device=dev)
+    at = length - n + n // 2
+    page = cache.table[0, at // 32].long()
+    if kind == "bf16":
+        cache.v[page, 0, at % 32, 5] = -math.inf
+        keep[n // 2:, :2, 5] = False
+    else:
+        cache.v_scale[page, 0, at % 32] = math.nan
+        keep[n // 2:, :2] = False
+    got = attend(cache, q, [n])
+    assert not bool(torch.isfinite(got[~keep]).any())
+    check(torch.where(keep, got, 0).to(BF16), torch.where(keep, want, 0), mag)
+
+
+@pytest.mark.parametrize("n", [1, 5, 70])
+def test_tiny_queries_and_large_keys(n):
+    """Rows of q down to bf16's subnormal numbers against keys whose scales make up for it:
+    the power of two that takes q into 16 bits loses nothing of them."""
+    dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(n)
+    cache = Cache("e4m3", [500, n], 2, 128, 64, seed=6, poison=False)
+    cache.k_scale = cache.k_scale * 2.0 ** 120
+    q = torch.randn((2 * n, 4, 128), device=dev, generator=g)
+    q = (q * torch.exp2(torch.randint(-128, -122, (2 * n, 1, 1), device=dev, generator=g).float())).to(BF16)
+    want, mag = attention_64(q, cache, [0, n, 2 * n], scale=1.0)
+    check(attend(cache, q, [n, n], scale=1.0), want, mag)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("d", [16, 48, 80, 112])
+@pytest.mark.parametrize("page", [16, 64])
+def test_odd_rows_of_strided_pages(kind, d, page):
+    """Rows of an odd number of 16 channels, in pages of a tensor that holds keys and values in turn."""
+    dev = _dev()
+    lengths, new = [1, 33, 700, 47], [1, 3, 2, 8]
+    cache = Cache(kind, lengths, 3, d, page, seed=d)
+    both = torch.stack([cache.k.view(torch.uint8), cache.v.view(torch.uint8)], 1)
+    cache.k, cache.v = (both[:, i].view(cache.k.dtype) for i in range(2))
+    g = torch.Generator(device=dev).manual_seed(page)
+    q = torch.randn((sum(new), 3, d), device=dev, generator=g).to(BF16)
+    want, mag = attention_64(q, cache, starts(new))
+    check(attend(cache, q, new), want, mag)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("n", [1, 9, 140])
 def test_sizes_far_apart(kind, n):
     """Values from 2^-24 to 2^24 and keys from 2^-16 to 1 from one token to the next, rows of q
