@@ -167,12 +167,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   const int split = static_cast<int>(blockIdx.x % cluster);
   const int hk = static_cast<int>(unit % a.H_kv);
   // the longest sequences first
-  __shared__ int costs[kMostRanked], found;
+  __shared__ int costs[kMostRanked], start_of[kMostRanked + 1], found;
   int b = static_cast<int>(unit / a.H_kv);
-  if (a.B > 1 && a.B <= kMostRanked)
+  PagedSeq seq;
+  if (a.B > 1 && a.B <= kMostRanked) {  // what is read for it is not read again
+    for (int i = threadIdx.x; i <= a.B; i += kThreads) start_of[i] = q_start_at(a, i);
     b = ranked(a.B, b, costs, &found, [&](int i) { return __ldg(a.lengths + i); });
-
-  PagedSeq seq = paged_seq(a, b);
+    seq = paged_seq(a, b, start_of[b], start_of[b + 1], costs[b]);
+  } else {
+    seq = paged_seq(a, b);
+  }
   if (seq.bad && hk == 0 && split == 0 && threadIdx.x == 0) paged_report(a.status);
   const int64_t all_rows = static_cast<int64_t>(seq.n) * a.group;
   if (all_rows == 0) return;  // the whole cluster

@@ -45,10 +45,10 @@ __device__ __forceinline__ void paged_report(int32_t* status) {
   if (status != nullptr) atomicCAS(status, 0, 5 /* DWA_ERR_DEVICE_CHECK */);
 }
 
-__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
+// From its number and what q_start and lengths say of it (lo, hi: unless there is no q_start).
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b, int64_t lo, int64_t hi, int length) {
   PagedSeq s;
   if (a.q_start != nullptr) {
-    const int64_t lo = __ldg(a.q_start + b), hi = __ldg(a.q_start + b + 1);
     const bool fine = lo >= 0 && lo <= hi && hi <= a.T;
     s.row0 = fine ? lo : 0;
     s.n = fine ? static_cast<int>(hi - lo) : 0;  // rows that cannot be told apart stay as they are
@@ -58,13 +58,20 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
     s.n = a.even;
     s.bad = false;
   }
-  s.length = __ldg(a.lengths + b);
+  s.length = length;
   if (s.length < 0 || s.length > (static_cast<int64_t>(a.max_pages) << a.page_log2) ||
       s.n > a.max_q) {
     s.bad = true;
     s.length = 0;
   }
   return s;
+}
+
+__device__ __forceinline__ int q_start_at(const PagedArgs& a, int b) {
+  return a.q_start != nullptr ? __ldg(a.q_start + b) : 0;
+}
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
+  return paged_seq(a, b, q_start_at(a, b), q_start_at(a, b + 1), __ldg(a.lengths + b));
 }
 
 // Blocks start in the order of their number, so the ones with the most keys should
