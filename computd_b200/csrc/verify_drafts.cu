@@ -12,9 +12,10 @@
 // and q where a draft fell), 8 V bytes at most: latency for one sequence, HBM
 // for many.  A cluster of blocks shares the row, each warp a contiguous piece;
 // the piece sums go through distributed shared memory, every block finds the
-// piece that holds the draw, and only its warp goes over its piece again.  Eight blocks
-// per sequence: 5.8 us for one (32000 tokens), 14 us for 64 (64400 tokens, 33 MB); with
-// four 7.7 and 17, with two 12 and 28.
+// piece that holds the draw, and only its warp goes over its piece again, to the row of
+// 128 that the draw is in.  Eight blocks per sequence: 5.2 us for one (32000 tokens), 12.3 us
+// for 64 (64400 tokens, 33 MB); with four 7.7 and 17, with two 12 and 28 (against 5.8 and 14
+// then, with every row of the piece scanned).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -104,6 +105,14 @@ __device__ __forceinline__ double ld_cluster_f64(const double* local, int rank) 
   return v;
 }
 
+// The halves of cluster_sync.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kVerifyThreads, 4)
     verify_drafts_kernel(const VerifyArgs a, const int cluster) {
@@ -183,6 +192,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4)
       if (lane >= o) before += y;
     }
     const double total = __shfl_sync(0xFFFFFFFFu, before, 31);
+    if (total > 0.0 || pass == 1) cluster_arrive();  // this warp has read the others' sums
     if (total > 0.0) {
       const double goal = u * total;
       before -= mine0 + mine1;  // within rounding: what this decides is decided once, below
@@ -197,15 +207,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 4)
       double run = __shfl_sync(0xFFFFFFFFu, first ? before : mid, src);
       if (at == rank * kVerifyWarps + warp) {
         mine = true;
-        bool found = false;
-        for (int i0 = lo; i0 < hi && !found; i0 += 128 * kBatch) {
+        // the row (of 128 entries) that the draw is in; where rounding keeps the running sum at
+        // the goal to the end, the last with weight
+        int i = -1;
+        bool in = false;
+        for (int i0 = lo; i0 < hi && !in; i0 += 128 * kBatch) {
           float x[kBatch][4], y[kBatch][4] = {};
           double row[kBatch];
 #pragma unroll
           for (int r = 0; r < kBatch; ++r) {
-            const int i = i0 + 128 * r + 4 * lane;
-            probs4(p, i, hi, a.wide, x[r]);
-            if (q != nullptr) probs4(q, i, hi, a.wide, y[r]);
+            const int k = i0 + 128 * r + 4 * lane;
+            probs4(p, k, hi, a.wide, x[r]);
+            if (q != nullptr) probs4(q, k, hi, a.wide, y[r]);
           }
 #pragma unroll
           for (int r = 0; r < kBatch; ++r) {
@@ -214,38 +227,40 @@ __global__ void __launch_bounds__(kVerifyThreads, 4)
             row[r] = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
           }
 #pragma unroll
-          for (int r = 0; r < kBatch; ++r) {
-            // a row is looked into where the draw is in it, and where it may be the last
-            // with weight: the answer then, where rounding keeps the running sum at the goal
-            if (found || !(row[r] > 0.0)) continue;
-            const int i = i0 + 128 * r + 4 * lane;
-            double w[4];
-            weights4(x[r], y[r], one - i, w);
-            const double four = (w[0] + w[1]) + (w[2] + w[3]);
-            double incl = four;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const double z = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-              if (lane >= o) incl += z;
+          for (int r = 0; r < kBatch; ++r)
+            if (!in && row[r] > 0.0) {
+              i = i0 + 128 * r + 4 * lane;
+              in = run + row[r] > goal;
+              if (!in) run += row[r];
             }
-            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, four > 0.0 && run + incl > goal);
-            const uint32_t any = __ballot_sync(0xFFFFFFFFu, four > 0.0);
-            int j = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;  // the last with weight
-            if (hit) {
-              double c = run + (incl - four);
+        }
+        // in it the first entry whose running sum passes the goal, or the last with weight
+        float x[4], y[4] = {};
+        double w[4];
+        probs4(p, i, hi, a.wide, x);
+        if (q != nullptr) probs4(q, i, hi, a.wide, y);
+        weights4(x, y, one - i, w);
+        const double four = (w[0] + w[1]) + (w[2] + w[3]);
+        double incl = four;
 #pragma unroll
-              for (int k = 2; k >= 0; --k) {
-                double head = c + w[0];
-                if (k > 0) head += w[1];
-                if (k > 1) head += w[2];
-                if (w[k] > 0.0 && head > goal) j = k;
-              }
-            }
-            token = __shfl_sync(0xFFFFFFFFu, i + j, hit ? __ffs(hit) - 1 : 31 - __clz(any));
-            found = hit != 0;
-            run += row[r];
+        for (int o = 1; o < 32; o <<= 1) {
+          const double z = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+          if (lane >= o) incl += z;
+        }
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in && four > 0.0 && run + incl > goal);
+        const uint32_t any = __ballot_sync(0xFFFFFFFFu, four > 0.0);
+        int j = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;  // the last with weight
+        if (hit) {
+          const double c = run + (incl - four);
+#pragma unroll
+          for (int k = 2; k >= 0; --k) {
+            double head = c + w[0];
+            if (k > 0) head += w[1];
+            if (k > 1) head += w[2];
+            if (w[k] > 0.0 && head > goal) j = k;
           }
         }
+        token = __shfl_sync(0xFFFFFFFFu, i + j, hit ? __ffs(hit) - 1 : 31 - __clz(any));
       }
       break;
     }
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4)
     for (int i = lane; i <= K; i += 32)
       a.out_tokens[b * (K + 1) + i] = i < kept ? a.tokens[b * K + i] : i == kept ? token : -1;
   }
-  cluster_sync();  // no block leaves while another reads its sums
+  cluster_wait();  // no block leaves while another reads its sums
 }
 
 }  // namespace
