@@ -13,6 +13,7 @@
 
 #include "dwa_internal.h"
 #include "dwa_retrieval.h"
+#include "f32x2.cuh"
 
 namespace dwa {
 
@@ -103,13 +104,22 @@ __device__ __forceinline__ void store_bf16(const Raw<kBf16, 8>& raw, uint16_t* d
 template <bool kBf16>
 __device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, bool keep, int lanes, int lane,
                                            uint8_t* cache, float* scales, int64_t row, int64_t srow, int d) {
-  float x[16];
-  as_f32(raw, x);
   // The largest magnitude as bits: NaN orders above infinity above every finite number.
   uint32_t top = 0;
   if (on) {
+    if constexpr (kBf16) {  // of both halves at once
+      uint32_t tops = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+      for (int i = 0; i < 2; ++i)
+        tops = __vmaxu2(__vmaxu2(tops, __vmaxu2(raw.w[i].x & 0x7FFF7FFFu, raw.w[i].y & 0x7FFF7FFFu)),
+                        __vmaxu2(raw.w[i].z & 0x7FFF7FFFu, raw.w[i].w & 0x7FFF7FFFu));
+      top = max(tops << 16, tops & 0xFFFF0000u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top = max(max(top, max(raw.w[i].x & 0x7FFFFFFFu, raw.w[i].y & 0x7FFFFFFFu)),
+                  max(raw.w[i].z & 0x7FFFFFFFu, raw.w[i].w & 0x7FFFFFFFu));
+    }
   }
   for (int o = lanes >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if (!keep) return;
@@ -118,6 +128,8 @@ __device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, b
   uint4 w = make_uint4(0, 0, 0, 0);
   float scale = __uint_as_float(0x7FC00000u);
   if (finite) {
+    float x[16];
+    as_f32(raw, x);
     // Tiny vectors are scaled up by 2^100, exactly, so that no remainder underflows: amax is
     // above 2^-70 or the scale above 2^-26 then.  (Remainders of quotients above 2^-11 are
     // above 2^-137; smaller quotients give the code 0 either way.)
@@ -132,8 +144,12 @@ __device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, b
     }
     const float s = fmaxf(quotient(most, 448.f, 1.f / 448.f), least);
     const float y = __frcp_rn(s);
+    const uint64_t y2 = pair(y, y), neg2 = pair(-s, -s);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = quotient(x[i], s, y);
+    for (int i = 0; i < 16; i += 2) {  // as quotient()
+      const uint64_t v = pair(x[i], x[i + 1]), q = mul2(v, y2);
+      unpair(fma2(fma2(q, neg2, v), y2, q), x[i], x[i + 1]);
+    }
     w = codes16(x);  // |x / s| <= 448 (1 + 2^-23), which rounds to 448 at most
     scale = s * down;
   }
