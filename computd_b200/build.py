@@ -98,7 +98,7 @@ def _build_host(verbose: bool) -> None:
                                       torch_dir / "include/torch/csrc/api/include", cuda_inc,
                                       sysconfig.get_paths()["include"])),
            str(HOST_SOURCE), "-o", str(tmp), f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-           "-lc10", "-lc10_cuda"]
+           "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -647,6 +647,36 @@ def verify_64(p, q, x, u, r, lengths):
     return kept_all, rows
 
 
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_outputs_of_their_own(mode):
+    """A call's outputs are contiguous, overlap nothing, and are ordinary tensors of the mode."""
+    import computd_b200 as cb
+
+    dev = _dev()
+    cache = Cache("bf16", [40], 3, 16, 16, seed=2)
+    slots = torch.arange(7, device=dev)
+
+    def same(x, y):  # bit for bit: page 0 is not in use and holds NaN
+        return torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+    probs = torch.full((5, 3, 9), 1 / 9, device=dev)
+    with mode():
+        k, v = cb.kv_cache_read(cache.k, cache.v, slots)
+        n, tokens = cb.verify_drafts(probs, torch.zeros((5, 2), dtype=torch.int32, device=dev), None,
+                                     torch.zeros((5, 2), device=dev), torch.zeros(5, device=dev))
+        o = attend(cache, torch.zeros((1, 3, 16), device=dev, dtype=BF16), [1])
+        for x, y in ((k, v), (tokens, n)):
+            assert x.is_contiguous() and y.is_contiguous() and x.is_inference() == torch.is_inference_mode_enabled()
+            assert y.data_ptr() >= x.data_ptr() + x.numel() * x.element_size()
+            kept = y.clone()
+            x.fill_(1)
+            x.record_stream(torch.cuda.Stream())
+            assert same(y, kept)
+        assert o.shape == (1, 3, 16) and o.is_contiguous() and not o.requires_grad
+        assert k.shape == v.shape == (7, 3, 16) and n.shape == (5,) and tokens.shape == (5, 3)
+        assert same(v, cache.v[0].transpose(0, 1)[:7])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
 @pytest.mark.parametrize("B,K,V", [(1, 4, 32000), (9, 1, 65), (5, 0, 1), (40, 7, 2001), (3, 40, 64400),
                                    (300, 3, 130)])
