@@ -148,7 +148,7 @@ template <bool kE4m3, int DP, int NT, int W, bool kLinear>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
-                      const int cluster, const int wide) {
+                      const int cluster, const int wide, const int rank) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
   constexpr int kWarps = W, kThreads = 32 * W;
   extern __shared__ uint8_t smem_raw[];
@@ -166,11 +166,11 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   const uint32_t unit = blockIdx.x / cluster;  // the grid has 32 bits
   const int split = static_cast<int>(blockIdx.x % cluster);
   const int hk = static_cast<int>(unit % a.H_kv);
-  // the longest sequences first
+  // the longest sequences first, where blocks share SMs or wait for one
   __shared__ int costs[kMostRanked], start_of[kMostRanked + 1], found;
   int b = static_cast<int>(unit / a.H_kv);
   PagedSeq seq;
-  if (a.B > 1 && a.B <= kMostRanked) {  // what is read for it is not read again
+  if (rank && a.B > 1 && a.B <= kMostRanked) {  // what is read for it is not read again
     for (int i = threadIdx.x; i <= a.B; i += kThreads) start_of[i] = q_start_at(a, i);
     b = ranked(a.B, b, costs, &found, [&](int i) { return __ldg(a.lengths + i); });
     seq = paged_seq(a, b, start_of[b], start_of[b + 1], costs[b]);
@@ -691,7 +691,8 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, cluster, wide ? 1 : 0);
+  return cudaLaunchKernelEx(&cfg, kKernel, mk, mv, a, cluster, wide ? 1 : 0,
+                            units * cluster > device_sm_count() ? 1 : 0);
 }
 
 // How a call is cut up: the longest context is split over 2^n blocks of 4 warps
@@ -701,7 +702,9 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
 // block each 212 us, 2 126, 4 132, 8 156; 64 up to 2048, 16 heads, bf16: 83, 97, 128.)
 // What still leaves half the SMs without a block gets 8 warps per block (one sequence of
 // 30000, 8 heads, 8 blocks each: 78 us with 4 warps, 46 with 8), not more: a block of 8
-// fills an SM, and clusters of them do not fit side by side.  (Step: 32 keys of an e4m3
+// fills an SM, and clusters of them do not fit side by side.  Two blocks of 4 warps become one
+// of 8 where every SM has at most one then: no cluster to join, no order to find (16 sequences
+// up to 256, 6 heads of 64: 5.8 us, 4.9 so; 32 of 512, 4 heads of 128, e4m3: 9.1, 7.9).  (Step: 32 keys of an e4m3
 // cache, 16 of a bf16 one.)
 //
 // Where d is an odd number of 16 channels (16, 48, 80, 112) rows can be read out of
@@ -719,6 +722,8 @@ cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stre
     if (!(blocks < 2 * sms ? per_warp >= 2 : blocks < 3 * sms && per_warp >= 8)) break;
     cluster *= 2;
   }
+  if (cluster == 2 && units <= sms && 2 * units > sms / 2)
+    return launch_rows<kE4m3, DP, NT, 8, kLinear>(a, units, 1, stream);
   return units * cluster <= sms / 2 && steps >= 8 * cluster
              ? launch_rows<kE4m3, DP, NT, 8, kLinear>(a, units, cluster, stream)
              : launch_rows<kE4m3, DP, NT, 4, kLinear>(a, units, cluster, stream);
