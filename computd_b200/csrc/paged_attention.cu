@@ -704,8 +704,8 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
 // 30000, 8 heads, 8 blocks each: 78 us with 4 warps, 46 with 8), not more: a block of 8
 // fills an SM, and clusters of them do not fit side by side.  Two blocks of 4 warps become one
 // of 8 where every SM has at most one then: no cluster to join, no order to find (16 sequences
-// up to 256, 6 heads of 64: 5.8 us, 4.9 so; 32 of 512, 4 heads of 128, e4m3: 9.1, 7.9).  (Step: 32 keys of an e4m3
-// cache, 16 of a bf16 one.)
+// up to 256, 6 heads of 64: 5.8 us, 4.9 so; 32 of 512, 4 heads of 128, e4m3: 9.1, 7.9).
+// (Step: 32 keys of an e4m3 cache, 16 of a bf16 one.)
 //
 // Where d is an odd number of 16 channels (16, 48, 80, 112) rows can be read out of
 // shared memory without a swizzle as well as with it, so a block of them comes as it lies

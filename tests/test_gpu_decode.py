@@ -240,6 +240,22 @@ def test_unseen_values_do_not_leak(n, d):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("n", [1, 3, 10])
+@pytest.mark.parametrize("B,heads,d,longest", [(20, 4, 64, 256), (20, 4, 128, 512), (40, 8, 64, 300),
+                                               (130, 2, 80, 200)])
+def test_many_ragged_sequences(kind, n, B, heads, d, longest):
+    """Every SM with one block, and with several that start longest first (or, for more sequences
+    than are ranked, in their own order); lengths from nothing to `longest`."""
+    dev = _dev()
+    lengths = [(37 * b * b + 11 * b) % (longest + 1) for b in range(B - 1)] + [longest]
+    cache = Cache(kind, lengths, heads, d, 32, seed=B + d)
+    g = torch.Generator(device=dev).manual_seed(n)
+    q = torch.randn((n * B, heads, d), device=dev, generator=g).to(BF16)
+    want, mag = attention_64(q, cache, starts([n] * B))
+    check(attend(cache, q, [n] * B), want, mag)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("n,heads,d", [(4, 2, 128), (4, 2, 80), (7, 2, 48), (300, 1, 128), (300, 1, 64)])
 def test_unseen_values_of_split_contexts(kind, n, heads, d):
     """The same where several blocks share the context: a value that is not finite in the middle of
