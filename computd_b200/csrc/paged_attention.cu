@@ -358,7 +358,15 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   int stage = 0, parity = 0;
   for (; block < n_blocks; block += step) {
     const int key0 = block * C::kKeys;
-    if (!mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr)) { bad_page = true; break; }
+    if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr))) {
+      // given up, by the whole warp: NaN, once the copies in flight have had as long again
+      bad_page = true;
+      for (int i = 0; i < C::kStages; ++i) {
+        if (block + i * step < n_blocks) mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr);
+        if (++stage == C::kStages) { stage = 0; parity ^= 1; }
+      }
+      break;
+    }
     const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kBoxes * C::kBoxBytes;
     // two sums per score: half the chain of dependent products
     float s[C::kSub][NT][4] = {}, s2[C::kSub][NT][4] = {};
