@@ -24,12 +24,14 @@
 // bf16 caches: P is used as the sum of two bf16 parts, so that only the result's
 // rounding is left.  e4m3 caches: codes become fp16 exactly, Q is scaled per row by
 // a power of two into fp16 (a part below 2^-37 of its largest is lost), the keys' scales multiply the scores,
-// and P times the values' scales, relative to a running power of two, is rounded to
-// fp16 (2^-11).
+// and P times the values' scales, relative to a power of two of the row's own, is rounded
+// to fp16 (2^-11).  (Relative to one above every value's scale, a row loses its bits to
+// values that it may not see, or sees without weight.)
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "dwa_internal.h"
 #include "paged_attention.cuh"
@@ -343,7 +345,15 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   float m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) { m[nt][0] = m[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f; }
-  float v_ref = 0.f, v_mul = 0.f;  // a power of two above the values' scales; kPScale over it
+  // e4m3: a column's o is in units of 2^(m + v_exp) / kPScale.  One v_exp, found in the first
+  // block, serves all columns while the values' scales stay between v_low and v_high (the
+  // loop's first form).  From the first block on where they do not, each column has its own, and
+  // v_room says how far m has risen since a weight set it: so much lower it still holds every
+  // weight so far (the second form: 12 rows over 1024 keys of 24 sequences, 16 heads of 80, 57
+  // us instead of 45; 64 sequences of 2048, 16 heads of 128, 101 instead of 97).
+  int v_exp[NT][2], v_all = 0;
+  float v_room[NT][2];
+  float v_mul = 0.f, v_low = 0.f, v_high = 0.f;
 
   // this lane's keys of a tile: rows g (and g + 8) of K, rows 2 t, 2 t + 1 (and + 8) of V
   constexpr bool kSwizzled = C::kRowBytes == 128 && !kLinear;
@@ -356,225 +366,288 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   };
 
   int stage = 0, parity = 0;
-  for (; block < n_blocks; block += step) {
-    const int key0 = block * C::kKeys;
-    if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr))) {
-      // given up, by the whole warp: NaN, once the copies in flight have had as long again
-      bad_page = true;
-      for (int i = 0; i < C::kStages; ++i) {
-        if (block + i * step < n_blocks) mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr);
-        if (++stage == C::kStages) { stage = 0; parity ^= 1; }
+  // Whether the rest is for the second form.
+  auto go = [&](auto apart_) -> bool {
+    constexpr bool kApart = decltype(apart_)::value;
+    for (; block < n_blocks; block += step) {
+      const int key0 = block * C::kKeys;
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr))) {
+        // given up, by the whole warp: NaN, once the copies in flight have had as long again
+        bad_page = true;
+        for (int i = 0; i < C::kStages; ++i) {
+          if (block + i * step < n_blocks) mbar_wait(bar0 + 8 * stage, parity, a.status, nullptr);
+          if (++stage == C::kStages) { stage = 0; parity ^= 1; }
+        }
+        return false;
       }
-      break;
-    }
-    const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kBoxes * C::kBoxBytes;
-    // two sums per score: half the chain of dependent products
-    float s[C::kSub][NT][4] = {}, s2[C::kSub][NT][4] = {};
+      const uint32_t kb = ring + stage * C::kStageBytes, vb = kb + C::kBoxes * C::kBoxBytes;
+      // two sums per score: half the chain of dependent products
+      float s[C::kSub][NT][4] = {}, s2[C::kSub][NT][4] = {};
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u) {
-      if constexpr (kE4m3) {
+      for (int u = 0; u < C::kSub; ++u) {
+        if constexpr (kE4m3) {
 #pragma unroll
-        for (int c = 0; c < kChunksK; ++c) {
-          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-          if (!kLinear || 16 * (4 * c + t) < a.d) {  // behind a linear row comes the next
-            lo = lds16(kb + u * tile_bytes + chunk_at(key_g, 4 * c + t));
-            hi = lds16(kb + u * tile_bytes + chunk_at(key_g + 8, 4 * c + t));
-          }
-          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t f[4] = {e4m3x2_f16x2(wl[i], 0), e4m3x2_f16x2(wh[i], 0),
-                                   e4m3x2_f16x2(wl[i], 1), e4m3x2_f16x2(wh[i], 1)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816<true>(i & 1 ? s2[u][nt] : s[u][nt], f, qf[nt][4 * c + i][0],
-                             qf[nt][4 * c + i][1]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kChunksK; ++c) {
-          const uint32_t box = kLinear ? kb : kb + (c >> 1) * C::kBoxBytes;
-          const int chunk = kLinear ? 4 * c + t : 4 * (c & 1) + t;
-          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-          if (!kLinear || 8 * chunk < a.d) {
-            lo = lds16(box + chunk_at(key_g, chunk));
-            hi = lds16(box + chunk_at(key_g + 8, chunk));
-          }
-          const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma16816<false>(s[u][nt], f0, qf[nt][2 * c][0], qf[nt][2 * c][1]);
-            mma16816<false>(s2[u][nt], f1, qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
-          }
-        }
-      }
-    }
-    const bool edge = key0 + C::kKeys > vis_min;
-    float sk[C::kSub][2], sv[C::kSub][2];
-    bool v_up = false;
-    if constexpr (kE4m3) {
-#pragma unroll
-      for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          sk[u][i] = scales[warp][stage][0][16 * u + 8 * i + key_g];
-          sv[u][i] = scales[warp][stage][1][16 * u + 8 * i + key_g];
-          if (edge && key0 + 16 * u + 8 * i + key_g >= vis_max) sv[u][i] = 0.f;
-          v_up = v_up || sv[u][i] > v_ref;
-        }
-    }
-    float v_shrink = 1.f;
-    if (kE4m3 && __any_sync(0xFFFFFFFFu, v_up)) {
-      float top = 0.f;  // of the numbers among the scales
-#pragma unroll
-      for (int u = 0; u < C::kSub; ++u) top = fmaxf(top, fmaxf(sv[u][0], sv[u][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-      const float up = power_above(top);
-      v_shrink = v_ref == 0.f ? 0.f : v_ref / up;
-      v_ref = up;
-      v_mul = kPScale / up;
-    }
-
-    // scores in units of log2, masked; the columns' maxima over the block
-    bool moved = kE4m3 && v_shrink != 1.f;
-    float shrink[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float top = m[nt][j];
-#pragma unroll
-        for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float x = (s[u][nt][2 * i + j] + s2[u][nt][2 * i + j]) *
-                      (kE4m3 ? sk[u][i] * factor[nt][j] : factor[nt][j]);
-            if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) x = -INFINITY;
-            s[u][nt][2 * i + j] = x;
-            top = fmaxf(top, x);
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-        const float was = m[nt][j];
-        shrink[nt][j] = 1.f;
-        if (top > was) {
-          shrink[nt][j] = was == -INFINITY ? 0.f : fast_exp2(was - top);
-          m[nt][j] = top;
-          moved = true;
-        }
-        const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-        float sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float p = fast_exp2(s[u][nt][2 * i + j] - ref);
-            sum += p;
-            if constexpr (kE4m3) {
-              p *= sv[u][i] * v_mul;
-              // a masked key's scale may be anything: its weight is 0, not 0 times that
-              if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) p = 0.f;
+          for (int c = 0; c < kChunksK; ++c) {
+            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+            if (!kLinear || 16 * (4 * c + t) < a.d) {  // behind a linear row comes the next
+              lo = lds16(kb + u * tile_bytes + chunk_at(key_g, 4 * c + t));
+              hi = lds16(kb + u * tile_bytes + chunk_at(key_g + 8, 4 * c + t));
             }
-            s[u][nt][2 * i + j] = p;
-          }
-        l[nt][j] = l[nt][j] * shrink[nt][j] + sum;
-      }
-    uint32_t pb[C::kSub][NT][2], pl[C::kSub][NT][2];
+            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u)
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t f[4] = {e4m3x2_f16x2(wl[i], 0), e4m3x2_f16x2(wh[i], 0),
+                                     e4m3x2_f16x2(wl[i], 1), e4m3x2_f16x2(wh[i], 1)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<true>(i & 1 ? s2[u][nt] : s[u][nt], f, qf[nt][4 * c + i][0],
+                               qf[nt][4 * c + i][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kChunksK; ++c) {
+            const uint32_t box = kLinear ? kb : kb + (c >> 1) * C::kBoxBytes;
+            const int chunk = kLinear ? 4 * c + t : 4 * (c & 1) + t;
+            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+            if (!kLinear || 8 * chunk < a.d) {
+              lo = lds16(box + chunk_at(key_g, chunk));
+              hi = lds16(box + chunk_at(key_g + 8, chunk));
+            }
+            const uint32_t f0[4] = {lo.x, hi.x, lo.y, hi.y}, f1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<false>(s[u][nt], f0, qf[nt][2 * c][0], qf[nt][2 * c][1]);
+              mma16816<false>(s2[u][nt], f1, qf[nt][2 * c + 1][0], qf[nt][2 * c + 1][1]);
+            }
+          }
+        }
+      }
+      const bool edge = key0 + C::kKeys > vis_min;
+      float sk[C::kSub][2], sv[C::kSub][2];
+      if constexpr (kE4m3) {
+        float top = 0.f, low = INFINITY;  // of the values' scales that are numbers, and not 0
+#pragma unroll
+        for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sk[u][i] = scales[warp][stage][0][16 * u + 8 * i + key_g];
+            sv[u][i] = scales[warp][stage][1][16 * u + 8 * i + key_g];
+            if (edge && key0 + 16 * u + 8 * i + key_g >= vis_max) sv[u][i] = 0.f;
+            const float x = fabsf(sv[u][i]);
+            top = fmaxf(top, x);
+            low = fminf(low, x == 0.f ? INFINITY : x);
+          }
+        if (!kApart && __any_sync(0xFFFFFFFFu, top > v_high || low < v_low)) {
+          if (v_mul == 0.f) {  // the first block
+            float most = top < INFINITY ? top : 0.f;
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 4));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 8));
+            most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 16));
+            v_all = max(exponent_above(most) + 11, kLeastExp);
+            v_mul = exp_scale(v_all);
+            v_low = kLowWeight / v_mul;
+            v_high = kMostWeight / v_mul;
+          }
+          // (every row's key of its m has had a weight of kLowWeight or more so far: no room)
+          if (__any_sync(0xFFFFFFFFu, top > v_high || low < v_low)) return true;
+        }
+      }
+
+      // scores in units of log2, masked; the columns' maxima over the block
+      bool moved = false;
+      float shrink[NT][2], rise[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float p0 = s[u][nt][2 * i], p1 = s[u][nt][2 * i + 1];
-          if constexpr (kE4m3) {
-            pb[u][nt][i] = transpose8x8(pack_f16(p0, p1));
-          } else {
-            const uint32_t big = pack_bf16(p0, p1);
-            pb[u][nt][i] = transpose8x8(big);
-            pl[u][nt][i] = transpose8x8(pack_bf16(p0 - __uint_as_float(big << 16),
-                                                  p1 - __uint_as_float(big & 0xFFFF0000u)));
+        for (int j = 0; j < 2; ++j) {
+          float top = m[nt][j];
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float x = (s[u][nt][2 * i + j] + s2[u][nt][2 * i + j]) *
+                        (kE4m3 ? sk[u][i] * factor[nt][j] : factor[nt][j]);
+              if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) x = -INFINITY;
+              s[u][nt][2 * i + j] = x;
+              top = fmaxf(top, x);
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+          const float was = m[nt][j];
+          shrink[nt][j] = 1.f;
+          rise[nt][j] = 0.f;
+          if (top > was) {
+            shrink[nt][j] = was == -INFINITY ? 0.f : fast_exp2(was - top);
+            m[nt][j] = top;
+            moved = true;
+            rise[nt][j] = top - was;
+          }
+          const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+          float sum = 0.f;
+#pragma unroll
+          for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float p = fast_exp2(s[u][nt][2 * i + j] - ref);
+              sum += p;
+              if constexpr (kE4m3) {
+                if (!kApart) p *= sv[u][i] * v_mul;
+                // a masked key's scale may be anything: its weight is 0, not 0 times that
+                if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) p = 0.f;
+              }
+              s[u][nt][2 * i + j] = p;
+            }
+          l[nt][j] = l[nt][j] * shrink[nt][j] + sum;
+        }
+      if constexpr (kApart) {
+#pragma unroll
+        for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sv[u][i] = fmaf(sv[u][i], 0.f, sv[u][i]);  // an infinity becomes NaN
+        auto weight = [&](int u, int nt, int i, int j) -> float {
+          const float x = s[u][nt][2 * i + j] * exp_scale(v_exp[nt][j]) * sv[u][i];
+          return edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j] ? 0.f : x;
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            v_room[nt][j] = rise[nt][j] == INFINITY ? kAllRoom : v_room[nt][j] + rise[nt][j];
+            for (int tries = 0; tries < 4; ++tries) {  // of an infinite weight only that it is too large is known
+              float top = 0.f;
+#pragma unroll
+              for (int u = 0; u < C::kSub; ++u)
+                top = fmaxf(top, fmaxf(fabsf(weight(u, nt, 0, j)), fabsf(weight(u, nt, 1, j))));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+              int up = 0;
+              if (top > kMostWeight) {
+                up = exponent_above(top);
+                v_room[nt][j] = 0.f;
+              } else if (top < kLowWeight && top > 0.f) {
+                up = -min(min(static_cast<int>(v_room[nt][j]), v_exp[nt][j] - kLeastExp), -exponent_above(top));
+                v_room[nt][j] += static_cast<float>(up);
+              }
+              v_exp[nt][j] += up;
+              const float f0 = pow2(-(up / 2)), f1 = pow2(-(up - up / 2));
+#pragma unroll
+              for (int k = 0; k < C::kSteps; ++k) {
+                o[nt][k][j] = o[nt][k][j] * f0 * f1;
+                o[nt][k][2 + j] = o[nt][k][2 + j] * f0 * f1;
+              }
+              if (!__any_sync(0xFFFFFFFFu, top == INFINITY)) break;
+            }
+            if (v_room[nt][j] > 0.5f * kAllRoom) v_room[nt][j] = 0.f;
+#pragma unroll
+            for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) s[u][nt][2 * i + j] = weight(u, nt, i, j);
+          }
+      }
+      uint32_t pb[C::kSub][NT][2], pl[C::kSub][NT][2];
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float p0 = s[u][nt][2 * i], p1 = s[u][nt][2 * i + 1];
+            if constexpr (kE4m3) {
+              pb[u][nt][i] = transpose8x8(pack_f16(p0, p1));
+            } else {
+              const uint32_t big = pack_bf16(p0, p1);
+              pb[u][nt][i] = transpose8x8(big);
+              pl[u][nt][i] = transpose8x8(pack_bf16(p0 - __uint_as_float(big << 16),
+                                                    p1 - __uint_as_float(big & 0xFFFF0000u)));
+            }
+          }
+      if (__any_sync(0xFFFFFFFFu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = shrink[nt][0], f1 = shrink[nt][1];
+#pragma unroll
+          for (int k = 0; k < C::kSteps; ++k) {
+            o[nt][k][0] *= f0; o[nt][k][1] *= f1;
+            o[nt][k][2] *= f0; o[nt][k][3] *= f1;
           }
         }
-    if (__any_sync(0xFFFFFFFFu, moved)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float f0 = shrink[nt][0] * v_shrink, f1 = shrink[nt][1] * v_shrink;
-#pragma unroll
-        for (int k = 0; k < C::kSteps; ++k) {
-          o[nt][k][0] *= f0; o[nt][k][1] *= f1;
-          o[nt][k][2] *= f0; o[nt][k][3] *= f1;
-        }
       }
+      // 16 bytes (8 for e4m3 at 64 channels) of four keys' values at a time
+      constexpr int kPieces = kE4m3 ? 1 : DP / 64;
+      constexpr int kWords = kE4m3 && DP == 64 ? 2 : 4;
+#pragma unroll
+      for (int u = 0; u < C::kSub; ++u)
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key_t[i & 1] + 8 * (i >> 1);
+            if constexpr (kWords == 2) {
+              const uint2 x = lds8(vb + u * tile_bytes + key * pitch + 8 * g);
+              w[i][0] = x.x; w[i][1] = x.y;
+            } else {
+              const uint4 x = lds16(vb + (kE4m3 ? u * tile_bytes : kLinear ? c * 128 : c * C::kBoxBytes) +
+                                    chunk_at(key, g));
+              w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+            }
+            if (edge) {  // keys that some row may not see: their values must not reach it as 0 * NaN
+              const int at = key0 + 16 * u + key;
+#pragma unroll
+              for (int k = 0; k < kWords; ++k) {
+                const int ch = 8 * (8 * c + g) + 2 * k;
+                if (at >= vis_max) w[i][k] = 0;
+                else if (!kE4m3 && at >= vis_min)
+                  w[i][k] = only_finite(w[i][k], at, &first_bad[ch], &first_bad[ch + 1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) {
+            if constexpr (kE4m3) {
+              // both keys' codes of a channel side by side, then four codes to fp16
+              const uint32_t a01 = __byte_perm(w[0][k], w[1][k], 0x5140);
+              const uint32_t b01 = __byte_perm(w[2][k], w[3][k], 0x5140);
+              const uint32_t a23 = __byte_perm(w[0][k], w[1][k], 0x7362);
+              const uint32_t b23 = __byte_perm(w[2][k], w[3][k], 0x7362);
+              const uint32_t f0[4] = {e4m3x2_f16x2(a01, 0), e4m3x2_f16x2(a01, 1),
+                                      e4m3x2_f16x2(b01, 0), e4m3x2_f16x2(b01, 1)};
+              const uint32_t f1[4] = {e4m3x2_f16x2(a23, 0), e4m3x2_f16x2(a23, 1),
+                                      e4m3x2_f16x2(b23, 0), e4m3x2_f16x2(b23, 1)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<true>(o[nt][2 * k], f0, pb[u][nt][0], pb[u][nt][1]);
+                mma16816<true>(o[nt][2 * k + 1], f1, pb[u][nt][0], pb[u][nt][1]);
+              }
+            } else {
+              const uint32_t f[4] = {
+                  __byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                  __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(o[nt][4 * c + k], f, pb[u][nt][0], pb[u][nt][1]);
+                mma16816<false>(o[nt][4 * c + k], f, pl[u][nt][0], pl[u][nt][1]);
+              }
+            }
+          }
+        }
+      __syncwarp();  // every lane has read the stage
+      const int ahead = block + C::kStages * step;
+      if (ahead < n_blocks) bring(ahead, stage);
+      if (++stage == C::kStages) { stage = 0; parity ^= 1; }
     }
-    // 16 bytes (8 for e4m3 at 64 channels) of four keys' values at a time
-    constexpr int kPieces = kE4m3 ? 1 : DP / 64;
-    constexpr int kWords = kE4m3 && DP == 64 ? 2 : 4;
+    return false;
+  };
+  const bool more = go(std::false_type{});
 #pragma unroll
-    for (int u = 0; u < C::kSub; ++u)
-#pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        uint32_t w[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = key_t[i & 1] + 8 * (i >> 1);
-          if constexpr (kWords == 2) {
-            const uint2 x = lds8(vb + u * tile_bytes + key * pitch + 8 * g);
-            w[i][0] = x.x; w[i][1] = x.y;
-          } else {
-            const uint4 x = lds16(vb + (kE4m3 ? u * tile_bytes : kLinear ? c * 128 : c * C::kBoxBytes) +
-                                  chunk_at(key, g));
-            w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
-          }
-          if (edge) {  // keys that some row may not see: their values must not reach it as 0 * NaN
-            const int at = key0 + 16 * u + key;
-#pragma unroll
-            for (int k = 0; k < kWords; ++k) {
-              const int ch = 8 * (8 * c + g) + 2 * k;
-              if (at >= vis_max) w[i][k] = 0;
-              else if (!kE4m3 && at >= vis_min)
-                w[i][k] = only_finite(w[i][k], at, &first_bad[ch], &first_bad[ch + 1]);
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-          if constexpr (kE4m3) {
-            // both keys' codes of a channel side by side, then four codes to fp16
-            const uint32_t a01 = __byte_perm(w[0][k], w[1][k], 0x5140);
-            const uint32_t b01 = __byte_perm(w[2][k], w[3][k], 0x5140);
-            const uint32_t a23 = __byte_perm(w[0][k], w[1][k], 0x7362);
-            const uint32_t b23 = __byte_perm(w[2][k], w[3][k], 0x7362);
-            const uint32_t f0[4] = {e4m3x2_f16x2(a01, 0), e4m3x2_f16x2(a01, 1),
-                                    e4m3x2_f16x2(b01, 0), e4m3x2_f16x2(b01, 1)};
-            const uint32_t f1[4] = {e4m3x2_f16x2(a23, 0), e4m3x2_f16x2(a23, 1),
-                                    e4m3x2_f16x2(b23, 0), e4m3x2_f16x2(b23, 1)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<true>(o[nt][2 * k], f0, pb[u][nt][0], pb[u][nt][1]);
-              mma16816<true>(o[nt][2 * k + 1], f1, pb[u][nt][0], pb[u][nt][1]);
-            }
-          } else {
-            const uint32_t f[4] = {
-                __byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
-                __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<false>(o[nt][4 * c + k], f, pb[u][nt][0], pb[u][nt][1]);
-              mma16816<false>(o[nt][4 * c + k], f, pl[u][nt][0], pl[u][nt][1]);
-            }
-          }
-        }
-      }
-    __syncwarp();  // every lane has read the stage
-    const int ahead = block + C::kStages * step;
-    if (ahead < n_blocks) bring(ahead, stage);
-    if (++stage == C::kStages) { stage = 0; parity ^= 1; }
+  for (int nt = 0; nt < NT; ++nt) {
+    v_exp[nt][0] = v_exp[nt][1] = v_all;
+    v_room[nt][0] = v_room[nt][1] = 0.f;
   }
+  if (kE4m3 && more) go(std::bool_constant<kE4m3>{});
   if (__any_sync(0xFFFFFFFFu, bad_page)) {
     if (lane == 0) paged_report(a.status);
 #pragma unroll
@@ -583,7 +656,6 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   __syncthreads();  // the rings' place is the partials' now
 
   // this warp's partial
-  const float v_back = kE4m3 ? v_ref / kPScale : 1.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -593,6 +665,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
       x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
       const int r = 8 * nt + 2 * t + j;
+      const float v_back = kE4m3 ? 1.f / exp_scale(v_exp[nt][j]) : 1.f;
       if (g == 0) {
         part_m[warp][r] = m[nt][j];
         part_l[warp][r] = x;

@@ -132,9 +132,21 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int high) {
   return r;
 }
 
-// e4m3 caches: P times a value's scale over a running power of two, times this,
-// stays below 65504 with P up to 2^4, and keeps fp16's 11 bits down to 2^-25.
-constexpr float kPScale = 2048.f;
+// e4m3 caches: a code's weight in its row is its probability p <= 1 times its value's scale,
+// in units of 2^v_exp / kPScale, chosen so that the row's largest weight lies between
+// kLowWeight and kMostWeight: fp16 holds 11 bits of everything down to 2^-20 of it then.
+constexpr float kPScale = 2048.f, kMostWeight = 32768.f, kLowWeight = 64.f;
+constexpr int kLeastExp = -110;    // a scale of 2^-126 still makes 2^-5
+constexpr float kAllRoom = 0x1p30f;  // of a row without weights so far
+__device__ __forceinline__ float pow2(int n) {  // -126 to 127
+  return __uint_as_float(static_cast<uint32_t>(127 + n) << 23);
+}
+// kPScale / 2^v_exp: v_exp is at most 127
+__device__ __forceinline__ float exp_scale(int v_exp) { return pow2(11 - v_exp); }
+// How far a unit has to rise so that weight x lies between 2^11 and 2^12 (an infinite one: 117).
+__device__ __forceinline__ int exponent_above(float x) {
+  return static_cast<int>(__float_as_uint(x) >> 23) - 127 - 11;
+}
 
 // A row of Q goes into fp16 times the power of two *up that puts its largest
 // magnitude `top` (f32 bits) in [2^13, 2^14): what falls below fp16's range then is
