@@ -785,7 +785,12 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     const int vis = live ? paged_visible(seq, row_token(row0 + r, a.group)) : 0;
     // least visible count in the warp: steps below it need no mask
     const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
-    float m = -INFINITY, l = 0.f, v_ref = 0.f;
+    // P = exp2(x + ref), l its sum: ref is -m, and kPBits more where that is exact enough (P up
+    // to 2^(11 + kSlack) is a number of fp16, 2^(16 + kSlack) is not)
+    auto ref_of = [](float top) -> float {
+      return top == -INFINITY ? 0.f : kE4m3 && fabsf(top) < 0x1p22f ? kPBits - top : -top;
+    };
+    float m = -INFINITY, l = 0.f, v_ref = 0.f, ref = 0.f;
     bool alive = true;
     for (int j = 0; j < steps; ++j) {
       if (!warp_wait(sh.s_ready[i], j)) { alive = false; break; }
@@ -833,15 +838,26 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       }
       const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
       const bool move = most > m + kSlack || (m == -INFINITY && most > m) || v_now != v_ref;
-      if (__any_sync(0xFFFFFFFFu, move)) {
-        const float m_new = fmaxf(m, most);
-        const float shrink = m == -INFINITY ? 0.f : fast_exp2(m - m_new);
+      const bool big = fabsf(most) >= 0x1p20f && fabsf(most) < INFINITY;
+      if (__any_sync(0xFFFFFFFFu, move || big)) {
+        // The product s factor is not rounded before ref is added to it below, most is: where
+        // scores are big the difference would count.
+        if (__any_sync(0xFFFFFFFFu, big)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * factor);
+          factor = 1.f;
+        }
+        const float m_new = fmaxf(m, most), ref_new = ref_of(m_new);
+        const float shrink = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);
         float shrink_o = shrink;
         if constexpr (kE4m3) {
           shrink_o = v_ref == 0.f ? 0.f : shrink * (v_ref / v_now);
           v_ref = v_now;
         }
         m = m_new;
+        ref = ref_new;
         l *= shrink;
         if (j > 0) {
           if (!warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
@@ -850,8 +866,6 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, shrink_o);
         }
       }
-      // fp16: P times kPScale, and l with it
-      const float ref = (m == -INFINITY ? 0.f : -m) + (kE4m3 ? kPBits : 0.f);
       const uint64_t factor2 = pair(factor, factor), ref2 = pair(ref, ref);
       uint64_t l2[2] = {0, 0};
       auto half = [&](int h) {
@@ -961,7 +975,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
                              o[k + 3] * v_back);
         }
       }
-      st_cluster_f32x2(there + C::kPartMl + 8 * slot, m, l);
+      st_cluster_f32x2(there + C::kPartMl + 8 * slot, m == -INFINITY ? m : -ref, l);
       if (sh.any_bad) {
         for (int at = threadIdx.x; at < cluster * kMaxChannels; at += 256)
           min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kMaxChannels]), at / kMaxChannels),

@@ -27,6 +27,7 @@ def _queries(n, heads, d, seed):
 
 # (new tokens, heads, heads of the cache): a few rows per head, two column tiles of them
 FORMS = [(2, 4, 2), (9, 2, 2)]
+ALL_FORMS = FORMS + [(140, 2, 2)]  # and many
 
 
 @pytest.mark.parametrize("new,heads,kv_heads", FORMS)
@@ -134,14 +135,18 @@ def test_hidden_scales_that_are_not_finite(new, heads, kv_heads, bad, what):
         assert not bool(torch.isfinite(got[-1]).any())
 
 
-@pytest.mark.parametrize("new,heads,kv_heads", FORMS)
-@pytest.mark.parametrize("log2", [20, 23])
-def test_large_scores(new, heads, kv_heads, log2):
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("length", [0, 1000])
+@pytest.mark.parametrize("new,heads,kv_heads", ALL_FORMS)
+@pytest.mark.parametrize("log2", [20, 23, 27, 60])
+def test_large_scores(new, heads, kv_heads, log2, length, kind):
     """Scores of 2^log2 and more, whose steps in f32 are a good part of 1: the outputs are those
-    of one key each, with no error but its value's and the result's rounding."""
-    lengths = [new + 120]
-    cache = Cache("e4m3", lengths, kv_heads, 64, 32, seed=new)
-    cache.v_scale *= torch.exp2(torch.arange(32, device="cuda") % 7 - 3.0)
+    of one key each, with no error but its value's and the result's rounding.  (1000 keys more:
+    over several blocks.)"""
+    lengths = [new + 120 + length]
+    cache = Cache(kind, lengths, kv_heads, 64, 32, seed=new)
+    if kind == "e4m3":
+        cache.v_scale *= torch.exp2(torch.arange(32, device="cuda") % 7 - 3.0)
     q = (_queries(new, heads, 64, seed=6).float() * 2.0 ** log2).to(BF16)
     # only rows with a clear winner: by 2^-8 of the largest score, far beyond the sums' error
     k, _ = cache.dense(0)
@@ -149,7 +154,7 @@ def test_large_scores(new, heads, kv_heads, log2):
     see = torch.arange(lengths[0], device="cuda") < (lengths[0] - new + 1 + torch.arange(new, device="cuda"))[:, None]
     top = s.masked_fill(~see[:, None], -math.inf).topk(2, -1).values
     clear = top[..., 0] - top[..., 1] > 2.0 ** -8 * s.abs().amax(-1)
-    assert float(clear.float().mean()) > 0.8
+    assert float(clear.float().mean()) > 0.7
     want, mag = attention_64(q, cache, [0, new])
     got = attend(cache, q, [new])
     check(got[clear], want[clear], mag[clear])
