@@ -143,6 +143,18 @@ __device__ __forceinline__ float pow2(int n) {  // -126 to 127
 }
 // kPScale / 2^v_exp: v_exp is at most 127
 __device__ __forceinline__ float exp_scale(int v_exp) { return pow2(11 - v_exp); }
+// A scale as m 2^e, exactly, with 1 <= |m| < 2 (smaller for subnormal numbers); what is not
+// finite becomes NaN.  Returns m.
+__device__ __forceinline__ float scale_parts(float x, int* e) {
+  const uint32_t w = __float_as_uint(x), field = (w >> 23) & 0xFFu;
+  *e = field == 0u || field == 0xFFu ? -126 : static_cast<int>(field) - 127;
+  return field == 0u      ? x * 0x1p126f
+         : field == 0xFFu ? __uint_as_float(0x7FC00000u)
+                          : __uint_as_float((w & 0x807FFFFFu) | 0x3F800000u);
+}
+__device__ __forceinline__ int exponent_of(float x) {  // x >= 0
+  return static_cast<int>(__float_as_uint(x) >> 23) - 127;
+}
 // How far a unit has to rise so that weight x lies between 2^11 and 2^12 (an infinite one: 117).
 __device__ __forceinline__ int exponent_above(float x) {
   return static_cast<int>(__float_as_uint(x) >> 23) - 127 - 11;
@@ -158,11 +170,6 @@ __device__ __forceinline__ float f16_row_scale(uint32_t top, float scale_log2, f
   const int n = min(13 - e, 126);
   *up = __uint_as_float(static_cast<uint32_t>(127 + n) << 23);
   return fmaxf(scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - n) << 23), 0x1p-126f);
-}
-
-// The power of two above x (x >= 0), at least 2^-100.
-__device__ __forceinline__ float power_above(float x) {
-  return fmaxf(__uint_as_float(__float_as_uint(x) & 0x7F800000u) * 2.f, 0x1p-100f);
 }
 
 // ---------------------------------------------------------------- clusters

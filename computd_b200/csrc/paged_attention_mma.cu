@@ -37,11 +37,16 @@
 // Warp 9: TMA, straight from the pages into the swizzled operand tiles.  bf16
 // caches: warps 10-11 look over the values of tiles that end behind what every row
 // sees, since 0 * NaN would reach rows that must not see it.  e4m3 caches: warps
-// 12-15 turn codes into fp16 operand tiles (code times scale, over a power of two above
-// the tile's scales, rounded to 2^-11), and Q is scaled per row by a power of two into
+// 12-15 turn codes into fp16 operand tiles (code times scale, over a power of two near
+// the first tile's scales, rounded to 2^-11), and Q is scaled per row by a power of two into
 // fp16, exactly.  (With the keys' scales multiplied into the scores instead, every
 // row's thread read 128 of them per step: 1499 us instead of 1333 for 4736 rows over
-// 16384 keys, 32 heads.)
+// 16384 keys, 32 heads.)  One power of two for all tokens would take the bits of those whose
+// scales are far smaller, for the sake of one that a row may not even see.  So from the step on
+// where scales leave a range of 2^12, operands keep their scales' mantissas only, and the row's
+// thread multiplies scores and weights by the powers of two after all, in units of its own: 2048
+// rows over 8192 keys, 32 heads, 283 us, and 550 to 590 where that starts at once.  (The check
+// and the second form's code cost the first 1 to 5 %.)
 //
 // Where there are few units of 256 rows, a cluster of blocks shares the keys of one
 // and joins its parts through distributed shared memory, in a fixed order.
@@ -55,6 +60,7 @@
 #include <atomic>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "dwa_internal.h"
 #include "f32x2.cuh"
@@ -93,14 +99,16 @@ constexpr int kMaxChannels = 128;
 constexpr int kMaxSplit = 8;
 constexpr float kSlack = 4.f;  // log2 of how far P may grow before m follows
 // e4m3 caches: P in fp16 times 2^11 (with kSlack still below 65504), keys and values
-// times 64 over a power of two above their scales (448 * 64 is below it too).
-constexpr float kPBits = 11.f, kCodeScale = 64.f;
+// times f, 8 over a power of two above the first tile's scales.  f may lie between 2^-5, where
+// the least code, 2^-9, still makes fp16's least normal number, and 2^7 (448 f below 65504).
+constexpr float kPBits = 11.f, kCodeScale = 8.f;
+constexpr int kScalesBelow = 8, kScalesAbove = 4;  // the scales' range around that power, in log2
 
 template <bool kE4m3, int DP>
 struct MmaCfg {
   static constexpr int kThreads = kE4m3 ? 512 : 384;
-  static constexpr int kSoftmaxRegs = kE4m3 ? 184 : 208;
-  static constexpr int kOtherRegs = kE4m3 ? 72 : 88;
+  static constexpr int kSoftmaxRegs = kE4m3 ? 176 : 208;
+  static constexpr int kOtherRegs = kE4m3 ? 80 : 88;
   static constexpr int kHalves = DP / 64;               // 128-byte wide column blocks
   static constexpr int kBlockBytes = kTile * 128;       // one of them: 16 KB
   static constexpr int kTileBytes = kHalves * kBlockBytes;
@@ -124,12 +132,17 @@ struct MmaShared {
   int abort;
   int bad_page;
   int any_bad;
-  int first_bad[kMaxChannels];  // least key with a value that is not finite (e4m3: [0], whole vectors)
-  // e4m3 only: the converting warps' largest scales of four tiles; the powers of two
-  // that keys and values of four steps are divided by
-  uint64_t tops_ready;
-  uint32_t tops[4][4];
-  float k_ref[4], v_ref[4];
+  int first_bad[kE4m3 ? 1 : kMaxChannels];  // least key with a value that is not finite (e4m3: whole vectors)
+  // e4m3 only: the powers of two that keys and values are divided by; the steps from which
+  // each key or value is divided by its own scale's instead, the lesser of the two, and those
+  // (as bf16) of three steps
+  float k_ref, v_ref;
+  int k_from, v_from, apart_from;
+  alignas(16) uint16_t k_pow[3][kE4m3 ? kTile : 8], v_pow[3][kE4m3 ? kTile : 8];
+  // between the converting warps: the first tile's largest and least scales (keys', values'),
+  // and which scales of two steps are out of range (keys' 1, values' 2)
+  uint64_t scales_ready, refs_ready;
+  uint32_t tops[2][4], lows[2][4], far[2][4];
 };
 
 // ---------------------------------------------------------------- tcgen05 pieces
@@ -203,6 +216,13 @@ __device__ __forceinline__ void tmem_scale_x16(uint32_t taddr, float f) {
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// The powers of two of an even key and the next.
+__device__ __forceinline__ void powers_at(const uint16_t* powers, int key, float& x, float& y) {
+  const uint32_t w = reinterpret_cast<const uint32_t*>(powers)[key >> 1];
+  x = __uint_as_float(w << 16);
+  y = __uint_as_float(w & 0xFFFF0000u);
 }
 
 // A K-step of 16 keys of a value tile: channels along the rows of 128 bytes (MN-major,
@@ -435,7 +455,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         mbar_init(bar(sh.empty[i]), 1);
       }
       mbar_init(bar(sh.s_free), 4);
-      mbar_init(bar(sh.tops_ready), 4);
+      mbar_init(bar(sh.scales_ready), 4);
+      mbar_init(bar(sh.refs_ready), 1);
       mbar_init(bar(sh.q_ready), 8);
       for (int i = 0; i < 2; ++i) {
         mbar_init(bar(sh.s_ready[i]), 1);
@@ -450,8 +471,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     __syncwarp();
     for (int it = 0; it < min(C::kStages, n_items); ++it) bring(it);  // no one to wait for
   }
+  constexpr int kBads = kE4m3 ? 1 : kMaxChannels;
   if (warp == 10)
-    for (int i = lane; i < kMaxChannels; i += 32) sh.first_bad[i] = 0x7FFFFFFF;
+    for (int i = lane; i < kBads; i += 32) sh.first_bad[i] = 0x7FFFFFFF;
   if (warp == 8) {
     tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
@@ -629,62 +651,85 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const int row0 = 32 * w + row8;
       constexpr int kPer = DP / 64;                 // 16-byte pieces of codes per row and lane
       constexpr int kSwizzle = DP == 128 ? 7 : 0;   // of the codes' 128-byte rows
-      // Thread t has key t of a tile: its scale is looked up two items ahead, its page
-      // three, and the warp's largest scale is published one ahead.
+      // Thread t has key t of a tile: its scales are looked up a step ahead, its page two.
       const int64_t head = static_cast<int64_t>(hk) << a.page_log2;
       const int page_mask = (1 << a.page_log2) - 1;
-      auto page_of = [&](int it) -> int {
-        const int key = (first_tile + (it >> 1)) * kTile + t;
-        return it < n_items && key < vis_max ? __ldg(table + (key >> a.page_log2)) : -1;
+      auto page_of = [&](int j) -> int {
+        const int key = (first_tile + j) * kTile + t;
+        return j < n_steps && key < vis_max ? __ldg(table + (key >> a.page_log2)) : -1;
       };
-      auto scale_of = [&](int it, int page) -> float {
+      auto scale_of = [&](const float* scales, int page) -> float {
         if (page < 0 || page >= a.n_pages) return 0.f;
-        return __ldg(((it & 1) ? a.v_scale : a.k_scale) + page * a.ld_scale_page + head +
-                     (t & page_mask));
+        return __ldg(scales + page * a.ld_scale_page + head + (t & page_mask));
       };
-      auto publish = [&](int it, float x) {  // numbers order like their bits; others count as 0
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, fabsf(x) < INFINITY ? __float_as_uint(fabsf(x)) : 0u);
-        if (lane == 0) sh.tops[it & 3][w] = top;
-        warp_arrive(sh.tops_ready);
+      // numbers order like their bits; what is not finite counts as 0, and 0 not at all
+      auto bits_of = [](float x) { return fabsf(x) < INFINITY ? __float_as_uint(fabsf(x)) : 0u; };
+      int page = page_of(0);
+      float k_now = scale_of(a.k_scale, page), v_now = scale_of(a.v_scale, page);
+      page = page_of(1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t bits = bits_of(i ? v_now : k_now);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, bits);
+        const uint32_t low = __reduce_min_sync(0xFFFFFFFFu, bits - 1u);
+        if (lane == 0) {
+          sh.tops[i][w] = top;
+          sh.lows[i][w] = low;
+        }
+      }
+      warp_arrive(sh.scales_ready);
+      const bool begun = warp_wait(sh.scales_ready, 0);
+      // The least bits of the keys' and values' scales in range, and whether (keys 1, values 2) they
+      // left it, so that each is divided by a power of two of its own.
+      uint32_t least[2], apart = 0u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t *tops = sh.tops[i], *lows = sh.lows[i];
+        const uint32_t top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+        const uint32_t low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
+        const int ref = min(max(top == 0u ? 127 : static_cast<int>(top >> 23) + 1, 20), 240);  // biased
+        least[i] = static_cast<uint32_t>(ref - kScalesBelow) << 23;
+        if (low != 0xFFFFFFFFu &&
+            (low + 1u < least[i] || top >= static_cast<uint32_t>(ref + kScalesAbove) << 23))
+          apart |= 1u << i;
+        if (t == 0) (i ? sh.v_ref : sh.k_ref) = pow2(ref - 127);
+      }
+      if (t == 0) {
+        sh.k_from = apart & 1u ? 0 : 0x7FFFFFFF;
+        sh.v_from = apart & 2u ? 0 : 0x7FFFFFFF;
+        sh.apart_from = apart ? 0 : 0x7FFFFFFF;
+        mbar_arrive(bar(sh.refs_ready));
+      }
+      auto out_of_range = [&](int i, float x) {
+        const uint32_t bits = bits_of(x);
+        return bits != 0u && bits - least[i] >= static_cast<uint32_t>(kScalesBelow + kScalesAbove) << 23;
       };
-      float now = scale_of(0, page_of(0)), next = scale_of(1, page_of(1)), v_ref = 0.f;
-      int page = page_of(2);
-      publish(0, now);
-      for (int it = 0; it < n_items; ++it) {
+      // An operand tile: codes to fp16 times their keys' factors.  What the places of this step's
+      // powers held was last read in step j - 3, which is over since the stage of this step's
+      // keys, where that one's values were, was free for the copy.
+      auto convert = [&](int it, float now) -> bool {
         const int st = it % C::kStages, j = it >> 1, key0 = (first_tile + j) * kTile;
-        const float after = scale_of(it + 2, page);
-        page = page_of(it + 3);
-        if (!warp_wait(sh.tops_ready, it)) break;
-        publish(it + 1, next);  // after the wait: no warp can be two phases ahead of another
-        const uint32_t* tops = sh.tops[it & 3];
-        float ref = power_above(__uint_as_float(max(max(tops[0], tops[1]), max(tops[2], tops[3]))));
-        if (!warp_wait(sh.full[st], it / C::kStages)) break;
-        // What this step's slots held was last read in step j - 4, which is over since
-        // this stage, whose tile was of step j - 2 or j - 3, was free for the copy.
-        if (it & 1) {
-          // values of all steps add up in O: their power of two only grows
-          v_ref = ref = fmaxf(ref, v_ref);
-          if (t == 0) sh.v_ref[j & 3] = ref;
-          // a vector that is NaN and that some row must not see becomes zeros, and is noted
-          if (!(fabsf(now) < INFINITY) && key0 + t >= vis_min) {
-            if (key0 + t < vis_max) {
-              atomicMin(&sh.first_bad[0], key0 + t);
-              sh.any_bad = 1;
-            }
-            now = 0.f;
+        if (!warp_wait(sh.full[st], it / C::kStages)) return false;
+        // a value vector that is NaN and that some row must not see becomes zeros, and is noted
+        if ((it & 1) && !(fabsf(now) < INFINITY) && key0 + t >= vis_min) {
+          if (key0 + t < vis_max) {
+            atomicMin(&sh.first_bad[0], key0 + t);
+            sh.any_bad = 1;
           }
-        } else if (t == 0) {
-          sh.k_ref[j & 3] = ref;
+          now = 0.f;
         }
         // this key's factor as the sum of two fp16: keys use both, so that a product has
         // its own rounding only (a score is 128 of them), values the first
-        const float f = now * (kCodeScale / ref);
+        float f = now * __uint_as_float((static_cast<uint32_t>(127 + 127 + 3 - kScalesBelow) << 23) - least[it & 1]);
+        if (apart & (it & 1 ? 2u : 1u)) {
+          int e;
+          f = scale_parts(now, &e);
+          (it & 1 ? sh.v_pow : sh.k_pow)[j % 3][t] = static_cast<uint16_t>((127 + e) << 7);
+        }
         const __half f_hi = __float2half_rn(f);
         const __half f_lo = __float2half_rn(f - __half2float(f_hi));
-        const uint32_t mul = static_cast<uint32_t>(__half_as_ushort(f_hi)) |
-                             (static_cast<uint32_t>(__half_as_ushort(f_lo)) << 16);
-        now = next;
-        next = after;
+        const uint32_t factors = static_cast<uint32_t>(__half_as_ushort(f_hi)) |
+                                 (static_cast<uint32_t>(__half_as_ushort(f_lo)) << 16);
         uint8_t* stage = smem + 2 * C::kTileBytes + st * C::kStageBytes;
         uint4 x[4][kPer];
 #pragma unroll
@@ -703,7 +748,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         __syncwarp();  // the rows' codes are read: their place may be written
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t both = __shfl_sync(0xFFFFFFFFu, mul, row8 + 8 * k);
+          const uint32_t both = __shfl_sync(0xFFFFFFFFu, factors, row8 + 8 * k);
           const uint32_t hi = __byte_perm(both, 0, 0x1010), lo = __byte_perm(both, 0, 0x3232);
 #pragma unroll
           for (int p = 0; p < kPer; ++p) {
@@ -726,7 +771,33 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           }
         }
         fence_proxy_async_smem();
-        warp_arrive(sh.ready[st]);
+        return true;
+      };
+      for (int j = 0; j < n_steps && begun; ++j) {
+        const float k_next = scale_of(a.k_scale, page), v_next = scale_of(a.v_scale, page);
+        page = page_of(j + 2);
+        if (!convert(2 * j, k_now)) break;
+        warp_arrive(sh.ready[(2 * j) % C::kStages]);
+        // Whether the next step's scales are in range, settled before this step's values are
+        // ready: who has waited for those knows.
+        uint32_t far = (__any_sync(0xFFFFFFFFu, out_of_range(0, k_next)) ? 1u : 0u) |
+                       (__any_sync(0xFFFFFFFFu, out_of_range(1, v_next)) ? 2u : 0u);
+        if (lane == 0) sh.far[j & 1][w] = far;
+        warp_arrive(sh.scales_ready);
+        if (!convert(2 * j + 1, v_now) || !warp_wait(sh.scales_ready, j + 1)) break;
+        const uint32_t* fars = sh.far[j & 1];
+        far = fars[0] | fars[1] | fars[2] | fars[3];
+        if (far & ~apart) {
+          if (t == 0) {
+            if (far & ~apart & 1u) sh.k_from = j + 1;
+            if (far & ~apart & 2u) sh.v_from = j + 1;
+            if (apart == 0u) sh.apart_from = j + 1;
+          }
+          apart |= far;
+        }
+        warp_arrive(sh.ready[(2 * j + 1) % C::kStages]);
+        k_now = k_next;
+        v_now = v_next;
       }
     }
     __syncwarp();
@@ -790,113 +861,216 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     auto ref_of = [](float top) -> float {
       return top == -INFINITY ? 0.f : kE4m3 && fabsf(top) < 0x1p22f ? kPBits - top : -top;
     };
-    float m = -INFINITY, l = 0.f, v_ref = 0.f, ref = 0.f;
+    float m = -INFINITY, l = 0.f, ref = 0.f;
     bool alive = true;
-    for (int j = 0; j < steps; ++j) {
-      if (!warp_wait(sh.s_ready[i], j)) { alive = false; break; }
-      tc_fence_after();
-      if (!warp_live) {  // no rows of its own: P's lanes hold what they hold, nobody reads O's
+    // e4m3: the scores' factor, and the step from which keys or values are divided by their own
+    // scales' powers of two.  From then on O is in units of 2^v_exp / kPScale, which may fall by
+    // v_room.
+    float k_factor = row_factor;
+    volatile int *const apart_from = &sh.apart_from, *const k_from = &sh.k_from, *const v_from = &sh.v_from;
+    int apart = 0x7FFFFFFF, v_exp = kLeastExp;
+    float v_room = kAllRoom;
+    if (kE4m3 && warp_live && steps > 0) {
+      alive = warp_wait(sh.refs_ready, 0);
+      k_factor = fmaxf(row_factor * sh.k_ref, 0x1p-126f);
+      apart = *apart_from;
+    }
+    int j = 0;
+    // The steps before `apart`, or the others.
+    auto go = [&](auto apart_) {
+      constexpr bool kApart = decltype(apart_)::value;
+      for (; j < steps && alive && (kApart || j < apart); ++j) {
+        if (!warp_wait(sh.s_ready[i], j)) { alive = false; break; }
+        tc_fence_after();
+        if (!warp_live) {  // no rows of its own: P's lanes hold what they hold, nobody reads O's
+          tc_fence_before();
+          warp_arrive(sh.s_free);
+          if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
+          warp_arrive(sh.p_ready[i]);
+          continue;
+        }
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_async(ts + 32 * c, s[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld_pin(s[c]);
         tc_fence_before();
         warp_arrive(sh.s_free);
-        if (j > 0 && !warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
-        warp_arrive(sh.p_ready[i]);
-        continue;
-      }
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_async(ts + 32 * c, s[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld_pin(s[c]);
-      tc_fence_before();
-      warp_arrive(sh.s_free);
-      const int key0 = (first_tile + j) * kTile;
-      const bool edge = key0 + kTile > vis_low;
-      float v_now = 0.f, factor = row_factor;
-      if constexpr (kE4m3) {
-        // the step's powers of two: the values' tile is converted right after the keys'
-        if (!warp_wait(sh.ready[(2 * j + 1) % C::kStages], (2 * j + 1) / C::kStages)) {
-          alive = false;
-          break;
+        const int key0 = (first_tile + j) * kTile;
+        const bool edge = key0 + kTile > vis_low;
+        float factor = k_factor;
+        if constexpr (kE4m3) {  // the values' tile is converted right after the keys'
+          if (!warp_wait(sh.ready[(2 * j + 1) % C::kStages], (2 * j + 1) / C::kStages)) {
+            alive = false;
+            break;
+          }
+          if (!kApart) apart = *apart_from;  // j + 1 at least
         }
-        v_now = sh.v_ref[j & 3];
-        factor = fmaxf(row_factor * sh.k_ref[j & 3], 0x1p-126f);
-      }
-      if (edge) {
+        if constexpr (kApart) {
+          if (j >= *k_from) {
+            const float whole = row_factor * kCodeScale;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (key0 + 32 * c + k >= vis) s[c][k] = 0xFF800000u;
-      }
-      float top[4];
+              for (int k = 0; k < 32; k += 2) {
+                float f0, f1;
+                powers_at(sh.k_pow[j % 3], 32 * c + k, f0, f1);
+                s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * (whole * f0));
+                s[c][k + 1] = __float_as_uint(__uint_as_float(s[c][k + 1]) * (whole * f1));
+              }
+          } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        top[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int k = 2; k < 32; k += 2)
-          top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-      }
-      const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
-      const bool move = most > m + kSlack || (m == -INFINITY && most > m) || v_now != v_ref;
-      const bool big = fabsf(most) >= 0x1p20f && fabsf(most) < INFINITY;
-      if (__any_sync(0xFFFFFFFFu, move || big)) {
-        // The product s factor is not rounded before ref is added to it below, most is: where
-        // scores are big the difference would count.
-        if (__any_sync(0xFFFFFFFFu, big)) {
+              for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * factor);
+          }
+          factor = 1.f;
+        }
+        if (edge) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * factor);
-          factor = 1.f;
+            for (int k = 0; k < 32; ++k)
+              if (key0 + 32 * c + k >= vis) s[c][k] = 0xFF800000u;
         }
-        const float m_new = fmaxf(m, most), ref_new = ref_of(m_new);
-        const float shrink = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);
-        float shrink_o = shrink;
-        if constexpr (kE4m3) {
-          shrink_o = v_ref == 0.f ? 0.f : shrink * (v_ref / v_now);
-          v_ref = v_now;
-        }
-        m = m_new;
-        ref = ref_new;
-        l *= shrink;
-        if (j > 0) {
-          if (!warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, shrink_o);
-        }
-      }
-      const uint64_t factor2 = pair(factor, factor), ref2 = pair(ref, ref);
-      uint64_t l2[2] = {0, 0};
-      auto half = [&](int h) {
-        uint32_t p[32];
+        float top[4];
 #pragma unroll
-        for (int k = 0; k < 64; k += 2) {
-          const int c = 2 * h + (k >> 5);
-          const uint64_t x = fma2(pair(__uint_as_float(s[c][k & 31]), __uint_as_float(s[c][(k & 31) + 1])),
-                                  factor2, ref2);
-          float p0, p1;
-          unpair(x, p0, p1);
-          const uint64_t y = pair(fast_exp2(p0), fast_exp2(p1));
-          l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], y);
-          unpair(y, p0, p1);
-          p[k >> 1] = kE4m3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+        for (int c = 0; c < 4; ++c) {
+          top[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
+#pragma unroll
+          for (int k = 2; k < 32; k += 2)
+            top[c] = max3(top[c], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
         }
-        if (h == 0 && j > 0) {  // the product that read the last P
-          alive = warp_wait(sh.p_free[i], j - 1);
-          tc_fence_after();
+        const float most = max3(fmaxf(top[0], top[1]), top[2], top[3]) * factor;
+        if constexpr (kApart) {
+          // Each value's power of two goes into its weight.
+          const bool v_apart = j >= *v_from;
+          const float v_unit = sh.v_ref / kCodeScale;
+          const float m_new = fmaxf(m, most), ref_new = m_new == -INFINITY ? 0.f : -m_new;
+          float turn = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);  // of O
+          v_room = m == -INFINITY ? kAllRoom : v_room + (m_new - m);
+          m = m_new;
+          ref = ref_new;
+          l *= turn;
+          float sum = 0.f, heaviest = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float f0 = v_unit, f1 = v_unit;
+              if (v_apart) powers_at(sh.v_pow[j % 3], 32 * c + k, f0, f1);
+              const float p0 = fast_exp2(__uint_as_float(s[c][k]) + ref), p1 = fast_exp2(__uint_as_float(s[c][k + 1]) + ref);
+              sum += p0 + p1;
+              f0 *= p0;
+              f1 *= p1;
+              heaviest = max3(heaviest, f0, f1);
+              s[c][k] = __float_as_uint(f0);
+              s[c][k + 1] = __float_as_uint(f1);
+            }
+          l += sum;
+          const int over = exponent_of(heaviest) - v_exp;  // of 2^11
+          int up = 0;
+          if (heaviest > 0.f && over > 3) {
+            up = over;
+            v_room = 0.f;
+          } else if (heaviest > 0.f && over < -5) {
+            up = -min(min(static_cast<int>(v_room), v_exp - kLeastExp), -over);
+            if (v_room < 0.5f * kAllRoom) up = max(up, -120);  // what O can take at a time
+            v_room += static_cast<float>(up);
+          }
+          if (heaviest > 0.f && v_room > 0.5f * kAllRoom) v_room = 0.f;
+          v_exp += up;
+          turn = turn * pow2(-(up / 2)) * pow2(-(up - up / 2));
+          if (j > 0) {
+            alive = warp_wait(sh.p_free[i], j - 1);
+            tc_fence_after();
+            if (alive && __any_sync(0xFFFFFFFFu, turn != 1.f)) {
+#pragma unroll 1
+              for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, turn);
+            }
+          }
+          const float unit = exp_scale(v_exp);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[32];
+#pragma unroll
+            for (int k = 0; k < 64; k += 2) {
+              const int c = 2 * h + (k >> 5);
+              p[k >> 1] = pack_f16(__uint_as_float(s[c][k & 31]) * unit, __uint_as_float(s[c][(k & 31) + 1]) * unit);
+            }
+            if (alive) tmem_st_x32(tp + 32 * h, p);
+          }
+          if (!alive) break;
+          tmem_wait_st();
+          tc_fence_before();
+          warp_arrive(sh.p_ready[i]);
+          continue;
         }
-        tmem_st_x32(tp + 32 * h, p);
-      };
-      half(0);
-      half(1);
-      if (!alive) break;
-      tmem_wait_st();
-      tc_fence_before();
-      warp_arrive(sh.p_ready[i]);
-      float l0, l1;
-      unpair(add2(l2[0], l2[1]), l0, l1);
-      l += l0 + l1;
+        const bool move = most > m + kSlack || (m == -INFINITY && most > m);
+        const bool big = fabsf(most) >= 0x1p20f && fabsf(most) < INFINITY;
+        if (__any_sync(0xFFFFFFFFu, move || big)) {
+          // The product s factor is not rounded before ref is added to it below, most is: where
+          // scores are big the difference would count.
+          if (__any_sync(0xFFFFFFFFu, big)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * factor);
+            factor = 1.f;
+          }
+          const float m_new = fmaxf(m, most), ref_new = ref_of(m_new);
+          const float shrink = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);
+          m = m_new;
+          ref = ref_new;
+          l *= shrink;
+          if (j > 0) {
+            if (!warp_wait(sh.p_free[i], j - 1)) { alive = false; break; }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < a.d; c += 16) tmem_scale_x16(to + c, shrink);
+          }
+        }
+        const uint64_t factor2 = pair(factor, factor), ref2 = pair(ref, ref);
+        uint64_t l2[2] = {0, 0};
+        auto half = [&](int h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int k = 0; k < 64; k += 2) {
+            const int c = 2 * h + (k >> 5);
+            const uint64_t x = fma2(pair(__uint_as_float(s[c][k & 31]), __uint_as_float(s[c][(k & 31) + 1])),
+                                    factor2, ref2);
+            float p0, p1;
+            unpair(x, p0, p1);
+            const uint64_t y = pair(fast_exp2(p0), fast_exp2(p1));
+            l2[(k >> 1) & 1] = add2(l2[(k >> 1) & 1], y);
+            unpair(y, p0, p1);
+            p[k >> 1] = kE4m3 ? pack_f16(p0, p1) : pack_bf16(p0, p1);
+          }
+          if (h == 0 && j > 0) {  // the product that read the last P
+            alive = warp_wait(sh.p_free[i], j - 1);
+            tc_fence_after();
+          }
+          tmem_st_x32(tp + 32 * h, p);
+        };
+        half(0);
+        half(1);
+        if (!alive) break;
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(sh.p_ready[i]);
+        float l0, l1;
+        unpair(add2(l2[0], l2[1]), l0, l1);
+        l += l0 + l1;
+      }
+    };
+    go(std::false_type{});
+    const bool rest = kE4m3 && warp_live && alive && j < steps;
+    if (rest) {
+      if (j > 0) {
+        v_exp = exponent_of(sh.v_ref / kCodeScale) + static_cast<int>(kPBits);
+        v_room = kPBits;  // which P and l lose
+      }
+      go(std::bool_constant<kE4m3>{});
     }
     if (steps > 0 && alive) alive = warp_wait(sh.p_free[i], steps - 1);
     tc_fence_after();
@@ -905,11 +1079,13 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     if (!alive || sh.bad_page) l = __uint_as_float(0x7FC00000u);
     if (sh.bad_page && threadIdx.x == 0) paged_report(a.status);
     // O is in units of P's power of two, which l has too, and of the values'
-    const float v_back = kE4m3 ? v_ref / kCodeScale : 1.f;
+    const float v_back = !kE4m3 ? 1.f
+                         : rest ? pow2(v_exp - static_cast<int>(kPBits))
+                                : sh.v_ref / kCodeScale;
     if (cluster == 1) {
       // through this warp's rows of Q's tile, which no product needs any more, so that
       // rows leave whole (a row per thread at 16 bytes a store took 7 us per block)
-      const float inv = (l == 0.f ? 0.f : 1.f / l) * v_back;
+      const float inv = 1.f / l;
       const bool some_bad = sh.any_bad;
       uint8_t* stage = smem + i * C::kTileBytes + 32 * (warp & 3) * (2 * DP);
       if (warp_live) {
@@ -923,7 +1099,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
             for (int k = 0; k < 32; ++k) o[k] = 0.f;
           }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = l == 0.f ? 0.f : o[k] * inv;
+          for (int k = 0; k < 32; ++k) o[k] = l == 0.f ? 0.f : o[k] * inv * v_back;
           if (some_bad) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)
@@ -977,9 +1153,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       }
       st_cluster_f32x2(there + C::kPartMl + 8 * slot, m == -INFINITY ? m : -ref, l);
       if (sh.any_bad) {
-        for (int at = threadIdx.x; at < cluster * kMaxChannels; at += 256)
-          min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kMaxChannels]), at / kMaxChannels),
-                          sh.first_bad[at % kMaxChannels]);
+        for (int at = threadIdx.x; at < cluster * kBads; at += 256)
+          min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kBads]), at / kBads), sh.first_bad[at % kBads]);
         if (threadIdx.x < cluster) st_cluster_s32(map_to_cta(smem_u32(&sh.any_bad), threadIdx.x), 1);
       }
       cluster_sync();
