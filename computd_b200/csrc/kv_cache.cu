@@ -146,13 +146,14 @@ __device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, b
     }
     const float s = fmaxf(quotient(most, 448.f, 1.f / 448.f), least);
     const float y = __frcp_rn(s);
-    const uint64_t y2 = pair(y, y), neg2 = pair(-s, -s);
+    const uint64_t neg2 = pair(-y, -y), s2 = pair(s, s);
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {  // as quotient()
-      const uint64_t v = pair(x[i], x[i + 1]), q = mul2(v, y2);
-      unpair(fma2(fma2(q, neg2, v), y2, q), x[i], x[i + 1]);
+    for (int i = 0; i < 16; i += 2) {  // as quotient(), but of -x: so the remainder of a zero, +0, leaves it its sign
+      const uint64_t v = pair(x[i], x[i + 1]), q = mul2(v, neg2);
+      unpair(fma2(fma2(q, s2, v), neg2, q), x[i], x[i + 1]);
     }
     w = codes16(x);  // |x / s| <= 448 (1 + 2^-23), which rounds to 448 at most
+    w = make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
     scale = s * down;
   }
   if (on) *reinterpret_cast<uint4*>(cache + row * d + 16 * lane) = w;
