@@ -24,7 +24,7 @@ constexpr int kWriteThreads = 256;
 // 4, 5), into codes (39.9, 42.3, 62.8), and f32.
 template <bool kE4m3, bool kSrcBf16>
 constexpr int kWriteBlocks = !kSrcBf16 ? 2 : kE4m3 ? 3 : 4;
-constexpr int kGroupTokens = 256;  // tokens of a block checked for repeated slots at a time
+constexpr int kBlockTokens = 32;  // at most; a longer call is cut into launches
 constexpr int kFilterBits = 8192;  // their slots' low bits
 
 __device__ __forceinline__ void report(int32_t* status) {
@@ -179,15 +179,18 @@ struct WriteArgs {
 // A block owns a run of tokens.  `lanes` neighbouring lanes hold one (token,
 // head) vector of K and of V; the amax is a shuffle over them.
 // Where slots repeat the last token must stay, whichever block writes first:
-// each block drops its tokens whose slot a later token names.  It looks the
-// slots after its own up in a filter of its own slots' low bits, so the whole
-// list is read once per block (from L2: 19 MB in all for 8192 tokens, against
-// the 200 MB of keys and values at 32 heads of 128).
+// each block drops its tokens whose slot a later token of the launch names.  It looks
+// the slots after its own up in a filter of its own slots' low bits, so a launch's list
+// is read once per block (from L2: 19 MB in all for 8192 tokens, against the 200 MB of
+// keys and values at 32 heads of 128).  More tokens than the resident blocks take, 14,208 from
+// bf16 to codes, are cut into launches, which the stream orders, so that time and looks grow
+// as the tokens do: 1,000,000 tokens of 8 heads of 128 take 2.6 ms (with 16, 64, 128 tokens per
+// block 2.6, 3.9, 8.3; in one launch 169), 20,000 47 us (50, 55, 55; 57).
 template <bool kE4m3, bool kSrcBf16>
 __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<kE4m3, kSrcBf16>)
     kv_write_kernel(const WriteArgs a) {
-  __shared__ int64_t own[kGroupTokens];
-  __shared__ int dropped[kGroupTokens];
+  __shared__ int64_t own[kBlockTokens];
+  __shared__ int dropped[kBlockTokens];
   __shared__ uint32_t filter[kFilterBits / 32];
 
   const int lanes = 1 << a.lanes_log2;
@@ -197,80 +200,77 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<kE4m3, kSrcBf16>)
   constexpr int kN = kLaneValues<kE4m3>;
   using Values = Raw<kSrcBf16, kN>;
   const bool on = kN * lane < a.d;
-  const int64_t t_end = min((blockIdx.x + 1) * a.tokens_per_block, a.T);
-  for (int64_t t0 = blockIdx.x * a.tokens_per_block; t0 < t_end; t0 += kGroupTokens) {
-    const int n = static_cast<int>(min(t_end - t0, static_cast<int64_t>(kGroupTokens)));
-    const int vectors = n * a.H;
-    // a round's values are under way while the round before is stored, the first ones
-    // while the slots are checked
-    auto load = [&](int i, int h, Values* k, Values* v) {
-      if (i < n && on) {
-        *k = load_raw<kSrcBf16, kN>(a.k, (t0 + i) * a.k_tok + h * a.k_head + kN * lane);
-        *v = load_raw<kSrcBf16, kN>(a.v, (t0 + i) * a.v_tok + h * a.v_head + kN * lane);
-      }
-    };
-    auto forward = [&](int* i, int* h) {  // to this group's next vector
-      *h += groups;
-      while (*h >= a.H) {
-        *h -= a.H;
-        ++*i;
-      }
-    };
-    Values k_now{}, v_now{};
-    int i_now = group / a.H, h_now = group % a.H;
-    load(i_now, h_now, &k_now, &v_now);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kFilterBits / 32; i += kWriteThreads) filter[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kWriteThreads) {
-      const int64_t s = a.slots[t0 + i];
-      const bool fine = s >= 0 && s < a.n_slots;
-      if (!fine && s != -1) report(a.status);
-      own[i] = s;
-      dropped[i] = fine ? 0 : 1;
-      if (fine) atomicOr(&filter[(s & (kFilterBits - 1)) >> 5], 1u << (s & 31));
+  const int64_t t0 = blockIdx.x * a.tokens_per_block;
+  const int n = static_cast<int>(min(a.T - t0, a.tokens_per_block));
+  const int vectors = n * a.H;
+  // a round's values are under way while the round before is stored, the first ones
+  // while the slots are checked
+  auto load = [&](int i, int h, Values* k, Values* v) {
+    if (i < n && on) {
+      *k = load_raw<kSrcBf16, kN>(a.k, (t0 + i) * a.k_tok + h * a.k_head + kN * lane);
+      *v = load_raw<kSrcBf16, kN>(a.v, (t0 + i) * a.v_tok + h * a.v_head + kN * lane);
     }
-    __syncthreads();
-    constexpr int kBatch = 8;  // slots that a thread looks at together
-    for (int64_t t = t0 + 1 + threadIdx.x; t < a.T; t += kBatch * kWriteThreads) {
-      int64_t s[kBatch];
+  };
+  auto forward = [&](int* i, int* h) {  // to this group's next vector
+    *h += groups;
+    while (*h >= a.H) {
+      *h -= a.H;
+      ++*i;
+    }
+  };
+  Values k_now{}, v_now{};
+  int i_now = group / a.H, h_now = group % a.H;
+  load(i_now, h_now, &k_now, &v_now);
+  for (int i = threadIdx.x; i < kFilterBits / 32; i += kWriteThreads) filter[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kWriteThreads) {
+    const int64_t s = a.slots[t0 + i];
+    const bool fine = s >= 0 && s < a.n_slots;
+    if (!fine && s != -1) report(a.status);
+    own[i] = s;
+    dropped[i] = fine ? 0 : 1;
+    if (fine) atomicOr(&filter[(s & (kFilterBits - 1)) >> 5], 1u << (s & 31));
+  }
+  __syncthreads();
+  constexpr int kBatch = 8;  // slots that a thread looks at together
+  for (int64_t t = t0 + 1 + threadIdx.x; t < a.T; t += kBatch * kWriteThreads) {
+    int64_t s[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        s[j] = t + j * kWriteThreads < a.T ? __ldg(a.slots + t + j * kWriteThreads) : -1;
+    for (int j = 0; j < kBatch; ++j)
+      s[j] = t + j * kWriteThreads < a.T ? __ldg(a.slots + t + j * kWriteThreads) : -1;
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (s[j] >= 0 && ((filter[(s[j] & (kFilterBits - 1)) >> 5] >> (s[j] & 31)) & 1u)) {
-          const int before = static_cast<int>(min(t + j * kWriteThreads - t0, static_cast<int64_t>(n)));
-          for (int i = 0; i < before; ++i)
-            if (own[i] == s[j]) dropped[i] = 1;
-        }
+    for (int j = 0; j < kBatch; ++j) {
+      if (s[j] >= 0 && ((filter[(s[j] & (kFilterBits - 1)) >> 5] >> (s[j] & 31)) & 1u)) {
+        const int before = static_cast<int>(min(t + j * kWriteThreads - t0, static_cast<int64_t>(n)));
+        for (int i = 0; i < before; ++i)
+          if (own[i] == s[j]) dropped[i] = 1;
       }
     }
-    __syncthreads();
-    for (int base = 0; base < vectors; base += groups) {
-      int i_next = i_now, h_next = h_now;
-      forward(&i_next, &h_next);
-      Values k_next{}, v_next{};
-      load(i_next, h_next, &k_next, &v_next);
-      const bool here = i_now < n;
-      const bool keep = here && !dropped[here ? i_now : 0];
-      const int64_t s = keep ? own[i_now] : 0;
-      const int64_t page = s >> a.page_log2, off = s & ((1 << a.page_log2) - 1);
-      const int64_t in_page = (static_cast<int64_t>(h_now) << a.page_log2) + off;
-      const int64_t row = page * a.ld_page + in_page;
-      const int64_t srow = page * a.ld_scale_page + in_page;
-      if constexpr (kE4m3) {
-        store_e4m3(k_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.k_cache), a.k_scale, row, srow, a.d);
-        store_e4m3(v_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.v_cache), a.v_scale, row, srow, a.d);
-      } else if (on && keep) {
-        store_bf16(k_now, static_cast<uint16_t*>(a.k_cache) + row * a.d + kN * lane);
-        store_bf16(v_now, static_cast<uint16_t*>(a.v_cache) + row * a.d + kN * lane);
-      }
-      k_now = k_next;
-      v_now = v_next;
-      i_now = i_next;
-      h_now = h_next;
+  }
+  __syncthreads();
+  for (int base = 0; base < vectors; base += groups) {
+    int i_next = i_now, h_next = h_now;
+    forward(&i_next, &h_next);
+    Values k_next{}, v_next{};
+    load(i_next, h_next, &k_next, &v_next);
+    const bool here = i_now < n;
+    const bool keep = here && !dropped[here ? i_now : 0];
+    const int64_t s = keep ? own[i_now] : 0;
+    const int64_t page = s >> a.page_log2, off = s & ((1 << a.page_log2) - 1);
+    const int64_t in_page = (static_cast<int64_t>(h_now) << a.page_log2) + off;
+    const int64_t row = page * a.ld_page + in_page;
+    const int64_t srow = page * a.ld_scale_page + in_page;
+    if constexpr (kE4m3) {
+      store_e4m3(k_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.k_cache), a.k_scale, row, srow, a.d);
+      store_e4m3(v_now, here && on, keep, lanes, lane, static_cast<uint8_t*>(a.v_cache), a.v_scale, row, srow, a.d);
+    } else if (on && keep) {
+      store_bf16(k_now, static_cast<uint16_t*>(a.k_cache) + row * a.d + kN * lane);
+      store_bf16(v_now, static_cast<uint16_t*>(a.v_cache) + row * a.d + kN * lane);
     }
+    k_now = k_next;
+    v_now = v_next;
+    i_now = i_next;
+    h_now = h_next;
   }
 }
 
@@ -408,16 +408,26 @@ cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, 
   const int per_sm = e4m3 ? (src_bf16 ? kWriteBlocks<true, true> : kWriteBlocks<true, false>)
                           : (src_bf16 ? kWriteBlocks<false, true> : kWriteBlocks<false, false>);
   const int64_t most = static_cast<int64_t>(per_sm) * device_sm_count();
-  a.tokens_per_block = (T + most - 1) / most;
-  const unsigned grid = static_cast<unsigned>((T + a.tokens_per_block - 1) / a.tokens_per_block);
-  if (e4m3) {
-    if (src_bf16) kv_write_kernel<true, true><<<grid, kWriteThreads, 0, stream>>>(a);
-    else kv_write_kernel<true, false><<<grid, kWriteThreads, 0, stream>>>(a);
-  } else {
-    if (src_bf16) kv_write_kernel<false, true><<<grid, kWriteThreads, 0, stream>>>(a);
-    else kv_write_kernel<false, false><<<grid, kWriteThreads, 0, stream>>>(a);
+  const int64_t launches = (T + most * kBlockTokens - 1) / (most * kBlockTokens);
+  const int64_t share = (T + launches - 1) / launches;  // tokens of one
+  const int64_t es = src_bf16 ? 2 : 4;
+  for (int64_t t = 0; t < T; t += share) {
+    a.T = std::min(share, T - t);
+    a.k = static_cast<const char*>(k) + t * k_tok * es;
+    a.v = static_cast<const char*>(v) + t * v_tok * es;
+    a.slots = slots + t;
+    a.tokens_per_block = (a.T + most - 1) / most;
+    const unsigned grid = static_cast<unsigned>((a.T + a.tokens_per_block - 1) / a.tokens_per_block);
+    if (e4m3) {
+      if (src_bf16) kv_write_kernel<true, true><<<grid, kWriteThreads, 0, stream>>>(a);
+      else kv_write_kernel<true, false><<<grid, kWriteThreads, 0, stream>>>(a);
+    } else {
+      if (src_bf16) kv_write_kernel<false, true><<<grid, kWriteThreads, 0, stream>>>(a);
+      else kv_write_kernel<false, false><<<grid, kWriteThreads, 0, stream>>>(a);
+    }
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   }
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 cudaError_t launch_kv_read(const KvCacheView& c, const int64_t* slots, int64_t T, void* k_out,
