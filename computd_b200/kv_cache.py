@@ -162,13 +162,14 @@ class PagedKVCache:
               n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(slots int64, positions int64) of the newest tokens of every sequence, row by row of
         a packed chunk of ``n_tokens`` rows: row q_start[b] + i is token lengths[b] - n + i of
-        sequence b.  Rows behind q_start[-1], and new tokens that ``lengths`` leaves no
-        place for, get slot -1."""
+        sequence b.  Rows of no sequence, and new tokens that ``lengths`` leaves no place
+        for, get slot -1."""
         row = torch.arange(n_tokens, device=q_start.device)
         start, length, table = q_start.long(), lengths.long(), block_table.long()
         seq = (torch.searchsorted(start, row, right=True) - 1).clamp(0, length.shape[0] - 1)
         position = length[seq] - start[seq + 1] + row
-        fine = (row < start[-1]) & (position >= 0) & (position < table.shape[1] * self.page_size)
+        fine = ((row >= start[seq]) & (row < start[seq + 1]) & (position >= 0)
+                & (position < table.shape[1] * self.page_size))
         at = torch.where(fine, position, 0)
         page = table[seq, at // self.page_size]
         return torch.where(fine, page * self.page_size + at % self.page_size, -1), at

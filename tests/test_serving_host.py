@@ -1,0 +1,42 @@
+"""CPU: the host side of the serving calls: where new tokens go."""
+import pytest
+import torch
+
+from computd_b200 import PagedKVCache
+
+
+def _cache(n_pages=40, page_size=16):
+    return PagedKVCache(1, n_pages, page_size, 2, 16, device="cpu")
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _slots_by_rows(cache, table, lengths, q_start, n):
+    """The definition, row by row."""
+    out = []
+    for row in range(n):
+        slot = -1
+        for b in range(len(lengths)):
+            if q_start[b] <= row < q_start[b + 1]:
+                position = lengths[b] - (q_start[b + 1] - row)
+                if 0 <= position < len(table[b]) * cache.page_size:
+                    page = table[b][position // cache.page_size]
+                    slot = page * cache.page_size + position % cache.page_size if page >= 0 else -2
+        out.append(slot)
+    return out
+
+
+@pytest.mark.parametrize("q_start", [[0, 3, 3, 10, 12], [2, 3, 7, 7, 9], [5, 5, 5, 5, 5], [4, 9, 9, 30, 30],
+                                     [3, 3, 4, 8, 20]])
+def test_slots_of_rows_in_and_outside_every_sequence(q_start):
+    """Rows before the first sequence's and behind the last one's have no slot; neither have new
+    tokens that the length leaves no place for."""
+    cache = _cache()
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(0))[:16].view(4, 4).tolist()
+    lengths = [40, 0, 17, 64]
+    slots, positions = cache.slots(_i32(table), _i32(lengths), _i32(q_start), 24)
+    assert slots.dtype == torch.int64 and positions.dtype == torch.int64
+    assert slots.tolist() == _slots_by_rows(cache, table, lengths, q_start, 24)
+    assert int(positions.min()) >= 0 and int(positions.max()) < 64
