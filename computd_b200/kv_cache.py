@@ -163,7 +163,7 @@ class PagedKVCache:
         """(slots int64, positions int64) of the newest tokens of every sequence, row by row of
         a packed chunk of ``n_tokens`` rows: row q_start[b] + i is token lengths[b] - n + i of
         sequence b.  Rows of no sequence, and new tokens that ``lengths`` leaves no place
-        for, get slot -1."""
+        for, get slot -1; tokens on a negative page get -2, which the calls report."""
         row = torch.arange(n_tokens, device=q_start.device)
         start, length, table = q_start.long(), lengths.long(), block_table.long()
         seq = (torch.searchsorted(start, row, right=True) - 1).clamp(0, length.shape[0] - 1)
@@ -172,7 +172,8 @@ class PagedKVCache:
                 & (position < table.shape[1] * self.page_size))
         at = torch.where(fine, position, 0)
         page = table[seq, at // self.page_size]
-        return torch.where(fine, page * self.page_size + at % self.page_size, -1), at
+        slot = torch.where(page < 0, -2, page * self.page_size + at % self.page_size)
+        return torch.where(fine, slot, -1), at
 
     def check(self) -> None:
         """Raise ``DWAError`` if a call so far met a bad slot, page, length or row range (waits

@@ -40,3 +40,14 @@ def test_slots_of_rows_in_and_outside_every_sequence(q_start):
     assert slots.dtype == torch.int64 and positions.dtype == torch.int64
     assert slots.tolist() == _slots_by_rows(cache, table, lengths, q_start, 24)
     assert int(positions.min()) >= 0 and int(positions.max()) < 64
+
+
+def test_slots_on_bad_pages_are_not_skipped():
+    """A negative page number gives a slot that the write reports (-1 would pass it over in silence);
+    one behind the last page gives one outside the cache."""
+    cache = _cache()
+    table = [[-1, 7, -3, 40]]
+    slots, _ = cache.slots(_i32(table), _i32([64]), _i32([0, 64]), 64)
+    assert slots.tolist() == _slots_by_rows(cache, table, [64], [0, 64], 64)
+    assert bool((slots[:16] == -2).all()) and bool((slots[32:48] == -2).all())
+    assert bool((slots[16:32] == 7 * 16 + torch.arange(16)).all()) and int(slots[48:].min()) >= 40 * 16
