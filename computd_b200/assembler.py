@@ -49,11 +49,15 @@ def lowrank_rows_workspace(M: int, k: int, n_rows: int, d_B: int,
     """The row-stationary path's scratch (``dwa_lowrank_delta_rows_workspace``
     bytes): one buffer per (device, current stream) that grows on demand and is
     shared by the calls on that stream, which the stream orders (the blocks of
-    a forward).  Calls on other streams get buffers of their own; a CUDA-graph
-    capture allocates its buffer from the graph's pool."""
+    a forward).  Calls on other streams get buffers of their own, and so does every
+    call that is captured, from its graph's pool: a stream's buffer is replaced when a
+    larger call comes, and a graph may be replayed after that, or beside another one."""
     need = int(_lib.load().dwa_lowrank_delta_rows_workspace(M, k, n_rows, d_B))
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(need, 256), dtype=torch.uint8, device=torch.device("cuda", index))
     key = (index, torch.cuda.current_stream(index).cuda_stream)
     ws = _ROWS_WORKSPACE.get(key)
     if ws is None or ws.numel() < need:
