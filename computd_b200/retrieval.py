@@ -389,6 +389,7 @@ class Retriever:
             raise _lib.DWAArgumentError(_lib.DWA_ERR_UNSUPPORTED_SHAPE, "Retriever",
                                         "no workspace plan for this shape")
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self.workspace[:4].zero_()  # the status word: 0 until a call leaves one
         # cross-shard exchange: "nvlink" (PeerExchange), "nccl" (all-gather +
         # merge) or "auto" (nvlink for an NCCL group of more than one rank)
         if exchange not in ("auto", "nvlink", "nccl"):
