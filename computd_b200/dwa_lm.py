@@ -58,9 +58,11 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .assembler import WeightAssembler
+from .assembly import _check_values
 from .kv_cache import PagedKVCache, verify_drafts
 from .lm_ops import aspect_queries, rope_qk
 from .retrieval import MultiAspectRetrieval, Retriever, project_keys_packed
+from .tiled_topk import _as_bf16_rows
 
 
 @dataclass(frozen=True)
@@ -134,6 +136,37 @@ class ChunkStep:
     q_start: torch.Tensor
     max_q: int
     padded: bool               # rows may follow the last sequence's
+
+
+def plan_rows(tokens: int) -> int:
+    """The row count that a chunk of ``tokens`` rows is planned for: a power of two up to one
+    tile of the score kernel (128 rows), whole tiles up to 1024, then eight counts to an
+    octave: 63 counts up to 65536 rows, and at most an eighth more rows above 1024."""
+    if tokens <= 128:
+        return 1 << max(tokens - 1, 0).bit_length()
+    step = max(128, 1 << ((tokens - 1).bit_length() - 4))
+    return -(-tokens // step) * step
+
+
+class ChunkPlan:
+    """A retrieval plan for chunks of up to its rows: what lies behind a chunk's queries is
+    whatever was there before, and dropped."""
+
+    def __init__(self, retriever: Retriever):
+        self.retriever = retriever
+        self.queries = torch.zeros((retriever.M, retriever.d_k), dtype=torch.bfloat16,
+                                   device=retriever.device)
+
+    @property
+    def keys(self) -> torch.Tensor:
+        return self.retriever.keys
+
+    def __call__(self, queries: torch.Tensor, params: torch.Tensor | None = None):
+        T = queries.shape[0]
+        if T == self.retriever.M:
+            return self.retriever(queries, params=params)
+        self.queries[:T].copy_(queries)
+        return tuple(x if x is None else x[:T] for x in self.retriever(self.queries, params=params))
 
 
 def _rope_theta(dh: int, device) -> torch.Tensor:
@@ -219,12 +252,12 @@ class DWABlock(nn.Module):
                 vectors: torch.Tensor | None = None) -> torch.Tensor:
         return self._assemble(self.attn(h), retriever, vectors)
 
-    def extend(self, h: torch.Tensor, retriever: Retriever, vectors: torch.Tensor | None,
+    def extend(self, h: torch.Tensor, plan: ChunkPlan, vectors: torch.Tensor | None,
                step: ChunkStep, layer: int) -> torch.Tensor:
         """``forward`` over the cache: h [1, T, C], the rows of ``step``."""
-        return self._assemble(self.attn.extend(h, step, layer), retriever, vectors)
+        return self._assemble(self.attn.extend(h, step, layer), plan, vectors)
 
-    def _assemble(self, h: torch.Tensor, retriever: Retriever,
+    def _assemble(self, h: torch.Tensor, retriever: Retriever | ChunkPlan,
                   vectors: torch.Tensor | None) -> torch.Tensor:
         B, S_len, C = h.shape
         cfg = self.cfg
@@ -273,21 +306,50 @@ class DWALM(nn.Module):
             if pool_keys is not None:
                 raise ValueError("with r > 0 the blocks project their own keys: pass pool_keys=None")
             self.vectors = pool_values
-            # one key buffer, rewritten by each block's projection before its retrieval
-            pool_keys = torch.empty((pool_values.shape[0], cfg.key_width), dtype=torch.bfloat16,
-                                    device=device)
             values = None
         else:
             if pool_keys is None or pool_keys.shape[1] != cfg.key_width:
                 raise ValueError(f"pool_keys must be [N, {cfg.key_width}]")
             self.vectors = None
-            values = pool_values
+            # converted once, not by every plan
+            pool_keys, values = _as_bf16_rows(pool_keys, "pool_keys"), _check_values(pool_values)
+
+        def plan(tokens: int) -> Retriever:
+            # r > 0: a key buffer of the plan's own, rewritten by each block's projection before
+            # its retrieval, so that plans may be in use at the same time
+            keys = pool_keys if pool_keys is not None else torch.empty(
+                (pool_values.shape[0], cfg.key_width), dtype=torch.bfloat16, device=device)
+            return Retriever(keys, values, tokens, cfg.top_k, lambda_sharp=cfg.lambda_sharp, T=cfg.T,
+                             use_sigmoid=cfg.use_sigmoid, group=group)
+
+        self._plan = plan
         # one retrieval plan shared by all blocks (same pool, same token count)
-        self._plan = lambda tokens: Retriever(pool_keys, values, tokens, cfg.top_k,
-                                              lambda_sharp=cfg.lambda_sharp, T=cfg.T,
-                                              use_sigmoid=cfg.use_sigmoid, group=group)
-        self.retriever = self._plan(cfg.tokens)
-        self._chunk_retrievers = {cfg.tokens: self.retriever}
+        self.retriever = plan(cfg.tokens)
+        self._chunk_plans: dict[int, ChunkPlan] = {}
+
+    def _chunk_plan(self, tokens: int) -> ChunkPlan:
+        """The plan of chunks of ``tokens`` rows; made where there is none."""
+        rows = plan_rows(tokens)
+        plan = self._chunk_plans.get(rows)
+        if plan is None:
+            plan = self._chunk_plans[rows] = ChunkPlan(self._plan(rows))
+        return plan
+
+    def _retrievers(self) -> list[Retriever]:
+        return [self.retriever] + [p.retriever for p in self._chunk_plans.values()]
+
+    def status(self) -> int:
+        """The first device status that a retrieval of any call so far left (0: none; waits for the
+        device)."""
+        torch.cuda.synchronize(self.embed.weight.device)
+        return next((s for s in (r.status() for r in self._retrievers()) if s), 0)
+
+    def close(self) -> None:
+        """Releases the plans' exchange buffers (collective on a sharded pool: every rank, after its
+        last call).  The model is unusable afterwards."""
+        for r in self._retrievers():
+            r.close()
+        self._chunk_plans.clear()
 
     @torch.no_grad()
     def forward(self, token_ids: torch.Tensor) -> torch.Tensor:
@@ -313,13 +375,14 @@ class DWALM(nn.Module):
         [B + 1]) of sequence b, or T / B rows each without ``q_start``.  ``lengths`` int32 [B]
         counts each sequence's tokens, the new ones with them, and ``block_table`` int32
         [B, max_pages] holds its pages.  ``max_q`` bounds the new tokens of any sequence.
-        Rows behind the last sequence (a padded batch; their tokens are in the vocabulary too)
-        attend to nothing.
+        Rows of no sequence (a padded batch; their tokens are in the vocabulary too) attend to
+        nothing.
 
-        The retrieval is planned once per row count T (a captured graph needs a call with its
-        T before), so a server pads T to a few counts; calls with the same T share the plan's
-        workspace and belong on one stream.  On a row-sharded pool every rank calls with the
-        same tokens."""
+        The retrieval is planned once for all row counts T that ``plan_rows`` rounds to the
+        same (a captured graph needs such a call before).  Calls that share a plan share its
+        buffers: they, and the graphs that hold them, belong on one stream.  Calls of different
+        plans, and ``forward``, may run on different streams at the same time.  On a row-sharded pool every rank calls with
+        the same tokens in the same order."""
         T = token_ids.shape[0]
         if token_ids.dim() != 1:
             raise ValueError("token_ids must be [T]")
@@ -333,9 +396,7 @@ class DWALM(nn.Module):
             max_q = T // B
         if T == 0:
             return torch.empty((0, self.cfg.vocab), dtype=self.fc2.weight.dtype, device=token_ids.device)
-        retriever = self._chunk_retrievers.get(T)
-        if retriever is None:
-            retriever = self._chunk_retrievers[T] = self._plan(T)
+        plan = self._chunk_plan(T)
         slots, positions = cache.slots(block_table, lengths, q_start, T)
         dh = self.cfg.d_model // self.cfg.n_heads
         f = torch.outer(positions.float(), _rope_theta(dh, positions.device))
@@ -344,7 +405,7 @@ class DWALM(nn.Module):
                          q_start, T if max_q is None else max_q, padded)
         h = self.embed_norm(self.embed_proj(self.embed(token_ids[None])))
         for i, blk in enumerate(self.blocks):
-            h = blk.extend(h, retriever, self.vectors, step, i)
+            h = blk.extend(h, plan, self.vectors, step, i)
         return self.fc2(F.gelu(self.fc1(self.head_norm(h))))[0]
 
     @torch.no_grad()

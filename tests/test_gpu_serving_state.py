@@ -58,3 +58,89 @@ def test_captured_rows_workspace_is_the_graphs_own():
     assert all(bool((x == 255).all()) for x in junk)
     for (_, out), x in zip(graphs, want):
         assert torch.equal(out, x)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _prompt(cfg, model, b, n, page_size=16):
+    """A cache of one layout, a table and n tokens of b sequences, alike for the same arguments."""
+    cache = model.new_cache(b * (-(-64 // page_size)), page_size=page_size)
+    table = torch.arange(cache.n_pages, device="cuda").int().view(b, -1)
+    ids = torch.randint(0, cfg.vocab, (b, n), device="cuda", generator=torch.Generator("cuda").manual_seed(b + n))
+    return cache, table, ids.reshape(-1), _i32([n] * b)
+
+
+@pytest.mark.parametrize("r", [0, 2])
+def test_plans_are_few_and_their_own(r):
+    """Chunks of every row count from 1 to 150 make eight plans and one of 256; with r > 0 each
+    has keys of its own; a plan's status and the model's are read; closed plans are gone."""
+    from test_gpu_lm_extend import _model
+
+    cfg, model = _model(r=r, dh=16 if r else 32, layers=1)
+    cache, table, ids, _ = _prompt(cfg, model, 3, 50)
+    for n in range(1, 151):
+        seqs = 1 if n <= 50 else 3
+        new = [n] if seqs == 1 else [50, 50, n - 100] if n > 100 else [50, n - 50, 0]
+        start = _i32([sum(new[:b]) for b in range(seqs + 1)])
+        model.extend(ids[:n], cache, table[:seqs], _i32(new), start, 50)
+    assert sorted(model._chunk_plans) == [1, 2, 4, 8, 16, 32, 64, 128, 256]
+    keys = [p.keys.data_ptr() for p in model._chunk_plans.values()] + [model.retriever.keys.data_ptr()]
+    assert len(set(keys)) == (len(keys) if r else 1)
+    assert model.status() == 0
+    plan = model._chunk_plans[64].retriever
+    was, plan.status = plan.status, lambda: 7
+    assert model.status() == 7
+    plan.status = was
+    cache.check()
+    model.close()
+    assert not model._chunk_plans
+
+
+@pytest.mark.parametrize("r", [0, 2])
+@pytest.mark.parametrize("T", [1, 3, 65, 127, 129, 190])
+def test_padded_plans_give_the_same(r, T):
+    """A chunk's retrieval over a plan of more rows is bit for bit that of a plan of its own, also
+    where the rows behind it held other queries."""
+    import computd_b200 as cb
+    from test_gpu_lm_extend import _model
+
+    from computd_b200.dwa_lm import ChunkPlan
+
+    cfg, model = _model(r=r, dh=16 if r else 32, layers=1)
+    keys = cb.new_normal(cfg.pool_rows, cfg.key_width, seed=5, stddev=cfg.key_width ** -0.5, device="cuda")
+    g = torch.Generator("cuda").manual_seed(T)
+    exact, padded = ChunkPlan(model._plan(T)), model._chunk_plan(T)
+    for plan in (exact, padded):
+        plan.keys.copy_(keys)
+    padded(torch.randn((padded.retriever.M, cfg.key_width), device="cuda", generator=g).bfloat16())
+    q = torch.randn((T, cfg.key_width), device="cuda", generator=g).bfloat16()
+    for x, y in zip(exact(q), padded(q)):
+        assert (x is None) == (y is None)
+        if x is not None:
+            assert x.shape[0] == y.shape[0] == T and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("r", [0, 2])
+def test_two_row_counts_on_two_streams(r):
+    """A prompt's chunk and single tokens of other sequences at the same time: what each alone gives."""
+    from test_gpu_lm_extend import _model
+
+    cfg, model = _model(r=r, dh=16 if r else 32, layers=4)
+    for blk in model.blocks[1:]:  # blocks whose keys differ: another block's are wrong
+        blk.retrieval.W_Q.copy_(blk.retrieval.W_Q.roll(1, -1))
+    work = [_prompt(cfg, model, 3, 60), _prompt(cfg, model, 2, 1), _prompt(cfg, model, 5, 7)]
+    call = lambda w: model.extend(w[2], w[0], w[1], w[3])  # noqa: E731
+    want = [call(w).clone() for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[] for _ in work]
+    for _ in range(30):
+        for w, s, out in zip(work, streams, got):
+            with torch.cuda.stream(s):
+                out.append(call(w))
+    torch.cuda.synchronize()
+    for x, out in zip(want, got):
+        assert all(torch.equal(x, y) for y in out)
+    assert model.status() == 0

@@ -51,3 +51,15 @@ def test_slots_on_bad_pages_are_not_skipped():
     assert slots.tolist() == _slots_by_rows(cache, table, [64], [0, 64], 64)
     assert bool((slots[:16] == -2).all()) and bool((slots[32:48] == -2).all())
     assert bool((slots[16:32] == 7 * 16 + torch.arange(16)).all()) and int(slots[48:].min()) >= 40 * 16
+
+
+def test_row_counts_are_planned_for_a_few():
+    from computd_b200.dwa_lm import plan_rows
+
+    counts = [plan_rows(t) for t in range(1, 65537)]
+    assert all(c >= t for t, c in enumerate(counts, 1)) and counts == sorted(counts)
+    assert len(set(counts)) == 63
+    assert all(plan_rows(c) == c for c in set(counts))
+    assert [plan_rows(t) for t in (0, 1, 2, 3, 64, 65, 128, 129, 1024, 1025)] == \
+        [1, 1, 2, 4, 64, 128, 128, 256, 1024, 1152]
+    assert all(8 * (c - t) <= t for t, c in enumerate(counts, 1) if t > 1024)
