@@ -422,7 +422,10 @@ class DWALM(nn.Module):
         ``block_table`` must have room for K + 1 more.  Sequence b has ``draft_lengths[b]``
         drafts (int32 [B], default K each); what follows them may be any number.  Returns (n_accepted int32 [B],
         tokens int32 [B, K + 1] as ``verify_drafts``, new lengths int32 [B]: the cached tokens
-        that stay).  tokens[b, n_accepted[b]] is the next step's ``last_tokens[b]``."""
+        that stay).  tokens[b, n_accepted[b]] is the next step's ``last_tokens[b]``.
+        ``temperature`` divides the logits and is positive (for the best token alone, a small one)."""
+        if not isinstance(temperature, torch.Tensor) and not 1e-30 <= temperature <= 1e30:
+            raise ValueError(f"temperature must be a positive number, of 1e-30 to 1e30 (got {temperature})")
         B, K = draft_tokens.shape
         chunk = torch.cat([last_tokens.view(B, 1).to(draft_tokens.dtype), draft_tokens], 1)
         chunk = chunk.clamp(0, self.cfg.vocab - 1)  # a draft outside falls below

@@ -63,3 +63,35 @@ def test_row_counts_are_planned_for_a_few():
     assert [plan_rows(t) for t in (0, 1, 2, 3, 64, 65, 128, 129, 1024, 1025)] == \
         [1, 1, 2, 4, 64, 128, 128, 256, 1024, 1152]
     assert all(8 * (c - t) <= t for t, c in enumerate(counts, 1) if t > 1024)
+
+
+class _Model:
+    """What ``DWALM.verify`` needs of a model; its chunk forward notes that it was called."""
+
+    def __init__(self, vocab=11):
+        from types import SimpleNamespace
+
+        self.cfg, self.calls = SimpleNamespace(vocab=vocab), []
+
+    def extend(self, token_ids, cache, block_table, lengths, *a, **kw):
+        self.calls.append((token_ids.tolist(), lengths.tolist()))
+        return torch.zeros((token_ids.shape[0], self.cfg.vocab))
+
+
+def _verify(model, cache, last, drafts, **kw):
+    from computd_b200.dwa_lm import DWALM
+
+    B, K = drafts.shape
+    a = dict(draft_probs=None, accept_u=torch.zeros(B, K), sample_u=torch.zeros(B), temperature=1.0,
+             draft_lengths=None)
+    a.update(kw)
+    return DWALM.verify(model, last, drafts, a.pop("draft_probs"), a.pop("accept_u"), a.pop("sample_u"), cache,
+                        torch.zeros((B, 4), dtype=torch.int32), torch.full((B,), 9, dtype=torch.int32), **a)
+
+
+@pytest.mark.parametrize("temperature", [0, 0.0, -1.0, float("nan"), float("inf"), 1e-46])
+def test_verify_refuses_temperatures(temperature):
+    model = _Model()
+    with pytest.raises(ValueError, match="temperature"):
+        _verify(model, _cache(), _i32([1, 2]), _i32([[3, 4], [5, 6]]), temperature=temperature)
+    assert not model.calls
