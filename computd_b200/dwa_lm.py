@@ -426,7 +426,21 @@ class DWALM(nn.Module):
         ``temperature`` divides the logits and is positive (for the best token alone, a small one)."""
         if not isinstance(temperature, torch.Tensor) and not 1e-30 <= temperature <= 1e30:
             raise ValueError(f"temperature must be a positive number, of 1e-30 to 1e30 (got {temperature})")
+        if draft_tokens.dim() != 2:
+            raise ValueError("draft_tokens must be int32 [B, K]")
         B, K = draft_tokens.shape
+        # before the chunk is written: verify_drafts would refuse these after it
+        for name, t, dtype, shape in (("draft_tokens", draft_tokens, torch.int32, (B, K)),
+                                      ("draft_probs", draft_probs, torch.float32, (B, K, self.cfg.vocab)),
+                                      ("accept_u", accept_u, torch.float32, (B, K)),
+                                      ("sample_u", sample_u, torch.float32, (B,)),
+                                      ("draft_lengths", draft_lengths, torch.int32, (B,))):
+            if t is None and name in ("draft_probs", "draft_lengths"):
+                continue
+            if t is None or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)}")
+        if last_tokens.numel() != B or last_tokens.is_floating_point():
+            raise ValueError(f"last_tokens must be integers [{B}]")
         chunk = torch.cat([last_tokens.view(B, 1).to(draft_tokens.dtype), draft_tokens], 1)
         chunk = chunk.clamp(0, self.cfg.vocab - 1)  # a draft outside falls below
         logits = self.extend(chunk.reshape(-1).long(), cache, block_table, lengths + (K + 1))

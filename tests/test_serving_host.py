@@ -95,3 +95,19 @@ def test_verify_refuses_temperatures(temperature):
     with pytest.raises(ValueError, match="temperature"):
         _verify(model, _cache(), _i32([1, 2]), _i32([[3, 4], [5, 6]]), temperature=temperature)
     assert not model.calls
+
+
+def test_verify_refuses_before_anything_is_written():
+    """What verify_drafts would refuse afterwards, with the chunk already in the cache."""
+    good = dict(last=_i32([1, 2]), drafts=_i32([[3, 4], [5, 6]]))
+    bad = [dict(drafts=good["drafts"].long()), dict(drafts=good["drafts"].float()), dict(drafts=_i32([3, 4])),
+           dict(last=_i32([1, 2, 3])), dict(last=torch.zeros(2)), dict(accept_u=torch.zeros(2, 3)),
+           dict(accept_u=torch.zeros(2, 2).double()), dict(sample_u=torch.zeros(3)),
+           dict(draft_probs=torch.zeros(2, 2, 12)), dict(draft_probs=torch.zeros(2, 2, 11).bfloat16()),
+           dict(draft_probs=torch.zeros(2, 11, 2).transpose(1, 2)), dict(draft_lengths=torch.zeros(2)),
+           dict(draft_lengths=_i32([1]))]
+    for kw in bad:
+        model, a = _Model(), {**good, **kw}
+        with pytest.raises(ValueError):
+            _verify(model, _cache(), a.pop("last"), a.pop("drafts"), **a)
+        assert not model.calls, kw
