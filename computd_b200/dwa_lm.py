@@ -422,7 +422,9 @@ class DWALM(nn.Module):
         ``block_table`` must have room for K + 1 more.  Sequence b has ``draft_lengths[b]``
         drafts (int32 [B], default K each); what follows them may be any number.  Returns (n_accepted int32 [B],
         tokens int32 [B, K + 1] as ``verify_drafts``, new lengths int32 [B]: the cached tokens
-        that stay).  tokens[b, n_accepted[b]] is the next step's ``last_tokens[b]``.
+        that stay).  tokens[b, n_accepted[b]] is the next step's ``last_tokens[b]``.  A last token
+        outside the vocabulary (the -1 of a step without probability mass) is reported in the
+        cache's status; its sequence gets no tokens, only -1, and stays as long as it was.
         ``temperature`` divides the logits and is positive (for the best token alone, a small one)."""
         if not isinstance(temperature, torch.Tensor) and not 1e-30 <= temperature <= 1e30:
             raise ValueError(f"temperature must be a positive number, of 1e-30 to 1e30 (got {temperature})")
@@ -443,11 +445,15 @@ class DWALM(nn.Module):
             raise ValueError(f"last_tokens must be integers [{B}]")
         chunk = torch.cat([last_tokens.view(B, 1).to(draft_tokens.dtype), draft_tokens], 1)
         chunk = chunk.clamp(0, self.cfg.vocab - 1)  # a draft outside falls below
+        last = last_tokens.view(B)
+        lost = (last < 0) | (last >= self.cfg.vocab)
         logits = self.extend(chunk.reshape(-1).long(), cache, block_table, lengths + (K + 1))
         probs = torch.softmax(logits.float().view(B, K + 1, -1) / temperature, -1)
         accepted, tokens = verify_drafts(probs, draft_tokens, draft_probs, accept_u, sample_u,
                                          draft_lengths=draft_lengths)
-        return accepted, tokens, lengths + 1 + accepted
+        cache.report(lost)
+        accepted = torch.where(lost, 0, accepted)
+        return accepted, torch.where(lost[:, None], -1, tokens), torch.where(lost, lengths, lengths + 1 + accepted)
 
 
 class GraphedForward:

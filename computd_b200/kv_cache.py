@@ -131,7 +131,7 @@ class PagedKVCache:
         if dtype is _E4M3:
             self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=_F32, device=device)
                                           for _ in range(2))
-        # DWA_ERR_DEVICE_CHECK once a call met a bad slot, page, length or row range
+        # DWA_ERR_DEVICE_CHECK once a call met a bad slot, page, length, row range or last token
         self.status = torch.zeros((), dtype=_I32, device=device)
 
     def _layer(self, layer: int):
@@ -175,14 +175,19 @@ class PagedKVCache:
         slot = torch.where(page < 0, -2, page * self.page_size + at % self.page_size)
         return torch.where(fine, slot, -1), at
 
+    def report(self, bad: torch.Tensor) -> None:
+        """Note in ``status``, as the calls do, where ``bad`` (bool, any shape) has a true value."""
+        code = torch.where(bad.any(), _lib.DWA_ERR_DEVICE_CHECK, 0).to(_I32)
+        self.status.copy_(torch.where(self.status == 0, code, self.status))
+
     def check(self) -> None:
-        """Raise ``DWAError`` if a call so far met a bad slot, page, length or row range (waits
-        for the device)."""
+        """Raise ``DWAError`` if a call so far met a bad slot, page, length, row range or last
+        token (waits for the device)."""
         code = int(self.status.item())
         if code:
             self.status.zero_()
-            raise _lib.DWAError(code, "PagedKVCache", "a slot, page number, length or row range was "
-                                "outside the cache or the call")
+            raise _lib.DWAError(code, "PagedKVCache", "a slot, page number, length, row range or last "
+                                "token was outside the cache, the call or the vocabulary")
 
 
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor,

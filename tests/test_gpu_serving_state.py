@@ -144,3 +144,38 @@ def test_two_row_counts_on_two_streams(r):
     for x, out in zip(want, got):
         assert all(torch.equal(x, y) for y in out)
     assert model.status() == 0
+
+
+def test_verify_with_a_lost_last_token():
+    """A sequence whose last token is -1, among others: reported, -1, unchanged; the others as alone;
+    captured and replayed it does the same."""
+    import computd_b200 as cb
+    from test_gpu_lm_extend import _model
+
+    cfg, model = _model(seed=4)
+    cache, table, ids, lengths = _prompt(cfg, model, 3, 20)
+    model.extend(ids, cache, table, lengths)
+    g = torch.Generator("cuda").manual_seed(1)
+    drafts = torch.randint(0, cfg.vocab, (3, 4), device="cuda", generator=g).int()
+    u, r = torch.zeros((3, 4), device="cuda"), torch.rand(3, device="cuda", generator=g)
+    good = _i32([3, 9, 60])
+    want = [t.clone() for t in model.verify(good, drafts, None, u, r, cache, table, lengths)]
+    cache.check()
+    last = _i32([3, -1, 60])
+    for _ in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = model.verify(last, drafts, None, u, r, cache, table, lengths)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                again = model.verify(last, drafts, None, u, r, cache, table, lengths)
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for (accepted, tokens, new) in (got, again):
+            for b in (0, 2):
+                assert all(torch.equal(x[b], y[b]) for x, y in zip((accepted, tokens, new), want))
+            assert accepted[1] == 0 and tokens[1].tolist() == [-1] * 5 and new[1] == 20
+        with pytest.raises(cb.DWAError):
+            cache.check()
+        cache.check()

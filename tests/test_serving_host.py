@@ -111,3 +111,30 @@ def test_verify_refuses_before_anything_is_written():
         with pytest.raises(ValueError):
             _verify(model, _cache(), a.pop("last"), a.pop("drafts"), **a)
         assert not model.calls, kw
+
+
+def test_verify_reports_last_tokens_outside_the_vocabulary(monkeypatch):
+    """Their sequences get no tokens and stay as long as they were, and the cache's status says so;
+    the others go on."""
+    import computd_b200.dwa_lm as lm
+    from computd_b200 import DWAError
+
+    def decide(probs, drafts, *a, **kw):
+        B, K = drafts.shape
+        return torch.arange(B, dtype=torch.int32) % (K + 1), torch.full((B, K + 1), 5, dtype=torch.int32)
+
+    monkeypatch.setattr(lm, "verify_drafts", decide)
+    for last, bad in (([1, -1, 10, 11, 2 ** 31 - 1], [1, 3, 4]), ([0, 10, 3, 4, 5], [])):
+        model, cache = _Model(), _cache()
+        accepted, tokens, lengths = _verify(model, cache, _i32(last), torch.full((5, 3), 2, dtype=torch.int32))
+        ids, asked = model.calls[0]
+        assert asked == [13] * 5 and all(0 <= x < 11 for x in ids)
+        for b in range(5):
+            assert accepted[b] == (0 if b in bad else b % 4)
+            assert tokens[b].tolist() == ([-1] * 4 if b in bad else [5] * 4)
+            assert lengths[b] == (9 if b in bad else 10 + b % 4)
+        assert lengths.dtype == accepted.dtype == tokens.dtype == torch.int32
+        if bad:
+            with pytest.raises(DWAError):
+                cache.check()
+        cache.check()
