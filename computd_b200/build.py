@@ -8,7 +8,8 @@ linked with a static CUDA runtime, so the library does not depend on the
 runtime version torch ships.  ``csrc/host/serving.cpp``, the Python side of the
 serving calls, becomes the extension module ``computd_b200/_serving.so`` (host
 compiler, torch's headers).  Objects are rebuilt when a source or header is
-newer than them.
+newer than them, the extension also when torch or Python is another than it was
+built for.
 """
 from __future__ import annotations
 
@@ -79,6 +80,27 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool, extra: list[str]) -
         raise RuntimeError(f"nvcc failed on {src.name}")
 
 
+def _host_built_for() -> str:
+    """What the extension module depends on beside its sources: the installed torch and Python."""
+    import torch
+
+    return f"{torch.__version__}\n{Path(torch.__file__).resolve().parent}\n{sys.version}\n"
+
+
+def _host_note() -> Path:
+    return BUILD_DIR / "serving_built_for.txt"
+
+
+def _note_host() -> None:
+    _host_note().write_text(_host_built_for())
+
+
+def _host_stale() -> bool:
+    note = _host_note()
+    return (_stale(HOST_PATH, [HOST_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__)])
+            or not note.exists() or note.read_text() != _host_built_for())
+
+
 def _build_host(verbose: bool) -> None:
     """The extension module of the serving calls, against the installed torch and Python."""
     import sysconfig
@@ -107,6 +129,7 @@ def _build_host(verbose: bool) -> None:
     if res.returncode != 0:
         raise RuntimeError(f"{cxx} failed on {HOST_SOURCE.name}")
     os.replace(tmp, HOST_PATH)
+    _note_host()
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
@@ -122,7 +145,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         objs.append(obj)
         if force or _stale(obj, [src, *headers, Path(__file__)]):
             jobs.append((src, obj))
-    host = force or _stale(HOST_PATH, [HOST_SOURCE, *INCLUDE_DIR.glob("*.h"), Path(__file__)])
+    host = force or _host_stale()
     if jobs or host:
         with cf.ThreadPoolExecutor(max_workers=min(len(jobs) + 1, os.cpu_count() or 4)) as ex:
             futs = [ex.submit(_compile, nvcc, s, o, verbose, extra) for s, o in jobs]
