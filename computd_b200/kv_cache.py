@@ -18,7 +18,8 @@ s // page_size.  Every call is asynchronous on the current stream, allocates
 nothing but its outputs, never waits for the device and can be captured in a
 CUDA graph; none has gradients.  Values that only the device sees (slots, page numbers, lengths) are
 checked there: a bad one leads to no access but to NaN rows (or a skipped write),
-and to ``DWA_ERR_DEVICE_CHECK`` in ``status``, an int32 device word, when given.
+and to ``DWA_ERR_DEVICE_CHECK`` in ``status``, an int32 device word, when given.  (Rows
+that a bad row range leaves to no sequence stay as they were.)
 """
 from __future__ import annotations
 
@@ -74,7 +75,8 @@ def kv_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Ten
     """Keys and values of slots ``slots`` (int64 [T]) as bf16 [T, H_kv, d] each.
 
     With ``out`` (two contiguous tensors) the rows of slot -1 stay as they were; without
-    it they are zeros."""
+    it they are zeros, and the two results are parts of one allocation: keeping (or saving)
+    one keeps both, unless it is cloned."""
     return (_host_module or _host()).kv_read(k_cache, v_cache, slots, k_scale, v_scale, out, status)
 
 
@@ -92,11 +94,13 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with them; ``block_table`` int32 [B, max_pages] holds their pages in order.  New
     token i of n attends to the first length - n + i + 1 tokens, query head h to
     key/value head h // (H / H_kv); ``scale`` defaults to d ** -0.5.  A row that sees
-    nothing is zeros; rows from q_start[B] on are left as they were in ``out``, and without
-    it hold anything.
+    nothing is zeros; rows of no sequence (before q_start[0], from q_start[B] on) are left as
+    they were in ``out``, and without it hold anything.
 
     ``max_q`` bounds the new tokens of any one sequence (default: T); the host picks
-    the kernel by it, so a close bound is faster.  A sequence with more gets NaN.
+    the kernel by it, so a close bound is faster.  A sequence with more gets NaN.  Up to 16
+    rows per key/value head (max_q H / H_kv) the probabilities over a bf16 cache keep 16 bits,
+    beyond that 8 (over an e4m3 cache 11 either way), as include/dwa_decode.h says.
 
     What a row may not see does not reach it, NaN and infinities included.  (A new
     token's value that is not finite makes the rows that do see it not finite in its
@@ -204,6 +208,6 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor,
     follows, so that the tokens are distributed as the target's.
 
     Returns (n_accepted int32 [B], tokens int32 [B, K + 1]: the standing drafts, the drawn
-    token, then -1)."""
+    token, then -1), two parts of one allocation."""
     return (_host_module or _host()).verify(target_probs, draft_tokens, draft_probs, accept_u, sample_u,
                                             draft_lengths)

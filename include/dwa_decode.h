@@ -18,7 +18,9 @@
  *
  * What only the device can see is checked there: a bad slot, page number,
  * length or row range never leads to an access; it writes DWA_ERR_DEVICE_CHECK
- * to *status (device int32, may be NULL) and NaN to the rows concerned.
+ * to *status (device int32, may be NULL) and NaN to the rows concerned.  (A row
+ * range that is none, descending or outside q, says of no row whose it is: rows that
+ * no other sequence has stay as they were.)
  */
 #ifndef DWA_DECODE_H_
 #define DWA_DECODE_H_
@@ -69,11 +71,15 @@ DWA_API dwa_status dwa_kv_read(const void* k_cache, const void* v_cache, const f
  *   j < length - n + i + 1,
  * with the key and value head h / (H / H_kv); no key, or no score above -inf,
  * gives zeros.  q, out bf16 [T][H][d] with row strides q_ld / out_ld (elements;
- * heads contiguous).  Rows from q_start[B] on are left as they were.  max_q
+ * heads contiguous).  Rows of no sequence are left as they were.  max_q
  * bounds every sequence's new tokens; a sequence may have 2^30 tokens.  Keys that
- * a row may not see do not reach it, whatever their bits.  A new token's value that
- * is not finite makes the rows that do see it not finite in its channel (an infinity
- * may become NaN).
+ * a row may not see do not reach it, whatever their bits and sizes.  A new token's
+ * value that is not finite makes the rows that do see it not finite in its channel (an
+ * infinity may become NaN).
+ * Rounding, beside f32 sums and the result's: up to 16 rows per key/value head
+ * (max_q H / H_kv), bf16 caches none (p_j as the sum of two bf16), e4m3 caches p_j
+ * times its value's scale to 11 bits; more rows, bf16 caches p_j to 8 bits, e4m3
+ * caches p_j, k_j and v_j to 11 bits each.
  */
 DWA_API dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
                                        const void* k_cache, const void* v_cache,
