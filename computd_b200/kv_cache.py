@@ -180,9 +180,10 @@ class PagedKVCache:
         return torch.where(fine, slot, -1), at
 
     def report(self, bad: torch.Tensor) -> None:
-        """Note in ``status``, as the calls do, where ``bad`` (bool, any shape) has a true value."""
-        code = torch.where(bad.any(), _lib.DWA_ERR_DEVICE_CHECK, 0).to(_I32)
-        self.status.copy_(torch.where(self.status == 0, code, self.status))
+        """Note in ``status`` that ``bad`` (bool, any shape) has a true value, if it has; by an atomic
+        maximum, as calls on other streams may note something at the same time."""
+        codes = torch.where(bad.flatten(), _lib.DWA_ERR_DEVICE_CHECK, 0).to(_I32)
+        self.status.view(1).scatter_reduce_(0, torch.zeros_like(codes, dtype=torch.int64), codes, "amax")
 
     def check(self) -> None:
         """Raise ``DWAError`` if a call so far met a bad slot, page, length, row range or last
