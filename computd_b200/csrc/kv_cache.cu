@@ -14,6 +14,7 @@
 #include "dwa_internal.h"
 #include "dwa_retrieval.h"
 #include "f32x2.cuh"
+#include "paged_attention.cuh"
 
 namespace dwa {
 
@@ -27,10 +28,6 @@ template <bool kE4m3, bool kSrcBf16>
 constexpr int kWriteBlocks = !kSrcBf16 ? 2 : kE4m3 ? 3 : 4;
 constexpr int kBlockTokens = 32;  // at most; a longer call is cut into launches
 constexpr int kFilterBits = 8192;  // their slots' low bits
-
-__device__ __forceinline__ void report(int32_t* status) {
-  if (status != nullptr) atomicCAS(status, 0, DWA_ERR_DEVICE_CHECK);
-}
 
 // Values of a lane: sixteen make 16 bytes of codes, eight 16 bytes of bf16.
 template <bool kE4m3>
@@ -227,7 +224,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<kE4m3, kSrcBf16>)
   for (int i = threadIdx.x; i < n; i += kWriteThreads) {
     const int64_t s = a.slots[t0 + i];
     const bool fine = s >= 0 && s < a.n_slots;
-    if (!fine && s != -1) report(a.status);
+    if (!fine && s != -1) paged_report(a.status);
     own[i] = s;
     dropped[i] = fine ? 0 : 1;
     if (fine) atomicOr(&filter[(s & (kFilterBits - 1)) >> 5], 1u << (s & 31));
@@ -375,7 +372,7 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a)
       put8<kE4m3>(k[i], k_out);
       put8<kE4m3>(v[i], v_out);
     } else {
-      if (!skipped) report(a.status);
+      if (!skipped) paged_report(a.status);
       const uint32_t fill = skipped ? 0u : 0x7FC07FC0u;  // zeros, or NaN for a slot outside the cache
       *reinterpret_cast<uint4*>(k_out) = make_uint4(fill, fill, fill, fill);
       *reinterpret_cast<uint4*>(v_out) = make_uint4(fill, fill, fill, fill);

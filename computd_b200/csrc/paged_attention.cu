@@ -135,16 +135,6 @@ __device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// (channel, token of the page, half of the channels, head, page)
-__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                              int y, int half, int head, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(half), "r"(head), "r"(page)
-      : "memory");
-}
-
 // kLinear: the rows of a block lie one behind the other, as in the page.
 template <bool kE4m3, int DP, int NT, int W, bool kLinear>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
@@ -277,19 +267,19 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
           bulk_load(dst + C::kBoxes * C::kBoxBytes + tile, rows_of(a.v, page1, y1), tile, bar);
         }
       } else if (C::kSub == 2) {
-        tma_load_rows(dst, &map_k, bar, 0, y, 0, hk, page0);
-        tma_load_rows(dst + 2 * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
+        tma_load_page(dst, &map_k, bar, 0, y, 0, hk, page0);
+        tma_load_page(dst + 2 * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
         if (two && !wide) {
           const int y1 = (key + 16) & page_mask;
-          tma_load_rows(dst + C::kBoxBytes, &map_k, bar, 0, y1, 0, hk, page1);
-          tma_load_rows(dst + 3 * C::kBoxBytes, &map_v, bar, 0, y1, 0, hk, page1);
+          tma_load_page(dst + C::kBoxBytes, &map_k, bar, 0, y1, 0, hk, page1);
+          tma_load_page(dst + 3 * C::kBoxBytes, &map_v, bar, 0, y1, 0, hk, page1);
         }
       } else {
-        tma_load_rows(dst, &map_k, bar, 0, y, 0, hk, page0);
-        tma_load_rows(dst + C::kHalves * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
+        tma_load_page(dst, &map_k, bar, 0, y, 0, hk, page0);
+        tma_load_page(dst + C::kHalves * C::kBoxBytes, &map_v, bar, 0, y, 0, hk, page0);
         if (C::kHalves == 2 && !wide) {
-          tma_load_rows(dst + C::kBoxBytes, &map_k, bar, 64, y, 0, hk, page0);
-          tma_load_rows(dst + 3 * C::kBoxBytes, &map_v, bar, 64, y, 0, hk, page0);
+          tma_load_page(dst + C::kBoxBytes, &map_k, bar, 64, y, 0, hk, page0);
+          tma_load_page(dst + 3 * C::kBoxBytes, &map_v, bar, 64, y, 0, hk, page0);
         }
       }
     }

@@ -219,6 +219,16 @@ __device__ __forceinline__ void min_cluster_s32(uint32_t addr, int x) {
 bool make_page_map(CUtensorMap* map, const void* ptr, const PagedArgs& a, int row_bytes, int box_rows,
                    int box_halves);
 
+// One box of it, at these coordinates.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                              int y, int half, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(half), "r"(head), "r"(page)
+      : "memory");
+}
+
 // Lets a kernel have its dynamic shared memory, once per device.
 template <auto kKernel>
 cudaError_t allow_smem_once(int bytes) {

@@ -296,17 +296,6 @@ __device__ __forceinline__ uint64_t desc64(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-// (channel, token of the page, half of the channels, head, page)
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
-                                            int y, int half, int head, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(half), "r"(head), "r"(page)
-      : "memory");
-}
-
-
 // Rows at equal distances as (new token, query head of the group), divided once.
 struct RowWalk {
   uint32_t token, head;
@@ -439,11 +428,11 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const CUtensorMap* map = (it & 1) ? &map_v : &map_k;
       const uint32_t dst = s_stage + st * C::kStageBytes;
       if constexpr (kE4m3) {
-        tma_load_5d(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, 0, hk, page);
+        tma_load_page(dst + C::kRawAt + lane * page_size * DP, map, full, 0, 0, 0, hk, page);
       } else {
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h)
-          tma_load_5d(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, 0, hk, page);
+          tma_load_page(dst + h * C::kBlockBytes + lane * page_size * 128, map, full, 64 * h, 0, 0, hk, page);
       }
     }
   };
