@@ -14,10 +14,12 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
 #include <cmath>
+#include <exception>
 #include <sstream>
 #include <string>
 
@@ -189,8 +191,8 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F&& body) {
     return body();
   } catch (const Refusal& e) {
     PyErr_SetString(e.type, e.what.c_str());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {  // as torch's own functions raise it: out of memory has a type of its own
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

@@ -179,3 +179,21 @@ def test_verify_with_a_lost_last_token():
         with pytest.raises(cb.DWAError):
             cache.check()
         cache.check()
+
+
+def test_an_output_that_does_not_fit_is_torchs_own_error():
+    """A server that makes room and tries again catches torch.OutOfMemoryError."""
+    import computd_b200 as cb
+
+    cache = torch.zeros((1, 64, 16, 128), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    slots = torch.full((1 << 18,), -1, dtype=torch.int64, device="cuda")  # 8 GB of keys and values
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (4 << 30)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            cb.kv_cache_read(cache, cache, slots)
+        k, v = cb.kv_cache_read(cache, cache, slots[:64])
+        assert not bool(k.any()) and not bool(v.any())
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
