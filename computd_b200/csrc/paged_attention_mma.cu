@@ -45,8 +45,8 @@
 // scales are far smaller, for the sake of one that a row may not even see.  So from the step on
 // where scales leave a range of 2^12, operands keep their scales' mantissas only, and the row's
 // thread multiplies scores and weights by the powers of two after all, in units of its own: 2048
-// rows over 8192 keys, 32 heads, 283 us, and 550 to 590 where that starts at once.  (The check
-// and the second form's code cost the first 1 to 5 %.)
+// rows over 8192 keys, 32 heads, 280 us, and 525 to 580 where that starts at once.  (The check
+// and the second form's code cost the first 2 to 4 %.)
 //
 // Where there are few units of 256 rows, a cluster of blocks shares the keys of one
 // and joins its parts through distributed shared memory, in a fixed order.
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         }
         // this key's factor as the sum of two fp16: keys use both, so that a product has
         // its own rounding only (a score is 128 of them), values the first
-        float f = now * __uint_as_float((static_cast<uint32_t>(127 + 127 + 3 - kScalesBelow) << 23) - least[it & 1]);
+        float f = now * __uint_as_float((static_cast<uint32_t>(127 + 127 + 3 - kScalesBelow) << 23) - (it & 1 ? least[1] : least[0]));
         if (apart & (it & 1 ? 2u : 1u)) {
           int e;
           f = scale_parts(now, &e);
@@ -762,31 +762,41 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         fence_proxy_async_smem();
         return true;
       };
-      for (int j = 0; j < n_steps && begun; ++j) {
-        const float k_next = scale_of(a.k_scale, page), v_next = scale_of(a.v_scale, page);
-        page = page_of(j + 2);
-        if (!convert(2 * j, k_now)) break;
-        warp_arrive(sh.ready[(2 * j) % C::kStages]);
+      // Keys and values in turn, by the same instructions: twice the code costs its fetch.
+      float k_next = 0.f, v_next = 0.f;
+#pragma unroll 1
+      for (int it = 0; it < n_items && begun; ++it) {
+        const int j = it >> 1;
+        if (!(it & 1)) {
+          k_next = scale_of(a.k_scale, page);
+          v_next = scale_of(a.v_scale, page);
+          page = page_of(j + 2);
+        }
+        if (!convert(it, it & 1 ? v_now : k_now)) break;
         // Whether the next step's scales are in range, settled before this step's values are
         // ready: who has waited for those knows.
-        uint32_t far = (__any_sync(0xFFFFFFFFu, out_of_range(0, k_next)) ? 1u : 0u) |
-                       (__any_sync(0xFFFFFFFFu, out_of_range(1, v_next)) ? 2u : 0u);
-        if (lane == 0) sh.far[j & 1][w] = far;
-        warp_arrive(sh.scales_ready);
-        if (!convert(2 * j + 1, v_now) || !warp_wait(sh.scales_ready, j + 1)) break;
-        const uint32_t* fars = sh.far[j & 1];
-        far = fars[0] | fars[1] | fars[2] | fars[3];
-        if (far & ~apart) {
-          if (t == 0) {
-            if (far & ~apart & 1u) sh.k_from = j + 1;
-            if (far & ~apart & 2u) sh.v_from = j + 1;
-            if (apart == 0u) sh.apart_from = j + 1;
+        if (it & 1) {
+          if (!warp_wait(sh.scales_ready, j + 1)) break;
+          const uint32_t* fars = sh.far[j & 1];
+          const uint32_t far = fars[0] | fars[1] | fars[2] | fars[3];
+          if (far & ~apart) {
+            if (t == 0) {
+              if (far & ~apart & 1u) sh.k_from = j + 1;
+              if (far & ~apart & 2u) sh.v_from = j + 1;
+              if (apart == 0u) sh.apart_from = j + 1;
+            }
+            apart |= far;
           }
-          apart |= far;
+          k_now = k_next;
+          v_now = v_next;
         }
-        warp_arrive(sh.ready[(2 * j + 1) % C::kStages]);
-        k_now = k_next;
-        v_now = v_next;
+        warp_arrive(sh.ready[it % C::kStages]);
+        if (!(it & 1)) {
+          const uint32_t far = (__any_sync(0xFFFFFFFFu, out_of_range(0, k_next)) ? 1u : 0u) |
+                               (__any_sync(0xFFFFFFFFu, out_of_range(1, v_next)) ? 2u : 0u);
+          if (lane == 0) sh.far[j & 1][w] = far;
+          warp_arrive(sh.scales_ready);
+        }
       }
     }
     __syncwarp();
@@ -845,12 +855,11 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     const int vis = live ? paged_visible(seq, row_token(row0 + r, a.group)) : 0;
     // least visible count in the warp: steps below it need no mask
     const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
-    // P = exp2(x + ref), l its sum: ref is -m, and kPBits more where that is exact enough (P up
-    // to 2^(11 + kSlack) is a number of fp16, 2^(16 + kSlack) is not)
-    auto ref_of = [](float top) -> float {
-      return top == -INFINITY ? 0.f : kE4m3 && fabsf(top) < 0x1p22f ? kPBits - top : -top;
-    };
-    float m = -INFINITY, l = 0.f, ref = 0.f;
+    // P = exp2(x + ref), l its sum, 0 until the row has seen a key: ref is minus the row's maximum
+    // when it was last set, and kPBits more where that is exact enough (P up to 2^(11 + kSlack)
+    // is a number of fp16, 2^(16 + kSlack) is not)
+    auto ref_of = [](float top) -> float { return kE4m3 && fabsf(top) < 0x1p22f ? kPBits - top : -top; };
+    float l = 0.f, ref = 0.f;
     bool alive = true;
     // e4m3: the scores' factor, and the step from which keys or values are divided by their own
     // scales' powers of two.  From then on O is in units of 2^v_exp / kPScale, which may fall by
@@ -935,10 +944,10 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           // Each value's power of two goes into its weight.
           const bool v_apart = j >= *v_from;
           const float v_unit = sh.v_ref / kCodeScale;
-          const float m_new = fmaxf(m, most), ref_new = m_new == -INFINITY ? 0.f : -m_new;
-          float turn = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);  // of O
-          v_room = m == -INFINITY ? kAllRoom : v_room + (m_new - m);
-          m = m_new;
+          const float top_was = l == 0.f ? -INFINITY : -ref, top_now = fmaxf(top_was, most);
+          const float ref_new = top_now == -INFINITY ? 0.f : -top_now;
+          float turn = l == 0.f ? 0.f : fast_exp2(ref_new - ref);  // of O
+          v_room = l == 0.f ? kAllRoom : v_room + (top_now - top_was);
           ref = ref_new;
           l *= turn;
           float sum = 0.f, heaviest = 0.f;
@@ -995,7 +1004,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           warp_arrive(sh.p_ready[i]);
           continue;
         }
-        const bool move = most > m + kSlack || (m == -INFINITY && most > m);
+        const bool move = most + ref > (kE4m3 ? kPBits : 0.f) + kSlack || (l == 0.f && most > -INFINITY);
         const bool big = fabsf(most) >= 0x1p20f && fabsf(most) < INFINITY;
         if (__any_sync(0xFFFFFFFFu, move || big)) {
           // The product s factor is not rounded before ref is added to it below, most is: where
@@ -1007,9 +1016,8 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
               for (int k = 0; k < 32; ++k) s[c][k] = __float_as_uint(__uint_as_float(s[c][k]) * factor);
             factor = 1.f;
           }
-          const float m_new = fmaxf(m, most), ref_new = ref_of(m_new);
-          const float shrink = m == -INFINITY ? 0.f : fast_exp2(ref_new - ref);
-          m = m_new;
+          const float ref_new = move ? ref_of(most) : ref;
+          const float shrink = l == 0.f ? 0.f : fast_exp2(ref_new - ref);
           ref = ref_new;
           l *= shrink;
           if (j > 0) {
@@ -1057,7 +1065,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     if (rest) {
       if (j > 0) {
         v_exp = exponent_of(sh.v_ref / kCodeScale) + static_cast<int>(kPBits);
-        v_room = kPBits;  // which P and l lose
+        v_room = 0.f;
       }
       go(std::bool_constant<kE4m3>{});
     }
@@ -1140,7 +1148,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
                              o[k + 3] * v_back);
         }
       }
-      st_cluster_f32x2(there + C::kPartMl + 8 * slot, m == -INFINITY ? m : -ref, l);
+      st_cluster_f32x2(there + C::kPartMl + 8 * slot, l == 0.f ? -INFINITY : -ref, l);
       if (sh.any_bad) {
         for (int at = threadIdx.x; at < cluster * kBads; at += 256)
           min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kBads]), at / kBads), sh.first_bad[at % kBads]);

@@ -79,7 +79,8 @@ DWA_API dwa_status dwa_kv_read(const void* k_cache, const void* v_cache, const f
  * Rounding, beside f32 sums and the result's: up to 16 rows per key/value head
  * (max_q H / H_kv), bf16 caches none (p_j as the sum of two bf16), e4m3 caches p_j
  * times its value's scale to 11 bits; more rows, bf16 caches p_j to 8 bits, e4m3
- * caches p_j, k_j and v_j to 11 bits each.
+ * caches p_j, k_j and v_j to 11 bits each.  (What p_j times its value's scale is below
+ * 2^-20 of the row's largest has fewer bits, below 2^-31 none.)
  */
 DWA_API dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
                                        const void* k_cache, const void* v_cache,
