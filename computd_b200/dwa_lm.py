@@ -156,6 +156,7 @@ class ChunkPlan:
         self.retriever = retriever
         self.queries = torch.zeros((retriever.M, retriever.d_k), dtype=torch.bfloat16,
                                    device=retriever.device)
+        self._head = (0, None, None)  # a row count, its part of the queries and of the results
 
     @property
     def keys(self) -> torch.Tensor:
@@ -165,8 +166,15 @@ class ChunkPlan:
         T = queries.shape[0]
         if T == self.retriever.M:
             return self.retriever(queries, params=params)
-        self.queries[:T].copy_(queries)
-        return tuple(x if x is None else x[:T] for x in self.retriever(self.queries, params=params))
+        rows, head, results = self._head
+        if rows != T:  # the blocks of a forward ask for the same
+            head = self.queries[:T]
+        head.copy_(queries)
+        whole = self.retriever(self.queries, params=params)  # the plan's own buffers, always the same
+        if rows != T:
+            results = tuple(x if x is None else x[:T] for x in whole)
+            self._head = (T, head, results)
+        return results
 
 
 def _rope_theta(dh: int, device) -> torch.Tensor:
