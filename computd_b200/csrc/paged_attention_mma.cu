@@ -33,8 +33,8 @@
 // P goes to its product in 16 bits: over a bf16 cache, whose values are bf16 and want P to be
 // too, with 8 bits (2 x 2048 rows over 4096 to 8192 keys: relative error 0.0023 against 64 bits,
 // 0.0017 with f32 probabilities, which is the result's own rounding).  A second part of P would
-// have no place: TMEM and shared memory are full, and the tensor pipe would need 3072 cycles a
-// step for it.
+// have no place: TMEM and shared memory are full, and its product would take the
+// tensor pipe half as long again.
 //
 // A block costs 9 to 11 thousand cycles before its first scores (launch, the sequence's numbers,
 // Q's 64 KB from all SMs at once) and 4 after its last, a split one 8 to 12.
