@@ -154,8 +154,9 @@ class ChunkPlan:
 
     def __init__(self, retriever: Retriever):
         self.retriever = retriever
-        self.queries = torch.zeros((retriever.M, retriever.d_k), dtype=torch.bfloat16,
-                                   device=retriever.device)
+        with torch.inference_mode(False):  # written in and out of that mode
+            self.queries = torch.zeros((retriever.M, retriever.d_k), dtype=torch.bfloat16,
+                                       device=retriever.device)
         self._head = (0, None, None)  # a row count, its part of the queries and of the results
 
     @property
@@ -168,7 +169,8 @@ class ChunkPlan:
             return self.retriever(queries, params=params)
         rows, head, results = self._head
         if rows != T:  # the blocks of a forward ask for the same
-            head = self.queries[:T]
+            with torch.inference_mode(False):
+                head = self.queries[:T]
         head.copy_(queries)
         whole = self.retriever(self.queries, params=params)  # the plan's own buffers, always the same
         if rows != T:

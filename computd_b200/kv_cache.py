@@ -136,7 +136,8 @@ class PagedKVCache:
             self.k_scale, self.v_scale = (torch.empty(shape[:4], dtype=_F32, device=device)
                                           for _ in range(2))
         # DWA_ERR_DEVICE_CHECK once a call met a bad slot, page, length, row range or last token
-        self.status = torch.zeros((), dtype=_I32, device=device)
+        with torch.inference_mode(False):  # written in and out of that mode
+            self.status = torch.zeros((), dtype=_I32, device=device)
 
     def _layer(self, layer: int):
         if not 0 <= layer < self.n_layers:

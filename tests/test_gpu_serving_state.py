@@ -197,3 +197,22 @@ def test_an_output_that_does_not_fit_is_torchs_own_error():
         assert not bool(k.any()) and not bool(v.any())
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+@pytest.mark.parametrize("first,then", [(True, False), (False, True)])
+def test_steps_in_and_out_of_inference_mode(first, then):
+    """Plans, caches and their padded rows made in one mode serve in the other."""
+    from test_gpu_lm_extend import _model
+
+    cfg, model = _model(r=2, dh=16, layers=2)
+    out = []
+    with torch.inference_mode(first):
+        cache, table, ids, lengths = _prompt(cfg, model, 3, 20)
+    for mode in (first, then, first):
+        with torch.inference_mode(mode):
+            out.append(model.extend(ids, cache, table, lengths).clone())
+            drafts = torch.full((3, 2), 5, dtype=torch.int32, device="cuda")
+            u, r = torch.zeros((3, 2), device="cuda"), torch.zeros(3, device="cuda")
+            model.verify(_i32([1, 2, 3]), drafts, None, u, r, cache, table, lengths)
+            cache.check()
+    assert torch.equal(out[0], out[1]) and torch.equal(out[0], out[2])

@@ -138,3 +138,16 @@ def test_verify_reports_last_tokens_outside_the_vocabulary(monkeypatch):
             with pytest.raises(DWAError):
                 cache.check()
         cache.check()
+
+
+@pytest.mark.parametrize("made,used", [(True, False), (False, True), (True, True)])
+def test_a_cache_serves_in_and_out_of_inference_mode(made, used):
+    from computd_b200 import DWAError
+
+    with torch.inference_mode(made):
+        cache = _cache()
+    with torch.inference_mode(used):
+        cache.report(torch.tensor([False, True]))
+        with pytest.raises(DWAError):
+            cache.check()
+        cache.check()
