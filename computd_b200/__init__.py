@@ -10,8 +10,8 @@ provides device memory, streams and torch.distributed plumbing only.
 from ._lib import DWA_MAX_K, DWAArgumentError, DWAError, load as load_library
 from .assembler import WeightAssembler, assemble_finish, lowrank_delta, usage_ema_update
 from .assembly import normalise_alpha, weighted_gather_into, weighted_value_sum
-from .kv_cache import (PagedKVCache, kv_cache_read, kv_cache_write, paged_attention,
-                       verify_drafts)
+from .kv_cache import (PagedKVCache, kv_cache_append, kv_cache_keep, kv_cache_read, kv_cache_write,
+                       paged_attention, paged_tree_attention, tree_masks, verify_drafts, verify_tree)
 from .pool import ShardSpec, init_normal, new_normal
 from .retrieval import (HostPipeline, HybridParts, MultiAspectRetrieval, PeerExchange, Retriever,
                         chip_topk, exchange_candidates, project_keys, project_keys_packed,
@@ -24,6 +24,7 @@ __all__ = [
     "WeightAssembler", "assemble_finish", "lowrank_delta", "usage_ema_update",
     "normalise_alpha", "weighted_gather_into", "weighted_value_sum", "MultiAspectRetrieval",
     "PagedKVCache", "kv_cache_read", "kv_cache_write", "paged_attention", "verify_drafts",
+    "kv_cache_append", "kv_cache_keep", "paged_tree_attention", "tree_masks", "verify_tree",
     "ShardSpec", "init_normal", "new_normal",
     "HostPipeline", "HybridParts", "PeerExchange", "Retriever", "chip_topk", "project_keys",
     "project_keys_packed", "exchange_candidates", "reduce_partials",

@@ -108,7 +108,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dwa_lm_aspect_queries": (_i32, [_c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p,
                                      _f32, _f32, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
                                      _c_void_p]),
-    # include/dwa_decode.h: the paged cache, attention over it, drafted tokens
+    # include/dwa_decode.h: the paged cache, attention over it, drafted tokens, trees of them
     "dwa_kv_write": (_i32, [_c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64,
                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64,
                             _i64, _c_void_p, _c_void_p]),
@@ -121,6 +121,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                    _i64, _c_void_p, _c_void_p]),
     "dwa_verify_drafts": (_i32, [_c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p,
                                  _c_void_p, _i64, _i32, _i32, _c_void_p, _c_void_p, _c_void_p]),
+    "dwa_kv_append": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i32, _i32, _i32, _i64, _i64,
+                             _i64, _i64, _i64, _i64, _c_void_p, _c_void_p, _i32, _i64, _i64, _c_void_p,
+                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i64,
+                             _i64, _c_void_p, _c_void_p, _c_void_p]),
+    "dwa_tree_masks": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p, _i32, _c_void_p,
+                              _c_void_p, _c_void_p]),
+    "dwa_paged_tree_attention": (_i32, [_c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p,
+                                        _c_void_p, _c_void_p, _i32, _i64, _i32, _i64, _i64, _c_void_p,
+                                        _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32,
+                                        _f32, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    "dwa_verify_tree": (_i32, [_c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
+                               _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "dwa_kv_keep": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,
+                           _i64, _i32, _i64, _i64, _c_void_p, _i64, _i32, _c_void_p, _c_void_p,
+                           _c_void_p, _i32, _i32, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -887,7 +887,7 @@ dwa_status dwa_lm_aspect_queries(const void* q, int64_t M, int32_t S, int32_t d_
 }  // extern "C"
 
 namespace {
-// The paged cache's part of the checks of dwa_kv_write, dwa_kv_read and dwa_paged_attention.
+// The paged cache's part of the checks of the calls that take one.
 dwa_status kv_cache_view(const char* fn, const void* k_cache, const void* v_cache,
                          const float* k_scale, const float* v_scale, int32_t H, int32_t d,
                          int64_t n_pages, int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
@@ -917,6 +917,71 @@ dwa_status kv_cache_view(const char* fn, const void* k_cache, const void* v_cach
   *out = dwa::KvCacheView{k_cache, v_cache, k_scale, v_scale, H, d, n_pages, page_size, ld_page,
                           k_scale ? ld_scale_page : 0};
   return DWA_OK;
+}
+
+// dwa_paged_attention, and with `words` words of a mask to a row dwa_paged_tree_attention.
+dwa_status paged_attention_call(const char* fn, const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
+                                const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, int32_t H_kv, int64_t n_pages,
+                                int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                                const int32_t* block_table, int64_t ld_table, int32_t max_pages,
+                                const int32_t* lengths, const int32_t* q_start, int32_t B,
+                                int32_t max_q, const int64_t* tree_mask, int32_t words, float scale,
+                                void* out, int64_t out_ld, int32_t* status, dwa_stream_t stream) {
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H_kv, d, n_pages,
+                                    page_size, ld_page, ld_scale_page, &c))
+    return st;
+  if (T < 0 || B < 0 || max_q < 0 || max_pages < 0 || H < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, B=%d, max_q=%d, max_pages=%d, H=%d)", fn,
+                (long long)T, B, max_q, max_pages, H);
+  if (words > 0 && max_q > 64ll * words)
+    return fail(DWA_ERR_INVALID_ARG, "%s: max_q=%d nodes need more than %d words of a mask", fn, max_q, words);
+  if (H % H_kv != 0)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: H=%d must be a multiple of H_kv=%d", fn, H, H_kv);
+  if (T > INT32_MAX || static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX ||
+      static_cast<int64_t>(max_pages) * page_size > (1 << 30))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, or over 2^30 tokens per sequence", fn);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale >= 0.f) || std::isinf(scale_log2))
+    return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite (log2(e) times it too) and not negative", fn);
+  if (T > 0 && !q_start && (B == 0 || T % B != 0 || T / B > max_q))
+    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal chunks of at most "
+                "max_q=%d", fn, (long long)T, B, max_q);
+  if (T == 0 || B == 0) return ok();
+  if (!q || !out || !lengths || (max_pages > 0 && !block_table))
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (words > 0 && (!tree_mask || !aligned(tree_mask, 8)))
+    return fail(DWA_ERR_INVALID_ARG, "%s: tree_mask must be an 8-byte aligned array", fn);
+  if (max_q == 0) return fail(DWA_ERR_INVALID_ARG, "%s: max_q = 0 with rows to compute", fn);
+  const int64_t width = static_cast<int64_t>(H) * d;
+  if (q_ld < width || out_ld < width || (max_pages > 0 && ld_table < max_pages))
+    return fail(DWA_ERR_INVALID_ARG, "%s: a row stride is below its row length", fn);
+  if (q_ld % 8 != 0 || out_ld % 8 != 0 || !aligned(q, 16) || !aligned(out, 16))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: q and out rows must be 16-byte aligned", fn);
+  if (!aligned(block_table, 4) || !aligned(lengths, 4) || !aligned(q_start, 4) || !aligned(status, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: int32 arrays must be 4-byte aligned", fn);
+  dwa::PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.q_ld = q_ld; a.out_ld = out_ld;
+  a.k = k_cache; a.v = v_cache; a.k_scale = k_scale; a.v_scale = v_scale;
+  a.ld_page = ld_page; a.ld_scale_page = c.ld_scale_page; a.n_pages = n_pages;
+  a.table = block_table; a.ld_table = ld_table; a.max_pages = max_pages;
+  a.page_log2 = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  a.lengths = lengths; a.q_start = q_start; a.T = T;
+  a.even = q_start ? 0 : static_cast<int>(T / B);
+  a.max_q = max_q; a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d;
+  // not 0: minus infinity times it marks what a row may not see
+  a.scale_log2 = std::max(scale_log2, 1.1754944e-38f);
+  a.status = status;
+  if (words > 0) {
+    a.tree = reinterpret_cast<const uint32_t*>(tree_mask);
+    a.tree_words = 2 * words;
+  }
+  cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  return ok();
 }
 }  // namespace
 
@@ -978,53 +1043,26 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
                                const int32_t* lengths, const int32_t* q_start, int32_t B,
                                int32_t max_q, float scale, void* out, int64_t out_ld,
                                int32_t* status, dwa_stream_t stream) {
-  const char* fn = "dwa_paged_attention";
-  dwa::KvCacheView c{};
-  if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H_kv, d, n_pages,
-                                    page_size, ld_page, ld_scale_page, &c))
-    return st;
-  if (T < 0 || B < 0 || max_q < 0 || max_pages < 0 || H < 1)
-    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, B=%d, max_q=%d, max_pages=%d, H=%d)", fn,
-                (long long)T, B, max_q, max_pages, H);
-  if (H % H_kv != 0)
-    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: H=%d must be a multiple of H_kv=%d", fn, H, H_kv);
-  if (T > INT32_MAX || static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX ||
-      static_cast<int64_t>(max_pages) * page_size > (1 << 30))
-    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, or over 2^30 tokens per sequence", fn);
-  const float scale_log2 = scale * 1.4426950408889634f;
-  if (!(scale >= 0.f) || std::isinf(scale_log2))
-    return fail(DWA_ERR_INVALID_ARG, "%s: scale must be finite (log2(e) times it too) and not negative", fn);
-  if (T > 0 && !q_start && (B == 0 || T % B != 0 || T / B > max_q))
-    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal chunks of at most "
-                "max_q=%d", fn, (long long)T, B, max_q);
-  if (T == 0 || B == 0) return ok();
-  if (!q || !out || !lengths || (max_pages > 0 && !block_table))
-    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
-  if (max_q == 0) return fail(DWA_ERR_INVALID_ARG, "%s: max_q = 0 with rows to compute", fn);
-  const int64_t width = static_cast<int64_t>(H) * d;
-  if (q_ld < width || out_ld < width || (max_pages > 0 && ld_table < max_pages))
-    return fail(DWA_ERR_INVALID_ARG, "%s: a row stride is below its row length", fn);
-  if (q_ld % 8 != 0 || out_ld % 8 != 0 || !aligned(q, 16) || !aligned(out, 16))
-    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: q and out rows must be 16-byte aligned", fn);
-  if (!aligned(block_table, 4) || !aligned(lengths, 4) || !aligned(q_start, 4) || !aligned(status, 4))
-    return fail(DWA_ERR_INVALID_ARG, "%s: int32 arrays must be 4-byte aligned", fn);
-  dwa::PagedArgs a{};
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = static_cast<uint16_t*>(out);
-  a.q_ld = q_ld; a.out_ld = out_ld;
-  a.k = k_cache; a.v = v_cache; a.k_scale = k_scale; a.v_scale = v_scale;
-  a.ld_page = ld_page; a.ld_scale_page = c.ld_scale_page; a.n_pages = n_pages;
-  a.table = block_table; a.ld_table = ld_table; a.max_pages = max_pages;
-  a.page_log2 = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
-  a.lengths = lengths; a.q_start = q_start; a.T = T;
-  a.even = q_start ? 0 : static_cast<int>(T / B);
-  a.max_q = max_q; a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d;
-  // not 0: minus infinity times it marks what a row may not see
-  a.scale_log2 = std::max(scale_log2, 1.1754944e-38f);
-  a.status = status;
-  cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(e, "dwa_paged_attention launch");
-  return ok();
+  return paged_attention_call("dwa_paged_attention", q, T, H, d, q_ld, k_cache, v_cache, k_scale, v_scale, H_kv,
+                              n_pages, page_size, ld_page, ld_scale_page, block_table, ld_table, max_pages,
+                              lengths, q_start, B, max_q, nullptr, 0, scale, out, out_ld, status, stream);
+}
+
+dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
+                                    const void* k_cache, const void* v_cache, const float* k_scale,
+                                    const float* v_scale, int32_t H_kv, int64_t n_pages,
+                                    int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                                    const int32_t* block_table, int64_t ld_table, int32_t max_pages,
+                                    const int32_t* lengths, const int32_t* q_start, int32_t B,
+                                    int32_t max_q, const int64_t* tree_mask, int32_t mask_words,
+                                    float scale, void* out, int64_t out_ld, int32_t* status,
+                                    dwa_stream_t stream) {
+  const char* fn = "dwa_paged_tree_attention";
+  if (mask_words < 1 || mask_words > (1 << 20))
+    return fail(DWA_ERR_INVALID_ARG, "%s: mask_words=%d must be positive (and 2^20 at most)", fn, mask_words);
+  return paged_attention_call(fn, q, T, H, d, q_ld, k_cache, v_cache, k_scale, v_scale, H_kv, n_pages, page_size,
+                              ld_page, ld_scale_page, block_table, ld_table, max_pages, lengths, q_start, B,
+                              max_q, tree_mask, mask_words, scale, out, out_ld, status, stream);
 }
 
 dwa_status dwa_verify_drafts(const void* target, const void* draft, int32_t probs_bf16,
@@ -1048,6 +1086,132 @@ dwa_status dwa_verify_drafts(const void* target, const void* draft, int32_t prob
                                             sample_u, draft_lengths, B, K, V, n_accepted, out_tokens,
                                             static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "dwa_verify_drafts launch");
+  return ok();
+}
+
+dwa_status dwa_kv_append(const void* q, const void* k, const void* v, int32_t src_bf16, int64_t T,
+                         int32_t H, int32_t H_kv, int32_t d, int64_t q_ld_tok, int64_t q_ld_head,
+                         int64_t k_ld_tok, int64_t k_ld_head, int64_t v_ld_tok, int64_t v_ld_head,
+                         const void* cos_t, const void* sin_t, int32_t tables_bf16, int64_t ld_table,
+                         int64_t n_positions, const int64_t* positions, const int64_t* slots,
+                         void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                         int64_t n_pages, int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                         void* q_out, int32_t* status, dwa_stream_t stream) {
+  const char* fn = "dwa_kv_append";
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H_kv, d, n_pages, page_size,
+                                    ld_page, ld_scale_page, &c))
+    return st;
+  if (T < 0 || T > INT32_MAX || n_positions < 0 || (q && H < 1))
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, n_positions=%lld, H=%d)", fn, (long long)T,
+                (long long)n_positions, H);
+  if (q && H > 65535) return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many heads", fn);
+  if (T == 0) return ok();
+  if (!k || !v || !slots || (q && !q_out) || (n_positions > 0 && (!cos_t || !sin_t)))
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  const int per16 = src_bf16 ? 8 : 4, table16 = tables_bf16 ? 8 : 4;
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || (q && (q_ld_tok % per16 || q_ld_head % per16)) ||
+      k_ld_tok % per16 || k_ld_head % per16 || v_ld_tok % per16 || v_ld_head % per16)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: q, k and v rows must be 16-byte aligned", fn);
+  if (!aligned(cos_t, 16) || !aligned(sin_t, 16) || ld_table % table16)
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: the tables' rows must be 16-byte aligned", fn);
+  if (!aligned(slots, 8) || !aligned(positions, 8) || (q && !aligned(q_out, 16)) || !aligned(status, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: misaligned array", fn);
+  if ((q && (q_ld_tok < 0 || q_ld_head < 0)) || k_ld_tok < 0 || k_ld_head < 0 || v_ld_tok < 0 || v_ld_head < 0 ||
+      ld_table < d / 2)
+    return fail(DWA_ERR_INVALID_ARG, "%s: a stride is negative, or below its row", fn);
+  dwa::KvAppendView x{};
+  x.q = q; x.k = k; x.v = v;
+  x.src_bf16 = src_bf16 != 0; x.tables_bf16 = tables_bf16 != 0;
+  x.H = q ? H : 0;
+  x.q_tok = q_ld_tok; x.q_head = q_ld_head; x.k_tok = k_ld_tok; x.k_head = k_ld_head;
+  x.v_tok = v_ld_tok; x.v_head = v_ld_head;
+  x.cos = cos_t; x.sin = sin_t; x.ld_table = ld_table; x.n_positions = n_positions;
+  x.positions = positions; x.q_out = q ? q_out : nullptr;
+  cudaError_t e = dwa::launch_kv_append(c, x, T, slots, status, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_kv_append launch");
+  return ok();
+}
+
+dwa_status dwa_tree_masks(const int32_t* parents, const int32_t* q_start, int64_t T, int32_t B, int32_t max_q,
+                          int64_t* mask, int32_t mask_words, int32_t* depth, int32_t* status,
+                          dwa_stream_t stream) {
+  const char* fn = "dwa_tree_masks";
+  if (T < 0 || B < 0 || max_q < 0 || mask_words < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, B=%d, max_q=%d, mask_words=%d)", fn, (long long)T, B,
+                max_q, mask_words);
+  if (T > INT32_MAX || max_q > dwa::tree_most_nodes() || mask_words > (1 << 20))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, or trees of more than %d nodes", fn,
+                dwa::tree_most_nodes());
+  if (max_q > 64ll * mask_words)
+    return fail(DWA_ERR_INVALID_ARG, "%s: max_q=%d nodes need more than %d words of a mask", fn, max_q, mask_words);
+  if (T > 0 && !q_start && (B == 0 || T % B != 0 || T / B > max_q))
+    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal trees of at most max_q=%d", fn,
+                (long long)T, B, max_q);
+  if (T == 0) return ok();
+  if (!parents || !mask || !depth) return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!aligned(parents, 4) || !aligned(q_start, 4) || !aligned(mask, 8) || !aligned(depth, 4) || !aligned(status, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: misaligned array", fn);
+  cudaError_t e = dwa::launch_tree_masks(parents, q_start, T, B, max_q, mask_words, mask, depth, status,
+                                         static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_tree_masks launch");
+  return ok();
+}
+
+dwa_status dwa_verify_tree(const void* target, int32_t probs_bf16, const int32_t* tokens, const int32_t* parents,
+                           const int32_t* q_start, const float* sample_u, int64_t T, int32_t B, int32_t steps,
+                           int32_t V, int32_t* n_accepted, int32_t* out_tokens, int32_t* path,
+                           dwa_stream_t stream) {
+  const char* fn = "dwa_verify_tree";
+  if (T < 0 || B < 0 || steps < 1 || V < 1)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (T=%lld, B=%d, steps=%d, V=%d)", fn, (long long)T, B, steps, V);
+  if (T > INT32_MAX || B > INT32_MAX / 8 || V > (1 << 30) || steps > (1 << 20))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many nodes, sequences, steps or tokens", fn);
+  if (T > 0 && !q_start && (B == 0 || T % B != 0))
+    return fail(DWA_ERR_INVALID_ARG, "%s: without q_start T=%lld must be B=%d equal trees", fn, (long long)T, B);
+  if (B == 0) return ok();
+  if ((T > 0 && (!target || !tokens || !parents)) || !sample_u || !n_accepted || !out_tokens || !path)
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (!aligned(target, probs_bf16 ? 2 : 4) || !aligned(tokens, 4) || !aligned(parents, 4) || !aligned(q_start, 4) ||
+      !aligned(sample_u, 4) || !aligned(n_accepted, 4) || !aligned(out_tokens, 4) || !aligned(path, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: misaligned array", fn);
+  cudaError_t e = dwa::launch_verify_tree(target, probs_bf16 ? 1 : 0, tokens, parents, q_start, sample_u, T, B, steps,
+                                          V, n_accepted, out_tokens, path, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_verify_tree launch");
+  return ok();
+}
+
+dwa_status dwa_kv_keep(void* k_cache, void* v_cache, float* k_scale, float* v_scale, int32_t layers,
+                       int64_t ld_layer, int64_t ld_scale_layer, int32_t H, int32_t d, int64_t n_pages,
+                       int32_t page_size, int64_t ld_page, int64_t ld_scale_page, const int32_t* block_table,
+                       int64_t ld_table, int32_t max_pages, const int32_t* start, const int32_t* path,
+                       const int32_t* n_accepted, int32_t B, int32_t steps, int32_t* status,
+                       dwa_stream_t stream) {
+  const char* fn = "dwa_kv_keep";
+  dwa::KvCacheView c{};
+  if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H, d, n_pages, page_size, ld_page,
+                                    ld_scale_page, &c))
+    return st;
+  if (layers < 1 || B < 0 || steps < 1 || max_pages < 0)
+    return fail(DWA_ERR_INVALID_ARG, "%s: bad sizes (layers=%d, B=%d, steps=%d, max_pages=%d)", fn, layers, B, steps,
+                max_pages);
+  if (layers > 65535 || steps > (1 << 20) || B > (1 << 20) ||
+      static_cast<int64_t>(max_pages) * page_size > (1 << 30))
+    return fail(DWA_ERR_UNSUPPORTED_SHAPE, "%s: too many layers, steps or sequences, or over 2^30 tokens each", fn);
+  if (layers > 1 && (ld_layer < 0 || ld_layer % (k_scale ? 16 : 8) || (k_scale && ld_scale_layer < 0)))
+    return fail(DWA_ERR_INVALID_ARG, "%s: layers must be 16-byte aligned, and their strides not negative", fn);
+  if (B == 0) return ok();
+  if (!start || !path || !n_accepted || (max_pages > 0 && !block_table))
+    return fail(DWA_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (max_pages > 0 && ld_table < max_pages)
+    return fail(DWA_ERR_INVALID_ARG, "%s: a row stride is below its row length", fn);
+  if (!aligned(block_table, 4) || !aligned(start, 4) || !aligned(path, 4) || !aligned(n_accepted, 4) ||
+      !aligned(status, 4))
+    return fail(DWA_ERR_INVALID_ARG, "%s: int32 arrays must be 4-byte aligned", fn);
+  cudaError_t e = dwa::launch_kv_keep(c, layers, layers > 1 ? ld_layer : 0, layers > 1 ? ld_scale_layer : 0,
+                                      block_table, ld_table, max_pages, start, path, n_accepted, B, steps, status,
+                                      static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "dwa_kv_keep launch");
   return ok();
 }
 

@@ -222,5 +222,28 @@ cudaError_t launch_verify_drafts(const void* target, const void* draft, int prob
                                  const int32_t* tokens, const float* accept_u, const float* sample_u,
                                  const int32_t* draft_lengths, int64_t B, int K, int V,
                                  int32_t* n_accepted, int32_t* out_tokens, cudaStream_t stream);
+// What dwa_kv_append puts into the cache, and its tables.
+struct KvAppendView {
+  const void *q, *k, *v;  // q null: keys and values only
+  bool src_bf16, tables_bf16;
+  int H;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  const void *cos, *sin;
+  int64_t ld_table, n_positions;
+  const int64_t* positions;
+  void* q_out;
+};
+cudaError_t launch_kv_append(const KvCacheView& c, const KvAppendView& x, int64_t T, const int64_t* slots,
+                             int32_t* status, cudaStream_t stream);
+cudaError_t launch_kv_keep(const KvCacheView& c, int layers, int64_t ld_layer, int64_t ld_scale_layer,
+                           const int32_t* table, int64_t ld_table, int max_pages, const int32_t* start,
+                           const int32_t* path, const int32_t* n_accepted, int64_t B, int steps,
+                           int32_t* status, cudaStream_t stream);
+int tree_most_nodes();
+cudaError_t launch_tree_masks(const int32_t* parents, const int32_t* q_start, int64_t T, int B, int max_q,
+                              int words, int64_t* mask, int32_t* depth, int32_t* status, cudaStream_t stream);
+cudaError_t launch_verify_tree(const void* target, int probs_bf16, const int32_t* tokens, const int32_t* parents,
+                               const int32_t* q_start, const float* u, int64_t T, int B, int steps, int V,
+                               int32_t* n_accepted, int32_t* out_tokens, int32_t* path, cudaStream_t stream);
 
 }  // namespace dwa

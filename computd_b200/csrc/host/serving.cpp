@@ -31,6 +31,11 @@ decltype(&dwa_kv_write) g_write = nullptr;
 decltype(&dwa_kv_read) g_read = nullptr;
 decltype(&dwa_paged_attention) g_attend = nullptr;
 decltype(&dwa_verify_drafts) g_verify = nullptr;
+decltype(&dwa_kv_append) g_append = nullptr;
+decltype(&dwa_kv_keep) g_keep = nullptr;
+decltype(&dwa_paged_tree_attention) g_attend_tree = nullptr;
+decltype(&dwa_tree_masks) g_masks = nullptr;
+decltype(&dwa_verify_tree) g_verify_tree = nullptr;
 PyObject* g_raise = nullptr;  // raises the package's error for a status and a function's name
 
 struct Refusal {
@@ -197,15 +202,22 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F&& body) {
   return nullptr;
 }
 
-// bind(write, read, attend, verify, raise): the entry points' addresses.
+// bind(write, read, attend, verify, append, keep, attend_tree, masks, verify_tree, raise): the entry
+// points' addresses.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[4];
+  unsigned long long a[9];
   PyObject* raise;
-  if (!PyArg_ParseTuple(args, "KKKKO", &a[0], &a[1], &a[2], &a[3], &raise)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &raise))
+    return nullptr;
   g_write = reinterpret_cast<decltype(g_write)>(a[0]);
   g_read = reinterpret_cast<decltype(g_read)>(a[1]);
   g_attend = reinterpret_cast<decltype(g_attend)>(a[2]);
   g_verify = reinterpret_cast<decltype(g_verify)>(a[3]);
+  g_append = reinterpret_cast<decltype(g_append)>(a[4]);
+  g_keep = reinterpret_cast<decltype(g_keep)>(a[5]);
+  g_attend_tree = reinterpret_cast<decltype(g_attend_tree)>(a[6]);
+  g_masks = reinterpret_cast<decltype(g_masks)>(a[7]);
+  g_verify_tree = reinterpret_cast<decltype(g_verify_tree)>(a[8]);
   Py_INCREF(raise);
   Py_XDECREF(g_raise);
   g_raise = raise;
@@ -276,10 +288,20 @@ PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+const at::Tensor& block_table_of(PyObject* o, int dev) {
+  const at::Tensor& table = tensor(o, "block_table");
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || !on(table, dev) ||
+      (table.size(1) > 1 && table.stride(1) != 1))
+    refuse("block_table must be int32 [B, max_pages], contiguous along its rows, on the cache's device "
+           "(got " + describe(table) + ")");
+  return table;
+}
+
 // (q, k_cache, v_cache, block_table, lengths, q_start, max_q, k_scale, v_scale, scale, out,
-// status) -> out
+// status), and with a tree also (..., tree_mask) -> out
+template <bool kTree>
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 12, [&]() -> PyObject* {
+  return guarded(n, kTree ? 13 : 12, [&]() -> PyObject* {
     const Cache c = cache_of(a[1], a[2], a[7], a[8]);
     const at::Tensor& q = tensor(a[0], "q");
     int64_t q_ld, q_head;
@@ -287,11 +309,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (q.scalar_type() != at::kBFloat16) refuse("q must be bfloat16 (got " + describe(q) + ")");
     if (q_head != c.d) refuse("q must be contiguous over heads and d");
     const int64_t T = q.size(0), heads = q.size(1), width = heads * c.d;
-    const at::Tensor& table = tensor(a[3], "block_table");
-    if (table.scalar_type() != at::kInt || table.dim() != 2 || !on(table, c.dev) ||
-        (table.size(1) > 1 && table.stride(1) != 1))
-      refuse("block_table must be int32 [B, max_pages], contiguous along its rows, on the cache's device "
-             "(got " + describe(table) + ")");
+    const at::Tensor& table = block_table_of(a[3], c.dev);
     const int64_t B = table.size(0), max_pages = table.size(1);
     const int32_t* lengths = array<int32_t>(a[4], at::kInt, {B}, c.dev, "lengths");
     const int32_t* q_start = nullptr;
@@ -312,6 +330,15 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (heads > INT32_MAX || B > INT32_MAX || max_pages > INT32_MAX || max_q > INT32_MAX || max_q < INT32_MIN)
       refuse("paged_attention: too many heads, sequences, pages or rows");
     int32_t* status = status_of(a[11], c.dev);
+    const int64_t* mask = nullptr;
+    int64_t words = 0;
+    if constexpr (kTree) {
+      const at::Tensor& m = tensor(a[12], "tree_mask");
+      words = m.dim() == 2 ? m.size(1) : 0;
+      mask = array<int64_t>(a[12], at::kLong, {T, words}, c.dev, "tree_mask");
+      if (words < 1 || words > INT32_MAX) refuse("tree_mask must have a word at least for every row");
+      if (a[6] == Py_None && max_q > 64 * words) max_q = 64 * words;  // T bounds a tree, and so do the words
+    }
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(c.dev));
     at::Tensor made;
     int64_t out_ld = width;
@@ -328,14 +355,20 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = o.data_ptr();
       if (T <= 1) out_ld = width;
     }
-    PyObject* ok = finish(
-        g_attend(q.data_ptr(), T, static_cast<int32_t>(heads), static_cast<int32_t>(c.d), T > 1 ? q_ld : width,
-                 c.k, c.v, c.k_scale, c.v_scale, static_cast<int32_t>(c.heads), c.n_pages,
-                 static_cast<int32_t>(c.page), c.ld_page, c.ld_scale, static_cast<int32_t*>(table.data_ptr()),
-                 B > 1 ? table.stride(0) : max_pages, static_cast<int32_t>(max_pages), lengths, q_start,
-                 static_cast<int32_t>(B), static_cast<int32_t>(max_q), static_cast<float>(scale), out, out_ld,
-                 status, c10::cuda::getCurrentCUDAStream(c.dev).stream()),
-        "dwa_paged_attention");
+    auto call = [&](auto entry, auto... more) {
+      return entry(q.data_ptr(), T, static_cast<int32_t>(heads), static_cast<int32_t>(c.d), T > 1 ? q_ld : width,
+                   c.k, c.v, c.k_scale, c.v_scale, static_cast<int32_t>(c.heads), c.n_pages,
+                   static_cast<int32_t>(c.page), c.ld_page, c.ld_scale,
+                   static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : max_pages,
+                   static_cast<int32_t>(max_pages), lengths, q_start, static_cast<int32_t>(B),
+                   static_cast<int32_t>(max_q), more..., static_cast<float>(scale), out, out_ld, status,
+                   c10::cuda::getCurrentCUDAStream(c.dev).stream());
+    };
+    PyObject* ok;
+    if constexpr (kTree)
+      ok = finish(call(g_attend_tree, mask, static_cast<int32_t>(words)), "dwa_paged_tree_attention");
+    else
+      ok = finish(call(g_attend), "dwa_paged_attention");
     if (ok == nullptr) return nullptr;
     Py_DECREF(ok);
     if (a[10] == Py_None) return wrap(made);
@@ -376,12 +409,224 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// (q or None, k, v, cos, sin, k_cache, v_cache, slots, positions or None, k_scale, v_scale,
+// q_out or None, status) -> the rotated q, or None
+PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 13, [&]() -> PyObject* {
+    const Cache c = cache_of(a[5], a[6], a[9], a[10]);
+    const at::Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+    const at::ScalarType type = k.scalar_type();
+    if ((type != at::kBFloat16 && type != at::kFloat) || v.scalar_type() != type)
+      refuse("q, k and v must all be bfloat16 or float32");
+    int64_t qt = 0, qh = 0, kt, kh, vt, vh;
+    rows_of(k, c.heads, c.d, c.dev, "k", &kt, &kh);
+    rows_of(v, c.heads, c.d, c.dev, "v", &vt, &vh);
+    const int64_t T = k.size(0);
+    if (v.size(0) != T) refuse("k and v must have the same number of tokens");
+    const at::Tensor &cos = tensor(a[3], "cos"), &sin = tensor(a[4], "sin");
+    const at::ScalarType table = cos.scalar_type();
+    if ((table != at::kBFloat16 && table != at::kFloat) || sin.scalar_type() != table || cos.dim() != 2 ||
+        cos.size(1) != c.d / 2 || sin.sizes() != cos.sizes() || !on(cos, c.dev) || !on(sin, c.dev) ||
+        (c.d > 2 && (cos.stride(1) != 1 || sin.stride(1) != 1)) ||
+        (cos.size(0) > 1 && cos.stride(0) != sin.stride(0)))
+      refuse("cos and sin must both be bfloat16 or float32 [n_positions, d / 2] with the same row stride, on the "
+             "cache's device (got " + describe(cos) + " and " + describe(sin) + ")");
+    const int64_t n_positions = cos.size(0), ld_table = n_positions > 1 ? cos.stride(0) : c.d / 2;
+    const int64_t* slots = array<int64_t>(a[7], at::kLong, {T}, c.dev, "slots");
+    const int64_t* positions = a[8] == Py_None ? nullptr : array<int64_t>(a[8], at::kLong, {T}, c.dev, "positions");
+    if (positions == nullptr && T > n_positions)
+      refuse("without positions cos and sin need a row for every token");
+    int32_t* status = status_of(a[12], c.dev);
+    const void* q_ptr = nullptr;
+    void* q_out = nullptr;
+    int64_t heads = 0;
+    at::Tensor made;
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(c.dev));
+    if (a[0] != Py_None) {
+      const at::Tensor& q = tensor(a[0], "q");
+      rows_of(q, -1, c.d, c.dev, "q", &qt, &qh);
+      heads = q.size(1);
+      if (q.scalar_type() != type || q.size(0) != T || heads < 1 || heads > INT32_MAX)
+        refuse("q must have k's type and number of tokens, and a head at least (got " + describe(q) + ")");
+      q_ptr = q.data_ptr();
+      if (a[11] == Py_None) {
+        made = fresh({T, heads, c.d}, at::kBFloat16, c.dev);
+        q_out = made.data_ptr();
+      } else {
+        q_out = array<void>(a[11], at::kBFloat16, {T, heads, c.d}, c.dev, "q_out");
+      }
+    } else if (a[11] != Py_None) {
+      refuse("q_out goes with q");
+    }
+    PyObject* ok = finish(
+        g_append(q_ptr, k.data_ptr(), v.data_ptr(), type == at::kBFloat16, T, static_cast<int32_t>(heads),
+                 static_cast<int32_t>(c.heads), static_cast<int32_t>(c.d), qt, qh, kt, kh, vt, vh, cos.data_ptr(),
+                 sin.data_ptr(), table == at::kBFloat16, ld_table, n_positions, positions, slots, c.k, c.v,
+                 c.k_scale, c.v_scale, c.n_pages, static_cast<int32_t>(c.page), c.ld_page, c.ld_scale, q_out,
+                 status, c10::cuda::getCurrentCUDAStream(c.dev).stream()),
+        "dwa_kv_append");
+    if (ok == nullptr || a[0] == Py_None) return ok;
+    Py_DECREF(ok);
+    if (a[11] == Py_None) return wrap(made);
+    Py_INCREF(a[11]);
+    return a[11];
+  });
+}
+
+// (parents, q_start or None, B or None, max_q or None, status) -> (mask, depth)
+PyObject* masks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    const at::Tensor& parents_t = tensor(a[0], "parents");
+    const int dev = device_of(parents_t, "parents");
+    if (parents_t.dim() != 1) refuse("parents must be int32 [T] (got " + describe(parents_t) + ")");
+    const int64_t T = parents_t.size(0);
+    const int32_t* parents = array<int32_t>(a[0], at::kInt, {T}, dev, "parents");
+    const int32_t* q_start = nullptr;
+    int64_t B = 1, max_q = T;
+    if (a[1] != Py_None) {
+      const at::Tensor& s = tensor(a[1], "q_start");
+      B = s.dim() == 1 ? s.size(0) - 1 : -1;
+      if (B < 0) refuse("q_start must be int32 [B + 1]");
+      q_start = array<int32_t>(a[1], at::kInt, {B + 1}, dev, "q_start");
+      if (a[2] != Py_None) refuse("n_trees goes without q_start");
+    } else if (a[2] != Py_None) {
+      B = PyLong_AsLongLong(a[2]);
+      if (PyErr_Occurred()) return nullptr;
+      if (B < 1 || T % B) refuse("n_trees must be positive and divide the number of nodes");
+      max_q = T / B;
+    }
+    if (a[3] != Py_None) {
+      max_q = PyLong_AsLongLong(a[3]);
+      if (PyErr_Occurred()) return nullptr;
+    }
+    if (B > INT32_MAX || max_q < 0 || max_q > INT32_MAX) refuse("tree_masks: too many trees, or a bad max_q");
+    int32_t* status = status_of(a[4], dev);
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const int64_t words = max_q > 64 ? (max_q + 63) / 64 : 1;
+    const at::Tensor mask = fresh({T, words}, at::kLong, dev), depth = fresh({T}, at::kInt, dev);
+    PyObject* ok = finish(g_masks(parents, q_start, T, static_cast<int32_t>(B), static_cast<int32_t>(max_q),
+                                  static_cast<int64_t*>(mask.data_ptr()), static_cast<int32_t>(words),
+                                  static_cast<int32_t*>(depth.data_ptr()), status,
+                                  c10::cuda::getCurrentCUDAStream(dev).stream()),
+                          "dwa_tree_masks");
+    if (ok == nullptr) return nullptr;
+    Py_DECREF(ok);
+    return Py_BuildValue("(NN)", wrap(mask), wrap(depth));
+  });
+}
+
+// (target_probs, tree_tokens, parents, sample_u, q_start or None) -> (accepted, tokens, path)
+PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 5, [&]() -> PyObject* {
+    const at::Tensor& target = tensor(a[0], "target_probs");
+    const int dev = device_of(target, "target_probs");
+    const at::ScalarType type = target.scalar_type();
+    if ((type != at::kFloat && type != at::kBFloat16) || target.dim() != 2 || !target.is_contiguous())
+      refuse("target_probs must be a contiguous float32 or bfloat16 [T, V] (got " + describe(target) + ")");
+    const int64_t T = target.size(0), V = target.size(1);
+    const int32_t* tokens = array<int32_t>(a[1], at::kInt, {T}, dev, "tree_tokens");
+    const int32_t* parents = array<int32_t>(a[2], at::kInt, {T}, dev, "parents");
+    const at::Tensor& u = tensor(a[3], "sample_u");
+    if (u.dim() != 2) refuse("sample_u must be float32 [B, steps] (got " + describe(u) + ")");
+    const int64_t B = u.size(0), steps = u.size(1);
+    const float* uniform = array<float>(a[3], at::kFloat, {B, steps}, dev, "sample_u");
+    const int32_t* q_start =
+        a[4] == Py_None ? nullptr : array<int32_t>(a[4], at::kInt, {B + 1}, dev, "q_start");
+    if (B > INT32_MAX || steps > INT32_MAX || V > INT32_MAX) refuse("verify_tree: too many sequences, steps or tokens");
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(dev));
+    const at::Tensor all = fresh({B * (2 * steps + 1)}, at::kInt, dev);
+    at::Tensor drawn = part_of(all, 0, {B, steps}), path = part_of(all, B * steps, {B, steps}),
+               accepted = part_of(all, 2 * B * steps, {B});
+    PyObject* ok = finish(g_verify_tree(target.data_ptr(), type == at::kBFloat16, tokens, parents, q_start, uniform, T,
+                                        static_cast<int32_t>(B), static_cast<int32_t>(steps),
+                                        static_cast<int32_t>(V), static_cast<int32_t*>(accepted.data_ptr()),
+                                        static_cast<int32_t*>(drawn.data_ptr()),
+                                        static_cast<int32_t*>(path.data_ptr()),
+                                        c10::cuda::getCurrentCUDAStream(dev).stream()),
+                          "dwa_verify_tree");
+    if (ok == nullptr) return nullptr;
+    Py_DECREF(ok);
+    return Py_BuildValue("(NNN)", wrap(accepted), wrap(drawn), wrap(path));
+  });
+}
+
+// (k_cache, v_cache, block_table, start, path, n_accepted, k_scale, v_scale, status); the caches are
+// one layer's, or [layers, n_pages, H_kv, page_size, d]
+PyObject* kv_keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const at::Tensor& k = tensor(a[0], "k_cache");
+    Cache c;
+    int64_t layers = 1, ld_layer = 0, ld_scale_layer = 0;
+    if (k.dim() == 5) {
+      const at::Tensor& v = tensor(a[1], "v_cache");
+      layers = k.size(0);
+      if (layers < 1) refuse("k_cache must have a layer at least");
+      if (v.sizes() != k.sizes() || v.strides() != k.strides())
+        refuse("v_cache must be like k_cache (type, shape, strides, device)");
+      ld_layer = k.stride(0);
+      at::Tensor parts[4] = {k.select(0, 0), v.select(0, 0)};
+      PyObject* of[4] = {nullptr, nullptr, a[6], a[7]};
+      for (int i = 2; i < 4; ++i)
+        if (of[i] != Py_None) {
+          const at::Tensor& scale = tensor(of[i], "scale");
+          if (scale.dim() != 4 || scale.size(0) != layers) refuse("scales must be f32 [layers, n_pages, H_kv, page_size]");
+          if (i == 3 && scale.stride(0) != ld_scale_layer) refuse("k_scale and v_scale must have the same strides");
+          ld_scale_layer = scale.stride(0);
+          parts[i] = scale.select(0, 0);
+        }
+      // of the first layer, as every call's
+      PyObject* held[4];
+      for (int i = 0; i < 4; ++i) {
+        if (parts[i].defined()) {
+          held[i] = wrap(parts[i]);
+        } else {
+          Py_INCREF(Py_None);
+          held[i] = Py_None;
+        }
+      }
+      struct Release {
+        PyObject** p;
+        ~Release() {
+          for (int i = 0; i < 4; ++i) Py_DECREF(p[i]);
+        }
+      } release{held};
+      c = cache_of(held[0], held[1], held[2], held[3]);
+    } else {
+      c = cache_of(a[0], a[1], a[6], a[7]);
+    }
+    const at::Tensor& table = block_table_of(a[2], c.dev);
+    const int64_t B = table.size(0), max_pages = table.size(1);
+    const int32_t* start = array<int32_t>(a[3], at::kInt, {B}, c.dev, "start");
+    const at::Tensor& path_t = tensor(a[4], "path");
+    if (path_t.dim() != 2) refuse("path must be int32 [B, steps] (got " + describe(path_t) + ")");
+    const int64_t steps = path_t.size(1);
+    const int32_t* path = array<int32_t>(a[4], at::kInt, {B, steps}, c.dev, "path");
+    const int32_t* kept = array<int32_t>(a[5], at::kInt, {B}, c.dev, "n_accepted");
+    int32_t* status = status_of(a[8], c.dev);
+    if (layers > INT32_MAX || B > INT32_MAX || steps > INT32_MAX || max_pages > INT32_MAX)
+      refuse("kv_cache_keep: too many layers, sequences, steps or pages");
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(c.dev));
+    return finish(g_keep(c.k, c.v, c.k_scale, c.v_scale, static_cast<int32_t>(layers), ld_layer, ld_scale_layer,
+                         static_cast<int32_t>(c.heads), static_cast<int32_t>(c.d), c.n_pages,
+                         static_cast<int32_t>(c.page), c.ld_page, c.ld_scale, static_cast<int32_t*>(table.data_ptr()),
+                         B > 1 ? table.stride(0) : max_pages, static_cast<int32_t>(max_pages), start, path, kept,
+                         static_cast<int32_t>(B), static_cast<int32_t>(steps), status,
+                         c10::cuda::getCurrentCUDAStream(c.dev).stream()),
+                  "dwa_kv_keep");
+  });
+}
+
 PyMethodDef g_methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
     {"kv_write", reinterpret_cast<PyCFunction>(kv_write), METH_FASTCALL, nullptr},
     {"kv_read", reinterpret_cast<PyCFunction>(kv_read), METH_FASTCALL, nullptr},
-    {"attend", reinterpret_cast<PyCFunction>(attend), METH_FASTCALL, nullptr},
+    {"attend", reinterpret_cast<PyCFunction>(attend<false>), METH_FASTCALL, nullptr},
     {"verify", reinterpret_cast<PyCFunction>(verify), METH_FASTCALL, nullptr},
+    {"kv_append", reinterpret_cast<PyCFunction>(kv_append), METH_FASTCALL, nullptr},
+    {"kv_keep", reinterpret_cast<PyCFunction>(kv_keep), METH_FASTCALL, nullptr},
+    {"attend_tree", reinterpret_cast<PyCFunction>(attend<true>), METH_FASTCALL, nullptr},
+    {"masks", reinterpret_cast<PyCFunction>(masks), METH_FASTCALL, nullptr},
+    {"verify_tree", reinterpret_cast<PyCFunction>(verify_tree), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, g_methods};

@@ -13,7 +13,7 @@
 
 #include "dwa_internal.h"
 #include "dwa_retrieval.h"
-#include "f32x2.cuh"
+#include "kv_store.cuh"
 #include "paged_attention.cuh"
 
 namespace dwa {
@@ -27,7 +27,6 @@ constexpr int kWriteThreads = 256;
 template <bool kE4m3, bool kSrcBf16>
 constexpr int kWriteBlocks = !kSrcBf16 ? 2 : kE4m3 ? 3 : 4;
 constexpr int kBlockTokens = 32;  // at most; a longer call is cut into launches
-constexpr int kFilterBits = 8192;  // their slots' low bits
 
 // Values of a lane: sixteen make 16 bytes of codes, eight 16 bytes of bf16.
 template <bool kE4m3>
@@ -63,24 +62,6 @@ __device__ __forceinline__ void as_f32(const Raw<kBf16, kN>& r, float (&x)[kN]) 
   }
 }
 
-// x / b correctly rounded, given y = 1 / b correctly rounded: with q = x y the remainder
-// x - q b is exact in an fma, and q + remainder y is the rounded quotient (Markstein,
-// 1990), as long as nothing underflows on the way.
-__device__ __forceinline__ float quotient(float x, float b, float y) {
-  const float q = x * y;
-  return fmaf(fmaf(-q, b, x), y, q);
-}
-
-__device__ __forceinline__ uint4 codes16(const float (&x)[16]) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    u[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]),
-                                                          __NV_SATFINITE, __NV_E4M3)) |
-           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]),
-                                                          __NV_SATFINITE, __NV_E4M3)) << 16;
-  return make_uint4(u[0], u[1], u[2], u[3]);
-}
 // Stores the eight values of this lane, rounded to bf16.
 template <bool kBf16>
 __device__ __forceinline__ void store_bf16(const Raw<kBf16, 8>& raw, uint16_t* dst) {
@@ -130,29 +111,7 @@ __device__ __forceinline__ void store_e4m3(const Raw<kBf16, 16>& raw, bool on, b
   if (finite) {
     float x[16];
     as_f32(raw, x);
-    // Tiny vectors are scaled up by 2^100, exactly, so that no remainder underflows: amax is
-    // above 2^-70 or the scale above 2^-26 then.  (Remainders of quotients above 2^-11 are
-    // above 2^-137; smaller quotients give the code 0 either way.)
-    float up = 1.f, down = 1.f, least = 0x1p-126f, most = amax;
-    if (!(amax > 0x1p-70f)) {
-      up = 0x1p100f;
-      down = 0x1p-100f;
-      least = 0x1p-26f;
-      most *= up;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= up;
-    }
-    const float s = fmaxf(quotient(most, 448.f, 1.f / 448.f), least);
-    const float y = __frcp_rn(s);
-    const uint64_t neg2 = pair(-y, -y), s2 = pair(s, s);
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {  // as quotient(), but of -x: so the remainder of a zero, +0, leaves it its sign
-      const uint64_t v = pair(x[i], x[i + 1]), q = mul2(v, neg2);
-      unpair(fma2(fma2(q, s2, v), neg2, q), x[i], x[i + 1]);
-    }
-    w = codes16(x);  // |x / s| <= 448 (1 + 2^-23), which rounds to 448 at most
-    w = make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
-    scale = s * down;
+    w = quantised16(x, amax, &scale);
   }
   if (on) *reinterpret_cast<uint4*>(cache + row * d + 16 * lane) = w;
   if (lane == 0) scales[srow] = scale;
@@ -219,33 +178,7 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks<kE4m3, kSrcBf16>)
   Values k_now{}, v_now{};
   int i_now = group / a.H, h_now = group % a.H;
   load(i_now, h_now, &k_now, &v_now);
-  for (int i = threadIdx.x; i < kFilterBits / 32; i += kWriteThreads) filter[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kWriteThreads) {
-    const int64_t s = a.slots[t0 + i];
-    const bool fine = s >= 0 && s < a.n_slots;
-    if (!fine && s != -1) paged_report(a.status);
-    own[i] = s;
-    dropped[i] = fine ? 0 : 1;
-    if (fine) atomicOr(&filter[(s & (kFilterBits - 1)) >> 5], 1u << (s & 31));
-  }
-  __syncthreads();
-  constexpr int kBatch = 8;  // slots that a thread looks at together
-  for (int64_t t = t0 + 1 + threadIdx.x; t < a.T; t += kBatch * kWriteThreads) {
-    int64_t s[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      s[j] = t + j * kWriteThreads < a.T ? __ldg(a.slots + t + j * kWriteThreads) : -1;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      if (s[j] >= 0 && ((filter[(s[j] & (kFilterBits - 1)) >> 5] >> (s[j] & 31)) & 1u)) {
-        const int before = static_cast<int>(min(t + j * kWriteThreads - t0, static_cast<int64_t>(n)));
-        for (int i = 0; i < before; ++i)
-          if (own[i] == s[j]) dropped[i] = 1;
-      }
-    }
-  }
-  __syncthreads();
+  settle_slots<kWriteThreads>(a.slots, a.T, t0, n, a.n_slots, own, dropped, filter, a.status);
   for (int base = 0; base < vectors; base += groups) {
     int i_next = i_now, h_next = h_now;
     forward(&i_next, &h_next);
@@ -378,12 +311,6 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a)
       *reinterpret_cast<uint4*>(v_out) = make_uint4(fill, fill, fill, fill);
     }
   }
-}
-
-int log2_at_least(int n) {
-  int l = 0;
-  while ((1 << l) < n) ++l;
-  return l;
 }
 
 }  // namespace

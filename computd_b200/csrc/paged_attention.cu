@@ -70,14 +70,19 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 // The halves of w (the values of one key at two channels) that are not finite
-// become 0 and note the key.
+// become 0 and note the key (of a tree the node, 0 to 15).
+template <bool kTree>
 __device__ __forceinline__ uint32_t only_finite(uint32_t w, int key, int* first_lo, int* first_hi) {
+  auto note = [&](int* at) {
+    if constexpr (kTree) atomicOr(at, 1 << key);
+    else atomicMin(at, key);
+  };
   if ((w & 0x7F80u) == 0x7F80u) {
-    atomicMin(first_lo, key);
+    note(first_lo);
     w &= 0xFFFF0000u;
   }
   if ((w & 0x7F800000u) == 0x7F800000u) {
-    atomicMin(first_hi, key);
+    note(first_hi);
     w &= 0x0000FFFFu;
   }
   return w;
@@ -135,8 +140,9 @@ __device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// kLinear: the rows of a block lie one behind the other, as in the page.
-template <bool kE4m3, int DP, int NT, int W, bool kLinear>
+// kLinear: the rows of a block lie one behind the other, as in the page.  kTree: the new tokens
+// (16 at most) see what the tree's masks say.
+template <bool kE4m3, int DP, int NT, int W, bool kLinear, bool kTree>
 __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const PagedArgs a,
@@ -148,7 +154,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   __shared__ float scales[kWarps][C::kStages][2][C::kScales];  // keys', values'
   __shared__ float part_m[kWarps][C::kRows], part_l[kWarps][C::kRows];
   __shared__ float block_m[C::kRows], block_l[C::kRows];
-  __shared__ int first_bad[DP];  // least key with a value that is not finite, by channel
+  // least key with a value that is not finite, by channel; trees: the nodes with one, as bits
+  __shared__ int first_bad[DP];
+  constexpr int kNoBad = kTree ? 0 : 0x7FFFFFFF;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   // one partial per warp, then (in warp 0's place) one per block
   float* const part_o = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)));
@@ -181,8 +189,20 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     return;
   }
   const int rows = static_cast<int>(all_rows);  // max_q bounds them to kRows
-  const int vis_min = paged_visible(seq, 0);
-  const int vis_max = paged_visible(seq, seq.n - 1);
+  const int prefix = tree_prefix(seq);
+  const int vis_min = kTree ? max(prefix, 0) : paged_visible(seq, 0);
+  const int vis_max = kTree ? seq.length : paged_visible(seq, seq.n - 1);
+  // Whether a row sees a key at the edge, of what paged_visible (or the tree's mask) says of it.
+  auto sees = [&](int key, int vis) -> bool {
+    if constexpr (kTree)
+      return key < vis_min || (key < vis_max && ((static_cast<uint32_t>(vis) >> (key - prefix)) & 1u));
+    else
+      return key < vis;
+  };
+  auto row_sees = [&](uint32_t token) -> int {
+    if constexpr (kTree) return static_cast<int>(__ldg(a.tree + (seq.row0 + token) * a.tree_words));
+    else return paged_visible(seq, token);
+  };
 
   // ------------------------------------------------ Q^T fragments, on their way
   // lane (g, t) holds row 8 nt + g at the channels its key chunks have
@@ -215,7 +235,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     for (int i = 0; i < C::kStages; ++i) mbar_init(bar0 + 8 * i, kE4m3 ? 33 : 1);  // with every lane's scales
     fence_mbar_init();
   }
-  for (int i = threadIdx.x; i < DP; i += kThreads) first_bad[i] = 0x7FFFFFFF;
+  for (int i = threadIdx.x; i < DP; i += kThreads) first_bad[i] = kNoBad;
   __syncthreads();
 
   const int n_blocks = (vis_max + C::kKeys - 1) / C::kKeys;
@@ -327,7 +347,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     for (int j = 0; j < 2; ++j) {
       factor[nt][j] = kE4m3 ? __shfl_sync(0xFFFFFFFFu, f, 4 * (2 * t + j)) : f;
       const int rc = 8 * nt + 2 * t + j;
-      vis[nt][j] = rc < rows ? paged_visible(seq, row_token(rc, a.group)) : 0;
+      vis[nt][j] = rc < rows ? row_sees(row_token(rc, a.group)) : 0;
     }
   }
 
@@ -458,7 +478,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
             for (int i = 0; i < 2; ++i) {
               float x = (s[u][nt][2 * i + j] + s2[u][nt][2 * i + j]) *
                         (kE4m3 ? sk[u][i] * factor[nt][j] : factor[nt][j]);
-              if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) x = -INFINITY;
+              if (edge && !sees(key0 + 16 * u + 8 * i + key_g, vis[nt][j])) x = -INFINITY;
               s[u][nt][2 * i + j] = x;
               top = fmaxf(top, x);
             }
@@ -485,7 +505,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
               if constexpr (kE4m3) {
                 if (!kApart) p *= sv[u][i] * v_mul;
                 // a masked key's scale may be anything: its weight is 0, not 0 times that
-                if (edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j]) p = 0.f;
+                if (edge && !sees(key0 + 16 * u + 8 * i + key_g, vis[nt][j])) p = 0.f;
               }
               s[u][nt][2 * i + j] = p;
             }
@@ -498,7 +518,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
           for (int i = 0; i < 2; ++i) sv[u][i] = fmaf(sv[u][i], 0.f, sv[u][i]);  // an infinity becomes NaN
         auto weight = [&](int u, int nt, int i, int j) -> float {
           const float x = s[u][nt][2 * i + j] * exp_scale(v_exp[nt][j]) * sv[u][i];
-          return edge && key0 + 16 * u + 8 * i + key_g >= vis[nt][j] ? 0.f : x;
+          return edge && !sees(key0 + 16 * u + 8 * i + key_g, vis[nt][j]) ? 0.f : x;
         };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -591,7 +611,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
                 const int ch = 8 * (8 * c + g) + 2 * k;
                 if (at >= vis_max) w[i][k] = 0;
                 else if (!kE4m3 && at >= vis_min)
-                  w[i][k] = only_finite(w[i][k], at, &first_bad[ch], &first_bad[ch + 1]);
+                  w[i][k] = only_finite<kTree>(w[i][k], kTree ? at - prefix : at, &first_bad[ch], &first_bad[ch + 1]);
               }
             }
           }
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
     if (ch >= a.d) continue;
     float ms[kMaxCluster], ls[kMaxCluster];
     float2 os[kMaxCluster];
-    int bad0 = 0x7FFFFFFF, bad1 = 0x7FFFFFFF;
+    int bad0 = kNoBad, bad1 = kNoBad;
     float top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
@@ -711,8 +731,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
         ls[c] = ld_cluster_f32(&block_l[r], c);
         os[c] = ld_cluster_f32x2(&part_o[r * DP + ch], c);
         if (!kE4m3) {
-          bad0 = min(bad0, ld_cluster_s32(&first_bad[ch], c));
-          bad1 = min(bad1, ld_cluster_s32(&first_bad[ch + 1], c));
+          const int x = ld_cluster_s32(&first_bad[ch], c), y = ld_cluster_s32(&first_bad[ch + 1], c);
+          bad0 = kTree ? bad0 | x : min(bad0, x);
+          bad1 = kTree ? bad1 | y : min(bad1, y);
         }
         top = fmaxf(top, ms[c]);
       }
@@ -728,9 +749,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
       }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const uint32_t row = r, token = row_token(row, a.group);
-    const int seen = paged_visible(seq, token);
-    x = bad0 < seen ? __uint_as_float(0x7FC00000u) : x * inv;
-    y = bad1 < seen ? __uint_as_float(0x7FC00000u) : y * inv;
+    const int seen = row_sees(token);
+    x = (kTree ? (bad0 & seen) != 0 : bad0 < seen) ? __uint_as_float(0x7FC00000u) : x * inv;
+    y = (kTree ? (bad1 & seen) != 0 : bad1 < seen) ? __uint_as_float(0x7FC00000u) : y * inv;
     *reinterpret_cast<uint32_t*>(a.out + (seq.row0 + token) * a.out_ld +
                                  (static_cast<int64_t>(hk) * a.group + row - token * a.group) * a.d + ch) =
         pack_bf16(x, y);
@@ -738,7 +759,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 1 : NT == 1 ? 3 : 2)
   if (cluster > 1) cluster_sync();  // no block leaves while another reads its partial
 }
 
-template <bool kE4m3, int DP, int NT, int W, bool kLinear>
+template <bool kE4m3, int DP, int NT, int W, bool kLinear, bool kTree>
 cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStream_t stream) {
   using C = RowsCfg<kE4m3, DP, NT, W>;
   CUtensorMap mk{}, mv{};
@@ -749,7 +770,7 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
                    !make_page_map(&mv, a.v, a, C::kRowBytes, box_rows, box_halves)))
     return cudaErrorInvalidValue;
   if (units * cluster > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
-  constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W, kLinear>;
+  constexpr auto kKernel = paged_rows_kernel<kE4m3, DP, NT, W, kLinear, kTree>;
   if (cudaError_t e = allow_smem_once<kKernel>(C::kSmem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
@@ -783,7 +804,7 @@ cudaError_t launch_rows(const PagedArgs& a, int64_t units, int cluster, cudaStre
 // in the page, in one bulk copy; a tiled copy goes row by row, two requests to a row that
 // crosses 128 bytes (64 sequences up to 2048, 16 heads of 80: e4m3 60 us, 46 so; bf16 63.7
 // and 62.2.  24 up to 1024 with drafts, e4m3: 18.7 and 15.8).
-template <bool kE4m3, int DP, int NT, bool kLinear>
+template <bool kE4m3, int DP, int NT, bool kLinear, bool kTree>
 cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stream) {
   const int64_t sms = device_sm_count();
   const int64_t steps = (static_cast<int64_t>(a.max_pages) << a.page_log2) / (kE4m3 ? 32 : 16);
@@ -794,30 +815,35 @@ cudaError_t launch_rows_cut(const PagedArgs& a, int64_t units, cudaStream_t stre
     cluster *= 2;
   }
   if (cluster == 2 && units <= sms && 2 * units > sms / 2)
-    return launch_rows<kE4m3, DP, NT, 8, kLinear>(a, units, 1, stream);
+    return launch_rows<kE4m3, DP, NT, 8, kLinear, kTree>(a, units, 1, stream);
   return units * cluster <= sms / 2 && steps >= 8 * cluster
-             ? launch_rows<kE4m3, DP, NT, 8, kLinear>(a, units, cluster, stream)
-             : launch_rows<kE4m3, DP, NT, 4, kLinear>(a, units, cluster, stream);
+             ? launch_rows<kE4m3, DP, NT, 8, kLinear, kTree>(a, units, cluster, stream)
+             : launch_rows<kE4m3, DP, NT, 4, kLinear, kTree>(a, units, cluster, stream);
 }
 
-template <bool kE4m3, int DP>
+template <bool kE4m3, int DP, bool kTree>
 cudaError_t launch_rows_nt(const PagedArgs& a, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
   const int64_t heads = static_cast<int64_t>(a.B) * a.H_kv;
   if (a.d % 32 != 0)
-    return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, true>(a, heads, stream)
-                     : launch_rows_cut<kE4m3, DP, 2, true>(a, heads, stream);
-  return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, false>(a, heads, stream)
-                   : launch_rows_cut<kE4m3, DP, 2, false>(a, heads, stream);
+    return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, true, kTree>(a, heads, stream)
+                     : launch_rows_cut<kE4m3, DP, 2, true, kTree>(a, heads, stream);
+  return rows <= 8 ? launch_rows_cut<kE4m3, DP, 1, false, kTree>(a, heads, stream)
+                   : launch_rows_cut<kE4m3, DP, 2, false, kTree>(a, heads, stream);
+}
+
+template <bool kTree>
+cudaError_t launch_few_rows(const PagedArgs& a, cudaStream_t stream) {
+  const bool e4m3 = a.k_scale != nullptr;
+  if (a.d <= 64) return e4m3 ? launch_rows_nt<true, 64, kTree>(a, stream) : launch_rows_nt<false, 64, kTree>(a, stream);
+  return e4m3 ? launch_rows_nt<true, 128, kTree>(a, stream) : launch_rows_nt<false, 128, kTree>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream) {
   if (static_cast<int64_t>(a.max_q) * a.group > kFewRows) return launch_paged_attention_mma(a, stream);
-  const bool e4m3 = a.k_scale != nullptr;
-  if (a.d <= 64) return e4m3 ? launch_rows_nt<true, 64>(a, stream) : launch_rows_nt<false, 64>(a, stream);
-  return e4m3 ? launch_rows_nt<true, 128>(a, stream) : launch_rows_nt<false, 128>(a, stream);
+  return a.tree != nullptr ? launch_few_rows<true>(a, stream) : launch_few_rows<false>(a, stream);
 }
 
 }  // namespace dwa

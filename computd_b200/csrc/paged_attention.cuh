@@ -31,6 +31,9 @@ struct PagedArgs {
   int d;
   float scale_log2;  // scale * log2(e)
   int32_t* status;
+  // Trees: the nodes that a row's new token sees, tree_words words of 32 bits to a token.
+  const uint32_t* tree;
+  int tree_words;
 };
 
 // One sequence as the device finds it.
@@ -95,6 +98,40 @@ __device__ __forceinline__ int ranked(int n, int rank, int* costs, int* found, F
 // Tokens that new token i may see.
 __device__ __forceinline__ int paged_visible(const PagedSeq& s, int i) {
   return max(s.length - s.n + i + 1, 0);
+}
+
+// Trees.  Every new token of a sequence sees the tokens before the first of them, and of the new
+// ones those that its mask names: node j is cached token length - n + j.
+__device__ __forceinline__ int tree_prefix(const PagedSeq& s) { return s.length - s.n; }  // below 0: nodes without a place
+// 32 keys from node `at` on that the token in row `row` of q sees, as bits; what lies before
+// node 0 is seen by all.
+__device__ __forceinline__ uint32_t tree_bits(const PagedArgs& a, int64_t row, int at) {
+  if (at <= -32) return 0xFFFFFFFFu;
+  const uint32_t* mask = a.tree + row * a.tree_words;
+  const int w = at >> 5;  // -1 where bits before node 0 are among them
+  const uint32_t lo = w < 0 ? 0xFFFFFFFFu : w < a.tree_words ? __ldg(mask + w) : 0u;
+  const uint32_t hi = w + 1 < a.tree_words ? __ldg(mask + w + 1) : 0u;
+  return __funnelshift_r(lo, hi, at & 31);
+}
+// Whether that token sees a node whose value is not finite: in channel ch of a bf16 cache, of an
+// e4m3 one at all.  (Only where a block met such a value.)
+template <bool kE4m3>
+__device__ __noinline__ bool tree_sees_bad(const PagedArgs& a, const PagedSeq& s, const int32_t* table, int hk,
+                                           int64_t row, int ch) {
+  const int prefix = tree_prefix(s);
+  for (int node = max(-prefix, 0); node < s.n; ++node) {
+    if (!(tree_bits(a, row, node) & 1u)) continue;
+    const int key = prefix + node, page = __ldg(table + (key >> a.page_log2));
+    if (page < 0 || page >= a.n_pages) continue;
+    const int64_t at = (static_cast<int64_t>(hk) << a.page_log2) + (key & ((1 << a.page_log2) - 1));
+    if constexpr (kE4m3) {
+      if (!(fabsf(__ldg(a.v_scale + page * a.ld_scale_page + at)) < INFINITY)) return true;
+    } else {
+      const uint16_t x = __ldg(static_cast<const uint16_t*>(a.v) + page * a.ld_page + at * a.d + ch);
+      if ((x & 0x7F80u) == 0x7F80u) return true;
+    }
+  }
+  return false;
 }
 
 // The new token of a row (rows are token-major, `group` query heads to a token).

@@ -333,7 +333,7 @@ __device__ __forceinline__ void regs_dec() {
 }
 
 
-template <bool kE4m3, int DP>
+template <bool kE4m3, int DP, bool kTree>
 __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const PagedArgs a, const int row_units, const int cluster) {
@@ -358,7 +358,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       const PagedSeq s = paged_seq(a, i % a.B);
       const int64_t first = static_cast<int64_t>(row_units - 1 - i / a.B) * 2 * kTile;
       const int64_t end = min(first + 2 * kTile, static_cast<int64_t>(s.n) * a.group);
-      return first < end ? paged_visible(s, row_token(static_cast<uint32_t>(end - 1), a.group)) : -1;
+      return first >= end ? -1
+             : kTree      ? s.length
+                          : paged_visible(s, row_token(static_cast<uint32_t>(end - 1), a.group));
     });
   const int ru = row_units - 1 - pair_of / a.B, b = pair_of % a.B;
   const PagedSeq seq = paged_seq(a, b);
@@ -381,9 +383,13 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
   const int rows0 = static_cast<int>(min(left, static_cast<int64_t>(kTile)));
   const int rows1 = static_cast<int>(max(min(left - kTile, static_cast<int64_t>(kTile)), int64_t{0}));
   const uint32_t row_0 = static_cast<uint32_t>(r0);  // below 2^31: max_q bounds it
-  const int vis_min = paged_visible(seq, row_token(row_0, a.group));
-  const int vis0 = paged_visible(seq, row_token(row_0 + rows0 - 1, a.group));
-  const int vis1 = rows1 > 0 ? paged_visible(seq, row_token(row_0 + kTile + rows1 - 1, a.group)) : 0;
+  const int prefix = tree_prefix(seq);
+  auto visible = [&](uint32_t row) -> int {  // keys before the one behind the last that the row sees
+    return kTree ? seq.length : paged_visible(seq, row_token(row, a.group));
+  };
+  const int vis_min = kTree ? max(prefix, 0) : visible(row_0);
+  const int vis0 = visible(row_0 + rows0 - 1);
+  const int vis1 = rows1 > 0 ? visible(row_0 + kTile + rows1 - 1) : 0;
   const int vis_max = max(vis0, vis1);
   // this block's share of the key tiles, and how far each row tile goes into it
   const int tiles_all = (vis_max + kTile - 1) / kTile;
@@ -858,9 +864,10 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     const bool live = r < rows;
     const bool warp_live = 32 * (warp & 3) < rows;
     const uint32_t row0 = static_cast<uint32_t>(r0) + i * kTile;
-    const int vis = live ? paged_visible(seq, row_token(row0 + r, a.group)) : 0;
+    const int vis = live ? visible(row0 + r) : 0;
+    const int64_t tree_row = seq.row0 + (live ? row_token(row0 + r, a.group) : 0);
     // least visible count in the warp: steps below it need no mask
-    const int vis_low = __reduce_min_sync(0xFFFFFFFFu, vis);
+    const int vis_low = kTree ? vis_min : __reduce_min_sync(0xFFFFFFFFu, vis);
     // P = exp2(x + ref), l its sum, 0 until the row has seen a key: ref is minus the row's maximum
     // when it was last set, and kPBits more where that is exact enough (P up to 2^(11 + kSlack)
     // is a number of fp16, 2^(16 + kSlack) is not)
@@ -932,10 +939,17 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         }
         if (edge) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            uint32_t seen = 0u;
+            if constexpr (kTree) {
+              const int end = vis - (key0 + 32 * c);  // no key of the sequence from there on
+              if (end > 0)
+                seen = tree_bits(a, tree_row, key0 + 32 * c - prefix) & (end >= 32 ? 0xFFFFFFFFu : (1u << end) - 1u);
+            }
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (key0 + 32 * c + k >= vis) s[c][k] = 0xFF800000u;
+              if (kTree ? !((seen >> k) & 1u) : key0 + 32 * c + k >= vis) s[c][k] = 0xFF800000u;
+          }
         }
         float top[4];
 #pragma unroll
@@ -1106,7 +1120,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           if (some_bad) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (sh.first_bad[kE4m3 ? 0 : 32 * c + k] < vis) o[k] = __uint_as_float(0x7FC00000u);
+              if (sh.first_bad[kE4m3 ? 0 : 32 * c + k] < vis &&
+                  (!kTree || tree_sees_bad<kE4m3>(a, seq, table, hk, tree_row, 32 * c + k)))
+                o[k] = __uint_as_float(0x7FC00000u);
           }
 #pragma unroll
           for (int k = 0; k < 32; k += 8)
@@ -1199,12 +1215,14 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         uint16_t* const out = a.out + (seq.row0 + token) * a.out_ld +
                               (static_cast<int64_t>(hk) * a.group + of_unit - token * a.group) * a.d + 4 * x;
         if (some_bad) {
-          const int vis_q = paged_visible(seq, token);
+          const int vis_q = visible(of_unit);
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (sh.first_bad[kE4m3 ? 0 : 16 * t + 4 * x + e] < vis_q) y[t][e] = __uint_as_float(0x7FC00000u);
+              if (sh.first_bad[kE4m3 ? 0 : 16 * t + 4 * x + e] < vis_q &&
+                  (!kTree || tree_sees_bad<kE4m3>(a, seq, table, hk, seq.row0 + token, 16 * t + 4 * x + e)))
+                y[t][e] = __uint_as_float(0x7FC00000u);
         }
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t)
@@ -1226,7 +1244,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
 // (a block fills an SM, and a cluster has to find its SMs in one part of the chip: 15 of 8
 // blocks on 148 SMs).  Also lets the kernel have its shared memory, and checks that the
 // launch brings the registers that the warps share out among themselves.
-template <bool kE4m3, int DP>
+template <bool kE4m3, int DP, bool kTree>
 cudaError_t configure_mma(cudaLaunchConfig_t cfg, const int** clusters) {
   using C = MmaCfg<kE4m3, DP>;
   static std::atomic<bool> done[64] = {};
@@ -1240,12 +1258,12 @@ cudaError_t configure_mma(cudaLaunchConfig_t cfg, const int** clusters) {
   const std::lock_guard<std::mutex> lock(once);
   if (done[dev].load(std::memory_order_relaxed)) return cudaSuccess;  // meanwhile
   cudaFuncAttributes attr;
-  if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_mma_kernel<kE4m3, DP>); e != cudaSuccess)
+  if (cudaError_t e = cudaFuncGetAttributes(&attr, paged_mma_kernel<kE4m3, DP, kTree>); e != cudaSuccess)
     return e;
   if (attr.numRegs * C::kThreads <
       256 * C::kSoftmaxRegs + (C::kThreads - 256) * C::kOtherRegs)
     return cudaErrorInvalidConfiguration;
-  if (cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<kE4m3, DP>,
+  if (cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<kE4m3, DP, kTree>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       e != cudaSuccess)
     return e;
@@ -1258,7 +1276,7 @@ cudaError_t configure_mma(cudaLaunchConfig_t cfg, const int** clusters) {
     cfg.gridDim = dim3(1u << i);
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&found[i], paged_mma_kernel<kE4m3, DP>, &cfg);
+    if (cudaError_t e = cudaOccupancyMaxActiveClusters(&found[i], paged_mma_kernel<kE4m3, DP, kTree>, &cfg);
         e != cudaSuccess)
       return e;
   }
@@ -1267,7 +1285,7 @@ cudaError_t configure_mma(cudaLaunchConfig_t cfg, const int** clusters) {
   return cudaSuccess;
 }
 
-template <bool kE4m3, int DP>
+template <bool kE4m3, int DP, bool kTree>
 cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   using C = MmaCfg<kE4m3, DP>;
   CUtensorMap mk, mv;
@@ -1283,7 +1301,7 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   const int* at_a_time;
-  if (cudaError_t e = configure_mma<kE4m3, DP>(cfg, &at_a_time); e != cudaSuccess) return e;
+  if (cudaError_t e = configure_mma<kE4m3, DP, kTree>(cfg, &at_a_time); e != cudaSuccess) return e;
   // How many blocks share a unit's keys: what takes clearly the fewest rounds of steps
   // (a step is 3000 to 3900 cycles), if every sequence were as long as the table allows.  A
   // block costs about three steps more than its keys, a split one six and more: its
@@ -1308,15 +1326,20 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, paged_mma_kernel<kE4m3, DP>, mk, mv, a, row_units, cluster);
+  return cudaLaunchKernelEx(&cfg, paged_mma_kernel<kE4m3, DP, kTree>, mk, mv, a, row_units, cluster);
+}
+
+template <bool kTree>
+cudaError_t launch_many_rows(const PagedArgs& a, cudaStream_t stream) {
+  const bool e4m3 = a.k_scale != nullptr;
+  if (a.d <= 64) return e4m3 ? launch_mma<true, 64, kTree>(a, stream) : launch_mma<false, 64, kTree>(a, stream);
+  return e4m3 ? launch_mma<true, 128, kTree>(a, stream) : launch_mma<false, 128, kTree>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_attention_mma(const PagedArgs& a, cudaStream_t stream) {
-  const bool e4m3 = a.k_scale != nullptr;
-  if (a.d <= 64) return e4m3 ? launch_mma<true, 64>(a, stream) : launch_mma<false, 64>(a, stream);
-  return e4m3 ? launch_mma<true, 128>(a, stream) : launch_mma<false, 128>(a, stream);
+  return a.tree != nullptr ? launch_many_rows<true>(a, stream) : launch_many_rows<false>(a, stream);
 }
 
 }  // namespace dwa

@@ -46,7 +46,8 @@ finish run in libdwa_b200.so.
 it takes the newest tokens of any number of sequences (prompts in pieces, single
 tokens, drafted ones), writes their keys and values and attends to the pages with
 ``kv_cache``'s kernels.  ``DWALM.verify`` scores drafted tokens that way and
-decides with ``verify_drafts`` which of them stand.
+decides with ``verify_drafts`` which of them stand; ``DWALM.verify_tree`` does so for
+trees of them, several candidates to a place.
 """
 from __future__ import annotations
 
@@ -59,7 +60,7 @@ import torch.nn.functional as F
 
 from .assembler import WeightAssembler
 from .assembly import _check_values
-from .kv_cache import PagedKVCache, verify_drafts
+from .kv_cache import PagedKVCache, tree_masks, verify_drafts, verify_tree
 from .lm_ops import aspect_queries, rope_qk
 from .retrieval import MultiAspectRetrieval, Retriever, project_keys_packed
 from .tiled_topk import _as_bf16_rows
@@ -136,6 +137,7 @@ class ChunkStep:
     q_start: torch.Tensor
     max_q: int
     padded: bool               # rows may follow the last sequence's
+    tree_mask: torch.Tensor | None = None  # int64 [T, W]: the rows are nodes of trees
 
 
 def plan_rows(tokens: int) -> int:
@@ -212,14 +214,16 @@ class CausalSelfAttention(nn.Module):
         their keys and values go into the cache, their queries attend to it."""
         _, T, C = x.shape
         qkv = self.qkv(self.norm(x))
-        q, k = rope_qk(qkv, step.cos, step.sin, self.h, self.dh)
-        q, k = (t.transpose(1, 2)[0] for t in (q, k))  # the kernel's token-major buffers
-        v = qkv[0, :, 2 * C:].view(T, self.h, self.dh)
-        step.cache.write(layer, k, v, step.slots)
+        q, k, v = (qkv[0, :, i * C:(i + 1) * C].view(T, self.h, self.dh) for i in range(3))
+        # rotated as forward's rope_qk does, bit for bit
+        q = step.cache.append(layer, q, k, v, step.cos, step.sin, step.slots)
         # the attention leaves a padded batch's last rows as they are
         out = torch.zeros((T, self.h, self.dh), dtype=q.dtype, device=q.device) if step.padded else None
-        o = step.cache.attend(layer, q, step.block_table, step.lengths, q_start=step.q_start,
-                              max_q=step.max_q, out=out)
+        kw = dict(q_start=step.q_start, max_q=step.max_q, out=out)
+        if step.tree_mask is None:
+            o = step.cache.attend(layer, q, step.block_table, step.lengths, **kw)
+        else:
+            o = step.cache.attend_tree(layer, q, step.block_table, step.lengths, step.tree_mask, **kw)
         return x + self.proj(o.view(1, T, C))
 
 
@@ -378,7 +382,7 @@ class DWALM(nn.Module):
     @torch.no_grad()
     def extend(self, token_ids: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor,
                lengths: torch.Tensor, q_start: torch.Tensor | None = None,
-               max_q: int | None = None) -> torch.Tensor:
+               max_q: int | None = None, *, parents: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [T, vocab] of the newest tokens of B sequences, whose earlier tokens are cached.
 
         ``token_ids`` [T] packs the new tokens: rows q_start[b] to q_start[b + 1] - 1 (int32
@@ -387,6 +391,10 @@ class DWALM(nn.Module):
         [B, max_pages] holds its pages.  ``max_q`` bounds the new tokens of any sequence.
         Rows of no sequence (a padded batch; their tokens are in the vocabulary too) attend to
         nothing.
+
+        With ``parents`` (int32 [T], as ``kv_cache.tree_masks`` takes them) a sequence's new tokens are the
+        nodes of a tree: each follows its parent, and sees the tokens cached before the tree, its
+        ancestors and itself.  (``max_q`` is 4096 at most then.)
 
         The retrieval is planned once for all row counts T that ``plan_rows`` rounds to the
         same (a captured graph needs such a call before).  Calls that share a plan share its
@@ -408,11 +416,18 @@ class DWALM(nn.Module):
             return torch.empty((0, self.cfg.vocab), dtype=self.fc2.weight.dtype, device=token_ids.device)
         plan = self._chunk_plan(T)
         slots, positions = cache.slots(block_table, lengths, q_start, T)
+        max_q = T if max_q is None else max_q
+        mask = None
+        if parents is not None:
+            mask, depth = tree_masks(parents, q_start=q_start, max_q=max_q, status=cache.status)
+            row, start = torch.arange(T, device=q_start.device), q_start.long()
+            node = row - start[(torch.searchsorted(start, row, right=True) - 1).clamp(0, B - 1)]
+            positions = positions - node + depth  # a node's place in its path, not in the cache
         dh = self.cfg.d_model // self.cfg.n_heads
         f = torch.outer(positions.float(), _rope_theta(dh, positions.device))
         dtype = self.embed.weight.dtype
         step = ChunkStep(cache, f.cos().to(dtype), f.sin().to(dtype), slots, block_table, lengths,
-                         q_start, T if max_q is None else max_q, padded)
+                         q_start, max_q, padded, mask)
         h = self.embed_norm(self.embed_proj(self.embed(token_ids[None])))
         for i, blk in enumerate(self.blocks):
             h = blk.extend(h, plan, self.vectors, step, i)
@@ -462,6 +477,53 @@ class DWALM(nn.Module):
         accepted, tokens = verify_drafts(probs, draft_tokens, draft_probs, accept_u, sample_u,
                                          draft_lengths=draft_lengths)
         cache.report(lost)
+        accepted = torch.where(lost, 0, accepted)
+        return accepted, torch.where(lost[:, None], -1, tokens), torch.where(lost, lengths, lengths + 1 + accepted)
+
+
+    @torch.no_grad()
+    def verify_tree(self, last_tokens: torch.Tensor, tree_tokens: torch.Tensor, parents: torch.Tensor,
+                    sample_u: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor,
+                    lengths: torch.Tensor, *,
+                    temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One speculative step with a tree of drafts for every sequence: score them all at once, walk
+        down as far as the drawn tokens are drafts, and keep that path in the cache.
+
+        Draft i = 1 .. N of sequence b is ``tree_tokens``[b, i - 1] (int32 [B, N]) and follows draft
+        ``parents``[b, i - 1] (int32 [B, N], or [N] for all; below i), or ``last_tokens``[b] (int [B], the sequence's
+        newest token, not yet cached) where that is 0; -1 where there is no such draft.  They are appended to the ``lengths`` (int32 [B])
+        cached tokens; the pages in ``block_table`` must have room for N + 1 more.  ``sample_u`` f32
+        [B, D + 1] are the uniform numbers of the draws, D the most drafts that may stand.  Returns
+        (n_accepted int32 [B], tokens int32 [B, D + 1]: the standing drafts, the token drawn after
+        them, then -1; new lengths int32 [B]: the cached tokens that stay).  tokens[b, n_accepted[b]] is
+        the next step's ``last_tokens[b]``.  A last token outside the vocabulary is reported in the cache's status; its
+        sequence gets no tokens, only -1, and stays as long as it was.  ``temperature`` as for ``verify``."""
+        if not isinstance(temperature, torch.Tensor) and not 1e-30 <= temperature <= 1e30:
+            raise ValueError(f"temperature must be a positive number, of 1e-30 to 1e30 (got {temperature})")
+        if tree_tokens.dim() != 2 or tree_tokens.dtype != torch.int32:
+            raise ValueError("tree_tokens must be int32 [B, N]")
+        B, N = tree_tokens.shape
+        if parents.dtype != torch.int32 or tuple(parents.shape) not in ((N,), (B, N)):
+            raise ValueError(f"parents must be int32 {[B, N]} or {[N]}")
+        if sample_u.dtype != torch.float32 or sample_u.dim() != 2 or sample_u.shape[0] != B \
+                or sample_u.shape[1] < 1 or not sample_u.is_contiguous():
+            raise ValueError(f"sample_u must be a contiguous torch.float32 [{B}, D + 1]")
+        if last_tokens.numel() != B or last_tokens.is_floating_point():
+            raise ValueError(f"last_tokens must be integers [{B}]")
+        if N + 1 > 4096:
+            raise ValueError(f"a tree has 4095 drafts at most (got {N})")
+        last = last_tokens.view(B)
+        lost = (last < 0) | (last >= self.cfg.vocab)
+        chunk = torch.cat([last.view(B, 1).to(torch.int32), tree_tokens], 1).reshape(-1)
+        above = torch.cat([torch.full((B, 1), -1, dtype=torch.int32, device=chunk.device),
+                           parents.expand(B, N)], 1).reshape(-1)
+        logits = self.extend(chunk.clamp(0, self.cfg.vocab - 1).long(), cache, block_table, lengths + (N + 1),
+                             parents=above)
+        probs = torch.softmax(logits.float() / temperature, -1)
+        # a draft outside the vocabulary is never drawn
+        accepted, tokens, path = verify_tree(probs, chunk, above, sample_u)
+        cache.report(lost)
+        cache.keep(block_table, lengths, path, torch.where(lost, -1, accepted))
         accepted = torch.where(lost, 0, accepted)
         return accepted, torch.where(lost[:, None], -1, tokens), torch.where(lost, lengths, lengths + 1 + accepted)
 

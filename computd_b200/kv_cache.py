@@ -10,6 +10,15 @@ a chunk forward over one (``DWALM.extend``, ``DWALM.verify``):
 * ``paged_attention`` attends from every sequence's newest tokens (one, a few
   drafted ones, a prompt's piece) to its pages.
 * ``verify_drafts`` holds drafted tokens against the target's probabilities.
+* ``kv_cache_append`` is ``kv_cache_write`` with the rotary embedding of the keys, and the
+  queries', on the way.
+* ``tree_masks``, ``paged_tree_attention``, ``verify_tree`` and ``kv_cache_keep`` do for a tree of drafted
+  tokens (several candidates to a place) what a chunk's causal attention and ``verify_drafts`` do for
+  one row of them (``DWALM.verify_tree``).
+
+A tree is a sequence's n newest tokens: node 0 the newest that stands, the others drafts, parents before
+children.  The cache holds node j as token length - n + j until ``kv_cache_keep`` moves the path that
+stood.
 
 A cache is a pair of tensors [n_pages, H_kv, page_size, d] (bf16, or
 float8_e4m3fn with f32 scales [n_pages, H_kv, page_size]); pages may be strided,
@@ -50,7 +59,9 @@ def _host():
                               ) from e
         host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                     for name in ("dwa_kv_write", "dwa_kv_read", "dwa_paged_attention",
-                                 "dwa_verify_drafts")), _lib.check)
+                                 "dwa_verify_drafts", "dwa_kv_append", "dwa_kv_keep",
+                                 "dwa_paged_tree_attention", "dwa_tree_masks", "dwa_verify_tree")),
+                  _lib.check)
         _host_module = host
     return _host_module
 
@@ -109,6 +120,90 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                             k_scale, v_scale, scale, out, status)
 
 
+def kv_cache_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                    sin: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, *,
+                    positions: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                    v_scale: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                    status: torch.Tensor | None = None) -> torch.Tensor | None:
+    """``kv_cache_write`` of T tokens whose keys are rotated for their positions on the way;
+    returns their queries rotated (bf16 [T, H, d]), or None without ``q``.
+
+    ``q`` [T, H, d], ``k`` and ``v`` [T, H_kv, d] (all bf16 or all f32; token and head strides as for
+    ``kv_cache_write``), ``cos`` and ``sin`` [n_positions, d / 2] (both bf16 or both f32), ``positions``
+    int64 [T] their rows (default: token t has row t).  With x1 = x[0::2] and x2 = x[1::2] a rotated vector is
+    [x1 cos - x2 sin, x1 sin + x2 cos].  bf16 tensors with bf16 tables round every step to bf16,
+    which equals ``lm_ops.rope_qk`` and ``kv_cache_write`` bit for bit; otherwise all is f32 and rounded once
+    (e4m3 keys are coded from their f32 values).  A position outside the tables makes its query
+    and keys NaN, and is reported."""
+    return (_host_module or _host()).kv_append(q, k, v, cos, sin, k_cache, v_cache, slots, positions, k_scale,
+                                               v_scale, q_out, status)
+
+
+def tree_masks(parents: torch.Tensor, *, q_start: torch.Tensor | None = None, n_trees: int | None = None,
+               max_q: int | None = None,
+               status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the nodes of trees see: (mask int64 [T, W], depth int32 [T]).
+
+    ``parents`` int32 [T] packs the trees' nodes, rows q_start[b] to q_start[b + 1] - 1 (int32
+    [B + 1]) of tree b, or ``n_trees`` equal trees (default one): the number of a node's parent in its
+    tree, which is below its own, or -1.  Bit j % 64 of word j // 64 of a node's row says that it is node j or
+    below it; its depth is the number of nodes above it.  W = ceil(max_q / 64) words, where ``max_q``
+    (default: T, or T / n_trees; 4096 at most) bounds a tree's nodes.  A parent that does not come before its node is reported
+    and counts as none; rows of no tree, and of one with more than ``max_q`` nodes, are zeros."""
+    return (_host_module or _host()).masks(parents, q_start, n_trees, max_q, status)
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_table: torch.Tensor, lengths: torch.Tensor, tree_mask: torch.Tensor, *,
+                         q_start: torch.Tensor | None = None, max_q: int | None = None,
+                         k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                         scale: float | None = None, out: torch.Tensor | None = None,
+                         status: torch.Tensor | None = None) -> torch.Tensor:
+    """``paged_attention`` of new tokens that are the nodes of trees (bf16 [T, H, d]).
+
+    Node i of a sequence's n new tokens attends to its first length - n tokens, and to node j (cached
+    as token length - n + j) where bit j % 64 of word j // 64 of its row of ``tree_mask`` (int64 [T, W])
+    is set: those of ``tree_masks``, or any others.  Bits from n on count for nothing; a node sees
+    itself only if its own bit is set, and one that sees nothing gets zeros.  ``max_q`` bounds a tree's
+    nodes, is 64 W at most, and decides as for ``paged_attention`` how many bits the probabilities
+    keep.  Everything else, the other arguments, rows of no sequence and values that are not finite,
+    is as there."""
+    return (_host_module or _host()).attend_tree(q, k_cache, v_cache, block_table, lengths, q_start, max_q,
+                                                 k_scale, v_scale, scale, out, status, tree_mask)
+
+
+def verify_tree(target_probs: torch.Tensor, tree_tokens: torch.Tensor, parents: torch.Tensor,
+                sample_u: torch.Tensor, *,
+                q_start: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The walk through verified trees.
+
+    ``target_probs`` [T, V] (f32 or bf16, contiguous) are the target's probabilities behind every node,
+    ``tree_tokens`` int32 [T] the nodes' tokens (node 0's is not looked at), ``parents`` int32 [T] as for
+    ``tree_masks``, ``sample_u`` f32 [B, steps] uniform in [0, 1); rows q_start[b] to q_start[b + 1] - 1
+    (int32 [B + 1]) are tree b, or T / B each.  From node 0 on, step s draws a token from the node's row (the lowest
+    index whose running sum exceeds sample_u[b, s] times the row's sum) and goes to the node's first
+    child with that token, or ends.  The tokens are distributed as the target's, whatever proposed
+    the drafts.  At most steps - 1 drafts are passed.
+
+    Returns (n_accepted int32 [B], tokens int32 [B, steps]: the passed drafts, the last drawn token,
+    then -1; path int32 [B, steps]: the nodes passed, 0 first, then -1), parts of one allocation."""
+    return (_host_module or _host()).verify_tree(target_probs, tree_tokens, parents, sample_u, q_start)
+
+
+def kv_cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
+                  path: torch.Tensor, n_accepted: torch.Tensor, *, k_scale: torch.Tensor | None = None,
+                  v_scale: torch.Tensor | None = None, status: torch.Tensor | None = None) -> None:
+    """Move the cached tokens of the paths that stood to where their sequences' tokens belong.
+
+    Sequence b's token start[b] + path[b, i] becomes token start[b] + i for i = 0 .. n_accepted[b]
+    (``start`` and ``n_accepted`` int32 [B], ``path`` int32 [B, steps], as ``verify_tree`` returns them), on the
+    pages of ``block_table`` (int32 [B, max_pages]).  The caches are one layer's, or all layers'
+    [layers, n_pages, H_kv, page_size, d].  Paths ascend; one that does not, or that leaves
+    the pages, is reported and its sequence stays as it was."""
+    (_host_module or _host()).kv_keep(k_cache, v_cache, block_table, start, path, n_accepted, k_scale, v_scale,
+                                      status)
+
+
 class PagedKVCache:
     """The keys and values of a model's layers on one set of pages.
 
@@ -152,6 +247,12 @@ class PagedKVCache:
         k_cache, v_cache, more = self._layer(layer)
         kv_cache_write(k, v, k_cache, v_cache, slots, **more)
 
+    def append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+               sin: torch.Tensor, slots: torch.Tensor, **kw) -> torch.Tensor | None:
+        """``kv_cache_append`` to one layer."""
+        k_cache, v_cache, more = self._layer(layer)
+        return kv_cache_append(q, k, v, cos, sin, k_cache, v_cache, slots, **more, **kw)
+
     def read(self, layer: int, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """``kv_cache_read`` from one layer."""
         k_cache, v_cache, more = self._layer(layer)
@@ -162,6 +263,18 @@ class PagedKVCache:
         """``paged_attention`` over one layer."""
         k_cache, v_cache, more = self._layer(layer)
         return paged_attention(q, k_cache, v_cache, block_table, lengths, **more, **kw)
+
+    def attend_tree(self, layer: int, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                    tree_mask: torch.Tensor, **kw) -> torch.Tensor:
+        """``paged_tree_attention`` over one layer."""
+        k_cache, v_cache, more = self._layer(layer)
+        return paged_tree_attention(q, k_cache, v_cache, block_table, lengths, tree_mask, **more, **kw)
+
+    def keep(self, block_table: torch.Tensor, start: torch.Tensor, path: torch.Tensor,
+             n_accepted: torch.Tensor) -> None:
+        """``kv_cache_keep`` in every layer, in one launch."""
+        kv_cache_keep(self.k, self.v, block_table, start, path, n_accepted, k_scale=self.k_scale,
+                      v_scale=self.v_scale, status=self.status)
 
     def slots(self, block_table: torch.Tensor, lengths: torch.Tensor, q_start: torch.Tensor,
               n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:

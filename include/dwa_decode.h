@@ -1,7 +1,7 @@
 /*
  * dwa_decode.h — the serving operators of this library's DWA language model:
  * a paged key/value cache (written, read back, attended to) and the
- * verification of drafted tokens.  Same conventions as dwa_retrieval.h:
+ * verification of drafted tokens, in chains or trees.  Same conventions as dwa_retrieval.h:
  * stream-ordered and asynchronous, arguments validated on the host (non-zero
  * status, nothing launched, when invalid), no allocation, bf16 buffers as
  * uint16 bit patterns, e4m3 buffers as bytes.
@@ -111,6 +111,92 @@ DWA_API dwa_status dwa_verify_drafts(const void* target, const void* draft, int3
                                      const float* sample_u, const int32_t* draft_lengths, int64_t B,
                                      int32_t K, int32_t V, int32_t* n_accepted, int32_t* out_tokens,
                                      dwa_stream_t stream);
+
+/*
+ * Writes T tokens' keys and values into the cache as dwa_kv_write does, the keys rotated
+ * for their positions, and their queries' rotation into q_out (bf16 [T][H][d] contiguous;
+ * q NULL: no queries, H and q_out are not looked at).  For a vector x with x1 = x[0::2], x2 = x[1::2]
+ * and row p = positions[t] (int64; NULL: t) of cos and sin ([n_positions][ld_table], d / 2
+ * used; both bf16 when tables_bf16 else f32)
+ *   [x1 cos - x2 sin, x1 sin + x2 cos].
+ * With bf16 q, k, v (src_bf16) and bf16 tables every product, sum and difference is rounded to bf16,
+ * as dwa_lm_rope_qk does; otherwise they are f32, and the result is rounded once where it is
+ * stored (an e4m3 key from its f32 values).  A position outside the tables makes its
+ * token's query and keys NaN (its values stay) and is reported in *status.
+ * Tables' rows 16-byte aligned; everything else as dwa_kv_write wants it.
+ */
+DWA_API dwa_status dwa_kv_append(const void* q, const void* k, const void* v, int32_t src_bf16, int64_t T,
+                                 int32_t H, int32_t H_kv, int32_t d, int64_t q_ld_tok, int64_t q_ld_head,
+                                 int64_t k_ld_tok, int64_t k_ld_head, int64_t v_ld_tok, int64_t v_ld_head,
+                                 const void* cos_t, const void* sin_t, int32_t tables_bf16, int64_t ld_table,
+                                 int64_t n_positions, const int64_t* positions, const int64_t* slots,
+                                 void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                 int64_t n_pages, int32_t page_size, int64_t ld_page, int64_t ld_scale_page,
+                                 void* q_out, int32_t* status, dwa_stream_t stream);
+
+/*
+ * Trees of drafted tokens.  Sequence b's tree is its new tokens, rows q_start[b] ..
+ * q_start[b + 1] - 1 of T packed ones (q_start NULL: T / B each): nodes 0, 1, ..., parents before
+ * children, parents[row] a node's parent's number (-1: none).
+ *
+ * dwa_tree_masks: mask (uint64 [T][mask_words]) gets in every node's row its own bit and its
+ * ancestors' (node j: bit j % 64 of word j / 64), depth (int32 [T]) the number of its ancestors.
+ * max_q (4096 at most) bounds the nodes of a tree; mask_words >= max_q / 64.  A node whose parent
+ * is not before it counts as one without a parent and is reported in *status; a tree of more than max_q
+ * nodes is reported and its rows are zeros, as rows of no sequence are.
+ */
+DWA_API dwa_status dwa_tree_masks(const int32_t* parents, const int32_t* q_start, int64_t T, int32_t B,
+                                  int32_t max_q, int64_t* mask, int32_t mask_words, int32_t* depth,
+                                  int32_t* status, dwa_stream_t stream);
+
+/*
+ * dwa_paged_attention for new tokens that are a tree's nodes: node i of n attends to the first
+ * length - n tokens, and to node j (token length - n + j) where bit j of its row of tree_mask
+ * (uint64 [T][mask_words], 8-byte aligned) is set.  Any bits may be; those from n on count for nothing.
+ * max_q is 64 mask_words at most.  All else, the rounding too, as there.
+ */
+DWA_API dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
+                                            const void* k_cache, const void* v_cache,
+                                            const float* k_scale, const float* v_scale, int32_t H_kv,
+                                            int64_t n_pages, int32_t page_size, int64_t ld_page,
+                                            int64_t ld_scale_page, const int32_t* block_table,
+                                            int64_t ld_table, int32_t max_pages, const int32_t* lengths,
+                                            const int32_t* q_start, int32_t B, int32_t max_q,
+                                            const int64_t* tree_mask, int32_t mask_words, float scale,
+                                            void* out, int64_t out_ld, int32_t* status,
+                                            dwa_stream_t stream);
+
+/*
+ * The walk through a verified tree: target [T][V] (f32, or bf16 when probs_bf16) holds the
+ * target's probabilities behind every node, tokens int32 [T] the nodes' tokens (node 0's is not
+ * looked at), sample_u f32 [B][steps] uniform numbers in [0, 1).  From node 0 on, step s draws the lowest
+ * index whose running sum of the node's row exceeds sample_u[b][s] times the row's sum (64-bit sums;
+ * entries that are not positive finite numbers count as 0).  Where a child of the node has that
+ * token the walk goes on there (the first such child), as long as s + 1 < steps; else it ends.
+ * n_accepted int32 [B]: the drafts passed; out_tokens int32 [B][steps]: the drawn tokens (the
+ * last is no draft; -1 where a row sums to nothing), then -1; path int32 [B][steps]: the nodes that
+ * were drawn from, 0 first, then -1.  A sequence without nodes has 0 and all -1.
+ */
+DWA_API dwa_status dwa_verify_tree(const void* target, int32_t probs_bf16, const int32_t* tokens,
+                                   const int32_t* parents, const int32_t* q_start, const float* sample_u,
+                                   int64_t T, int32_t B, int32_t steps, int32_t V, int32_t* n_accepted,
+                                   int32_t* out_tokens, int32_t* path, dwa_stream_t stream);
+
+/*
+ * Moves the cached tokens of a path to where a sequence's tokens belong, in `layers` layers
+ * (ld_layer elements and ld_scale_layer scales apart): sequence b's token start[b] + path[b][i] to
+ * start[b] + i, for i = 0 .. n_accepted[b] (int32; path int32 [B][steps]), on the pages of
+ * block_table.  Paths ascend, so every token moves as it was before the call.  n_accepted below
+ * 0, or 0 with a negative path[b][0]: nothing.  A path that does not ascend, is longer than
+ * steps, or leaves the pages is reported in *status, and its sequence stays as it was.
+ */
+DWA_API dwa_status dwa_kv_keep(void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                               int32_t layers, int64_t ld_layer, int64_t ld_scale_layer, int32_t H,
+                               int32_t d, int64_t n_pages, int32_t page_size, int64_t ld_page,
+                               int64_t ld_scale_page, const int32_t* block_table, int64_t ld_table,
+                               int32_t max_pages, const int32_t* start, const int32_t* path,
+                               const int32_t* n_accepted, int32_t B, int32_t steps, int32_t* status,
+                               dwa_stream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
