@@ -130,7 +130,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dwa_paged_tree_attention": (_i32, [_c_void_p, _i64, _i32, _i32, _i64, _c_void_p, _c_void_p,
                                         _c_void_p, _c_void_p, _i32, _i64, _i32, _i64, _i64, _c_void_p,
                                         _i64, _i32, _c_void_p, _c_void_p, _i32, _i32, _c_void_p, _i32,
-                                        _f32, _c_void_p, _i64, _c_void_p, _c_void_p]),
+                                        _f32, _c_void_p, _i64, _c_void_p, ctypes.c_size_t, _c_void_p,
+                                        _c_void_p]),
+    "dwa_paged_tree_attention_workspace": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "dwa_verify_tree": (_i32, [_c_void_p, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32,
                                _i32, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "dwa_kv_keep": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64, _i32, _i32,

@@ -927,7 +927,8 @@ dwa_status paged_attention_call(const char* fn, const void* q, int64_t T, int32_
                                 const int32_t* block_table, int64_t ld_table, int32_t max_pages,
                                 const int32_t* lengths, const int32_t* q_start, int32_t B,
                                 int32_t max_q, const int64_t* tree_mask, int32_t words, float scale,
-                                void* out, int64_t out_ld, int32_t* status, dwa_stream_t stream) {
+                                void* out, int64_t out_ld, void* workspace, size_t workspace_bytes,
+                                int32_t* status, dwa_stream_t stream) {
   dwa::KvCacheView c{};
   if (dwa_status st = kv_cache_view(fn, k_cache, v_cache, k_scale, v_scale, H_kv, d, n_pages,
                                     page_size, ld_page, ld_scale_page, &c))
@@ -979,7 +980,15 @@ dwa_status paged_attention_call(const char* fn, const void* q, int64_t T, int32_
     a.tree = reinterpret_cast<const uint32_t*>(tree_mask);
     a.tree_words = 2 * words;
   }
-  cudaError_t e = dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
+  if (words > 0) {
+    const size_t need = dwa::tree_attention_workspace(a);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+      return fail(DWA_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned and have %zu bytes (got %zu)", fn, need,
+                  workspace_bytes);
+  }
+  cudaError_t e = words > 0
+                      ? dwa::launch_paged_tree_attention(a, workspace, static_cast<cudaStream_t>(stream))
+                      : dwa::launch_paged_attention(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, fn);
   return ok();
 }
@@ -1045,7 +1054,7 @@ dwa_status dwa_paged_attention(const void* q, int64_t T, int32_t H, int32_t d, i
                                int32_t* status, dwa_stream_t stream) {
   return paged_attention_call("dwa_paged_attention", q, T, H, d, q_ld, k_cache, v_cache, k_scale, v_scale, H_kv,
                               n_pages, page_size, ld_page, ld_scale_page, block_table, ld_table, max_pages,
-                              lengths, q_start, B, max_q, nullptr, 0, scale, out, out_ld, status, stream);
+                              lengths, q_start, B, max_q, nullptr, 0, scale, out, out_ld, nullptr, 0, status, stream);
 }
 
 dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
@@ -1055,14 +1064,27 @@ dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H, int32_t
                                     const int32_t* block_table, int64_t ld_table, int32_t max_pages,
                                     const int32_t* lengths, const int32_t* q_start, int32_t B,
                                     int32_t max_q, const int64_t* tree_mask, int32_t mask_words,
-                                    float scale, void* out, int64_t out_ld, int32_t* status,
-                                    dwa_stream_t stream) {
+                                    float scale, void* out, int64_t out_ld, void* workspace,
+                                    size_t workspace_bytes, int32_t* status, dwa_stream_t stream) {
   const char* fn = "dwa_paged_tree_attention";
   if (mask_words < 1 || mask_words > (1 << 20))
     return fail(DWA_ERR_INVALID_ARG, "%s: mask_words=%d must be positive (and 2^20 at most)", fn, mask_words);
   return paged_attention_call(fn, q, T, H, d, q_ld, k_cache, v_cache, k_scale, v_scale, H_kv, n_pages, page_size,
                               ld_page, ld_scale_page, block_table, ld_table, max_pages, lengths, q_start, B,
-                              max_q, tree_mask, mask_words, scale, out, out_ld, status, stream);
+                              max_q, tree_mask, mask_words, scale, out, out_ld, workspace, workspace_bytes, status,
+                              stream);
+}
+
+size_t dwa_paged_tree_attention_workspace(int32_t H, int32_t d, int32_t H_kv, int32_t page_size, int32_t max_pages,
+                                          int32_t B, int32_t max_q) {
+  if (H < 1 || H_kv < 1 || H % H_kv != 0 || d < 1 || max_pages < 0 || B < 0 || max_q < 0 || page_size < 1 ||
+      static_cast<int64_t>(max_q) * (H / H_kv) > INT32_MAX)
+    return 0;
+  dwa::PagedArgs a{};
+  a.max_pages = max_pages;
+  while ((1 << a.page_log2) < page_size) ++a.page_log2;
+  a.B = B; a.H = H; a.H_kv = H_kv; a.group = H / H_kv; a.d = d; a.max_q = max_q;
+  return dwa::tree_attention_workspace(a);
 }
 
 dwa_status dwa_verify_drafts(const void* target, const void* draft, int32_t probs_bf16,

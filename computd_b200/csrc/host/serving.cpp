@@ -22,6 +22,7 @@
 #include <exception>
 #include <sstream>
 #include <string>
+#include <tuple>
 
 #include "dwa_decode.h"
 
@@ -34,6 +35,7 @@ decltype(&dwa_verify_drafts) g_verify = nullptr;
 decltype(&dwa_kv_append) g_append = nullptr;
 decltype(&dwa_kv_keep) g_keep = nullptr;
 decltype(&dwa_paged_tree_attention) g_attend_tree = nullptr;
+decltype(&dwa_paged_tree_attention_workspace) g_tree_workspace = nullptr;
 decltype(&dwa_tree_masks) g_masks = nullptr;
 decltype(&dwa_verify_tree) g_verify_tree = nullptr;
 PyObject* g_raise = nullptr;  // raises the package's error for a status and a function's name
@@ -202,12 +204,13 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F&& body) {
   return nullptr;
 }
 
-// bind(write, read, attend, verify, append, keep, attend_tree, masks, verify_tree, raise): the entry
-// points' addresses.
+// bind(write, read, attend, verify, append, keep, attend_tree, its workspace, masks, verify_tree,
+// raise): the entry points' addresses.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[9];
+  unsigned long long a[10];
   PyObject* raise;
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &raise))
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9],
+                        &raise))
     return nullptr;
   g_write = reinterpret_cast<decltype(g_write)>(a[0]);
   g_read = reinterpret_cast<decltype(g_read)>(a[1]);
@@ -216,8 +219,9 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_append = reinterpret_cast<decltype(g_append)>(a[4]);
   g_keep = reinterpret_cast<decltype(g_keep)>(a[5]);
   g_attend_tree = reinterpret_cast<decltype(g_attend_tree)>(a[6]);
-  g_masks = reinterpret_cast<decltype(g_masks)>(a[7]);
-  g_verify_tree = reinterpret_cast<decltype(g_verify_tree)>(a[8]);
+  g_tree_workspace = reinterpret_cast<decltype(g_tree_workspace)>(a[7]);
+  g_masks = reinterpret_cast<decltype(g_masks)>(a[8]);
+  g_verify_tree = reinterpret_cast<decltype(g_verify_tree)>(a[9]);
   Py_INCREF(raise);
   Py_XDECREF(g_raise);
   g_raise = raise;
@@ -355,20 +359,32 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = o.data_ptr();
       if (T <= 1) out_ld = width;
     }
-    auto call = [&](auto entry, auto... more) {
-      return entry(q.data_ptr(), T, static_cast<int32_t>(heads), static_cast<int32_t>(c.d), T > 1 ? q_ld : width,
-                   c.k, c.v, c.k_scale, c.v_scale, static_cast<int32_t>(c.heads), c.n_pages,
-                   static_cast<int32_t>(c.page), c.ld_page, c.ld_scale,
-                   static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : max_pages,
-                   static_cast<int32_t>(max_pages), lengths, q_start, static_cast<int32_t>(B),
-                   static_cast<int32_t>(max_q), more..., static_cast<float>(scale), out, out_ld, status,
-                   c10::cuda::getCurrentCUDAStream(c.dev).stream());
+    const void* stream = c10::cuda::getCurrentCUDAStream(c.dev).stream();
+    auto call = [&](auto entry, auto tree, auto space) {
+      const auto before = std::make_tuple(
+          q.data_ptr(), T, static_cast<int32_t>(heads), static_cast<int32_t>(c.d), T > 1 ? q_ld : width, c.k, c.v,
+          c.k_scale, c.v_scale, static_cast<int32_t>(c.heads), c.n_pages, static_cast<int32_t>(c.page), c.ld_page,
+          c.ld_scale, static_cast<int32_t*>(table.data_ptr()), B > 1 ? table.stride(0) : max_pages,
+          static_cast<int32_t>(max_pages), lengths, q_start, static_cast<int32_t>(B), static_cast<int32_t>(max_q));
+      return std::apply(entry, std::tuple_cat(before, tree, std::make_tuple(static_cast<float>(scale), out, out_ld),
+                                              space, std::make_tuple(status, const_cast<void*>(stream))));
     };
     PyObject* ok;
-    if constexpr (kTree)
-      ok = finish(call(g_attend_tree, mask, static_cast<int32_t>(words)), "dwa_paged_tree_attention");
-    else
-      ok = finish(call(g_attend), "dwa_paged_attention");
+    if constexpr (kTree) {
+      const size_t bytes =
+          T > 0 && max_q > 0 ? g_tree_workspace(static_cast<int32_t>(heads), static_cast<int32_t>(c.d),
+                                                static_cast<int32_t>(c.heads), static_cast<int32_t>(c.page),
+                                                static_cast<int32_t>(max_pages), static_cast<int32_t>(B),
+                                                static_cast<int32_t>(max_q))
+                             : 0;
+      at::Tensor held;  // freed in the stream's order
+      if (bytes > 0) held = fresh({static_cast<int64_t>(bytes)}, at::kByte, c.dev);
+      ok = finish(call(g_attend_tree, std::make_tuple(mask, static_cast<int32_t>(words)),
+                       std::make_tuple(bytes > 0 ? held.data_ptr() : nullptr, bytes)),
+                  "dwa_paged_tree_attention");
+    } else {
+      ok = finish(call(g_attend, std::tuple<>(), std::tuple<>()), "dwa_paged_attention");
+    }
     if (ok == nullptr) return nullptr;
     Py_DECREF(ok);
     if (a[10] == Py_None) return wrap(made);

@@ -42,9 +42,6 @@ namespace dwa {
 namespace {
 
 constexpr int kMaxCluster = 8;
-// Rows per key/value head that this kernel takes; more go to the tcgen05 kernel.  At 20
-// rows (16 sequences of 4096, 8 heads of 128, bf16) that one takes 58 us, this one (in two passes) 165.
-constexpr int kFewRows = 16;
 
 template <bool kF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -843,7 +840,14 @@ cudaError_t launch_few_rows(const PagedArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream) {
   if (static_cast<int64_t>(a.max_q) * a.group > kFewRows) return launch_paged_attention_mma(a, stream);
-  return a.tree != nullptr ? launch_few_rows<true>(a, stream) : launch_few_rows<false>(a, stream);
+  return launch_few_rows<false>(a, stream);
+}
+
+cudaError_t launch_paged_tree_attention(const PagedArgs& a, void* workspace, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
+  return rows <= kFewRows    ? launch_few_rows<true>(a, stream)
+         : rows <= kTreeRows ? launch_tree_attention(a, workspace, stream)
+                             : launch_paged_attention_mma(a, stream);
 }
 
 }  // namespace dwa

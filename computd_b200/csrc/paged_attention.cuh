@@ -1,6 +1,6 @@
-// paged_attention.cuh — what the two kernels of the attention over the paged
+// paged_attention.cuh — what the kernels of the attention over the paged
 // cache share (paged_attention.cu: few rows per key/value head;
-// paged_attention_mma.cu: many).
+// paged_attention_mma.cu: many; tree_attention.cu: many of a tree's nodes).
 #pragma once
 
 #include <atomic>
@@ -35,6 +35,13 @@ struct PagedArgs {
   const uint32_t* tree;
   int tree_words;
 };
+
+// Rows per key/value head that paged_attention.cu takes; more go to a tcgen05 kernel.  At 20
+// rows (16 sequences of 4096, 8 heads of 128, bf16) that one (paged_attention_mma.cu) takes 58 us, this one (in two passes) 165.
+constexpr int kFewRows = 16;
+
+// Rows that tree_attention.cu takes.
+constexpr int kTreeRows = 32;
 
 // One sequence as the device finds it.
 struct PagedSeq {
@@ -116,7 +123,7 @@ __device__ __forceinline__ uint32_t tree_bits(const PagedArgs& a, int64_t row, i
 // Whether that token sees a node whose value is not finite: in channel ch of a bf16 cache, of an
 // e4m3 one at all.  (Only where a block met such a value.)
 template <bool kE4m3>
-__device__ __noinline__ bool tree_sees_bad(const PagedArgs& a, const PagedSeq& s, const int32_t* table, int hk,
+__device__ __noinline__ bool tree_sees_bad(const PagedArgs& a, const PagedSeq s, const int32_t* table, int hk,
                                            int64_t row, int ch) {
   const int prefix = tree_prefix(s);
   for (int node = max(-prefix, 0); node < s.n; ++node) {

@@ -1,0 +1,1368 @@
+// tree_attention.cu — attention of a tree's nodes over the paged cache on tcgen05, for
+// more rows per key/value head than paged_attention.cu takes.
+//
+// A row is one (node, query head of the group), node-major.  A unit is up to N (32, 64 or 128) rows of one
+// key/value head; it goes over the sequence's keys 128 at a time, its products transposed:
+//
+//   S^T = K Q^T       128 keys by N rows     tcgen05, K and Q in shared memory, S in TMEM
+//   P   = exp2(S - a) a thread per key and 16 or 32 rows
+//   O^T += V^T P      128 channels by N rows tcgen05, V and P in shared memory, O in TMEM
+//
+// so that neither the tensor pipe nor the exponentials work on rows that are not there: a tile
+// of 128 rows would be 50 to 87 % empty for a tree of 16 to 64 nodes.  A key's scales
+// (e4m3) are one number of its thread's.
+//
+// What a row's weights are relative to, a, is not its maximum but anything that keeps them in
+// range; it moves when a score passes the limit, which every step asks by a vote, and only
+// then are maxima taken across keys.  The limit is 2^60 for bf16 (whose range is f32's) and for e4m3
+// what keeps a weight times its value's scale below 2^15 in fp16.
+//
+// Rounding: bf16 caches none beside f32 sums (P is the sum of two bf16 parts).  e4m3: codes are
+// exact; Q is, per row, a power of two times the sum of two e4m3 numbers, exactly down to 2^-9 of the
+// row's largest value and to 2^-18 of that below (so that keys go into their product as they lie in the
+// cache, at twice the rate of fp16 and without a conversion); P times the value's scale is
+// rounded to fp16, 11 bits.
+//
+// Bound by HBM up to 64 rows, by the softmax's issue slots and the conversion of the values beyond.
+// Work is cut by steps, not by units, where sequences are long: each block takes an equal share of
+// all steps, whatever sequence they belong to, and writes a unit that it has only a part of to
+// a workspace, from which a second kernel joins the parts in a fixed order.
+//
+// Sixteen warps: softmax (four to a scheduler: with eight, each its 64 columns, a step's chain of TMEM
+// loads, exponentials and stores was twice as long).  One warp: tcgen05.mma.  Two: TMA, straight from the pages.  Two
+// look over the values of the tree's nodes (bf16), since 0 * NaN would reach rows that must not see
+// it, or turn the values' codes into fp16 (e4m3).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "dwa_internal.h"
+#include "f32x2.cuh"
+#include "paged_attention.cuh"
+#include "sm100_ptx.cuh"
+
+namespace dwa {
+
+namespace {
+
+constexpr int kTile = 128;        // keys per step
+constexpr int kBlock = kTile * 128;  // bytes of 128 rows of 128 bytes
+constexpr int kLeastShare = 8;    // of a block, in steps
+// What a unit costs beside its steps: Q, first references and the way out.  Work is shared out in
+// steps and these, so that short sequences' units do not pile up in a few blocks (24 ragged ones of 50 to 1500 tokens,
+// 16 heads of 80: 112 us without).
+constexpr int kUnitCost = 4;
+constexpr int kSmemLimit = 227 * 1024;
+
+template <bool kE4m3, int DP, int N>
+struct TreeCfg {
+  static constexpr int kThreads = 640, kSoftmax = 512, kSoftmaxRegs = 104, kOtherRegs = 64;
+  // Four warpgroups: up to 64 columns two for each of alternate tiles of keys; what shares a tile
+  // shares out its columns.
+  static constexpr bool kSplit = N <= 64;
+  static constexpr int kSharers = kSplit ? 2 : 4;
+  static constexpr int kChunks = N / 16 / kSharers;            // sixteens of columns of a warpgroup
+  static constexpr int kHalves = DP / 64;
+  static constexpr int kQPart = N * 128;                       // 64 bf16 channels, or 128 codes
+  static constexpr int kQBytes = (kE4m3 ? 2 : kHalves) * kQPart;
+  // bf16: both parts of P side by side, as columns of one product; of 128 columns one part
+  static constexpr bool kTwoParts = !kE4m3 && kSplit;
+  static constexpr int kPCols = (kTwoParts ? 2 : 1) * N;
+  static constexpr int kPBytes = (kPCols + 63) / 64 * kBlock;  // of a buffer
+  static constexpr int kPBufs = kSplit ? 2 : 1;
+  static constexpr int kKBytes = (kE4m3 ? 1 : kHalves) * kBlock;
+  // Codes of values arrive where their fp16 values go (128 channels: the second block), or behind it.
+  static constexpr int kRawAt = kBlock;
+  static constexpr int kVBytes = kHalves * kBlock + (kE4m3 && DP == 64 ? kTile * 64 : 0);
+  static constexpr int kStatic = 3072;  // at most
+  // e4m3: scales of the keys and values of eight tiles: keys are up to kKStages + 2 tiles ahead of the softmax
+  static constexpr int kScaleBytes = kE4m3 ? 2 * kTile * 4 : 0, kScaleSlots = 8;
+  static constexpr int kLeft = kSmemLimit - 1024 - kStatic - kQBytes - kPBufs * kPBytes - kScaleSlots * kScaleBytes;
+  static constexpr bool fits(int k, int v) { return k * kKBytes + v * kVBytes <= kLeft; }
+  // Scores run two tiles ahead, so that a tile of values is held longer than one of keys.
+  static constexpr int kVStages = fits(2, 4) ? 4 : fits(2, 3) ? 3 : 2;
+  static constexpr int kKStages = fits(4, kVStages) ? 4 : fits(3, kVStages) ? 3 : 2;
+  static_assert(fits(kKStages, kVStages) && kKStages + 2 < kScaleSlots, "tiles fit");
+  static constexpr int kKAt = kQBytes, kVAt = kKAt + kKStages * kKBytes, kPAt = kVAt + kVStages * kVBytes;
+  static constexpr int kScalesAt = kPAt + kPBufs * kPBytes;
+  static constexpr int kSmem = 1024 + kScalesAt + kScaleSlots * kScaleBytes;
+  // TMEM: two S, then O of each P buffer
+  static constexpr int kColsUsed = 2 * N + kPBufs * kPCols;
+  static constexpr int kTmemCols = kColsUsed > 256 ? 512 : kColsUsed > 128 ? 256 : 128;
+};
+
+// ---------------------------------------------------------------- work
+struct Part {
+  int hk, rb;          // key/value head, block of rows
+  int tile0, n, steps; // its tiles of 128 keys (n = 0: nothing to read) of the unit's `steps`
+  int64_t row0;        // the sequence, as PagedSeq has it, and its pages
+  int seq_n, length;
+  int64_t table;
+  bool bad, whole, last;  // last: there is no such part, the block is done
+};
+
+struct Plan {       // of a block
+  int64_t g, end;   // cost, counted over all units: of each kUnitCost, then its steps
+  int b;            // the sequence of cost g, and the cost before it
+  int64_t base;
+  int64_t total, share;
+};
+
+// Tiles and blocks of rows of a sequence.  (One step for rows that see no key, or get NaN.)
+__device__ __forceinline__ int64_t tree_steps(const PagedSeq& s) {
+  return s.n == 0 ? 0 : s.bad ? 1 : max((s.length + kTile - 1) / kTile, 1);
+}
+template <int N>
+__device__ __forceinline__ int64_t tree_blocks(const PagedArgs& a, const PagedSeq& s) {
+  return (static_cast<int64_t>(s.n) * a.group + N - 1) / N;
+}
+
+// Block c's share of `blocks` blocks', found by the block together; `scratch` is shared memory.
+constexpr int kPlanScratch = 32 + 3;  // 64-bit words
+template <int N, int kThreads>
+__device__ __forceinline__ Plan make_plan(const PagedArgs& a, int c, int blocks, int64_t* scratch) {
+  int64_t* const warp_sums = scratch;
+  unsigned long long& all = reinterpret_cast<unsigned long long&>(scratch[32]);
+  int64_t &found_base = scratch[33], &found_b = scratch[34];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto steps_of = [&](int b) -> int64_t {
+    if (b >= a.B) return 0;
+    const PagedSeq s = paged_seq(a, b);
+    return s.n == 0 ? 0 : (kUnitCost + tree_steps(s)) * tree_blocks<N>(a, s) * a.H_kv;
+  };
+  if (threadIdx.x == 0) {
+    all = 0;
+    found_b = a.B;
+    found_base = 0;
+  }
+  __syncthreads();
+  int64_t mine = 0;
+  const int64_t first = steps_of(threadIdx.x);
+  mine = first;
+  for (int b = threadIdx.x + kThreads; b < a.B; b += kThreads) mine += steps_of(b);
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
+  if (lane == 0 && mine) atomicAdd(&all, static_cast<unsigned long long>(mine));
+  __syncthreads();
+  Plan p;
+  p.total = static_cast<int64_t>(all);
+  p.share = max((p.total + blocks - 1) / blocks, static_cast<int64_t>(kLeastShare));
+  p.g = min(c * p.share, p.total);
+  p.end = min(p.g + p.share, p.total);
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {  // the sequence that has step g
+    const int b = b0 + threadIdx.x;
+    const int64_t w = b0 == 0 ? first : steps_of(b);
+    int64_t incl = w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    int64_t base = before, sum = 0;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) base += warp_sums[i];
+      sum += warp_sums[i];
+    }
+    base += incl - w;
+    if (b < a.B && p.g >= base && p.g < base + w) {
+      found_b = b;
+      found_base = base;
+    }
+    before += sum;
+    __syncthreads();
+    if (p.g < before) break;
+  }
+  p.b = static_cast<int>(found_b);
+  p.base = found_base;
+  return p;
+}
+
+__device__ __forceinline__ void set_seq(Part& p, const PagedArgs& a, int b, const PagedSeq& s) {
+  p.row0 = s.row0;
+  p.seq_n = s.n;
+  p.length = s.length;
+  p.bad = s.bad;
+  p.table = static_cast<int64_t>(b) * a.ld_table;
+}
+// The next part of the block's share, if there is one; *of_unit: where in its unit's cost the share, or
+// the unit, begins.
+template <int N>
+__device__ __forceinline__ bool next_part(const PagedArgs& a, Plan& w, Part& p, int64_t* of_unit) {
+  while (w.g < w.end) {
+    PagedSeq seq;
+    int64_t steps, blocks;
+    while (true) {
+      seq = paged_seq(a, w.b);
+      steps = tree_steps(seq);
+      blocks = tree_blocks<N>(a, seq);
+      const int64_t all = seq.n == 0 ? 0 : (kUnitCost + steps) * blocks * a.H_kv;
+      if (w.g - w.base < all) break;
+      w.base += all;
+      ++w.b;
+    }
+    const int64_t local = w.g - w.base, cost = kUnitCost + steps;
+    int64_t unit;
+    if (local >> 32) unit = local / cost;
+    else unit = static_cast<uint32_t>(local) / static_cast<uint32_t>(cost);  // cost: below 2^24
+    const int64_t from = local - unit * cost, to = min(cost, from + (w.end - w.g));
+    w.g += to - from;
+    const int64_t tile0 = max(from - kUnitCost, int64_t{0}), tile1 = max(to - kUnitCost, int64_t{0});
+    if (tile1 == tile0) continue;  // the next block begins it
+    set_seq(p, a, w.b, seq);
+    p.hk = (unit | blocks) >> 32 ? static_cast<int>(unit / blocks)
+                                 : static_cast<int>(static_cast<uint32_t>(unit) / static_cast<uint32_t>(blocks));
+    p.rb = static_cast<int>(unit - p.hk * blocks);
+    p.tile0 = static_cast<int>(tile0);
+    p.steps = static_cast<int>(steps);
+    p.n = seq.bad || seq.length == 0 ? 0 : static_cast<int>(tile1 - tile0);
+    p.whole = tile1 - tile0 == steps;
+    p.last = false;
+    *of_unit = from;
+    return true;
+  }
+  return false;
+}
+
+// ---------------------------------------------------------------- tcgen05 pieces
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// D[tmem] (+)= A[smem] B[smem]^T, by the elected lane of a converged warp
+template <bool kF8>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add,
+                                       uint32_t one) {
+  if constexpr (kF8)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t one) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Uses of the registers stay behind it.
+__device__ __forceinline__ void tmem_wait_x16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+
+// 16 keys of an operand whose other axis lies along rows of 128 bytes (64 16-bit elements, the
+// next 64 kBlock on), a key to a row, 128-byte swizzle.
+__device__ __forceinline__ uint64_t by_key_desc(uint32_t addr) {
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  desc |= static_cast<uint64_t>((kBlock >> 4) & 0x3FFFu) << 16;  // LBO: 64 elements on
+  desc |= static_cast<uint64_t>(1024u >> 4) << 32;               // SBO: 8 keys on
+  desc |= static_cast<uint64_t>(1u) << 46;
+  desc |= static_cast<uint64_t>(2u) << 61;
+  return desc;
+}
+
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A bounded wait of a whole converged warp, which goes on or gives up together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status, volatile int* abort_flag) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  if (__all_sync(kAll, mbar_test(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    if (__all_sync(kAll, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(kAll, *abort_flag != 0)) return false;
+    if (__any_sync(kAll, globaltimer_ns() - t0 > kWaitLimitNs)) {
+      if (status) atomicCAS(status, 0, kStatusTimeout);
+      *abort_flag = 1;
+      __syncwarp();
+      return false;
+    }
+  }
+}
+// The same for two at once.
+__device__ __forceinline__ bool warp_wait2(uint32_t x, uint32_t parity_x, uint32_t y, uint32_t parity_y, int* status,
+                                           volatile int* abort_flag) {
+  if (__all_sync(0xFFFFFFFFu, mbar_test(x, parity_x) & mbar_test(y, parity_y))) return true;
+  return warp_wait(x, parity_x, status, abort_flag) && warp_wait(y, parity_y, status, abort_flag);
+}
+// The kThreads threads of a named barrier together; whether any asks.
+template <int kThreads>
+__device__ __forceinline__ bool group_any(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x)), "r"(id), "n"(kThreads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void group_sync(int id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Numbers by the order of signed integers (NaN above, or below, all).
+__device__ __forceinline__ int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7FFFFFFF)); }
+
+// Sixteen columns' values of 32 lanes summed over the lanes: lane l gets column l / 2's.
+__device__ __forceinline__ float sum16(float (&v)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 8, o = 16; w >= 1; w >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int k = 0; k < w; ++k) {
+      const float send = up ? v[k] : v[k + w], keep = up ? v[k + w] : v[k];
+      v[k] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+    }
+  }
+  return v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 1);
+}
+// The largest of a warp's numbers (NaN counts for nothing).
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------- the kernel
+template <bool kE4m3, int N>
+struct TreeShared {
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], part_full[4], part_empty[4];
+  uint64_t scales_full[kE4m3 ? 8 : 1];
+  uint64_t q_ready, s_ready[2], s_free[2], p_ready[2], p_free[2];
+  uint32_t tmem;
+  int abort;
+  Part parts[4];                // under way, by their number
+  int bad_page[8], any_bad[8];
+  alignas(16) float neg_a[N <= 64 ? 2 * N : N];  // minus what a column's weights are relative to (of each side)
+  alignas(16) float f[kE4m3 ? N : 4];     // its scores' factor, to log2 units
+  int most[N <= 64 ? 2 * N : N];  // across keys, ordered
+  int row[N];                   // of q
+  uint32_t tops[4][4];          // e4m3: scales' exponents
+  float shift[2];               // of each side
+};
+
+struct TreeArgs {
+  PagedArgs p;
+  float* parts;   // null: every block has whole units
+  int row_units;  // blocks of rows of a sequence, at most (without parts)
+};
+
+// A part's place in the workspace: a, l and O's power of two by rows, then O.
+template <int DP, int N>
+__device__ __forceinline__ float* part_at(float* parts, int block, bool begins) {
+  return parts + (static_cast<int64_t>(block) * 2 + (begins ? 1 : 0)) * (N * (DP + 3));
+}
+
+template <bool kE4m3, int DP, int N>
+__global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          const __grid_constant__ TreeArgs ta) {
+  using C = TreeCfg<kE4m3, DP, N>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ TreeShared<kE4m3, N> sh;
+  static_assert(sizeof(TreeShared<kE4m3, N>) <= C::kStatic, "as much as is left for it");
+  const PagedArgs& a = ta.p;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kMma = C::kSoftmax / 32, kTma = kMma + 1, kPlanner = kMma + 3;  // warps; two for TMA
+
+  // ------------------------------------------------ the block's work
+  Plan plan{};
+  if (ta.parts != nullptr) {
+    plan = make_plan<N, C::kThreads>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem));
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b < a.B; b += C::kThreads)
+        if (paged_seq(a, b).bad) paged_report(a.status);
+    if (plan.g >= plan.end) return;
+  }
+
+  // ------------------------------------------------ set-up
+  auto bar = [&](const uint64_t& x) { return smem_u32(&x); };
+  if (warp == kPlanner && lane == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(sh.k_full[i]), 1);
+      mbar_init(bar(sh.k_empty[i]), 1);
+      mbar_init(bar(sh.v_full[i]), 1);
+      mbar_init(bar(sh.part_full[i]), 1);
+      mbar_init(bar(sh.part_empty[i]), kPlanner);  // a warp each
+      mbar_init(bar(sh.v_empty[i]), 1);
+    }
+    for (int i = 0; i < 8; ++i) sh.bad_page[i] = sh.any_bad[i] = 0;
+    for (int i = 0; i < (kE4m3 ? 8 : 1); ++i) mbar_init(bar(sh.scales_full[i]), 1);
+    mbar_init(bar(sh.q_ready), C::kSoftmax / 32);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(sh.s_ready[i]), 1);
+      mbar_init(bar(sh.s_free[i]), 4 * C::kSharers);
+      mbar_init(bar(sh.p_ready[i]), 4 * C::kSharers);
+      mbar_init(bar(sh.p_free[i]), 1);
+    }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMma) {
+    tmem_alloc(smem_u32(&sh.tmem), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm_s = sh.tmem, tm_o = sh.tmem + 2 * N;  // S: + N (it & 1); O: + kPCols (P's buffer)
+  // the buffer of P and O that tile `it` goes through, and which use of it that is
+  auto p_buf = [](int it) -> int { return C::kSplit ? it & 1 : 0; };
+  auto p_use = [](int it) -> int { return C::kSplit ? it >> 1 : it; };
+  int* const status = a.status;
+  volatile int* const abort_flag = &sh.abort;
+  auto wait = [&](const uint64_t& x, int phase) -> bool {
+    return warp_wait(bar(x), phase & 1, status, abort_flag);
+  };
+  auto wait2 = [&](const uint64_t& x, int phase_x, const uint64_t& y, int phase_y) -> bool {
+    return warp_wait2(bar(x), phase_x & 1, bar(y), phase_y & 1, status, abort_flag);
+  };
+  auto warp_arrive = [&](const uint64_t& x) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(x));
+  };
+  const uint32_t s_k = base + C::kKAt, s_v = base + C::kVAt, s_p = base + C::kPAt;
+  auto rows_of = [&](int seq_n, int rb) -> int {  // of the unit
+    return static_cast<int>(min(static_cast<int64_t>(seq_n) * a.group - static_cast<int64_t>(rb) * N,
+                                static_cast<int64_t>(N)));
+  };
+
+  if (warp >= kMma) {
+    regs_dec<C::kOtherRegs>();
+    if (warp == kPlanner) {
+      // ---------------------------------------------- the parts, a few ahead
+      Plan w = plan;
+      for (int part = 0;; ++part) {
+        Part p{};
+        if (ta.parts != nullptr) {
+          int64_t at;
+          p.last = !next_part<N>(a, w, p, &at);
+        } else {  // one unit: (sequence, head, block of rows)
+          const uint32_t unit = blockIdx.x, of_seq = unit / static_cast<uint32_t>(ta.row_units);
+          const int b = static_cast<int>(of_seq / static_cast<uint32_t>(a.H_kv));
+          const PagedSeq seq = paged_seq(a, b);
+          set_seq(p, a, b, seq);
+          p.rb = static_cast<int>(unit - of_seq * ta.row_units);
+          p.hk = static_cast<int>(of_seq - static_cast<uint32_t>(b) * a.H_kv);
+          p.steps = static_cast<int>(tree_steps(seq));
+          p.n = seq.bad || seq.length == 0 ? 0 : p.steps;
+          p.whole = true;
+          p.last = part > 0 || !(p.rb < tree_blocks<N>(a, seq) || (seq.bad && p.rb == 0));
+        }
+        if (part >= 4 && !wait(sh.part_empty[part & 3], (part >> 2) - 1)) break;
+        if (lane == 0) {
+          sh.parts[part & 3] = p;
+          mbar_arrive(bar(sh.part_full[part & 3]));
+        }
+        __syncwarp();
+        if (p.last) break;
+      }
+    } else if (warp != kMma) {
+      // ---------------------------------------------- TMA: a warp for keys, one for values
+      const bool values = warp == kTma + 1;
+      const int stages = values ? C::kVStages : C::kKStages, stage_bytes = values ? C::kVBytes : C::kKBytes;
+      const uint32_t tiles = values ? s_v + (kE4m3 ? C::kRawAt : 0) : s_k;
+      const uint32_t full0 = values ? bar(sh.v_full[0]) : bar(sh.k_full[0]);
+      const uint32_t empty0 = values ? bar(sh.v_empty[0]) : bar(sh.k_empty[0]);
+      const CUtensorMap* map = values ? &map_v : &map_k;
+      const int row_bytes = values && kE4m3 ? DP : 128;
+      const int page_size = 1 << a.page_log2, of_tile = kTile >> a.page_log2;  // pages of a tile: 1 to 8
+      int stage = 0, use = 0, slot = 0;
+      bool ok = true;
+      for (int part = 0; ok && (ok = wait(sh.part_full[part & 3], part >> 2)); ++part) {
+        const Part& p = sh.parts[part & 3];
+        if (p.last) break;
+        const int32_t* table = a.table + p.table;
+        const int n = p.n, hk = p.hk, page0 = p.tile0 * of_tile;
+        const int pages = (p.length + page_size - 1) >> a.page_log2;
+        warp_arrive(sh.part_empty[part & 3]);
+        int held = 0;  // the pages of the next 4 to 32 tiles, a page to a lane
+        for (int j = 0; j < n; ++j) {
+          const int at = (j * of_tile) & 31;
+          if (at == 0) {
+            const int i = page0 + j * of_tile + lane;
+            held = i < pages ? __ldg(table + i) : 0;
+            if (held < 0 || held >= a.n_pages) {
+              if (i < page0 + n * of_tile) sh.bad_page[part & 7] = 1;  // read page 0 in its place; the rows become NaN
+              held = 0;
+            }
+          }
+          const int here = min(of_tile, pages - page0 - j * of_tile);
+          const uint32_t full = full0 + 8 * stage;
+          if (use > 0 && !(ok = warp_wait(empty0 + 8 * stage, (use - 1) & 1, status, abort_flag))) break;
+          // Both tiles' scales come with the keys.  (Their slot has been read: see kScaleSlots.)
+          const bool scales = kE4m3 && !values;
+          const uint32_t slot_full = bar(sh.scales_full[kE4m3 ? slot : 0]);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full, static_cast<uint32_t>(here * page_size * row_bytes) * (kE4m3 ? 1 : C::kHalves));
+            if (scales) mbar_arrive_expect_tx(slot_full, static_cast<uint32_t>(here * page_size) * 8);
+          }
+          __syncwarp();
+          uint32_t dst = tiles + stage * stage_bytes;
+          for (int q = 0; q < here; ++q, dst += page_size * row_bytes) {
+            const int page = __shfl_sync(0xFFFFFFFFu, held, at + q);
+            if (lane == 0) {
+#pragma unroll
+              for (int h = 0; h < (kE4m3 ? 1 : C::kHalves); ++h)
+                tma_load_page(dst + h * kBlock, map, full, 64 * h, 0, 0, hk, page);
+              if (scales) {
+                const int64_t from = page * a.ld_scale_page + (static_cast<int64_t>(hk) << a.page_log2);
+                const uint32_t to = base + C::kScalesAt + slot * C::kScaleBytes + q * page_size * 4;
+                bulk_load(to, a.k_scale + from, page_size * 4, slot_full);
+                bulk_load(to + kTile * 4, a.v_scale + from, page_size * 4, slot_full);
+              }
+            }
+          }
+          slot = (slot + 1) % C::kScaleSlots;
+          if (++stage == stages) {
+            stage = 0;
+            ++use;
+          }
+        }
+      }
+      // after an abort nobody else waits for the copies in flight
+      if (*abort_flag) {
+        for (int i = 0; i < stages && (use > 0 || stage > 0); ++i) {
+          if (--stage < 0) {
+            stage = stages - 1;
+            --use;
+          }
+          mbar_wait(full0 + 8 * stage, use & 1, status, nullptr);
+          if (kE4m3 && !values) {  // the same tile's scales
+            slot = (slot + C::kScaleSlots - 1) % C::kScaleSlots;
+            mbar_wait(bar(sh.scales_full[kE4m3 ? slot : 0]), ((use * stages + stage) / C::kScaleSlots) & 1, status, nullptr);
+          }
+        }
+      }
+    } else {
+      // ---------------------------------------------- tcgen05.mma
+      constexpr uint32_t kM = kTile / 16 << 24;
+      constexpr uint32_t kF16 = kE4m3 ? 0u : (1u << 7) | (1u << 10);  // fp16 or bf16
+      const int k_steps = kE4m3 ? (a.d + 31) / 32 : a.d / 16;
+      const uint32_t one = elect_one();
+      // Only a descriptor's start address changes: its low word by constants, so that the one issuing
+      // lane spends a few instructions per product.
+      const uint32_t k_hi = static_cast<uint32_t>(sw128_kmajor_desc(0) >> 32), k_lo = static_cast<uint32_t>(sw128_kmajor_desc(0));
+      const uint32_t v_hi = static_cast<uint32_t>(by_key_desc(0) >> 32), v_lo = static_cast<uint32_t>(by_key_desc(0));
+      auto desc = [](uint32_t lo, uint32_t hi) -> uint64_t {
+        uint64_t r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+        return r;
+      };
+      auto addr = [](uint32_t x) -> uint32_t { return (x >> 4) & 0x3FFFu; };
+      const bool full_d = a.d == DP;
+      int it = 0, parts = 0;
+      bool ok = true;
+      for (int part = 0; ok && (ok = wait(sh.part_full[part & 3], part >> 2)); ++part) {
+        const Part& p = sh.parts[part & 3];
+        if (p.last) break;
+        const int n = p.n;
+        const uint32_t cols = static_cast<uint32_t>((rows_of(p.seq_n, p.rb) + 15) & ~15);
+        warp_arrive(sh.part_empty[part & 3]);
+        if (n == 0) continue;
+        const uint32_t idesc_s = (1u << 4) | kF16 | (cols / 8 << 17) | kM;
+        const uint32_t idesc_o = (1u << 4) | kF16 | (1u << 15) | (1u << 16) | ((C::kPCols - N + cols) / 8 << 17) | kM;
+        ok = wait(sh.q_ready, parts++);
+        auto scores = [&](int i) -> bool {  // S = K_i Q^T
+          const int ks = i % C::kKStages;
+          const bool again = i >= 2;  // S has been used before
+          if (!wait2(sh.k_full[ks], i / C::kKStages, again ? sh.s_free[i & 1] : sh.k_full[ks],
+                     again ? (i >> 1) - 1 : i / C::kKStages))
+            return false;
+          tc_fence_after();
+          const uint32_t d = tm_s + N * (i & 1);
+          const uint32_t kt = k_lo + addr(s_k + ks * C::kKBytes), qt = k_lo + addr(base);
+          auto step = [&](int s) {
+            if constexpr (kE4m3) {
+              mma_ss<true>(d, desc(kt + 2 * s, k_hi), desc(qt + 2 * s, k_hi), idesc_s, s > 0, one);
+              mma_ss<true>(d, desc(kt + 2 * s, k_hi), desc(qt + C::kQPart / 16 + 2 * s, k_hi), idesc_s, 1, one);
+            } else {
+              mma_ss<false>(d, desc(kt + ((s >> 2) * kBlock + (s & 3) * 32) / 16, k_hi),
+                            desc(qt + ((s >> 2) * C::kQPart + (s & 3) * 32) / 16, k_hi), idesc_s, s > 0, one);
+            }
+          };
+          if (full_d) {
+#pragma unroll
+            for (int s = 0; s < DP / (kE4m3 ? 32 : 16); ++s) step(s);
+          } else {
+#pragma unroll 1
+            for (int s = 0; s < k_steps; ++s) step(s);
+          }
+          commit(bar(sh.s_ready[i & 1]), one);
+          commit(bar(sh.k_empty[ks]), one);
+          return true;
+        };
+        // Scores two tiles ahead: a warpgroup finds its next ones when it has written its weights.
+        const int first = it;
+        if (ok) ok = scores(it);
+        if (ok && n > 1) ok = scores(it + 1);
+        for (int j = 0; j < n && ok; ++j, ++it) {
+          // the tile after next goes where this one's scores have been read
+          if (j + 2 < n && !(ok = scores(first + j + 2))) break;
+          const int vs = it % C::kVStages, buf = p_buf(it);
+          // (values have been waited for, and made ready, by those who wrote the weights)
+          if (!(ok = wait(sh.p_ready[buf], p_use(it)))) break;
+          tc_fence_after();
+          const uint32_t vt = v_lo + addr(s_v + vs * C::kVBytes), pt = v_lo + addr(s_p + C::kPBytes * buf);
+#pragma unroll
+          for (int s = 0; s < kTile / 16; ++s)
+            mma_ss<false>(tm_o + C::kPCols * buf, desc(vt + 128 * s, v_hi), desc(pt + 128 * s, v_hi), idesc_o,
+                          j >= C::kPBufs || s > 0, one);
+          commit(bar(sh.p_free[buf]), one);
+          commit(bar(sh.v_empty[vs]), one);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    regs_inc<C::kSoftmaxRegs>();
+    const int wg = warp >> 2, quad = warp & 3, t = threadIdx.x & 127;
+    const int group_bar = 1 + wg, side = C::kSplit ? wg >> 1 : 0, sharer = wg % C::kSharers;  // side: of the tiles
+    const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+    auto all_sync = [&]() { asm volatile("barrier.cta.sync 5, 512;" ::: "memory"); };
+    auto chunk_of = [&](int i) { return C::kSharers * i + sharer; };  // sixteens of columns
+    // this warpgroup's columns, i < 16 kChunks
+    auto column = [&](int i) { return 16 * chunk_of(i >> 4) + (i & 15); };
+    float* const neg_a = sh.neg_a + side * N;
+    int* const mosts = sh.most + side * N;
+    // columns' numbers, while nothing reads P
+    float* const sums = reinterpret_cast<float*>(smem + C::kPAt);  // [side][quad][N]: of weights
+    float* const weights = sums + 1024;                            // [side][N]: of the accumulators
+    int64_t* const places = reinterpret_cast<int64_t*>(weights + 2 * N);
+    // Where weights have to stay: e4m3 below 2^15 with their values' scales, and by themselves below
+    // 2^105, so that their sums are f32; when a moves it leaves this much room.
+    constexpr float kMost = kE4m3 ? 105.f : 60.f, kRoom = kE4m3 ? 5.f : 60.f;
+    bool alive = true;
+    auto hold = [&](const uint64_t& x, int phase) {  // after an abort nothing is waited for any more
+      if (alive) alive = wait(x, phase);
+    };
+    int it0 = 0;
+    for (int part = 0;; ++part) {
+      hold(sh.part_full[part & 3], part >> 2);
+      // together, and only behind the last part's reads of the columns' numbers; all stop, or none
+      if (group_any<C::kSoftmax>(5, !alive)) break;
+      const Part& p = sh.parts[part & 3];
+      if (p.last) break;
+      const int64_t all_rows = static_cast<int64_t>(p.seq_n) * a.group;
+      if (p.bad) {
+        if (ta.parts == nullptr && p.hk == 0 && p.rb == 0 && threadIdx.x == 0) paged_report(a.status);
+        // rows N rb .., and without parts, where max_q does not bound them, every row_units-th block
+        const int64_t by = ta.parts == nullptr ? static_cast<int64_t>(ta.row_units) * N : all_rows;
+        for (int64_t r0 = static_cast<int64_t>(p.rb) * N; r0 < all_rows; r0 += by)
+          for (int64_t i = threadIdx.x; i < min(static_cast<int64_t>(N), all_rows - r0) * a.d; i += C::kSoftmax) {
+            const int64_t row = r0 + i / a.d;
+            a.out[(p.row0 + row / a.group) * a.out_ld +
+                  (static_cast<int64_t>(p.hk) * a.group + row % a.group) * a.d + i % a.d] = 0x7FC0u;
+          }
+        warp_arrive(sh.part_empty[part & 3]);
+        continue;
+      }
+      const int n = p.n, tile0 = p.tile0, rows = rows_of(p.seq_n, p.rb), cols = (rows + 15) & ~15;
+      const int prefix = p.length - p.seq_n, vis_min = max(prefix, 0), vis_max = p.length;
+      // ---------------------------------------------- the rows of Q
+      {
+        constexpr int kPerRow = C::kSoftmax / N;  // threads
+        const int c = threadIdx.x / kPerRow, piece0 = threadIdx.x % kPerRow;
+        const uint32_t row = static_cast<uint32_t>(p.rb) * N + c;
+        const bool live = c < rows;
+        const uint32_t token = live ? row_token(row, a.group) : 0, head = live ? row - token * a.group : 0;
+        const uint16_t* src = a.q + (p.row0 + token) * a.q_ld + (static_cast<int64_t>(p.hk) * a.group + head) * a.d;
+        constexpr int kPieces = (DP / 8 + kPerRow - 1) / kPerRow;  // of 16 bytes
+        uint4 x[kPieces];
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const int piece = piece0 + k * kPerRow;
+          x[k] = make_uint4(0, 0, 0, 0);
+          if (live && 8 * piece < a.d) x[k] = __ldg(reinterpret_cast<const uint4*>(src) + piece);
+        }
+        if (piece0 == 0) {
+          sh.row[c] = static_cast<int>(p.row0 + token);
+#pragma unroll
+          for (int k = 0; k < (C::kSplit ? 2 : 1); ++k) {
+            sh.neg_a[k * N + c] = live ? INFINITY : 0.f;
+            sh.most[k * N + c] = ordered(-INFINITY);
+          }
+        }
+        if constexpr (kE4m3) {
+          uint32_t tops = 0;
+#pragma unroll
+          for (int k = 0; k < kPieces; ++k)
+            tops = __vmaxu2(__vmaxu2(tops, __vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu)),
+                            __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu));
+          uint32_t top = max(tops << 16, tops & 0xFFFF0000u);
+#pragma unroll
+          for (int o = 1; o < kPerRow; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+          // times the power of two that puts the largest magnitude in [2^7, 2^8); a row that is not
+          // finite gets NaN from its factor
+          const bool finite = top < 0x7F800000u;
+          const int e = top == 0 || !finite ? 7 : static_cast<int>(top >> 23) - 127;
+          const int m = min(7 - e, 126);
+          const float up = pow2(m);
+          if (piece0 == 0)
+            sh.f[c] = finite ? fmaxf(a.scale_log2 * pow2(-m), 0x1p-126f) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+          for (int k = 0; k < 16 / kPerRow; ++k) {  // of all 128 channels: those from d on are zeros
+            const int piece = piece0 + k * kPerRow;
+            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+            if (k < kPieces && finite) {
+              const uint4& v = x[k < kPieces ? k : 0];
+              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e2 = 0; e2 < 4; ++e2) {
+                const float y0 = __uint_as_float(u[e2] << 16) * up, y1 = __uint_as_float(u[e2] & 0xFFFF0000u) * up;
+                uint16_t h, l;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(y1), "f"(y0));
+                const uint32_t back = e4m3x2_f16x2(h, 0);
+                float b0, b1;
+                asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}"
+                    : "=f"(b0), "=f"(b1) : "r"(back));
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(l) : "f"(y1 - b1), "f"(y0 - b0));
+                hi[e2 >> 1] |= static_cast<uint32_t>(h) << (16 * (e2 & 1));
+                lo[e2 >> 1] |= static_cast<uint32_t>(l) << (16 * (e2 & 1));
+              }
+            }
+            uint8_t* dst = smem + c * 128 + (((piece >> 1) ^ (c & 7)) << 4) + 8 * (piece & 1);
+            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(dst + C::kQPart) = make_uint2(lo[0], lo[1]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < kPieces; ++k) {
+            const int piece = piece0 + k * kPerRow;
+            if (piece < DP / 8)
+              *reinterpret_cast<uint4*>(smem + (piece >> 3) * C::kQPart + c * 128 + (((piece & 7) ^ (c & 7)) << 4)) = x[k];
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      if (n > 0) warp_arrive(sh.q_ready);
+
+      uint64_t l[C::kChunks][8];  // sums of weights, in pairs of columns
+#pragma unroll
+      for (int i = 0; i < C::kChunks; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l[i][e] = 0;
+      // The tiles of this side: j0, j0 + kPBufs, ...
+      const int j0 = C::kSplit ? (side - it0) & 1 : 0;
+      float g = 1.f, shift = 0.f;  // e4m3: values' scales go times g = 2^-shift
+      all_sync();  // the columns' numbers are there
+      for (int j = j0; j < n; j += C::kPBufs) {
+        const int it = it0 + j, buf = p_buf(it);
+        const uint32_t ts = tm_s + N * (it & 1) + lanes;
+        const int key = (tile0 + j) * kTile + t;
+        const bool edge = (tile0 + j + 1) * kTile > vis_min;
+        // Which of this warp's 32 keys the columns' rows see: lane l has column l's bits.
+        uint32_t win = 0u;
+        if (edge) {
+          const int key_w = key - lane, left = vis_max - key_w;  // the warp's first key, keys from there on
+          const uint32_t valid = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1u : 0u;
+          if (lane < 16 * C::kChunks && valid) win = tree_bits(a, sh.row[column(lane)], key_w - prefix) & valid;
+        }
+        // The columns of sixteen i whose rows do not see this thread's key, as bits.
+        auto unseen = [&](int i) -> uint32_t {
+          uint32_t r = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r |= ((__shfl_sync(0xFFFFFFFFu, win, 16 * i + e) >> lane) & 1u) << e;
+          return ~r;
+        };
+        hold(sh.s_ready[it & 1], it >> 1);
+        tc_fence_after();
+        float sk = 1.f, sv = 1.f, limit = kMost;
+        if constexpr (kE4m3) {
+          hold(sh.scales_full[it % C::kScaleSlots], it / C::kScaleSlots);
+          const float* scales = reinterpret_cast<const float*>(smem + C::kScalesAt + (it % C::kScaleSlots) * C::kScaleBytes);
+          const bool valid = key < vis_max;
+          sk = valid ? scales[t] : 0.f;
+          sv = valid ? scales[kTile + t] : 0.f;
+          if (j == j0) {
+            // g: one over a power of two near the first tile's largest scale.  (Not above 2^60: where
+            // that tile holds nothing but zeros, whose scale is 2^-126, numbers may follow.)
+            const uint32_t bits = fabsf(sv) < INFINITY ? __float_as_uint(fabsf(sv)) : 0u;
+            const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, bits);
+            if (lane == 0) sh.tops[wg][quad] = top;
+            group_sync(group_bar);
+            const uint32_t most = max(max(sh.tops[wg][0], sh.tops[wg][1]), max(sh.tops[wg][2], sh.tops[wg][3]));
+            const int e = most == 0 ? 0 : static_cast<int>(most >> 23) - 127;
+            shift = static_cast<float>(min(max(e, -60), 120));
+            g = pow2(-static_cast<int>(shift));
+          }
+          sv = fmaf(sv, 0.f, sv) * g;  // an infinity becomes NaN
+          limit = fminf(kMost, 15.f - fast_log2(fabsf(sv)));
+        }
+        // Scores relative to a, in log2 units, of one sixteen of columns; and which rows do not see the
+        // key (which may leave a score of -inf to those that do).
+        const uint64_t sk2 = pair(sk, sk), scale2 = pair(a.scale_log2, a.scale_log2);
+        // (Two sixteens of columns are fetched twice: held until the vote is over they went to the stack.)
+        float x[16];
+        uint32_t hidden = 0;
+        auto fetch = [&](int i) {
+          const int c0 = 16 * chunk_of(i);
+          uint32_t s[16];
+          tmem_ld_x16(ts + c0, s);
+          tmem_wait_x16(s);
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const ulonglong2 ref = *reinterpret_cast<const ulonglong2*>(&neg_a[c0 + e]);
+            uint64_t s01 = pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            uint64_t s23 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+            if constexpr (kE4m3) {
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sh.f[c0 + e]);
+              s01 = fma2(mul2(s01, sk2), f.x, ref.x);
+              s23 = fma2(mul2(s23, sk2), f.y, ref.y);
+            } else {
+              s01 = fma2(s01, scale2, ref.x);
+              s23 = fma2(s23, scale2, ref.y);
+            }
+            unpair(s01, x[e], x[e + 1]);
+            unpair(s23, x[e + 2], x[e + 3]);
+          }
+          hidden = 0;
+          if (edge) {
+            hidden = unseen(i);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if ((hidden >> e) & 1u) x[e] = -INFINITY;
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < C::kChunks; ++i)
+          if (16 * chunk_of(i) < cols) {
+            fetch(i);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) top = max3(top, x[e], x[e + 1]);
+          }
+        if (group_any<128>(group_bar, top > limit)) {
+          // ------------------------------------------ a moves: the columns' maxima across keys
+#pragma unroll 1
+          for (int i = 0; i < C::kChunks; ++i) {
+            const int c0 = 16 * chunk_of(i);
+            if (c0 >= cols) break;
+            uint32_t s[16];
+            tmem_ld_x16(ts + c0, s);
+            tmem_wait_x16(s);
+            const uint32_t not_seen = edge ? unseen(i) : 0u;
+            float most = -INFINITY;  // lane e: column e's
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float z = __uint_as_float(s[e]) * sk * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) - limit;
+              if ((not_seen >> e) & 1u) z = -INFINITY;
+              const float largest = warp_max(z);
+              if ((lane & 15) == e) most = largest;
+            }
+            if (lane < 16 && most == most) atomicMax(&mosts[c0 + lane], ordered(most));
+          }
+          group_sync(group_bar);
+          if (j >= C::kPBufs) {
+            hold(sh.p_free[buf], p_use(it) - 1);
+            tc_fence_after();
+#pragma unroll
+            for (int i = 0; i < C::kChunks; ++i) {
+              const int c0 = 16 * chunk_of(i);
+              if (c0 < cols) {
+                float shrink[16];
+                bool moved = false;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float was = -neg_a[c0 + e], most = from_ordered(mosts[c0 + e]);
+                  shrink[e] = most > was ? fast_exp2(was - (most + kRoom)) : 1.f;
+                  moved |= most > was;
+                }
+                if (moved) {  // the same for all threads
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) l[i][e] = mul2(l[i][e], pair(shrink[2 * e], shrink[2 * e + 1]));
+#pragma unroll 1
+                  for (int h = 0; h < C::kPCols; h += N) {
+                    uint32_t o[16];
+                    const uint32_t to = tm_o + C::kPCols * buf + lanes + h + c0;
+                    tmem_ld_x16(to, o);
+                    tmem_wait_x16(o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink[e]);
+                    tmem_st_x16(to, o);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                  }
+                }
+              }
+            }
+          }
+          group_sync(group_bar);
+          if (t < 16 * C::kChunks) {
+            const int c = column(t);
+            const float most = from_ordered(mosts[c]);
+            if (most > -neg_a[c]) neg_a[c] = -(most + kRoom);
+            mosts[c] = ordered(-INFINITY);
+          }
+          group_sync(group_bar);
+          if constexpr (C::kChunks == 1) {
+            if (16 * chunk_of(0) < cols) fetch(0);
+          }
+        }
+        // ------------------------------------------ weights
+        if (C::kChunks == 1 || 16 * chunk_of(0) >= cols) {
+          tc_fence_before();
+          warp_arrive(sh.s_free[it & 1]);
+        }
+        if (p_use(it) > 0) hold(sh.p_free[buf], p_use(it) - 1);
+        uint8_t* const prow = smem + C::kPAt + C::kPBytes * buf + t * 128;
+        auto put = [&](int c, const uint32_t (&v)[8]) {  // at columns c .. c + 15
+          uint8_t* const block = prow + (c >> 6) * kBlock;
+          const int piece = (c & 63) >> 3;
+          *reinterpret_cast<uint4*>(block + ((piece ^ (t & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(block + (((piece + 1) ^ (t & 7)) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
+        };
+        const uint64_t sv2 = pair(sv, sv), minus = pair(-1.f, -1.f);
+#pragma unroll
+        for (int i = 0; i < C::kChunks; ++i) {
+          const int c0 = 16 * chunk_of(i);
+          if (c0 < cols) {
+            if constexpr (C::kChunks > 1) {
+              fetch(i);
+              if (i + 1 == C::kChunks || 16 * chunk_of(i + 1) >= cols) {  // this warpgroup's last
+                tc_fence_before();
+                warp_arrive(sh.s_free[it & 1]);
+              }
+            }
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint64_t w = pair(fast_exp2(x[2 * e]), fast_exp2(x[2 * e + 1]));
+              l[i][e] = add2(l[i][e], w);
+              float p0, p1;
+              if constexpr (kE4m3) {
+                w = mul2(w, sv2);
+                unpair(w, p0, p1);
+                if (edge) {  // a hidden key's scale may be anything
+                  if ((hidden >> (2 * e)) & 1u) p0 = 0.f;
+                  if ((hidden >> (2 * e + 1)) & 1u) p1 = 0.f;
+                }
+                hi[e] = pack_f16(p0, p1);
+              } else {
+                unpair(w, p0, p1);
+                hi[e] = pack_bf16(p0, p1);
+                if constexpr (C::kTwoParts) {
+                  unpair(fma2(pair(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xFFFF0000u)), minus, w), p0, p1);
+                  lo[e] = pack_bf16(p0, p1);
+                }
+              }
+            }
+            put(c0, hi);
+            if constexpr (C::kTwoParts) put(N + c0, lo);
+          }
+        }
+        // ------------------------------------------ this side's values of the tile
+        {
+          const int vs = it % C::kVStages;
+          uint8_t* const stage = smem + C::kVAt + vs * C::kVBytes;
+          const int left = vis_max - (tile0 + j) * kTile;
+          if constexpr (kE4m3) {
+            // Codes to fp16.  A warp has eight rows at a time, four lanes a row: codes 16 c .. and 64 +
+            // 16 c .. of it (c = lane & 3).  Neighbouring groups of four take rows r and r ^ 5, so that neither
+            // the reads nor the writes meet in a bank.
+            hold(sh.v_full[vs], it / C::kVStages);
+            constexpr int kPer = DP / 64, kWarps = 4 * C::kSharers, kRounds = kTile / 8 / kWarps;
+            const int c = lane & 3, pair_row = (lane >> 3) & 3, row8 = (lane & 4) ? pair_row ^ 5 : pair_row;
+            uint4 u[kRounds][kPer];
+#pragma unroll
+            for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+              for (int q = 0; q < kPer; ++q) {
+                const int r = 8 * (warp % kWarps + kWarps * k) + row8;
+                u[k][q] = *reinterpret_cast<const uint4*>(stage + C::kRawAt + r * DP +
+                                                          (((c + 4 * q) ^ (DP == 128 ? row8 : 0)) << 4));
+                if (r >= left) u[k][q] = make_uint4(0, 0, 0, 0);  // not this sequence's
+              }
+            __syncwarp();  // the rows' codes are read: their place may be written
+#pragma unroll
+            for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+              for (int q = 0; q < kPer; ++q) {
+                const uint4& v = u[k][q];
+                uint8_t* row = stage + q * kBlock + (8 * (warp % kWarps + kWarps * k) + row8) * 128;
+                *reinterpret_cast<uint4*>(row + (((2 * c) ^ row8) << 4)) =
+                    make_uint4(e4m3x2_f16x2(v.x, 0), e4m3x2_f16x2(v.x, 1), e4m3x2_f16x2(v.y, 0), e4m3x2_f16x2(v.y, 1));
+                *reinterpret_cast<uint4*>(row + (((2 * c + 1) ^ row8) << 4)) =
+                    make_uint4(e4m3x2_f16x2(v.z, 0), e4m3x2_f16x2(v.z, 1), e4m3x2_f16x2(v.w, 0), e4m3x2_f16x2(v.w, 1));
+              }
+          } else {
+            hold(sh.v_full[vs], it / C::kVStages);
+            if (edge) {  // values that not every row sees: 0 * NaN would reach rows that must not see it
+              const int pc = lane & 7, r_of = 4 * (warp % (4 * C::kSharers)) + (lane >> 3);
+#pragma unroll 1
+              for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll 2
+                for (int r = r_of; r < kTile; r += 16 * C::kSharers) {
+                  uint4* const at = reinterpret_cast<uint4*>(stage + h * kBlock + r * 128 + pc * 16);
+                  const int of = (tile0 + j) * kTile + r;
+                  if (r >= left) {
+                    *at = make_uint4(0, 0, 0, 0);
+                  } else if (of >= vis_min) {
+                    auto finite = [](uint32_t u) -> uint32_t {
+                      if ((u & 0x7F80u) == 0x7F80u) u &= 0xFFFF0000u;
+                      if ((u & 0x7F800000u) == 0x7F800000u) u &= 0x0000FFFFu;
+                      return u;
+                    };
+                    const uint4 x = *at, y = make_uint4(finite(x.x), finite(x.y), finite(x.z), finite(x.w));
+                    if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                      *at = y;
+                      sh.any_bad[part & 7] = 1;
+                    }
+                  }
+                }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        warp_arrive(sh.p_ready[buf]);
+      }
+      // ---------------------------------------------- out
+      const int first_of = it0;
+      it0 += n;
+      // the last tile of this side, if it had any, is in O
+      if (n > j0) {
+        const int last = first_of + j0 + (n - 1 - j0) / C::kPBufs * C::kPBufs;
+        hold(sh.p_free[p_buf(last)], p_use(last));
+      }
+      tc_fence_after();
+      tc_fence_before();
+      all_sync();  // nothing reads P any more, and O is whole
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < C::kChunks; ++i)
+        if (16 * chunk_of(i) < cols) {
+          float v[16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) unpair(l[i][e], v[2 * e], v[2 * e + 1]);
+          const float sum = sum16(v);
+          if (!(lane & 1)) sums[(4 * side + quad) * N + 16 * chunk_of(i) + (lane >> 1)] = sum;
+        }
+      if (kE4m3 && sharer == 0 && t == 0) sh.shift[side] = n > j0 ? shift : -INFINITY;
+      const bool bad_page = n > 0 && sh.bad_page[part & 7], some_bad = !kE4m3 && n > 0 && sh.any_bad[part & 7];
+      if (threadIdx.x == 0 && bad_page) paged_report(a.status);
+      all_sync();
+      float* const part_to = p.whole ? nullptr : part_at<DP, N>(ta.parts, blockIdx.x, tile0 == 0);
+      const int ch = 32 * quad + lane;
+      if constexpr (kE4m3) shift = C::kSplit ? fmaxf(fmaxf(sh.shift[0], sh.shift[1]), -60.f) : fmaxf(sh.shift[0], -60.f);
+      const float back = kE4m3 ? pow2(static_cast<int>(shift)) : 1.f;
+      // is there anything in the O of P's buffers?
+      const bool have0 = C::kSplit ? n > ((0 - first_of) & 1) : n > 0, have1 = C::kSplit && n > ((1 - first_of) & 1);
+      if (threadIdx.x < cols) {  // a thread settles a column: the weights of both accumulators, the sum and the place
+        const int c = threadIdx.x;
+        auto sum_of = [&](int of) {
+          const float* x = sums + 4 * of * N + c;
+          return (x[0] + x[N]) + (x[2 * N] + x[3 * N]);
+        };
+        float f0 = 1.f, f1 = 0.f, top = -sh.neg_a[c], total = sum_of(0);
+        if constexpr (C::kSplit) {
+          const float a0 = top, a1 = -sh.neg_a[N + c];
+          top = fmaxf(a0, a1);
+          f0 = a0 == -INFINITY ? 1.f : fast_exp2(a0 - top);  // nothing seen: sums and O are 0, or NaN to stay
+          f1 = a1 == -INFINITY ? 1.f : fast_exp2(a1 - top);
+          total = f0 * total + f1 * sum_of(1);
+        }
+        if (bad_page || !alive) total = __uint_as_float(0x7FC00000u);
+        float inv = total == 0.f ? 0.f : 1.f / total;
+        int64_t place = 3 * N + c * DP;
+        if (part_to != nullptr) {
+          part_to[c] = top;
+          part_to[N + c] = total;
+          part_to[2 * N + c] = shift;
+          inv = 1.f;
+        } else {
+          const int64_t row = static_cast<int64_t>(p.rb) * N + c, token = sh.row[c] - p.row0;
+          place = static_cast<int64_t>(sh.row[c]) * a.out_ld + (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d;
+        }
+        places[c] = place;
+        if constexpr (kE4m3 && C::kSplit) {
+          f0 *= fast_exp2(sh.shift[0] - shift);
+          f1 *= fast_exp2(sh.shift[1] - shift);
+        }
+        weights[c] = f0 * inv;
+        weights[N + c] = f1 * inv;
+      }
+      all_sync();
+#pragma unroll 1
+      for (int c0 = 16 * wg; c0 < cols; c0 += 64) {
+        float y[16] = {};
+#pragma unroll
+        for (int b = 0; b < C::kPBufs; ++b)
+          if (b ? have1 : have0) {
+            constexpr int kParts = C::kPCols / N;
+            uint32_t o[kParts][16];
+#pragma unroll
+            for (int h = 0; h < kParts; ++h) tmem_ld_x16(tm_o + lanes + C::kPCols * b + N * h + c0, o[h]);
+#pragma unroll
+            for (int h = 0; h < kParts; ++h) tmem_wait_x16(o[h]);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(&weights[N * b + c0 + e]);
+              const float w4[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                float v = __uint_as_float(o[0][e + k]);
+                if constexpr (kParts > 1) v += __uint_as_float(o[kParts - 1][e + k]);
+                y[e + k] = fmaf(v, w4[k], y[e + k]);
+              }
+            }
+          }
+        if (some_bad) {
+          PagedSeq seq;
+          seq.row0 = p.row0;
+          seq.n = p.seq_n;
+          seq.length = vis_max;
+          seq.bad = false;
+#pragma unroll 1
+          for (int e = 0; e < 16; ++e) {
+            const bool bad = c0 + e < rows && ch < a.d &&
+                             tree_sees_bad<kE4m3>(a, seq, a.table + p.table, p.hk, sh.row[c0 + e], ch);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (bad && k == e) y[k] = __uint_as_float(0x7FC00000u);
+          }
+        }
+        if (part_to != nullptr) {
+          if (ch < DP) {
+            float* const to = part_to + 3 * N + c0 * DP + ch;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (c0 + e < rows) to[e * DP] = y[e];
+          }
+        } else if (ch < a.d) {
+          uint16_t* const to = a.out + ch;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)  // a sum of 0 has made y 0, or left it NaN
+            if (c0 + e < rows) to[places[c0 + e]] = __bfloat16_as_ushort(__float2bfloat16_rn(y[e] * back));
+        }
+      }
+      tc_fence_before();
+      if (threadIdx.x == 0) sh.bad_page[part & 7] = sh.any_bad[part & 7] = 0;
+      warp_arrive(sh.part_empty[part & 3]);
+    }
+  }
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    tmem_dealloc(sh.tmem, C::kTmemCols);
+  }
+}
+
+// Joins the parts of the units that more than one block has: block (c, y) rows kJoinRows y .. of
+// the unit that the boundary between blocks c and c + 1 is the first to cut, a warp to a row.
+constexpr int kJoinRows = 8, kJoinThreads = 32 * kJoinRows;
+template <int DP, int N>
+__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_constant__ TreeArgs ta, const int blocks) {
+  const PagedArgs& a = ta.p;
+  const int c = static_cast<int>(blockIdx.x) + 1;
+  __shared__ int64_t scratch[kPlanScratch];
+  Plan w = make_plan<N, kJoinThreads>(a, c, blocks, scratch);
+  Part p;
+  // The first part that block c begins, if the boundary cuts its unit and is the first to do so.
+  int64_t at = 0;
+  const bool some = next_part<N>(a, w, p, &at) && p.tile0 > 0 && at - w.share <= kUnitCost && !p.bad;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are there
+  if (!some) return;
+  const int others = static_cast<int>((kUnitCost + p.steps - at + w.share - 1) / w.share);  // blocks c, c + 1, ...
+  const int rows = static_cast<int>(min(static_cast<int64_t>(p.seq_n) * a.group - static_cast<int64_t>(p.rb) * N,
+                                        static_cast<int64_t>(N)));
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  auto part = [&](int i) -> const float* {
+    return i == 0 ? part_at<DP, N>(ta.parts, c - 1, true) : part_at<DP, N>(ta.parts, c + i - 1, false);
+  };
+  // Sums and outputs each relative to the largest of theirs so far.
+  constexpr int kPer = DP / 32;  // channels of a lane
+  float top = -INFINITY, o_top = -INFINITY, sum = 0.f, y[kPer] = {};
+#pragma unroll 4
+  for (int i = 0; i <= others; ++i) {
+    const float* x = part(i);
+    const float ref = x[r], l = x[N + r], o_ref = ref + x[2 * N + r];
+    float o[kPer];
+    if constexpr (kPer == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(x + 3 * N + r * DP + 4 * lane);
+      o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(x + 3 * N + r * DP + 2 * lane);
+      o[0] = v.x; o[1] = v.y;
+    }
+    // a part whose keys the row does not see has no reference and l = 0 (or NaN, which has to stay)
+    if (ref > top) {
+      sum *= fast_exp2(top - ref);
+      top = ref;
+    }
+    float f = 1.f, back = 1.f;
+    if (ref != -INFINITY) {
+      if (o_ref > o_top) {
+        back = fast_exp2(o_top - o_ref);
+        o_top = o_ref;
+      }
+      f = fast_exp2(o_ref - o_top);
+      sum = fmaf(fast_exp2(ref - top), l, sum);
+    } else {
+      sum += l;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) y[k] = fmaf(f, o[k], back * y[k]);
+  }
+  const uint32_t row = static_cast<uint32_t>(p.rb) * N + r, token = row_token(row, a.group);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum, unit = fast_exp2(o_top - top);
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) y[k] = sum == 0.f && y[k] == y[k] ? 0.f : y[k] * inv * unit;
+  if (kPer * lane < a.d) {
+    uint16_t* const to = a.out + (p.row0 + token) * a.out_ld +
+                         (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d + kPer * lane;
+    if constexpr (kPer == 4)
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    else
+      *reinterpret_cast<uint32_t*>(to) = pack_bf16(y[0], y[1]);
+  }
+}
+
+// Whether blocks take shares of all steps: not where, were every sequence as long as its table
+// allows, a block would have a few only.
+bool shares_steps(const PagedArgs& a, int n, int64_t* units) {
+  const int64_t row_units = (static_cast<int64_t>(a.max_q) * a.group + n - 1) / n;
+  *units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
+  const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
+  return *units * steps > 6 * static_cast<int64_t>(device_sm_count());
+}
+
+// Lets the kernel have its shared memory, and checks that the launch brings the registers that the
+// warps share out among themselves; once per device.
+template <bool kE4m3, int DP, int N>
+cudaError_t configure_tree() {
+  using C = TreeCfg<kE4m3, DP, N>;
+  static std::atomic<bool> done[64] = {};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  cudaFuncAttributes attr;
+  if (cudaError_t e = cudaFuncGetAttributes(&attr, tree_attention_kernel<kE4m3, DP, N>); e != cudaSuccess) return e;
+  if (attr.numRegs / 8 * 8 * C::kThreads < C::kSoftmax * C::kSoftmaxRegs + (C::kThreads - C::kSoftmax) * C::kOtherRegs)
+    return cudaErrorInvalidConfiguration;
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<kE4m3, DP, N>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e == cudaSuccess && dev < 64) done[dev].store(true, std::memory_order_release);
+  return e;
+}
+
+template <bool kE4m3, int DP, int N>
+cudaError_t launch_tree(const PagedArgs& a, float* workspace, cudaStream_t stream) {
+  using C = TreeCfg<kE4m3, DP, N>;
+  CUtensorMap mk, mv;
+  const int box_rows = 1 << a.page_log2;
+  if (!make_page_map(&mk, a.k, a, 128, box_rows, 1) ||
+      !make_page_map(&mv, a.v, a, kE4m3 ? DP : 128, box_rows, 1))
+    return cudaErrorInvalidValue;
+  constexpr auto kKernel = tree_attention_kernel<kE4m3, DP, N>;
+  if (cudaError_t e = configure_tree<kE4m3, DP, N>(); e != cudaSuccess) return e;
+  TreeArgs t{};
+  t.p = a;
+  int64_t units;
+  const bool shared = shares_steps(a, N, &units);
+  t.parts = shared ? workspace : nullptr;
+  t.row_units = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + N - 1) / N);
+  const int64_t grid = shared ? device_sm_count() : units;
+  if (grid > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
+  kKernel<<<static_cast<unsigned>(grid), C::kThreads, C::kSmem, stream>>>(mk, mv, t);
+  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess || !shared) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid - 1), N / kJoinRows);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_parts_kernel<DP, N>, t, static_cast<int>(grid));
+}
+
+}  // namespace
+
+size_t tree_attention_workspace(const PagedArgs& a) {
+  const int64_t most_rows = static_cast<int64_t>(a.max_q) * a.group;
+  int64_t units;
+  if (most_rows <= kFewRows || most_rows > kTreeRows || !shares_steps(a, kTreeRows, &units)) return 0;
+  return static_cast<size_t>(device_sm_count()) * 2 * kTreeRows * ((a.d <= 64 ? 64 : 128) + 3) * sizeof(float);
+}
+
+cudaError_t launch_tree_attention(const PagedArgs& a, void* workspace, cudaStream_t stream) {
+  float* ws = static_cast<float*>(workspace);
+  const bool e4m3 = a.k_scale != nullptr;
+  if (a.d <= 64)
+    return e4m3 ? launch_tree<true, 64, kTreeRows>(a, ws, stream) : launch_tree<false, 64, kTreeRows>(a, ws, stream);
+  return e4m3 ? launch_tree<true, 128, kTreeRows>(a, ws, stream) : launch_tree<false, 128, kTreeRows>(a, ws, stream);
+}
+
+}  // namespace dwa

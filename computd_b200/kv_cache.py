@@ -60,7 +60,8 @@ def _host():
         host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                     for name in ("dwa_kv_write", "dwa_kv_read", "dwa_paged_attention",
                                  "dwa_verify_drafts", "dwa_kv_append", "dwa_kv_keep",
-                                 "dwa_paged_tree_attention", "dwa_tree_masks", "dwa_verify_tree")),
+                                 "dwa_paged_tree_attention", "dwa_paged_tree_attention_workspace",
+                                 "dwa_tree_masks", "dwa_verify_tree")),
                   _lib.check)
         _host_module = host
     return _host_module
@@ -165,9 +166,10 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     as token length - n + j) where bit j % 64 of word j // 64 of its row of ``tree_mask`` (int64 [T, W])
     is set: those of ``tree_masks``, or any others.  Bits from n on count for nothing; a node sees
     itself only if its own bit is set, and one that sees nothing gets zeros.  ``max_q`` bounds a tree's
-    nodes, is 64 W at most, and decides as for ``paged_attention`` how many bits the probabilities
-    keep.  Everything else, the other arguments, rows of no sequence and values that are not finite,
-    is as there."""
+    nodes, is 64 W at most, and picks the kernel: up to 32 rows per key/value head the
+    probabilities over a bf16 cache keep 16 bits, beyond that 8 (over an e4m3 cache 11 either way), as
+    include/dwa_decode.h says.  Everything else, the other arguments, rows of no sequence and values that are not
+    finite, is as there."""
     return (_host_module or _host()).attend_tree(q, k_cache, v_cache, block_table, lengths, q_start, max_q,
                                                  k_scale, v_scale, scale, out, status, tree_mask)
 

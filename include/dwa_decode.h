@@ -153,7 +153,10 @@ DWA_API dwa_status dwa_tree_masks(const int32_t* parents, const int32_t* q_start
  * dwa_paged_attention for new tokens that are a tree's nodes: node i of n attends to the first
  * length - n tokens, and to node j (token length - n + j) where bit j of its row of tree_mask
  * (uint64 [T][mask_words], 8-byte aligned) is set.  Any bits may be; those from n on count for nothing.
- * max_q is 64 mask_words at most.  All else, the rounding too, as there.
+ * max_q is 64 mask_words at most.  All else as there, but the rounding of 17 to 32 rows per
+ * key/value head: bf16 caches none (p_j as the sum of two bf16), e4m3 caches p_j times its value's
+ * scale to 11 bits, and q to 2^-18 of its row's largest value.  workspace: 16-byte aligned, of
+ * dwa_paged_tree_attention_workspace bytes (0: none) for the current device; it holds nothing between calls.
  */
 DWA_API dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H, int32_t d, int64_t q_ld,
                                             const void* k_cache, const void* v_cache,
@@ -163,8 +166,10 @@ DWA_API dwa_status dwa_paged_tree_attention(const void* q, int64_t T, int32_t H,
                                             int64_t ld_table, int32_t max_pages, const int32_t* lengths,
                                             const int32_t* q_start, int32_t B, int32_t max_q,
                                             const int64_t* tree_mask, int32_t mask_words, float scale,
-                                            void* out, int64_t out_ld, int32_t* status,
-                                            dwa_stream_t stream);
+                                            void* out, int64_t out_ld, void* workspace,
+                                            size_t workspace_bytes, int32_t* status, dwa_stream_t stream);
+DWA_API size_t dwa_paged_tree_attention_workspace(int32_t H, int32_t d, int32_t H_kv, int32_t page_size,
+                                                  int32_t max_pages, int32_t B, int32_t max_q);
 
 /*
  * The walk through a verified tree: target [T][V] (f32, or bf16 when probs_bf16) holds the

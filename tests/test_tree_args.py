@@ -36,7 +36,7 @@ def attention(**kw):
         a["q"], a["T"], a["heads"], c["d"], a["q_ld"], c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"], c["H"],
         c["n_pages"], c["page_size"], c["ld_page"], c["ld_scale"], a["table"], a["ld_table"], a["max_pages"],
         a["lengths"], a["q_start"], a["B"], a["max_q"], a["mask"], a["words"], a["scale"], a["out"], a["out_ld"],
-        a["status"], None)
+        None, 0, a["status"], None)
 
 
 def keep(**kw):
