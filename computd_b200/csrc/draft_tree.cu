@@ -4,8 +4,9 @@
 // A tree is the n newest tokens of a sequence, parents before children; node 0 is the
 // sequence's newest token, the others are drafts.
 //
-// Masks: a node's row has its own bit and its ancestors'.  A thread per node walks up; since
-// parents have lower numbers the bits come in descending order, a word at a time.
+// Masks: a node's row has its own bit and its ancestors'.  Up to 128 nodes by doubling, in log2(depth) rounds;
+// beyond, a thread per node walks up: since parents have lower numbers the bits come in
+// descending order, a word at a time.
 //
 // Walk: at node 0 a token t is drawn from the node's row of probabilities; where a child has t
 // the walk goes on from there, else it ends with t.  Given the tree t is distributed as
@@ -13,9 +14,9 @@
 // pass of the model reaches.  Running sums are 64-bit, good to 1e-16 of their total, so
 // the outcome does not hang on their order.
 //
-// One row of V entries per step of the path is read.  A cluster of blocks shares it, each warp a contiguous piece; the
-// pieces' sums go through distributed shared memory, the warp whose piece holds the draw
-// finds it and tells every block.
+// One row of V entries per step of the path is read.  A cluster of blocks shares it, each lane a
+// contiguous chunk (32 entries of 64400: one round of loads); the warps' sums go through distributed shared memory, the
+// warp whose piece holds the draw finds it and tells every block.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -33,6 +34,7 @@ namespace {
 // ---------------------------------------------------------------- masks
 constexpr int kMaskThreads = 128;
 constexpr int kMostNodes = 4096;  // of a tree
+constexpr int kShortWords = 2;    // up to 128 nodes
 
 struct MaskArgs {
   const int32_t *parents, *q_start;
@@ -79,6 +81,42 @@ __global__ void __launch_bounds__(kMaskThreads) tree_masks_kernel(const MaskArgs
     up[i] = p;
   }
   if (__syncthreads_or(bad) && threadIdx.x == 0) paged_report(a.status);
+  if (a.words <= kShortWords) {
+    // Few words: a node takes what the node that it has come to sees, twice as far each time.
+    uint64_t* const seen = reinterpret_cast<uint64_t*>(up + ((a.max_q + 1) & ~1));
+    static_assert(64 * kShortWords <= kMaskThreads, "a node to a thread");
+    const int i = threadIdx.x;
+    uint64_t bits[kShortWords];
+    int at = i < n ? up[i] : -1;
+#pragma unroll
+    for (int w = 0; w < kShortWords; ++w) {
+      bits[w] = i >> 6 == w ? 1ull << (i & 63) : 0;
+      if (i < n) seen[i * kShortWords + w] = bits[w];
+    }
+    while (__syncthreads_or(at >= 0)) {
+      if (at >= 0) {
+#pragma unroll
+        for (int w = 0; w < kShortWords; ++w) bits[w] |= seen[at * kShortWords + w];
+        at = up[at];
+      }
+      __syncthreads();
+      if (i < n) {
+        up[i] = at;
+#pragma unroll
+        for (int w = 0; w < kShortWords; ++w) seen[i * kShortWords + w] = bits[w];
+      }
+    }
+    if (i < n) {
+      int depth = -1;
+#pragma unroll
+      for (int w = 0; w < kShortWords; ++w) {
+        depth += __popcll(bits[w]);
+        if (w < a.words) a.mask[(lo + i) * a.words + w] = bits[w];
+      }
+      a.depth[lo + i] = depth;
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < n; i += kMaskThreads) {
     uint64_t* row = a.mask + (lo + i) * a.words;
     int w = i >> 6, depth = -1;
@@ -104,7 +142,8 @@ __global__ void __launch_bounds__(kMaskThreads) tree_masks_kernel(const MaskArgs
 constexpr int kWalkThreads = 256;
 constexpr int kWalkWarps = kWalkThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBatch = 4;
+constexpr int kBatch = 8;      // of four entries, under way together
+constexpr int kHeldNodes = 2;  // of a lane
 
 struct WalkArgs {
   const void* target;
@@ -112,7 +151,7 @@ struct WalkArgs {
   const float* u;
   int64_t T;
   int even, B, steps, V;
-  int piece;  // entries per warp, a multiple of 4
+  int chunk;  // entries per lane, a multiple of 4: a warp's lie side by side
   int wide;   // rows may be read four entries at a time
   int32_t *n_accepted, *out_tokens, *path;
 };
@@ -149,9 +188,20 @@ __device__ __forceinline__ double sum4(const float (&x)[4]) {
   return (static_cast<double>(x[0]) + static_cast<double>(x[1])) +
          (static_cast<double>(x[2]) + static_cast<double>(x[3]));
 }
-__device__ __forceinline__ double warp_sum(double x) {
+template <typename T>
+__device__ __forceinline__ double weight1(const T* at) {
+  float x;
+  if constexpr (sizeof(T) == 2) x = __uint_as_float(static_cast<uint32_t>(__ldg(at)) << 16);
+  else x = __ldg(at);
+  x = fmaxf(x, 0.f);  // NaN too
+  return x < INFINITY ? static_cast<double>(x) : 0.0;
+}
+__device__ __forceinline__ double warp_scan(double x) {  // inclusive
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if ((threadIdx.x & 31) >= o) x += y;
+  }
   return x;
 }
 __device__ __forceinline__ double ld_cluster_f64(const double* local, int rank) {
@@ -180,24 +230,32 @@ __global__ void __launch_bounds__(kWalkThreads, 4) verify_tree_kernel(const Walk
   }
   const bool writes = rank == 0 && threadIdx.x == 0;
   const int pieces = cluster * kWalkWarps;
-  const int lo = min((rank * kWalkWarps + warp) * a.piece, V);
-  const int hi = min(lo + a.piece, V);
+  const int lo = static_cast<int>(min((static_cast<int64_t>(rank * kWalkWarps + warp) * 32 + lane) * a.chunk, static_cast<int64_t>(V)));
+  const int hi = min(lo + a.chunk, V);  // this lane's entries
+  // The first nodes' parents and tokens, some to a lane, are there before the first draw.
+  int held_parent[kHeldNodes], held_token[kHeldNodes];
+#pragma unroll
+  for (int k = 0; k < kHeldNodes; ++k) {
+    const int i = 32 * k + lane;
+    held_parent[k] = i < n ? __ldg(a.parents + row0 + i) : -1;
+    held_token[k] = i < n ? __ldg(a.tokens + row0 + i) : -1;
+  }
   int node = 0, kept = 0, step = 0;
   bool going = n > 0;
   for (; going; ++step) {
     const int set = step & 1;
     const T* p = static_cast<const T*>(a.target) + (row0 + node) * V;
     const double u = __ldg(a.u + b * a.steps + step);
-    double s = 0.0;
-    for (int i0 = lo; i0 < hi; i0 += 128 * kBatch) {
+    double own = 0.0;
+    for (int i0 = lo; i0 < hi; i0 += 4 * kBatch) {
       float x[kBatch][4];
 #pragma unroll
-      for (int r = 0; r < kBatch; ++r) weights4(p, i0 + 128 * r + 4 * lane, hi, a.wide, x[r]);
+      for (int r = 0; r < kBatch; ++r) weights4(p, i0 + 4 * r, hi, a.wide, x[r]);
 #pragma unroll
-      for (int r = 0; r < kBatch; ++r) s += sum4(x[r]);
+      for (int r = 0; r < kBatch; ++r) own += sum4(x[r]);
     }
-    s = warp_sum(s);
-    if (lane == 0) sums[set][warp] = s;
+    const double upto = warp_scan(own);  // of the warp's piece
+    if (lane == 31) sums[set][warp] = upto;
     cluster_sync();
     // Lane l has the sums of pieces 2 l and 2 l + 1, and by a scan what lies before them;
     // every warp computes the same.
@@ -207,12 +265,7 @@ __global__ void __launch_bounds__(kWalkThreads, 4) verify_tree_kernel(const Walk
       mine0 = ld_cluster_f64(&sums[set][k], c);
       mine1 = ld_cluster_f64(&sums[set][k + 1], c);
     }
-    double before = mine0 + mine1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xFFFFFFFFu, before, o);
-      if (lane >= o) before += y;
-    }
+    double before = warp_scan(mine0 + mine1);
     const double total = __shfl_sync(0xFFFFFFFFu, before, 31);
     if (total > 0.0) {
       const double goal = u * total;
@@ -227,49 +280,35 @@ __global__ void __launch_bounds__(kWalkThreads, 4) verify_tree_kernel(const Walk
       const int at = __shfl_sync(0xFFFFFFFFu, 2 * lane + (early ? 0 : 1), src);
       double run = __shfl_sync(0xFFFFFFFFu, early ? before : mid, src);
       if (at == rank * kWalkWarps + warp) {
-        // the run of 128 entries that the draw is in; where rounding keeps the running sum at the
-        // goal to the end, the last with weight
-        int i = -1;
-        bool in = false;
-        for (int i0 = lo; i0 < hi && !in; i0 += 128 * kBatch) {
-          float x[kBatch][4];
-          double row[kBatch];
-#pragma unroll
-          for (int r = 0; r < kBatch; ++r) weights4(p, i0 + 128 * r + 4 * lane, hi, a.wide, x[r]);
-#pragma unroll
-          for (int r = 0; r < kBatch; ++r) row[r] = warp_sum(sum4(x[r]));
-#pragma unroll
-          for (int r = 0; r < kBatch; ++r)
-            if (!in && row[r] > 0.0) {
-              i = i0 + 128 * r + 4 * lane;
-              in = run + row[r] > goal;
-              if (!in) run += row[r];
-            }
-        }
-        // in it the first entry whose running sum passes the goal, or the last with weight
-        float x[4];
-        weights4(p, i, hi, a.wide, x);
-        const double four = sum4(x);
-        double incl = four;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double z = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-          if (lane >= o) incl += z;
-        }
-        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, in && four > 0.0 && run + incl > goal);
-        const uint32_t any = __ballot_sync(0xFFFFFFFFu, four > 0.0);
-        int j = x[3] > 0.f ? 3 : x[2] > 0.f ? 2 : x[1] > 0.f ? 1 : 0;  // the last with weight
-        if (hit) {
-          const double c = run + (incl - four);
-#pragma unroll
-          for (int k = 2; k >= 0; --k) {
-            double head = c + static_cast<double>(x[0]);
-            if (k > 0) head += static_cast<double>(x[1]);
-            if (k > 1) head += static_cast<double>(x[2]);
-            if (x[k] > 0.f && head > goal) j = k;
+        // The first lane whose running sum passes the goal, or where rounding keeps it at the goal the last
+        // with weight; then of its entries, again shared out among the lanes, the lane's; then the entry.
+        auto lane_of = [&](double sum, double incl) -> int {
+          const uint32_t hit = __ballot_sync(0xFFFFFFFFu, sum > 0.0 && run + incl > goal);
+          const uint32_t any = __ballot_sync(0xFFFFFFFFu, sum > 0.0);
+          return hit ? __ffs(hit) - 1 : 31 - __clz(any);
+        };
+        int l = lane_of(own, upto);
+        run += __shfl_sync(0xFFFFFFFFu, upto - own, l);
+        const int first = __shfl_sync(0xFFFFFFFFu, lo, l), end = __shfl_sync(0xFFFFFFFFu, hi, l);
+        const int per = (a.chunk + 31) / 32, from = min(first + lane * per, end), to = min(from + per, end);
+        double part = 0.0;
+        for (int i = from; i < to; ++i) part += weight1(p + i);
+        const double incl = warp_scan(part);
+        l = lane_of(part, incl);
+        int found = from;
+        if (lane == l) {
+          double c = run + (incl - part);
+          int last = from;
+          bool in = false;
+          for (int i = from; i < to && !in; ++i) {
+            const double w = weight1(p + i);
+            c += w;
+            if (w > 0.0) last = i;
+            in = w > 0.0 && c > goal;
           }
+          found = last;
         }
-        const int token = __shfl_sync(0xFFFFFFFFu, i + j, hit ? __ffs(hit) - 1 : 31 - __clz(any));
+        const int token = __shfl_sync(0xFFFFFFFFu, found, l);
         if (lane < cluster) st_cluster_s32(map_to_cta(smem_u32(&drawn[set]), lane), token);
       }
     }
@@ -277,14 +316,22 @@ __global__ void __launch_bounds__(kWalkThreads, 4) verify_tree_kernel(const Walk
     const int token = total > 0.0 ? *static_cast<volatile int*>(&drawn[set]) : -1;
     // the first child that has it: every warp for itself
     int child = INT_MAX;
-    if (token >= 0 && step + 1 < a.steps)
-      for (int i0 = 1; i0 < n && child == INT_MAX; i0 += 32) {
+    if (token >= 0 && step + 1 < a.steps) {
+#pragma unroll
+      for (int k = 0; k < kHeldNodes; ++k) {
+        const int i = 32 * k + lane;
+        const uint32_t all =
+            __ballot_sync(0xFFFFFFFFu, i > node && held_parent[k] == node && held_token[k] == token);
+        if (all && child == INT_MAX) child = 32 * k + __ffs(all) - 1;
+      }
+      for (int i0 = 32 * kHeldNodes; i0 < n && child == INT_MAX; i0 += 32) {
         const int i = i0 + lane;
         const bool fits = i < n && __ldg(a.parents + row0 + i) == node && i > node &&
                           __ldg(a.tokens + row0 + i) == token;
         const uint32_t all = __ballot_sync(0xFFFFFFFFu, fits);
         if (all) child = i0 + __ffs(all) - 1;
       }
+    }
     if (writes) {
       a.out_tokens[b * a.steps + step] = token;
       a.path[b * a.steps + step] = node;
@@ -316,7 +363,8 @@ cudaError_t launch_tree_masks(const int32_t* parents, const int32_t* q_start, in
   a.even = q_start ? 0 : static_cast<int>(T / B);
   a.max_q = max_q; a.B = B; a.words = words;
   a.mask = reinterpret_cast<uint64_t*>(mask); a.depth = depth; a.status = status;
-  tree_masks_kernel<<<static_cast<unsigned>(B), kMaskThreads, max_q * sizeof(int32_t), stream>>>(a);
+  const size_t smem = ((max_q + 1) & ~1) * sizeof(int32_t) + (words <= kShortWords ? max_q * kShortWords * 8 : 0);
+  tree_masks_kernel<<<static_cast<unsigned>(B), kMaskThreads, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -331,8 +379,8 @@ cudaError_t launch_verify_tree(const void* target, int probs_bf16, const int32_t
   // one block per 2048 entries, up to the portable cluster size
   int cluster = 1;
   while (cluster < kMaxCluster && cluster * 2048 < V) cluster *= 2;
-  const int pieces = cluster * kWalkWarps;
-  a.piece = (((V + pieces - 1) / pieces) + 3) & ~3;
+  const int lanes = cluster * kWalkThreads;
+  a.chunk = (((V + lanes - 1) / lanes) + 3) & ~3;
   a.wide = V % 4 == 0 && reinterpret_cast<uintptr_t>(target) % (probs_bf16 ? 8 : 16) == 0;
 
   cudaLaunchConfig_t cfg{};

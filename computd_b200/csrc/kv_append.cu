@@ -27,7 +27,10 @@ namespace dwa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerSm = 2;
+// Blocks per SM, which decide how many loads are under way: bf16 into a bf16 cache 2, 3, 4 (8191 tokens, 32 over 8 heads
+// of 128: 69, 54, 50 us); codes and f32 need the registers.
+template <bool kE4m3, bool kSrcBf16>
+constexpr int kBlocks = !kSrcBf16 ? 2 : kE4m3 ? 3 : 4;
 constexpr int kBlockTokens = 32;  // at most; a longer call is cut into launches
 
 // Sixteen neighbouring values of a row.
@@ -103,7 +106,7 @@ struct AppendArgs {
 // the vectors of its tokens (token by token: queries, keys, values), a round's values under way
 // while the round before is stored.
 template <bool kE4m3, bool kSrcBf16, bool kTabBf16>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) kv_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocks<kE4m3, kSrcBf16>) kv_append_kernel(const AppendArgs a) {
   __shared__ int64_t own[kBlockTokens];
   __shared__ int dropped[kBlockTokens];
   __shared__ uint32_t filter[kFilterBits / 32];
@@ -253,7 +256,10 @@ cudaError_t launch_kv_append(const KvCacheView& c, const KvAppendView& x, int64_
   a.ld_page = c.ld_page / c.d; a.ld_scale_page = c.ld_scale_page;
   a.lanes_log2 = log2_at_least(c.d / 16);
   a.status = status;
-  const int64_t most = static_cast<int64_t>(kBlocksPerSm) * device_sm_count();
+  const bool e4m3 = c.k_scale != nullptr;
+  const int per_sm = e4m3 ? (x.src_bf16 ? kBlocks<true, true> : kBlocks<true, false>)
+                          : (x.src_bf16 ? kBlocks<false, true> : kBlocks<false, false>);
+  const int64_t most = static_cast<int64_t>(per_sm) * device_sm_count();
   const int64_t launches = (T + most * kBlockTokens - 1) / (most * kBlockTokens);
   const int64_t share = (T + launches - 1) / launches;  // tokens of one
   const int64_t es = x.src_bf16 ? 2 : 4;
@@ -273,7 +279,7 @@ cudaError_t launch_kv_append(const KvCacheView& c, const KvAppendView& x, int64_
     const int64_t rounds = (static_cast<int64_t>(a.tokens_per_block) * (a.H + 2 * a.H_kv) + groups - 1) / groups;
     a.parts = static_cast<int>(std::max<int64_t>(1, std::min(rounds, most / runs)));
     const unsigned grid = static_cast<unsigned>(runs * a.parts);
-    if (c.k_scale != nullptr) {
+    if (e4m3) {
       if (x.src_bf16) launch_one<true, true>(a, x.tables_bf16, grid, stream);
       else launch_one<true, false>(a, x.tables_bf16, grid, stream);
     } else {

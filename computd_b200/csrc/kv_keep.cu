@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStaged = 256;  // moves whose pages and places are looked up together
-constexpr int kBatch = 4;     // tokens under way together
+constexpr int kBatch = 16;    // tokens under way together (with 4 of 12 layers' long paths 11.3 us)
 
 struct KeepArgs {
   uint8_t *k, *v;
