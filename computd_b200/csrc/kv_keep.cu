@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStaged = 256;  // moves whose pages and places are looked up together
-constexpr int kBatch = 16;    // tokens under way together (with 4 of 12 layers' long paths 11.3 us)
+constexpr int kBatch = 8;     // tokens under way together
 
 struct KeepArgs {
   uint8_t *k, *v;
@@ -39,9 +39,27 @@ struct KeepArgs {
   int32_t* status;
 };
 
+struct Move {  // a token's page and place in it, before and after
+  int64_t from_page, to_page;
+  int from, to;
+};
+
+// A thread's part of moves k0 .. k1 - 1, in their order.
+template <typename T, typename F>
+__device__ __forceinline__ void move(const Move* moves, int k0, int k1, F&& at) {
+  for (int k = k0; k < k1; k += kBatch) {
+    T held[kBatch];
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e)
+      if (k + e < k1) held[e] = *at(moves[k + e].from_page, moves[k + e].from);
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e)
+      if (k + e < k1) *at(moves[k + e].to_page, moves[k + e].to) = held[e];
+  }
+}
+
 __global__ void __launch_bounds__(kThreads) kv_keep_kernel(const KeepArgs a) {
-  __shared__ int64_t from[kStaged], to[kStaged];      // bytes of a layer to the head's first vector's place
-  __shared__ int64_t from_s[kStaged], to_s[kStaged];  // scales
+  __shared__ Move moves[kStaged];
   __shared__ int first;
   const int64_t b = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x % a.parts);
@@ -54,67 +72,51 @@ __global__ void __launch_bounds__(kThreads) kv_keep_kernel(const KeepArgs a) {
   // nodes ascend: from the first that moves on all do
   if (threadIdx.x == 0) first = n + 1;
   __syncthreads();
+  const int mask = (1 << a.page_log2) - 1;
   bool bad = n >= a.steps || start < 0;
   for (int i = threadIdx.x; i <= n && !bad; i += kThreads) {
     const int64_t node = __ldg(path + i), before = i > 0 ? __ldg(path + i - 1) : -1;
     bad = node <= before || start + node >= tokens;
     if (bad || node == i) continue;
-    const int p = __ldg(table + ((start + node) >> a.page_log2)), q = __ldg(table + ((start + i) >> a.page_log2));
+    const int64_t p = __ldg(table + ((start + node) >> a.page_log2)), q = __ldg(table + ((start + i) >> a.page_log2));
     bad = p < 0 || p >= a.n_pages || q < 0 || q >= a.n_pages;
     atomicMin(&first, i);
+    if (i < kStaged) moves[i] = Move{p, q, static_cast<int>((start + node) & mask), static_cast<int>((start + i) & mask)};
   }
   if (__syncthreads_or(bad)) {  // the sequence's tokens stay where they are
     if (part == 0 && threadIdx.x == 0) paged_report(a.status);
     return;
   }
-  const int mask = (1 << a.page_log2) - 1;
-  for (int i0 = first; i0 <= n; i0 += kStaged) {
-    const int i = i0 + threadIdx.x;
-    if (i <= n && threadIdx.x < kStaged) {
-      const int64_t old = start + __ldg(path + i), now = start + i;
-      const int64_t p = __ldg(table + (old >> a.page_log2)), q = __ldg(table + (now >> a.page_log2));
-      from[threadIdx.x] = p * a.ld_page + (old & mask) * a.row_bytes;
-      to[threadIdx.x] = q * a.ld_page + (now & mask) * a.row_bytes;
-      from_s[threadIdx.x] = p * a.ld_scale_page + (old & mask);
-      to_s[threadIdx.x] = q * a.ld_scale_page + (now & mask);
+  const int pieces = a.row_bytes >> 4;
+  for (int i0 = 0; i0 <= n; i0 += kStaged) {
+    if (i0 > 0) {  // the first are there already
+      __syncthreads();
+      const int i = i0 + threadIdx.x;
+      if (i <= n && i >= first) {
+        const int64_t old = start + __ldg(path + i), now = start + i;
+        moves[threadIdx.x] = Move{__ldg(table + (old >> a.page_log2)), __ldg(table + (now >> a.page_log2)),
+                                  static_cast<int>(old & mask), static_cast<int>(now & mask)};
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    const int m = min(n + 1 - i0, kStaged);
-    const int pieces = a.row_bytes >> 4;
-    for (int64_t c = static_cast<int64_t>(part) * kThreads + threadIdx.x; c < a.columns;
+    const int k0 = max(first - i0, 0), k1 = min(n + 1 - i0, kStaged);
+    if (k0 >= k1) continue;
+    for (int64_t c = static_cast<int64_t>(part) * kThreads + threadIdx.x; c < a.columns + a.scales;
          c += static_cast<int64_t>(a.parts) * kThreads) {
-      const int64_t vec = c / pieces;  // (layer, keys or values, head)
-      const int h = static_cast<int>(vec % a.H);
+      const bool scale = c >= a.columns;
+      const int64_t vec = scale ? c - a.columns : c / pieces;  // (layer, keys or values, head)
       const int64_t side = vec / a.H;
-      uint8_t* base = ((side & 1) ? a.v : a.k) + (side >> 1) * a.ld_layer +
-                      ((static_cast<int64_t>(h) << a.page_log2) * a.row_bytes) + (c - vec * pieces) * 16;
-      for (int k = 0; k < m; k += kBatch) {
-        uint4 held[kBatch];
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (k + e < m) held[e] = *reinterpret_cast<const uint4*>(base + from[k + e]);
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (k + e < m) *reinterpret_cast<uint4*>(base + to[k + e]) = held[e];
+      const int64_t head = (vec - side * a.H) << a.page_log2;
+      if (scale) {
+        float* const base = ((side & 1) ? a.v_scale : a.k_scale) + (side >> 1) * a.ld_scale_layer + head;
+        move<float>(moves, k0, k1, [&](int64_t page, int at) { return base + page * a.ld_scale_page + at; });
+      } else {
+        uint8_t* const base = ((side & 1) ? a.v : a.k) + (side >> 1) * a.ld_layer + head * a.row_bytes + (c - vec * pieces) * 16;
+        move<uint4>(moves, k0, k1, [&](int64_t page, int at) {
+          return reinterpret_cast<uint4*>(base + page * a.ld_page + static_cast<int64_t>(at) * a.row_bytes);
+        });
       }
     }
-    for (int64_t c = static_cast<int64_t>(part) * kThreads + threadIdx.x; c < a.scales;
-         c += static_cast<int64_t>(a.parts) * kThreads) {
-      const int h = static_cast<int>(c % a.H);
-      const int64_t side = c / a.H;
-      float* base = ((side & 1) ? a.v_scale : a.k_scale) + (side >> 1) * a.ld_scale_layer +
-                    (static_cast<int64_t>(h) << a.page_log2);
-      for (int k = 0; k < m; k += kBatch) {
-        float held[kBatch];
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (k + e < m) held[e] = base[from_s[k + e]];
-#pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-          if (k + e < m) base[to_s[k + e]] = held[e];
-      }
-    }
-    __syncthreads();
   }
 }
 
@@ -139,7 +141,7 @@ cudaError_t launch_kv_keep(const KvCacheView& c, int layers, int64_t ld_layer, i
   a.columns = vectors * (a.row_bytes / 16);
   a.scales = e4m3 ? vectors : 0;
   const int64_t most = (4 * static_cast<int64_t>(device_sm_count()) + B - 1) / B;  // blocks of a sequence
-  a.parts = static_cast<int>(std::max<int64_t>(1, std::min((a.columns + kThreads - 1) / kThreads, most)));
+  a.parts = static_cast<int>(std::max<int64_t>(1, std::min((a.columns + a.scales + kThreads - 1) / kThreads, most)));
   a.status = status;
   kv_keep_kernel<<<static_cast<unsigned>(B * a.parts), kThreads, 0, stream>>>(a);
   return cudaGetLastError();
