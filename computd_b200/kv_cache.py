@@ -166,9 +166,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     as token length - n + j) where bit j % 64 of word j // 64 of its row of ``tree_mask`` (int64 [T, W])
     is set: those of ``tree_masks``, or any others.  Bits from n on count for nothing; a node sees
     itself only if its own bit is set, and one that sees nothing gets zeros.  ``max_q`` bounds a tree's
-    nodes, is 64 W at most, and picks the kernel: up to 32 rows per key/value head the
-    probabilities over a bf16 cache keep 16 bits, beyond that 8 (over an e4m3 cache 11 either way), as
-    include/dwa_decode.h says.  Everything else, the other arguments, rows of no sequence and values that are not
+    nodes, is 64 W at most, and picks the kernel with the sizes of ``q`` and ``block_table``: up to 32
+    rows per key/value head, and 64 where tables are narrow, the probabilities over a bf16 cache keep 16
+    bits, beyond that 8 (over an e4m3 cache 11 either way), as include/dwa_decode.h says.  Everything else, the other arguments, rows of no sequence and values that are not
     finite, is as there."""
     return (_host_module or _host()).attend_tree(q, k_cache, v_cache, block_table, lengths, q_start, max_q,
                                                  k_scale, v_scale, scale, out, status, tree_mask)
