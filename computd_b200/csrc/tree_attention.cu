@@ -1,16 +1,15 @@
 // tree_attention.cu — attention of a tree's nodes over the paged cache on tcgen05, for
 // more rows per key/value head than paged_attention.cu takes.
 //
-// A row is one (node, query head of the group), node-major.  A unit is up to N (32, 64 or 128) rows of one
-// key/value head; it goes over the sequence's keys 128 at a time, its products transposed:
+// A row is one (node, query head of the group), node-major.  A unit is up to 32 rows of one key/value
+// head; it goes over the sequence's keys 128 at a time, its products transposed:
 //
-//   S^T = K Q^T       128 keys by N rows     tcgen05, K and Q in shared memory, S in TMEM
-//   P   = exp2(S - a) a thread per key and 16 or 32 rows
-//   O^T += V^T P      128 channels by N rows tcgen05, V and P in shared memory, O in TMEM
+//   S^T = K Q^T       128 keys by 32 rows     tcgen05, K and Q in shared memory, S in TMEM
+//   P   = exp2(S - a) a thread per key and 16 rows
+//   O^T += V^T P      128 channels by 32 rows tcgen05, V and P in shared memory, O in TMEM
 //
 // so that neither the tensor pipe nor the exponentials work on rows that are not there: a tile
-// of 128 rows would be 50 to 87 % empty for a tree of 16 to 64 nodes.  A key's scales
-// (e4m3) are one number of its thread's.
+// of 128 rows would be 75 to 87 % empty.  A key's scales (e4m3) are one number of its thread's.
 //
 // What a row's weights are relative to, a, is not its maximum but anything that keeps them in
 // range; it moves when a score passes the limit, which every step asks by a vote, and only
@@ -23,15 +22,20 @@
 // cache, at twice the rate of fp16 and without a conversion); P times the value's scale is
 // rounded to fp16, 11 bits.
 //
-// Bound by HBM up to 64 rows, by the softmax's issue slots and the conversion of the values beyond.
-// Work is cut by steps, not by units, where sequences are long: each block takes an equal share of
-// all steps, whatever sequence they belong to, and writes a unit that it has only a part of to
-// a workspace, from which a second kernel joins the parts in a fixed order.
+// Bound by HBM where contexts are long and all as long: 16 sequences of 32 nodes over 4096 tokens, 16 heads of
+// 128 channels, bf16, 93 us, 5.7 TB/s; else by the length of a step's chain (loads from TMEM, vote, exponentials,
+// stores, product) and by what a unit costs beside its steps: 20 to 32 nodes over 300 to 4096 tokens 56 us, 4.8 TB/s
+// (floor 41); one sequence over 4096 20 us, e4m3 22.  (More rows are no work for this layout: a thread reads
+// its columns' references, 4 bytes each, from shared memory, which with 64 or 128 columns takes as long as all
+// else.)
+// Work is cut by steps, not by units: each block takes an equal share of all steps, whatever sequence they
+// belong to, and writes a unit that it has only a part of to a workspace, from which a second
+// kernel joins the parts in a fixed order.
 //
-// Sixteen warps: softmax (four to a scheduler: with eight, each its 64 columns, a step's chain of TMEM
-// loads, exponentials and stores was twice as long).  One warp: tcgen05.mma.  Two: TMA, straight from the pages.  Two
-// look over the values of the tree's nodes (bf16), since 0 * NaN would reach rows that must not see
-// it, or turn the values' codes into fp16 (e4m3).
+// Sixteen warps: softmax, a warpgroup to sixteen columns of every other tile (with eight warps a step's
+// chain was twice as long); e4m3: they turn the values' codes into fp16 too, bf16: they look over
+// the values of the tree's nodes, since 0 * NaN would reach rows that must not see it.  One warp: tcgen05.mma.  Two:
+// TMA, straight from the pages.  One: the block's next parts.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -49,7 +53,7 @@ namespace dwa {
 
 namespace {
 
-constexpr int kLeastShare = 8;    // of a block, in steps
+constexpr int kLeastShare = 6;    // of a block, in steps
 // What a unit costs beside its steps: Q, first references and the way out.  Work is shared out in
 // steps and these, so that short sequences' units do not pile up in a few blocks (24 ragged ones of 50 to 1500 tokens,
 // 16 heads of 80: 112 us without).
@@ -59,19 +63,15 @@ constexpr int kSmemLimit = 227 * 1024;
 template <bool kE4m3, int DP, int N>
 struct TreeCfg {
   static constexpr int kThreads = 640, kSoftmax = 512, kSoftmaxRegs = 104, kOtherRegs = 64;
-  // Four warpgroups: up to 64 columns two for each of alternate tiles of keys; what shares a tile
-  // shares out its columns.
-  static constexpr bool kSplit = N <= 64;
-  static constexpr int kSharers = kSplit ? 2 : 4;
-  static constexpr int kChunks = N / 16 / kSharers;            // sixteens of columns of a warpgroup
+  // Four warpgroups: two for each of alternate tiles of keys (a side), each with sixteen columns.
+  static constexpr int kSharers = 2;
+  static_assert(N == 16 * kSharers);
   static constexpr int kHalves = DP / 64;
   static constexpr int kQPart = N * 128;                       // 64 bf16 channels, or 128 codes
   static constexpr int kQBytes = (kE4m3 ? 2 : kHalves) * kQPart;
-  // bf16: both parts of P side by side, as columns of one product; of 128 columns one part
-  static constexpr bool kTwoParts = !kE4m3 && kSplit;
-  static constexpr int kPCols = (kTwoParts ? 2 : 1) * N;
-  static constexpr int kPBytes = (kPCols + 63) / 64 * kBlock;  // of a buffer
-  static constexpr int kPBufs = kSplit ? 2 : 1;
+  static constexpr int kPCols = (kE4m3 ? 1 : 2) * N;           // bf16: both parts of P side by side, in one product
+  static constexpr int kPBytes = kBlock;                       // of a buffer, and a side has one
+  static constexpr int kPBufs = 2;
   static constexpr int kKBytes = (kE4m3 ? 1 : kHalves) * kBlock;
   // Codes of values arrive where their fp16 values go (128 channels: the second block), or behind it.
   static constexpr int kRawAt = kBlock;
@@ -245,9 +245,9 @@ struct TreeShared {
   int abort;
   Part parts[4];                // under way, by their number
   int bad_page[8], any_bad[8];
-  alignas(16) float neg_a[N <= 64 ? 2 * N : N];  // minus what a column's weights are relative to (of each side)
+  alignas(16) float neg_a[2 * N];  // minus what a column's weights are relative to (of each side)
   alignas(16) float f[kE4m3 ? N : 4];     // its scores' factor, to log2 units
-  int most[N <= 64 ? 2 * N : N];  // across keys, ordered
+  int most[2 * N];  // across keys, ordered
   int row[N];                   // of q
   uint32_t tops[4][4];          // e4m3: scales' exponents
   float shift[2];               // of each side
@@ -321,8 +321,8 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
   tc_fence_after();
   const uint32_t tm_s = sh.tmem, tm_o = sh.tmem + 2 * N;  // S: + N (it & 1); O: + kPCols (P's buffer)
   // the buffer of P and O that tile `it` goes through, and which use of it that is
-  auto p_buf = [](int it) -> int { return C::kSplit ? it & 1 : 0; };
-  auto p_use = [](int it) -> int { return C::kSplit ? it >> 1 : it; };
+  auto p_buf = [](int it) -> int { return it & 1; };
+  auto p_use = [](int it) -> int { return it >> 1; };
   int* const status = a.status;
   volatile int* const abort_flag = &sh.abort;
   auto wait = [&](const uint64_t& x, int phase) -> bool {
@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(x));
   };
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // join_parts_kernel, where there is room
   const uint32_t s_k = base + C::kKAt, s_v = base + C::kVAt, s_p = base + C::kPAt;
   auto rows_of = [&](int seq_n, int rb) -> int {  // of the unit
     return static_cast<int>(min(static_cast<int64_t>(seq_n) * a.group - static_cast<int64_t>(rb) * N,
@@ -531,12 +532,9 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
   } else {
     regs_inc<C::kSoftmaxRegs>();
     const int wg = warp >> 2, quad = warp & 3, t = threadIdx.x & 127;
-    const int group_bar = 1 + wg, side = C::kSplit ? wg >> 1 : 0, sharer = wg % C::kSharers;  // side: of the tiles
+    const int group_bar = 1 + wg, side = wg >> 1, c0 = 16 * (wg % C::kSharers);  // c0: this warpgroup's columns
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     auto all_sync = [&]() { asm volatile("barrier.cta.sync 5, 512;" ::: "memory"); };
-    auto chunk_of = [&](int i) { return C::kSharers * i + sharer; };  // sixteens of columns
-    // this warpgroup's columns, i < 16 kChunks
-    auto column = [&](int i) { return 16 * chunk_of(i >> 4) + (i & 15); };
     float* const neg_a = sh.neg_a + side * N;
     int* const mosts = sh.most + side * N;
     // columns' numbers, while nothing reads P
@@ -592,7 +590,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
         if (piece0 == 0) {
           sh.row[c] = static_cast<int>(p.row0 + token);
 #pragma unroll
-          for (int k = 0; k < (C::kSplit ? 2 : 1); ++k) {
+          for (int k = 0; k < 2; ++k) {
             sh.neg_a[k * N + c] = live ? INFINITY : 0.f;
             sh.most[k * N + c] = ordered(-INFINITY);
           }
@@ -651,13 +649,12 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
       fence_proxy_async_smem();
       if (n > 0) warp_arrive(sh.q_ready);
 
-      uint64_t l[C::kChunks][8];  // sums of weights, in pairs of columns
+      const bool mine = c0 < cols;
+      uint64_t l[8];  // sums of weights, in pairs of columns
 #pragma unroll
-      for (int i = 0; i < C::kChunks; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) l[i][e] = 0;
+      for (int e = 0; e < 8; ++e) l[e] = 0;
       // The tiles of this side: j0, j0 + kPBufs, ...
-      const int j0 = C::kSplit ? (side - it0) & 1 : 0;
+      const int j0 = (side - it0) & 1;
       float g = 1.f, shift = 0.f;  // e4m3: values' scales go times g = 2^-shift
       all_sync();  // the columns' numbers are there
       for (int j = j0; j < n; j += C::kPBufs) {
@@ -670,15 +667,13 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
         if (edge) {
           const int key_w = key - lane, left = vis_max - key_w;  // the warp's first key, keys from there on
           const uint32_t valid = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1u : 0u;
-          if (lane < 16 * C::kChunks && valid) win = tree_bits(a, sh.row[column(lane)], key_w - prefix) & valid;
+          if (lane < 16 && valid) win = tree_bits(a, sh.row[c0 + lane], key_w - prefix) & valid;
         }
-        // The columns of sixteen i whose rows do not see this thread's key, as bits.
-        auto unseen = [&](int i) -> uint32_t {
-          uint32_t r = 0;
+        uint32_t hidden = 0;  // columns whose rows do not see this thread's key (which may leave -inf to those that do)
+        if (edge) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) r |= ((__shfl_sync(0xFFFFFFFFu, win, 16 * i + e) >> lane) & 1u) << e;
-          return ~r;
-        };
+          for (int e = 0; e < 16; ++e) hidden |= (~(__shfl_sync(0xFFFFFFFFu, win, e) >> lane) & 1u) << e;
+        }
         hold(sh.s_ready[it & 1], it >> 1);
         tc_fence_after();
         float sk = 1.f, sv = 1.f, limit = kMost;
@@ -703,14 +698,10 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           sv = fmaf(sv, 0.f, sv) * g;  // an infinity becomes NaN
           limit = fminf(kMost, 15.f - fast_log2(fabsf(sv)));
         }
-        // Scores relative to a, in log2 units, of one sixteen of columns; and which rows do not see the
-        // key (which may leave a score of -inf to those that do).
+        // Scores relative to a, in log2 units.
         const uint64_t sk2 = pair(sk, sk), scale2 = pair(a.scale_log2, a.scale_log2);
-        // (Two sixteens of columns are fetched twice: held until the vote is over they went to the stack.)
-        float x[16];
-        uint32_t hidden = 0;
-        auto fetch = [&](int i) {
-          const int c0 = 16 * chunk_of(i);
+        float x[16], top = -INFINITY;
+        auto fetch = [&]() {
           uint32_t s[16];
           tmem_ld_x16(ts + c0, s);
           tmem_wait_x16(s);
@@ -730,139 +721,103 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
             unpair(s01, x[e], x[e + 1]);
             unpair(s23, x[e + 2], x[e + 3]);
           }
-          hidden = 0;
           if (edge) {
-            hidden = unseen(i);
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               if ((hidden >> e) & 1u) x[e] = -INFINITY;
           }
         };
-        float top = -INFINITY;
+        if (mine) {
+          fetch();
 #pragma unroll
-        for (int i = 0; i < C::kChunks; ++i)
-          if (16 * chunk_of(i) < cols) {
-            fetch(i);
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) top = max3(top, x[e], x[e + 1]);
-          }
+          for (int e = 0; e < 16; e += 2) top = max3(top, x[e], x[e + 1]);
+        }
         if (group_any<128>(group_bar, top > limit)) {
           // ------------------------------------------ a moves: the columns' maxima across keys
-#pragma unroll 1
-          for (int i = 0; i < C::kChunks; ++i) {
-            const int c0 = 16 * chunk_of(i);
-            if (c0 >= cols) break;
-            uint32_t s[16];
-            tmem_ld_x16(ts + c0, s);
-            tmem_wait_x16(s);
-            const uint32_t not_seen = edge ? unseen(i) : 0u;
-            float most = -INFINITY;  // lane e: column e's
+          uint32_t s[16];
+          tmem_ld_x16(ts + c0, s);
+          tmem_wait_x16(s);
+          float most = -INFINITY;  // lane e: column e's
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float z = __uint_as_float(s[e]) * sk * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) - limit;
-              if ((not_seen >> e) & 1u) z = -INFINITY;
-              const float largest = warp_max(z);
-              if ((lane & 15) == e) most = largest;
-            }
-            if (lane < 16 && most == most) atomicMax(&mosts[c0 + lane], ordered(most));
+          for (int e = 0; e < 16; ++e) {
+            float z = __uint_as_float(s[e]) * sk * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) - limit;
+            if ((hidden >> e) & 1u) z = -INFINITY;
+            const float largest = warp_max(z);
+            if ((lane & 15) == e) most = largest;
           }
+          if (lane < 16 && most == most) atomicMax(&mosts[c0 + lane], ordered(most));
           group_sync(group_bar);
           if (j >= C::kPBufs) {
             hold(sh.p_free[buf], p_use(it) - 1);
             tc_fence_after();
+            float shrink[16];
+            bool moved = false;
 #pragma unroll
-            for (int i = 0; i < C::kChunks; ++i) {
-              const int c0 = 16 * chunk_of(i);
-              if (c0 < cols) {
-                float shrink[16];
-                bool moved = false;
+            for (int e = 0; e < 16; ++e) {
+              const float was = -neg_a[c0 + e], now = from_ordered(mosts[c0 + e]);
+              shrink[e] = now > was ? fast_exp2(was - (now + kRoom)) : 1.f;
+              moved |= now > was;
+            }
+            if (moved) {  // the same for all threads
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float was = -neg_a[c0 + e], most = from_ordered(mosts[c0 + e]);
-                  shrink[e] = most > was ? fast_exp2(was - (most + kRoom)) : 1.f;
-                  moved |= most > was;
-                }
-                if (moved) {  // the same for all threads
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) l[i][e] = mul2(l[i][e], pair(shrink[2 * e], shrink[2 * e + 1]));
+              for (int e = 0; e < 8; ++e) l[e] = mul2(l[e], pair(shrink[2 * e], shrink[2 * e + 1]));
 #pragma unroll 1
-                  for (int h = 0; h < C::kPCols; h += N) {
-                    uint32_t o[16];
-                    const uint32_t to = tm_o + C::kPCols * buf + lanes + h + c0;
-                    tmem_ld_x16(to, o);
-                    tmem_wait_x16(o);
+              for (int h = 0; h < C::kPCols; h += N) {
+                uint32_t o[16];
+                const uint32_t to = tm_o + C::kPCols * buf + lanes + h + c0;
+                tmem_ld_x16(to, o);
+                tmem_wait_x16(o);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink[e]);
-                    tmem_st_x16(to, o);
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                  }
-                }
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink[e]);
+                tmem_st_x16(to, o);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
               }
             }
           }
           group_sync(group_bar);
-          if (t < 16 * C::kChunks) {
-            const int c = column(t);
-            const float most = from_ordered(mosts[c]);
-            if (most > -neg_a[c]) neg_a[c] = -(most + kRoom);
-            mosts[c] = ordered(-INFINITY);
+          if (t < 16) {
+            const float now = from_ordered(mosts[c0 + t]);
+            if (now > -neg_a[c0 + t]) neg_a[c0 + t] = -(now + kRoom);
+            mosts[c0 + t] = ordered(-INFINITY);
           }
           group_sync(group_bar);
-          if constexpr (C::kChunks == 1) {
-            if (16 * chunk_of(0) < cols) fetch(0);
-          }
+          fetch();
         }
+        tc_fence_before();
+        warp_arrive(sh.s_free[it & 1]);
         // ------------------------------------------ weights
-        if (C::kChunks == 1 || 16 * chunk_of(0) >= cols) {
-          tc_fence_before();
-          warp_arrive(sh.s_free[it & 1]);
-        }
         if (p_use(it) > 0) hold(sh.p_free[buf], p_use(it) - 1);
-        uint8_t* const prow = smem + C::kPAt + C::kPBytes * buf + t * 128;
-        auto put = [&](int c, const uint32_t (&v)[8]) {  // at columns c .. c + 15
-          uint8_t* const block = prow + (c >> 6) * kBlock;
-          const int piece = (c & 63) >> 3;
-          *reinterpret_cast<uint4*>(block + ((piece ^ (t & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<uint4*>(block + (((piece + 1) ^ (t & 7)) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
-        };
-        const uint64_t sv2 = pair(sv, sv), minus = pair(-1.f, -1.f);
+        if (mine) {
+          uint8_t* const prow = smem + C::kPAt + C::kPBytes * buf + t * 128;
+          auto put = [&](int c, const uint32_t (&v)[8]) {  // at columns c .. c + 15
+            const int piece = c >> 3;
+            *reinterpret_cast<uint4*>(prow + ((piece ^ (t & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(prow + (((piece + 1) ^ (t & 7)) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
+          };
+          const uint64_t sv2 = pair(sv, sv), minus = pair(-1.f, -1.f);
+          uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int i = 0; i < C::kChunks; ++i) {
-          const int c0 = 16 * chunk_of(i);
-          if (c0 < cols) {
-            if constexpr (C::kChunks > 1) {
-              fetch(i);
-              if (i + 1 == C::kChunks || 16 * chunk_of(i + 1) >= cols) {  // this warpgroup's last
-                tc_fence_before();
-                warp_arrive(sh.s_free[it & 1]);
+          for (int e = 0; e < 8; ++e) {
+            uint64_t w = pair(fast_exp2(x[2 * e]), fast_exp2(x[2 * e + 1]));
+            l[e] = add2(l[e], w);
+            float p0, p1;
+            if constexpr (kE4m3) {
+              w = mul2(w, sv2);
+              unpair(w, p0, p1);
+              if (edge) {  // a hidden key's scale may be anything
+                if ((hidden >> (2 * e)) & 1u) p0 = 0.f;
+                if ((hidden >> (2 * e + 1)) & 1u) p1 = 0.f;
               }
+              hi[e] = pack_f16(p0, p1);
+            } else {
+              unpair(w, p0, p1);
+              hi[e] = pack_bf16(p0, p1);
+              unpair(fma2(pair(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xFFFF0000u)), minus, w), p0, p1);
+              lo[e] = pack_bf16(p0, p1);
             }
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              uint64_t w = pair(fast_exp2(x[2 * e]), fast_exp2(x[2 * e + 1]));
-              l[i][e] = add2(l[i][e], w);
-              float p0, p1;
-              if constexpr (kE4m3) {
-                w = mul2(w, sv2);
-                unpair(w, p0, p1);
-                if (edge) {  // a hidden key's scale may be anything
-                  if ((hidden >> (2 * e)) & 1u) p0 = 0.f;
-                  if ((hidden >> (2 * e + 1)) & 1u) p1 = 0.f;
-                }
-                hi[e] = pack_f16(p0, p1);
-              } else {
-                unpair(w, p0, p1);
-                hi[e] = pack_bf16(p0, p1);
-                if constexpr (C::kTwoParts) {
-                  unpair(fma2(pair(__uint_as_float(hi[e] << 16), __uint_as_float(hi[e] & 0xFFFF0000u)), minus, w), p0, p1);
-                  lo[e] = pack_bf16(p0, p1);
-                }
-              }
-            }
-            put(c0, hi);
-            if constexpr (C::kTwoParts) put(N + c0, lo);
           }
+          put(c0, hi);
+          if constexpr (!kE4m3) put(N + c0, lo);
         }
         // ------------------------------------------ this side's values of the tile
         {
@@ -942,39 +897,33 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
       tc_fence_before();
       all_sync();  // nothing reads P any more, and O is whole
       tc_fence_after();
+      if (mine) {
+        float v[16];
 #pragma unroll
-      for (int i = 0; i < C::kChunks; ++i)
-        if (16 * chunk_of(i) < cols) {
-          float v[16];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) unpair(l[i][e], v[2 * e], v[2 * e + 1]);
-          const float sum = sum16(v);
-          if (!(lane & 1)) sums[(4 * side + quad) * N + 16 * chunk_of(i) + (lane >> 1)] = sum;
-        }
-      if (kE4m3 && sharer == 0 && t == 0) sh.shift[side] = n > j0 ? shift : -INFINITY;
+        for (int e = 0; e < 8; ++e) unpair(l[e], v[2 * e], v[2 * e + 1]);
+        const float sum = sum16(v);
+        if (!(lane & 1)) sums[(4 * side + quad) * N + c0 + (lane >> 1)] = sum;
+      }
+      if (kE4m3 && c0 == 0 && t == 0) sh.shift[side] = n > j0 ? shift : -INFINITY;
       const bool bad_page = n > 0 && sh.bad_page[part & 7], some_bad = !kE4m3 && n > 0 && sh.any_bad[part & 7];
       if (threadIdx.x == 0 && bad_page) paged_report(a.status);
       all_sync();
       float* const part_to = p.whole ? nullptr : part_at<DP, N>(ta.parts, blockIdx.x, tile0 == 0);
       const int ch = 32 * quad + lane;
-      if constexpr (kE4m3) shift = C::kSplit ? fmaxf(fmaxf(sh.shift[0], sh.shift[1]), -60.f) : fmaxf(sh.shift[0], -60.f);
+      if constexpr (kE4m3) shift = fmaxf(fmaxf(sh.shift[0], sh.shift[1]), -60.f);
       const float back = kE4m3 ? pow2(static_cast<int>(shift)) : 1.f;
       // is there anything in the O of P's buffers?
-      const bool have0 = C::kSplit ? n > ((0 - first_of) & 1) : n > 0, have1 = C::kSplit && n > ((1 - first_of) & 1);
+      const bool have0 = n > ((0 - first_of) & 1), have1 = n > ((1 - first_of) & 1);
       if (threadIdx.x < cols) {  // a thread settles a column: the weights of both accumulators, the sum and the place
         const int c = threadIdx.x;
         auto sum_of = [&](int of) {
           const float* x = sums + 4 * of * N + c;
           return (x[0] + x[N]) + (x[2 * N] + x[3 * N]);
         };
-        float f0 = 1.f, f1 = 0.f, top = -sh.neg_a[c], total = sum_of(0);
-        if constexpr (C::kSplit) {
-          const float a0 = top, a1 = -sh.neg_a[N + c];
-          top = fmaxf(a0, a1);
-          f0 = a0 == -INFINITY ? 1.f : fast_exp2(a0 - top);  // nothing seen: sums and O are 0, or NaN to stay
-          f1 = a1 == -INFINITY ? 1.f : fast_exp2(a1 - top);
-          total = f0 * total + f1 * sum_of(1);
-        }
+        const float a0 = -sh.neg_a[c], a1 = -sh.neg_a[N + c], top = fmaxf(a0, a1);
+        float f0 = a0 == -INFINITY ? 1.f : fast_exp2(a0 - top);  // nothing seen: sums and O are 0, or NaN to stay
+        float f1 = a1 == -INFINITY ? 1.f : fast_exp2(a1 - top);
+        float total = f0 * sum_of(0) + f1 * sum_of(1);
         if (bad_page || !alive) total = __uint_as_float(0x7FC00000u);
         float inv = total == 0.f ? 0.f : 1.f / total;
         int64_t place = 3 * N + c * DP;
@@ -988,7 +937,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           place = static_cast<int64_t>(sh.row[c]) * a.out_ld + (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d;
         }
         places[c] = place;
-        if constexpr (kE4m3 && C::kSplit) {
+        if constexpr (kE4m3) {
           f0 *= fast_exp2(sh.shift[0] - shift);
           f1 *= fast_exp2(sh.shift[1] - shift);
         }
@@ -996,8 +945,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
         weights[N + c] = f1 * inv;
       }
       all_sync();
-#pragma unroll 1
-      for (int c0 = 16 * wg; c0 < cols; c0 += 64) {
+      if (side == 0 && mine) {
         float y[16] = {};
 #pragma unroll
         for (int b = 0; b < C::kPBufs; ++b)
@@ -1132,13 +1080,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
   }
 }
 
-// Whether blocks take shares of all steps: not where, were every sequence as long as its table
-// allows, a block would have a few only.
+// Whether blocks take shares of all steps: not where, were every sequence as long as its table allows, a
+// block would have a few only and a unit is short.  (Shares cost 4 to 6 us: one sequence, 16 heads of 128
+// channels, bf16, over 1024, 2048 and 4096 tokens 14.0, 20.1 and 32.6 us whole, 16.8, 17.4 and 20.1 shared.)
 bool shares_steps(const PagedArgs& a, int n, int64_t* units) {
   const int64_t row_units = (static_cast<int64_t>(a.max_q) * a.group + n - 1) / n;
   *units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
-  return *units * steps > 6 * static_cast<int64_t>(device_sm_count());
+  return *units * steps > 6 * static_cast<int64_t>(device_sm_count()) || steps >= 2 * kLeastShare;
 }
 
 // Lets the kernel have its shared memory, and checks that the launch brings the registers that the
