@@ -6,7 +6,8 @@
 //
 // Masks: a node's row has its own bit and its ancestors'.  Up to 128 nodes by doubling, in log2(depth) rounds;
 // beyond, a thread per node walks up: since parents have lower numbers the bits come in
-// descending order, a word at a time.
+// descending order, a word at a time.  Latency: one tree of 16 nodes 2.1 us, 64 of 33 to 128 2.9 (walking up
+// 6.4).
 //
 // Walk: at node 0 a token t is drawn from the node's row of probabilities; where a child has t
 // the walk goes on from there, else it ends with t.  Given the tree t is distributed as
@@ -17,6 +18,8 @@
 // One row of V entries per step of the path is read.  A cluster of blocks shares it, each lane a
 // contiguous chunk (32 entries of 64400: one round of loads); the warps' sums go through distributed shared memory, the
 // warp whose piece holds the draw finds it and tells every block.
+// Latency, a row after the other: one tree over 32000 entries 6.7 us, 32 over 64400 with up to nine draws 14 (18
+// with a row's entries dealt out by single vectors).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -76,7 +76,7 @@ struct TreeCfg {
   // Codes of values arrive where their fp16 values go (128 channels: the second block), or behind it.
   static constexpr int kRawAt = kBlock;
   static constexpr int kVBytes = kHalves * kBlock + (kE4m3 && DP == 64 ? kTile * 64 : 0);
-  static constexpr int kStatic = 3072;  // at most
+  static constexpr int kStatic = 3 * 1024;  // at most
   // e4m3: scales of the keys and values of eight tiles: keys are up to kKStages + 2 tiles ahead of the softmax
   static constexpr int kScaleBytes = kE4m3 ? 2 * kTile * 4 : 0, kScaleSlots = 8;
   static constexpr int kLeft = kSmemLimit - 1024 - kStatic - kQBytes - kPBufs * kPBytes - kScaleSlots * kScaleBytes;
