@@ -43,24 +43,6 @@ constexpr int kFewRows = 16;
 // Rows that tree_attention.cu takes, and the blocks of rows of tree_attention_short.cu, which takes two.
 constexpr int kTreeRows = 32;
 
-// Whether tree_attention_short.cu takes a call of more than kFewRows rows: contexts, by the table's width,
-// of few steps of 128 keys for as many blocks as there are, so that a block with a unit of its own is through
-// about when the others are.  Measured with 128 channels, us, contexts all as long and ragged ones, this kernel and else:
-//   32 rows, bf16:   64 units over 1024 16.5 and 16.5 (else 14.1, 14.1), over 128 8.5 (9.4)
-//                    128 units over 1024 17.0 and 16.5 (24.9, 24.1), over 4096 61.0 and 56.7 (57.8, 41.7)
-//                    256 units over 2048 49.3 and 39.1 (60.2, 44.1), over 4096 86.8 and 67.9 (96.7, 65.9)
-//                    1024 units over 512 66.8 and 51.7 (74.7, 78.4)
-//   64 rows, bf16:   256 heads over 512 29.0 and 24.6 (31.5, 30.0), over 2048 73.3 and 47.3 (66.8, 45.6)
-//   64 rows, e4m3:   256 heads over 2048 78.0 and 48.1 (80.9, 54.4), over 4096 137.8 and 91.0 (136.2, 96.2)
-// More rows than 64 read the same keys too often: 128 rows of 128 heads over 128 tokens 20.3 (12.0).
-inline bool tree_is_short(const PagedArgs& a) {
-  const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-  const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + 127) / 128;
-  const int64_t units = static_cast<int64_t>(a.B) * a.H_kv;
-  if (rows <= kTreeRows) return 8 * steps < units;
-  return rows <= 2 * kTreeRows && steps <= (a.k_scale != nullptr ? 16 : 8) && 4 * steps <= units;
-}
-
 // One sequence as the device finds it.
 struct PagedSeq {
   int64_t row0;   // first row of q

@@ -1080,14 +1080,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
   }
 }
 
-// Whether blocks take shares of all steps: not where, were every sequence as long as its table allows, a
-// block would have a few only and a unit is short.  (Shares cost 4 to 6 us: one sequence, 16 heads of 128
-// channels, bf16, over 1024, 2048 and 4096 tokens 14.0, 20.1 and 32.6 us whole, 16.8, 17.4 and 20.1 shared.)
+// Whether blocks take shares of all steps, were every sequence as long as its table allows.  Where every
+// unit can have a block: from the length on where halves of units and their join cost less than the longest
+// unit, which is the later the more blocks have one.  (bf16, 16 heads of 128 channels, contexts all as long and
+// ragged, us whole and shared: 2 sequences of 1536 17.5, 17.2 and 18.3, 18.0, of 4096 33.5, 32.6 and 22.3, 21.5;
+// 8 of 2048 28.5, 21.1 and 35.6, 24.7, of 4096 47.1, 37.3 and 54.9, 38.1, of 6000 64.1, 50.4 and 72.3, 47.7.)
+// Else where a block gets more than a few steps.
 bool shares_steps(const PagedArgs& a, int n, int64_t* units) {
-  const int64_t row_units = (static_cast<int64_t>(a.max_q) * a.group + n - 1) / n;
+  const int64_t row_units = (static_cast<int64_t>(a.max_q) * a.group + n - 1) / n, sms = device_sm_count();
   *units = static_cast<int64_t>(a.B) * a.H_kv * row_units;
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
-  return *units * steps > 6 * static_cast<int64_t>(device_sm_count()) || steps >= 2 * kLeastShare;
+  if (*units <= sms) return steps * sms > 8 * sms + 28 * *units;
+  return *units * steps > 6 * sms;
 }
 
 // Lets the kernel have its shared memory, and checks that the launch brings the registers that the

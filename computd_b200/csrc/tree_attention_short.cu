@@ -746,6 +746,24 @@ cudaError_t launch_short(const PagedArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+// Whether a call of more than kFewRows rows comes here: where there are more units than SMs, and contexts, by
+// the table's width, are short for that, so that a block with a unit of its own is through about when the
+// others are; and where a unit is one step.  Measured with 128 channels, us, contexts all as long and ragged
+// ones, here and else:
+//   32 rows, bf16:   128 units over 128 8.8 and 9.0 (else 9.4, 9.5), over 1024 17.3 and 16.7 (14.9, 14.4)
+//                    256 units over 1024 30.6 and 20.3 (39.6, 29.0), over 4096 86.8 and 67.9 (94.2, 63.9)
+//                    1024 units over 512 67.0 and 51.7 (72.3, 73.2), over 2048 183 and 101 (180, 109)
+//   64 rows, bf16:   256 heads over 512 29.0 and 24.6 (31.5, 30.0), over 2048 73.3 and 47.3 (66.8, 45.6)
+//   64 rows, e4m3:   256 heads over 2048 78.0 and 48.1 (80.9, 54.4), over 4096 137.8 and 91.0 (136.2, 96.2)
+// More rows than 64 read the same keys too often: 128 rows of 128 heads over 128 tokens 20.3 (12.0).
+bool tree_is_short(const PagedArgs& a) {
+  const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
+  const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
+  const int64_t units = static_cast<int64_t>(a.B) * a.H_kv;
+  if (rows <= kTreeRows) return steps <= 1 || (units > device_sm_count() && 8 * steps < units);
+  return rows <= 2 * kTreeRows && steps <= (a.k_scale != nullptr ? 16 : 8) && 4 * steps <= units;
+}
+
 cudaError_t launch_tree_attention_short(const PagedArgs& a, cudaStream_t stream) {
   const bool e4m3 = a.k_scale != nullptr;
   if (a.d <= 64) return e4m3 ? launch_short<true, 64>(a, stream) : launch_short<false, 64>(a, stream);
