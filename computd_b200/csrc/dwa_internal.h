@@ -221,6 +221,7 @@ cudaError_t launch_paged_attention_mma(const PagedArgs& a, cudaStream_t stream);
 cudaError_t launch_paged_tree_attention(const PagedArgs& a, void* workspace, cudaStream_t stream);
 cudaError_t launch_tree_attention(const PagedArgs& a, void* workspace, cudaStream_t stream);  // many rows
 size_t tree_attention_workspace(const PagedArgs& a);
+bool tree_has_room(const PagedArgs& a);
 bool tree_is_short(const PagedArgs& a);
 cudaError_t launch_tree_attention_short(const PagedArgs& a, cudaStream_t stream);  // short contexts
 cudaError_t launch_verify_drafts(const void* target, const void* draft, int probs_bf16,

@@ -845,10 +845,10 @@ cudaError_t launch_paged_attention(const PagedArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_paged_tree_attention(const PagedArgs& a, void* workspace, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-  return rows <= kFewRows    ? launch_few_rows<true>(a, stream)
-         : tree_is_short(a)  ? launch_tree_attention_short(a, stream)
-         : rows <= kTreeRows ? launch_tree_attention(a, workspace, stream)
-                             : launch_paged_attention_mma(a, stream);
+  return rows <= kFewRows   ? launch_few_rows<true>(a, stream)
+         : tree_is_short(a) ? launch_tree_attention_short(a, stream)
+         : tree_has_room(a) ? launch_tree_attention(a, workspace, stream)
+                            : launch_paged_attention_mma(a, stream);
 }
 
 }  // namespace dwa

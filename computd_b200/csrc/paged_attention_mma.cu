@@ -64,6 +64,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <mutex>
 #include <type_traits>
@@ -1305,24 +1306,27 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   // How many blocks share a unit's keys: what takes clearly the fewest rounds of steps
   // (a step is 3000 to 3900 cycles), if every sequence were as long as the table allows.  A
   // block costs about three steps more than its keys, a split one six and more: its
-  // part goes through distributed shared memory.  Trees of sequences at different points of
-  // their answers: there the longest unit takes its time whatever the others do, and with the longest first
-  // all are through about a third of a unit behind the mean of half the table's length.  (16 trees of 33 to 64
-  // nodes, 8 e4m3 heads of 4 query heads and 128 channels: over 2000 to 16384 tokens 278 us whole, 163 in two,
-  // 200 in four; over 16384 each 315, 324 and 355; over 2048 each 49, 69 and 102.)
+  // part goes through distributed shared memory.  Trees are of sequences at different points of their
+  // answers: there the longest unit takes its time whatever the others do, and with the longest first all are
+  // through about a third of a unit behind the mean of half the table's length; what gains more by this, in
+  // proportion, than it loses by the first.  (16 trees of 33 to 64 nodes, 8 e4m3 heads of 4 query heads and 128
+  // channels: over 2000 to 16384 tokens 278 us whole, 163 in two, 200 in four; over 16384 each 315, 324 and
+  // 355; over 2048 each 49, 69 and 102.  80 units of 64 rows over 3000 tokens each, bf16, 42 whole, 57 in two;
+  // ragged 41 and 33.)
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
-  auto cost_of = [&](int c, int64_t fit) -> int64_t {
+  auto cost_of = [&](int c, int64_t fit) -> double {
     const int64_t own = (steps + c - 1) / c, more = c == 1 ? 3 : 6 + c / 4;
-    if (!kTree || a.B == 1) return ((units + fit - 1) / fit) * (own + more);
-    return std::max(own + more, units * (own / 2 + more) / fit + own / 3);
+    const double equal = static_cast<double>((units + fit - 1) / fit * (own + more));
+    if (!kTree || a.B == 1) return equal;
+    return std::sqrt(equal * static_cast<double>(std::max(own + more, units * (own / 2 + more) / fit + own / 3)));
   };
   int cluster = 1;
-  int64_t best = cost_of(1, at_a_time[0]);
+  double best = cost_of(1, at_a_time[0]);
   for (int i = 1; 1 << i <= kMaxSplit; ++i) {
     const int c = 1 << i;
     if (at_a_time[i] < 1) break;
-    const int64_t cost = cost_of(c, at_a_time[i]);
-    if (10 * cost < 9 * best) {
+    const double cost = cost_of(c, at_a_time[i]);
+    if (10.0 * cost < (kTree ? 9.2 : 9.0) * best) {
       best = cost;
       cluster = c;
     }

@@ -761,7 +761,7 @@ bool tree_is_short(const PagedArgs& a) {
   const int64_t steps = ((static_cast<int64_t>(a.max_pages) << a.page_log2) + kTile - 1) / kTile;
   const int64_t units = static_cast<int64_t>(a.B) * a.H_kv;
   if (rows <= kTreeRows) return steps <= 1 || (units > device_sm_count() && 8 * steps < units);
-  return rows <= 2 * kTreeRows && steps <= (a.k_scale != nullptr ? 16 : 8) && 4 * steps <= units;
+  return rows <= 2 * kTreeRows && steps <= (a.k_scale != nullptr ? 16 : 8) && 4 * steps <= units && !tree_has_room(a);
 }
 
 cudaError_t launch_tree_attention_short(const PagedArgs& a, cudaStream_t stream) {

@@ -154,7 +154,7 @@ DWA_API dwa_status dwa_tree_masks(const int32_t* parents, const int32_t* q_start
  * length - n tokens, and to node j (token length - n + j) where bit j of its row of tree_mask
  * (uint64 [T][mask_words], 8-byte aligned) is set.  Any bits may be; those from n on count for nothing.
  * max_q is 64 mask_words at most.  All else as there, but the rounding of 17 to 32 rows per
- * key/value head, and of up to 64 where tables are narrow for the number of sequences: bf16 caches none (p_j as
+ * key/value head, and of up to 64 over narrow tables: bf16 caches none (p_j as
  * the sum of two bf16), e4m3 caches p_j times its value's scale to 11 bits, and q to 2^-18 of its
  * row's largest value.  workspace: 16-byte aligned, of
  * dwa_paged_tree_attention_workspace bytes (0: none) for the current device; it holds nothing between calls.
