@@ -1091,6 +1091,9 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
       go(std::bool_constant<kE4m3>{});
     }
     if (steps > 0 && alive) alive = warp_wait(sh.p_free[i], steps - 1);
+    // (Q's rows come from all warps: one whose tile has no keys may be here before they are in place, and goes
+    // through them on its way out.)
+    if (steps == 0 && alive) alive = warp_wait(sh.q_ready, 0);
     tc_fence_after();
     // ---------------------------------------------- out
     const bool have = steps > 0 && alive;

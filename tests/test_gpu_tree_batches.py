@@ -51,6 +51,27 @@ def test_more_trees_than_are_ranked(kind, rows):
     check(attend(cache, q, new, seen), *tree_attention_64(q, cache, starts(new), seen))
 
 
+@pytest.mark.parametrize("d,heads,kv_heads,most", [(112, 64, 16, 100), (80, 192, 24, 33), (128, 16, 16, 200), (64, 64, 16, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_sequences_without_cached_tokens_get_zeros(d, heads, kv_heads, most, causal):
+    """Among many others, of more rows than one block takes at once."""
+    import computd_b200 as cb
+
+    rng = random.Random(d)
+    new = [rng.randint(most // 2, most) for _ in range(140)]
+    lengths = [0 if rng.random() < 0.5 else rng.randint(1, 130) for _ in new]
+    cache = Cache("bf16", lengths, kv_heads, d, 64, seed=d)
+    q = torch.randn((sum(new), heads, d), device="cuda", generator=_gen(d)).to(BF16)
+    start, mask = _i32(starts(new)), None if causal else words_of(masks_of(new, "tree", 3), -(-most // 64))
+    empty = torch.repeat_interleave(cache.len == 0, torch.tensor(new, device="cuda"))
+    for _ in range(5):
+        if causal:
+            got = cb.paged_attention(q, cache.k, cache.v, cache.table, cache.len, q_start=start, max_q=most)
+        else:
+            got = cb.paged_tree_attention(q, cache.k, cache.v, cache.table, cache.len, mask, q_start=start, max_q=most)
+        assert bool((got[empty] == 0).all()) and not bool(torch.isnan(got).any())
+
+
 @pytest.mark.parametrize("rows", [24, 60, 128, 300])
 @pytest.mark.parametrize("lengths", [[700] * 3, [5000, 130, 2100], [20000], [1300, 9000, 1, 400]])
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
