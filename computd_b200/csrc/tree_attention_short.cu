@@ -20,8 +20,8 @@
 // step is a chain of product, vote, exponentials, product.  So two blocks share an SM, each with half of
 // its shared memory and registers, and none has more to find out than its own sequence: no shares, no
 // parts to join.  16 sequences of 32 nodes, 16 heads of 128 channels, over 128 and 1024 tokens: bf16 11 and
-// 30 us, e4m3 12 and 26; a block to an SM that shares out the steps 18 and 42, 18 and 41.  24 ragged ones of 5 to 40
-// nodes over 50 to 1500 tokens, 16 heads of 80, e4m3: 47 us, 66 in tiles of 128 rows.  Long contexts
+// 30 us, e4m3 12 and 26; a block to an SM that shares out the steps 17 and 40, 18 and 38.  24 ragged ones of 5 to 40
+// nodes over 50 to 1500 tokens, 16 heads of 80, e4m3: 45 us, 66 in tiles of 128 rows.  Long contexts
 // turn this round: the longest unit has a block to itself (see tree_is_short).
 //
 // Eight warps: softmax, sixteen columns to each four; e4m3: they turn the values' codes into fp16 too.  One warp:
