@@ -2,8 +2,9 @@
 // sequence's earlier tokens: token start + path[i] to start + i, in every layer.
 //
 // Latency first (a few tokens per sequence): one launch for all layers, heads, keys and
-// values.  Node numbers ascend along a path, so a place is never below the number of the token that moves
-// there, and a token moves before its own place is needed: a thread that moves a
+// values.  Node numbers ascend along a path from 0 or more, so a place i is never above the number of the node
+// that moves there (which every thread checks of its own nodes before it looks up their pages), and a token
+// moves before its own place is needed: a thread that moves a
 // vector's 16 bytes of one token after the other needs no second copy of them.  32 paths of up to 12 tokens in
 // 12 layers of 16 8-bit heads of 128: 9.0 us, 2.3 TB/s of scattered 128-byte rows, two dependent rounds of loads
 // (path and table, then the rows) before the stores.
@@ -81,7 +82,8 @@ __global__ void __launch_bounds__(kThreads) kv_keep_kernel(const KeepArgs a) {
   bool bad = n >= a.steps || start < 0;
   for (int i = threadIdx.x; i <= n && !bad; i += kThreads) {
     const int64_t node = i == own ? own_node : __ldg(path + i), before = i == own ? own_before : __ldg(path + i - 1);
-    bad = node <= before || start + node >= tokens;
+    // With i <= node both lookups are inside the table, whatever the rest of the path says.
+    bad = node <= before || node < i || start + node >= tokens;
     if (bad || node == i) continue;
     const int64_t p = __ldg(table + ((start + node) >> a.page_log2)), q = __ldg(table + ((start + i) >> a.page_log2));
     bad = p < 0 || p >= a.n_pages || q < 0 || q >= a.n_pages;
