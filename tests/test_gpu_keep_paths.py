@@ -1,10 +1,17 @@
-"""GPU: kv_cache_keep of bad paths of many nodes."""
+"""GPU: kv_cache_keep of paths longer than a look at three nodes, of one layer by itself, and in
+caches whose pages and layers lie apart."""
+import random
+
 import pytest
 import torch
-from test_gpu_decode import BF16
+from test_gpu_decode import BF16, E4M3, quantise
 from test_gpu_draft_trees import _gen, _i32, keep_plain
 
 pytestmark = pytest.mark.gpu
+
+
+def _bytes(x):
+    return x.view(torch.uint8) if x.dtype == E4M3 else x
 
 
 def _bad_path(which, n):
@@ -43,3 +50,42 @@ def test_bad_paths_are_reported_and_move_nothing(which, n, start, pages_of):
     status = torch.zeros((), dtype=torch.int32, device="cuda")
     cb.kv_cache_keep(k, v, table, _i32([start] * 2), _i32(rows), _i32(kept), status=status)
     assert int(status) == 5 and torch.equal(k, want[0][0]) and torch.equal(v, want[1][0])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("layers", [None, 1, 3])
+@pytest.mark.parametrize("H,d,page,n,steps", [(2, 80, 16, 40, 7), (1, 16, 128, 600, 300), (3, 128, 32, 64, 12)])
+def test_layers_and_pages_that_lie_apart(kind, layers, H, d, page, n, steps):
+    """`layers` None: one layer's caches, of four dimensions.  Nothing between the pages changes."""
+    import computd_b200 as cb
+
+    rng = random.Random(n)
+    B, each = 4, -(-(n + 20) // page) + 1
+    L, pages = layers or 1, B * each + 1
+    wide = []
+    for seed in (1, 2):
+        x = torch.randn((L, 2, pages, 3, H, page, d), device="cuda", generator=_gen(seed)).to(BF16)
+        wide.append(x)
+    if kind == "e4m3":
+        (k, ks), (v, vs) = quantise(wide[0]), quantise(wide[1])
+        wide = [k, v, ks, vs]
+    before = [x.clone() for x in wide]
+    views = [x[:, 1, :, 2] for x in wide]  # every other layer, every third page
+    assert not any(x.is_contiguous() for x in views)
+    table = torch.randperm(pages, device="cuda", generator=_gen(3))[:B * each].view(B, each).int()
+    start = [rng.randrange(20) for _ in range(B)]
+    kept = [min(steps, n) - 1, -1, rng.randrange(1, steps), rng.randrange(1, steps)]
+    path = [sorted(rng.sample(range(n), max(m, 0) + 1)) for m in kept]
+    want = [x.clone() for x in views]
+    keep_plain(want, table.tolist(), start, path, kept, page)
+    assert not torch.equal(_bytes(want[0]), _bytes(views[0]))
+    status = torch.zeros((), dtype=torch.int32, device="cuda")
+    args = views if layers else [x[0] for x in views]
+    scales = dict(zip(("k_scale", "v_scale"), args[2:]))
+    cb.kv_cache_keep(args[0], args[1], table, _i32(start), _i32([p + [-1] * (steps - len(p)) for p in path]),
+                     _i32(kept), status=status, **scales)
+    assert int(status) == 0
+    for x, y, w, old in zip(views, want, wide, before):
+        assert torch.equal(_bytes(x), _bytes(y))
+        x.copy_(old[:, 1, :, 2])
+        assert torch.equal(_bytes(w), _bytes(old))
