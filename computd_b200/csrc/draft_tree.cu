@@ -38,6 +38,7 @@ namespace {
 constexpr int kMaskThreads = 128;
 constexpr int kMostNodes = 4096;  // of a tree
 constexpr int kShortWords = 2;    // up to 128 nodes
+constexpr int kRowBits = 8192;    // rows that are told apart at a time where a range is bad
 
 struct MaskArgs {
   const int32_t *parents, *q_start;
@@ -47,8 +48,49 @@ struct MaskArgs {
   int32_t *depth, *status;
 };
 
-__global__ void __launch_bounds__(kMaskThreads) tree_masks_kernel(const MaskArgs a) {
-  extern __shared__ int32_t up[];  // this sequence's parents
+// Sequence b's rows; whether they are any.
+__device__ __forceinline__ bool rows_of(const MaskArgs& a, int b, int64_t* lo, int64_t* hi) {
+  *lo = __ldg(a.q_start + b);
+  *hi = __ldg(a.q_start + b + 1);
+  return *lo >= 0 && *lo <= *hi && *hi <= a.T;
+}
+// Whether one of sequences 0 .. n - 1 has a range that is none; the block together.
+__device__ __forceinline__ bool any_bad_range(const MaskArgs& a, int n) {
+  bool bad = false;
+  for (int i = threadIdx.x; i < n && !bad; i += kMaskThreads) {
+    int64_t lo, hi;
+    bad = !rows_of(a, i, &lo, &hi);
+  }
+  return __syncthreads_or(bad);
+}
+// Zeros to the rows that no sequence has, wherever they are: kRowBits rows at a time the ranges set their bits.
+__device__ __noinline__ void clear_free_rows(const MaskArgs& a) {
+  __shared__ uint32_t taken[kRowBits / 32];
+  for (int64_t first = 0; first < a.T; first += kRowBits) {
+    for (int i = threadIdx.x; i < kRowBits / 32; i += kMaskThreads) taken[i] = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < a.B; b += kMaskThreads) {
+      int64_t lo, hi;
+      if (!rows_of(a, b, &lo, &hi)) continue;
+      const int from = static_cast<int>(min(max(lo - first, int64_t{0}), int64_t{kRowBits}));
+      const int to = static_cast<int>(min(max(hi - first, int64_t{0}), int64_t{kRowBits}));
+      for (int t = from; t < to; t = (t | 31) + 1) {
+        const int n = min(to - t, 32 - (t & 31));
+        atomicOr(&taken[t >> 5], (n == 32 ? 0xFFFFFFFFu : (1u << n) - 1u) << (t & 31));
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(a.T - first, int64_t{kRowBits}); i += kMaskThreads) {
+      if ((taken[i >> 5] >> (i & 31)) & 1u) continue;
+      for (int w = 0; w < a.words; ++w) a.mask[(first + i) * a.words + w] = 0;
+      a.depth[first + i] = 0;
+    }
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(kMaskThreads) tree_masks_kernel(const __grid_constant__ MaskArgs a) {
+  extern __shared__ __align__(16) int32_t up[];  // this sequence's parents
   const int b = blockIdx.x;
   int64_t lo = static_cast<int64_t>(b) * a.even, hi = lo + a.even;
   auto clear = [&](int64_t from, int64_t to) {  // rows of no sequence see nothing
@@ -58,14 +100,16 @@ __global__ void __launch_bounds__(kMaskThreads) tree_masks_kernel(const MaskArgs
     }
   };
   if (a.q_start != nullptr) {
-    lo = __ldg(a.q_start + b);
-    hi = __ldg(a.q_start + b + 1);
-    const bool fine = lo >= 0 && lo <= hi && hi <= a.T;
-    if (b == 0) clear(0, min(max(lo, int64_t{0}), a.T));
-    if (b == a.B - 1) clear(min(max(hi, int64_t{0}), a.T), a.T);
-    if (!fine) {  // rows that cannot be told apart stay as they are
+    const bool fine = rows_of(a, b, &lo, &hi);
+    if (!fine) {  // the first such sequence's block sees to all rows of no sequence
       if (threadIdx.x == 0) paged_report(a.status);
+      if (!any_bad_range(a, b)) clear_free_rows(a);
       return;
+    }
+    const bool ends = (b == 0 && lo > 0) || (b == a.B - 1 && hi < a.T);
+    if (ends && !any_bad_range(a, a.B)) {  // ranges follow one another: rows of no sequence are before and behind
+      if (b == 0) clear(0, lo);
+      if (b == a.B - 1) clear(hi, a.T);
     }
   }
   if (hi - lo > a.max_q) {
