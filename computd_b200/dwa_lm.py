@@ -214,6 +214,8 @@ class CausalSelfAttention(nn.Module):
         their keys and values go into the cache, their queries attend to it."""
         _, T, C = x.shape
         qkv = self.qkv(self.norm(x))
+        if qkv.dtype != torch.bfloat16 or step.cos.dtype != torch.bfloat16:  # as forward's rope_qk: before pages change
+            raise ValueError(f"qkv and cos / sin must be bf16 (got {qkv.dtype} and {step.cos.dtype})")
         q, k, v = (qkv[0, :, i * C:(i + 1) * C].view(T, self.h, self.dh) for i in range(3))
         # rotated as forward's rope_qk does, bit for bit
         q = step.cache.append(layer, q, k, v, step.cos, step.sin, step.slots)
