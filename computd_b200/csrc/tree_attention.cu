@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           sh.row[c] = static_cast<int>(p.row0 + token);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            sh.neg_a[k * N + c] = live ? INFINITY : 0.f;
+            sh.neg_a[k * N + c] = live ? kUnset : 0.f;
             sh.most[k * N + c] = ordered(-INFINITY);
           }
         }
@@ -921,8 +921,7 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           return (x[0] + x[N]) + (x[2 * N] + x[3 * N]);
         };
         const float a0 = -sh.neg_a[c], a1 = -sh.neg_a[N + c], top = fmaxf(a0, a1);
-        float f0 = a0 == -INFINITY ? 1.f : fast_exp2(a0 - top);  // nothing seen: sums and O are 0, or NaN to stay
-        float f1 = a1 == -INFINITY ? 1.f : fast_exp2(a1 - top);
+        float f0 = fast_exp2(a0 - top), f1 = fast_exp2(a1 - top);  // nothing seen: sums and O are 0, or NaN to stay
         float total = f0 * sum_of(0) + f1 * sum_of(1);
         if (bad_page || !alive) total = __uint_as_float(0x7FC00000u);
         float inv = total == 0.f ? 0.f : 1.f / total;
@@ -1047,22 +1046,18 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
       const float2 v = *reinterpret_cast<const float2*>(x + 3 * N + r * DP + 2 * lane);
       o[0] = v.x; o[1] = v.y;
     }
-    // a part whose keys the row does not see has no reference and l = 0 (or NaN, which has to stay)
+    // a part whose keys the row does not see has the least reference and l = 0 (or NaN, which has to stay)
     if (ref > top) {
       sum *= fast_exp2(top - ref);
       top = ref;
     }
-    float f = 1.f, back = 1.f;
-    if (ref != -INFINITY) {
-      if (o_ref > o_top) {
-        back = fast_exp2(o_top - o_ref);
-        o_top = o_ref;
-      }
-      f = fast_exp2(o_ref - o_top);
-      sum = fmaf(fast_exp2(ref - top), l, sum);
-    } else {
-      sum += l;
+    float back = 1.f;
+    if (o_ref > o_top) {
+      back = fast_exp2(o_top - o_ref);
+      o_top = o_ref;
     }
+    const float f = fast_exp2(o_ref - o_top);
+    sum = fmaf(fast_exp2(ref - top), l, sum);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) y[k] = fmaf(f, o[k], back * y[k]);
   }

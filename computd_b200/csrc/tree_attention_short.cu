@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
       }
       if (piece0 == 0) {
         sh.row[c] = static_cast<int>(p.seq.row0 + token);
-        sh.neg_a[c] = live ? INFINITY : 0.f;
+        sh.neg_a[c] = live ? kUnset : 0.f;
         sh.most[c] = ordered(-INFINITY);
       }
       if constexpr (kE4m3) {

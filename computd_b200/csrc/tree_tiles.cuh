@@ -13,6 +13,9 @@ namespace {
 
 constexpr int kTile = 128;           // keys per step
 constexpr int kBlock = kTile * 128;  // bytes of 128 rows of 128 bytes
+// Minus the reference of a column that has seen no score yet: any score moves it, but a score of minus infinity
+// (from which minus infinity could not be subtracted) keeps the weight 0.
+constexpr float kUnset = 0x1.FFFFFEp127f;
 
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
