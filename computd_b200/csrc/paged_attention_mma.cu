@@ -127,7 +127,8 @@ struct MmaCfg {
   static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kStageBytes;
   // at the end a split block's parts take Q's and the operands' place
   static constexpr int kPartMl = 2 * kTile * DP * 4;    // behind O
-  static constexpr int kPartBytes = kPartMl + 2 * kTile * 8;
+  static constexpr int kPartUnit = kPartMl + 2 * kTile * 8;  // e4m3
+  static constexpr int kPartBytes = kPartUnit + (kE4m3 ? 2 * kTile * 4 : 0);
   static_assert(kPartBytes <= 2 * kTileBytes + kStages * kStageBytes, "parts fit");
 };
 
@@ -337,7 +338,7 @@ __device__ __forceinline__ void regs_dec() {
 template <bool kE4m3, int DP, bool kTree>
 __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const PagedArgs a, const int row_units, const int cluster) {
+                     const __grid_constant__ PagedArgs a, const int row_units, const int cluster) {
   using C = MmaCfg<kE4m3, DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ MmaShared<kE4m3> sh;
@@ -1100,10 +1101,10 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
     if (!alive || sh.bad_page) l = __uint_as_float(0x7FC00000u);
     if (sh.bad_page && threadIdx.x == 0) paged_report(a.status);
     // O is in units of P's power of two, which l has too, and of the values'
-    const float v_back = !kE4m3 ? 1.f
-                         : rest ? pow2(v_exp - static_cast<int>(kPBits))
-                                : sh.v_ref / kCodeScale;
     if (cluster == 1) {
+      const float v_back = !kE4m3 ? 1.f
+                           : rest ? pow2(v_exp - static_cast<int>(kPBits))
+                                  : sh.v_ref / kCodeScale;
       // through this warp's rows of Q's tile, which no product needs any more, so that
       // rows leave whole (a row per thread at 16 bytes a store took 7 us per block)
       const float inv = 1.f / l;
@@ -1170,11 +1171,14 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           const uint32_t dst = there + (((slot >> 5) * (DP / 4) + 8 * c) * 32 + (slot & 31)) * 16;
 #pragma unroll
           for (int k = 0; k < 32; k += 4)
-            st_cluster_f32x4(dst + 128 * k, o[k] * v_back, o[k + 1] * v_back, o[k + 2] * v_back,
-                             o[k + 3] * v_back);
+            st_cluster_f32x4(dst + 128 * k, o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
       st_cluster_f32x2(there + C::kPartMl + 8 * slot, l == 0.f ? -INFINITY : -ref, l);
+      // the values' power of two goes with a part, not into it: sums that are not yet divided by l would leave f32
+      if constexpr (kE4m3)
+        st_cluster_s32(there + C::kPartUnit + 4 * slot,
+                       rest ? v_exp - static_cast<int>(kPBits) : exponent_of(sh.v_ref / kCodeScale));
       if (sh.any_bad) {
         for (int at = threadIdx.x; at < cluster * kBads; at += 256)
           min_cluster_s32(map_to_cta(smem_u32(&sh.first_bad[at % kBads]), at / kBads), sh.first_bad[at % kBads]);
@@ -1192,6 +1196,17 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         for (int c = 0; c < cluster; ++c)
           top = fmaxf(top, *reinterpret_cast<const float*>(smem + C::kPartMl + 8 * ((c << log2_rows) + row)));
         float y[DP / 16][4] = {};
+        // y is in units of 2^unit, about the largest of the parts' units times their weights
+        int unit = -4096;
+        if constexpr (kE4m3) {
+          for (int c = 0; c < cluster; ++c) {
+            const int at = (c << log2_rows) + row;
+            const float m = *reinterpret_cast<const float*>(smem + C::kPartMl + 8 * at);
+            if (m > -INFINITY)
+              unit = max(unit, *reinterpret_cast<const int*>(smem + C::kPartUnit + 4 * at) +
+                                   static_cast<int>(fmaxf(m - top, -1024.f)));
+          }
+        }
 #pragma unroll 1
         for (int c = 0; c < cluster; ++c) {
           const int at = (c << log2_rows) + row;
@@ -1203,18 +1218,36 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
           // a part without keys has l = 0 (or NaN, which has to stay)
           const float weight = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
           sum += ml.x == -INFINITY ? ml.y : weight * ml.y;
-          if (weight != 0.f) {  // else what is there may be anything
+          float of_o = weight;
+          if constexpr (kE4m3)
+            of_o = ml.x == -INFINITY ? 0.f
+                                     : fast_exp2((ml.x - top) + static_cast<float>(
+                                           *reinterpret_cast<const int*>(smem + C::kPartUnit + 4 * at) - unit));
+          if (of_o != 0.f) {  // else what is there may be anything
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
-              y[t][0] += weight * o[t].x;
-              y[t][1] += weight * o[t].y;
-              y[t][2] += weight * o[t].z;
-              y[t][3] += weight * o[t].w;
+              y[t][0] += of_o * o[t].x;
+              y[t][1] += of_o * o[t].y;
+              y[t][2] += of_o * o[t].z;
+              y[t][3] += of_o * o[t].w;
             }
           }
         }
         if (row >= row_end) continue;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if constexpr (kE4m3) {  // in two steps: the unit has more than f32's exponents
+          unit = min(max(unit, -250), 250);
+          const float one = inv * pow2(unit / 2), two = pow2(unit - unit / 2);
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[t][e] = y[t][e] * one * two;
+        } else {
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[t][e] *= inv;
+        }
         const uint32_t of_unit = row_0 + (split << log2_rows) + row, token = row_token(of_unit, a.group);
         uint16_t* const out = a.out + (seq.row0 + token) * a.out_ld +
                               (static_cast<int64_t>(hk) * a.group + of_unit - token * a.group) * a.d + 4 * x;
@@ -1232,7 +1265,7 @@ __global__ void __launch_bounds__(MmaCfg<kE4m3, DP>::kThreads, 1)
         for (int t = 0; t < DP / 16; ++t)
           if (16 * t < a.d)  // d is a multiple of 16
             *reinterpret_cast<uint2*>(out + 16 * t) =
-                make_uint2(pack_bf16(y[t][0] * inv, y[t][1] * inv), pack_bf16(y[t][2] * inv, y[t][3] * inv));
+                make_uint2(pack_bf16(y[t][0], y[t][1]), pack_bf16(y[t][2], y[t][3]));
       }
     }
     tc_fence_before();
