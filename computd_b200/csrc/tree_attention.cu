@@ -14,7 +14,8 @@
 // What a row's weights are relative to, a, is not its maximum but anything that keeps them in
 // range; it moves when a score passes the limit, which every step asks by a vote, and only
 // then are maxima taken across keys.  The limit is 2^60 for bf16 (whose range is f32's) and for e4m3
-// what keeps a weight times its value's scale below 2^15 in fp16.
+// what keeps a weight times its value's scale below 2^15 in fp16.  Scores of 2^20 and more, and values' scales 2^90 apart,
+// take the careful steps of tree_tiles.cuh.
 //
 // Rounding: bf16 caches none beside f32 sums (P is the sum of two bf16 parts).  e4m3: codes are
 // exact; Q is, per row, a power of two times the sum of two e4m3 numbers, exactly down to 2^-9 of the
@@ -250,7 +251,9 @@ struct TreeShared {
   int most[2 * N];  // across keys, ordered
   int row[N];                   // of q
   uint32_t tops[4][4];          // e4m3: scales' exponents
-  float shift[2];               // of each side
+  float d[kE4m3 ? 2 * N : 4];   // e4m3: O's units are 2^d beside the references', of each side
+  float shrink_l[2 * N], shrink_o[2 * N];
+  int careful[4];               // of each warpgroup
 };
 
 struct TreeArgs {
@@ -259,7 +262,7 @@ struct TreeArgs {
   int row_units;  // blocks of rows of a sequence, at most (without parts)
 };
 
-// A part's place in the workspace: a, l and O's power of two by rows, then O.
+// A part's place in the workspace: a, l and the exponent of O's unit beside 2^a by rows, then O.
 template <int DP, int N>
 __device__ __forceinline__ float* part_at(float* parts, int block, bool begins) {
   return parts + (static_cast<int64_t>(block) * 2 + (begins ? 1 : 0)) * (N * (DP + 3));
@@ -541,9 +544,11 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
     float* const sums = reinterpret_cast<float*>(smem + C::kPAt);  // [side][quad][N]: of weights
     float* const weights = sums + 1024;                            // [side][N]: of the accumulators
     int64_t* const places = reinterpret_cast<int64_t*>(weights + 2 * N);
+    float* const halves = reinterpret_cast<float*>(places + N);    // e4m3: roots of O's units, which have more than f32's exponents
     // Where weights have to stay: e4m3 below 2^15 with their values' scales, and by themselves below
     // 2^105, so that their sums are f32; when a moves it leaves this much room.
-    constexpr float kMost = kE4m3 ? 105.f : 60.f, kRoom = kE4m3 ? 5.f : 60.f;
+    // (kLeast: where a value's scale is 2^90 and more beside 1 / g.)
+    constexpr float kMost = kE4m3 ? 105.f : 60.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 60.f;
     bool alive = true;
     auto hold = [&](const uint64_t& x, int phase) {  // after an abort nothing is waited for any more
       if (alive) alive = wait(x, phase);
@@ -587,12 +592,14 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           x[k] = make_uint4(0, 0, 0, 0);
           if (live && 8 * piece < a.d) x[k] = __ldg(reinterpret_cast<const uint4*>(src) + piece);
         }
+        if (threadIdx.x < 4) sh.careful[threadIdx.x] = 0;
         if (piece0 == 0) {
           sh.row[c] = static_cast<int>(p.row0 + token);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             sh.neg_a[k * N + c] = live ? kUnset : 0.f;
             sh.most[k * N + c] = ordered(-INFINITY);
+            if constexpr (kE4m3) sh.d[k * N + c] = 0.f;
           }
         }
         if constexpr (kE4m3) {
@@ -655,7 +662,8 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
       for (int e = 0; e < 8; ++e) l[e] = 0;
       // The tiles of this side: j0, j0 + kPBufs, ...
       const int j0 = (side - it0) & 1;
-      float g = 1.f, shift = 0.f;  // e4m3: values' scales go times g = 2^-shift
+      float g = 1.f;               // e4m3: values' scales go times g = 2^-d
+      bool careful = false;        // as tree_tiles.cuh has it
       all_sync();  // the columns' numbers are there
       for (int j = j0; j < n; j += C::kPBufs) {
         const int it = it0 + j, buf = p_buf(it);
@@ -692,11 +700,13 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
             group_sync(group_bar);
             const uint32_t most = max(max(sh.tops[wg][0], sh.tops[wg][1]), max(sh.tops[wg][2], sh.tops[wg][3]));
             const int e = most == 0 ? 0 : static_cast<int>(most >> 23) - 127;
-            shift = static_cast<float>(min(max(e, -60), 120));
-            g = pow2(-static_cast<int>(shift));
+            const int shift = min(max(e, -60), 120);
+            g = pow2(-shift);
+            if (t < 16) sh.d[side * N + c0 + t] = static_cast<float>(shift);
           }
           sv = fmaf(sv, 0.f, sv) * g;  // an infinity becomes NaN
-          limit = fminf(kMost, 15.f - fast_log2(fabsf(sv)));
+          limit = 15.f - fast_log2(fabsf(sv));
+          if (!(limit > kLeast && limit < kMost)) limit = -INFINITY;  // beyond what one g allows: any score asks
         }
         // Scores relative to a, in log2 units.
         const uint64_t sk2 = pair(sk, sk), scale2 = pair(a.scale_log2, a.scale_log2);
@@ -712,8 +722,8 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
             uint64_t s23 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
             if constexpr (kE4m3) {
               const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sh.f[c0 + e]);
-              s01 = fma2(mul2(s01, sk2), f.x, ref.x);
-              s23 = fma2(mul2(s23, sk2), f.y, ref.y);
+              s01 = fma2(mul2(s01, f.x), sk2, ref.x);
+              s23 = fma2(mul2(s23, f.y), sk2, ref.y);
             } else {
               s01 = fma2(s01, scale2, ref.x);
               s23 = fma2(s23, scale2, ref.y);
@@ -727,12 +737,12 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
               if ((hidden >> e) & 1u) x[e] = -INFINITY;
           }
         };
-        if (mine) {
+        if (mine && !careful) {
           fetch();
 #pragma unroll
           for (int e = 0; e < 16; e += 2) top = max3(top, x[e], x[e + 1]);
         }
-        if (group_any<128>(group_bar, top > limit)) {
+        if (!careful && group_any<128>(group_bar, top > limit)) {
           // ------------------------------------------ a moves: the columns' maxima across keys
           uint32_t s[16];
           tmem_ld_x16(ts + c0, s);
@@ -740,14 +750,17 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           float most = -INFINITY;  // lane e: column e's
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float z = __uint_as_float(s[e]) * sk * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) - limit;
+            float z = __uint_as_float(s[e]) * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) * sk - limit;
             if ((hidden >> e) & 1u) z = -INFINITY;
             const float largest = warp_max(z);
             if ((lane & 15) == e) most = largest;
           }
           if (lane < 16 && most == most) atomicMax(&mosts[c0 + lane], ordered(most));
+          if (most > -INFINITY && fabsf(most) >= kBig) sh.careful[wg] = 1;
           group_sync(group_bar);
-          if (j >= C::kPBufs) {
+          __syncwarp();
+          careful = *static_cast<volatile int*>(&sh.careful[wg]) != 0;
+          if (j >= C::kPBufs && !careful) {
             hold(sh.p_free[buf], p_use(it) - 1);
             tc_fence_after();
             float shrink[16];
@@ -777,17 +790,30 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           group_sync(group_bar);
           if (t < 16) {
             const float now = from_ordered(mosts[c0 + t]);
-            if (now > -neg_a[c0 + t]) neg_a[c0 + t] = -(now + kRoom);
+            if (!careful && now > -neg_a[c0 + t]) neg_a[c0 + t] = -(now + kRoom);
             mosts[c0 + t] = ordered(-INFINITY);
           }
           group_sync(group_bar);
-          fetch();
+          __syncwarp();
+          if (!careful) fetch();
+        }
+        if (careful) {
+          if (p_use(it) > 0) hold(sh.p_free[buf], p_use(it) - 1);
+          tc_fence_after();
+          const int at = side * N + c0;
+          const float scale_v = kE4m3 && key < vis_max
+                                    ? reinterpret_cast<const float*>(smem + C::kScalesAt + (it % C::kScaleSlots) * C::kScaleBytes)[kTile + t]
+                                    : 0.f;
+          careful_step<kE4m3, N>(CarefulColumns{sh.neg_a + at, sh.d + (kE4m3 ? at : 0), sh.most + at, sh.shrink_l + at,
+                                                sh.shrink_o + at, sh.f + (kE4m3 ? c0 : 0)},
+                                 group_bar, ts + c0, tm_o + C::kPCols * buf + lanes + c0, j >= C::kPBufs, hidden,
+                                 a.scale_log2, sk, scale_v, smem + C::kPAt + C::kPBytes * buf + t * 128, c0, l);
         }
         tc_fence_before();
         warp_arrive(sh.s_free[it & 1]);
         // ------------------------------------------ weights
         if (p_use(it) > 0) hold(sh.p_free[buf], p_use(it) - 1);
-        if (mine) {
+        if (mine && !careful) {
           uint8_t* const prow = smem + C::kPAt + C::kPBytes * buf + t * 128;
           auto put = [&](int c, const uint32_t (&v)[8]) {  // at columns c .. c + 15
             const int piece = c >> 3;
@@ -904,14 +930,11 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
         const float sum = sum16(v);
         if (!(lane & 1)) sums[(4 * side + quad) * N + c0 + (lane >> 1)] = sum;
       }
-      if (kE4m3 && c0 == 0 && t == 0) sh.shift[side] = n > j0 ? shift : -INFINITY;
       const bool bad_page = n > 0 && sh.bad_page[part & 7], some_bad = !kE4m3 && n > 0 && sh.any_bad[part & 7];
       if (threadIdx.x == 0 && bad_page) paged_report(a.status);
       all_sync();
       float* const part_to = p.whole ? nullptr : part_at<DP, N>(ta.parts, blockIdx.x, tile0 == 0);
       const int ch = 32 * quad + lane;
-      if constexpr (kE4m3) shift = fmaxf(fmaxf(sh.shift[0], sh.shift[1]), -60.f);
-      const float back = kE4m3 ? pow2(static_cast<int>(shift)) : 1.f;
       // is there anything in the O of P's buffers?
       const bool have0 = n > ((0 - first_of) & 1), have1 = n > ((1 - first_of) & 1);
       if (threadIdx.x < cols) {  // a thread settles a column: the weights of both accumulators, the sum and the place
@@ -922,24 +945,27 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
         };
         const float a0 = -sh.neg_a[c], a1 = -sh.neg_a[N + c], top = fmaxf(a0, a1);
         float f0 = fast_exp2(a0 - top), f1 = fast_exp2(a1 - top);  // nothing seen: sums and O are 0, or NaN to stay
-        float total = f0 * sum_of(0) + f1 * sum_of(1);
+        float total = f0 * sum_of(0) + f1 * sum_of(1), unit = 0.f;  // 2^unit: O's unit beside that of 2^top
+        if constexpr (kE4m3) {
+          const float d0 = fmaxf((a0 - top) + sh.d[c], kLeastUnit), d1 = fmaxf((a1 - top) + sh.d[N + c], kLeastUnit);
+          unit = fmaxf(d0, d1);
+          f0 = fast_exp2(d0 - unit);
+          f1 = fast_exp2(d1 - unit);
+        }
         if (bad_page || !alive) total = __uint_as_float(0x7FC00000u);
         float inv = total == 0.f ? 0.f : 1.f / total;
         int64_t place = 3 * N + c * DP;
         if (part_to != nullptr) {
           part_to[c] = top;
           part_to[N + c] = total;
-          part_to[2 * N + c] = shift;
+          part_to[2 * N + c] = unit;
           inv = 1.f;
         } else {
           const int64_t row = static_cast<int64_t>(p.rb) * N + c, token = sh.row[c] - p.row0;
           place = static_cast<int64_t>(sh.row[c]) * a.out_ld + (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d;
         }
         places[c] = place;
-        if constexpr (kE4m3) {
-          f0 *= fast_exp2(sh.shift[0] - shift);
-          f1 *= fast_exp2(sh.shift[1] - shift);
-        }
+        if constexpr (kE4m3) halves[c] = fast_exp2(0.5f * unit);
         weights[c] = f0 * inv;
         weights[N + c] = f1 * inv;
       }
@@ -993,7 +1019,10 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
           uint16_t* const to = a.out + ch;
 #pragma unroll
           for (int e = 0; e < 16; ++e)  // a sum of 0 has made y 0, or left it NaN
-            if (c0 + e < rows) to[places[c0 + e]] = __bfloat16_as_ushort(__float2bfloat16_rn(y[e] * back));
+            if (c0 + e < rows) {
+              if constexpr (kE4m3) y[e] = y[e] * halves[c0 + e] * halves[c0 + e];
+              to[places[c0 + e]] = __bfloat16_as_ushort(__float2bfloat16_rn(y[e]));
+            }
         }
       }
       tc_fence_before();
@@ -1031,13 +1060,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
   auto part = [&](int i) -> const float* {
     return i == 0 ? part_at<DP, N>(ta.parts, c - 1, true) : part_at<DP, N>(ta.parts, c + i - 1, false);
   };
-  // Sums and outputs each relative to the largest of theirs so far.
+  // Sums and outputs each relative to the largest of theirs so far: 2^top, and 2^(top + unit).
   constexpr int kPer = DP / 32;  // channels of a lane
-  float top = -INFINITY, o_top = -INFINITY, sum = 0.f, y[kPer] = {};
+  float top = -kUnset, unit = kLeastUnit, sum = 0.f, y[kPer] = {};
 #pragma unroll 4
   for (int i = 0; i <= others; ++i) {
     const float* x = part(i);
-    const float ref = x[r], l = x[N + r], o_ref = ref + x[2 * N + r];
+    const float ref = x[r], l = x[N + r];
     float o[kPer];
     if constexpr (kPer == 4) {
       const float4 v = *reinterpret_cast<const float4*>(x + 3 * N + r * DP + 4 * lane);
@@ -1049,22 +1078,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
     // a part whose keys the row does not see has the least reference and l = 0 (or NaN, which has to stay)
     if (ref > top) {
       sum *= fast_exp2(top - ref);
+      unit = fmaxf(unit + (top - ref), kLeastUnit);
       top = ref;
     }
+    const float own = fmaxf((ref - top) + x[2 * N + r], kLeastUnit);
     float back = 1.f;
-    if (o_ref > o_top) {
-      back = fast_exp2(o_top - o_ref);
-      o_top = o_ref;
+    if (own > unit) {
+      back = fast_exp2(unit - own);
+      unit = own;
     }
-    const float f = fast_exp2(o_ref - o_top);
+    const float f = fast_exp2(own - unit);
     sum = fmaf(fast_exp2(ref - top), l, sum);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) y[k] = fmaf(f, o[k], back * y[k]);
   }
   const uint32_t row = static_cast<uint32_t>(p.rb) * N + r, token = row_token(row, a.group);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum, unit = fast_exp2(o_top - top);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum, half = fast_exp2(0.5f * unit);
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) y[k] = sum == 0.f && y[k] == y[k] ? 0.f : y[k] * inv * unit;
+  for (int k = 0; k < kPer; ++k) y[k] = sum == 0.f && y[k] == y[k] ? 0.f : y[k] * inv * half * half;
   if (kPer * lane < a.d) {
     uint16_t* const to = a.out + (p.row0 + token) * a.out_ld +
                          (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d + kPer * lane;

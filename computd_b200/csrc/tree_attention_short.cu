@@ -10,7 +10,8 @@
 //   O^T += V^T P      128 channels by 32 rows  tcgen05, V and P in shared memory, O in TMEM
 //
 // What a row's weights are relative to, a, moves only when a score passes the limit (2^60 for bf16, for e4m3
-// what keeps a weight times its value's scale below 2^15), which every step asks by a vote.
+// what keeps a weight times its value's scale below 2^15), which every step asks by a vote.  Scores of 2^20 and more, and
+// values' scales 2^90 apart, take the careful steps of tree_tiles.cuh.
 //
 // Rounding: bf16 caches none beside f32 sums (P is the sum of two bf16 parts).  e4m3: codes are
 // exact; Q is, per row, a power of two times the sum of two e4m3 numbers, exactly down to 2^-9 of the
@@ -115,6 +116,9 @@ struct ShortShared {
   int most[N];                  // across keys, ordered
   int row[N];                   // of q
   uint32_t tops[2][4];          // e4m3: scales' exponents
+  float d[kE4m3 ? N : 4];       // e4m3: O's units are 2^d beside the references'
+  float shrink_l[N], shrink_o[N];
+  int careful[2];               // of each warpgroup
 };
 
 template <bool kE4m3, int DP, int N>
@@ -342,9 +346,11 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
     float* const sums = reinterpret_cast<float*>(smem + C::kPAt);  // [quad][N]: of weights
     float* const weights = sums + 4 * N;
     int64_t* const places = reinterpret_cast<int64_t*>(weights + N);
+    float* const halves = reinterpret_cast<float*>(places + N);    // e4m3: roots of O's units, which have more than f32's exponents
     // Where weights have to stay: e4m3 below 2^15 with their values' scales, and by themselves below
     // 2^105, so that their sums are f32; when a moves it leaves this much room.
-    constexpr float kMost = kE4m3 ? 105.f : 60.f, kRoom = kE4m3 ? 5.f : 60.f;
+    // (kLeast: where a value's scale is 2^90 and more beside 1 / g.)
+    constexpr float kMost = kE4m3 ? 105.f : 60.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 60.f;
     bool alive = true;
     auto hold = [&](const uint64_t& x, int phase) {  // after an abort nothing is waited for any more
       if (alive) alive = wait(x, phase);
@@ -367,10 +373,12 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
         x[k] = make_uint4(0, 0, 0, 0);
         if (live && 8 * piece < a.d) x[k] = __ldg(reinterpret_cast<const uint4*>(src) + piece);
       }
+      if (threadIdx.x < 2) sh.careful[threadIdx.x] = 0;
       if (piece0 == 0) {
         sh.row[c] = static_cast<int>(p.seq.row0 + token);
         sh.neg_a[c] = live ? kUnset : 0.f;
         sh.most[c] = ordered(-INFINITY);
+        if constexpr (kE4m3) sh.d[c] = 0.f;
       }
       if constexpr (kE4m3) {
         uint32_t tops = 0;
@@ -429,24 +437,86 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
     uint64_t l[8];  // sums of weights, in pairs of columns
 #pragma unroll
     for (int e = 0; e < 8; ++e) l[e] = 0;
-    float g = 1.f, shift = 0.f;  // e4m3: values' scales go times g = 2^-shift
+    float g = 1.f;  // e4m3: values' scales go times g = 2^-d
+    // Columns whose rows do not see this thread's key of a tile (which may leave -inf to those that do).
+    auto hidden_in = [&](int it) -> uint32_t {
+      const int key_w = it * kTile + t - lane, left = vis_max - key_w;  // the warp's first key, keys from there on
+      if ((it + 1) * kTile <= vis_min) return 0u;
+      // which of the warp's 32 keys the columns' rows see: lane l has column l's bits
+      const uint32_t valid = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1u : 0u;
+      uint32_t win = 0u, hidden = 0u;
+      if (lane < 16 && valid) win = tree_bits(a, sh.row[c0 + lane], key_w - prefix) & valid;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) hidden |= (~(__shfl_sync(0xFFFFFFFFu, win, e) >> lane) & 1u) << e;
+      return hidden;
+    };
+    // A tile's values, made ready for their product, which the weights have been for.
+    auto give_values = [&](int it) {
+      const int vs = it % C::kVStages;
+      uint8_t* const stage = smem + C::kVAt + vs * C::kVBytes;
+      const int left = vis_max - it * kTile;
+      hold(sh.v_full[vs], it / C::kVStages);
+      if constexpr (kE4m3) {
+        // Codes to fp16.  A warp has eight rows at a time, four lanes a row: codes 16 c .. and 64 +
+        // 16 c .. of it (c = lane & 3).  Neighbouring groups of four take rows r and r ^ 5, so that neither
+        // the reads nor the writes meet in a bank.
+        constexpr int kPer = DP / 64, kWarps = C::kSoftmax / 32, kRounds = kTile / 8 / kWarps;
+        const int c = lane & 3, pair_row = (lane >> 3) & 3, row8 = (lane & 4) ? pair_row ^ 5 : pair_row;
+        uint4 u[kRounds][kPer];
+#pragma unroll
+        for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) {
+            const int r = 8 * (warp + kWarps * k) + row8;
+            u[k][q] = *reinterpret_cast<const uint4*>(stage + r * DP + (((c + 4 * q) ^ (DP == 128 ? row8 : 0)) << 4));
+            if (r >= left) u[k][q] = make_uint4(0, 0, 0, 0);  // not this sequence's
+          }
+        warp_arrive(sh.v_empty[vs]);
+#pragma unroll
+        for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+          for (int q = 0; q < kPer; ++q) {
+            const uint4& v = u[k][q];
+            uint8_t* row = smem + C::kWideAt + q * kBlock + (8 * (warp + kWarps * k) + row8) * 128;
+            *reinterpret_cast<uint4*>(row + (((2 * c) ^ row8) << 4)) =
+                make_uint4(e4m3x2_f16x2(v.x, 0), e4m3x2_f16x2(v.x, 1), e4m3x2_f16x2(v.y, 0), e4m3x2_f16x2(v.y, 1));
+            *reinterpret_cast<uint4*>(row + (((2 * c + 1) ^ row8) << 4)) =
+                make_uint4(e4m3x2_f16x2(v.z, 0), e4m3x2_f16x2(v.z, 1), e4m3x2_f16x2(v.w, 0), e4m3x2_f16x2(v.w, 1));
+          }
+      } else if ((it + 1) * kTile > vis_min) {  // values that not every row sees: 0 * NaN would reach rows that must not see it
+        const int pc = lane & 7;
+#pragma unroll 1
+        for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll 2
+          for (int r = 4 * warp + (lane >> 3); r < kTile; r += C::kSoftmax / 8) {
+            uint4* const at = reinterpret_cast<uint4*>(stage + h * kBlock + r * 128 + pc * 16);
+            if (r >= left) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else if (it * kTile + r >= vis_min) {
+              auto finite = [](uint32_t u) -> uint32_t {
+                if ((u & 0x7F80u) == 0x7F80u) u &= 0xFFFF0000u;
+                if ((u & 0x7F800000u) == 0x7F800000u) u &= 0x0000FFFFu;
+                return u;
+              };
+              const uint4 v = *at, y = make_uint4(finite(v.x), finite(v.y), finite(v.z), finite(v.w));
+              if (v.x != y.x || v.y != y.y || v.z != y.z || v.w != y.w) {
+                *at = y;
+                sh.any_bad = 1;
+              }
+            }
+          }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      warp_arrive(sh.p_ready);
+    };
     all_sync();  // the columns' numbers are there
-    for (int it = 0; it < n; ++it) {
+    int it = 0;
+    for (; it < n; ++it) {
       const uint32_t ts = tm_s + N * (it & 1) + lanes + c0;
       const int key = it * kTile + t;
       const bool edge = (it + 1) * kTile > vis_min;
-      // Which of this warp's 32 keys the columns' rows see: lane l has column l's bits.
-      uint32_t win = 0u;
-      if (edge) {
-        const int key_w = key - lane, left = vis_max - key_w;  // the warp's first key, keys from there on
-        const uint32_t valid = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1u : 0u;
-        if (lane < 16 && valid) win = tree_bits(a, sh.row[c0 + lane], key_w - prefix) & valid;
-      }
-      uint32_t hidden = 0;  // columns whose rows do not see this thread's key (which may leave -inf to those that do)
-      if (edge) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) hidden |= (~(__shfl_sync(0xFFFFFFFFu, win, e) >> lane) & 1u) << e;
-      }
+      const uint32_t hidden = hidden_in(it);
       hold(sh.s_ready[it & 1], it >> 1);
       tc_fence_after();
       float sk = 1.f, sv = 1.f, limit = kMost;
@@ -465,11 +535,13 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
           group_sync(group_bar);
           const uint32_t most = max(max(sh.tops[wg][0], sh.tops[wg][1]), max(sh.tops[wg][2], sh.tops[wg][3]));
           const int e = most == 0 ? 0 : static_cast<int>(most >> 23) - 127;
-          shift = static_cast<float>(min(max(e, -60), 120));
-          g = pow2(-static_cast<int>(shift));
+          const int shift = min(max(e, -60), 120);
+          g = pow2(-shift);
+          if (t < 16) sh.d[c0 + t] = static_cast<float>(shift);
         }
         sv = fmaf(sv, 0.f, sv) * g;  // an infinity becomes NaN
-        limit = fminf(kMost, 15.f - fast_log2(fabsf(sv)));
+        limit = 15.f - fast_log2(fabsf(sv));
+        if (!(limit > kLeast && limit < kMost)) limit = -INFINITY;  // beyond what one g allows: any score asks
       }
       // Scores relative to a, in log2 units.
       const uint64_t sk2 = pair(sk, sk), scale2 = pair(a.scale_log2, a.scale_log2);
@@ -485,8 +557,8 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
           uint64_t s23 = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
           if constexpr (kE4m3) {
             const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&sh.f[c0 + e]);
-            s01 = fma2(mul2(s01, sk2), f.x, ref.x);
-            s23 = fma2(mul2(s23, sk2), f.y, ref.y);
+            s01 = fma2(mul2(s01, f.x), sk2, ref.x);
+            s23 = fma2(mul2(s23, f.y), sk2, ref.y);
           } else {
             s01 = fma2(s01, scale2, ref.x);
             s23 = fma2(s23, scale2, ref.y);
@@ -513,13 +585,16 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
         float most = -INFINITY;  // lane e: column e's
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          float z = __uint_as_float(s[e]) * sk * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) - limit;
+          float z = __uint_as_float(s[e]) * (kE4m3 ? sh.f[c0 + e] : a.scale_log2) * sk - limit;
           if ((hidden >> e) & 1u) z = -INFINITY;
           const float largest = warp_max(z);
           if ((lane & 15) == e) most = largest;
         }
         if (lane < 16 && most == most) atomicMax(&sh.most[c0 + lane], ordered(most));
+        if (most > -INFINITY && fabsf(most) >= kBig) sh.careful[wg] = 1;
         group_sync(group_bar);
+        __syncwarp();
+        if (*static_cast<volatile int*>(&sh.careful[wg]) != 0) break;  // the same for all threads
         if (it > 0) {
           hold(sh.p_free, it - 1);
           tc_fence_after();
@@ -553,6 +628,7 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
           sh.most[c0 + t] = ordered(-INFINITY);
         }
         group_sync(group_bar);
+        __syncwarp();
         fetch();
       }
       tc_fence_before();
@@ -591,66 +667,33 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
         put(c0, hi);
         if constexpr (!kE4m3) put(N + c0, lo);
       }
-      // ------------------------------------------ the tile's values
-      {
-        const int vs = it % C::kVStages;
-        uint8_t* const stage = smem + C::kVAt + vs * C::kVBytes;
-        const int left = vis_max - it * kTile;
-        hold(sh.v_full[vs], it / C::kVStages);
+      give_values(it);
+    }
+    // ---------------------------------------------- careful steps (see tree_tiles.cuh), from tile `it` on
+    if (it < n) {
+      if (t < 16) sh.most[c0 + t] = ordered(-INFINITY);
+      group_sync(group_bar);
+      for (; it < n; ++it) {
+        const int key = it * kTile + t;
+        const uint32_t hidden = hidden_in(it);
+        hold(sh.s_ready[it & 1], it >> 1);
+        float sk = 1.f, sv = 1.f;
         if constexpr (kE4m3) {
-          // Codes to fp16.  A warp has eight rows at a time, four lanes a row: codes 16 c .. and 64 +
-          // 16 c .. of it (c = lane & 3).  Neighbouring groups of four take rows r and r ^ 5, so that neither
-          // the reads nor the writes meet in a bank.
-          constexpr int kPer = DP / 64, kWarps = C::kSoftmax / 32, kRounds = kTile / 8 / kWarps;
-          const int c = lane & 3, pair_row = (lane >> 3) & 3, row8 = (lane & 4) ? pair_row ^ 5 : pair_row;
-          uint4 u[kRounds][kPer];
-#pragma unroll
-          for (int k = 0; k < kRounds; ++k)
-#pragma unroll
-            for (int q = 0; q < kPer; ++q) {
-              const int r = 8 * (warp + kWarps * k) + row8;
-              u[k][q] = *reinterpret_cast<const uint4*>(stage + r * DP + (((c + 4 * q) ^ (DP == 128 ? row8 : 0)) << 4));
-              if (r >= left) u[k][q] = make_uint4(0, 0, 0, 0);  // not this sequence's
-            }
-          warp_arrive(sh.v_empty[vs]);
-#pragma unroll
-          for (int k = 0; k < kRounds; ++k)
-#pragma unroll
-            for (int q = 0; q < kPer; ++q) {
-              const uint4& v = u[k][q];
-              uint8_t* row = smem + C::kWideAt + q * kBlock + (8 * (warp + kWarps * k) + row8) * 128;
-              *reinterpret_cast<uint4*>(row + (((2 * c) ^ row8) << 4)) =
-                  make_uint4(e4m3x2_f16x2(v.x, 0), e4m3x2_f16x2(v.x, 1), e4m3x2_f16x2(v.y, 0), e4m3x2_f16x2(v.y, 1));
-              *reinterpret_cast<uint4*>(row + (((2 * c + 1) ^ row8) << 4)) =
-                  make_uint4(e4m3x2_f16x2(v.z, 0), e4m3x2_f16x2(v.z, 1), e4m3x2_f16x2(v.w, 0), e4m3x2_f16x2(v.w, 1));
-            }
-        } else if (edge) {  // values that not every row sees: 0 * NaN would reach rows that must not see it
-          const int pc = lane & 7;
-#pragma unroll 1
-          for (int h = 0; h < C::kHalves; ++h)
-#pragma unroll 2
-            for (int r = 4 * warp + (lane >> 3); r < kTile; r += C::kSoftmax / 8) {
-              uint4* const at = reinterpret_cast<uint4*>(stage + h * kBlock + r * 128 + pc * 16);
-              if (r >= left) {
-                *at = make_uint4(0, 0, 0, 0);
-              } else if (it * kTile + r >= vis_min) {
-                auto finite = [](uint32_t u) -> uint32_t {
-                  if ((u & 0x7F80u) == 0x7F80u) u &= 0xFFFF0000u;
-                  if ((u & 0x7F800000u) == 0x7F800000u) u &= 0x0000FFFFu;
-                  return u;
-                };
-                const uint4 v = *at, y = make_uint4(finite(v.x), finite(v.y), finite(v.z), finite(v.w));
-                if (v.x != y.x || v.y != y.y || v.z != y.z || v.w != y.w) {
-                  *at = y;
-                  sh.any_bad = 1;
-                }
-              }
-            }
+          hold(sh.scales_full[it % C::kScaleSlots], it / C::kScaleSlots);
+          const float* scales = reinterpret_cast<const float*>(smem + C::kScalesAt + (it % C::kScaleSlots) * C::kScaleBytes);
+          sk = key < vis_max ? scales[t] : 0.f;
+          sv = key < vis_max ? scales[kTile + t] : 0.f;
         }
+        if (it > 0) hold(sh.p_free, it - 1);
+        tc_fence_after();
+        careful_step<kE4m3, N>(CarefulColumns{sh.neg_a + c0, sh.d + (kE4m3 ? c0 : 0), sh.most + c0, sh.shrink_l + c0,
+                                              sh.shrink_o + c0, sh.f + (kE4m3 ? c0 : 0)},
+                               group_bar, tm_s + N * (it & 1) + lanes + c0, tm_o + lanes + c0, it > 0, hidden,
+                               a.scale_log2, sk, sv, smem + C::kPAt + t * 128, c0, l);
+        tc_fence_before();
+        warp_arrive(sh.s_free[it & 1]);
+        give_values(it);
       }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      warp_arrive(sh.p_ready);
     }
     // ---------------------------------------------- out
     if (n > 0) hold(sh.p_free, n - 1);  // the last product
@@ -669,7 +712,6 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
     if (threadIdx.x == 0 && bad_page) paged_report(a.status);
     all_sync();
     const int ch = 32 * quad + lane;
-    const float back = pow2(static_cast<int>(shift));
     if (threadIdx.x < cols) {  // a thread settles a column
       const int c = threadIdx.x;
       const float* x = sums + c;
@@ -678,6 +720,7 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
       const int64_t row = static_cast<int64_t>(p.rb) * N + c, token = sh.row[c] - p.seq.row0;
       places[c] = static_cast<int64_t>(sh.row[c]) * a.out_ld + (static_cast<int64_t>(p.hk) * a.group + row - token * a.group) * a.d;
       weights[c] = total == 0.f ? 0.f : 1.f / total;
+      if constexpr (kE4m3) halves[c] = fast_exp2(0.5f * sh.d[c]);
     }
     all_sync();
     if (mine) {
@@ -715,7 +758,10 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
         uint16_t* const to = a.out + ch;
 #pragma unroll
         for (int e = 0; e < 16; ++e)  // a sum of 0 has made y 0, or left it NaN
-          if (c0 + e < rows) to[places[c0 + e]] = __bfloat16_as_ushort(__float2bfloat16_rn(y[e] * back));
+          if (c0 + e < rows) {
+            if constexpr (kE4m3) y[e] = y[e] * halves[c0 + e] * halves[c0 + e];
+            to[places[c0 + e]] = __bfloat16_as_ushort(__float2bfloat16_rn(y[e]));
+          }
       }
     }
     tc_fence_before();

@@ -1,11 +1,13 @@
 // tree_tiles.cuh — what the kernels of tree_attention.cu and tree_attention_short.cu share: their
-// tcgen05 instructions and descriptors, bounded waits, and numbers across lanes.
+// tcgen05 instructions and descriptors, bounded waits, numbers across lanes, and steps over numbers far apart.
 #pragma once
 
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
+#include "f32x2.cuh"
+#include "paged_attention.cuh"
 #include "sm100_ptx.cuh"
 
 namespace dwa {
@@ -74,6 +76,15 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ float tmem_ld_x1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r) : : "memory");
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void tmem_st_x1(uint32_t taddr, float x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(x)) : "memory");
 }
 
 // 16 keys of an operand whose other axis lies along rows of 128 bytes (64 16-bit elements, the
@@ -170,6 +181,125 @@ __device__ __forceinline__ float warp_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// ---------------------------------------------------------------- careful steps
+// A step's weights are 2^(S - a) with a reference a that stays unless a score passes a limit, and over an e4m3
+// cache times the value's scale over one power of two for all tiles.  That has its range: where scores are 2^kBig
+// and more, f32's steps at their size are a good part of 1, and a difference of numbers rounded apart is off by
+// them; and a value's scale 2^90 away from the first tile's largest leaves fp16.  From the first tile with either
+// on, a warpgroup's steps of the unit are careful ones:
+//   t = S rounded to f32 as a number of its own, b = the column's maximum of t so far,
+//   weights 2^(t - b), at most 1, in the sum; in the product, over an e4m3 cache, m 2^((t - b) + e - d), where the
+//   value's scale is m 2^e and d follows the largest of (t - b) + e, so that the row's largest is 2^10 at least
+//   (and every weight down to 2^-24 of it keeps fp16's 11 bits).
+// So O is in units of 2^(b + d).  b and d only meet differences: sums of both would lose d beside a large b.
+// (Three passes over the scores, a column at a time: 16 trees of 20 to 32 nodes over 300 to 4096 tokens, 16 heads of 128,
+// with scores of 2^24, bf16 97 us instead of 56, e4m3 124 instead of 53.)
+constexpr float kBig = 0x1p20f;
+constexpr float kLeastUnit = -0x1p100f;  // the exponent d where nothing has any weight
+
+// The sixteen columns of a warpgroup, in shared memory.
+struct CarefulColumns {
+  float* neg_b;      // minus b
+  float* d;          // e4m3
+  int* most;         // across keys, ordered; minus infinity between uses
+  float* shrink_l;   // of the sums, and of O
+  float* shrink_o;
+  const float* f;    // e4m3: the scores' factors
+};
+
+// The weights of this thread's key in sixteen columns, whose scores are at TMEM column `ts`, into its row of P
+// (at columns c0 .. and, bf16, the second parts kApart further) and their sums l.  `to`: O's columns, rescaled
+// where they move and have_o says that there are any; the products into them so far are done.  hidden: columns
+// that do not see the key.  The 128 threads of named barrier `id` together.
+template <bool kE4m3, int kApart>
+__device__ __forceinline__ void careful_step(const CarefulColumns& at, int id, uint32_t ts, uint32_t to, bool have_o,
+                                             uint32_t hidden, float scale_log2, float sk, float sv, uint8_t* prow, int c0,
+                                             uint64_t (&l)[8]) {
+  const int t = threadIdx.x & 127, lane = threadIdx.x & 31;
+  int exp_v = 0;
+  const float m = kE4m3 ? scale_parts(sv, &exp_v) : 1.f;
+  const float e_v = static_cast<float>(exp_v);
+  auto together = [&]() {
+    group_sync(id);
+    __syncwarp();
+  };
+  // (A load of the whole warp: it stands in no branch that threads may take apart.)
+  auto score = [&](int e) -> float {
+    const float s = tmem_ld_x1(ts + e);
+    const float x = kE4m3 ? __fmul_rn(__fmul_rn(s, at.f[e]), sk) : __fmul_rn(s, scale_log2);
+    return (hidden >> e) & 1u ? -INFINITY : x;
+  };
+  // columns' maxima of `value` across the keys, which NaN is not among
+  auto maxima = [&](auto&& value) {
+    float most = -INFINITY;
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {
+      const float largest = warp_max(value(e, score(e)));
+      if ((lane & 15) == e) most = largest;
+    }
+    if (lane < 16 && most == most) atomicMax(&at.most[lane], ordered(most));
+    together();
+  };
+  maxima([](int, float x) -> float { return x; });
+  if (t < 16) {
+    const float was = -at.neg_b[t], now = fmaxf(was, from_ordered(at.most[t]));
+    at.shrink_l[t] = at.shrink_o[t] = fast_exp2(was - now);
+    if constexpr (kE4m3) at.d[t] = fmaxf(at.d[t] + (was - now), kLeastUnit);
+    at.neg_b[t] = -now;
+    at.most[t] = ordered(-INFINITY);
+  }
+  together();
+  if constexpr (kE4m3) {
+    maxima([&](int e, float x) -> float { return m != 0.f ? (x + at.neg_b[e]) + e_v : -INFINITY; });
+    if (t < 16) {
+      const float was = at.d[t], now = fmaxf(was, from_ordered(at.most[t]) - 10.f);
+      at.shrink_o[t] = fast_exp2(was - now);
+      at.d[t] = now;
+      at.most[t] = ordered(-INFINITY);
+    }
+    together();
+  }
+  if (have_o) {
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e) {
+      const float by = at.shrink_o[e];
+      if (by == 1.f) continue;  // the same for all threads
+#pragma unroll
+      for (int h = 0; h < (kE4m3 ? 1 : 2); ++h) tmem_st_x1(to + kApart * h + e, tmem_ld_x1(to + kApart * h + e) * by);
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  }
+#pragma unroll 1
+  for (int e = 0; e < 16; e += 2) {
+    float w[2], p[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float x = score(e + k), rel = x + at.neg_b[e + k];
+      w[k] = x == -INFINITY ? 0.f : fast_exp2(rel);
+      p[k] = w[k];
+      if constexpr (kE4m3) {
+        p[k] = fast_exp2((rel + e_v) - at.d[e + k]) * m;
+        if (m == 0.f || ((hidden >> (e + k)) & 1u)) p[k] = 0.f;  // d says nothing of the one, the other's scale may be anything
+      }
+    }
+    const uint64_t by = pair(at.shrink_l[e], at.shrink_l[e + 1]), more = pair(w[0], w[1]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (2 * k == e) l[k] = fma2(l[k], by, more);
+    auto put = [&](int c, uint32_t v) {
+      *reinterpret_cast<uint32_t*>(prow + (((c >> 3) ^ (t & 7)) << 4) + 2 * (c & 7)) = v;
+    };
+    if constexpr (kE4m3) {
+      put(c0 + e, pack_f16(p[0], p[1]));
+    } else {
+      const uint32_t hi = pack_bf16(p[0], p[1]);
+      put(c0 + e, hi);
+      put(kApart + c0 + e,
+          pack_bf16(p[0] - __uint_as_float(hi << 16), p[1] - __uint_as_float(hi & 0xFFFF0000u)));
+    }
+  }
 }
 
 }  // namespace
