@@ -13,7 +13,7 @@
 //
 // What a row's weights are relative to, a, is not its maximum but anything that keeps them in
 // range; it moves when a score passes the limit, which every step asks by a vote, and only
-// then are maxima taken across keys.  The limit is 2^60 for bf16 (whose range is f32's) and for e4m3
+// then are maxima taken across keys.  The limit is 2^20 for bf16 (whose range is f32's) and for e4m3
 // what keeps a weight times its value's scale below 2^15 in fp16.  Scores of 2^20 and more, and values' scales 2^90 apart,
 // take the careful steps of tree_tiles.cuh.
 //
@@ -545,10 +545,11 @@ __global__ void __launch_bounds__(TreeCfg<kE4m3, DP, N>::kThreads, 1)
     float* const weights = sums + 1024;                            // [side][N]: of the accumulators
     int64_t* const places = reinterpret_cast<int64_t*>(weights + 2 * N);
     float* const halves = reinterpret_cast<float*>(places + N);    // e4m3: roots of O's units, which have more than f32's exponents
-    // Where weights have to stay: e4m3 below 2^15 with their values' scales, and by themselves below
-    // 2^105, so that their sums are f32; when a moves it leaves this much room.
+    // Where weights have to stay: bf16 below 2^20, so that their sums with values of 2^100 are f32; e4m3 below
+    // 2^15 with their values' scales, and by themselves below 2^105, so that their sums are f32.  When a moves it
+    // leaves this much room.
     // (kLeast: where a value's scale is 2^90 and more beside 1 / g.)
-    constexpr float kMost = kE4m3 ? 105.f : 60.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 60.f;
+    constexpr float kMost = kE4m3 ? 105.f : 20.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 20.f;
     bool alive = true;
     auto hold = [&](const uint64_t& x, int phase) {  // after an abort nothing is waited for any more
       if (alive) alive = wait(x, phase);

@@ -9,7 +9,7 @@
 //   P   = exp2(S - a) a thread per key and 16 rows
 //   O^T += V^T P      128 channels by 32 rows  tcgen05, V and P in shared memory, O in TMEM
 //
-// What a row's weights are relative to, a, moves only when a score passes the limit (2^60 for bf16, for e4m3
+// What a row's weights are relative to, a, moves only when a score passes the limit (2^20 for bf16, for e4m3
 // what keeps a weight times its value's scale below 2^15), which every step asks by a vote.  Scores of 2^20 and more, and
 // values' scales 2^90 apart, take the careful steps of tree_tiles.cuh.
 //
@@ -347,10 +347,11 @@ __global__ void __launch_bounds__(ShortCfg<kE4m3, DP, N>::kThreads, 2)
     float* const weights = sums + 4 * N;
     int64_t* const places = reinterpret_cast<int64_t*>(weights + N);
     float* const halves = reinterpret_cast<float*>(places + N);    // e4m3: roots of O's units, which have more than f32's exponents
-    // Where weights have to stay: e4m3 below 2^15 with their values' scales, and by themselves below
-    // 2^105, so that their sums are f32; when a moves it leaves this much room.
+    // Where weights have to stay: bf16 below 2^20, so that their sums with values of 2^100 are f32; e4m3 below
+    // 2^15 with their values' scales, and by themselves below 2^105, so that their sums are f32.  When a moves it
+    // leaves this much room.
     // (kLeast: where a value's scale is 2^90 and more beside 1 / g.)
-    constexpr float kMost = kE4m3 ? 105.f : 60.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 60.f;
+    constexpr float kMost = kE4m3 ? 105.f : 20.f, kLeast = -75.f, kRoom = kE4m3 ? 5.f : 20.f;
     bool alive = true;
     auto hold = [&](const uint64_t& x, int phase) {  // after an abort nothing is waited for any more
       if (alive) alive = wait(x, phase);

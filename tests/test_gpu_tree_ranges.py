@@ -318,3 +318,24 @@ def test_sizes_far_apart(form, kind):
     check(attend(cache, q, [n, n], seen), want, mag)
     big = (q.float().sign() * 2.0 ** 20).to(BF16)
     assert bool(torch.isfinite(attend(cache, big, [n, n], seen)).all())
+
+
+@forms
+@pytest.mark.parametrize("log2", [-100, 60, 100])
+def test_large_values_behind_rising_scores(form, log2):
+    """bf16 values of any size, with scores that rise by 50 (in powers of two) along the context: what weights
+    are relative to moves with them, and sums stay in f32's range."""
+    n, heads, kv_heads, length = FORMS[form]
+    cache = Cache("bf16", [length], kv_heads, 64, 32, seed=n)
+    page, off = _tokens(cache, 0, list(range(length)))
+    rise = torch.arange(length, device="cuda") / length * 50 * math.log(2)  # q's first channel is 8, the scale 1/8
+    cache.k[page, :, off] = (cache.k[page, :, off].float() / 16).to(BF16)
+    cache.k[page, :, off, 0] = rise[:, None].to(BF16).expand(-1, kv_heads)
+    cache.v[page, :, off] = (cache.v[page, :, off].float() * 2.0 ** log2).to(BF16)
+    q = _queries(n, heads, 64, 3)
+    q[..., 0] = 8.0
+    seen = masks_of([n], "tree", 6)
+    want, mag = tree_attention_64(q, cache, [0, n], seen)
+    got = attend(cache, q, [n], seen)
+    assert bool(torch.isfinite(got).all())
+    check(got.double() * 2.0 ** -log2, want * 2.0 ** -log2, mag * 2.0 ** -log2)
