@@ -1346,9 +1346,9 @@ cudaError_t launch_mma(const PagedArgs& a, cudaStream_t stream) {
   // answers: there the longest unit takes its time whatever the others do, and with the longest first all are
   // through about a third of a unit behind the mean of half the table's length; what gains more by this, in
   // proportion, than it loses by the first.  (16 trees of 33 to 64 nodes, 8 e4m3 heads of 4 query heads and 128
-  // channels: over 2000 to 16384 tokens 278 us whole, 163 in two, 200 in four; over 16384 each 315, 324 and
-  // 355; over 2048 each 49, 69 and 102.  80 units of 64 rows over 3000 tokens each, bf16, 42 whole, 57 in two;
-  // ragged 41 and 33.)  Clearly the fewest is a tenth fewer, of trees a twelfth: in between, parts save ragged contexts
+  // channels: over 2000 to 16384 tokens 278 us whole, 160 in two, 195 in four; over 16384 each 318, 337 and
+  // 355; over 2048 each 51, 70 and 100.  80 units of 64 rows over 3000 tokens each, bf16, 44 whole, 55 in two;
+  // ragged 42 and 31.)  Clearly the fewest is a tenth fewer, of trees a twelfth: in between, parts save ragged contexts
   // more than they cost equal ones (whole and in two, bf16 and e4m3: 16 trees of 80 nodes over 8576 tokens, 8 heads,
   // ragged 97 and 73, 127 and 86, equal 97 and 113, 134 and 143; 9 over 5248, 12 heads, ragged 62 and 39, 79 and 48,
   // equal 63 and 79, 83 and 97; 3 over 1152, 16 heads, either 21 and 18, 26 and 22).

@@ -24,9 +24,9 @@
 // rounded to fp16, 11 bits.
 //
 // Bound by HBM where contexts are long and all as long: 16 sequences of 32 nodes over 4096 tokens, 16 heads of
-// 128 channels, bf16, 93 us, 5.7 TB/s; else by the length of a step's chain (loads from TMEM, vote, exponentials,
+// 128 channels, bf16, 94 us, 5.7 TB/s; else by the length of a step's chain (loads from TMEM, vote, exponentials,
 // stores, product) and by what a unit costs beside its steps: 20 to 32 nodes over 300 to 4096 tokens 56 us, 4.8 TB/s
-// (floor 41); one sequence over 4096 20 us, e4m3 22.  (More rows are no work for this layout: a thread reads
+// (floor 41); one sequence over 4096 20 us, e4m3 21.  (More rows are no work for this layout: a thread reads
 // its columns' references, 4 bytes each, from shared memory, which with 64 or 128 columns takes as long as all
 // else.)
 // Work is cut by steps, not by units: each block takes an equal share of all steps, whatever sequence they

@@ -21,7 +21,7 @@
 // step is a chain of product, vote, exponentials, product.  So two blocks share an SM, each with half of
 // its shared memory and registers, and none has more to find out than its own sequence: no shares, no
 // parts to join.  16 sequences of 32 nodes, 16 heads of 128 channels, over 128 and 1024 tokens: bf16 11 and
-// 30 us, e4m3 12 and 26; a block to an SM that shares out the steps 17 and 40, 18 and 38.  24 ragged ones of 5 to 40
+// 31 us, e4m3 12 and 25; a block to an SM that shares out the steps 17 and 40, 18 and 38.  24 ragged ones of 5 to 40
 // nodes over 50 to 1500 tokens, 16 heads of 80, e4m3: 45 us, 66 in tiles of 128 rows.  Long contexts
 // turn this round: the longest unit has a block to itself (see tree_is_short).
 //
@@ -800,8 +800,9 @@ cudaError_t launch_short(const PagedArgs& a, cudaStream_t stream) {
 //   32 rows, bf16:   128 units over 128 8.8 and 9.0 (else 9.4, 9.5), over 1024 17.3 and 16.7 (14.9, 14.4)
 //                    256 units over 1024 30.6 and 20.3 (39.6, 29.0), over 4096 86.8 and 67.9 (94.2, 63.9)
 //                    1024 units over 512 67.0 and 51.7 (72.3, 73.2), over 2048 183 and 101 (180, 109)
-//   64 rows, bf16:   256 heads over 512 29.0 and 24.6 (31.5, 30.0), over 2048 73.3 and 47.3 (66.8, 45.6)
-//   64 rows, e4m3:   256 heads over 2048 78.0 and 48.1 (80.9, 54.4), over 4096 137.8 and 91.0 (136.2, 96.2)
+//   64 rows, bf16:   256 heads over 512 29.6 and 23.5 (29.4, 24.9), over 1024 46.6 and 30.1 (41.5, 30.7: with 8 bits
+//                    of the probabilities instead of 16), over 2048 73.8 and 46.7 (63.6, 42.9)
+//   64 rows, e4m3:   256 heads over 2048 77.1 and 45.8 (78.2, 50.1), over 4096 136.2 and 71.8 (133.8, 77.2)
 // More rows than 64 read the same keys too often: 128 rows of 128 heads over 128 tokens 20.3 (12.0).
 bool tree_is_short(const PagedArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;

@@ -150,7 +150,8 @@ def tree_masks(parents: torch.Tensor, *, q_start: torch.Tensor | None = None, n_
     tree, which is below its own, or -1.  Bit j % 64 of word j // 64 of a node's row says that it is node j or
     below it; its depth is the number of nodes above it.  W = ceil(max_q / 64) words, where ``max_q``
     (default: T, or T / n_trees; 4096 at most) bounds a tree's nodes.  A parent that does not come before its node is reported
-    and counts as none; rows of no tree, and of one with more than ``max_q`` nodes, are zeros."""
+    and counts as none; rows of no tree (those too
+    that only a bad range of rows covers, which is reported), and of one with more than ``max_q`` nodes, are zeros."""
     return (_host_module or _host()).masks(parents, q_start, n_trees, max_q, status)
 
 
@@ -200,7 +201,7 @@ def kv_cache_keep(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
     Sequence b's token start[b] + path[b, i] becomes token start[b] + i for i = 0 .. n_accepted[b]
     (``start`` and ``n_accepted`` int32 [B], ``path`` int32 [B, steps], as ``verify_tree`` returns them), on the
     pages of ``block_table`` (int32 [B, max_pages]).  The caches are one layer's, or all layers'
-    [layers, n_pages, H_kv, page_size, d].  Paths ascend; one that does not, or that leaves
+    [layers, n_pages, H_kv, page_size, d].  Paths ascend from 0 or more; one that does not, or that leaves
     the pages, is reported and its sequence stays as it was."""
     (_host_module or _host()).kv_keep(k_cache, v_cache, block_table, start, path, n_accepted, k_scale, v_scale,
                                       status)

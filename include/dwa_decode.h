@@ -13,7 +13,7 @@
  * inside a page is contiguous.  Slot s is token s % page_size of page
  * s / page_size.  page_size is 16, 32, 64 or 128; d is a multiple of 16 in
  * [16, 128].  NULL scales mean a bf16 cache.  Pages and their scales are 16-byte
- * aligned (ld_page a multiple of d, ld_scale_page of 4).  Codes are numbers
+ * aligned (ld_page a multiple of d, ld_scale_page of 4).  Codes are numbers, scales finite or NaN
  * (dwa_kv_write makes no NaN code: what it cannot store has a NaN scale).
  *
  * What only the device can see is checked there: a bad slot, page number,
@@ -143,7 +143,8 @@ DWA_API dwa_status dwa_kv_append(const void* q, const void* k, const void* v, in
  * ancestors' (node j: bit j % 64 of word j / 64), depth (int32 [T]) the number of its ancestors.
  * max_q (4096 at most) bounds the nodes of a tree; mask_words >= max_q / 64.  A node whose parent
  * is not before it counts as one without a parent and is reported in *status; a tree of more than max_q
- * nodes is reported and its rows are zeros, as rows of no sequence are.
+ * nodes is reported and its rows are zeros, as rows of no sequence are (those too that only a bad
+ * range covers).
  */
 DWA_API dwa_status dwa_tree_masks(const int32_t* parents, const int32_t* q_start, int64_t T, int32_t B,
                                   int32_t max_q, int64_t* mask, int32_t mask_words, int32_t* depth,
@@ -192,7 +193,7 @@ DWA_API dwa_status dwa_verify_tree(const void* target, int32_t probs_bf16, const
  * Moves the cached tokens of a path to where a sequence's tokens belong, in `layers` layers
  * (ld_layer elements and ld_scale_layer scales apart): sequence b's token start[b] + path[b][i] to
  * start[b] + i, for i = 0 .. n_accepted[b] (int32; path int32 [B][steps]), on the pages of
- * block_table.  Paths ascend, so every token moves as it was before the call.  n_accepted below
+ * block_table.  Paths ascend from 0 or more, so every token moves as it was before the call.  n_accepted below
  * 0, or 0 with a negative path[b][0]: nothing.  A path that does not ascend, is longer than
  * steps, or leaves the pages is reported in *status, and its sequence stays as it was.
  */
