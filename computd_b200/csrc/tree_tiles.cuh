@@ -187,7 +187,7 @@ __device__ __forceinline__ float warp_max(float x) {
 // A step's weights are 2^(S - a) with a reference a that stays unless a score passes a limit, and over an e4m3
 // cache times the value's scale over one power of two for all tiles.  That has its range: where scores are 2^kBig
 // and more, f32's steps at their size are a good part of 1, and a difference of numbers rounded apart is off by
-// them; and a value's scale 2^90 away from the first tile's largest leaves fp16.  From the first tile with either
+// them; and a value's scale 2^90 away from the first tile's largest leaves fp16 (that of a vector of zeros, 2^-126, is).  From the first tile with either
 // on, a warpgroup's steps of the unit are careful ones:
 //   t = S rounded to f32 as a number of its own, b = the column's maximum of t so far,
 //   weights 2^(t - b), at most 1, in the sum; in the product, over an e4m3 cache, m 2^((t - b) + e - d), where the
